@@ -234,6 +234,85 @@ int nhip_linear_cross_entropy(const nhip_lce_desc *desc, const void *h, const vo
                               void *workspace);
 int nhip_linear_cross_entropy_workspace(const nhip_lce_desc *desc, size_t *bytes);
 
+/* ---- head norms and rotation (no counterpart in the reference: its programs write them out in primitives) -------- *
+ *
+ * Queries [B, S, N, D] and keys [B, S, Nkv, D], each row of D elements divided by the root of its mean square plus eps,
+ * times a weight [D] (null: ones), and its first rot elements turned by position: pair i of row p as
+ * (a, b) -> (a cos - b sin, b cos + a sin) with cos and sin float32 [table_rows, rot / 2], read at row p. Pairs are elements
+ * i and i + rot / 2, or 2 i and 2 i + 1 where interleaved. p is the positions' value of the row's token (int32 or int64
+ * [B, S], contiguous; null: 0 .. S - 1), clamped into the table. Strides in elements, the D axis contiguous; float32, bf16
+ * or f16, one type for all but the tables. rot is even and at most D, D at most 1024; seq is below 2^30. Everything
+ * between is float32. A tensor may have no heads, and a batch no tokens. */
+enum {
+    NHIP_POS_NONE = 0,
+    NHIP_POS_I32 = 1,
+    NHIP_POS_I64 = 2,
+};
+typedef struct {
+    int64_t batch, seq, heads, kv_heads, head_dim, rot, table_rows;
+    int64_t q_b, q_s, q_n, k_b, k_s, k_n;          /* the heads read */
+    int64_t oq_b, oq_s, oq_n, ok_b, ok_s, ok_n;    /* the heads written; backward: dq and dk */
+    int64_t dq_b, dq_s, dq_n, dk_b, dk_s, dk_n;    /* backward only: the outputs' cotangents */
+    int32_t dtype, positions, interleaved;         /* NHIP_F32/BF16/F16; NHIP_POS_* */
+    float eps;
+} nhip_heads_desc;
+
+int nhip_qk_norm_rope(const nhip_heads_desc *desc, const void *q, const void *k, const void *q_weight, const void *k_weight,
+                      const float *cos, const float *sin, const void *positions, void *q_out, void *k_out);
+/* Its gradients from the outputs' cotangents d_q_out and d_k_out: dq, dk, and d_q_weight, d_k_weight (float32 sums over all
+ * rows, in a fixed order, rounded once). Any of the four may be null: then it is not computed. `workspace` of nhip_qk_norm_rope_workspace bytes. */
+int nhip_qk_norm_rope_bwd(const nhip_heads_desc *desc, const void *q, const void *k, const void *q_weight,
+                          const void *k_weight, const float *cos, const float *sin, const void *positions,
+                          const void *d_q_out, const void *d_k_out, void *dq, void *dk, void *d_q_weight, void *d_k_weight,
+                          void *workspace);
+int nhip_qk_norm_rope_workspace(const nhip_heads_desc *desc, size_t *bytes);
+
+/* ---- gated projections (no counterpart in the reference) -------------------------------------------------------- *
+ *
+ * h [m, n] = act(x gate^T) * (x up^T) for x [m, k] and weights [n, k], bf16 or f16, contiguous along k, rows x_m and w_n
+ * elements apart (both weights), h's rows h_m. The sums are float32 and rounded once, in h. g and u (both or neither):
+ * float32 [m, n], the two products, which nhip_gated_linear_grad needs. */
+enum {
+    NHIP_ACT_SILU = 0,
+    NHIP_ACT_GELU = 1,     /* the tanh form */
+    NHIP_ACT_RELU = 2,
+    NHIP_ACT_SIGMOID = 3,
+};
+typedef struct {
+    int64_t m, n, k;
+    int64_t x_m, w_n, h_m;   /* h_m: nhip_gated_linear_grad's dh rows */
+    int32_t dtype, activation;
+    int32_t config;          /* -1: the default for the shape; else an index below nhip_gated_config_count */
+} nhip_gated_desc;
+
+int nhip_gated_linear(const nhip_gated_desc *desc, const void *x, const void *gate, const void *up, void *h, float *g, float *u);
+/* Number of kernels nhip_gated_linear has (for tests and timing); a config the operands cannot take fails. */
+int nhip_gated_config_count(int *count);
+/* [dg | du] ([m, 2 n], contiguous, the type of dh) of dh [m, n]: dg = dh u act'(g), du = dh act(g), each rounded once. */
+int nhip_gated_linear_grad(const nhip_gated_desc *desc, const void *dh, const float *g, const float *u, void *dgu);
+
+/* ---- gradient clipping (no counterpart in the reference) -------------------------------------------------------- *
+ *
+ * norm = the root of the sum of squares of every element of every tensor, summed in float64; each tensor times
+ * min(1, max_norm / (norm + eps)), that factor float32 (a NaN norm gives NaNs), rounded once into its own type. A tensor
+ * with a null `out` counts for the norm only; `out` may be `in`. max_norm_at: a device float64 that is read in place of
+ * max_norm, or null. norm, scale (that factor): float32 on the device, or null. Two launches for each 120 tensors. */
+typedef struct {
+    const void *in;
+    void *out;
+    int64_t numel;
+    int32_t dtype;   /* NHIP_F32, NHIP_BF16 or NHIP_F16 */
+    int32_t pad;
+} nhip_clip_tensor;
+typedef struct {
+    int64_t count;   /* tensors */
+    double max_norm, eps;
+} nhip_clip_desc;
+
+int nhip_clip_grad_norm(const nhip_clip_desc *desc, const nhip_clip_tensor *tensors, const double *max_norm_at, float *norm,
+                        float *scale, void *workspace);
+int nhip_clip_grad_norm_workspace(const nhip_clip_desc *desc, size_t *bytes);
+
 /* ---- static plans (lumen/plan/run.rs:356-427 execute; lumen/plan/step/cuda.rs:17-63) ----------------- *
  *
  * A plan is a list of steps run in order on the stream: generated kernels (a function of a loaded module)
@@ -262,6 +341,13 @@ enum {
     NHIP_STEP_COPY = 4,       /* desc: uint64 bytes; pointers: dst, src */
     NHIP_STEP_FILL = 5,       /* desc: uint64 bytes, uint32 byte value; pointers: dst */
     NHIP_STEP_LCE = 6,        /* desc: nhip_lce_desc; pointers: h, w, target, out, workspace */
+    NHIP_STEP_HEADS = 7,      /* desc: nhip_heads_desc; pointers as nhip_qk_norm_rope's, those left out null */
+    NHIP_STEP_HEADS_BWD = 8,  /* desc: nhip_heads_desc; pointers as nhip_qk_norm_rope_bwd's */
+    NHIP_STEP_GATED = 9,      /* desc: nhip_gated_desc; pointers: x, gate, up, h (and g, u) */
+    NHIP_STEP_GATED_GRAD = 10, /* desc: nhip_gated_desc; pointers: dh, g, u, dgu */
+    NHIP_STEP_CLIP = 11,      /* desc: nhip_clip_desc, then its nhip_clip_tensors (in and out ignored); pointers: max_norm_at
+                                 (or none), norm, scale (or none), workspace, then tensor i's in at 4 + 2 i and out at
+                                 5 + 2 i (or none) */
 };
 
 int nhip_plan_create(void **plan);

@@ -27,9 +27,12 @@ def _accumulate(cts, v, c):
 
 
 def backward(out, ct, tape, leaves):
-    """The gradient of each of ``leaves`` (None where ``out`` does not depend on it) for cotangent ``ct``."""
-    if (ct.dtype, tuple(ct.shape)) != (out.dtype, tuple(out.shape)):
-        raise TypeError(f"backward: a gradient must have its value's type, got {ct.dtype}{list(ct.shape)} for {out!r}")
+    """The gradient of each of ``leaves`` (None where ``out`` does not depend on it) for cotangent ``ct``; of several
+    results, tuples of which ``out`` and ``ct`` are, their sum."""
+    results, given = (out, ct) if isinstance(out, tuple) else ((out,), (ct,))
+    for o, c in zip(results, given):
+        if (c.dtype, tuple(c.shape)) != (o.dtype, tuple(o.shape)):
+            raise TypeError(f"backward: a gradient must have its value's type, got {c.dtype}{list(c.shape)} for {o!r}")
     graph = tracer.current_graph()
     tape = cross_entropy.substitute(tape)
     # Values that depend on a float leaf: only their nodes are differentiated.
@@ -43,12 +46,15 @@ def backward(out, ct, tape, leaves):
                 continue
             live.update(outs)
             linear.append(node)
-    if out.var not in live:
+    if not any(o.var in live for o in results):
         return [None for _ in leaves]
-    cts = {out.var: ct}
+    cts = {}
     saved = graph.backward
     graph.backward = True
     try:
+        for o, c in zip(results, given):
+            if o.var in live:
+                _accumulate(cts, o.var, c)
         for name, inputs, params, outv in reversed(linear):
             if name == FUNCTION:
                 _function_transpose(params, outv, cts, live)
@@ -92,7 +98,8 @@ def _zeros(var):
 
 
 def vjp(fn, *primals):
-    """``fn(*primals)`` and a function from its cotangent to the primals' (``jax.vjp``)."""
+    """``fn(*primals)`` and a function from its cotangent to the primals' (``jax.vjp``); of a function of several
+    results, tuples of both."""
     tape = []
     tracer._TAPES.append(tape)
     try:
@@ -102,6 +109,10 @@ def vjp(fn, *primals):
     leaves = [p for p in primals if isinstance(p, TracedTensor)]
 
     def pullback(ct):
+        if isinstance(out, (tuple, list)):
+            if not isinstance(ct, (tuple, list)) or len(ct) != len(out):
+                raise TypeError(f"vjp: {len(out)} results take as many cotangents, got {ct!r}")
+            return tuple(backward(tuple(out), tuple(ct), tape, leaves))
         return tuple(backward(out, ct, tape, leaves))
 
     return out, pullback

@@ -13,7 +13,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libnhip.so")
-SOURCES = ["runtime.cpp", "kernels.hip", "attention.hip"]
+SOURCES = ["runtime.cpp", "kernels.hip", "attention.hip", "operators.hip"]
 # Per-source flags. The flash backward's dK/dV kernel holds ~330 registers (one wave a SIMD); with MFMA
 # results in VGPRs the allocator keeps the K/V operands in AGPRs instead of shuttling the dK/dV accumulators
 # between AGPRs and VGPRs on every tile.

@@ -18,6 +18,7 @@ from __future__ import annotations
 import math
 from dataclasses import dataclass, field, replace
 
+from lumen_amd.compiler import operators
 from lumen_amd.graph.ir import ELEMENTWISE, Graph
 
 LAYOUT = {"reshape", "broadcast_in_dim", "transpose", "slice", "concatenate", "swap_pairs"}
@@ -264,8 +265,11 @@ def fuse(graph: Graph, fuse_loops=True, packed=frozenset()) -> list:
             node = nodes[0]
             kind = {"dot_general": "dot"}.get(node.prim, node.prim)
             if node.prim == "fusion":
-                kind = {"flash_attention": "flash_fwd", "flash_attention_backward": "flash_bwd"}[node.params["name"]]
+                kind = {"flash_attention": "flash_fwd", "flash_attention_backward": "flash_bwd", **operators.KINDS}[
+                    node.params["name"]]
             st = Step(kind, nodes, outs)
+            if kind in operators.KINDS.values():
+                st.scratch = operators.scratch_bytes(graph, node)
             if kind in ("flash_fwd", "flash_bwd"):
                 q = graph.types[node.inputs[0]]
                 if kind == "flash_bwd":

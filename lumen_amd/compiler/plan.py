@@ -20,7 +20,7 @@ from lumen_amd import autotune
 from lumen_amd import dtypes as D
 from lumen_amd import native as nv
 from lumen_amd.compiler import attention as attn_pass
-from lumen_amd.compiler import codegen, fusion, kcache, merge, passes, remat, schedule
+from lumen_amd.compiler import codegen, fusion, kcache, merge, operators, passes, remat, schedule
 from lumen_amd.config import config
 from lumen_amd.graph.ir import Graph
 
@@ -168,6 +168,8 @@ def compile_graph(graph: Graph, packable=()) -> tuple[Graph, list]:
     positions ``packable``,
     simplify again. Returns the graph and merge_dots' packs (weight input positions stored back to back)."""
     g = passes.frontend(graph)
+    if config.compiler.fuse:
+        g = operators.clip_in_consumers(g)
     if config.compiler.flash_attention:
         g = attn_pass.match(g)
         g = passes.frontend(g)
@@ -435,6 +437,7 @@ class Plan:
                 c = st.outputs[0]
                 last_use[c] = max(last_use.get(c, si), si)
 
+        layouts = operators.layouts(self.steps)
         converted = []
         for si, st in enumerate(self.steps):
             if st.kind == "alias":
@@ -447,7 +450,7 @@ class Plan:
                     loc = Loc(src.base, src.offset, _contig(t.shape), t.dtype, t.shape)
                 else:
                     loc = _view_of(n.prim, n.params, src, g.types[n.output])
-                if loc is not None:
+                if loc is not None and operators.reads(loc, layouts.get(n.output)):
                     self.loc[n.output] = loc
                     base_of[n.output] = base_of.get(n.inputs[0], n.inputs[0])
                     continue
@@ -909,6 +912,10 @@ class Plan:
                 kind, desc, ops = attn_pass.lower(self, st)
                 rr = (nv.Reloc * len(ops))(*[reloc(i, l) for i, l in enumerate(ops)])
                 call("nhip_plan_add_builtin", plan, kind, C.byref(desc), C.sizeof(desc), rr, len(ops))
+            elif st.kind in operators.KINDS.values():
+                kind, desc, ops = operators.lower(self, st)
+                rr = (nv.Reloc * len(ops))(*[reloc(i, l) for i, l in ops])
+                call("nhip_plan_add_builtin", plan, kind, desc, len(desc), rr, len(ops))
             elif st.kind == "linear_cross_entropy":
                 n = st.nodes[0]
                 desc = self._lce_desc(n)
@@ -1313,7 +1320,7 @@ class Plan:
 
     def cost(self, si):
         """Algorithmic ``(flops, bytes)`` of step ``si``: dots 2 m n k, flash attention 4 B N Sq Sk D (half of it
-        causal; the backward 2.5x), loop kernels the bytes of their operands' distinct elements and outputs."""
+        causal; the backward 2.5x), gated projections 4 m n k, loop kernels the bytes of their operands' distinct elements and outputs."""
         st = self.steps[si]
         g = self.graph
 
@@ -1345,6 +1352,9 @@ class Plan:
                 sk = k.shape[1]
             f = 4 * b * h * sq * sk * d * (0.5 if n.params["causal"] else 1.0)
             return (f if st.kind == "flash_fwd" else 2.5 * f), io
+        if st.kind == "gated_fwd":
+            x, w = (g.types[v] for v in st.nodes[0].inputs[:2])
+            return 4 * x.numel() * w.shape[0], io
         return 0, io
 
     def describe(self):

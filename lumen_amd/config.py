@@ -46,6 +46,8 @@ class CompilerFlags:
     fused_linear_cross_entropy: bool = True
     # rows a chunk of the fused linear cross entropy backward (None: off, the reference's default)
     fused_linear_cross_entropy_chunk_size: int | None = None
+    # qk_norm_rope, gated_linear and clip_grad_norm run as kernels of their own (off: traced as their primitives)
+    fused_operators: bool = True
     _version: int = 0
 
     def __setattr__(self, name, value):

@@ -1,0 +1,368 @@
+// The gate and up projections of a gated MLP with the activation and the product in their store:
+//
+//   h[t, f] = act(g) u,  g = sum over k of x[t, k] gate[f, k],  u = sum over k of x[t, k] up[f, k]
+//
+// for bf16/f16 x [m, k] and weights [n, k], all contiguous along k. MFMA bounds it (4 m n k operations); the two products
+// share x, and computing both of an element's sums in one lane means that neither g nor u need be written: 2 m n elements
+// not stored and not read again. The sums stay float32 until h is rounded, once. In training the backward needs g and u,
+// which are then stored too, in float32: their rounding to 16 bits would be the largest error of the gradients
+// (three roundings on the way to dx instead of two), and 16 m n bytes of traffic are 7% of the six products' time at
+// [4096, 2048] x [8192, 2048].
+//
+// Three kernels by size and alignment (gated_kind):
+//  * gated_stream: gemm_stream_tile with PAIR 1, tiles of 256 rows x 128 columns or 128 x 64;
+//  * gated_skinny: at most 64 rows, 16 columns a workgroup, the waves divide k (as gemm_skinny);
+//  * gated_any: rows of any length and alignment, 64 x 32 or 128 x 64 tiles through registers.
+//
+// The backward's elementwise half (gated_grad_kernel) turns dh, g and u into [dg | du], one row of 2 n a token, HBM-bound:
+//   du = dh act(g), dg = dh u act'(g)
+// so that [dg | du] is the operand of one product for both weight gradients and of one for dx.
+#pragma once
+
+#include "gemm.h"
+#include "gemm_skinny.h"
+
+namespace nhipk {
+
+enum { kGatedSilu = 0, kGatedGelu = 1, kGatedRelu = 2, kGatedSigmoid = 3 };
+
+constexpr float kLog2e = 1.44269504088896341f;
+
+// 1 / (1 + exp(-x)): x = -inf gives 0, +inf 1, NaN NaN.
+__device__ __forceinline__ float gated_sigmoid(float x) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * x));
+}
+
+// GELU's tanh form written as a sigmoid: (1 + tanh(v)) / 2 = 1 / (1 + exp(-2 v)).
+constexpr float kGeluC = 0.7978845608f, kGeluA = 0.044715f;
+
+__device__ __forceinline__ float gated_act(int act, float g) {
+    if (act == kGatedSilu) return g * gated_sigmoid(g);
+    if (act == kGatedGelu) return g * gated_sigmoid(2.0f * kGeluC * (g + kGeluA * g * g * g));
+    if (act == kGatedRelu) return g <= 0.0f ? 0.0f : g;  // a NaN stays
+    return gated_sigmoid(g);
+}
+
+// act(g) and its derivative.
+__device__ __forceinline__ void gated_act_grad(int act, float g, float &a, float &da) {
+    if (act == kGatedSilu) {
+        const float s = gated_sigmoid(g);
+        a = g * s;
+        da = s * (1.0f + g * (1.0f - s));
+    } else if (act == kGatedGelu) {
+        const float s = gated_sigmoid(2.0f * kGeluC * (g + kGeluA * g * g * g));
+        a = g * s;
+        da = s + a * (1.0f - s) * (2.0f * kGeluC) * (1.0f + 3.0f * kGeluA * g * g);
+    } else if (act == kGatedRelu) {
+        a = g <= 0.0f ? 0.0f : g;
+        da = g > 0.0f ? 1.0f : 0.0f;
+    } else {
+        const float s = gated_sigmoid(g);
+        a = s;
+        da = s * (1.0f - s);
+    }
+}
+
+// Where a kernel's sums go: h (16-bit, rows h_m apart), and g and u (float32, [m, n]) unless null.
+struct GatedOut {
+    void *h;
+    float *g, *u;
+    int32_t act, dtype;  // dtype: 1 bf16, 2 f16
+
+    // One element, for the kernels that store from registers.
+    __device__ __forceinline__ void one(const GemmShape &s, int64_t row, int64_t col, float gv, float uv) const {
+        const float v = gated_act(act, gv) * uv;
+        uint16_t *p = static_cast<uint16_t *>(h) + row * s.d_m + col;
+        *p = dtype == 1 ? f32_to_bf16(v) : f32_to_f16(v);
+        if (g) {
+            g[row * s.n + col] = gv;
+            u[row * s.n + col] = uv;
+        }
+    }
+
+    // gemm_stream_tile's sums of one wave: acc[i][j] and acc[i][j + FN / 2] hold g and u of the same elements, row
+    // 32 i + l32, column 32 j + 8 (e / 4) + 4 (lane / 32) + e % 4. Through the wave's own LDS rows, 64 rows at a time, so
+    // that rows go out in 16-byte pieces; only this wave writes and reads them, which needs no barrier.
+    template <int FM, int FN, int WCOLS>
+    __device__ __forceinline__ void store(const GemmShape &s, const f32x16_t (&acc)[FM][FN], char *stage, int64_t rbase,
+                                          int64_t cbase, int lane) const {
+        constexpr int WC = WCOLS / 2, P = WC * 4 + 16;
+        const int l32 = lane & 31, hl = lane >> 5;
+        GemmShape full = s;  // of g and u
+        full.d_m = s.n;
+        auto out = [&](int half, auto value, const GemmShape &shape, const AnyStore &to) {
+#pragma unroll
+            for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+                for (int j = 0; j < FN / 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const f32x16_t &g_ = acc[2 * half + ii][j], &u_ = acc[2 * half + ii][j + FN / 2];
+                        *reinterpret_cast<float4 *>(stage + (32 * ii + l32) * P + (32 * j + 2 * e + 4 * hl) * 4) =
+                            make_float4(value(g_[e], u_[e]), value(g_[e + 1], u_[e + 1]), value(g_[e + 2], u_[e + 2]),
+                                        value(g_[e + 3], u_[e + 3]));
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            wave_order();
+            stream_store_rows<WC, P>(shape, to, 0, stage, rbase + 64 * half, cbase, lane);
+            wave_order();
+        };
+#pragma unroll
+        for (int half = 0; half < FM / 2; ++half) {
+            if (g) {
+                out(half, [](float a, float) { return a; }, full, AnyStore{g, 0});
+                out(half, [](float, float b) { return b; }, full, AnyStore{u, 0});
+            }
+            // the activation is the same for every element: its branch is taken once
+            if (act == kGatedSilu) out(half, [](float a, float b) { return gated_act(kGatedSilu, a) * b; }, s, AnyStore{h, dtype});
+            else if (act == kGatedGelu) out(half, [](float a, float b) { return gated_act(kGatedGelu, a) * b; }, s, AnyStore{h, dtype});
+            else if (act == kGatedRelu) out(half, [](float a, float b) { return gated_act(kGatedRelu, a) * b; }, s, AnyStore{h, dtype});
+            else out(half, [](float a, float b) { return gated_act(kGatedSigmoid, a) * b; }, s, AnyStore{h, dtype});
+        }
+    }
+
+    // The wave's LDS writes before its reads of them, and the other way round.
+    __device__ __forceinline__ static void wave_order() {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+};
+
+// TM x TM / 2 tiles; WN and KL as gemm_stream's.
+template <bool F16, int TM, int WN, int KL, bool BUF>
+__global__ __launch_bounds__(128 * WN) __attribute__((amdgpu_waves_per_eu(TM == 256 ? WN / 2 : 2, TM == 256 ? WN / 2 : 2))) void
+gated_stream(GemmShape s, const uint16_t *__restrict__ x, const uint16_t *__restrict__ gate, const uint16_t *__restrict__ up,
+             GatedOut out) {
+    extern __shared__ __align__(1024) char smem[];
+    gemm_stream_tile<F16, 64, WN, false, false, BUF, GatedOut, TM, KL, 1>(s, x, gate, out, smem, up);
+}
+
+// Few rows: a workgroup takes 16 columns of both weights, its NW waves divide k 64 at a time, fragments straight from
+// memory (v_mfma_f32_16x16x32: 16 rows of 64 contiguous bytes), the waves' sums added through LDS in wave order. Reading
+// the weights once is all the work.
+template <bool F16, int MT, int NW>
+__global__ __launch_bounds__(64 * NW) void gated_skinny(GemmShape s, const uint16_t *__restrict__ x,
+                                                         const uint16_t *__restrict__ gate, const uint16_t *__restrict__ up,
+                                                         GatedOut out) {
+    constexpr int U = MT == 1 ? 2 : 1;  // chunks of 64 k in flight
+    __shared__ f32x4_t sums[NW][2][MT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+    const int64_t n0 = int64_t(blockIdx.x) * 16;
+    // rows past the last one: the last one again, never stored
+    const int64_t row = min(n0 + l16, s.n - 1) * s.b_n + 8 * g;
+    const uint16_t *pb[2] = {gate + row, up + row};
+    const uint16_t *pa[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) pa[i] = x + min(int64_t(16 * i + l16), s.m - 1) * s.a_m + 8 * g;
+
+    f32x4_t acc[2][MT];
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[w][i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    const int k = int(s.k), step = 64 * NW;
+    int k0 = 64 * wave;
+    for (; k0 + (U - 1) * step + 64 <= k; k0 += U * step) {
+        uint4 fb[U][2][2], fa[U][2][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) fb[u][c][w] = *reinterpret_cast<const uint4 *>(pb[w] + k0 + u * step + 32 * c);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) fa[u][c][i] = *reinterpret_cast<const uint4 *>(pa[i] + k0 + u * step + 32 * c);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) acc[w][i] = mfma16<F16>(fa[u][c][i], fb[u][c][w], acc[w][i]);
+    }
+    for (; k0 < k; k0 += step)  // the last chunks, a lane's 8 k past the end as zeros
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const bool in = k0 + 32 * c + 8 * g < k;
+            const uint4 zero = make_uint4(0, 0, 0, 0);
+            const uint4 f0 = in ? *reinterpret_cast<const uint4 *>(pb[0] + k0 + 32 * c) : zero;
+            const uint4 f1 = in ? *reinterpret_cast<const uint4 *>(pb[1] + k0 + 32 * c) : zero;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const uint4 fa = in ? *reinterpret_cast<const uint4 *>(pa[i] + k0 + 32 * c) : zero;
+                acc[0][i] = mfma16<F16>(fa, f0, acc[0][i]);
+                acc[1][i] = mfma16<F16>(fa, f1, acc[1][i]);
+            }
+        }
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sums[wave][w][i][lane] = acc[w][i];
+    __syncthreads();
+    // C layout of a 16 x 16 block: lane holds column lane % 16, rows 4 (lane / 16) + e
+    if (wave >= MT) return;
+    f32x4_t gv = sums[0][0][wave][lane], uv = sums[0][1][wave][lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) gv += sums[w][0][wave][lane], uv += sums[w][1][wave][lane];
+    const int64_t col = n0 + l16, r0 = 16 * wave + 4 * g;
+    if (col >= s.n) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (r0 + e < s.m) out.one(s, r0 + e, col, gv[e], uv[e]);
+}
+
+// Rows of any length and alignment (load8_any), k of any size: BM rows x BN / 2 columns a workgroup, WM x WN waves, the
+// tile's B lines the gate's BN / 2 rows and then the up projection's, double-buffered through registers.
+template <bool F16, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM *WN * 64) void gated_any(GemmShape s, const uint16_t *__restrict__ x,
+                                                          const uint16_t *__restrict__ gate,
+                                                          const uint16_t *__restrict__ up, GatedOut out) {
+    constexpr int BK = 64, T = WM * WN * 64, P = BK + 8, CH = BK / 8, H = BN / 2;
+    constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
+    constexpr int VA = BM * CH / T, VB = BN * CH / T;
+    static_assert(BM * CH % T == 0 && BN * CH % T == 0 && FN % 2 == 0 && FM > 0, "tile loads divide evenly, pairs of columns");
+    extern __shared__ __align__(16) uint16_t lds[];
+    uint16_t *As = lds, *Bs = lds + 2 * BM * P;
+    int tm, tn;
+    tile_of(blockIdx.x, s.tiles_m, s.tiles_n, tm, tn);
+    const int64_t m0 = int64_t(tm) * BM, n0 = int64_t(tn) * H;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int wm = wave / WN, wn = wave % WN, h = lane >> 5, l32 = lane & 31;
+    uint4 ra[VA], rb[VB];
+    auto load = [&](int64_t k0) {
+#pragma unroll
+        for (int v = 0; v < VA; ++v) {
+            const int idx = t + v * T, line = idx / CH, ch = idx % CH;
+            const int64_t gm = m0 + line, gk = k0 + ch * 8;
+            ra[v] = gm < s.m && gk < s.k ? load8_any(x + gm * s.a_m + gk, s.k - gk) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int v = 0; v < VB; ++v) {
+            const int idx = t + v * T, line = idx / CH, ch = idx % CH;
+            const int64_t gn = n0 + (line < H ? line : line - H), gk = k0 + ch * 8;
+            rb[v] = gn < s.n && gk < s.k ? load8_any((line < H ? gate : up) + gn * s.b_n + gk, s.k - gk) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int v = 0; v < VA; ++v) {
+            const int idx = t + v * T;
+            *reinterpret_cast<uint4 *>(As + buf * BM * P + idx / CH * P + idx % CH * 8) = ra[v];
+        }
+#pragma unroll
+        for (int v = 0; v < VB; ++v) {
+            const int idx = t + v * T;
+            *reinterpret_cast<uint4 *>(Bs + buf * BN * P + idx / CH * P + idx % CH * 8) = rb[v];
+        }
+    };
+    f32x16_t acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+    const int ktiles = int((s.k + BK - 1) / BK);
+    load(0);
+    put(0);
+    __syncthreads();
+    for (int kt = 0; kt < ktiles; ++kt) {
+        const int buf = kt & 1;
+        if (kt + 1 < ktiles) load(int64_t(kt + 1) * BK);
+        const uint16_t *as = As + buf * BM * P, *bs = Bs + buf * BN * P;
+#pragma unroll
+        for (int kk = 0; kk < BK; kk += 16) {
+            uint4 fa[FM], fb[FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const uint4 *>(as + (wm * TM + 32 * i + l32) * P + kk + 8 * h);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const int line = j / (FN / 2) * H + wn * (TN / 2) + 32 * (j % (FN / 2)) + l32;
+                fb[j] = *reinterpret_cast<const uint4 *>(bs + line * P + kk + 8 * h);
+            }
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = Mfma<F16>::run(fa[i], fb[j], acc[i][j]);
+        }
+        if (kt + 1 < ktiles) put(buf ^ 1);
+        __syncthreads();
+    }
+    // C layout of a 32 x 32 block: lane holds column lane % 32, rows 8 * (e / 4) + 4 * (lane / 32) + e % 4
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN / 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int64_t r = m0 + wm * TM + 32 * i + 8 * (e / 4) + 4 * h + e % 4;
+                const int64_t c = n0 + wn * (TN / 2) + 32 * j + l32;
+                if (r < s.m && c < s.n) out.one(s, r, c, acc[i][j][e], acc[i][j + FN / 2][e]);
+            }
+}
+
+template <int BM, int BN>
+constexpr int gated_any_lds_bytes() { return 2 * (BM + BN) * (64 + 8) * 2; }
+
+// [dg | du] of 8 elements a thread (V 8: n, the strides and the pointers multiples of 16 bytes) or of one (V 1).
+struct GatedGrad {
+    const void *dh;
+    const float *g, *u;
+    void *out;  // [m, 2 n]
+    int64_t m, n, dh_m;
+    int32_t act;
+};
+template <typename T, int V>
+__global__ __launch_bounds__(256) void gated_grad_kernel(GatedGrad a) {
+    const int64_t per = a.n / V, total = a.m * per;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+        const int64_t row = i / per, col = (i - row * per) * V;
+        const T *dh = static_cast<const T *>(a.dh) + row * a.dh_m + col;
+        const float *g = a.g + row * a.n + col, *u = a.u + row * a.n + col;
+        T *out = static_cast<T *>(a.out) + row * 2 * a.n + col;
+        float d[V], gv[V], uv[V];
+        if constexpr (V == 8) {
+            const uint4 r = *reinterpret_cast<const uint4 *>(dh);
+            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const T lo{uint16_t(w[k] & 0xffff)}, hi{uint16_t(w[k] >> 16)};
+                d[2 * k] = load_as_f32(&lo), d[2 * k + 1] = load_as_f32(&hi);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k += 4) {
+                const float4 p = *reinterpret_cast<const float4 *>(g + k), q = *reinterpret_cast<const float4 *>(u + k);
+                gv[k] = p.x, gv[k + 1] = p.y, gv[k + 2] = p.z, gv[k + 3] = p.w;
+                uv[k] = q.x, uv[k + 1] = q.y, uv[k + 2] = q.z, uv[k + 3] = q.w;
+            }
+        } else {
+            d[0] = load_as_f32(dh), gv[0] = *g, uv[0] = *u;
+        }
+        T dg[V], du[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            float act, grad;
+            gated_act_grad(a.act, gv[k], act, grad);
+            store_f32_as(&dg[k], d[k] * uv[k] * grad);
+            store_f32_as(&du[k], d[k] * act);
+        }
+        if constexpr (V == 8) {
+            uint4 p, q;
+            __builtin_memcpy(&p, dg, 16);
+            __builtin_memcpy(&q, du, 16);
+            *reinterpret_cast<uint4 *>(out) = p;
+            *reinterpret_cast<uint4 *>(out + a.n) = q;
+        } else {
+            out[0] = dg[0];
+            out[a.n] = du[0];
+        }
+    }
+}
+
+}  // namespace nhipk

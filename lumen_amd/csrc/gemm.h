@@ -468,15 +468,27 @@ __device__ __forceinline__ void for_tiles(int ktiles, F &&tile) {
     tiles_block<S>(kt, ktiles - kt, tile);
 }
 
+// The tile line of B fragment j's first row. With PAIR 1 the first half of a wave's fragments are the first operand's
+// columns and the second half the second operand's same columns, so that a lane holds both of an element's sums.
+template <int PAIR, int TN, int WCOLS>
+__device__ __forceinline__ int stream_line(int wn, int j) {
+    if constexpr (PAIR == 1) return j / (WCOLS / 64) * (TN / 2) + wn * (WCOLS / 2) + 32 * (j % (WCOLS / 64));
+    else return wn * WCOLS + 32 * j;
+}
+
 // One workgroup's 256 x 256 output tile. `out` is AnyStore (a plain store of D), or a generated epilogue
 // functor called as out(row, col, float4, pre) with the float32 sums of four consecutive columns (col a
 // multiple of 4, within m x n) and pre = out.load(row, col), its other operands read ahead. `smem` holds gemm_stream_lds_bytes<BK, WN>() bytes.
 // KL, the k loop: 0 fragments of the next k step read under the current step's MFMAs; 1 (XPF) that read also
 // across k tiles; 2 (ping-pong) the two waves of each SIMD alternate between a memory phase and an MFMA phase;
 // 3 (k tile 64, two stages, four waves) the cross-tile read placed by hand with the loads split in halves.
-template <bool F16, int BK, int WN, bool AT, bool BT, bool BUF, class Out, int TM = 256, int KL = 0>
+// PAIR 1: two products of A, by B and by b2 of the same shape and strides: half of the tile's columns are B's, half the
+// same columns of b2, and out.store takes the pairs of sums. PAIR 2: B's first k / 2 rows of k are b's, the others b2's
+// (k / 2 a multiple of BK).
+template <bool F16, int BK, int WN, bool AT, bool BT, bool BUF, class Out, int TM = 256, int KL = 0, int PAIR = 0>
 __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint16_t *__restrict__ a,
-                                                 const uint16_t *__restrict__ b, const Out &out, char *smem) {
+                                                 const uint16_t *__restrict__ b, const Out &out, char *smem,
+                                                 const uint16_t *__restrict__ b2 = nullptr) {
     constexpr int NW = 2 * WN;       // wavefronts (2 x WN)
     constexpr int WR = TM / 2;       // rows a wave
     constexpr int FM = WR / 32;      // 32-row MFMA tiles a wave
@@ -493,7 +505,9 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     tile_of(blockIdx.x, s.tiles_m, s.tiles_n, tm, tn);
     int64_t oa, ob, od;
     batch_offsets(s, blockIdx.y, oa, ob, od);
-    const int64_t m0 = int64_t(tm) * TM, n0 = int64_t(tn) * TM;
+    static_assert(PAIR != 1 || (!BT && FN % 2 == 0), "a pair's halves are rows of k");
+    constexpr int TNB = PAIR == 1 ? TM / 2 : TM;  // columns of one B operand in the tile
+    const int64_t m0 = int64_t(tm) * TM, n0 = int64_t(tn) * TNB;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / WN, wn = wave % WN;
     const int h = lane >> 5, l32 = lane & 31, g = lane >> 4, s16 = lane & 15;
@@ -509,14 +523,18 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     // per-lane 32-bit offset fixed for the whole k loop plus a uniform k offset, with no per-load address
     // arithmetic, and rows past m / n read zeros. Operands whose tile span exceeds 2^31 bytes use 64-bit
     // global addresses instead.
-    const int64_t mrem = s.m - m0 < TM ? s.m - m0 : TM, nrem = s.n - n0 < TM ? s.n - n0 : TM;
+    const int64_t mrem = s.m - m0 < TM ? s.m - m0 : TM, nrem = s.n - n0 < TNB ? s.n - n0 : TNB;
+    const int64_t kb = PAIR == 2 ? s.k / 2 : s.k;  // k of one B operand
     const int64_t abytes = AT ? ((s.k - 1) * s.a_k + mrem) * 2 : ((mrem - 1) * s.a_m + s.k) * 2;
-    const int64_t bbytes = BT ? ((s.k - 1) * s.b_k + nrem) * 2 : ((nrem - 1) * s.b_n + s.k) * 2;
+    const int64_t bbytes = BT ? ((kb - 1) * s.b_k + nrem) * 2 : ((nrem - 1) * s.b_n + kb) * 2;
     constexpr bool buf = BUF;  // the launcher checked stream_buffer_ok()
     const __amdgpu_buffer_rsrc_t rsa = __builtin_amdgcn_make_buffer_rsrc(
         (void *)(AT ? pa + m0 : pa + m0 * s.a_m), (short)0, int(abytes), 0x00020000);
     const __amdgpu_buffer_rsrc_t rsb = __builtin_amdgcn_make_buffer_rsrc(
         (void *)(BT ? pb + n0 : pb + n0 * s.b_n), (short)0, int(bbytes), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rsb2 = __builtin_amdgcn_make_buffer_rsrc(
+        (void *)(PAIR == 0 ? b2 : BT ? b2 + n0 : b2 + n0 * s.b_n), (short)0, int(PAIR == 0 ? 0 : bbytes), 0x00020000);
+    (void)rsb2;
     auto issue = [&](int st, int kt, int lo, int hi) {
         char *base = smem + st * STAGE_BYTES;
         const int64_t k0 = int64_t(kt) * BK;
@@ -548,6 +566,26 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
         for (int i = 0; i < TB::segs / NW; ++i) {
             if (TA::segs / NW + i < lo || TA::segs / NW + i >= hi) continue;
             const int seg = wave_u + NW * i;
+            if constexpr (PAIR != 0) {
+                // PAIR 1: the upper half of a wave's segments is the second operand's; PAIR 2: the upper half of k is
+                const bool up = PAIR == 1 ? i >= TB::segs / NW / 2 : k0 >= kb;
+                const int line = seg * TB::lines_per_seg + lane / TB::chunks - (PAIR == 1 && up ? TNB : 0), c = lane % TB::chunks;
+                const int64_t k1 = PAIR == 2 && up ? k0 - kb : k0;
+                if constexpr (buf) {
+                    const uint32_t vo = BT ? uint32_t((line * s.b_k + ((c ^ mnmaj_swz(line)) << 3)) * 2)
+                                           : uint32_t((line * s.b_n + ((c ^ kmaj_swz<BK>(line)) << 3)) * 2);
+                    const uint32_t so = BT ? uint32_t(k1 * s.b_k * 2) : uint32_t(k1 * 2);
+                    glds_void_t *to = (glds_void_t *)(base + TA::bytes + seg * 1024);
+                    if (up) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsb2, to, 16, vo, so, 0, 0);
+                    else __builtin_amdgcn_raw_ptr_buffer_load_lds(rsb, to, 16, vo, so, 0, 0);
+                } else {
+                    const uint16_t *p = up ? b2 : pb;
+                    if (BT) p += (k1 + line) * s.b_k + min(n0 + ((c ^ mnmaj_swz(line)) << 3), s.n - 8);
+                    else p += min(n0 + line, s.n - 1) * s.b_n + k1 + ((c ^ kmaj_swz<BK>(line)) << 3);
+                    __builtin_amdgcn_global_load_lds(p, (glds_void_t *)(base + TA::bytes + seg * 1024), 16, 0, 0);
+                }
+                continue;
+            }
             const int line = seg * TB::lines_per_seg + lane / TB::chunks, c = lane % TB::chunks;
             if constexpr (buf) {
                 const uint32_t vo = BT ? uint32_t((line * s.b_k + ((c ^ mnmaj_swz(line)) << 3)) * 2)
@@ -613,7 +651,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
         auto read1 = [&](const char *ta_, int buf, int kk, int q) {  // q-th fragment: A 0, B 0 .. FN - 1, A 1 ..
             const char *tb_ = ta_ + TA::bytes;
             if (q == 0) fa[buf][0] = frag(ta_, wm * WR, kk, std::integral_constant<bool, AT>{});
-            else if (q <= FN) fb[buf][q - 1] = frag(tb_, wn * WCOLS + 32 * (q - 1), kk, std::integral_constant<bool, BT>{});
+            else if (q <= FN) fb[buf][q - 1] = frag(tb_, stream_line<PAIR, TM, WCOLS>(wn, q - 1), kk, std::integral_constant<bool, BT>{});
             else fa[buf][q - FN] = frag(ta_, wm * WR + 32 * (q - FN), kk, std::integral_constant<bool, AT>{});
         };
         issue(0, 0, 0, LPS);
@@ -694,7 +732,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
 #pragma unroll
                 for (int ii = 0; ii < FM; ++ii) fa[i][ii] = frag(ta, wm * WR + 32 * ii, 16 * i, std::integral_constant<bool, AT>{});
 #pragma unroll
-                for (int j = 0; j < FN; ++j) fb[i][j] = frag(tb, wn * WCOLS + 32 * j, 16 * i, std::integral_constant<bool, BT>{});
+                for (int j = 0; j < FN; ++j) fb[i][j] = frag(tb, stream_line<PAIR, TM, WCOLS>(wn, j), 16 * i, std::integral_constant<bool, BT>{});
             }
             wait_tiles(min(STAGES - 2, ktiles - 2 - kt));
             __builtin_amdgcn_sched_barrier(0);
@@ -729,7 +767,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
             const char *tb = ta + TA::bytes;
             fa[buf][0] = frag(ta, wm * WR, kk, std::integral_constant<bool, AT>{});
 #pragma unroll
-            for (int j = 0; j < FN; ++j) fb[buf][j] = frag(tb, wn * WCOLS + 32 * j, kk, std::integral_constant<bool, BT>{});
+            for (int j = 0; j < FN; ++j) fb[buf][j] = frag(tb, stream_line<PAIR, TM, WCOLS>(wn, j), kk, std::integral_constant<bool, BT>{});
 #pragma unroll
             for (int i = 1; i < FM; ++i) fa[buf][i] = frag(ta, wm * WR + 32 * i, kk, std::integral_constant<bool, AT>{});
         };
@@ -764,7 +802,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
             auto read1 = [&](const char *ta_, int buf, int kk, int q) {  // q-th fragment in read()'s order
                 const char *tb_ = ta_ + TA::bytes;
                 if (q == 0) fa[buf][0] = frag(ta_, wm * WR, kk, std::integral_constant<bool, AT>{});
-                else if (q <= FN) fb[buf][q - 1] = frag(tb_, wn * WCOLS + 32 * (q - 1), kk, std::integral_constant<bool, BT>{});
+                else if (q <= FN) fb[buf][q - 1] = frag(tb_, stream_line<PAIR, TM, WCOLS>(wn, q - 1), kk, std::integral_constant<bool, BT>{});
                 else fa[buf][q - FN] = frag(ta_, wm * WR + 32 * (q - FN), kk, std::integral_constant<bool, AT>{});
             };
             for_tiles<STAGES>(ktiles, [&](int kt, auto pc) {
@@ -859,7 +897,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
         auto read = [&](int buf, int kk) {  // in the order the MFMAs (i-major) first use them
             fa[buf][0] = frag(ta, wm * WR, kk, std::integral_constant<bool, AT>{});
 #pragma unroll
-            for (int j = 0; j < FN; ++j) fb[buf][j] = frag(tb, wn * WCOLS + 32 * j, kk, std::integral_constant<bool, BT>{});
+            for (int j = 0; j < FN; ++j) fb[buf][j] = frag(tb, stream_line<PAIR, TM, WCOLS>(wn, j), kk, std::integral_constant<bool, BT>{});
 #pragma unroll
             for (int i = 1; i < FM; ++i) fa[buf][i] = frag(ta, wm * WR + 32 * i, kk, std::integral_constant<bool, AT>{});
         };
@@ -896,10 +934,14 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
 
     // acc[i][j][e]: row m0 + wm*WR + 32 i + l32, column n0 + wn*WCOLS + 32 j + 8 (e / 4) + 4 h + e % 4.
     // Staged through LDS as float32, 64 rows of the wave at a time, then written row-wise.
-    const int64_t rbase = m0 + wm * WR, cbase = n0 + wn * WCOLS;
+    const int64_t rbase = m0 + wm * WR, cbase = n0 + wn * (PAIR == 1 ? WCOLS / 2 : WCOLS);
     constexpr int PITCH = gemm_stream_stage_pitch<WN, TM>();
     __syncthreads();  // operand stages are dead: reuse LDS for the output
     char *stage = smem + wave * (64 * PITCH);
+    if constexpr (PAIR == 1) {
+        out.template store<FM, FN, WCOLS>(s, acc, stage, rbase, cbase, lane);
+        return;
+    } else {
     // a generated epilogue reads its other operands with Out::load(row, col) into Out::Pre, kPrefetch chunks of
     // four columns at a time: the first group's loads are issued before the sums are staged, so their latency
     // overlaps the staging and the barrier instead of stalling every chunk
@@ -967,6 +1009,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
             const int64_t gc = cbase + 4 * lane;
             if (lane < CPR && gc < s.n && rbase < s.m) out.colsum_add(gc, colsum);
         }
+    }
     }
 }
 
@@ -1213,7 +1256,7 @@ __host__ __device__ inline bool stream_buffer_ok(int64_t m, int64_t n, int64_t k
 
 // Split-k reduction: D[z, r, c] = sum over splits of the float32 partials P[split][z][r][c] (contiguous,
 // `mn` = m * n elements a batch), in split order, rounded once to D's dtype.
-__global__ __launch_bounds__(256) void gemm_splitk_reduce(GemmShape s, const float *__restrict__ part, int splits,
+static __global__ __launch_bounds__(256) void gemm_splitk_reduce(GemmShape s, const float *__restrict__ part, int splits,
                                                            int64_t total, AnyStore out) {
     const int64_t mn = s.m * s.n;
     out.visit([&](auto stf) {

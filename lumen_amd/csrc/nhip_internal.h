@@ -26,5 +26,15 @@ int flash_bwd_on(hipStream_t s, const nhip_attn_desc *d, const void *q, const vo
 int fill_on(hipStream_t s, void *dst, size_t bytes, unsigned char value);
 int lce_on(hipStream_t s, const nhip_lce_desc *d, const void *h, const void *w, const void *target, float *out,
            void *ws);
+int heads_on(hipStream_t s, const nhip_heads_desc *d, const void *q, const void *k, const void *qw, const void *kw,
+             const float *cos, const float *sin, const void *pos, void *oq, void *ok);
+int heads_bwd_on(hipStream_t s, const nhip_heads_desc *d, const void *q, const void *k, const void *qw, const void *kw,
+                 const float *cos, const float *sin, const void *pos, const void *doq, const void *dok, void *dq, void *dk,
+                 void *dqw, void *dkw, void *ws);
+int gated_on(hipStream_t s, const nhip_gated_desc *d, const void *x, const void *gate, const void *up, void *h, float *g,
+             float *u);
+int gated_grad_on(hipStream_t s, const nhip_gated_desc *d, const void *dh, const float *g, const float *u, void *dgu);
+int clip_on(hipStream_t s, const nhip_clip_desc *d, const nhip_clip_tensor *t, const double *max_at, float *norm,
+            float *scale, void *ws);
 
 }  // namespace nhip

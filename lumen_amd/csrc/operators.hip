@@ -1,0 +1,467 @@
+// C entry points of the head norms with rotation (heads.h), the gated projections (gated.h) and gradient clipping (clip.h).
+#include <cstring>
+
+#include "clip.h"
+#include "gated.h"
+#include "heads.h"
+#include "nhip_internal.h"
+
+using namespace nhipk;
+
+namespace nhip {
+namespace {
+
+bool on(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// ---- heads ----------------------------------------------------------------------------------------------
+
+constexpr int64_t kHeadsLaunchRows = int64_t(1) << 30;  // heads of a launch: row arithmetic is 32-bit
+constexpr int64_t kHeadsBlocks = 1024;                  // workgroups of a backward launch: their partial sums are read again
+
+FastDiv fast_div(uint32_t d) {
+    FastDiv f{d, 0, 0};
+    while (f.shift < 31 && (uint32_t(1) << f.shift) < d) ++f.shift;
+    f.mul = uint32_t(((uint64_t(1) << 32) * ((uint64_t(1) << f.shift) - d)) / d + 1);
+    return f;
+}
+
+int heads_check(const nhip_heads_desc *d, const char *what) {
+    const std::string at(what);
+    if (d->batch < 0 || d->seq < 0 || d->heads < 0 || d->kv_heads < 0) return fail(at + ": negative sizes");
+    if (d->head_dim < 1 || d->head_dim > kHeadsMost)
+        return fail(at + ": a head dim of " + std::to_string(d->head_dim) + ": 1 to " + std::to_string(kHeadsMost));
+    if (d->rot < 0 || d->rot > d->head_dim || d->rot % 2)
+        return fail(at + ": " + std::to_string(d->rot) + " rotated elements: an even number up to the head dim");
+    if (d->seq >= (int64_t(1) << 30) || d->heads >= (int64_t(1) << 20) || d->kv_heads >= (int64_t(1) << 20))
+        return fail(at + ": sequences below 2^30 and heads below 2^20");
+    if (d->table_rows < 1 && d->rot > 0 && d->batch * d->seq > 0) return fail(at + ": an empty table");
+    if (d->dtype != NHIP_F32 && d->dtype != NHIP_BF16 && d->dtype != NHIP_F16) return fail(at + ": heads are float32, bf16 or f16");
+    if (d->positions < NHIP_POS_NONE || d->positions > NHIP_POS_I64) return fail(at + ": positions are int32, int64 or none");
+    return 0;
+}
+
+// Tokens of one launch.
+int64_t heads_tokens(const nhip_heads_desc *d) {
+    int64_t most = d->heads > d->kv_heads ? d->heads : d->kv_heads;
+    most = kHeadsLaunchRows / (most > 0 ? most : 1);
+    const int64_t tokens = d->batch * d->seq;
+    return tokens < most ? tokens : most;
+}
+
+// Elements a chunk of the vector kernels, or 0: the general kernel. Both of a row's chunks start on a chunk's bytes.
+struct HeadsPlan {
+    int e, lanes;
+    int64_t launches;
+};
+
+bool heads_strides(const nhip_heads_desc *d, int e, bool bwd) {
+    const int64_t st[] = {d->q_b,  d->q_s,  d->q_n,  d->k_b,  d->k_s,  d->k_n,  d->oq_b, d->oq_s, d->oq_n,
+                          d->ok_b, d->ok_s, d->ok_n, d->dq_b, d->dq_s, d->dq_n, d->dk_b, d->dk_s, d->dk_n};
+    for (int i = 0; i < (bwd ? 18 : 12); ++i)
+        if (st[i] % e) return false;
+    return true;
+}
+
+HeadsPlan heads_plan(const nhip_heads_desc *d, bool bwd, std::initializer_list<const void *> heads, const float *cos,
+                     const float *sin) {
+    HeadsPlan p;
+    const int64_t tokens = d->batch * d->seq, each = heads_tokens(d);
+    p.launches = each ? (tokens + each - 1) / each : 0;
+    p.e = 0;
+    for (int e : {8, 4}) {
+        if (e == 8 && d->dtype == NHIP_F32) continue;  // 4 elements are 16 bytes
+        const size_t bytes = size_t(e) * (d->dtype == NHIP_F32 ? 4 : 2);
+        bool ok = d->head_dim % (2 * e) == 0 && d->rot % (2 * e) == 0 && d->head_dim / (2 * e) <= 64 && heads_strides(d, e, bwd);
+        for (const void *h : heads) ok = ok && on(h, bytes);
+        ok = ok && on(cos, 16) && on(sin, 16);
+        if (ok) {
+            p.e = e;
+            break;
+        }
+    }
+    const int64_t need = p.e ? d->head_dim / (2 * p.e) : d->rot / 2 + (d->head_dim - d->rot + 1) / 2;
+    p.lanes = p.e ? 1 : 32;
+    while (p.lanes < need && p.lanes < 64) p.lanes *= 2;
+    return p;
+}
+
+// Workgroups of tensor `rows` of a backward launch of `both` rows in all.
+int64_t heads_bwd_blocks(int64_t rows, int64_t both) {
+    if (rows == 0) return 0;
+    const int64_t share = (kHeadsBlocks * rows + both - 1) / both, need = (rows + 7) / 8;
+    return share < need ? share : need;
+}
+
+struct HeadsBlocks {
+    int64_t q, k;
+};
+HeadsBlocks heads_parts(const nhip_heads_desc *d) {
+    const int64_t t = heads_tokens(d), q = t * d->heads, k = t * d->kv_heads;
+    return {heads_bwd_blocks(q, q + k), heads_bwd_blocks(k, q + k)};
+}
+
+size_t heads_workspace(const nhip_heads_desc *d) {
+    const int64_t tokens = d->batch * d->seq, each = heads_tokens(d);
+    if (each == 0) return 0;
+    const HeadsBlocks b = heads_parts(d);
+    return size_t((tokens + each - 1) / each) * size_t(b.q + b.k) * size_t(d->head_dim) * 4;
+}
+
+template <typename T, int E>
+int heads_launch_fwd(hipStream_t st, HeadsArgs &a, int64_t most) {
+    // four rows a group of lanes where that still leaves every CU two workgroups: [4, 4096, 16 + 16, 128] in one launch
+    const uint32_t groups = 256 / a.lanes;
+    const bool many = most / (4 * groups) >= 512;
+    const uint32_t per = groups * (many ? 4 : 1);
+    for (HeadsTensor &t : a.t) t.blocks = (t.rows + per - 1) / per;
+    const uint32_t grid = a.t[0].blocks + a.t[1].blocks;
+    if (!grid) return 0;
+    if (many) hipLaunchKernelGGL((heads_fwd_kernel<T, E, 4>), dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((heads_fwd_kernel<T, E, 1>), dim3(grid), dim3(256), 0, st, a);
+    return check(hipGetLastError(), "heads_fwd_kernel launch");
+}
+
+template <typename T>
+int heads_launch(hipStream_t st, HeadsArgs &a, int e, bool bwd) {
+    const int64_t rows = int64_t(a.t[0].rows) + a.t[1].rows;
+    if (!bwd) {
+        if constexpr (!std::is_same<T, float>::value)
+            if (e == 8) return heads_launch_fwd<T, 8>(st, a, rows);
+        if (e == 4) return heads_launch_fwd<T, 4>(st, a, rows);
+        for (HeadsTensor &t : a.t) {
+            const int64_t blocks = (int64_t(t.rows) * a.lanes + 255) / 256;
+            t.blocks = uint32_t(blocks < 16384 ? blocks : 16384);
+        }
+        const uint32_t grid = a.t[0].blocks + a.t[1].blocks;
+        if (!grid) return 0;
+        hipLaunchKernelGGL((heads_any_kernel<T, false>), dim3(grid), dim3(256), 0, st, a);
+        return check(hipGetLastError(), "heads_any_kernel launch");
+    }
+    const uint32_t grid = a.t[0].blocks + a.t[1].blocks;
+    if (!grid) return 0;
+    if constexpr (!std::is_same<T, float>::value) {
+        if (e == 8) {
+            hipLaunchKernelGGL((heads_bwd_kernel<T, 8, 2>), dim3(grid), dim3(256), 0, st, a);
+            return check(hipGetLastError(), "heads_bwd_kernel launch");
+        }
+    }
+    if (e == 4) hipLaunchKernelGGL((heads_bwd_kernel<T, 4, 2>), dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((heads_any_kernel<T, true>), dim3(grid), dim3(256), 0, st, a);
+    return check(hipGetLastError(), "heads_bwd_kernel launch");
+}
+
+HeadsArgs heads_args(const nhip_heads_desc *d, const HeadsPlan &p, const void *q, const void *k, const void *qw, const void *kw,
+                     const float *cos, const float *sin, const void *pos) {
+    HeadsArgs a;
+    std::memset(&a, 0, sizeof(a));
+    HeadsTensor &x = a.t[0], &y = a.t[1];
+    x.x = q, y.x = k, x.w = qw, y.w = kw;
+    x.x_b = d->q_b, x.x_s = d->q_s, x.x_n = d->q_n, y.x_b = d->k_b, y.x_s = d->k_s, y.x_n = d->k_n;
+    x.y_b = d->oq_b, x.y_s = d->oq_s, x.y_n = d->oq_n, y.y_b = d->ok_b, y.y_s = d->ok_s, y.y_n = d->ok_n;
+    x.dy_b = d->dq_b, x.dy_s = d->dq_s, x.dy_n = d->dq_n, y.dy_b = d->dk_b, y.dy_s = d->dk_s, y.dy_n = d->dk_n;
+    x.heads = fast_div(uint32_t(d->heads > 0 ? d->heads : 1));
+    y.heads = fast_div(uint32_t(d->kv_heads > 0 ? d->kv_heads : 1));
+    a.cos = cos, a.sin = sin;
+    a.positions = d->positions == NHIP_POS_NONE ? nullptr : pos;
+    a.pos64 = d->positions == NHIP_POS_I64;
+    a.table_rows = d->table_rows > 0 ? d->table_rows : 1;
+    a.seq = d->seq;
+    a.seq_div = fast_div(uint32_t(d->seq > 0 ? d->seq : 1));
+    a.d = int(d->head_dim), a.rot = int(d->rot), a.interleaved = d->interleaved != 0;
+    a.lanes = p.lanes;
+    a.eps = d->eps;
+    return a;
+}
+
+template <class F>
+int by_type(int dtype, F &&f) {
+    if (dtype == NHIP_F32) return f(float{});
+    if (dtype == NHIP_BF16) return f(bf16_t{});
+    return f(f16_t{});
+}
+
+}  // namespace
+
+int heads_on(hipStream_t st, const nhip_heads_desc *d, const void *q, const void *k, const void *qw, const void *kw,
+             const float *cos, const float *sin, const void *pos, void *oq, void *ok) {
+    if (heads_check(d, "nhip_qk_norm_rope")) return 1;
+    if (d->positions != NHIP_POS_NONE && !pos && d->batch * d->seq > 0) return fail("nhip_qk_norm_rope: no positions");
+    const HeadsPlan p = heads_plan(d, false, {q, k, qw, kw, oq, ok}, cos, sin);
+    HeadsArgs a = heads_args(d, p, q, k, qw, kw, cos, sin, pos);
+    a.t[0].y = oq, a.t[1].y = ok;
+    const int64_t tokens = d->batch * d->seq, each = heads_tokens(d);
+    for (int64_t t0 = 0; t0 < tokens; t0 += each) {
+        const int64_t n = tokens - t0 < each ? tokens - t0 : each;
+        a.token0 = t0;
+        a.t[0].rows = uint32_t(n * d->heads), a.t[1].rows = uint32_t(n * d->kv_heads);
+        if (by_type(d->dtype, [&](auto t) { return heads_launch<decltype(t)>(st, a, p.e, false); })) return 1;
+    }
+    return 0;
+}
+
+int heads_bwd_on(hipStream_t st, const nhip_heads_desc *d, const void *q, const void *k, const void *qw, const void *kw,
+                 const float *cos, const float *sin, const void *pos, const void *doq, const void *dok, void *dq, void *dk,
+                 void *dqw, void *dkw, void *ws) {
+    if (heads_check(d, "nhip_qk_norm_rope_bwd")) return 1;
+    const int64_t tokens = d->batch * d->seq, each = heads_tokens(d);
+    if (d->positions != NHIP_POS_NONE && !pos && tokens > 0) return fail("nhip_qk_norm_rope_bwd: no positions");
+    if ((dqw || dkw) && !ws && heads_workspace(d) > 0) return fail("nhip_qk_norm_rope_bwd: no workspace");
+    const HeadsPlan p = heads_plan(d, true, {q, k, qw, kw, doq, dok, dq, dk}, cos, sin);
+    HeadsArgs a = heads_args(d, p, q, k, qw, kw, cos, sin, pos);
+    a.t[0].dy = doq, a.t[1].dy = dok, a.t[0].y = dq, a.t[1].y = dk;
+    const HeadsBlocks b = heads_parts(d);
+    float *pq = static_cast<float *>(ws), *pk = pq ? pq + p.launches * b.q * d->head_dim : nullptr;
+    for (int64_t i = 0; i < p.launches; ++i) {
+        const int64_t t0 = i * each, n = tokens - t0 < each ? tokens - t0 : each;
+        a.token0 = t0;
+        a.t[0].rows = uint32_t(n * d->heads), a.t[1].rows = uint32_t(n * d->kv_heads);
+        a.t[0].blocks = uint32_t(b.q), a.t[1].blocks = uint32_t(b.k);
+        a.t[0].part = dqw ? pq + i * b.q * d->head_dim : nullptr;
+        a.t[1].part = dkw ? pk + i * b.k * d->head_dim : nullptr;
+        if (by_type(d->dtype, [&](auto t) { return heads_launch<decltype(t)>(st, a, p.e, true); })) return 1;
+    }
+    if (!dqw && !dkw) return 0;
+    HeadsSum s;
+    s.part[0] = pq, s.part[1] = pk, s.out[0] = dqw, s.out[1] = dkw;
+    s.rows[0] = uint32_t(p.launches * b.q), s.rows[1] = uint32_t(p.launches * b.k);
+    s.d = int(d->head_dim);
+    return by_type(d->dtype, [&](auto t) {
+        hipLaunchKernelGGL((heads_sum_kernel<decltype(t)>), dim3(unsigned((d->head_dim + 63) / 64), 2), dim3(1024), 0, st, s);
+        return check(hipGetLastError(), "heads_sum_kernel launch");
+    });
+}
+
+// ---- gated projections ----------------------------------------------------------------------------------
+
+namespace {
+
+enum { kSkinnyCfg = 0, kStream256a, kStream256b, kStream128Cfg, kAny128, kAny64, kGatedConfigs };
+
+int gated_check(const nhip_gated_desc *d, const char *what) {
+    const std::string at(what);
+    if (d->m < 0 || d->n < 0 || d->k < 0) return fail(at + ": negative sizes");
+    if (d->dtype != NHIP_BF16 && d->dtype != NHIP_F16) return fail(at + ": bf16 or f16");
+    if (d->activation < NHIP_ACT_SILU || d->activation > NHIP_ACT_SIGMOID) return fail(at + ": unknown activation");
+    return 0;
+}
+
+bool gated_rows16(const nhip_gated_desc *d, const void *x, const void *gate, const void *up) {
+    return d->x_m % 8 == 0 && d->w_n % 8 == 0 && on(x, 16) && on(gate, 16) && on(up, 16);
+}
+
+bool gated_takes(const nhip_gated_desc *d, int cfg, bool rows16) {
+    switch (cfg) {
+        case kSkinnyCfg: return rows16 && d->m <= 64 && d->k % 8 == 0 && d->k < (int64_t(1) << 30);
+        case kStream256a:
+        case kStream256b:
+        case kStream128Cfg: return rows16 && d->k % 64 == 0;
+        default: return true;
+    }
+}
+
+int64_t tiles(int64_t m, int64_t bm, int64_t n, int64_t bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); }
+
+int gated_default(const nhip_gated_desc *d, bool rows16) {
+    if (gated_takes(d, kSkinnyCfg, rows16)) return kSkinnyCfg;
+    if (gated_takes(d, kStream128Cfg, rows16)) {
+        if (tiles(d->m, 256, d->n, 128) >= 256) return kStream256b;
+        if (tiles(d->m, 128, d->n, 64) >= 128) return kStream128Cfg;
+    }
+    return tiles(d->m, 128, d->n, 64) >= 512 ? kAny128 : kAny64;
+}
+
+template <class K>
+int gated_go(hipStream_t st, K kern, GemmShape s, int bm, int bn, int threads, int lds, const void *x, const void *gate,
+             const void *up, const GatedOut &out) {
+    s.tiles_m = int((s.m + bm - 1) / bm);
+    s.tiles_n = int((s.n + bn - 1) / bn);
+    if (int64_t(s.tiles_m) * s.tiles_n > 0x7fffffff) return fail("nhip_gated_linear: too many tiles");
+    if (lds > 64 * 1024 &&
+        check(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
+              "hipFuncSetAttribute"))
+        return 1;
+    hipLaunchKernelGGL(kern, dim3(unsigned(s.tiles_m * s.tiles_n)), dim3(threads), lds, st, s, static_cast<const uint16_t *>(x),
+                       static_cast<const uint16_t *>(gate), static_cast<const uint16_t *>(up), out);
+    return check(hipGetLastError(), "gated kernel launch");
+}
+
+template <bool F16>
+int gated_run(hipStream_t st, int cfg, const GemmShape &s, const void *x, const void *gate, const void *up, const GatedOut &o) {
+    const bool buf = stream_buffer_ok(s.m, s.n, s.k, false, false, s.a_m, 1, 1, s.b_n);
+    constexpr int lds4 = gemm_stream_lds_bytes<64, 2>(), lds8 = gemm_stream_lds_bytes<64, 4>();
+    constexpr int lds1 = gemm_stream_lds_bytes<64, 2, 128>();
+    switch (cfg) {
+        case kSkinnyCfg: {
+            if (s.m <= 16) return gated_go(st, gated_skinny<F16, 1, 8>, s, 64, 16, 512, 0, x, gate, up, o);
+            if (s.m <= 32) return gated_go(st, gated_skinny<F16, 2, 8>, s, 64, 16, 512, 0, x, gate, up, o);
+            return gated_go(st, gated_skinny<F16, 4, 4>, s, 64, 16, 256, 0, x, gate, up, o);
+        }
+        case kStream256a:
+            if (buf) return gated_go(st, gated_stream<F16, 256, 2, 3, true>, s, 256, 128, 256, lds4, x, gate, up, o);
+            return gated_go(st, gated_stream<F16, 256, 2, 3, false>, s, 256, 128, 256, lds4, x, gate, up, o);
+        case kStream256b:
+            if (buf) return gated_go(st, gated_stream<F16, 256, 4, 3, true>, s, 256, 128, 512, lds8, x, gate, up, o);
+            return gated_go(st, gated_stream<F16, 256, 4, 3, false>, s, 256, 128, 512, lds8, x, gate, up, o);
+        case kStream128Cfg:
+            if (buf) return gated_go(st, gated_stream<F16, 128, 2, 0, true>, s, 128, 64, 256, lds1, x, gate, up, o);
+            return gated_go(st, gated_stream<F16, 128, 2, 0, false>, s, 128, 64, 256, lds1, x, gate, up, o);
+        case kAny128:
+            return gated_go(st, gated_any<F16, 128, 128, 2, 2>, s, 128, 64, 256, gated_any_lds_bytes<128, 128>(), x, gate, up, o);
+        default:
+            return gated_go(st, gated_any<F16, 64, 64, 2, 1>, s, 64, 32, 128, gated_any_lds_bytes<64, 64>(), x, gate, up, o);
+    }
+}
+
+}  // namespace
+
+int gated_on(hipStream_t st, const nhip_gated_desc *d, const void *x, const void *gate, const void *up, void *h, float *g,
+             float *u) {
+    if (gated_check(d, "nhip_gated_linear")) return 1;
+    if (!g != !u) return fail("nhip_gated_linear: g and u go together");
+    if (d->m == 0 || d->n == 0) return 0;
+    GemmShape s;
+    std::memset(&s, 0, sizeof(s));
+    s.m = d->m, s.n = d->n, s.k = d->k;
+    s.a_m = d->x_m, s.a_k = 1, s.b_k = 1, s.b_n = d->w_n, s.d_m = d->h_m, s.d_n = 1;
+    const bool rows16 = gated_rows16(d, x, gate, up);
+    int cfg = d->config;
+    if (d->k == 0) cfg = kAny64;  // the sums are zeros: no tile is read
+    else if (cfg < 0) cfg = gated_default(d, rows16);
+    else if (cfg >= kGatedConfigs || !gated_takes(d, cfg, rows16))
+        return fail("nhip_gated_linear: config " + std::to_string(cfg) + " does not take these operands");
+    const GatedOut o{h, g, u, d->activation, d->dtype};
+    return d->dtype == NHIP_F16 ? gated_run<true>(st, cfg, s, x, gate, up, o) : gated_run<false>(st, cfg, s, x, gate, up, o);
+}
+
+int gated_grad_on(hipStream_t st, const nhip_gated_desc *d, const void *dh, const float *g, const float *u, void *dgu) {
+    if (gated_check(d, "nhip_gated_linear_grad")) return 1;
+    if (d->m == 0 || d->n == 0) return 0;
+    GatedGrad a{dh, g, u, dgu, d->m, d->n, d->h_m, d->activation};
+    const bool vec = d->n % 8 == 0 && d->h_m % 8 == 0 && on(dh, 16) && on(g, 16) && on(u, 16) && on(dgu, 16);
+    const int64_t work = d->m * (vec ? d->n / 8 : d->n), blocks = (work + 255) / 256;
+    const dim3 grid(unsigned(blocks < 8192 ? blocks : 8192));
+    if (d->dtype == NHIP_F16) {
+        if (vec) hipLaunchKernelGGL((gated_grad_kernel<f16_t, 8>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((gated_grad_kernel<f16_t, 1>), grid, dim3(256), 0, st, a);
+    } else {
+        if (vec) hipLaunchKernelGGL((gated_grad_kernel<bf16_t, 8>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((gated_grad_kernel<bf16_t, 1>), grid, dim3(256), 0, st, a);
+    }
+    return check(hipGetLastError(), "gated_grad_kernel launch");
+}
+
+// ---- gradient clipping ----------------------------------------------------------------------------------
+
+namespace {
+
+// Launches of at least one table, and the most workgroups one leaves a sum for.
+int64_t clip_launches(int64_t count) { return count <= 0 ? 1 : (count + kClipTensors - 1) / kClipTensors; }
+
+}  // namespace
+
+int clip_on(hipStream_t st, const nhip_clip_desc *d, const nhip_clip_tensor *t, const double *max_at, float *norm,
+            float *scale, void *ws) {
+    if (d->count < 0) return fail("nhip_clip_grad_norm: negative count");
+    if (!ws) return fail("nhip_clip_grad_norm: no workspace");
+    bool outs = false;
+    for (int64_t i = 0; i < d->count; ++i) {
+        if (t[i].numel < 0) return fail("nhip_clip_grad_norm: negative element count");
+        if (t[i].dtype != NHIP_F32 && t[i].dtype != NHIP_BF16 && t[i].dtype != NHIP_F16)
+            return fail("nhip_clip_grad_norm: tensors are float32, bf16 or f16");
+        if (t[i].numel > 0 && !t[i].in) return fail("nhip_clip_grad_norm: a tensor without memory");
+        outs = outs || (t[i].out && t[i].numel > 0);
+    }
+    const int64_t launches = clip_launches(d->count);
+    double *part = static_cast<double *>(ws);
+    int parts = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        // the norm alone takes one workgroup of the second pass
+        for (int64_t l = 0; l < (pass == 1 && !outs ? 1 : launches); ++l) {
+            ClipTable c;
+            const int64_t first = l * kClipTensors;
+            c.tensors = int(d->count - first < kClipTensors ? d->count - first : kClipTensors);
+            int64_t chunks = 0;
+            for (int i = 0; i < c.tensors; ++i) {
+                const nhip_clip_tensor &x = t[first + i];
+                c.in[i] = x.in, c.out[i] = x.out, c.numel[i] = x.numel, c.dtype[i] = uint8_t(x.dtype);
+                c.first[i] = uint32_t(chunks);
+                chunks += (x.numel + kClipChunk - 1) / kClipChunk;
+                if (chunks > 0x7fffffff) return fail("nhip_clip_grad_norm: over 2^45 elements");
+            }
+            c.first[c.tensors] = uint32_t(chunks);
+            if (pass == 0) {
+                c.blocks = uint32_t(chunks < kClipBlocks ? (chunks ? chunks : 1) : kClipBlocks);
+                hipLaunchKernelGGL(clip_squares_kernel, dim3(c.blocks), dim3(256), 0, st, c, part + parts);
+                if (check(hipGetLastError(), "clip_squares_kernel launch")) return 1;
+                parts += int(c.blocks);
+            } else {
+                c.blocks = uint32_t(!outs || chunks == 0 ? 1 : chunks < 2 * kClipBlocks ? chunks : 2 * kClipBlocks);
+                if (!outs) c.first[c.tensors] = 0;
+                hipLaunchKernelGGL(clip_scale_kernel, dim3(c.blocks), dim3(256), 0, st, c, part, parts, max_at, d->max_norm,
+                                   d->eps, l == 0 ? norm : nullptr, l == 0 ? scale : nullptr);
+                if (check(hipGetLastError(), "clip_scale_kernel launch")) return 1;
+            }
+        }
+    }
+    return 0;
+}
+
+}  // namespace nhip
+
+using namespace nhip;
+
+extern "C" {
+
+#define NHIP_STREAM(st)                    \
+    hipStream_t st = stream_of_current(); \
+    if (!st) return fail("no HIP stream: call nhip_set_device first")
+
+int nhip_qk_norm_rope(const nhip_heads_desc *desc, const void *q, const void *k, const void *q_weight, const void *k_weight,
+                      const float *cos, const float *sin, const void *positions, void *q_out, void *k_out) {
+    NHIP_STREAM(st);
+    return heads_on(st, desc, q, k, q_weight, k_weight, cos, sin, positions, q_out, k_out);
+}
+
+int nhip_qk_norm_rope_bwd(const nhip_heads_desc *desc, const void *q, const void *k, const void *q_weight,
+                          const void *k_weight, const float *cos, const float *sin, const void *positions,
+                          const void *d_q_out, const void *d_k_out, void *dq, void *dk, void *d_q_weight, void *d_k_weight,
+                          void *workspace) {
+    NHIP_STREAM(st);
+    return heads_bwd_on(st, desc, q, k, q_weight, k_weight, cos, sin, positions, d_q_out, d_k_out, dq, dk, d_q_weight,
+                        d_k_weight, workspace);
+}
+
+int nhip_qk_norm_rope_workspace(const nhip_heads_desc *desc, size_t *bytes) {
+    if (heads_check(desc, "nhip_qk_norm_rope_workspace")) return 1;
+    *bytes = heads_workspace(desc);
+    return 0;
+}
+
+int nhip_gated_linear(const nhip_gated_desc *desc, const void *x, const void *gate, const void *up, void *h, float *g, float *u) {
+    NHIP_STREAM(st);
+    return gated_on(st, desc, x, gate, up, h, g, u);
+}
+
+int nhip_gated_config_count(int *count) {
+    *count = kGatedConfigs;
+    return 0;
+}
+
+int nhip_gated_linear_grad(const nhip_gated_desc *desc, const void *dh, const float *g, const float *u, void *dgu) {
+    NHIP_STREAM(st);
+    return gated_grad_on(st, desc, dh, g, u, dgu);
+}
+
+int nhip_clip_grad_norm(const nhip_clip_desc *desc, const nhip_clip_tensor *tensors, const double *max_norm_at, float *norm,
+                        float *scale, void *workspace) {
+    NHIP_STREAM(st);
+    return clip_on(st, desc, tensors, max_norm_at, norm, scale, workspace);
+}
+
+int nhip_clip_grad_norm_workspace(const nhip_clip_desc *desc, size_t *bytes) {
+    if (desc->count < 0) return fail("nhip_clip_grad_norm_workspace: negative count");
+    *bytes = size_t(clip_launches(desc->count)) * kClipBlocks * sizeof(double);
+    return 0;
+}
+
+}  // extern "C"

@@ -470,9 +470,9 @@ int nhip_plan_add_launch(void *plan, void *function, const uint32_t grid[3], con
 
 int nhip_plan_add_builtin(void *plan, int kind, const void *desc, size_t desc_bytes, const nhip_reloc *relocs,
                           size_t nrelocs) {
-    if (kind < NHIP_STEP_GEMM || kind > NHIP_STEP_LCE) return fail("nhip_plan_add_builtin: unknown step kind");
+    if (kind < NHIP_STEP_GEMM || kind > NHIP_STEP_CLIP) return fail("nhip_plan_add_builtin: unknown step kind");
     // the descriptor must hold what run_steps reads for the kind
-    size_t need = 0;
+    size_t need = 0, pointers = 16;
     switch (kind) {
         case NHIP_STEP_GEMM: need = sizeof(nhip_gemm_desc); break;
         case NHIP_STEP_FLASH_FWD:
@@ -480,11 +480,25 @@ int nhip_plan_add_builtin(void *plan, int kind, const void *desc, size_t desc_by
         case NHIP_STEP_COPY: need = 8; break;
         case NHIP_STEP_FILL: need = 12; break;
         case NHIP_STEP_LCE: need = sizeof(nhip_lce_desc); break;
+        case NHIP_STEP_HEADS:
+        case NHIP_STEP_HEADS_BWD: need = sizeof(nhip_heads_desc); break;
+        case NHIP_STEP_GATED:
+        case NHIP_STEP_GATED_GRAD: need = sizeof(nhip_gated_desc); break;
+        case NHIP_STEP_CLIP: {
+            need = sizeof(nhip_clip_desc);
+            if (desc && desc_bytes >= need) {
+                const int64_t count = static_cast<const nhip_clip_desc *>(desc)->count;
+                if (count < 0 || count > (int64_t(1) << 24)) return fail("nhip_plan_add_builtin: bad tensor count");
+                need += size_t(count) * sizeof(nhip_clip_tensor);
+                pointers = 4 + 2 * size_t(count);
+            }
+            break;
+        }
     }
     if (!desc || desc_bytes < need)
         return fail("nhip_plan_add_builtin: a descriptor of " + std::to_string(desc_bytes) + " bytes for a step kind " +
                     "that reads " + std::to_string(need));
-    if (check_relocs(relocs, nrelocs, 16, false)) return 1;
+    if (check_relocs(relocs, nrelocs, pointers, false)) return 1;
     Step s;
     s.kind = kind;
     s.args.assign(static_cast<const unsigned char *>(desc), static_cast<const unsigned char *>(desc) + desc_bytes);
@@ -599,6 +613,22 @@ static int run_steps(Plan *plan, void *workspace, void *const *inputs, size_t ni
             continue;
         }
         void *ptrs[16] = {nullptr};
+        if (st.kind == NHIP_STEP_CLIP) {  // any number of pointers: the tensors' go into the step's own table
+            nhip_clip_desc *d = reinterpret_cast<nhip_clip_desc *>(st.args.data());
+            nhip_clip_tensor *t = reinterpret_cast<nhip_clip_tensor *>(d + 1);
+            for (int64_t k = 0; k < d->count; ++k) t[k].in = nullptr, t[k].out = nullptr;
+            for (auto &r : st.relocs) {
+                void *p;
+                if (resolve(r, &p)) return 1;
+                if (r.slot < 4) ptrs[r.slot] = p;
+                else if (r.slot % 2) t[(r.slot - 4) / 2].out = p;
+                else t[(r.slot - 4) / 2].in = p;
+            }
+            if (clip_on(s, d, t, static_cast<const double *>(ptrs[0]), static_cast<float *>(ptrs[1]),
+                        static_cast<float *>(ptrs[2]), ptrs[3]))
+                return fail("plan step " + std::to_string(i) + ": " + g_error);
+            continue;
+        }
         for (auto &r : st.relocs)
             if (resolve(r, &ptrs[r.slot])) return 1;
         int rc = 0;
@@ -625,6 +655,24 @@ static int run_steps(Plan *plan, void *workspace, void *const *inputs, size_t ni
             case NHIP_STEP_LCE:
                 rc = lce_on(s, reinterpret_cast<const nhip_lce_desc *>(st.args.data()), ptrs[0], ptrs[1], ptrs[2],
                             static_cast<float *>(ptrs[3]), ptrs[4]);
+                break;
+            case NHIP_STEP_HEADS:
+                rc = heads_on(s, reinterpret_cast<const nhip_heads_desc *>(st.args.data()), ptrs[0], ptrs[1], ptrs[2],
+                              ptrs[3], static_cast<const float *>(ptrs[4]), static_cast<const float *>(ptrs[5]), ptrs[6],
+                              ptrs[7], ptrs[8]);
+                break;
+            case NHIP_STEP_HEADS_BWD:
+                rc = heads_bwd_on(s, reinterpret_cast<const nhip_heads_desc *>(st.args.data()), ptrs[0], ptrs[1], ptrs[2],
+                                  ptrs[3], static_cast<const float *>(ptrs[4]), static_cast<const float *>(ptrs[5]),
+                                  ptrs[6], ptrs[7], ptrs[8], ptrs[9], ptrs[10], ptrs[11], ptrs[12], ptrs[13]);
+                break;
+            case NHIP_STEP_GATED:
+                rc = gated_on(s, reinterpret_cast<const nhip_gated_desc *>(st.args.data()), ptrs[0], ptrs[1], ptrs[2],
+                              ptrs[3], static_cast<float *>(ptrs[4]), static_cast<float *>(ptrs[5]));
+                break;
+            case NHIP_STEP_GATED_GRAD:
+                rc = gated_grad_on(s, reinterpret_cast<const nhip_gated_desc *>(st.args.data()), ptrs[0],
+                                   static_cast<const float *>(ptrs[1]), static_cast<const float *>(ptrs[2]), ptrs[3]);
                 break;
             case NHIP_STEP_FILL: {
                 uint64_t n;

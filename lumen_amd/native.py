@@ -17,7 +17,10 @@ _lib = None
 NHIP_F32, NHIP_BF16, NHIP_F16 = 0, 1, 2
 NHIP_BASE_WORKSPACE, NHIP_BASE_INPUT = 0, 1
 NHIP_STEP_GEMM, NHIP_STEP_FLASH_FWD, NHIP_STEP_FLASH_BWD, NHIP_STEP_COPY, NHIP_STEP_FILL, NHIP_STEP_LCE = 1, 2, 3, 4, 5, 6
+NHIP_STEP_HEADS, NHIP_STEP_HEADS_BWD, NHIP_STEP_GATED, NHIP_STEP_GATED_GRAD, NHIP_STEP_CLIP = 7, 8, 9, 10, 11
 NHIP_LCE_I32, NHIP_LCE_I64 = 0, 1
+NHIP_POS_NONE, NHIP_POS_I32, NHIP_POS_I64 = 0, 1, 2
+NHIP_ACT = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 NHIP_GEMM_EXACT, NHIP_GEMM_FOLD, NHIP_GEMM_FEW_ROWS, NHIP_GEMM_TILED, NHIP_GEMM_ANY = range(5)
 
 
@@ -85,6 +88,34 @@ class AttnDesc(C.Structure):
     ]
 
 
+class HeadsDesc(C.Structure):
+    """``nhip_heads_desc``: head norms and rotation of queries and keys (include/nhip.h)."""
+
+    _fields_ = [(n, C.c_int64) for n in ("batch", "seq", "heads", "kv_heads", "head_dim", "rot", "table_rows")] + [
+        (f"{t}_{a}", C.c_int64) for t in ("q", "k", "oq", "ok", "dq", "dk") for a in ("b", "s", "n")
+    ] + [("dtype", C.c_int32), ("positions", C.c_int32), ("interleaved", C.c_int32), ("eps", C.c_float)]
+
+
+class GatedDesc(C.Structure):
+    """``nhip_gated_desc``: act(x gate^T) * (x up^T) (include/nhip.h)."""
+
+    _fields_ = [(n, C.c_int64) for n in ("m", "n", "k", "x_m", "w_n", "h_m")] + [
+        (n, C.c_int32) for n in ("dtype", "activation", "config")
+    ]
+
+
+class ClipTensor(C.Structure):
+    """``nhip_clip_tensor``: one gradient and where it goes scaled."""
+
+    _fields_ = [("in_", C.c_void_p), ("out", C.c_void_p), ("numel", C.c_int64), ("dtype", C.c_int32), ("pad", C.c_int32)]
+
+
+class ClipDesc(C.Structure):
+    """``nhip_clip_desc``: the tensors' count, the norm's bound and the eps it is divided with."""
+
+    _fields_ = [("count", C.c_int64), ("max_norm", C.c_double), ("eps", C.c_double)]
+
+
 class Reloc(C.Structure):
     _fields_ = [
         ("slot", C.c_uint32),
@@ -139,6 +170,14 @@ SIGNATURES = {
     "nhip_flash_bwd_workspace": ([C.POINTER(AttnDesc), C.POINTER(C.c_size_t)], C.c_int),
     "nhip_attn_config_count": ([C.POINTER(C.c_int)], C.c_int),
     "nhip_flash_bwd_noalloc": ([C.POINTER(AttnDesc)] + [C.c_void_p] * 9, C.c_int),
+    "nhip_qk_norm_rope": ([C.POINTER(HeadsDesc)] + [C.c_void_p] * 9, C.c_int),
+    "nhip_qk_norm_rope_bwd": ([C.POINTER(HeadsDesc)] + [C.c_void_p] * 14, C.c_int),
+    "nhip_qk_norm_rope_workspace": ([C.POINTER(HeadsDesc), C.POINTER(C.c_size_t)], C.c_int),
+    "nhip_gated_linear": ([C.POINTER(GatedDesc)] + [C.c_void_p] * 6, C.c_int),
+    "nhip_gated_config_count": ([C.POINTER(C.c_int)], C.c_int),
+    "nhip_gated_linear_grad": ([C.POINTER(GatedDesc)] + [C.c_void_p] * 4, C.c_int),
+    "nhip_clip_grad_norm": ([C.POINTER(ClipDesc), C.POINTER(ClipTensor)] + [C.c_void_p] * 4, C.c_int),
+    "nhip_clip_grad_norm_workspace": ([C.POINTER(ClipDesc), C.POINTER(C.c_size_t)], C.c_int),
     "nhip_plan_create": ([C.POINTER(C.c_void_p)], C.c_int),
     "nhip_plan_destroy": ([C.c_void_p], C.c_int),
     "nhip_plan_add_launch": (

@@ -185,7 +185,7 @@ typedef struct {
 
 typedef struct {
     char name[40];
-    int out, nin, ins[64], nparams;
+    int out, nin, *ins, nparams;
     Param params[8];
 } Node;
 
@@ -315,6 +315,7 @@ static Graph *parse_graph(Cursor *c) {
         next_token(c, n->name, sizeof n->name);
         n->out = (int)next_int(c);
         n->nin = (int)next_int(c);
+        n->ins = (int *)calloc(n->nin ? n->nin : 1, sizeof(int));
         for (int k = 0; k < n->nin; ++k) n->ins[k] = (int)next_int(c);
         n->nparams = (int)next_int(c);
         for (int k = 0; k < n->nparams; ++k) parse_param(c, &n->params[k]);
@@ -329,9 +330,11 @@ static Graph *parse_graph(Cursor *c) {
 
 static void free_graph(Graph *g) {
     if (!g) return;
-    for (int i = 0; i < g->nnodes; ++i)
+    for (int i = 0; i < g->nnodes; ++i) {
         for (int k = 0; k < g->nodes[i].nparams; ++k)
             if (g->nodes[i].params[k].kind == 'g') free_graph(g->nodes[i].params[k].body);
+        free(g->nodes[i].ins);
+    }
     free(g->types);
     free(g->inputs);
     free(g->outputs);
@@ -1152,8 +1155,8 @@ static Values *eval_graph(const Graph *g, Values *inputs) {
     for (int i = 0; i < g->noutputs; ++i) last[g->outputs[i]] = g->nnodes;
     for (int i = 0; i < g->nnodes; ++i) {
         const Node *nd = &g->nodes[i];
-        Values *args[64];
-        const Type *types[64];
+        Values **args = (Values **)calloc(nd->nin ? nd->nin : 1, sizeof(Values *));
+        const Type **types = (const Type **)calloc(nd->nin ? nd->nin : 1, sizeof(Type *));
         for (int k = 0; k < nd->nin; ++k) {
             args[k] = &env[nd->ins[k]];
             types[k] = &g->types[nd->ins[k]];
@@ -1181,6 +1184,8 @@ static Values *eval_graph(const Graph *g, Values *inputs) {
             }
         }
         have[nd->out] = 1;
+        free(args);
+        free(types);
         for (int k = 0; k < nd->nin; ++k) {
             const int u = nd->ins[k];
             if (last[u] == i && have[u] && !extra[u]) {

@@ -1,0 +1,327 @@
+"""qk_norm_rope, gated_linear and clip_grad_norm on the CPU: what they compute (the oracle on their traced bodies against
+plain float64 NumPy), their gradients against the formula's differences, their refusals, and the plans they become."""
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import lumen_amd as L
+import lumen_amd.functional as F
+from lumen_amd import dtypes as D
+from lumen_amd import native as nv
+from lumen_amd.compiler.plan import Plan
+from oracle import oracle
+from tests import operator_math as M
+
+
+def _graph(fn, *arrays, dtypes=None):
+    metas = [L.empty(list(a.shape), dt or D.canonical(a.dtype), "meta") for a, dt in zip(arrays, dtypes or [None] * len(arrays))]
+    return L.make_graph(fn)(*metas)
+
+
+def _run(fn, *arrays, fused=True):
+    """The oracle's outputs of ``fn`` on float32/float64 arrays (their own dtypes)."""
+    with L.config.compiler.patch(fused_operators=fused):
+        g = _graph(fn, *arrays)
+    return [np.asarray(v, np.float64) for v in oracle.values(g, list(arrays))], g
+
+
+# ---- values and gradients, float64 (traced as primitives) and float32 (one fusion)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("d,rot,interleaved,weights,positions", [
+    (16, 16, False, True, False), (16, 8, True, True, True), (10, 6, False, False, True), (7, 2, True, True, False),
+    (8, 0, False, True, True), (1, 0, False, False, False)])
+def test_heads_values_and_gradients(dtype, d, rot, interleaved, weights, positions):
+    """Both directions against float64 NumPy. float32: about 3 D + 20 roundings of 2^-24 a value, relative to the largest
+    value of the tensor; a weight's gradient sums B S N = 18 rows more. float64 the same with 2^-53."""
+    rng = np.random.default_rng(d + rot)
+    b, s, n, nkv = 2, 3, 3, 1
+    x = M.heads_inputs(rng, b, s, n, nkv, d, rot, table=9, dtype=dtype, weights=weights, positions=positions)
+    names = list(x)
+
+    def fn(*args):
+        t = dict(zip(names, args))
+        keep = [m for m in ("q", "k", "wq", "wk") if m in t]
+
+        def f(*leaves):
+            v = {**t, **dict(zip(keep, leaves))}
+            return F.qk_norm_rope(v["q"], v["k"], v["cos"], v["sin"], v.get("wq"), v.get("wk"), positions=v.get("positions"),
+                                  eps=1e-3, interleaved=interleaved)
+
+        out, pull = L.vjp(f, *(t[m] for m in keep))
+        return [*out, *pull((t["gq"], t["gk"]))]
+
+    got, g = _run(fn, *x.values())
+    fusions = [m.params["name"] for m in g.nodes if m.prim == "fusion"]
+    assert fusions == (["qk_norm_rope", "qk_norm_rope_backward"] if dtype == "float32" else [])
+    want = M.heads(x, 1e-3, interleaved)
+    step = 2.0**-24 if dtype == "float32" else 2.0**-53
+    for a, w in zip(got, want):
+        assert a.shape == w.shape
+        assert np.abs(a - w).max() <= step * (3 * d + 40) * max(1.0, np.abs(w).max())
+
+
+def test_heads_gradient_against_differences():
+    """The float64 gradient of every input against central differences of the value (step 1e-6: 1e-9 from the third
+    derivative and 1e-10 from the rounding of the values)."""
+    rng = np.random.default_rng(3)
+    x = M.heads_inputs(rng, 1, 3, 2, 1, 8, 6, table=5, dtype="float64", weights=True, positions=True)
+    want = M.heads(x, 1e-3, False)
+    grads = dict(zip(("q", "k", "wq", "wk"), want[2:]))
+
+    def value(x):
+        yq, yk = M.heads(x, 1e-3, False)[:2]
+        return (yq * x["gq"]).sum() + (yk * x["gk"]).sum()
+
+    for name, g in grads.items():
+        assert np.abs(g - M.differences(value, x, name)).max() <= 1e-7, name
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("activation", M.ACTIVATIONS)
+def test_gated_values_and_gradients(activation, dtype):
+    """float32: sums of K = 11 and F = 6 products (each rounded) and a few more roundings; float64 the same."""
+    rng = np.random.default_rng(len(activation))
+    x, gate, up, dh = (rng.standard_normal(s).astype(dtype) for s in ((2, 4, 11), (6, 11), (6, 11), (2, 4, 6)))
+
+    def fn(x, gate, up, dh):
+        h, pull = L.vjp(lambda x, gate, up: F.gated_linear(x, gate, up, activation=activation), x, gate, up)
+        return [h, *pull(dh)]
+
+    got, g = _run(fn, x, gate, up, dh)
+    step = 2.0**-24 if dtype == "float32" else 2.0**-53
+    for a, w in zip(got, M.gated(x, gate, up, dh, activation)):
+        assert a.shape == w.shape
+        assert np.abs(a - w).max() <= step * 100 * max(1.0, np.abs(w).max())
+
+
+@pytest.mark.parametrize("activation", M.ACTIVATIONS)
+def test_gated_gradient_against_differences(activation):
+    rng = np.random.default_rng(8)
+    x = {n: rng.standard_normal(s) for n, s in (("x", (3, 5)), ("gate", (4, 5)), ("up", (4, 5)), ("dh", (3, 4)))}
+    grads = M.gated(*x.values(), activation)[1:]
+    for name, g in zip(("x", "gate", "up"), grads):
+        diff = M.differences(lambda x: (M.gated(*x.values(), activation)[0] * x["dh"]).sum(), x, name)
+        assert np.abs(g - diff).max() <= 1e-6, name
+
+
+def test_gated_16_bit_is_two_fusions_and_ordinary_products():
+    g = _graph(lambda x, gate, up, dh: (lambda h, pull: [h, *pull(dh)])(*L.vjp(F.gated_linear, x, gate, up)),
+               *(np.zeros(s, np.uint16) for s in ((64, 64), (128, 64), (128, 64), (64, 128))), dtypes=["bfloat16"] * 4)
+    assert [n.params["name"] for n in g.nodes if n.prim == "fusion"] == ["gated_linear", "gated_linear_grad"]
+    forward = _graph(F_gated, *(np.zeros(s, np.uint16) for s in ((64, 64), (128, 64), (128, 64))), dtypes=["bfloat16"] * 3)
+    plan = Plan(forward, build_kernels=False)
+    assert [st.kind for st in plan.steps] == ["gated_fwd"] and len(plan.steps[0].outputs) == 1  # g and u are not stored
+
+
+def F_gated(x, gate, up):
+    return [F.gated_linear(x, gate, up)]
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_clip_values(fused):
+    """float32 and float64 tensors, a 0-d one and an empty one; over the bound, below it, and with a traced bound."""
+    rng = np.random.default_rng(5)
+    xs = [rng.standard_normal(s).astype(np.float32) for s in ((5, 3), (), (7,), (0, 4))]
+    norm = np.sqrt(sum((x.astype(np.float64)**2).sum() for x in xs))
+    for bound in (0.5 * norm, 2 * norm, 0.0):
+        got, g = _run(lambda *xs: (lambda c, n: [n, *c])(*F.clip_grad_norm(xs, float(bound))), *xs, fused=fused)
+        assert sum(n.prim == "fusion" for n in g.nodes) == fused
+        scale = min(1.0, bound / (norm + 1e-6))
+        assert abs(got[0] - norm) <= 2.0**-24 * norm
+        for a, x in zip(got[1:], xs):
+            assert np.abs(a - x * scale).max(initial=0) <= 2.0**-23 * np.abs(x).max(initial=0)
+    traced = L.make_graph(lambda bound, *xs: (lambda c, n: [n, *c])(*F.clip_grad_norm(xs, bound)))(
+        0.5 * float(norm), *[L.empty(list(x.shape), "float32", "meta") for x in xs])
+    tensors = [v for v in traced.inputs if traced.types[v].dtype == "float32"]
+    arrays = dict(zip(tensors, xs))
+    got = oracle.values(traced, [arrays.get(v, np.array(0.5 * norm)) for v in traced.inputs])
+    assert np.abs(got[1] - 0.5 * xs[0]).max() <= 1e-6
+
+
+def test_clip_of_extreme_values():
+    """Squares that overflow and underflow float32, an infinity and a NaN."""
+    big = np.array([3e38, -1e38], np.float32)
+    tiny = np.array([1e-30, 3e-30], np.float32)
+    clip = lambda x: (lambda c, n: [n, *c])(*F.clip_grad_norm([x], 1.0, eps=0.0))  # noqa: E731
+    (norm, out), _ = _run(clip, big)
+    np.testing.assert_allclose(out, big / np.float64(np.hypot(3e38, 1e38)), rtol=1e-6)
+    (norm, out), _ = _run(clip, tiny)
+    np.testing.assert_allclose(norm, np.sqrt(10) * 1e-30, rtol=1e-6)
+    assert np.array_equal(out, tiny.astype(np.float64))
+    (norm, out), _ = _run(clip, np.array([np.inf, 2.0], np.float32))
+    assert np.isinf(norm) and np.isnan(out[0]) and out[1] == 0
+    (norm, out), _ = _run(clip, np.array([np.nan, 2.0], np.float32))
+    assert np.isnan(norm) and np.isnan(out).all()
+
+
+def test_clip_of_many_tensors():
+    """More tensors than a launch's table holds: one step, every result."""
+    xs = [np.full((3,), i, np.float32) for i in range(130)]
+    got, g = _run(lambda *xs: (lambda c, n: [n, *c])(*F.clip_grad_norm(xs, 1.0)), *xs)
+    norm = np.sqrt(3 * sum(i * i for i in range(130)))
+    assert abs(got[0] - norm) <= 1e-6 * norm and len(got) == 131
+    np.testing.assert_allclose(got[-1], 129 / (norm + 1e-6), rtol=1e-6)
+
+
+# ---- refusals
+
+
+def _m(shape, dtype="bfloat16"):
+    return L.empty(list(shape), dtype, "meta")
+
+
+BAD_HEADS = {
+    "3-D query": (ValueError, "4-D", dict(q=(2, 3, 8))),
+    "head dims differ": (ValueError, "differ in batch", dict(k=(2, 3, 1, 16))),
+    "sequences differ": (ValueError, "differ in batch", dict(k=(2, 4, 1, 8))),
+    "integer heads": (TypeError, "floating-point", dict(dtype="int32")),
+    "16-bit table": (ValueError, "cos is not a float32", dict(table="bfloat16")),
+    "table too wide": (ValueError, "do not turn pairs", dict(cos=(9, 5), sin=(9, 5))),
+    "tables differ": (ValueError, "do not turn pairs", dict(cos=(9, 4), sin=(9, 3))),
+    "short table": (ValueError, "tables of 2 positions", dict(cos=(2, 4), sin=(2, 4))),
+    "weight of another size": (TypeError, "query weight must be", dict(wq=(4,))),
+    "positions of another shape": (ValueError, "positions must be", dict(positions=(2, 4))),
+    "float positions": (ValueError, "positions must be", dict(positions=(2, 3), ptype="float32")),
+    "negative eps": (ValueError, "eps must be", dict(eps=-1.0)),
+    "eps that is no number": (ValueError, "eps must be", dict(eps=float("nan"))),
+}
+
+
+@pytest.mark.parametrize("name", sorted(BAD_HEADS))
+def test_heads_refusals(name):
+    error, match, c = BAD_HEADS[name]
+    dt = c.get("dtype", "bfloat16")
+    args = [_m(c.get("q", (2, 3, 4, 8)), dt), _m(c.get("k", (2, 3, 1, 8)), dt), _m(c.get("cos", (9, 4)), c.get("table", "float32")),
+            _m(c.get("sin", (9, 4)), "float32"), _m(c.get("wq", (8,)), dt)]
+    if "positions" in c:
+        args.append(_m(c["positions"], c.get("ptype", "int32")))
+    with pytest.raises(error, match=match):
+        L.make_graph(lambda q, k, cos, sin, wq, p=None: list(
+            F.qk_norm_rope(q, k, cos, sin, wq, positions=p, eps=c.get("eps"))))(*args)
+
+
+def test_heads_of_two_dtypes_are_refused():
+    with pytest.raises(TypeError, match="convert them to one"):
+        L.make_graph(lambda q, k, c, s: list(F.qk_norm_rope(q, k, c, s)))(
+            _m((1, 2, 2, 8)), _m((1, 2, 2, 8), "float32"), _m((2, 4), "float32"), _m((2, 4), "float32"))
+
+
+@pytest.mark.parametrize("x,gate,up,dtypes,activation,error,match", [
+    ((4, 8), (6, 7), (6, 8), None, "silu", ValueError, "gate weight must be"),
+    ((4, 8), (6, 8), (5, 8), None, "silu", ValueError, "differ"),
+    ((4, 8), (6, 8, 1), (6, 8), None, "silu", ValueError, "gate weight must be"),
+    ((4, 8), (6, 8), (6, 8), ("bfloat16", "float32", "bfloat16"), "silu", TypeError, "convert them to one"),
+    ((4, 8), (6, 8), (6, 8), ("int32",) * 3, "silu", TypeError, "floating-point"),
+    ((4, 8), (6, 8), (6, 8), None, "swish", ValueError, "activation must be one of"),
+])
+def test_gated_refusals(x, gate, up, dtypes, activation, error, match):
+    with pytest.raises(error, match=match):
+        L.make_graph(lambda x, g, u: F.gated_linear(x, g, u, activation=activation))(
+            *(_m(s, d) for s, d in zip((x, gate, up), dtypes or ("bfloat16",) * 3)))
+
+
+def test_clip_refusals():
+    def clip(*args, **kw):
+        return lambda x: (lambda c, n: [n, *c])(*F.clip_grad_norm([x], *args, **kw))
+
+    for fn, error, match in [
+        (clip(-1.0), ValueError, "max_norm must be at least 0"), (clip(float("nan")), ValueError, "max_norm"),
+        (clip("1"), ValueError, "max_norm"), (clip(1.0, eps=-1.0), ValueError, "eps"),
+        (lambda x: F.clip_grad_norm(x, 1.0)[1], TypeError, "list or tuple"),
+        (lambda x: F.clip_grad_norm([], 1.0)[1], ValueError, "no gradients"),
+        (lambda x: F.clip_grad_norm([2.0], 1.0)[1], TypeError, "gradients are tensors"),
+        (lambda x: F.clip_grad_norm([x], x)[1], TypeError, "float scalar"),
+        (lambda x: L.grad(lambda x: F.clip_grad_norm([x], 1.0)[1])(x), NotImplementedError, "no gradient"),
+    ]:
+        with pytest.raises(error, match=match):
+            L.make_graph(fn)(_m((4,), "float32"))
+    with pytest.raises(TypeError, match="floating-point"):
+        L.make_graph(clip(1.0))(_m((4,), "int32"))
+
+
+def test_vjp_of_several_results():
+    """A pullback of several results takes as many cotangents and sums what they send back."""
+    x = np.array([1.0, 2.0])
+
+    def fn(x):
+        out, pull = L.vjp(lambda x: (x * x, x * 3.0), x)
+        return [*out, *pull((x, x))]
+
+    got, _ = _run(fn, x)
+    assert np.array_equal(got[2], 2 * x * x + 3 * x)
+    with pytest.raises(TypeError, match="2 results take as many"):
+        L.make_graph(lambda x: list(L.vjp(lambda x: (x * x, x * 3.0), x)[1](x)))(_m((2,), "float32"))
+
+
+def test_abi_refusals():
+    """Bad descriptors are refused before anything is queued (no GPU here: what passes fails for its missing stream)."""
+    def heads(**kw):
+        d = dict(batch=1, seq=4, heads=2, kv_heads=1, head_dim=64, rot=64, table_rows=4, dtype=1)
+        return nv.HeadsDesc(**{**d, **kw})
+
+    n = C.c_size_t()
+    for bad, match in [(heads(head_dim=0), "head dim"), (heads(head_dim=1025), "head dim"), (heads(rot=3), "rotated"),
+                       (heads(rot=66), "rotated"), (heads(table_rows=0), "empty table"), (heads(dtype=3), "float32, bf16"),
+                       (heads(positions=3), "positions"), (heads(seq=1 << 30), "2\\^30"), (heads(batch=-1), "negative")]:
+        with pytest.raises(RuntimeError, match=match):
+            nv.call("nhip_qk_norm_rope_workspace", C.byref(bad), C.byref(n))
+    nv.call("nhip_qk_norm_rope_workspace", C.byref(heads()), C.byref(n))
+    assert n.value == 2 * 64 * 4  # one workgroup for the queries' 8 heads, one for the keys' 4
+    nv.call("nhip_clip_grad_norm_workspace", C.byref(nv.ClipDesc(count=121)), C.byref(n))
+    assert n.value == 2 * 1024 * 8
+    with pytest.raises(RuntimeError, match="negative count"):
+        nv.call("nhip_clip_grad_norm_workspace", C.byref(nv.ClipDesc(count=-1)), C.byref(n))
+    plan = C.c_void_p()
+    nv.call("nhip_plan_create", C.byref(plan))
+    d = nv.ClipDesc(count=3)
+    rr = (nv.Reloc * 1)(nv.Reloc(slot=10))
+    with pytest.raises(RuntimeError, match="descriptor of"):
+        nv.call("nhip_plan_add_builtin", plan, nv.NHIP_STEP_CLIP, bytes(d), len(bytes(d)), rr, 0)
+    full = bytes(d) + bytes((nv.ClipTensor * 3)())
+    with pytest.raises(RuntimeError, match="slot"):
+        nv.call("nhip_plan_add_builtin", plan, nv.NHIP_STEP_CLIP, full, len(full), rr, 1)
+    nv.call("nhip_plan_destroy", plan)
+
+
+# ---- plans
+
+
+def test_operands_that_are_no_rows_are_copied():
+    """A merged projection's heads are read in place through their strides; a transposed operand, whose rows a view would
+    not keep contiguous, becomes a copy."""
+    def packed(x, cos, sin):
+        q, k = x[:, :, :128].reshape(1, 6, 2, 64), x[:, :, 128:192].reshape(1, 6, 1, 64)
+        return list(F.qk_norm_rope(q, k, cos, sin))
+
+    plan = Plan(L.make_graph(packed)(_m((1, 6, 256)), _m((8, 32), "float32"), _m((8, 32), "float32")), build_kernels=False)
+    kinds = [st.kind for st in plan.steps]
+    assert kinds.count("heads_fwd") == 1 and "loop" not in kinds
+    plan = Plan(L.make_graph(lambda xt, g, ut: [F.gated_linear(xt.t(), g, ut.t())])(
+        _m((64, 32)), _m((48, 64)), _m((64, 48))), build_kernels=False)
+    step = plan.steps[-1]
+    assert step.kind == "gated_fwd" and [st.kind for st in plan.steps].count("loop") >= 1
+    for v in step.nodes[0].inputs:
+        assert plan.loc[v].strides[-1] == 1
+
+
+def test_clipped_gradients_scale_in_the_update_that_reads_them():
+    """An update p - lr clipped(g) reads g and the scale: the clipping step writes the norm alone, with the same values."""
+    def step(p, q, gp, gq):
+        (cp, cq), norm = F.clip_grad_norm([gp, gq], 0.5)
+        return [norm, p - 0.1 * cp, q - 0.1 * cq]
+
+    def plan_of():
+        g = L.make_graph(step)(*[_m(s) for s in ((8, 16), (5,), (8, 16), (5,))])
+        return Plan(g, build_kernels=False), g
+
+    plan, g = plan_of()
+    (clip,) = [st for st in plan.steps if st.kind == "clip"]
+    assert len(clip.outputs) == 2  # the norm and the scale
+    rng = np.random.default_rng(0)
+    xs = [D.bf16_bits(rng.standard_normal(s).astype(np.float32)) for s in ((8, 16), (5,), (8, 16), (5,))]
+    for a, b in zip(oracle.run(g, xs), oracle.run(plan.graph, xs)):
+        assert np.array_equal(a, b)
