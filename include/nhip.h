@@ -271,7 +271,9 @@ int nhip_qk_norm_rope_workspace(const nhip_heads_desc *desc, size_t *bytes);
  *
  * h [m, n] = act(x gate^T) * (x up^T) for x [m, k] and weights [n, k], bf16 or f16, contiguous along k, rows x_m and w_n
  * elements apart (both weights), h's rows h_m. The sums are float32 and rounded once, in h. g and u (both or neither):
- * float32 [m, n], the two products, which nhip_gated_linear_grad needs. */
+ * float32 [m, n], the two products, which nhip_gated_linear_grad needs. Rows of a multiple of 8 elements that start on 16
+ * bytes are read in place (such operands have to start there); others, above 64 rows of x, through `workspace`, of
+ * nhip_gated_linear_workspace bytes from a 16-byte address. */
 enum {
     NHIP_ACT_SILU = 0,
     NHIP_ACT_GELU = 1,     /* the tanh form */
@@ -285,11 +287,19 @@ typedef struct {
     int32_t config;          /* -1: the default for the shape; else an index below nhip_gated_config_count */
 } nhip_gated_desc;
 
-int nhip_gated_linear(const nhip_gated_desc *desc, const void *x, const void *gate, const void *up, void *h, float *g, float *u);
+int nhip_gated_linear(const nhip_gated_desc *desc, const void *x, const void *gate, const void *up, void *h, float *g, float *u,
+                      void *workspace);
+int nhip_gated_linear_workspace(const nhip_gated_desc *desc, size_t *bytes);
 /* Number of kernels nhip_gated_linear has (for tests and timing); a config the operands cannot take fails. */
 int nhip_gated_config_count(int *count);
 /* [dg | du] ([m, 2 n], contiguous, the type of dh) of dh [m, n]: dg = dh u act'(g), du = dh act(g), each rounded once. */
 int nhip_gated_linear_grad(const nhip_gated_desc *desc, const void *dh, const float *g, const float *u, void *dgu);
+/* D = A[:, :k / 2] B + A[:, k / 2:] B2 for A [m, k] along k and B, B2 [k / 2, n] along n, bf16 or f16, with one float32 sum
+ * over both: the input's gradient of A = [dg | du] and the two weights. Whole rows (strides of at least their length) of
+ * multiples of 8 elements from 16-byte addresses, k / 2 and n multiples of 8, no batches; config and splits are the
+ * library's. `workspace` of nhip_gemm_pair_workspace bytes. */
+int nhip_gemm_pair(const nhip_gemm_desc *desc, const void *a, const void *b, const void *b2, void *d, void *workspace);
+int nhip_gemm_pair_workspace(const nhip_gemm_desc *desc, size_t *bytes);
 
 /* ---- gradient clipping (no counterpart in the reference) -------------------------------------------------------- *
  *
@@ -343,11 +353,12 @@ enum {
     NHIP_STEP_LCE = 6,        /* desc: nhip_lce_desc; pointers: h, w, target, out, workspace */
     NHIP_STEP_HEADS = 7,      /* desc: nhip_heads_desc; pointers as nhip_qk_norm_rope's, those left out null */
     NHIP_STEP_HEADS_BWD = 8,  /* desc: nhip_heads_desc; pointers as nhip_qk_norm_rope_bwd's */
-    NHIP_STEP_GATED = 9,      /* desc: nhip_gated_desc; pointers: x, gate, up, h (and g, u) */
+    NHIP_STEP_GATED = 9,      /* desc: nhip_gated_desc; pointers: x, gate, up, h, g, u (or neither), workspace (or none) */
     NHIP_STEP_GATED_GRAD = 10, /* desc: nhip_gated_desc; pointers: dh, g, u, dgu */
     NHIP_STEP_CLIP = 11,      /* desc: nhip_clip_desc, then its nhip_clip_tensors (in and out ignored); pointers: max_norm_at
                                  (or none), norm, scale (or none), workspace, then tensor i's in at 4 + 2 i and out at
                                  5 + 2 i (or none) */
+    NHIP_STEP_PAIR = 12,      /* desc: nhip_gemm_desc; pointers: a, b, b2, d, workspace (or none) */
 };
 
 int nhip_plan_create(void **plan);

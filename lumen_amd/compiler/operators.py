@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 
+from lumen_amd import dtypes as D
 from lumen_amd.graph.ir import ELEMENTWISE, Graph
 
 KINDS = {
@@ -16,10 +17,14 @@ KINDS = {
     "qk_norm_rope_backward": "heads_bwd",
     "gated_linear": "gated_fwd",
     "gated_linear_grad": "gated_grad",
+    "gemm_pair": "pair",
     "clip_grad_norm": "clip",
 }
 NHIP_DT = {"float32": 0, "bfloat16": 1, "float16": 2}
-ROWS, DENSE = "rows", "dense"  # the last axis contiguous; every axis
+# The last axis contiguous; and rows that start on 16 bytes, or all of a length that the library copies itself; every axis
+# contiguous; and from 16 bytes on.
+ROWS, WIDE_ROWS, DENSE, WIDE = "rows", "wide rows", "dense", "wide"
+STRICTER = [ROWS, WIDE_ROWS, DENSE, WIDE]
 
 
 def _wants(node):
@@ -28,7 +33,9 @@ def _wants(node):
     if name.startswith("qk_norm_rope"):
         return [ROWS if r in ("q", "k", "gq", "gk") else DENSE for r in node.params["roles"]]
     if name == "gated_linear":
-        return [ROWS, DENSE, DENSE]
+        return [WIDE_ROWS, WIDE, WIDE]
+    if name == "gemm_pair":
+        return [WIDE] * 3
     if name == "gated_linear_grad":
         return [ROWS, DENSE, DENSE]
     return [DENSE] * len(node.inputs)
@@ -40,15 +47,23 @@ def layouts(steps) -> dict:
     for st in steps:
         if st.kind in KINDS.values():
             for v, want in zip(st.nodes[0].inputs, _wants(st.nodes[0])):
-                out[v] = DENSE if DENSE in (want, out.get(v)) else ROWS
+                out[v] = max(want, out.get(v, ROWS), key=STRICTER.index)
     return out
 
 
 def reads(loc, want) -> bool:
     """Whether a place has the layout ``want`` (None: any)."""
-    if want == DENSE:
+    if want is None:
+        return True
+    if want in (WIDE, WIDE_ROWS) and loc.offset * D.size_of(loc.dtype) % 16:
+        return False
+    if want in (DENSE, WIDE):
         return loc.contiguous()
-    return want is None or not loc.shape or loc.shape[-1] == 1 or loc.strides[-1] == 1
+    if loc.shape and loc.shape[-1] != 1 and loc.strides[-1] != 1:
+        return False
+    if want == WIDE_ROWS and loc.shape[-1] % 8 == 0:  # [rows, k]; tiles of 256 rows within 2^31 bytes
+        return loc.strides[0] % 8 == 0 and 256 * loc.strides[0] + loc.shape[-1] < 1 << 30
+    return True
 
 
 def _heads_desc(node, types):
@@ -80,6 +95,10 @@ def scratch_bytes(graph, node) -> int:
     n, name = C.c_size_t(), node.params["name"]
     if name == "qk_norm_rope_backward":
         nv.call("nhip_qk_norm_rope_workspace", C.byref(_heads_desc(node, _roles(graph, node))), C.byref(n))
+    elif name == "gated_linear":
+        nv.call("nhip_gated_linear_workspace", C.byref(_gated_node_desc(graph, node)), C.byref(n))
+    elif name == "gemm_pair":
+        nv.call("nhip_gemm_pair_workspace", C.byref(_pair_desc(graph, node)), C.byref(n))
     elif name == "clip_grad_norm":
         nv.call("nhip_clip_grad_norm_workspace", C.byref(nv.ClipDesc(count=len(_clip_grads(node)))), C.byref(n))
     return -(-n.value // 256) * 256
@@ -99,7 +118,8 @@ def lower(plan, step):
     name = step.nodes[0].params["name"]
     if name.startswith("qk_norm_rope"):
         return _lower_heads(plan, step)
-    return {"gated_linear": _lower_gated, "gated_linear_grad": _lower_gated_grad, "clip_grad_norm": _lower_clip}[name](plan, step)
+    return {"gated_linear": _lower_gated, "gated_linear_grad": _lower_gated_grad, "gemm_pair": _lower_pair,
+            "clip_grad_norm": _lower_clip}[name](plan, step)
 
 
 def _slots(places):
@@ -141,16 +161,37 @@ def _gated_desc(dtype, activation, m, n, k):
     return d
 
 
+def _gated_node_desc(graph, node):
+    x, gate = (graph.types[v] for v in node.inputs[:2])
+    return _gated_desc(x.dtype, node.params["activation"], x.shape[0], gate.shape[0], x.shape[1])
+
+
 def _lower_gated(plan, step):
     from lumen_amd import native as nv
 
-    node, g = step.nodes[0], plan.graph
-    x, gate = (g.types[v] for v in node.inputs[:2])
-    d = _gated_desc(x.dtype, node.params["activation"], x.shape[0], gate.shape[0], x.shape[1])
+    node = step.nodes[0]
+    d = _gated_node_desc(plan.graph, node)
     places = [plan.loc[v] for v in node.inputs]
     d.x_m = places[0].strides[0]
     out = _outputs(plan, step)
-    return nv.NHIP_STEP_GATED, bytes(d), _slots(places + [out[0], out.get(1), out.get(2)])
+    return nv.NHIP_STEP_GATED, bytes(d), _slots(places + [out[0], out.get(1), out.get(2), plan.scratch.get(id(step))])
+
+
+def _pair_desc(graph, node):
+    from lumen_amd import native as nv
+
+    a, b = (graph.types[v] for v in node.inputs[:2])
+    dt = NHIP_DT[a.dtype]
+    return nv.GemmDesc(m=a.shape[0], n=b.shape[1], k=a.shape[1], a_dtype=dt, b_dtype=dt, d_dtype=dt, a_m=a.shape[1], a_k=1,
+                       b_k=b.shape[1], b_n=1, d_m=b.shape[1], d_n=1, config=-1)
+
+
+def _lower_pair(plan, step):
+    from lumen_amd import native as nv
+
+    node = step.nodes[0]
+    return nv.NHIP_STEP_PAIR, bytes(_pair_desc(plan.graph, node)), _slots(
+        [plan.loc[v] for v in node.inputs] + [_outputs(plan, step)[0], plan.scratch.get(id(step))])
 
 
 def _lower_gated_grad(plan, step):

@@ -9,10 +9,10 @@
 // (three roundings on the way to dx instead of two), and 16 m n bytes of traffic are 7% of the six products' time at
 // [4096, 2048] x [8192, 2048].
 //
-// Three kernels by size and alignment (gated_kind):
-//  * gated_stream: gemm_stream_tile with PAIR 1, tiles of 256 rows x 128 columns or 128 x 64;
-//  * gated_skinny: at most 64 rows, 16 columns a workgroup, the waves divide k (as gemm_skinny);
-//  * gated_any: rows of any length and alignment, 64 x 32 or 128 x 64 tiles through registers.
+// Two kernels (gated_default):
+//  * gated_stream: gemm_stream_tile with PAIR 1, tiles of 256 rows x 128 columns or 128 x 64; rows that it cannot read in
+//    place (no multiple of 8 elements, off 16 bytes) are copied first (gated_pad_kernel);
+//  * gated_skinny: at most 64 rows, 16 columns a workgroup, the waves divide k (as gemm_skinny).
 //
 // The backward's elementwise half (gated_grad_kernel) turns dh, g and u into [dg | du], one row of 2 n a token, HBM-bound:
 //   du = dh act(g), dg = dh u act'(g)
@@ -129,25 +129,31 @@ struct GatedOut {
     }
 };
 
-// TM x TM / 2 tiles; WN and KL as gemm_stream's.
-template <bool F16, int TM, int WN, int KL, bool BUF>
-__global__ __launch_bounds__(128 * WN) __attribute__((amdgpu_waves_per_eu(TM == 256 ? WN / 2 : 2, TM == 256 ? WN / 2 : 2))) void
-gated_stream(GemmShape s, const uint16_t *__restrict__ x, const uint16_t *__restrict__ gate, const uint16_t *__restrict__ up,
-             GatedOut out) {
+// TM x TM / 2 tiles: 256 with 8 waves and the k loop placed by hand (with 4 waves the store's 512 registers spill: [16384, 2048] x
+// [8192, 2048] 909 us, 1140), 128 with 4 waves, two workgroups a CU.
+template <bool F16, int TM>
+__global__ __launch_bounds__(TM * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_stream(
+    GemmShape s, const uint16_t *__restrict__ x, const uint16_t *__restrict__ gate, const uint16_t *__restrict__ up,
+    GatedOut out) {
     extern __shared__ __align__(1024) char smem[];
-    gemm_stream_tile<F16, 64, WN, false, false, BUF, GatedOut, TM, KL, 1>(s, x, gate, out, smem, up);
+    gemm_stream_tile<F16, 64, TM / 64, false, false, true, GatedOut, TM, TM == 256 ? 3 : 0, 1>(s, x, gate, out, smem, up);
 }
 
 // Few rows: a workgroup takes 16 columns of both weights, its NW waves divide k 64 at a time, fragments straight from
 // memory (v_mfma_f32_16x16x32: 16 rows of 64 contiguous bytes), the waves' sums added through LDS in wave order. Reading
 // the weights once is all the work.
-template <bool F16, int MT, int NW>
+// ANY: rows of any length and alignment.
+template <bool F16, int MT, int NW, bool ANY>
 __global__ __launch_bounds__(64 * NW) void gated_skinny(GemmShape s, const uint16_t *__restrict__ x,
                                                          const uint16_t *__restrict__ gate, const uint16_t *__restrict__ up,
                                                          GatedOut out) {
     constexpr int U = MT == 1 ? 2 : 1;  // chunks of 64 k in flight
     __shared__ f32x4_t sums[NW][2][MT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+    auto get = [](const uint16_t *p) {
+        if constexpr (ANY) return load8_any(p, 8);
+        else return *reinterpret_cast<const uint4 *>(p);
+    };
     const int64_t n0 = int64_t(blockIdx.x) * 16;
     // rows past the last one: the last one again, never stored
     const int64_t row = min(n0 + l16, s.n - 1) * s.b_n + 8 * g;
@@ -170,13 +176,13 @@ __global__ __launch_bounds__(64 * NW) void gated_skinny(GemmShape s, const uint1
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int w = 0; w < 2; ++w) fb[u][c][w] = *reinterpret_cast<const uint4 *>(pb[w] + k0 + u * step + 32 * c);
+                for (int w = 0; w < 2; ++w) fb[u][c][w] = get(pb[w] + k0 + u * step + 32 * c);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int i = 0; i < MT; ++i) fa[u][c][i] = *reinterpret_cast<const uint4 *>(pa[i] + k0 + u * step + 32 * c);
+                for (int i = 0; i < MT; ++i) fa[u][c][i] = get(pa[i] + k0 + u * step + 32 * c);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -189,13 +195,15 @@ __global__ __launch_bounds__(64 * NW) void gated_skinny(GemmShape s, const uint1
     for (; k0 < k; k0 += step)  // the last chunks, a lane's 8 k past the end as zeros
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const bool in = k0 + 32 * c + 8 * g < k;
-            const uint4 zero = make_uint4(0, 0, 0, 0);
-            const uint4 f0 = in ? *reinterpret_cast<const uint4 *>(pb[0] + k0 + 32 * c) : zero;
-            const uint4 f1 = in ? *reinterpret_cast<const uint4 *>(pb[1] + k0 + 32 * c) : zero;
+            const int left = k - (k0 + 32 * c + 8 * g);
+            auto tail = [&](const uint16_t *p) {
+                if constexpr (ANY) return left > 0 ? load8_any(p + k0 + 32 * c, left) : make_uint4(0, 0, 0, 0);
+                else return left > 0 ? get(p + k0 + 32 * c) : make_uint4(0, 0, 0, 0);
+            };
+            const uint4 f0 = tail(pb[0]), f1 = tail(pb[1]);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                const uint4 fa = in ? *reinterpret_cast<const uint4 *>(pa[i] + k0 + 32 * c) : zero;
+                const uint4 fa = tail(pa[i]);
                 acc[0][i] = mfma16<F16>(fa, f0, acc[0][i]);
                 acc[1][i] = mfma16<F16>(fa, f1, acc[1][i]);
             }
@@ -217,98 +225,35 @@ __global__ __launch_bounds__(64 * NW) void gated_skinny(GemmShape s, const uint1
         if (r0 + e < s.m) out.one(s, r0 + e, col, gv[e], uv[e]);
 }
 
-// Rows of any length and alignment (load8_any), k of any size: BM rows x BN / 2 columns a workgroup, WM x WN waves, the
-// tile's B lines the gate's BN / 2 rows and then the up projection's, double-buffered through registers.
-template <bool F16, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM *WN * 64) void gated_any(GemmShape s, const uint16_t *__restrict__ x,
-                                                          const uint16_t *__restrict__ gate,
-                                                          const uint16_t *__restrict__ up, GatedOut out) {
-    constexpr int BK = 64, T = WM * WN * 64, P = BK + 8, CH = BK / 8, H = BN / 2;
-    constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
-    constexpr int VA = BM * CH / T, VB = BN * CH / T;
-    static_assert(BM * CH % T == 0 && BN * CH % T == 0 && FN % 2 == 0 && FM > 0, "tile loads divide evenly, pairs of columns");
-    extern __shared__ __align__(16) uint16_t lds[];
-    uint16_t *As = lds, *Bs = lds + 2 * BM * P;
-    int tm, tn;
-    tile_of(blockIdx.x, s.tiles_m, s.tiles_n, tm, tn);
-    const int64_t m0 = int64_t(tm) * BM, n0 = int64_t(tn) * H;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int wm = wave / WN, wn = wave % WN, h = lane >> 5, l32 = lane & 31;
-    uint4 ra[VA], rb[VB];
-    auto load = [&](int64_t k0) {
-#pragma unroll
-        for (int v = 0; v < VA; ++v) {
-            const int idx = t + v * T, line = idx / CH, ch = idx % CH;
-            const int64_t gm = m0 + line, gk = k0 + ch * 8;
-            ra[v] = gm < s.m && gk < s.k ? load8_any(x + gm * s.a_m + gk, s.k - gk) : make_uint4(0, 0, 0, 0);
+// Rows of any length, alignment or distance, as gated_stream reads them: each of x's m rows and the weights' 2 n copied to
+// rows of kp = k rounded up to 8 elements, 16 bytes a thread, zeros past k. A pass over the operands that a product of many
+// rows hides and one of few rows does not need (gated_skinny reads any rows): [16384, 2047] x [8192, 2047] 60 of 970 us.
+struct GatedPad {
+    const uint16_t *src[3];
+    uint16_t *dst[3];
+    int64_t rows[3], ld[3], k, kp;
+};
+static __global__ __launch_bounds__(256) void gated_pad_kernel(GatedPad a) {
+    const int64_t per = a.kp / 8;
+    for (int which = 0; which < 3; ++which) {
+        const int64_t total = a.rows[which] * per;
+        for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+            const int64_t row = i / per, c = (i - row * per) * 8;
+            *reinterpret_cast<uint4 *>(a.dst[which] + row * a.kp + c) = load8_any(a.src[which] + row * a.ld[which] + c, a.k - c);
         }
-#pragma unroll
-        for (int v = 0; v < VB; ++v) {
-            const int idx = t + v * T, line = idx / CH, ch = idx % CH;
-            const int64_t gn = n0 + (line < H ? line : line - H), gk = k0 + ch * 8;
-            rb[v] = gn < s.n && gk < s.k ? load8_any((line < H ? gate : up) + gn * s.b_n + gk, s.k - gk) : make_uint4(0, 0, 0, 0);
-        }
-    };
-    auto put = [&](int buf) {
-#pragma unroll
-        for (int v = 0; v < VA; ++v) {
-            const int idx = t + v * T;
-            *reinterpret_cast<uint4 *>(As + buf * BM * P + idx / CH * P + idx % CH * 8) = ra[v];
-        }
-#pragma unroll
-        for (int v = 0; v < VB; ++v) {
-            const int idx = t + v * T;
-            *reinterpret_cast<uint4 *>(Bs + buf * BN * P + idx / CH * P + idx % CH * 8) = rb[v];
-        }
-    };
-    f32x16_t acc[FM][FN];
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-    const int ktiles = int((s.k + BK - 1) / BK);
-    load(0);
-    put(0);
-    __syncthreads();
-    for (int kt = 0; kt < ktiles; ++kt) {
-        const int buf = kt & 1;
-        if (kt + 1 < ktiles) load(int64_t(kt + 1) * BK);
-        const uint16_t *as = As + buf * BM * P, *bs = Bs + buf * BN * P;
-#pragma unroll
-        for (int kk = 0; kk < BK; kk += 16) {
-            uint4 fa[FM], fb[FN];
-#pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const uint4 *>(as + (wm * TM + 32 * i + l32) * P + kk + 8 * h);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                const int line = j / (FN / 2) * H + wn * (TN / 2) + 32 * (j % (FN / 2)) + l32;
-                fb[j] = *reinterpret_cast<const uint4 *>(bs + line * P + kk + 8 * h);
-            }
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = Mfma<F16>::run(fa[i], fb[j], acc[i][j]);
-        }
-        if (kt + 1 < ktiles) put(buf ^ 1);
-        __syncthreads();
     }
-    // C layout of a 32 x 32 block: lane holds column lane % 32, rows 8 * (e / 4) + 4 * (lane / 32) + e % 4
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN / 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int64_t r = m0 + wm * TM + 32 * i + 8 * (e / 4) + 4 * h + e % 4;
-                const int64_t c = n0 + wn * (TN / 2) + 32 * j + l32;
-                if (r < s.m && c < s.n) out.one(s, r, c, acc[i][j][e], acc[i][j + FN / 2][e]);
-            }
 }
 
-template <int BM, int BN>
-constexpr int gated_any_lds_bytes() { return 2 * (BM + BN) * (64 + 8) * 2; }
+// D = A[:, :k / 2] B + A[:, k / 2:] B2 (the input's gradient: A = [dg | du], the weights as they lie): one accumulator over
+// both products, or (splits) float32 parts of the k tiles that gemm_splitk_reduce adds. Two products and their sum write
+// and read 8 m n bytes more.
+template <bool F16, int TM>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TM == 256 ? 1 : 2, TM == 256 ? 1 : 2))) void gemm_pair(
+    GemmShape s, const uint16_t *__restrict__ a, const uint16_t *__restrict__ b, const uint16_t *__restrict__ b2, AnyStore out,
+    int k_part) {
+    extern __shared__ __align__(1024) char smem[];
+    gemm_stream_tile<F16, 64, 2, false, true, true, AnyStore, TM, TM == 256 ? 3 : 0, 2>(s, a, b, out, smem, b2, k_part);
+}
 
 // [dg | du] of 8 elements a thread (V 8: n, the strides and the pointers multiples of 16 bytes) or of one (V 1).
 struct GatedGrad {

@@ -483,12 +483,12 @@ __device__ __forceinline__ int stream_line(int wn, int j) {
 // across k tiles; 2 (ping-pong) the two waves of each SIMD alternate between a memory phase and an MFMA phase;
 // 3 (k tile 64, two stages, four waves) the cross-tile read placed by hand with the loads split in halves.
 // PAIR 1: two products of A, by B and by b2 of the same shape and strides: half of the tile's columns are B's, half the
-// same columns of b2, and out.store takes the pairs of sums. PAIR 2: B's first k / 2 rows of k are b's, the others b2's
-// (k / 2 a multiple of BK).
+// same columns of b2, and out.store takes the pairs of sums. PAIR 2: the sum of two products, A's first k / 2 columns by b
+// and the others by b2, part blockIdx.z of it over k_part of the k tiles. k (k / 2) is a multiple of 8 there, and operands are within the buffers' reach.
 template <bool F16, int BK, int WN, bool AT, bool BT, bool BUF, class Out, int TM = 256, int KL = 0, int PAIR = 0>
 __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint16_t *__restrict__ a,
                                                  const uint16_t *__restrict__ b, const Out &out, char *smem,
-                                                 const uint16_t *__restrict__ b2 = nullptr) {
+                                                 const uint16_t *__restrict__ b2 = nullptr, int k_part = 0) {
     constexpr int NW = 2 * WN;       // wavefronts (2 x WN)
     constexpr int WR = TM / 2;       // rows a wave
     constexpr int FM = WR / 32;      // 32-row MFMA tiles a wave
@@ -505,7 +505,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     tile_of(blockIdx.x, s.tiles_m, s.tiles_n, tm, tn);
     int64_t oa, ob, od;
     batch_offsets(s, blockIdx.y, oa, ob, od);
-    static_assert(PAIR != 1 || (!BT && FN % 2 == 0), "a pair's halves are rows of k");
+    static_assert(PAIR == 0 || (BUF && !AT && BT == (PAIR == 2) && FN % 2 == 0), "the pairs' layouts");
     constexpr int TNB = PAIR == 1 ? TM / 2 : TM;  // columns of one B operand in the tile
     const int64_t m0 = int64_t(tm) * TM, n0 = int64_t(tn) * TNB;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -513,10 +513,14 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     const int h = lane >> 5, l32 = lane & 31, g = lane >> 4, s16 = lane & 15;
     // one wave a SIMD (WN = 2): the wave index as a scalar, so the loads' LDS destinations are scalar arithmetic
     const int wave_u = WN == 2 ? __builtin_amdgcn_readfirstlane(wave) : wave;
-    const int64_t ks = int64_t(blockIdx.z) * s.k;  // split-k: this workgroup's first k
+    const int64_t ks = PAIR == 0 ? int64_t(blockIdx.z) * s.k : 0;  // split-k: this workgroup's first k
     od += int64_t(blockIdx.z) * s.d_split;
     const uint16_t *pa = a + oa + ks * s.a_k, *pb = b + ob + ks * s.b_k;
-    const int ktiles = int(s.k / BK);
+    const int64_t kb = PAIR == 2 ? s.k / 2 : s.k;  // k of one B operand
+    // PAIR: k tiles of one operand, the last of them perhaps in part; part blockIdx.z takes k_part of all of them
+    const int kth = int((kb + BK - 1) / BK), kfirst = PAIR == 2 ? int(blockIdx.z) * k_part : 0;
+    const int ktiles = PAIR == 0 ? int(s.k / BK) : PAIR == 1 ? kth : min(k_part, 2 * kth - kfirst);
+    (void)kth, (void)kfirst;
 
     // issues this wave's loads [lo, hi) of tile kt into stage st (A segments first, then B)
     // Buffer resources over this tile's rows of A and B (columns when mn-contiguous): the loads then take a
@@ -524,9 +528,9 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     // arithmetic, and rows past m / n read zeros. Operands whose tile span exceeds 2^31 bytes use 64-bit
     // global addresses instead.
     const int64_t mrem = s.m - m0 < TM ? s.m - m0 : TM, nrem = s.n - n0 < TNB ? s.n - n0 : TNB;
-    const int64_t kb = PAIR == 2 ? s.k / 2 : s.k;  // k of one B operand
     const int64_t abytes = AT ? ((s.k - 1) * s.a_k + mrem) * 2 : ((mrem - 1) * s.a_m + s.k) * 2;
-    const int64_t bbytes = BT ? ((kb - 1) * s.b_k + nrem) * 2 : ((nrem - 1) * s.b_n + kb) * 2;
+    const int64_t bbytes = PAIR == 0 ? (BT ? ((s.k - 1) * s.b_k + nrem) * 2 : ((nrem - 1) * s.b_n + s.k) * 2)
+                                     : (BT ? ((kb - 1) * s.b_k + nrem) * 2 : ((nrem - 1) * s.b_n + kb) * 2);
     constexpr bool buf = BUF;  // the launcher checked stream_buffer_ok()
     const __amdgpu_buffer_rsrc_t rsa = __builtin_amdgcn_make_buffer_rsrc(
         (void *)(AT ? pa + m0 : pa + m0 * s.a_m), (short)0, int(abytes), 0x00020000);
@@ -538,11 +542,23 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     auto issue = [&](int st, int kt, int lo, int hi) {
         char *base = smem + st * STAGE_BYTES;
         const int64_t k0 = int64_t(kt) * BK;
+        // PAIR: whether the tile is the second operand's, and its first k there; a chunk past that operand's k is read
+        // out of the buffer's bounds, as zeros
+        const bool second = PAIR == 2 && kfirst + kt >= kth;
+        const int64_t k1 = PAIR == 2 ? int64_t(kfirst + kt - (second ? kth : 0)) * BK : k0;
+        (void)second, (void)k1;
 #pragma unroll
         for (int i = 0; i < TA::segs / NW; ++i) {
             if (i < lo || i >= hi) continue;
             const int seg = wave_u + NW * i;
             const int line = seg * TA::lines_per_seg + lane / TA::chunks, c = lane % TA::chunks;
+            if constexpr (PAIR != 0) {
+                const int kc = (c ^ kmaj_swz<BK>(line)) << 3;
+                const uint32_t vo = k1 + kc < kb ? uint32_t((line * s.a_m + kc) * 2) : 0x80000000u;
+                const uint32_t so = uint32_t((k1 + (second ? kb : 0)) * 2);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, (glds_void_t *)(base + seg * 1024), 16, vo, so, 0, 0);
+                continue;
+            }
             if constexpr (buf) {
                 const uint32_t vo = AT ? uint32_t((line * s.a_k + ((c ^ mnmaj_swz(line)) << 3)) * 2)
                                        : uint32_t((line * s.a_m + ((c ^ kmaj_swz<BK>(line)) << 3)) * 2);
@@ -567,23 +583,17 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
             if (TA::segs / NW + i < lo || TA::segs / NW + i >= hi) continue;
             const int seg = wave_u + NW * i;
             if constexpr (PAIR != 0) {
-                // PAIR 1: the upper half of a wave's segments is the second operand's; PAIR 2: the upper half of k is
-                const bool up = PAIR == 1 ? i >= TB::segs / NW / 2 : k0 >= kb;
+                // PAIR 1: the upper half of a wave's segments is the second operand's
+                const bool up = PAIR == 1 ? i >= TB::segs / NW / 2 : second;
                 const int line = seg * TB::lines_per_seg + lane / TB::chunks - (PAIR == 1 && up ? TNB : 0), c = lane % TB::chunks;
-                const int64_t k1 = PAIR == 2 && up ? k0 - kb : k0;
-                if constexpr (buf) {
-                    const uint32_t vo = BT ? uint32_t((line * s.b_k + ((c ^ mnmaj_swz(line)) << 3)) * 2)
-                                           : uint32_t((line * s.b_n + ((c ^ kmaj_swz<BK>(line)) << 3)) * 2);
-                    const uint32_t so = BT ? uint32_t(k1 * s.b_k * 2) : uint32_t(k1 * 2);
-                    glds_void_t *to = (glds_void_t *)(base + TA::bytes + seg * 1024);
-                    if (up) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsb2, to, 16, vo, so, 0, 0);
-                    else __builtin_amdgcn_raw_ptr_buffer_load_lds(rsb, to, 16, vo, so, 0, 0);
-                } else {
-                    const uint16_t *p = up ? b2 : pb;
-                    if (BT) p += (k1 + line) * s.b_k + min(n0 + ((c ^ mnmaj_swz(line)) << 3), s.n - 8);
-                    else p += min(n0 + line, s.n - 1) * s.b_n + k1 + ((c ^ kmaj_swz<BK>(line)) << 3);
-                    __builtin_amdgcn_global_load_lds(p, (glds_void_t *)(base + TA::bytes + seg * 1024), 16, 0, 0);
-                }
+                const int kc = (c ^ kmaj_swz<BK>(line)) << 3;  // of a line of k
+                // mn-contiguous: a line past k lies past the buffer
+                const uint32_t vo = BT ? uint32_t((line * s.b_k + ((c ^ mnmaj_swz(line)) << 3)) * 2)
+                                       : k1 + kc < kb ? uint32_t((line * s.b_n + kc) * 2) : 0x80000000u;
+                const uint32_t so = BT ? uint32_t(k1 * s.b_k * 2) : uint32_t(k1 * 2);
+                glds_void_t *to = (glds_void_t *)(base + TA::bytes + seg * 1024);
+                if (up) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsb2, to, 16, vo, so, 0, 0);
+                else __builtin_amdgcn_raw_ptr_buffer_load_lds(rsb, to, 16, vo, so, 0, 0);
                 continue;
             }
             const int line = seg * TB::lines_per_seg + lane / TB::chunks, c = lane % TB::chunks;

@@ -32,7 +32,8 @@ int heads_bwd_on(hipStream_t s, const nhip_heads_desc *d, const void *q, const v
                  const float *cos, const float *sin, const void *pos, const void *doq, const void *dok, void *dq, void *dk,
                  void *dqw, void *dkw, void *ws);
 int gated_on(hipStream_t s, const nhip_gated_desc *d, const void *x, const void *gate, const void *up, void *h, float *g,
-             float *u);
+             float *u, void *ws);
+int pair_on(hipStream_t s, const nhip_gemm_desc *d, const void *a, const void *b, const void *b2, void *out, void *ws);
 int gated_grad_on(hipStream_t s, const nhip_gated_desc *d, const void *dh, const float *g, const float *u, void *dgu);
 int clip_on(hipStream_t s, const nhip_clip_desc *d, const nhip_clip_tensor *t, const double *max_at, float *norm,
             float *scale, void *ws);

@@ -235,7 +235,7 @@ int heads_bwd_on(hipStream_t st, const nhip_heads_desc *d, const void *q, const 
 
 namespace {
 
-enum { kSkinnyCfg = 0, kStream256a, kStream256b, kStream128Cfg, kAny128, kAny64, kGatedConfigs };
+enum { kSkinnyCfg = 0, kStream256, kStream128Cfg, kGatedConfigs };
 
 int gated_check(const nhip_gated_desc *d, const char *what) {
     const std::string at(what);
@@ -245,29 +245,25 @@ int gated_check(const nhip_gated_desc *d, const char *what) {
     return 0;
 }
 
-bool gated_rows16(const nhip_gated_desc *d, const void *x, const void *gate, const void *up) {
-    return d->x_m % 8 == 0 && d->w_n % 8 == 0 && on(x, 16) && on(gate, 16) && on(up, 16);
-}
-
-bool gated_takes(const nhip_gated_desc *d, int cfg, bool rows16) {
-    switch (cfg) {
-        case kSkinnyCfg: return rows16 && d->m <= 64 && d->k % 8 == 0 && d->k < (int64_t(1) << 30);
-        case kStream256a:
-        case kStream256b:
-        case kStream128Cfg: return rows16 && d->k % 64 == 0;
-        default: return true;
-    }
-}
-
 int64_t tiles(int64_t m, int64_t bm, int64_t n, int64_t bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); }
 
-int gated_default(const nhip_gated_desc *d, bool rows16) {
-    if (gated_takes(d, kSkinnyCfg, rows16)) return kSkinnyCfg;
-    if (gated_takes(d, kStream128Cfg, rows16)) {
-        if (tiles(d->m, 256, d->n, 128) >= 256) return kStream256b;
-        if (tiles(d->m, 128, d->n, 64) >= 128) return kStream128Cfg;
-    }
-    return tiles(d->m, 128, d->n, 64) >= 512 ? kAny128 : kAny64;
+bool gated_skinny_ok(const nhip_gated_desc *d) { return d->m <= 64 && d->k < (int64_t(1) << 30); }
+
+int gated_default(const nhip_gated_desc *d) {
+    if (gated_skinny_ok(d)) return kSkinnyCfg;
+    return tiles(d->m, 256, d->n, 128) >= 256 ? kStream256 : kStream128Cfg;
+}
+
+// Whether gated_stream can read rows of these lengths and distances in place (from 16-byte addresses).
+bool gated_rows(const nhip_gated_desc *d) {
+    return d->k % 8 == 0 && d->x_m % 8 == 0 && d->w_n % 8 == 0 &&
+           stream_buffer_ok(d->m, d->n, d->k, false, false, d->x_m, 1, 1, d->w_n);
+}
+
+size_t gated_workspace(const nhip_gated_desc *d) {
+    const int cfg = d->config < 0 ? gated_default(d) : d->config;
+    if (cfg == kSkinnyCfg || gated_rows(d)) return 0;
+    return size_t(d->m + 2 * d->n) * size_t((d->k + 7) / 8 * 8) * 2;
 }
 
 template <class K>
@@ -275,7 +271,7 @@ int gated_go(hipStream_t st, K kern, GemmShape s, int bm, int bn, int threads, i
              const void *up, const GatedOut &out) {
     s.tiles_m = int((s.m + bm - 1) / bm);
     s.tiles_n = int((s.n + bn - 1) / bn);
-    if (int64_t(s.tiles_m) * s.tiles_n > 0x7fffffff) return fail("nhip_gated_linear: too many tiles");
+    if ((s.m + bm - 1) / bm * ((s.n + bn - 1) / bn) > 0x7fffffff) return fail("nhip_gated_linear: too many tiles");
     if (lds > 64 * 1024 &&
         check(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
               "hipFuncSetAttribute"))
@@ -285,52 +281,62 @@ int gated_go(hipStream_t st, K kern, GemmShape s, int bm, int bn, int threads, i
     return check(hipGetLastError(), "gated kernel launch");
 }
 
+template <bool F16, bool ANY>
+int gated_few(hipStream_t st, const GemmShape &s, const void *x, const void *gate, const void *up, const GatedOut &o) {
+    if (s.m <= 16) return gated_go(st, gated_skinny<F16, 1, 8, ANY>, s, 64, 16, 512, 0, x, gate, up, o);
+    if (s.m <= 32) return gated_go(st, gated_skinny<F16, 2, 8, ANY>, s, 64, 16, 512, 0, x, gate, up, o);
+    return gated_go(st, gated_skinny<F16, 4, 4, ANY>, s, 64, 16, 256, 0, x, gate, up, o);
+}
+
 template <bool F16>
-int gated_run(hipStream_t st, int cfg, const GemmShape &s, const void *x, const void *gate, const void *up, const GatedOut &o) {
-    const bool buf = stream_buffer_ok(s.m, s.n, s.k, false, false, s.a_m, 1, 1, s.b_n);
-    constexpr int lds4 = gemm_stream_lds_bytes<64, 2>(), lds8 = gemm_stream_lds_bytes<64, 4>();
-    constexpr int lds1 = gemm_stream_lds_bytes<64, 2, 128>();
-    switch (cfg) {
-        case kSkinnyCfg: {
-            if (s.m <= 16) return gated_go(st, gated_skinny<F16, 1, 8>, s, 64, 16, 512, 0, x, gate, up, o);
-            if (s.m <= 32) return gated_go(st, gated_skinny<F16, 2, 8>, s, 64, 16, 512, 0, x, gate, up, o);
-            return gated_go(st, gated_skinny<F16, 4, 4>, s, 64, 16, 256, 0, x, gate, up, o);
+int gated_run(hipStream_t st, int cfg, GemmShape s, const void *x, const void *gate, const void *up, const GatedOut &o, bool in_place,
+              void *ws) {
+    if (cfg == kSkinnyCfg) return in_place ? gated_few<F16, false>(st, s, x, gate, up, o) : gated_few<F16, true>(st, s, x, gate, up, o);
+    if (!in_place) {
+        GatedPad p;
+        p.k = s.k, p.kp = (s.k + 7) / 8 * 8;
+        const void *src[3] = {x, gate, up};
+        uint16_t *to = static_cast<uint16_t *>(ws);
+        for (int i = 0; i < 3; ++i) {
+            p.src[i] = static_cast<const uint16_t *>(src[i]);
+            p.rows[i] = i ? s.n : s.m, p.ld[i] = i ? s.b_n : s.a_m;
+            p.dst[i] = to;
+            to += p.rows[i] * p.kp;
         }
-        case kStream256a:
-            if (buf) return gated_go(st, gated_stream<F16, 256, 2, 3, true>, s, 256, 128, 256, lds4, x, gate, up, o);
-            return gated_go(st, gated_stream<F16, 256, 2, 3, false>, s, 256, 128, 256, lds4, x, gate, up, o);
-        case kStream256b:
-            if (buf) return gated_go(st, gated_stream<F16, 256, 4, 3, true>, s, 256, 128, 512, lds8, x, gate, up, o);
-            return gated_go(st, gated_stream<F16, 256, 4, 3, false>, s, 256, 128, 512, lds8, x, gate, up, o);
-        case kStream128Cfg:
-            if (buf) return gated_go(st, gated_stream<F16, 128, 2, 0, true>, s, 128, 64, 256, lds1, x, gate, up, o);
-            return gated_go(st, gated_stream<F16, 128, 2, 0, false>, s, 128, 64, 256, lds1, x, gate, up, o);
-        case kAny128:
-            return gated_go(st, gated_any<F16, 128, 128, 2, 2>, s, 128, 64, 256, gated_any_lds_bytes<128, 128>(), x, gate, up, o);
-        default:
-            return gated_go(st, gated_any<F16, 64, 64, 2, 1>, s, 64, 32, 128, gated_any_lds_bytes<64, 64>(), x, gate, up, o);
+        const int64_t blocks = ((s.m > s.n ? s.m : s.n) * (p.kp / 8) + 255) / 256;
+        hipLaunchKernelGGL(gated_pad_kernel, dim3(unsigned(blocks < 4096 ? (blocks ? blocks : 1) : 4096)), dim3(256), 0, st, p);
+        if (check(hipGetLastError(), "gated_pad_kernel launch")) return 1;
+        x = p.dst[0], gate = p.dst[1], up = p.dst[2];
+        s.k = s.a_m = s.b_n = p.kp;
     }
+    if (cfg == kStream256)
+        return gated_go(st, gated_stream<F16, 256>, s, 256, 128, 512, gemm_stream_lds_bytes<64, 4>(), x, gate, up, o);
+    return gated_go(st, gated_stream<F16, 128>, s, 128, 64, 256, gemm_stream_lds_bytes<64, 2, 128>(), x, gate, up, o);
 }
 
 }  // namespace
 
 int gated_on(hipStream_t st, const nhip_gated_desc *d, const void *x, const void *gate, const void *up, void *h, float *g,
-             float *u) {
+             float *u, void *ws) {
     if (gated_check(d, "nhip_gated_linear")) return 1;
     if (!g != !u) return fail("nhip_gated_linear: g and u go together");
     if (d->m == 0 || d->n == 0) return 0;
+    int cfg = d->config < 0 ? gated_default(d) : d->config;
+    if (cfg >= kGatedConfigs || (cfg == kSkinnyCfg && !gated_skinny_ok(d)))
+        return fail("nhip_gated_linear: config " + std::to_string(cfg) + " does not take these operands");
     GemmShape s;
     std::memset(&s, 0, sizeof(s));
     s.m = d->m, s.n = d->n, s.k = d->k;
     s.a_m = d->x_m, s.a_k = 1, s.b_k = 1, s.b_n = d->w_n, s.d_m = d->h_m, s.d_n = 1;
-    const bool rows16 = gated_rows16(d, x, gate, up);
-    int cfg = d->config;
-    if (d->k == 0) cfg = kAny64;  // the sums are zeros: no tile is read
-    else if (cfg < 0) cfg = gated_default(d, rows16);
-    else if (cfg >= kGatedConfigs || !gated_takes(d, cfg, rows16))
-        return fail("nhip_gated_linear: config " + std::to_string(cfg) + " does not take these operands");
+    const bool rows = cfg == kSkinnyCfg ? d->k % 8 == 0 && d->x_m % 8 == 0 && d->w_n % 8 == 0 : gated_rows(d);
+    const bool in_place = rows && on(x, 16) && on(gate, 16) && on(up, 16);
+    if (!in_place && cfg != kSkinnyCfg) {
+        if (rows) return fail("nhip_gated_linear: operands of such rows start on 16 bytes");
+        if (!ws || !on(ws, 16)) return fail("nhip_gated_linear: no workspace, or one off 16 bytes");
+    }
     const GatedOut o{h, g, u, d->activation, d->dtype};
-    return d->dtype == NHIP_F16 ? gated_run<true>(st, cfg, s, x, gate, up, o) : gated_run<false>(st, cfg, s, x, gate, up, o);
+    return d->dtype == NHIP_F16 ? gated_run<true>(st, cfg, s, x, gate, up, o, in_place, ws)
+                                : gated_run<false>(st, cfg, s, x, gate, up, o, in_place, ws);
 }
 
 int gated_grad_on(hipStream_t st, const nhip_gated_desc *d, const void *dh, const float *g, const float *u, void *dgu) {
@@ -348,6 +354,99 @@ int gated_grad_on(hipStream_t st, const nhip_gated_desc *d, const void *dh, cons
         else hipLaunchKernelGGL((gated_grad_kernel<bf16_t, 1>), grid, dim3(256), 0, st, a);
     }
     return check(hipGetLastError(), "gated_grad_kernel launch");
+}
+
+namespace {
+
+// The tile and the parts of a pair's k: as many parts as make the tiles' rounds on the chip the shortest, each round as
+// long as its k, the parts' writing and reading added. The rates are the split dots' (Plan._split_us), whose loops these are.
+struct PairPlan {
+    int tm, splits, k_part;
+};
+PairPlan pair_plan(const nhip_gemm_desc *d) {
+    const int half = int((d->k / 2 + 63) / 64), total = 2 * half;
+    PairPlan best{128, 1, total};
+    double least = 0;
+    for (int tm : {256, 128})
+        for (int s : {1, 2, 4, 8}) {
+            if (s > 1 && (total / s < 8 || int64_t(s) * d->m * d->n * 4 > (int64_t(64) << 20))) continue;
+            const int part = (total + s - 1) / s, parts = (total + part - 1) / part;
+            const double t = double(tiles(d->m, tm, d->n, tm)) * parts;
+            // 256: a workgroup a CU; 128: two, one alone taking 0.79 of a round of both
+            double rounds = tm == 256 ? double((int64_t(t) + 255) / 256) : double(int64_t(t) / 512);
+            const int64_t rest = int64_t(t) % 512;
+            if (tm == 128) rounds += rest == 0 ? 0.0 : rest <= 256 ? 0.79 : 1.0;
+            const double us = 6.2 + 64.0 * part * (tm == 256 ? 0.02355 : 0.0142) * rounds +
+                              (parts > 1 ? 4.2 + 8.0 * parts * double(d->m) * double(d->n) / 6.13e6 : 0.0);
+            if (least == 0 || us < least) least = us, best = PairPlan{tm, parts, part};
+        }
+    return best;
+}
+
+size_t pair_workspace(const nhip_gemm_desc *d) {
+    const PairPlan p = pair_plan(d);
+    return p.splits > 1 ? size_t(p.splits) * size_t(d->m) * size_t(d->n) * 4 : 0;
+}
+
+int pair_check(const nhip_gemm_desc *d) {
+    if (d->m < 0 || d->n < 0 || d->k < 0) return fail("nhip_gemm_pair: negative sizes");
+    if (d->a_dtype != d->b_dtype || (d->a_dtype != NHIP_BF16 && d->a_dtype != NHIP_F16)) return fail("nhip_gemm_pair: bf16 or f16");
+    if (d->nbatch || d->a_k != 1 || d->b_n != 1 || d->k % 16 || d->n % 8 || d->a_m % 8 || d->b_k % 8 || d->a_m < d->k || d->b_k < d->n)
+        return fail("nhip_gemm_pair: no batches, A along k and B along n in whole rows, both halves of k and n multiples of 8");
+    const int64_t lim = int64_t(1) << 31;
+    if ((255 * d->a_m + d->k) * 2 >= lim || (d->k / 2 * d->b_k + 256) * 2 >= lim || d->k >= lim)
+        return fail("nhip_gemm_pair: an operand's tile spans 2^31 bytes");
+    return 0;
+}
+
+template <bool F16, int TM>
+int pair_go(hipStream_t st, GemmShape s, const PairPlan &p, const void *a, const void *b, const void *b2, const AnyStore &out) {
+    s.tiles_m = int((s.m + TM - 1) / TM);
+    s.tiles_n = int((s.n + TM - 1) / TM);
+    if (tiles(s.m, TM, s.n, TM) > 0x7fffffff) return fail("nhip_gemm_pair: too many tiles");
+    constexpr int lds = gemm_stream_lds_bytes<64, 2, TM>();
+    auto kern = gemm_pair<F16, TM>;
+    if (check(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
+              "hipFuncSetAttribute"))
+        return 1;
+    hipLaunchKernelGGL(kern, dim3(unsigned(s.tiles_m * s.tiles_n), 1, unsigned(p.splits)), dim3(256), lds, st, s,
+                       static_cast<const uint16_t *>(a), static_cast<const uint16_t *>(b), static_cast<const uint16_t *>(b2), out,
+                       p.k_part);
+    return check(hipGetLastError(), "gemm_pair launch");
+}
+
+}  // namespace
+
+int pair_on(hipStream_t st, const nhip_gemm_desc *d, const void *a, const void *b, const void *b2, void *out, void *ws) {
+    if (pair_check(d)) return 1;
+    if (d->m == 0 || d->n == 0) return 0;
+    if (!on(a, 16) || !on(b, 16) || !on(b2, 16)) return fail("nhip_gemm_pair: operands start on 16 bytes");
+    GemmShape s;
+    std::memset(&s, 0, sizeof(s));
+    s.m = d->m, s.n = d->n, s.k = d->k;
+    s.a_m = d->a_m, s.a_k = 1, s.b_k = d->b_k, s.b_n = 1;
+    s.d_m = d->d_m, s.d_n = d->d_n;
+    const AnyStore to{out, d->d_dtype};
+    if (d->k == 0) {  // a sum of nothing
+        hipLaunchKernelGGL(gemm_splitk_reduce, dim3(1024), dim3(256), 0, st, s, nullptr, 0, d->m * d->n, to);
+        return check(hipGetLastError(), "gemm_splitk_reduce launch");
+    }
+    const PairPlan p = pair_plan(d);
+    GemmShape parts = s;
+    AnyStore first = to;
+    if (p.splits > 1) {
+        if (!ws) return fail("nhip_gemm_pair: no workspace");
+        parts.d_m = d->n, parts.d_n = 1, parts.d_split = d->m * d->n;
+        first = AnyStore{ws, 0};
+    }
+    const int rc = d->a_dtype == NHIP_F16
+                       ? (p.tm == 256 ? pair_go<true, 256>(st, parts, p, a, b, b2, first) : pair_go<true, 128>(st, parts, p, a, b, b2, first))
+                       : (p.tm == 256 ? pair_go<false, 256>(st, parts, p, a, b, b2, first) : pair_go<false, 128>(st, parts, p, a, b, b2, first));
+    if (rc || p.splits == 1) return rc;
+    const int64_t total = d->m * d->n, blocks = (total + 255) / 256;
+    hipLaunchKernelGGL(gemm_splitk_reduce, dim3(unsigned(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, s,
+                       static_cast<const float *>(ws), p.splits, total, to);
+    return check(hipGetLastError(), "gemm_splitk_reduce launch");
 }
 
 // ---- gradient clipping ----------------------------------------------------------------------------------
@@ -437,9 +536,27 @@ int nhip_qk_norm_rope_workspace(const nhip_heads_desc *desc, size_t *bytes) {
     return 0;
 }
 
-int nhip_gated_linear(const nhip_gated_desc *desc, const void *x, const void *gate, const void *up, void *h, float *g, float *u) {
+int nhip_gated_linear(const nhip_gated_desc *desc, const void *x, const void *gate, const void *up, void *h, float *g, float *u,
+                      void *workspace) {
     NHIP_STREAM(st);
-    return gated_on(st, desc, x, gate, up, h, g, u);
+    return gated_on(st, desc, x, gate, up, h, g, u, workspace);
+}
+
+int nhip_gated_linear_workspace(const nhip_gated_desc *desc, size_t *bytes) {
+    if (gated_check(desc, "nhip_gated_linear_workspace")) return 1;
+    *bytes = gated_workspace(desc);
+    return 0;
+}
+
+int nhip_gemm_pair(const nhip_gemm_desc *desc, const void *a, const void *b, const void *b2, void *d, void *workspace) {
+    NHIP_STREAM(st);
+    return pair_on(st, desc, a, b, b2, d, workspace);
+}
+
+int nhip_gemm_pair_workspace(const nhip_gemm_desc *desc, size_t *bytes) {
+    if (pair_check(desc)) return 1;
+    *bytes = pair_workspace(desc);
+    return 0;
 }
 
 int nhip_gated_config_count(int *count) {

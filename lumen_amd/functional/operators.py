@@ -256,13 +256,24 @@ class _GatedLinear(Function):
             d = dh.to(acc)
             return [F.cat([(d * u * da).to(dtype), (d * a).to(dtype)], 1)]
 
-        # [dg | du] in one tensor: one product for both weight gradients, and one operand of dx
+        # [dg | du] in one tensor: one operand of dx, whose two products then share their sums
         (dgu,) = _operator("gated_linear_grad", dtype in ("bfloat16", "float16"), [dh, g, u], body,
                            activation=ctx.activation)
-        dw = dot(dgu, x, (((0,), (0,)), ((), ())), acc, dtype)
-        dx = prims.dot_general(dgu[:, :n], gate, (((1,), (0,)), ((), ())), acc) \
-            + prims.dot_general(dgu[:, n:], up, (((1,), (0,)), ((), ())), acc)
-        return dx.to(dtype), dw[:n], dw[n:]
+        dw = [dot(dgu[:, lo:lo + n], x, (((0,), (0,)), ((), ())), acc, dtype) for lo in (0, n)]
+
+        def product(dgu, gate, up):
+            dims = (((1,), (0,)), ((), ()))
+            return [(prims.dot_general(dgu[:, :n], gate, dims, acc) + prims.dot_general(dgu[:, n:], up, dims, acc)).to(dtype)]
+
+        (dx,) = _operator("gemm_pair", _pair_taken(gate), [dgu, gate, up], product)
+        return dx, dw[0], dw[1]
+
+
+def _pair_taken(weight):
+    """Whether nhip_gemm_pair takes ``[dg | du]`` and weights of this type: whole 16-byte rows, a tile within 2^31 bytes."""
+    n, k = weight.shape
+    return (weight.dtype in ("bfloat16", "float16") and n > 0 and k > 0 and n % 8 == 0 and k % 8 == 0
+            and n * k < (1 << 30) - 1024 and n < 1 << 21)
 
 
 def gated_linear(input, gate_weight, up_weight, activation="silu"):

@@ -111,7 +111,8 @@ def test_gated_gradient_against_differences(activation):
 def test_gated_16_bit_is_two_fusions_and_ordinary_products():
     g = _graph(lambda x, gate, up, dh: (lambda h, pull: [h, *pull(dh)])(*L.vjp(F.gated_linear, x, gate, up)),
                *(np.zeros(s, np.uint16) for s in ((64, 64), (128, 64), (128, 64), (64, 128))), dtypes=["bfloat16"] * 4)
-    assert [n.params["name"] for n in g.nodes if n.prim == "fusion"] == ["gated_linear", "gated_linear_grad"]
+    assert [n.params["name"] for n in g.nodes if n.prim == "fusion"] == ["gated_linear", "gated_linear_grad",
+                                                                                          "gemm_pair"]
     forward = _graph(F_gated, *(np.zeros(s, np.uint16) for s in ((64, 64), (128, 64), (128, 64))), dtypes=["bfloat16"] * 3)
     plan = Plan(forward, build_kernels=False)
     assert [st.kind for st in plan.steps] == ["gated_fwd"] and len(plan.steps[0].outputs) == 1  # g and u are not stored
@@ -275,6 +276,17 @@ def test_abi_refusals():
     assert n.value == 2 * 1024 * 8
     with pytest.raises(RuntimeError, match="negative count"):
         nv.call("nhip_clip_grad_norm_workspace", C.byref(nv.ClipDesc(count=-1)), C.byref(n))
+    for kw, match in [(dict(m=-1), "negative"), (dict(dtype=0), "bf16 or f16"), (dict(activation=4), "activation")]:
+        with pytest.raises(RuntimeError, match=match):
+            nv.call("nhip_gated_linear_workspace", C.byref(nv.GatedDesc(**{**dict(m=1, n=1, k=1, dtype=1, config=-1), **kw})), C.byref(n))
+    for m, k, want in [(64, 515, 0), (65, 512, 0), (65, 515, (65 + 2 * 8) * 520 * 2)]:  # few rows are read as they are
+        nv.call("nhip_gated_linear_workspace", C.byref(nv.GatedDesc(m=m, n=8, k=k, x_m=k, w_n=k, dtype=1, config=-1)), C.byref(n))
+        assert n.value == want
+    for kw, match in [(dict(k=24), "multiples of 8"), (dict(a_dtype=0, b_dtype=0), "bf16 or f16"), (dict(a_m=63), "whole rows"),
+                      (dict(m=-1), "negative"), (dict(b_k=1 << 31), "2\\^31")]:
+        pair = dict(m=64, n=64, k=128, a_dtype=1, b_dtype=1, d_dtype=1, a_m=128, a_k=1, b_k=64, b_n=1, d_m=64, d_n=1)
+        with pytest.raises(RuntimeError, match=match):
+            nv.call("nhip_gemm_pair_workspace", C.byref(nv.GemmDesc(**{**pair, **kw})), C.byref(n))
     plan = C.c_void_p()
     nv.call("nhip_plan_create", C.byref(plan))
     d = nv.ClipDesc(count=3)
