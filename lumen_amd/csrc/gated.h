@@ -139,6 +139,19 @@ __global__ __launch_bounds__(TM * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     gemm_stream_tile<F16, 64, TM / 64, false, false, true, GatedOut, TM, TM == 256 ? 3 : 0, 1>(s, x, gate, out, smem, up);
 }
 
+// 8 elements at p of any alignment as 4-byte words, which memory reads at full width where words at 2-byte addresses take
+// several passes (one row of [1, 2047] x 2 [8192, 2047]: 31.7 us so, 20.6 with words; [64, 2047] 81, 40): the words that hold them, 5 of
+// them where p is in a word's middle, and no others, so no read leaves the words that the row lies in.
+__device__ __forceinline__ uint4 load8_words(const uint16_t *p) {
+    typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(4)));
+    const uint32_t odd = uint32_t(reinterpret_cast<uintptr_t>(p)) & 2;
+    const uint32_t *q = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(p) - odd);
+    const words4 v = *reinterpret_cast<const words4 *>(q);
+    const uint32_t last = q[odd ? 4 : 3], shift = odd * 8;
+    return make_uint4(__builtin_amdgcn_alignbit(v[1], v[0], shift), __builtin_amdgcn_alignbit(v[2], v[1], shift),
+                      __builtin_amdgcn_alignbit(v[3], v[2], shift), __builtin_amdgcn_alignbit(last, v[3], shift));
+}
+
 // Few rows: a workgroup takes 16 columns of both weights, its NW waves divide k 64 at a time, fragments straight from
 // memory (v_mfma_f32_16x16x32: 16 rows of 64 contiguous bytes), the waves' sums added through LDS in wave order. Reading
 // the weights once is all the work.
@@ -151,7 +164,7 @@ __global__ __launch_bounds__(64 * NW) void gated_skinny(GemmShape s, const uint1
     __shared__ f32x4_t sums[NW][2][MT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
     auto get = [](const uint16_t *p) {
-        if constexpr (ANY) return load8_any(p, 8);
+        if constexpr (ANY) return load8_words(p);
         else return *reinterpret_cast<const uint4 *>(p);
     };
     const int64_t n0 = int64_t(blockIdx.x) * 16;
@@ -239,7 +252,8 @@ static __global__ __launch_bounds__(256) void gated_pad_kernel(GatedPad a) {
         const int64_t total = a.rows[which] * per;
         for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
             const int64_t row = i / per, c = (i - row * per) * 8;
-            *reinterpret_cast<uint4 *>(a.dst[which] + row * a.kp + c) = load8_any(a.src[which] + row * a.ld[which] + c, a.k - c);
+            const uint16_t *src = a.src[which] + row * a.ld[which] + c;
+            *reinterpret_cast<uint4 *>(a.dst[which] + row * a.kp + c) = a.k - c >= 8 ? load8_words(src) : load8_any(src, a.k - c);
         }
     }
 }

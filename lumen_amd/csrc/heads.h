@@ -105,25 +105,26 @@ __device__ __forceinline__ HeadsLane heads_lane(const HeadsArgs &a, int l) {
     return r;
 }
 
-// (v0, v1) turned by the pairs' angles; back: by minus them.
-template <int E>
-__device__ __forceinline__ void heads_turn(float (&v0)[E], float (&v1)[E], const float (&c)[E], const float (&s)[E],
+// (v0, v1) turned by the pairs' angles, or (BACK) by minus them.
+template <bool BACK, int E>
+__device__ __forceinline__ void heads_turn(float (&v0)[E], float (&v1)[E], const float (&c)[E], const float (&sn)[E],
                                            bool interleaved) {
+    auto s = [&](int i) { return BACK ? -sn[i] : sn[i]; };
     if (interleaved) {
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) {
             const float a = v0[2 * i], b = v0[2 * i + 1], p = v1[2 * i], q = v1[2 * i + 1];
-            v0[2 * i] = a * c[i] - b * s[i];
-            v0[2 * i + 1] = b * c[i] + a * s[i];
-            v1[2 * i] = p * c[E / 2 + i] - q * s[E / 2 + i];
-            v1[2 * i + 1] = q * c[E / 2 + i] + p * s[E / 2 + i];
+            v0[2 * i] = a * c[i] - b * s(i);
+            v0[2 * i + 1] = b * c[i] + a * s(i);
+            v1[2 * i] = p * c[E / 2 + i] - q * s(E / 2 + i);
+            v1[2 * i + 1] = q * c[E / 2 + i] + p * s(E / 2 + i);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             const float a = v0[i], b = v1[i];
-            v0[i] = a * c[i] - b * s[i];
-            v1[i] = b * c[i] + a * s[i];
+            v0[i] = a * c[i] - b * s(i);
+            v1[i] = b * c[i] + a * s(i);
         }
     }
 }
@@ -169,69 +170,58 @@ __device__ __forceinline__ void heads_table(const float *p, float (&v)[E]) {
     }
 }
 
-// U rows a group of lanes, all of their reads issued before the first is used.
-template <typename T, int E, int U>
+// One row a group of lanes. More rows a lane at a time only cost waves: at [4, 4096, 16 + 16, 128] in bf16 one row takes 48.4 us
+// (5.5 TB/s), two 57.5, four 65.4.
+template <typename T, int E>
 __global__ __launch_bounds__(256) void heads_fwd_kernel(HeadsArgs a) {
     typedef HeadsChunk<T, E> C;
     const bool second = blockIdx.x >= a.t[0].blocks;
     const HeadsTensor &t = a.t[second];
-    const uint32_t block = blockIdx.x - (second ? a.t[0].blocks : 0);
-    const int lane = threadIdx.x & 63;
-    const uint32_t groups = 256 / a.lanes, group = threadIdx.x / a.lanes;
-    const HeadsLane ln = heads_lane<E>(a, lane & (a.lanes - 1));
-    float w0[E], w1[E];
+    const uint32_t row = (blockIdx.x - (second ? a.t[0].blocks : 0)) * (256 / a.lanes) + threadIdx.x / a.lanes;
+    const HeadsLane ln = heads_lane<E>(a, threadIdx.x & (a.lanes - 1));
+    const bool in = row < t.rows && ln.in;
+    const HeadsRow r = heads_row(a, t, row < t.rows ? row : 0);
+    float v0[E], v1[E], w0[E], w1[E], c[E], s[E], sq = 0.0f;
 #pragma unroll
     for (int i = 0; i < E; ++i) w0[i] = w1[i] = 1.0f;
-    if (t.w && ln.in) {
+    if (t.w && ln.in) {  // before the rows: their wait is then the only one
         const T *w = static_cast<const T *>(t.w);
         C::get(*reinterpret_cast<const typename C::raw *>(w + ln.c0), w0);
         C::get(*reinterpret_cast<const typename C::raw *>(w + ln.c1), w1);
     }
-    HeadsRow r[U];
-    typename C::raw x0[U], x1[U];
-    float c[U][E], s[U][E];
-    bool in[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint32_t row = (block * U + u) * groups + group;
-        in[u] = row < t.rows;
-        r[u] = heads_row(a, t, in[u] ? row : 0);
-        in[u] = in[u] && ln.in;
-        if (in[u]) {
-            const T *x = static_cast<const T *>(t.x) + r[u].b * t.x_b + int64_t(r[u].s) * t.x_s + int64_t(r[u].h) * t.x_n;
-            x0[u] = *reinterpret_cast<const typename C::raw *>(x + ln.c0);
-            x1[u] = *reinterpret_cast<const typename C::raw *>(x + ln.c1);
-            if (ln.turned) {
-                heads_table<E>(a.cos + r[u].p * (a.rot / 2) + ln.pair, c[u]);
-                heads_table<E>(a.sin + r[u].p * (a.rot / 2) + ln.pair, s[u]);
-            }
+    typename C::raw x0, x1;
+    if (in) {
+        const T *x = static_cast<const T *>(t.x) + r.b * t.x_b + int64_t(r.s) * t.x_s + int64_t(r.h) * t.x_n;
+        x0 = *reinterpret_cast<const typename C::raw *>(x + ln.c0);
+        x1 = *reinterpret_cast<const typename C::raw *>(x + ln.c1);
+        if (ln.turned) {
+            heads_table<E>(a.cos + r.p * (a.rot / 2) + ln.pair, c);
+            heads_table<E>(a.sin + r.p * (a.rot / 2) + ln.pair, s);
         }
     }
-    const float over_d = 1.0f / float(a.d);
+    if (in) {
+        C::get(x0, v0);
+        C::get(x1, v1);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        float v0[E], v1[E], sq = 0.0f;
-        if (in[u]) {
-            C::get(x0[u], v0);
-            C::get(x1[u], v1);
-#pragma unroll
-            for (int i = 0; i < E; ++i) sq += v0[i] * v0[i] + v1[i] * v1[i];
-        }
-        sq = heads_sum(sq, a.lanes);
-        if (!in[u]) continue;
-        const float inv = rsqrtf(sq * over_d + a.eps);
-#pragma unroll
-        for (int i = 0; i < E; ++i) v0[i] = v0[i] * inv * w0[i], v1[i] = v1[i] * inv * w1[i];
-        if (ln.turned) heads_turn<E>(v0, v1, c[u], s[u], a.interleaved);
-        T *y = static_cast<T *>(t.y) + r[u].b * t.y_b + int64_t(r[u].s) * t.y_s + int64_t(r[u].h) * t.y_n;
-        *reinterpret_cast<typename C::raw *>(y + ln.c0) = C::put(v0);
-        *reinterpret_cast<typename C::raw *>(y + ln.c1) = C::put(v1);
+        for (int i = 0; i < E; ++i) sq += v0[i] * v0[i] + v1[i] * v1[i];
     }
+    sq = heads_sum(sq, a.lanes);
+    if (!in) return;
+    const float inv = rsqrtf(sq / float(a.d) + a.eps);
+#pragma unroll
+    for (int i = 0; i < E; ++i) v0[i] = v0[i] * inv * w0[i], v1[i] = v1[i] * inv * w1[i];
+    if (ln.turned) heads_turn<false, E>(v0, v1, c, s, a.interleaved);
+    T *y = static_cast<T *>(t.y) + r.b * t.y_b + int64_t(r.s) * t.y_s + int64_t(r.h) * t.y_n;
+    *reinterpret_cast<typename C::raw *>(y + ln.c0) = C::put(v0);
+    *reinterpret_cast<typename C::raw *>(y + ln.c1) = C::put(v1);
 }
 
-// The backward. Workgroups walk a tensor's rows, each group of lanes U of them at a time; a lane keeps the weight
-// gradient of its own 2 E elements over all of them, and a workgroup writes one row of D partial sums.
-template <typename T, int E, int U>
+// The backward. Workgroups walk a tensor's rows, each group of lanes one at a time; a lane keeps the weight gradient of its
+// own 2 E elements over all of them, and a workgroup writes one row of D partial sums. Its registers leave three workgroups
+// a CU (E 8): launched as two rounds of them the case above takes 82 us (4.9 TB/s), as 1024 workgroups 100, with two rows at
+// a time 90 at best, with the next row's reads ahead of this one's work 82, with the weights read again for each row (four
+// workgroups a CU) 85.
+template <typename T, int E>
 __global__ __launch_bounds__(256) void heads_bwd_kernel(HeadsArgs a) {
     typedef HeadsChunk<T, E> C;
     __shared__ float sums[4][64][2 * E + 1];
@@ -241,9 +231,9 @@ __global__ __launch_bounds__(256) void heads_bwd_kernel(HeadsArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t groups = 256 / a.lanes, group = threadIdx.x / a.lanes;
     const HeadsLane ln = heads_lane<E>(a, lane & (a.lanes - 1));
-    float w0[E], w1[E], g0[E], g1[E];
+    float g0[E], g1[E], w0[E], w1[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) w0[i] = w1[i] = 1.0f, g0[i] = g1[i] = 0.0f;
+    for (int i = 0; i < E; ++i) g0[i] = g1[i] = 0.0f, w0[i] = w1[i] = 1.0f;
     if (t.w && ln.in) {
         const T *w = static_cast<const T *>(t.w);
         C::get(*reinterpret_cast<const typename C::raw *>(w + ln.c0), w0);
@@ -251,67 +241,52 @@ __global__ __launch_bounds__(256) void heads_bwd_kernel(HeadsArgs a) {
     }
     const float over_d = 1.0f / float(a.d);
     // 64-bit: the last step may pass 2^32
-    for (uint64_t base = uint64_t(block) * U * groups; base < t.rows; base += uint64_t(t.blocks) * U * groups) {
-        HeadsRow r[U];
-        typename C::raw x0[U], x1[U], y0[U], y1[U];
-        float c[U][E], s[U][E];
-        bool in[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint64_t row = base + u * groups + group;
-            in[u] = row < t.rows;
-            r[u] = heads_row(a, t, in[u] ? uint32_t(row) : 0);
-            in[u] = in[u] && ln.in;
-            if (in[u]) {
-                const T *x = static_cast<const T *>(t.x) + r[u].b * t.x_b + int64_t(r[u].s) * t.x_s + int64_t(r[u].h) * t.x_n;
-                const T *dy = static_cast<const T *>(t.dy) + r[u].b * t.dy_b + int64_t(r[u].s) * t.dy_s + int64_t(r[u].h) * t.dy_n;
-                x0[u] = *reinterpret_cast<const typename C::raw *>(x + ln.c0);
-                x1[u] = *reinterpret_cast<const typename C::raw *>(x + ln.c1);
-                y0[u] = *reinterpret_cast<const typename C::raw *>(dy + ln.c0);
-                y1[u] = *reinterpret_cast<const typename C::raw *>(dy + ln.c1);
-                if (ln.turned) {
-                    heads_table<E>(a.cos + r[u].p * (a.rot / 2) + ln.pair, c[u]);
-                    heads_table<E>(a.sin + r[u].p * (a.rot / 2) + ln.pair, s[u]);
-                }
+    for (uint64_t base = uint64_t(block) * groups; base < t.rows; base += uint64_t(t.blocks) * groups) {
+        const bool in = base + group < t.rows && ln.in;
+        const HeadsRow r = heads_row(a, t, base + group < t.rows ? uint32_t(base + group) : 0);
+        typename C::raw x0, x1, y0, y1;
+        float c[E], s[E];
+        if (in) {
+            const T *x = static_cast<const T *>(t.x) + r.b * t.x_b + int64_t(r.s) * t.x_s + int64_t(r.h) * t.x_n;
+            const T *dy = static_cast<const T *>(t.dy) + r.b * t.dy_b + int64_t(r.s) * t.dy_s + int64_t(r.h) * t.dy_n;
+            x0 = *reinterpret_cast<const typename C::raw *>(x + ln.c0);
+            x1 = *reinterpret_cast<const typename C::raw *>(x + ln.c1);
+            y0 = *reinterpret_cast<const typename C::raw *>(dy + ln.c0);
+            y1 = *reinterpret_cast<const typename C::raw *>(dy + ln.c1);
+            if (ln.turned) {
+                heads_table<E>(a.cos + r.p * (a.rot / 2) + ln.pair, c);
+                heads_table<E>(a.sin + r.p * (a.rot / 2) + ln.pair, s);
             }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float v0[E], v1[E], z0[E], z1[E], sq = 0.0f, dot = 0.0f;
-            if (in[u]) {
-                C::get(x0[u], v0);
-                C::get(x1[u], v1);
-                C::get(y0[u], z0);
-                C::get(y1[u], z1);
-                if (ln.turned) {
-#pragma unroll
-                    for (int i = 0; i < E; ++i) s[u][i] = -s[u][i];
-                    heads_turn<E>(z0, z1, c[u], s[u], a.interleaved);
-                }
-#pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    sq += v0[i] * v0[i] + v1[i] * v1[i];
-                    dot += z0[i] * w0[i] * v0[i] + z1[i] * w1[i] * v1[i];
-                }
-            }
-            sq = heads_sum(sq, a.lanes);
-            dot = heads_sum(dot, a.lanes);
-            if (!in[u]) continue;
-            const float inv = rsqrtf(sq * over_d + a.eps);
-            const float mean = dot * over_d * inv;
+        float v0[E], v1[E], z0[E], z1[E], sq = 0.0f, dot = 0.0f;
+        if (in) {
+            C::get(x0, v0);
+            C::get(x1, v1);
+            C::get(y0, z0);
+            C::get(y1, z1);
+            if (ln.turned) heads_turn<true, E>(z0, z1, c, s, a.interleaved);
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const float h0 = v0[i] * inv, h1 = v1[i] * inv;
-                g0[i] += z0[i] * h0;
-                g1[i] += z1[i] * h1;
-                z0[i] = inv * (z0[i] * w0[i] - h0 * mean);
-                z1[i] = inv * (z1[i] * w1[i] - h1 * mean);
+                sq += v0[i] * v0[i] + v1[i] * v1[i];
+                dot += z0[i] * w0[i] * v0[i] + z1[i] * w1[i] * v1[i];
             }
-            if (!t.y) continue;  // the weight's gradient alone
-            T *dx = static_cast<T *>(t.y) + r[u].b * t.y_b + int64_t(r[u].s) * t.y_s + int64_t(r[u].h) * t.y_n;
-            *reinterpret_cast<typename C::raw *>(dx + ln.c0) = C::put(z0);
-            *reinterpret_cast<typename C::raw *>(dx + ln.c1) = C::put(z1);
         }
+        sq = heads_sum(sq, a.lanes);
+        dot = heads_sum(dot, a.lanes);
+        if (!in) continue;
+        const float inv = rsqrtf(sq * over_d + a.eps), mean = dot * over_d * inv;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float h0 = v0[i] * inv, h1 = v1[i] * inv;
+            g0[i] += z0[i] * h0;
+            g1[i] += z1[i] * h1;
+            z0[i] = inv * (z0[i] * w0[i] - h0 * mean);
+            z1[i] = inv * (z1[i] * w1[i] - h1 * mean);
+        }
+        if (!t.y) continue;  // the weight's gradient alone
+        T *dx = static_cast<T *>(t.y) + r.b * t.y_b + int64_t(r.s) * t.y_s + int64_t(r.h) * t.y_n;
+        *reinterpret_cast<typename C::raw *>(dx + ln.c0) = C::put(z0);
+        *reinterpret_cast<typename C::raw *>(dx + ln.c1) = C::put(z1);
     }
     if (!t.part) return;
     // over the wave's groups by lane exchange, over the waves through LDS, both in a fixed order

@@ -16,7 +16,10 @@ bool on(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % b
 // ---- heads ----------------------------------------------------------------------------------------------
 
 constexpr int64_t kHeadsLaunchRows = int64_t(1) << 30;  // heads of a launch: row arithmetic is 32-bit
-constexpr int64_t kHeadsBlocks = 1024;                  // workgroups of a backward launch: their partial sums are read again
+// Workgroups of a backward launch at most: each leaves a row of partial sums that is read again. Two rounds of the three
+// that fit a CU with chunks of 8 elements, 2048 otherwise ([4, 4096, 16 + 16, 128] in chunks of 4: 1536 101 us, 2048 88,
+// 4096 87, whose sums take 2 us longer).
+constexpr int64_t kHeadsBlocks8 = 1536, kHeadsBlocks = 2048;
 
 FastDiv fast_div(uint32_t d) {
     FastDiv f{d, 0, 0};
@@ -85,49 +88,44 @@ HeadsPlan heads_plan(const nhip_heads_desc *d, bool bwd, std::initializer_list<c
     return p;
 }
 
-// Workgroups of tensor `rows` of a backward launch of `both` rows in all.
-int64_t heads_bwd_blocks(int64_t rows, int64_t both) {
-    if (rows == 0) return 0;
-    const int64_t share = (kHeadsBlocks * rows + both - 1) / both, need = (rows + 7) / 8;
-    return share < need ? share : need;
-}
-
 struct HeadsBlocks {
     int64_t q, k;
 };
-HeadsBlocks heads_parts(const nhip_heads_desc *d) {
-    const int64_t t = heads_tokens(d), q = t * d->heads, k = t * d->kv_heads;
-    return {heads_bwd_blocks(q, q + k), heads_bwd_blocks(k, q + k)};
+// Workgroups of a backward launch for the queries and the keys, in proportion to their rows: four rows a group of lanes, but
+// a workgroup a CU before that ([3, 331, 6 + 2, 80]: 497 workgroups of one row each leave as many rows to sum).
+HeadsBlocks heads_blocks(const nhip_heads_desc *d, int lanes, int64_t cap) {
+    const int64_t t = heads_tokens(d), q = t * d->heads, k = t * d->kv_heads, groups = 256 / lanes;
+    auto share = [&](int64_t rows) -> int64_t {
+        if (rows == 0) return 0;
+        const int64_t need = (rows + groups - 1) / groups, part = 256 * rows / (q + k) + 1;
+        const int64_t want = need / 4 > part ? need / 4 : (need < part ? need : part), most = cap * rows / (q + k) + 1;
+        return want < most ? want : most;
+    };
+    return {share(q), share(k)};
 }
 
 size_t heads_workspace(const nhip_heads_desc *d) {
     const int64_t tokens = d->batch * d->seq, each = heads_tokens(d);
     if (each == 0) return 0;
-    const HeadsBlocks b = heads_parts(d);
-    return size_t((tokens + each - 1) / each) * size_t(b.q + b.k) * size_t(d->head_dim) * 4;
+    return size_t((tokens + each - 1) / each) * size_t(kHeadsBlocks + 2) * size_t(d->head_dim) * 4;
 }
 
 template <typename T, int E>
-int heads_launch_fwd(hipStream_t st, HeadsArgs &a, int64_t most) {
-    // four rows a group of lanes where that still leaves every CU two workgroups: [4, 4096, 16 + 16, 128] in one launch
+int heads_launch_fwd(hipStream_t st, HeadsArgs &a) {
     const uint32_t groups = 256 / a.lanes;
-    const bool many = most / (4 * groups) >= 512;
-    const uint32_t per = groups * (many ? 4 : 1);
-    for (HeadsTensor &t : a.t) t.blocks = (t.rows + per - 1) / per;
+    for (HeadsTensor &t : a.t) t.blocks = (t.rows + groups - 1) / groups;
     const uint32_t grid = a.t[0].blocks + a.t[1].blocks;
     if (!grid) return 0;
-    if (many) hipLaunchKernelGGL((heads_fwd_kernel<T, E, 4>), dim3(grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((heads_fwd_kernel<T, E, 1>), dim3(grid), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((heads_fwd_kernel<T, E>), dim3(grid), dim3(256), 0, st, a);
     return check(hipGetLastError(), "heads_fwd_kernel launch");
 }
 
 template <typename T>
 int heads_launch(hipStream_t st, HeadsArgs &a, int e, bool bwd) {
-    const int64_t rows = int64_t(a.t[0].rows) + a.t[1].rows;
     if (!bwd) {
         if constexpr (!std::is_same<T, float>::value)
-            if (e == 8) return heads_launch_fwd<T, 8>(st, a, rows);
-        if (e == 4) return heads_launch_fwd<T, 4>(st, a, rows);
+            if (e == 8) return heads_launch_fwd<T, 8>(st, a);
+        if (e == 4) return heads_launch_fwd<T, 4>(st, a);
         for (HeadsTensor &t : a.t) {
             const int64_t blocks = (int64_t(t.rows) * a.lanes + 255) / 256;
             t.blocks = uint32_t(blocks < 16384 ? blocks : 16384);
@@ -141,11 +139,11 @@ int heads_launch(hipStream_t st, HeadsArgs &a, int e, bool bwd) {
     if (!grid) return 0;
     if constexpr (!std::is_same<T, float>::value) {
         if (e == 8) {
-            hipLaunchKernelGGL((heads_bwd_kernel<T, 8, 2>), dim3(grid), dim3(256), 0, st, a);
+            hipLaunchKernelGGL((heads_bwd_kernel<T, 8>), dim3(grid), dim3(256), 0, st, a);
             return check(hipGetLastError(), "heads_bwd_kernel launch");
         }
     }
-    if (e == 4) hipLaunchKernelGGL((heads_bwd_kernel<T, 4, 2>), dim3(grid), dim3(256), 0, st, a);
+    if (e == 4) hipLaunchKernelGGL((heads_bwd_kernel<T, 4>), dim3(grid), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((heads_any_kernel<T, true>), dim3(grid), dim3(256), 0, st, a);
     return check(hipGetLastError(), "heads_bwd_kernel launch");
 }
@@ -209,7 +207,7 @@ int heads_bwd_on(hipStream_t st, const nhip_heads_desc *d, const void *q, const 
     const HeadsPlan p = heads_plan(d, true, {q, k, qw, kw, doq, dok, dq, dk}, cos, sin);
     HeadsArgs a = heads_args(d, p, q, k, qw, kw, cos, sin, pos);
     a.t[0].dy = doq, a.t[1].dy = dok, a.t[0].y = dq, a.t[1].y = dk;
-    const HeadsBlocks b = heads_parts(d);
+    const HeadsBlocks b = heads_blocks(d, p.lanes, p.e == 8 ? kHeadsBlocks8 : kHeadsBlocks);
     float *pq = static_cast<float *>(ws), *pk = pq ? pq + p.launches * b.q * d->head_dim : nullptr;
     for (int64_t i = 0; i < p.launches; ++i) {
         const int64_t t0 = i * each, n = tokens - t0 < each ? tokens - t0 : each;

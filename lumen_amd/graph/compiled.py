@@ -46,7 +46,9 @@ class Compiled:
         return data[0].device if data else ("meta:0" if tensors else "hip:0")
 
     def _key(self, args, target):
-        return (tuple(nn.structure(a) for a in args), target, config.compiler.key())
+        # a tensor argument by its type alone (what nn.structure says of one, without a call for each)
+        parts = [(a.dtype, a.shape) if type(a) is Tensor and not a._is_parameter else nn.structure(a) for a in args]
+        return (tuple(parts), target, config.compiler.key())
 
     def _prepare(self, args):
         target = self._target(args)
@@ -163,7 +165,8 @@ class Compiled:
 
     def __call__(self, *args):
         target, (traced, plan, workspace, recipe) = self._prepare(args)
-        ran = plan is not None and not any(isinstance(a, Tensor) and device_type(a.device) == "meta" for a in args)
+        ran = plan is not None and not any(isinstance(a, Tensor) and a.device != target and device_type(a.device) == "meta"
+                                           for a in args)
         if not ran:
             g = traced.graph
             outs = [Tensor(g.types[v].dtype, g.types[v].shape, "meta") for v in g.outputs]
@@ -183,7 +186,7 @@ class Compiled:
                 else:
                     t = traced.weights[k]._placed(target)
                 keep.append(t)
-            ptrs = self._run(plan, workspace, traced, [t.data_ptr() for t in keep], keep)
+            ptrs = self._run(plan, workspace, traced, [t._buffer.ptr + t._offset for t in keep], keep)
             self._last_buffers = (workspace.ptr, ptrs)
             # outputs computed over the weight they replace, or views of the workspace
             outs = [keep[i] if i is not None else Tensor.on_device(dtype, shape, target, workspace, offset)
@@ -194,7 +197,8 @@ class Compiled:
             self._keep = keep
         for i, path, value in traced.static_writes:
             nn.assign(args[i], path, value)
-        return _rebuild(traced.out, iter(outs))
+        flat = traced.out_list
+        return _rebuild(traced.out, iter(outs)) if flat is None else flat(outs[:traced.n_returned])
 
 
 class _Recipe:

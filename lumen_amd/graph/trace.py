@@ -4,6 +4,7 @@ scalars (weakly typed, ``_scalar_dtype``), and weights the function assigns (``c
 
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass, field
 
 from lumen_amd import nn
@@ -23,6 +24,12 @@ class Traced:
     written: list = field(default_factory=list)   # weight indices whose new values are extra outputs
     n_returned: int = 0
     static_writes: list = field(default_factory=list)  # (arg index, path, value) static scalars assigned
+
+    @functools.cached_property
+    def out_list(self):
+        """``list`` or ``tuple`` where the function returned that of tensors alone, else None."""
+        flat = type(self.out) in (list, tuple) and all(isinstance(v, TracedTensor) for v in self.out)
+        return type(self.out) if flat else None
 
 
 def tree_leaves(x):

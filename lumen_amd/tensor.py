@@ -70,6 +70,9 @@ class Tensor:
     """A tensor of ``dtype`` and ``shape`` on ``device``; hip data is ``buffer`` at byte ``offset``,
     contiguous row-major."""
 
+    _host = _pending = grad = _placements = None
+    _is_parameter = False
+
     def __init__(self, dtype, shape, device="cpu", host=None, buffer=None, offset=0):
         self.dtype = D.canonical(dtype)
         self.shape = tuple(int(s) for s in shape)
@@ -86,10 +89,8 @@ class Tensor:
     def on_device(cls, dtype, shape, device, buffer, offset):
         """A device tensor over ``buffer`` whose canonical dtype, shape tuple and device name the caller has."""
         t = cls.__new__(cls)
-        t.dtype, t.shape, t.device = dtype, shape, device
-        t._host, t._buffer, t._offset = None, buffer, offset
-        t._is_parameter, t._placements, t._pending, t.grad = False, {}, None, None
-        return t
+        t.dtype, t.shape, t.device, t._buffer, t._offset = dtype, shape, device, buffer, offset
+        return t  # the rest as the class has it: no host data, no weight
 
     # -- basics
     @property
