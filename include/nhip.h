@@ -292,14 +292,17 @@ int nhip_gated_linear(const nhip_gated_desc *desc, const void *x, const void *ga
 int nhip_gated_linear_workspace(const nhip_gated_desc *desc, size_t *bytes);
 /* Number of kernels nhip_gated_linear has (for tests and timing); a config the operands cannot take fails. */
 int nhip_gated_config_count(int *count);
-/* [dg | du] ([m, 2 n], contiguous, the type of dh) of dh [m, n]: dg = dh u act'(g), du = dh act(g), each rounded once. */
+/* [dg | du] of dh [m, n]: dg = dh u act'(g), du = dh act(g), each rounded once to the type of dh, as one contiguous matrix
+ * of m rows: n of dg, zeros up to a multiple of 8, n of du, zeros again. */
 int nhip_gated_linear_grad(const nhip_gated_desc *desc, const void *dh, const float *g, const float *u, void *dgu);
-/* D = A[:, :k / 2] B + A[:, k / 2:] B2 for A [m, k] along k and B, B2 [k / 2, n] along n, bf16 or f16, with one float32 sum
- * over both: the input's gradient of A = [dg | du] and the two weights. Whole rows (strides of at least their length) of
- * multiples of 8 elements from 16-byte addresses, k / 2 and n multiples of 8, no batches; config and splits are the
- * library's. `workspace` of nhip_gemm_pair_workspace bytes. */
-int nhip_gemm_pair(const nhip_gemm_desc *desc, const void *a, const void *b, const void *b2, void *d, void *workspace);
-int nhip_gemm_pair_workspace(const nhip_gemm_desc *desc, size_t *bytes);
+/* dx [m, k] = dg gate + du up with one float32 sum over both, and d_gate, d_up [n, k] = dg^T x, du^T x, contiguous, each
+ * rounded once (d_up may be null: then it is not computed); sums in a fixed order. dgu is nhip_gated_linear_grad's, from a 16-byte address; x and weights of whole
+ * 16-byte rows (n, k and the strides multiples of 8) start on 16 bytes, others are copied. `workspace` of
+ * nhip_gated_backward_workspace bytes (enough for either), from a 16-byte address. Weights are below 2^31 bytes. */
+int nhip_gated_input_grad(const nhip_gated_desc *desc, const void *dgu, const void *gate, const void *up, void *dx,
+                          void *workspace);
+int nhip_gated_weight_grad(const nhip_gated_desc *desc, const void *dgu, const void *x, void *d_gate, void *d_up, void *workspace);
+int nhip_gated_backward_workspace(const nhip_gated_desc *desc, size_t *bytes);
 
 /* ---- gradient clipping (no counterpart in the reference) -------------------------------------------------------- *
  *
@@ -358,7 +361,8 @@ enum {
     NHIP_STEP_CLIP = 11,      /* desc: nhip_clip_desc, then its nhip_clip_tensors (in and out ignored); pointers: max_norm_at
                                  (or none), norm, scale (or none), workspace, then tensor i's in at 4 + 2 i and out at
                                  5 + 2 i (or none) */
-    NHIP_STEP_PAIR = 12,      /* desc: nhip_gemm_desc; pointers: a, b, b2, d, workspace (or none) */
+    NHIP_STEP_GATED_INPUT = 12,  /* desc: nhip_gated_desc; pointers: dgu, gate, up, dx, workspace (or none) */
+    NHIP_STEP_GATED_WEIGHT = 13, /* desc: nhip_gated_desc; pointers: dgu, x, d_gate, d_up, workspace (or none) */
 };
 
 int nhip_plan_create(void **plan);

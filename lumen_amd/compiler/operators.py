@@ -17,7 +17,8 @@ KINDS = {
     "qk_norm_rope_backward": "heads_bwd",
     "gated_linear": "gated_fwd",
     "gated_linear_grad": "gated_grad",
-    "gemm_pair": "pair",
+    "gated_input_grad": "gated_input",
+    "gated_weight_grad": "gated_weight",
     "clip_grad_norm": "clip",
 }
 NHIP_DT = {"float32": 0, "bfloat16": 1, "float16": 2}
@@ -34,8 +35,8 @@ def _wants(node):
         return [ROWS if r in ("q", "k", "gq", "gk") else DENSE for r in node.params["roles"]]
     if name == "gated_linear":
         return [WIDE_ROWS, WIDE, WIDE]
-    if name == "gemm_pair":
-        return [WIDE] * 3
+    if name in ("gated_input_grad", "gated_weight_grad"):
+        return [WIDE] * len(node.inputs)
     if name == "gated_linear_grad":
         return [ROWS, DENSE, DENSE]
     return [DENSE] * len(node.inputs)
@@ -97,8 +98,8 @@ def scratch_bytes(graph, node) -> int:
         nv.call("nhip_qk_norm_rope_workspace", C.byref(_heads_desc(node, _roles(graph, node))), C.byref(n))
     elif name == "gated_linear":
         nv.call("nhip_gated_linear_workspace", C.byref(_gated_node_desc(graph, node)), C.byref(n))
-    elif name == "gemm_pair":
-        nv.call("nhip_gemm_pair_workspace", C.byref(_pair_desc(graph, node)), C.byref(n))
+    elif name in ("gated_input_grad", "gated_weight_grad"):
+        nv.call("nhip_gated_backward_workspace", C.byref(_gated_backward_desc(graph, node)), C.byref(n))
     elif name == "clip_grad_norm":
         nv.call("nhip_clip_grad_norm_workspace", C.byref(nv.ClipDesc(count=len(_clip_grads(node)))), C.byref(n))
     return -(-n.value // 256) * 256
@@ -118,7 +119,8 @@ def lower(plan, step):
     name = step.nodes[0].params["name"]
     if name.startswith("qk_norm_rope"):
         return _lower_heads(plan, step)
-    return {"gated_linear": _lower_gated, "gated_linear_grad": _lower_gated_grad, "gemm_pair": _lower_pair,
+    return {"gated_linear": _lower_gated, "gated_linear_grad": _lower_gated_grad,
+            "gated_input_grad": _lower_gated_backward, "gated_weight_grad": _lower_gated_backward,
             "clip_grad_norm": _lower_clip}[name](plan, step)
 
 
@@ -177,21 +179,20 @@ def _lower_gated(plan, step):
     return nv.NHIP_STEP_GATED, bytes(d), _slots(places + [out[0], out.get(1), out.get(2), plan.scratch.get(id(step))])
 
 
-def _pair_desc(graph, node):
-    from lumen_amd import native as nv
-
-    a, b = (graph.types[v] for v in node.inputs[:2])
-    dt = NHIP_DT[a.dtype]
-    return nv.GemmDesc(m=a.shape[0], n=b.shape[1], k=a.shape[1], a_dtype=dt, b_dtype=dt, d_dtype=dt, a_m=a.shape[1], a_k=1,
-                       b_k=b.shape[1], b_n=1, d_m=b.shape[1], d_n=1, config=-1)
+def _gated_backward_desc(graph, node):
+    dgu, other = (graph.types[v] for v in node.inputs[:2])  # the gate weight [features, k], or x [tokens, k]
+    return _gated_desc(dgu.dtype, "silu", dgu.shape[0], node.params["features"], other.shape[1])
 
 
-def _lower_pair(plan, step):
+def _lower_gated_backward(plan, step):
     from lumen_amd import native as nv
 
     node = step.nodes[0]
-    return nv.NHIP_STEP_PAIR, bytes(_pair_desc(plan.graph, node)), _slots(
-        [plan.loc[v] for v in node.inputs] + [_outputs(plan, step)[0], plan.scratch.get(id(step))])
+    kind = nv.NHIP_STEP_GATED_INPUT if step.kind == "gated_input" else nv.NHIP_STEP_GATED_WEIGHT
+    out = _outputs(plan, step)
+    places = [plan.loc[v] for v in node.inputs]
+    places += [out[0], out.get(1)] if step.kind == "gated_weight" else [out[0]]
+    return kind, bytes(_gated_backward_desc(plan.graph, node)), _slots(places + [plan.scratch.get(id(step))])
 
 
 def _lower_gated_grad(plan, step):

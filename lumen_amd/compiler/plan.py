@@ -1355,9 +1355,9 @@ class Plan:
         if st.kind == "gated_fwd":
             x, w = (g.types[v] for v in st.nodes[0].inputs[:2])
             return 4 * x.numel() * w.shape[0], io
-        if st.kind == "pair":
-            a, b = (g.types[v] for v in st.nodes[0].inputs[:2])
-            return 2 * a.numel() * b.shape[1], io
+        if st.kind in ("gated_input", "gated_weight"):
+            dgu, other = (g.types[v] for v in st.nodes[0].inputs[:2])
+            return 2 * dgu.numel() * other.shape[1], io
         return 0, io
 
     def describe(self):

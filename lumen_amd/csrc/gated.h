@@ -131,12 +131,15 @@ struct GatedOut {
 
 // TM x TM / 2 tiles: 256 with 8 waves and the k loop placed by hand (with 4 waves the store's 512 registers spill: [16384, 2048] x
 // [8192, 2048] 909 us, 1140), 128 with 4 waves, two workgroups a CU.
-template <bool F16, int TM>
-__global__ __launch_bounds__(TM * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void gated_stream(
+// KL, ST: the k loop and its stages: 3 (256), 0 with two stages (128), or 1 with three (128, one workgroup a CU): where the
+// tiles leave one workgroup a CU anyway and k is long enough, its loads two tiles ahead hide their latency ([128, 2048] x [8192, 2048]
+// 27.4 -> 19.6 us, [1463, 3392] x [712, 3392] 41.2 -> 28.9; [300, 512] x [2048, 512] 7.8 -> 8.4).
+template <bool F16, int TM, int KL, int ST = 0>
+__global__ __launch_bounds__(TM * 2) __attribute__((amdgpu_waves_per_eu(ST ? 1 : 2, ST ? 1 : 2))) void gated_stream(
     GemmShape s, const uint16_t *__restrict__ x, const uint16_t *__restrict__ gate, const uint16_t *__restrict__ up,
     GatedOut out) {
     extern __shared__ __align__(1024) char smem[];
-    gemm_stream_tile<F16, 64, TM / 64, false, false, true, GatedOut, TM, TM == 256 ? 3 : 0, 1>(s, x, gate, out, smem, up);
+    gemm_stream_tile<F16, 64, TM / 64, false, false, true, GatedOut, TM, KL, 1, ST>(s, x, gate, out, smem, up);
 }
 
 // 8 elements at p of any alignment as 4-byte words, which memory reads at full width where words at 2-byte addresses take
@@ -244,47 +247,63 @@ __global__ __launch_bounds__(64 * NW) void gated_skinny(GemmShape s, const uint1
 struct GatedPad {
     const uint16_t *src[3];
     uint16_t *dst[3];
-    int64_t rows[3], ld[3], k, kp;
+    int64_t rows[3], to_rows[3], ld[3], k, kp;  // to_rows: rows written, those past `rows` zeros
 };
 static __global__ __launch_bounds__(256) void gated_pad_kernel(GatedPad a) {
     const int64_t per = a.kp / 8;
     for (int which = 0; which < 3; ++which) {
-        const int64_t total = a.rows[which] * per;
+        const int64_t total = a.to_rows[which] * per;
         for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
             const int64_t row = i / per, c = (i - row * per) * 8;
             const uint16_t *src = a.src[which] + row * a.ld[which] + c;
-            *reinterpret_cast<uint4 *>(a.dst[which] + row * a.kp + c) = a.k - c >= 8 ? load8_words(src) : load8_any(src, a.k - c);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (row < a.rows[which]) v = a.k - c >= 8 ? load8_words(src) : load8_any(src, a.k - c);
+            *reinterpret_cast<uint4 *>(a.dst[which] + row * a.kp + c) = v;
         }
     }
 }
 
-// D = A[:, :k / 2] B + A[:, k / 2:] B2 (the input's gradient: A = [dg | du], the weights as they lie): one accumulator over
-// both products, or (splits) float32 parts of the k tiles that gemm_splitk_reduce adds. Two products and their sum write
-// and read 8 m n bytes more.
+// The input's gradient: D = A[:, :k / 2] B + A[:, k / 2:] B2 with A = [dg | du] and the weights as they lie: one
+// accumulator over both products, or (parts of k) float32 sums that gemm_splitk_reduce adds. Two products and their sum write
+// and read 8 m n bytes more: [4096, 2048] of k 2 x 8192 243 us, 325.
 template <bool F16, int TM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TM == 256 ? 1 : 2, TM == 256 ? 1 : 2))) void gemm_pair(
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TM == 256 ? 1 : 2, TM == 256 ? 1 : 2))) void gated_input_grad(
     GemmShape s, const uint16_t *__restrict__ a, const uint16_t *__restrict__ b, const uint16_t *__restrict__ b2, AnyStore out,
     int k_part) {
     extern __shared__ __align__(1024) char smem[];
     gemm_stream_tile<F16, 64, 2, false, true, true, AnyStore, TM, TM == 256 ? 3 : 0, 2>(s, a, b, out, smem, b2, k_part);
 }
 
-// [dg | du] of 8 elements a thread (V 8: n, the strides and the pointers multiples of 16 bytes) or of one (V 1).
+// The weights' gradients: D_i = A_i^T X for the two halves of A = [dg | du], one batch each, over tokens of any number.
+template <bool F16, int TM>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TM == 256 ? 1 : 2, TM == 256 ? 1 : 2))) void gated_weight_grad(
+    GemmShape s, const uint16_t *__restrict__ a, const uint16_t *__restrict__ b, const uint16_t *, AnyStore out, int k_part) {
+    extern __shared__ __align__(1024) char smem[];
+    gemm_stream_tile<F16, 64, 2, true, true, true, AnyStore, TM, TM == 256 ? 3 : 0, 3>(s, a, b, out, smem, nullptr, k_part);
+}
+
+// [dg | du] of 8 elements a thread (V 8: n, the strides and the pointers multiples of 16 bytes) or of one (V 1). Each half
+// of a row has np elements, n rounded up to 8, the last ones zeros: the products read whole chunks.
 struct GatedGrad {
     const void *dh;
     const float *g, *u;
-    void *out;  // [m, 2 n]
-    int64_t m, n, dh_m;
+    void *out;  // [m, 2 np]
+    int64_t m, n, np, dh_m;
     int32_t act;
 };
 template <typename T, int V>
 __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGrad a) {
-    const int64_t per = a.n / V, total = a.m * per;
+    const int64_t per = a.np / V, total = a.m * per;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
         const int64_t row = i / per, col = (i - row * per) * V;
         const T *dh = static_cast<const T *>(a.dh) + row * a.dh_m + col;
         const float *g = a.g + row * a.n + col, *u = a.u + row * a.n + col;
-        T *out = static_cast<T *>(a.out) + row * 2 * a.n + col;
+        T *out = static_cast<T *>(a.out) + row * 2 * a.np + col;
+        if (V == 1 && col >= a.n) {
+            store_f32_as(out, 0.0f);
+            store_f32_as(out + a.np, 0.0f);
+            continue;
+        }
         float d[V], gv[V], uv[V];
         if constexpr (V == 8) {
             const uint4 r = *reinterpret_cast<const uint4 *>(dh);
@@ -316,10 +335,10 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGrad a) {
             __builtin_memcpy(&p, dg, 16);
             __builtin_memcpy(&q, du, 16);
             *reinterpret_cast<uint4 *>(out) = p;
-            *reinterpret_cast<uint4 *>(out + a.n) = q;
+            *reinterpret_cast<uint4 *>(out + a.np) = q;
         } else {
             out[0] = dg[0];
-            out[a.n] = du[0];
+            out[a.np] = du[0];
         }
     }
 }

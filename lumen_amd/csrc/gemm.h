@@ -377,9 +377,9 @@ constexpr int gemm_stream_stages() { return TM == 256 ? (128 * 1024) / (2 * 256 
 template <int WN, int TM = 256>
 constexpr int gemm_stream_stage_pitch() { return (TM / WN) * 4 + 16; }
 // LDS: the operand stages, or the epilogue's staging (float32 rows), whichever is larger.
-template <int BK, int WN, int TM = 256>
+template <int BK, int WN, int TM = 256, int ST = 0>
 constexpr int gemm_stream_lds_bytes() {
-    constexpr int ops = gemm_stream_stages<BK, TM>() * 2 * TM * BK * 2;
+    constexpr int ops = (ST ? ST : gemm_stream_stages<BK, TM>()) * 2 * TM * BK * 2;
     constexpr int epi = 2 * WN * 64 * gemm_stream_stage_pitch<WN, TM>();
     return ops > epi ? ops : epi;
 }
@@ -482,11 +482,14 @@ __device__ __forceinline__ int stream_line(int wn, int j) {
 // KL, the k loop: 0 fragments of the next k step read under the current step's MFMAs; 1 (XPF) that read also
 // across k tiles; 2 (ping-pong) the two waves of each SIMD alternate between a memory phase and an MFMA phase;
 // 3 (k tile 64, two stages, four waves) the cross-tile read placed by hand with the loads split in halves.
+// ST: the stages in LDS (0: gemm_stream_stages).
 // PAIR 1: two products of A, by B and by b2 of the same shape and strides: half of the tile's columns are B's, half the
 // same columns of b2, and out.store takes the pairs of sums. PAIR 2: the sum of two products, A's first k / 2 columns by b
-// and the others by b2, part blockIdx.z of it over k_part of the k tiles. k (k / 2) is a multiple of 8 there, and operands
-// are within the buffers' reach.
-template <bool F16, int BK, int WN, bool AT, bool BT, bool BUF, class Out, int TM = 256, int KL = 0, int PAIR = 0>
+// and the others by b2, part blockIdx.z of it over k_part of the k tiles. k (k / 2) is a multiple of 8 there. PAIR 3:
+// one product of operands contiguous along m and n, k of any size, in parts like PAIR 2. Rows along n (and m) hold whole
+// chunks of 8 elements whatever n is. Operands are within the buffers'
+// reach.
+template <bool F16, int BK, int WN, bool AT, bool BT, bool BUF, class Out, int TM = 256, int KL = 0, int PAIR = 0, int ST = 0>
 __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint16_t *__restrict__ a,
                                                  const uint16_t *__restrict__ b, const Out &out, char *smem,
                                                  const uint16_t *__restrict__ b2 = nullptr, int k_part = 0) {
@@ -495,7 +498,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     constexpr int FM = WR / 32;      // 32-row MFMA tiles a wave
     constexpr int WCOLS = TM / WN;   // columns a wave
     constexpr int FN = WCOLS / 32;   // 32-column MFMA tiles a wave
-    constexpr int STAGES = gemm_stream_stages<BK, TM>();
+    constexpr int STAGES = ST ? ST : gemm_stream_stages<BK, TM>();
     using TA = StreamTile<BK, AT, TM>;
     using TB = StreamTile<BK, BT, TM>;
     constexpr int STAGE_BYTES = TA::bytes + TB::bytes;
@@ -506,7 +509,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     tile_of(blockIdx.x, s.tiles_m, s.tiles_n, tm, tn);
     int64_t oa, ob, od;
     batch_offsets(s, blockIdx.y, oa, ob, od);
-    static_assert(PAIR == 0 || (BUF && !AT && BT == (PAIR == 2) && FN % 2 == 0), "the pairs' layouts");
+    static_assert(PAIR == 0 || (BUF && AT == (PAIR == 3) && BT == (PAIR >= 2) && FN % 2 == 0), "the pairs' layouts");
     constexpr int TNB = PAIR == 1 ? TM / 2 : TM;  // columns of one B operand in the tile
     const int64_t m0 = int64_t(tm) * TM, n0 = int64_t(tn) * TNB;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -516,29 +519,35 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     const int wave_u = WN == 2 ? __builtin_amdgcn_readfirstlane(wave) : wave;
     const int64_t ks = PAIR == 0 ? int64_t(blockIdx.z) * s.k : 0;  // split-k: this workgroup's first k
     od += int64_t(blockIdx.z) * s.d_split;
-    const uint16_t *pa = a + oa + ks * s.a_k, *pb = b + ob + ks * s.b_k;
+    // PAIR 2 and 3: the part's first k tile; PAIR 3: the operands from its first k on
+    const int kfirst = PAIR >= 2 ? int(blockIdx.z) * k_part : 0;
+    const int64_t kp = PAIR == 3 ? int64_t(kfirst) * BK : ks;
+    const uint16_t *pa = a + oa + kp * s.a_k, *pb = b + ob + kp * s.b_k;
     const int64_t kb = PAIR == 2 ? s.k / 2 : s.k;  // k of one B operand
-    // PAIR: k tiles of one operand, the last of them perhaps in part; part blockIdx.z takes k_part of all of them
-    const int kth = int((kb + BK - 1) / BK), kfirst = PAIR == 2 ? int(blockIdx.z) * k_part : 0;
-    const int ktiles = PAIR == 0 ? int(s.k / BK) : PAIR == 1 ? kth : min(k_part, 2 * kth - kfirst);
-    (void)kth, (void)kfirst;
+    // PAIR: k tiles of one operand, the last of them perhaps in part; a part takes k_part of all of them
+    const int kth = int((kb + BK - 1) / BK);
+    const int ktiles = PAIR == 0 ? int(s.k / BK) : PAIR == 1 ? kth : min(k_part, (PAIR == 2 ? 2 * kth : kth) - kfirst);
+    const int64_t krows = PAIR == 3 ? min(s.k - kp, int64_t(k_part) * BK) : kb;
+    (void)kth, (void)kfirst, (void)krows;
 
     // issues this wave's loads [lo, hi) of tile kt into stage st (A segments first, then B)
     // Buffer resources over this tile's rows of A and B (columns when mn-contiguous): the loads then take a
     // per-lane 32-bit offset fixed for the whole k loop plus a uniform k offset, with no per-load address
     // arithmetic, and rows past m / n read zeros. Operands whose tile span exceeds 2^31 bytes use 64-bit
     // global addresses instead.
-    const int64_t mrem = s.m - m0 < TM ? s.m - m0 : TM, nrem = s.n - n0 < TNB ? s.n - n0 : TNB;
-    const int64_t abytes = AT ? ((s.k - 1) * s.a_k + mrem) * 2 : ((mrem - 1) * s.a_m + s.k) * 2;
+    int64_t mrem = s.m - m0 < TM ? s.m - m0 : TM, nrem = s.n - n0 < TNB ? s.n - n0 : TNB;
+    if constexpr (PAIR >= 2) nrem = (nrem + 7) & ~int64_t(7);  // rows along n (and m) hold whole chunks
+    if constexpr (PAIR == 3) mrem = (mrem + 7) & ~int64_t(7);
+    const int64_t abytes = PAIR == 3 ? ((krows - 1) * s.a_k + mrem) * 2 : AT ? ((s.k - 1) * s.a_k + mrem) * 2 : ((mrem - 1) * s.a_m + s.k) * 2;
     const int64_t bbytes = PAIR == 0 ? (BT ? ((s.k - 1) * s.b_k + nrem) * 2 : ((nrem - 1) * s.b_n + s.k) * 2)
-                                     : (BT ? ((kb - 1) * s.b_k + nrem) * 2 : ((nrem - 1) * s.b_n + kb) * 2);
+                                     : (BT ? ((krows - 1) * s.b_k + nrem) * 2 : ((nrem - 1) * s.b_n + kb) * 2);
     constexpr bool buf = BUF;  // the launcher checked stream_buffer_ok()
     const __amdgpu_buffer_rsrc_t rsa = __builtin_amdgcn_make_buffer_rsrc(
         (void *)(AT ? pa + m0 : pa + m0 * s.a_m), (short)0, int(abytes), 0x00020000);
     const __amdgpu_buffer_rsrc_t rsb = __builtin_amdgcn_make_buffer_rsrc(
         (void *)(BT ? pb + n0 : pb + n0 * s.b_n), (short)0, int(bbytes), 0x00020000);
     const __amdgpu_buffer_rsrc_t rsb2 = __builtin_amdgcn_make_buffer_rsrc(
-        (void *)(PAIR == 0 ? b2 : BT ? b2 + n0 : b2 + n0 * s.b_n), (short)0, int(PAIR == 0 ? 0 : bbytes), 0x00020000);
+        (void *)(PAIR == 0 || PAIR == 3 ? b2 : BT ? b2 + n0 : b2 + n0 * s.b_n), (short)0, int(PAIR == 0 || PAIR == 3 ? 0 : bbytes), 0x00020000);
     (void)rsb2;
     auto issue = [&](int st, int kt, int lo, int hi) {
         char *base = smem + st * STAGE_BYTES;
@@ -555,8 +564,9 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
             const int line = seg * TA::lines_per_seg + lane / TA::chunks, c = lane % TA::chunks;
             if constexpr (PAIR != 0) {
                 const int kc = (c ^ kmaj_swz<BK>(line)) << 3;
-                const uint32_t vo = k1 + kc < kb ? uint32_t((line * s.a_m + kc) * 2) : 0x80000000u;
-                const uint32_t so = uint32_t((k1 + (second ? kb : 0)) * 2);
+                const uint32_t vo = AT ? uint32_t((line * s.a_k + ((c ^ mnmaj_swz(line)) << 3)) * 2)
+                                       : k1 + kc < kb ? uint32_t((line * s.a_m + kc) * 2) : 0x80000000u;
+                const uint32_t so = AT ? uint32_t(k0 * s.a_k * 2) : uint32_t((k1 + (second ? kb : 0)) * 2);
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rsa, (glds_void_t *)(base + seg * 1024), 16, vo, so, 0, 0);
                 continue;
             }

@@ -10,7 +10,7 @@
 // Nothing but x is kept from the forward: inv costs the backward no read that it does not make anyway.
 //
 // HBM bounds both: a row is read once and written once (the backward reads x and dy), everything between in float32.
-// A lane holds both elements of its pairs, 2 E of them in two 16-byte (or 8-byte) chunks, so the turn needs no
+// A lane holds both elements of its pairs, 2 E of them in two chunks of 16 (8, 4) bytes, so the turn needs no
 // exchange and the row sums are the only ones, over the D / (2 E) lanes of a row. A workgroup takes consecutive heads,
 // so its reads are contiguous; the table's rows come from L1.
 #pragma once
@@ -56,6 +56,12 @@ struct HeadsChunk<float, 4> {
     __device__ __forceinline__ static void get(const raw &r, float (&v)[4]) { v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w; }
     __device__ __forceinline__ static raw put(const float (&v)[4]) { return make_float4(v[0], v[1], v[2], v[3]); }
 };
+template <>
+struct HeadsChunk<float, 2> {
+    typedef float2 raw;
+    __device__ __forceinline__ static void get(const raw &r, float (&v)[2]) { v[0] = r.x, v[1] = r.y; }
+    __device__ __forceinline__ static raw put(const float (&v)[2]) { return make_float2(v[0], v[1]); }
+};
 __device__ __forceinline__ float heads_up(bf16_t, uint32_t bits) { return bf16_to_f32(uint16_t(bits)); }
 __device__ __forceinline__ float heads_up(f16_t, uint32_t bits) { return f16_to_f32(uint16_t(bits)); }
 __device__ __forceinline__ uint32_t heads_down(bf16_t, float v) { return f32_to_bf16(v); }
@@ -85,6 +91,13 @@ struct HeadsChunk<T, 4> {
     __device__ __forceinline__ static raw put(const float (&v)[4]) {
         return make_uint2(heads_down(T{}, v[0]) | heads_down(T{}, v[1]) << 16, heads_down(T{}, v[2]) | heads_down(T{}, v[3]) << 16);
     }
+};
+
+template <typename T>
+struct HeadsChunk<T, 2> {
+    typedef uint32_t raw;
+    __device__ __forceinline__ static void get(const raw &r, float (&v)[2]) { v[0] = heads_up(T{}, r & 0xffff), v[1] = heads_up(T{}, r >> 16); }
+    __device__ __forceinline__ static raw put(const float (&v)[2]) { return heads_down(T{}, v[0]) | heads_down(T{}, v[1]) << 16; }
 };
 
 // Where a lane's two chunks lie in a row, and its first pair: pairs[e] couples chunk 0's element e with chunk 1's, or
@@ -163,10 +176,15 @@ __device__ __forceinline__ HeadsRow heads_row(const HeadsArgs &a, const HeadsTen
 
 template <int E>
 __device__ __forceinline__ void heads_table(const float *p, float (&v)[E]) {
+    if constexpr (E == 2) {
+        const float2 q = *reinterpret_cast<const float2 *>(p);
+        v[0] = q.x, v[1] = q.y;
+    } else {
 #pragma unroll
-    for (int i = 0; i < E; i += 4) {
-        const float4 q = *reinterpret_cast<const float4 *>(p + i);
-        v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
+        for (int i = 0; i < E; i += 4) {
+            const float4 q = *reinterpret_cast<const float4 *>(p + i);
+            v[i] = q.x, v[i + 1] = q.y, v[i + 2] = q.z, v[i + 3] = q.w;
+        }
     }
 }
 

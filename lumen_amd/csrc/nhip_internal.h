@@ -33,7 +33,10 @@ int heads_bwd_on(hipStream_t s, const nhip_heads_desc *d, const void *q, const v
                  void *dqw, void *dkw, void *ws);
 int gated_on(hipStream_t s, const nhip_gated_desc *d, const void *x, const void *gate, const void *up, void *h, float *g,
              float *u, void *ws);
-int pair_on(hipStream_t s, const nhip_gemm_desc *d, const void *a, const void *b, const void *b2, void *out, void *ws);
+int gated_input_grad_on(hipStream_t s, const nhip_gated_desc *d, const void *dgu, const void *gate, const void *up, void *dx,
+                        void *ws);
+int gated_weight_grad_on(hipStream_t s, const nhip_gated_desc *d, const void *dgu, const void *x, void *dgate, void *dup,
+                         void *ws);
 int gated_grad_on(hipStream_t s, const nhip_gated_desc *d, const void *dh, const float *g, const float *u, void *dgu);
 int clip_on(hipStream_t s, const nhip_clip_desc *d, const nhip_clip_tensor *t, const double *max_at, float *norm,
             float *scale, void *ws);

@@ -71,12 +71,12 @@ HeadsPlan heads_plan(const nhip_heads_desc *d, bool bwd, std::initializer_list<c
     const int64_t tokens = d->batch * d->seq, each = heads_tokens(d);
     p.launches = each ? (tokens + each - 1) / each : 0;
     p.e = 0;
-    for (int e : {8, 4}) {
+    for (int e : {8, 4, 2}) {
         if (e == 8 && d->dtype == NHIP_F32) continue;  // 4 elements are 16 bytes
         const size_t bytes = size_t(e) * (d->dtype == NHIP_F32 ? 4 : 2);
         bool ok = d->head_dim % (2 * e) == 0 && d->rot % (2 * e) == 0 && d->head_dim / (2 * e) <= 64 && heads_strides(d, e, bwd);
         for (const void *h : heads) ok = ok && on(h, bytes);
-        ok = ok && on(cos, 16) && on(sin, 16);
+        ok = ok && on(cos, e == 2 ? 8 : 16) && on(sin, e == 2 ? 8 : 16);
         if (ok) {
             p.e = e;
             break;
@@ -98,8 +98,8 @@ HeadsBlocks heads_blocks(const nhip_heads_desc *d, int lanes, int64_t cap) {
     auto share = [&](int64_t rows) -> int64_t {
         if (rows == 0) return 0;
         const int64_t need = (rows + groups - 1) / groups, part = 256 * rows / (q + k) + 1;
-        const int64_t want = need / 4 > part ? need / 4 : (need < part ? need : part), most = cap * rows / (q + k) + 1;
-        return want < most ? want : most;
+        const int64_t want = need / 4 > part ? need / 4 : (need < part ? need : part), most = cap * rows / (q + k);  // both within the cap: one workgroup over it is a round
+        return want < most ? want : most > 0 ? most : 1;
     };
     return {share(q), share(k)};
 }
@@ -126,6 +126,7 @@ int heads_launch(hipStream_t st, HeadsArgs &a, int e, bool bwd) {
         if constexpr (!std::is_same<T, float>::value)
             if (e == 8) return heads_launch_fwd<T, 8>(st, a);
         if (e == 4) return heads_launch_fwd<T, 4>(st, a);
+        if (e == 2) return heads_launch_fwd<T, 2>(st, a);
         for (HeadsTensor &t : a.t) {
             const int64_t blocks = (int64_t(t.rows) * a.lanes + 255) / 256;
             t.blocks = uint32_t(blocks < 16384 ? blocks : 16384);
@@ -144,6 +145,7 @@ int heads_launch(hipStream_t st, HeadsArgs &a, int e, bool bwd) {
         }
     }
     if (e == 4) hipLaunchKernelGGL((heads_bwd_kernel<T, 4>), dim3(grid), dim3(256), 0, st, a);
+    else if (e == 2) hipLaunchKernelGGL((heads_bwd_kernel<T, 2>), dim3(grid), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((heads_any_kernel<T, true>), dim3(grid), dim3(256), 0, st, a);
     return check(hipGetLastError(), "heads_bwd_kernel launch");
 }
@@ -233,7 +235,7 @@ int heads_bwd_on(hipStream_t st, const nhip_heads_desc *d, const void *q, const 
 
 namespace {
 
-enum { kSkinnyCfg = 0, kStream256, kStream128Cfg, kGatedConfigs };
+enum { kSkinnyCfg = 0, kStream256, kStream128Cfg, kDeepCfg, kGatedConfigs };
 
 int gated_check(const nhip_gated_desc *d, const char *what) {
     const std::string at(what);
@@ -249,7 +251,9 @@ bool gated_skinny_ok(const nhip_gated_desc *d) { return d->m <= 64 && d->k < (in
 
 int gated_default(const nhip_gated_desc *d) {
     if (gated_skinny_ok(d)) return kSkinnyCfg;
-    return tiles(d->m, 256, d->n, 128) >= 256 ? kStream256 : kStream128Cfg;
+    if (tiles(d->m, 256, d->n, 128) >= 256) return kStream256;
+    // one workgroup a CU: 6.5 us and 0.0080 a k with three stages, 4 and 0.0115 with two
+    return tiles(d->m, 128, d->n, 64) <= 256 && d->k >= 768 ? kDeepCfg : kStream128Cfg;
 }
 
 // Whether gated_stream can read rows of these lengths and distances in place (from 16-byte addresses).
@@ -279,6 +283,25 @@ int gated_go(hipStream_t st, K kern, GemmShape s, int bm, int bn, int threads, i
     return check(hipGetLastError(), "gated kernel launch");
 }
 
+// Copies `count` matrices of rows of k elements to whole rows of 16-byte chunks at ws, one after the other.
+int gated_pad(hipStream_t st, GatedPad &p, int count, const void *const *src, const int64_t *rows, const int64_t *to_rows,
+              const int64_t *ld, int64_t k, void *ws) {
+    std::memset(&p, 0, sizeof(p));
+    p.k = k, p.kp = (k + 7) / 8 * 8;
+    uint16_t *to = static_cast<uint16_t *>(ws);
+    int64_t most = 1;
+    for (int i = 0; i < count; ++i) {
+        p.src[i] = static_cast<const uint16_t *>(src[i]);
+        p.rows[i] = rows[i], p.to_rows[i] = to_rows[i], p.ld[i] = ld[i];
+        p.dst[i] = to;
+        to += to_rows[i] * p.kp;
+        if (to_rows[i] > most) most = to_rows[i];
+    }
+    const int64_t blocks = (most * (p.kp / 8) + 255) / 256;
+    hipLaunchKernelGGL(gated_pad_kernel, dim3(unsigned(blocks < 4096 ? (blocks ? blocks : 1) : 4096)), dim3(256), 0, st, p);
+    return check(hipGetLastError(), "gated_pad_kernel launch");
+}
+
 template <bool F16, bool ANY>
 int gated_few(hipStream_t st, const GemmShape &s, const void *x, const void *gate, const void *up, const GatedOut &o) {
     if (s.m <= 16) return gated_go(st, gated_skinny<F16, 1, 8, ANY>, s, 64, 16, 512, 0, x, gate, up, o);
@@ -292,24 +315,17 @@ int gated_run(hipStream_t st, int cfg, GemmShape s, const void *x, const void *g
     if (cfg == kSkinnyCfg) return in_place ? gated_few<F16, false>(st, s, x, gate, up, o) : gated_few<F16, true>(st, s, x, gate, up, o);
     if (!in_place) {
         GatedPad p;
-        p.k = s.k, p.kp = (s.k + 7) / 8 * 8;
+        const int64_t rows[3] = {s.m, s.n, s.n}, ld[3] = {s.a_m, s.b_n, s.b_n};
         const void *src[3] = {x, gate, up};
-        uint16_t *to = static_cast<uint16_t *>(ws);
-        for (int i = 0; i < 3; ++i) {
-            p.src[i] = static_cast<const uint16_t *>(src[i]);
-            p.rows[i] = i ? s.n : s.m, p.ld[i] = i ? s.b_n : s.a_m;
-            p.dst[i] = to;
-            to += p.rows[i] * p.kp;
-        }
-        const int64_t blocks = ((s.m > s.n ? s.m : s.n) * (p.kp / 8) + 255) / 256;
-        hipLaunchKernelGGL(gated_pad_kernel, dim3(unsigned(blocks < 4096 ? (blocks ? blocks : 1) : 4096)), dim3(256), 0, st, p);
-        if (check(hipGetLastError(), "gated_pad_kernel launch")) return 1;
+        if (gated_pad(st, p, 3, src, rows, rows, ld, s.k, ws)) return 1;
         x = p.dst[0], gate = p.dst[1], up = p.dst[2];
         s.k = s.a_m = s.b_n = p.kp;
     }
     if (cfg == kStream256)
-        return gated_go(st, gated_stream<F16, 256>, s, 256, 128, 512, gemm_stream_lds_bytes<64, 4>(), x, gate, up, o);
-    return gated_go(st, gated_stream<F16, 128>, s, 128, 64, 256, gemm_stream_lds_bytes<64, 2, 128>(), x, gate, up, o);
+        return gated_go(st, gated_stream<F16, 256, 3>, s, 256, 128, 512, gemm_stream_lds_bytes<64, 4>(), x, gate, up, o);
+    if (cfg == kDeepCfg)
+        return gated_go(st, gated_stream<F16, 128, 1, 3>, s, 128, 64, 256, gemm_stream_lds_bytes<64, 2, 128, 3>(), x, gate, up, o);
+    return gated_go(st, gated_stream<F16, 128, 0>, s, 128, 64, 256, gemm_stream_lds_bytes<64, 2, 128>(), x, gate, up, o);
 }
 
 }  // namespace
@@ -340,9 +356,10 @@ int gated_on(hipStream_t st, const nhip_gated_desc *d, const void *x, const void
 int gated_grad_on(hipStream_t st, const nhip_gated_desc *d, const void *dh, const float *g, const float *u, void *dgu) {
     if (gated_check(d, "nhip_gated_linear_grad")) return 1;
     if (d->m == 0 || d->n == 0) return 0;
-    GatedGrad a{dh, g, u, dgu, d->m, d->n, d->h_m, d->activation};
+    const int64_t np = (d->n + 7) / 8 * 8;
+    GatedGrad a{dh, g, u, dgu, d->m, d->n, np, d->h_m, d->activation};
     const bool vec = d->n % 8 == 0 && d->h_m % 8 == 0 && on(dh, 16) && on(g, 16) && on(u, 16) && on(dgu, 16);
-    const int64_t work = d->m * (vec ? d->n / 8 : d->n), blocks = (work + 255) / 256;
+    const int64_t work = d->m * (vec ? np / 8 : np), blocks = (work + 255) / 256;
     const dim3 grid(unsigned(blocks < 8192 ? blocks : 8192));
     if (d->dtype == NHIP_F16) {
         if (vec) hipLaunchKernelGGL((gated_grad_kernel<f16_t, 8>), grid, dim3(256), 0, st, a);
@@ -356,95 +373,165 @@ int gated_grad_on(hipStream_t st, const nhip_gated_desc *d, const void *dh, cons
 
 namespace {
 
-// The tile and the parts of a pair's k: as many parts as make the tiles' rounds on the chip the shortest, each round as
-// long as its k, the parts' writing and reading added. The rates are the split dots' (Plan._split_us), whose loops these are.
-struct PairPlan {
-    int tm, splits, k_part;
+// The tile and the parts of a product of z batches over `total` k tiles of 64: as many parts as make the tiles' rounds on the
+// chip the shortest, each round as long as its k, the parts' writing and reading added. The rates are the split dots'
+// (Plan._split_us), whose loops these are. longest: k tiles that a part may have at most.
+struct PartPlan {
+    int tm, parts, k_part;
 };
-PairPlan pair_plan(const nhip_gemm_desc *d) {
-    const int half = int((d->k / 2 + 63) / 64), total = 2 * half;
-    PairPlan best{128, 1, total};
+PartPlan part_plan(int64_t m, int64_t n, int64_t z, int64_t total, int64_t longest) {
+    PartPlan best{0, 0, 0};
     double least = 0;
+    if (total < 1) total = 1;  // no tokens: nothing is launched, the workspace is asked for all the same
     for (int tm : {256, 128})
-        for (int s : {1, 2, 4, 8}) {
-            if (s > 1 && (total / s < 8 || int64_t(s) * d->m * d->n * 4 > (int64_t(64) << 20))) continue;
-            const int part = (total + s - 1) / s, parts = (total + part - 1) / part;
-            const double t = double(tiles(d->m, tm, d->n, tm)) * parts;
+        for (int s = 1; s <= 64; s *= 2) {
+            const int64_t part = (total + s - 1) / s, parts = (total + part - 1) / part;
+            if (part > longest) continue;
+            if (best.tm && parts > 1 && (part < 8 || parts * z * m * n * 4 > (int64_t(64) << 20))) continue;
+            const int64_t t = tiles(m, tm, n, tm) * z * parts;
             // 256: a workgroup a CU; 128: two, one alone taking 0.79 of a round of both
-            double rounds = tm == 256 ? double((int64_t(t) + 255) / 256) : double(int64_t(t) / 512);
-            const int64_t rest = int64_t(t) % 512;
+            double rounds = tm == 256 ? double((t + 255) / 256) : double(t / 512);
+            const int64_t rest = t % 512;
             if (tm == 128) rounds += rest == 0 ? 0.0 : rest <= 256 ? 0.79 : 1.0;
-            const double us = 6.2 + 64.0 * part * (tm == 256 ? 0.02355 : 0.0142) * rounds +
-                              (parts > 1 ? 4.2 + 8.0 * parts * double(d->m) * double(d->n) / 6.13e6 : 0.0);
-            if (least == 0 || us < least) least = us, best = PairPlan{tm, parts, part};
+            const double us = 6.2 + 64.0 * double(part) * (tm == 256 ? 0.02355 : 0.0142) * rounds +
+                              (parts > 1 ? 4.2 + 8.0 * double(parts) * double(z * m) * double(n) / 6.13e6 : 0.0);
+            if (least == 0 || us < least) least = us, best = PartPlan{tm, int(parts), int(part)};
         }
     return best;
 }
 
-size_t pair_workspace(const nhip_gemm_desc *d) {
-    const PairPlan p = pair_plan(d);
-    return p.splits > 1 ? size_t(p.splits) * size_t(d->m) * size_t(d->n) * 4 : 0;
+int64_t whole(int64_t n) { return (n + 7) / 8 * 8; }  // rounded up to 16 bytes of elements
+
+// The input's gradient, [m, k] of [dg | du] [m, 2 whole(n)] and the weights [n, k].
+PartPlan input_grad_plan(const nhip_gated_desc *d) { return part_plan(d->m, d->k, 1, 2 * ((whole(d->n) + 63) / 64), int64_t(1) << 30); }
+
+// The weights' gradients, [n, k] each: a part's rows of [dg | du] and of x lie within 2^31 bytes.
+PartPlan weight_grad_plan(const nhip_gated_desc *d) {
+    const int64_t row = 2 * whole(d->n) > whole(d->x_m) ? 2 * whole(d->n) : whole(d->x_m);
+    return part_plan(d->n, d->k, 2, (d->m + 63) / 64, ((int64_t(1) << 30) - 1024) / (64 * (row > 0 ? row : 1)));
 }
 
-int pair_check(const nhip_gemm_desc *d) {
-    if (d->m < 0 || d->n < 0 || d->k < 0) return fail("nhip_gemm_pair: negative sizes");
-    if (d->a_dtype != d->b_dtype || (d->a_dtype != NHIP_BF16 && d->a_dtype != NHIP_F16)) return fail("nhip_gemm_pair: bf16 or f16");
-    if (d->nbatch || d->a_k != 1 || d->b_n != 1 || d->k % 16 || d->n % 8 || d->a_m % 8 || d->b_k % 8 || d->a_m < d->k || d->b_k < d->n)
-        return fail("nhip_gemm_pair: no batches, A along k and B along n in whole rows, both halves of k and n multiples of 8");
-    const int64_t lim = int64_t(1) << 31;
-    if ((255 * d->a_m + d->k) * 2 >= lim || (d->k / 2 * d->b_k + 256) * 2 >= lim || d->k >= lim)
-        return fail("nhip_gemm_pair: an operand's tile spans 2^31 bytes");
+bool weights_whole(const nhip_gated_desc *d) { return d->n % 8 == 0 && d->k % 8 == 0 && d->w_n % 8 == 0; }
+bool input_whole(const nhip_gated_desc *d) { return d->k % 8 == 0 && d->x_m % 8 == 0; }
+
+int backward_check(const nhip_gated_desc *d, const char *what) {
+    if (gated_check(d, what)) return 1;
+    if (d->n >= (int64_t(1) << 21) || whole(d->n) * (d->w_n > whole(d->k) ? d->w_n : whole(d->k)) >= (int64_t(1) << 30) - 1024 ||
+        weight_grad_plan(d).tm == 0)
+        return fail(std::string(what) + ": weights or rows of 2^31 bytes");
     return 0;
 }
 
-template <bool F16, int TM>
-int pair_go(hipStream_t st, GemmShape s, const PairPlan &p, const void *a, const void *b, const void *b2, const AnyStore &out) {
-    s.tiles_m = int((s.m + TM - 1) / TM);
-    s.tiles_n = int((s.n + TM - 1) / TM);
-    if (tiles(s.m, TM, s.n, TM) > 0x7fffffff) return fail("nhip_gemm_pair: too many tiles");
-    constexpr int lds = gemm_stream_lds_bytes<64, 2, TM>();
-    auto kern = gemm_pair<F16, TM>;
+size_t input_grad_pad(const nhip_gated_desc *d) {
+    return weights_whole(d) ? 0 : size_t(2 * whole(d->n)) * size_t(whole(d->k)) * 2;
+}
+size_t weight_grad_pad(const nhip_gated_desc *d) { return input_whole(d) ? 0 : size_t(d->m) * size_t(whole(d->k)) * 2; }
+size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+
+size_t backward_workspace(const nhip_gated_desc *d) {
+    const PartPlan i = input_grad_plan(d), w = weight_grad_plan(d);
+    const size_t a = up16(input_grad_pad(d)) + (i.parts > 1 ? size_t(i.parts) * size_t(d->m) * size_t(d->k) * 4 : 0);
+    const size_t b = up16(weight_grad_pad(d)) + (w.parts > 1 ? size_t(w.parts) * 2 * size_t(d->n) * size_t(d->k) * 4 : 0);
+    return a > b ? a : b;
+}
+
+template <class K>
+int part_go(hipStream_t st, K kern, GemmShape s, int tm, int64_t z, const PartPlan &p, int lds, const void *a, const void *b,
+            const void *b2, const AnyStore &to, void *ws) {
+    s.tiles_m = int((s.m + tm - 1) / tm);
+    s.tiles_n = int((s.n + tm - 1) / tm);
+    if (tiles(s.m, tm, s.n, tm) > 0x7fffffff) return fail("nhip_gated_linear_grad: too many tiles");
+    GemmShape parts = s;
+    AnyStore first = to;
+    if (p.parts > 1) {
+        parts.d_m = s.n, parts.d_n = 1, parts.d_batch[0] = s.m * s.n, parts.d_split = z * s.m * s.n;
+        first = AnyStore{ws, 0};
+    }
     if (check(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
               "hipFuncSetAttribute"))
         return 1;
-    hipLaunchKernelGGL(kern, dim3(unsigned(s.tiles_m * s.tiles_n), 1, unsigned(p.splits)), dim3(256), lds, st, s,
-                       static_cast<const uint16_t *>(a), static_cast<const uint16_t *>(b), static_cast<const uint16_t *>(b2), out,
+    hipLaunchKernelGGL(kern, dim3(unsigned(s.tiles_m * s.tiles_n), unsigned(z), unsigned(p.parts)), dim3(256), lds, st, parts,
+                       static_cast<const uint16_t *>(a), static_cast<const uint16_t *>(b), static_cast<const uint16_t *>(b2), first,
                        p.k_part);
-    return check(hipGetLastError(), "gemm_pair launch");
+    const int rc = check(hipGetLastError(), "gated backward launch");
+    if (rc || p.parts == 1) return rc;
+    const int64_t total = z * s.m * s.n, blocks = (total + 255) / 256;
+    hipLaunchKernelGGL(gemm_splitk_reduce, dim3(unsigned(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, s,
+                       static_cast<const float *>(ws), p.parts, total, to);
+    return check(hipGetLastError(), "gemm_splitk_reduce launch");
 }
+
+// A result of no terms.
+int zero_grad(hipStream_t st, void *out, int64_t elements) { return fill_on(st, out, size_t(elements) * 2, 0); }
 
 }  // namespace
 
-int pair_on(hipStream_t st, const nhip_gemm_desc *d, const void *a, const void *b, const void *b2, void *out, void *ws) {
-    if (pair_check(d)) return 1;
-    if (d->m == 0 || d->n == 0) return 0;
-    if (!on(a, 16) || !on(b, 16) || !on(b2, 16)) return fail("nhip_gemm_pair: operands start on 16 bytes");
+int gated_input_grad_on(hipStream_t st, const nhip_gated_desc *d, const void *dgu, const void *gate, const void *up, void *dx,
+                        void *ws) {
+    if (backward_check(d, "nhip_gated_input_grad")) return 1;
+    if (d->m == 0 || d->k == 0) return 0;
+    if (d->n == 0) return zero_grad(st, dx, d->m * d->k);
+    const PartPlan p = input_grad_plan(d);
+    if (!ws && (p.parts > 1 || !weights_whole(d))) return fail("nhip_gated_input_grad: no workspace");
+    if (!on(dgu, 16) || !on(ws, 16)) return fail("nhip_gated_input_grad: [dg | du] and the workspace start on 16 bytes");
     GemmShape s;
     std::memset(&s, 0, sizeof(s));
-    s.m = d->m, s.n = d->n, s.k = d->k;
-    s.a_m = d->a_m, s.a_k = 1, s.b_k = d->b_k, s.b_n = 1;
-    s.d_m = d->d_m, s.d_n = d->d_n;
-    const AnyStore to{out, d->d_dtype};
-    if (d->k == 0) {  // a sum of nothing
-        hipLaunchKernelGGL(gemm_splitk_reduce, dim3(1024), dim3(256), 0, st, s, nullptr, 0, d->m * d->n, to);
-        return check(hipGetLastError(), "gemm_splitk_reduce launch");
+    const int64_t np = whole(d->n);
+    s.m = d->m, s.n = d->k, s.k = 2 * np;
+    s.a_m = 2 * np, s.a_k = 1, s.b_k = d->w_n, s.b_n = 1, s.d_m = d->k, s.d_n = 1;
+    if (!weights_whole(d)) {
+        GatedPad pad;
+        const void *src[2] = {gate, up};
+        const int64_t rows[2] = {d->n, d->n}, to_rows[2] = {np, np}, ld[2] = {d->w_n, d->w_n};
+        if (gated_pad(st, pad, 2, src, rows, to_rows, ld, d->k, ws)) return 1;
+        gate = pad.dst[0], up = pad.dst[1];
+        s.b_k = pad.kp;
+        ws = static_cast<char *>(ws) + up16(input_grad_pad(d));
+    } else if (!on(gate, 16) || !on(up, 16)) {
+        return fail("nhip_gated_input_grad: weights of whole rows start on 16 bytes");
     }
-    const PairPlan p = pair_plan(d);
-    GemmShape parts = s;
-    AnyStore first = to;
-    if (p.splits > 1) {
-        if (!ws) return fail("nhip_gemm_pair: no workspace");
-        parts.d_m = d->n, parts.d_n = 1, parts.d_split = d->m * d->n;
-        first = AnyStore{ws, 0};
+    const AnyStore to{dx, d->dtype};
+    constexpr int lds256 = gemm_stream_lds_bytes<64, 2>(), lds128 = gemm_stream_lds_bytes<64, 2, 128>();
+    if (d->dtype == NHIP_F16)
+        return p.tm == 256 ? part_go(st, gated_input_grad<true, 256>, s, 256, 1, p, lds256, dgu, gate, up, to, ws)
+                           : part_go(st, gated_input_grad<true, 128>, s, 128, 1, p, lds128, dgu, gate, up, to, ws);
+    return p.tm == 256 ? part_go(st, gated_input_grad<false, 256>, s, 256, 1, p, lds256, dgu, gate, up, to, ws)
+                       : part_go(st, gated_input_grad<false, 128>, s, 128, 1, p, lds128, dgu, gate, up, to, ws);
+}
+
+int gated_weight_grad_on(hipStream_t st, const nhip_gated_desc *d, const void *dgu, const void *x, void *dgate, void *dup, void *ws) {
+    if (backward_check(d, "nhip_gated_weight_grad")) return 1;
+    if (d->n == 0 || d->k == 0) return 0;
+    if (d->m == 0) return zero_grad(st, dgate, d->n * d->k) || (dup && zero_grad(st, dup, d->n * d->k));
+    const int64_t z = dup ? 2 : 1;
+    const PartPlan p = weight_grad_plan(d);
+    if (!ws && (p.parts > 1 || !input_whole(d))) return fail("nhip_gated_weight_grad: no workspace");
+    if (!on(dgu, 16) || !on(ws, 16)) return fail("nhip_gated_weight_grad: [dg | du] and the workspace start on 16 bytes");
+    if (!on(dgate, 2) || !on(dup, 2)) return fail("nhip_gated_weight_grad: results start on an element");
+    GemmShape s;
+    std::memset(&s, 0, sizeof(s));
+    const int64_t np = whole(d->n);
+    s.m = d->n, s.n = d->k, s.k = d->m;
+    s.a_m = 1, s.a_k = 2 * np, s.b_k = d->x_m, s.b_n = 1, s.d_m = d->k, s.d_n = 1;
+    s.nbatch = 1, s.batch[0] = z, s.a_batch[0] = np;
+    // the second result as the first one's batch, wherever it lies
+    if (dup) s.d_batch[0] = (static_cast<char *>(dup) - static_cast<char *>(dgate)) / 2;
+    if (!input_whole(d)) {
+        GatedPad pad;
+        if (gated_pad(st, pad, 1, &x, &d->m, &d->m, &d->x_m, d->k, ws)) return 1;
+        x = pad.dst[0];
+        s.b_k = pad.kp;
+        ws = static_cast<char *>(ws) + up16(weight_grad_pad(d));
+    } else if (!on(x, 16)) {
+        return fail("nhip_gated_weight_grad: whole rows of x start on 16 bytes");
     }
-    const int rc = d->a_dtype == NHIP_F16
-                       ? (p.tm == 256 ? pair_go<true, 256>(st, parts, p, a, b, b2, first) : pair_go<true, 128>(st, parts, p, a, b, b2, first))
-                       : (p.tm == 256 ? pair_go<false, 256>(st, parts, p, a, b, b2, first) : pair_go<false, 128>(st, parts, p, a, b, b2, first));
-    if (rc || p.splits == 1) return rc;
-    const int64_t total = d->m * d->n, blocks = (total + 255) / 256;
-    hipLaunchKernelGGL(gemm_splitk_reduce, dim3(unsigned(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, s,
-                       static_cast<const float *>(ws), p.splits, total, to);
-    return check(hipGetLastError(), "gemm_splitk_reduce launch");
+    const AnyStore to{dgate, d->dtype};
+    constexpr int lds256 = gemm_stream_lds_bytes<64, 2>(), lds128 = gemm_stream_lds_bytes<64, 2, 128>();
+    if (d->dtype == NHIP_F16)
+        return p.tm == 256 ? part_go(st, gated_weight_grad<true, 256>, s, 256, z, p, lds256, dgu, x, nullptr, to, ws)
+                           : part_go(st, gated_weight_grad<true, 128>, s, 128, z, p, lds128, dgu, x, nullptr, to, ws);
+    return p.tm == 256 ? part_go(st, gated_weight_grad<false, 256>, s, 256, z, p, lds256, dgu, x, nullptr, to, ws)
+                       : part_go(st, gated_weight_grad<false, 128>, s, 128, z, p, lds128, dgu, x, nullptr, to, ws);
 }
 
 // ---- gradient clipping ----------------------------------------------------------------------------------
@@ -546,14 +633,20 @@ int nhip_gated_linear_workspace(const nhip_gated_desc *desc, size_t *bytes) {
     return 0;
 }
 
-int nhip_gemm_pair(const nhip_gemm_desc *desc, const void *a, const void *b, const void *b2, void *d, void *workspace) {
+int nhip_gated_input_grad(const nhip_gated_desc *desc, const void *dgu, const void *gate, const void *up, void *dx,
+                          void *workspace) {
     NHIP_STREAM(st);
-    return pair_on(st, desc, a, b, b2, d, workspace);
+    return gated_input_grad_on(st, desc, dgu, gate, up, dx, workspace);
 }
 
-int nhip_gemm_pair_workspace(const nhip_gemm_desc *desc, size_t *bytes) {
-    if (pair_check(desc)) return 1;
-    *bytes = pair_workspace(desc);
+int nhip_gated_weight_grad(const nhip_gated_desc *desc, const void *dgu, const void *x, void *d_gate, void *d_up, void *workspace) {
+    NHIP_STREAM(st);
+    return gated_weight_grad_on(st, desc, dgu, x, d_gate, d_up, workspace);
+}
+
+int nhip_gated_backward_workspace(const nhip_gated_desc *desc, size_t *bytes) {
+    if (backward_check(desc, "nhip_gated_backward_workspace")) return 1;
+    *bytes = backward_workspace(desc);
     return 0;
 }
 

@@ -249,31 +249,34 @@ class _GatedLinear(Function):
     @staticmethod
     def backward(ctx, dh):
         x, gate, up, g, u = ctx.saved_tensors
-        n, acc, dtype = gate.shape[0], accum_dtype(x.dtype), x.dtype
+        (t, k), n, acc, dtype = x.shape, gate.shape[0], accum_dtype(x.dtype), x.dtype
+        whole = -(-n // 8) * 8  # each half of [dg | du] in whole 16-byte chunks
 
-        def body(dh, g, u):
+        def grad(dh, g, u):
             a, da = _activated_grad(ctx.activation, g)
             d = dh.to(acc)
-            return [F.cat([(d * u * da).to(dtype), (d * a).to(dtype)], 1)]
+            halves = [(d * u * da).to(dtype), (d * a).to(dtype)]
+            if whole != n:
+                pad = prims.full((t, whole - n), 0.0, dtype)
+                halves = [halves[0], pad, halves[1], pad]
+            return [F.cat(halves, 1)]
 
-        # [dg | du] in one tensor: one operand of dx, whose two products then share their sums
-        (dgu,) = _operator("gated_linear_grad", dtype in ("bfloat16", "float16"), [dh, g, u], body,
-                           activation=ctx.activation)
-        dw = [dot(dgu[:, lo:lo + n], x, (((0,), (0,)), ((), ())), acc, dtype) for lo in (0, n)]
-
-        def product(dgu, gate, up):
+        def input_grad(dgu, gate, up):
             dims = (((1,), (0,)), ((), ()))
-            return [(prims.dot_general(dgu[:, :n], gate, dims, acc) + prims.dot_general(dgu[:, n:], up, dims, acc)).to(dtype)]
+            return [(prims.dot_general(dgu[:, :n], gate, dims, acc)
+                     + prims.dot_general(dgu[:, whole:whole + n], up, dims, acc)).to(dtype)]
 
-        (dx,) = _operator("gemm_pair", _pair_taken(gate), [dgu, gate, up], product)
+        def weight_grad(dgu, x):
+            return [dot(dgu[:, lo:lo + n], x, (((0,), (0,)), ((), ())), acc, dtype) for lo in (0, whole)]
+
+        taken = dtype in ("bfloat16", "float16")
+        (dgu,) = _operator("gated_linear_grad", taken, [dh, g, u], grad, activation=ctx.activation)
+        taken = taken and n < 1 << 21 and whole * -(-k // 8) * 8 < (1 << 30) - 1024
+        (dx,) = _operator("gated_input_grad", taken, [dgu, gate, up], input_grad, features=n)
+        # tokens in whole k tiles and whole rows: the plan's own dots, which take an update of the weight into their stores
+        dots = t % 64 == 0 and n % 8 == 0 and k % 8 == 0
+        dw = _operator("gated_weight_grad", taken and not dots, [dgu, x], weight_grad, features=n)
         return dx, dw[0], dw[1]
-
-
-def _pair_taken(weight):
-    """Whether nhip_gemm_pair takes ``[dg | du]`` and weights of this type: whole 16-byte rows, a tile within 2^31 bytes."""
-    n, k = weight.shape
-    return (weight.dtype in ("bfloat16", "float16") and n > 0 and k > 0 and n % 8 == 0 and k % 8 == 0
-            and n * k < (1 << 30) - 1024 and n < 1 << 21)
 
 
 def gated_linear(input, gate_weight, up_weight, activation="silu"):

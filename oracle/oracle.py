@@ -72,7 +72,7 @@ def _param(key, v) -> list[str]:
 
 # Parameters the oracle does not read (labels, compiler annotations).
 _SKIP = {"label", "name", "ty", "view", "in_place", "kernel", "role", "q_dims", "k_dims", "v_dims", "scale", "causal",
-         "roles", "eps", "interleaved", "activation", "max_norm"}
+         "roles", "eps", "interleaved", "activation", "max_norm", "features"}
 
 
 def serialize(g: Graph) -> str:

@@ -285,6 +285,9 @@ GATED = [
     (5, 7, 3, "gelu", "float16"),
     (1, 1, 1, "silu", "bfloat16"),
     (70, 515, 131, "relu", "float16"),
+    (128, 64, 128, "silu", "bfloat16"),
+    (1000, 32, 36, "gelu", "bfloat16"),
+    (90, 1024, 48, "silu", "bfloat16"),
 ]
 
 
@@ -348,7 +351,7 @@ def test_every_gated_kernel(hip, t, k, n, save):
             if save:
                 _near(s[:t * n].astype(np.float64).reshape(t, n), x @ w.T, e * (np.abs(x) @ np.abs(w).T), config)
             assert np.all(s[t * n if save else 0:] == 77.0), config
-    assert ran >= 2
+    assert ran >= 3
     with pytest.raises(RuntimeError, match="does not take these operands"):
         _gated_abi(x, gate, up, "bfloat16", "silu", count.value, save)
 
@@ -375,7 +378,7 @@ def test_gated_of_values_that_are_not_finite(hip):
     want = M.gated(x, gate, up, np.zeros((40, 48)), "silu")[0]
     tol = _gated_tolerances(x, gate, up, np.zeros((40, 48)), "silu", "bfloat16")[0]
     x[3, 5], x[8, 0] = np.nan, np.inf
-    for config in (0, 1, 2):
+    for config in (0, 1, 2, 3):
         h = _gated_abi(x, gate, up, "bfloat16", "silu", config, False)[0][:40 * 48]
         got = D.to_numpy_values(h, "bfloat16").astype(np.float64).reshape(40, 48)
         rest = [i for i in range(40) if i not in (3, 8)]
@@ -396,7 +399,7 @@ def test_gated_past_32_bit_offsets(hip):
     want = M.gated(x, gate, up, np.zeros((3, 32)), "silu")[0]
     tol = _gated_tolerances(x, gate, up, np.zeros((3, 32)), "silu", "bfloat16")[0]
     ws = Dev(nbytes=2 * 64 * (3 + 2 * 32))
-    for config in (0, 1, 2):
+    for config in (0, 1, 2, 3):
         desc = nv.GatedDesc(m=3, n=32, k=64, x_m=far, w_n=64, h_m=32, dtype=1, activation=0, config=config)
         size = C.c_size_t()
         nv.call("nhip_gated_linear_workspace", C.byref(desc), C.byref(size))
@@ -405,30 +408,67 @@ def test_gated_past_32_bit_offsets(hip):
         _near(D.to_numpy_values(h.get((3, 32), np.uint16), "bfloat16").astype(np.float64), want, tol, config)
 
 
-@pytest.mark.parametrize("m,half,n,dtype", [(1, 8, 8, "bfloat16"), (130, 64, 64, "float16"), (257, 72, 136, "bfloat16"),
-                                            (40, 1416, 520, "float16"), (512, 4096, 264, "bfloat16"), (300, 2056, 72, "bfloat16")])
-def test_gemm_pair(hip, m, half, n, dtype):
-    """A[:, :k / 2] B + A[:, k / 2:] B2, whole and in parts, halves that end inside a k tile, beside values of the other
-    half that are not finite in other rows, and nothing written behind the result."""
-    rng = np.random.default_rng(m)
-    a, b, b2 = (_round(rng.standard_normal(s), dtype) for s in ((m, 2 * half), (half, n), (half, n)))
-    if m > 3:
-        a[2, half] = np.inf
-    dev = [Dev(np.ascontiguousarray(D.from_values(np.asarray(v, np.float32), dtype))) for v in (a, b, b2)]
-    dt = {"bfloat16": 1, "float16": 2}[dtype]
-    desc = nv.GemmDesc(m=m, n=n, k=2 * half, a_dtype=dt, b_dtype=dt, d_dtype=dt, a_m=2 * half, a_k=1, b_k=n, b_n=1, d_m=n, d_n=1)
+@pytest.mark.parametrize("t,k,n,dtype", [(1, 8, 8, "bfloat16"), (130, 64, 64, "float16"), (257, 136, 72, "bfloat16"),
+                                         (40, 520, 1416, "float16"), (512, 264, 4096, "bfloat16"), (300, 72, 2056, "bfloat16"),
+                                         (929, 167, 333, "bfloat16"), (3000, 65, 130, "float16"), (7, 1, 1, "bfloat16")])
+def test_gated_backward_kernels(hip, t, k, n, dtype):
+    """dx, d_gate and d_up of [dg | du] through the ABI: whole and in parts, sizes that end inside a tile of k or a chunk,
+    one row that is not finite, a d_up left out, and nothing written behind a result."""
+    rng = np.random.default_rng(t)
+    whole = -(-n // 8) * 8
+    x, gate, up, _ = _gated_case(t + k, t, k, n, dtype)
+    dg, du = (_round(rng.standard_normal((t, n)), dtype) for _ in range(2))
+    dgu = np.zeros((t, 2 * whole))
+    dgu[:, :n], dgu[:, whole:whole + n] = dg, du
+    bad = dgu.copy()
+    bad[t // 2, whole] = np.inf
+    bits = lambda v: np.ascontiguousarray(D.from_values(np.asarray(v, np.float32), dtype))  # noqa: E731
+    ddgu, dbad, dx_, dgate, dup = (Dev(bits(v)) for v in (dgu, bad, x, gate, up))
+    desc = nv.GatedDesc(m=t, n=n, k=k, x_m=k, w_n=k, dtype={"bfloat16": 1, "float16": 2}[dtype], config=-1)
     size = C.c_size_t()
-    nv.call("nhip_gemm_pair_workspace", C.byref(desc), C.byref(size))
-    ws, out = Dev(nbytes=size.value), Dev(np.full(m * n + 64, 0x4242, np.uint16))
-    nv.call("nhip_gemm_pair", C.byref(desc), *(v.ptr for v in dev), out.ptr, ws.ptr if size.value else None)
-    bits = out.get((m * n + 64,), np.uint16)
-    got = D.to_numpy_values(bits[:m * n].view(D.storage(dtype)), dtype).astype(np.float64).reshape(m, n)
-    assert np.all(bits[m * n:] == 0x4242)
-    rows = [i for i in range(m) if i != 2 or m <= 3]
-    want = a[rows, :half] @ b + a[rows, half:] @ b2
-    mags = np.abs(a[rows, :half]) @ np.abs(b) + np.abs(a[rows, half:]) @ np.abs(b2)
-    _near(got[rows], want, U[dtype] * np.abs(want) + F32 * (2 * half + 16) * mags)
-    assert m <= 3 or not np.isfinite(got[2]).any()
+    nv.call("nhip_gated_backward_workspace", C.byref(desc), C.byref(size))
+    ws = Dev(nbytes=size.value)
+
+    def outputs(count, rows):
+        return [Dev(np.full(rows * k + 64, 0x4242, np.uint16)) for _ in range(count)]
+
+    def values(dev, rows):
+        raw = dev.get((rows * k + 64,), np.uint16)
+        assert np.all(raw[rows * k:] == 0x4242)
+        return D.to_numpy_values(raw[:rows * k].view(D.storage(dtype)), dtype).astype(np.float64).reshape(rows, k)
+
+    for a in (ddgu, dbad):
+        (out,) = outputs(1, t)
+        nv.call("nhip_gated_input_grad", C.byref(desc), a.ptr, dgate.ptr, dup.ptr, out.ptr, ws.ptr if size.value else None)
+        got, want = values(out, t), dg @ gate + du @ up
+        rows = [i for i in range(t) if a is ddgu or i != t // 2]
+        mags = np.abs(dg) @ np.abs(gate) + np.abs(du) @ np.abs(up)
+        _near(got[rows], want[rows], (U[dtype] * np.abs(want) + F32 * (2 * n + 16) * mags)[rows], "dx")
+    for with_up in (True, False):
+        d_gate, d_up = outputs(2, n)
+        nv.call("nhip_gated_weight_grad", C.byref(desc), ddgu.ptr, dx_.ptr, d_gate.ptr, d_up.ptr if with_up else None,
+                ws.ptr if size.value else None)
+        for out, d in [(d_gate, dg), (d_up, du)][:1 + with_up]:
+            want = d.T @ x
+            _near(values(out, n), want, U[dtype] * np.abs(want) + F32 * (t + 16) * (np.abs(d).T @ np.abs(x)), "dw")
+        if not with_up:
+            assert np.all(d_up.get((n * k + 64,), np.uint16) == 0x4242)
+
+
+def test_gated_gradient_of_one_weight_and_of_no_tokens(hip):
+    """The gate's gradient alone, the up projection's alone, and zeros for an empty batch."""
+    x, gate, up, dh = _gated_case(12, 100, 72, 56, "bfloat16")
+    want, tol = M.gated(x, gate, up, dh, "silu"), _gated_tolerances(x, gate, up, dh, "silu", "bfloat16")
+    for i, name in ((2, "gate"), (3, "up")):
+        def fn(x, gate, up, dh):
+            f = (lambda w: F.gated_linear(x, w, up)) if name == "gate" else (lambda w: F.gated_linear(x, gate, w))
+            return list(L.vjp(f, gate if name == "gate" else up)[1](dh))
+
+        got = _values(L.compile(fn, device="hip")(*(_tensor(v, "bfloat16") for v in (x, gate, up, dh)))[0])
+        _near(got, want[i], tol[i], name)
+    out = L.compile(_gated_program("silu"), device="hip")(*(_tensor(v, "bfloat16") for v in (x[:0], gate, up, dh[:0])))
+    assert [tuple(t.shape) for t in out] == [(0, 56), (0, 72), (56, 72), (56, 72)] and not _values(out[2]).any() \
+        and not _values(out[3]).any()
 
 
 # ---- clipping

@@ -112,7 +112,11 @@ def test_gated_16_bit_is_two_fusions_and_ordinary_products():
     g = _graph(lambda x, gate, up, dh: (lambda h, pull: [h, *pull(dh)])(*L.vjp(F.gated_linear, x, gate, up)),
                *(np.zeros(s, np.uint16) for s in ((64, 64), (128, 64), (128, 64), (64, 128))), dtypes=["bfloat16"] * 4)
     assert [n.params["name"] for n in g.nodes if n.prim == "fusion"] == ["gated_linear", "gated_linear_grad",
-                                                                                          "gemm_pair"]
+                                                                                          "gated_input_grad"]
+    # tokens and features that are not whole tiles and chunks: the weights' gradients by the operator's own kernel
+    ragged = _graph(lambda x, gate, up, dh: (lambda h, pull: [h, *pull(dh)])(*L.vjp(F.gated_linear, x, gate, up)),
+                    *(np.zeros(s, np.uint16) for s in ((65, 64), (127, 64), (127, 64), (65, 127))), dtypes=["bfloat16"] * 4)
+    assert [n.params["name"] for n in ragged.nodes if n.prim == "fusion"][2:] == ["gated_input_grad", "gated_weight_grad"]
     forward = _graph(F_gated, *(np.zeros(s, np.uint16) for s in ((64, 64), (128, 64), (128, 64))), dtypes=["bfloat16"] * 3)
     plan = Plan(forward, build_kernels=False)
     assert [st.kind for st in plan.steps] == ["gated_fwd"] and len(plan.steps[0].outputs) == 1  # g and u are not stored
@@ -282,11 +286,15 @@ def test_abi_refusals():
     for m, k, want in [(64, 515, 0), (65, 512, 0), (65, 515, (65 + 2 * 8) * 520 * 2)]:  # few rows are read as they are
         nv.call("nhip_gated_linear_workspace", C.byref(nv.GatedDesc(m=m, n=8, k=k, x_m=k, w_n=k, dtype=1, config=-1)), C.byref(n))
         assert n.value == want
-    for kw, match in [(dict(k=24), "multiples of 8"), (dict(a_dtype=0, b_dtype=0), "bf16 or f16"), (dict(a_m=63), "whole rows"),
-                      (dict(m=-1), "negative"), (dict(b_k=1 << 31), "2\\^31")]:
-        pair = dict(m=64, n=64, k=128, a_dtype=1, b_dtype=1, d_dtype=1, a_m=128, a_k=1, b_k=64, b_n=1, d_m=64, d_n=1)
+    for kw, match in [(dict(m=-1), "negative"), (dict(dtype=0), "bf16 or f16"), (dict(n=1 << 21), "2\\^31"),
+                      (dict(n=1 << 15, k=1 << 15), "2\\^31")]:
+        d = nv.GatedDesc(**{**dict(m=64, n=64, k=64, x_m=64, w_n=64, dtype=1, config=-1), **kw})
         with pytest.raises(RuntimeError, match=match):
-            nv.call("nhip_gemm_pair_workspace", C.byref(nv.GemmDesc(**{**pair, **kw})), C.byref(n))
+            nv.call("nhip_gated_backward_workspace", C.byref(d), C.byref(n))
+    for m, n_, k, want in [(64, 64, 64, 0), (64, 63, 64, 2 * 64 * 64 * 2), (65, 64, 63, 2 * 64 * 64 * 2), (4096, 64, 63, 4096 * 64 * 2),
+                           (0, 64, 64, 0), (64, 0, 64, 0), (64, 64, 0, 0), (0, 0, 0, 0)]:
+        nv.call("nhip_gated_backward_workspace", C.byref(nv.GatedDesc(m=m, n=n_, k=k, x_m=k, w_n=k, dtype=1, config=-1)), C.byref(n))
+        assert n.value >= want and (want or not n.value)
     plan = C.c_void_p()
     nv.call("nhip_plan_create", C.byref(plan))
     d = nv.ClipDesc(count=3)
