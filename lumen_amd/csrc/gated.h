@@ -52,7 +52,8 @@ __device__ __forceinline__ void gated_act_grad(int act, float g, float &a, float
     } else if (act == kGatedGelu) {
         const float s = gated_sigmoid(2.0f * kGeluC * (g + kGeluA * g * g * g));
         a = g * s;
-        da = s + a * (1.0f - s) * (2.0f * kGeluC) * (1.0f + 3.0f * kGeluA * g * g);
+        const float t = a * (1.0f - s) * (2.0f * kGeluC);  // 0 for large g, and g * g may be infinite
+        da = s + t + 3.0f * kGeluA * (t * g) * g;
     } else if (act == kGatedRelu) {
         a = g <= 0.0f ? 0.0f : g;
         da = g > 0.0f ? 1.0f : 0.0f;

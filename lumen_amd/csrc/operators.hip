@@ -247,19 +247,27 @@ int gated_check(const nhip_gated_desc *d, const char *what) {
 
 int64_t tiles(int64_t m, int64_t bm, int64_t n, int64_t bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); }
 
+// The stream kernels' k: some, and 256 rows of it within the 2^31 bytes of a buffer.
+bool gated_stream_ok(const nhip_gated_desc *d) { return d->k > 0 && d->k < (int64_t(1) << 21); }
 bool gated_skinny_ok(const nhip_gated_desc *d) { return d->m <= 64 && d->k < (int64_t(1) << 30); }
-
-int gated_default(const nhip_gated_desc *d) {
-    if (gated_skinny_ok(d)) return kSkinnyCfg;
-    if (tiles(d->m, 256, d->n, 128) >= 256) return kStream256;
-    // one workgroup a CU: 6.5 us and 0.0080 a k with three stages, 4 and 0.0115 with two
-    return tiles(d->m, 128, d->n, 64) <= 256 && d->k >= 768 ? kDeepCfg : kStream128Cfg;
-}
 
 // Whether gated_stream can read rows of these lengths and distances in place (from 16-byte addresses).
 bool gated_rows(const nhip_gated_desc *d) {
     return d->k % 8 == 0 && d->x_m % 8 == 0 && d->w_n % 8 == 0 &&
            stream_buffer_ok(d->m, d->n, d->k, false, false, d->x_m, 1, 1, d->w_n);
+}
+
+int gated_default(const nhip_gated_desc *d) {
+    if (gated_skinny_ok(d)) {
+        // 33 to 64 rows of weights that leave gated_skinny more than a workgroup a CU, which then run one after the other:
+        // tiles of 128 rows are faster though half of one is empty ([64, 2048] x [8192, 2048] 19.2 us, 24.1, [64, 4096] x
+        // [11008, 4096] 33.9, 64.8; of 4096 features [64, 1024] 11.8, 8.2; of 32 rows [32, 2048] x [8192, 2048] 19.2, 18.3)
+        const bool wide = d->m > 32 && d->n > 4096 && d->k >= 768 && gated_stream_ok(d) && gated_rows(d);
+        return wide ? kDeepCfg : kSkinnyCfg;
+    }
+    if (tiles(d->m, 256, d->n, 128) >= 256) return kStream256;
+    // one workgroup a CU: 6.5 us and 0.0080 a k with three stages, 4 and 0.0115 with two
+    return tiles(d->m, 128, d->n, 64) <= 256 && d->k >= 768 ? kDeepCfg : kStream128Cfg;
 }
 
 size_t gated_workspace(const nhip_gated_desc *d) {
@@ -336,7 +344,7 @@ int gated_on(hipStream_t st, const nhip_gated_desc *d, const void *x, const void
     if (!g != !u) return fail("nhip_gated_linear: g and u go together");
     if (d->m == 0 || d->n == 0) return 0;
     int cfg = d->config < 0 ? gated_default(d) : d->config;
-    if (cfg >= kGatedConfigs || (cfg == kSkinnyCfg && !gated_skinny_ok(d)))
+    if (cfg >= kGatedConfigs || !(cfg == kSkinnyCfg ? gated_skinny_ok(d) : gated_stream_ok(d)))
         return fail("nhip_gated_linear: config " + std::to_string(cfg) + " does not take these operands");
     GemmShape s;
     std::memset(&s, 0, sizeof(s));
@@ -629,6 +637,7 @@ int nhip_gated_linear(const nhip_gated_desc *desc, const void *x, const void *ga
 
 int nhip_gated_linear_workspace(const nhip_gated_desc *desc, size_t *bytes) {
     if (gated_check(desc, "nhip_gated_linear_workspace")) return 1;
+    if (!gated_skinny_ok(desc) && !gated_stream_ok(desc)) return fail("nhip_gated_linear_workspace: 1 to 2^21 - 1 elements a row");
     *bytes = gated_workspace(desc);
     return 0;
 }

@@ -22,6 +22,7 @@ from lumen_amd.graph.tracer import TracedTensor, accum_dtype, broadcast_to, dot,
 
 KERNEL_DTYPES = ("float32", "bfloat16", "float16")
 MAX_HEAD = 1024  # a head's elements in the head kernels
+MAX_ROW = 1 << 21  # elements of a row of the gated projections: tiles of rows within 2^31 bytes
 ACTIVATIONS = ("silu", "gelu", "relu", "sigmoid")
 
 
@@ -107,7 +108,7 @@ class _QKNormRope(Function):
                 out.append(_turn(z, c, n, interleaved).to(q.dtype))
             return out
 
-        return _operator("qk_norm_rope", _heads_taken(q), operands, body, roles=roles, eps=float(eps),
+        return _operator("qk_norm_rope", _heads_taken(q, k), operands, body, roles=roles, eps=float(eps),
                          interleaved=bool(interleaved))
 
     @staticmethod
@@ -132,7 +133,7 @@ class _QKNormRope(Function):
                     dw.append(F.sum(dz * xhat, (0, 1, 2)).to(q.dtype))
             return dx + dw
 
-        out = _operator("qk_norm_rope_backward", _heads_taken(q), operands + [gq, gk], body, roles=roles + ("gq", "gk"),
+        out = _operator("qk_norm_rope_backward", _heads_taken(q, k), operands + [gq, gk], body, roles=roles + ("gq", "gk"),
                         eps=float(eps), interleaved=bool(interleaved))
         dw = iter(out[2:])
         return (out[0], out[1], next(dw) if wq is not None else None, next(dw) if wk is not None else None,
@@ -145,8 +146,9 @@ def _heads_operands(q, k, wq, wk, cos, sin, positions):
     return [x for _, x in named], tuple(n for n, _ in named)
 
 
-def _heads_taken(q):
-    return q.dtype in KERNEL_DTYPES and 0 < q.shape[3] <= MAX_HEAD and q.shape[1] < 1 << 30
+def _heads_taken(q, k):
+    return q.dtype in KERNEL_DTYPES and 0 < q.shape[3] <= MAX_HEAD and q.shape[1] < 1 << 30 \
+        and max(q.shape[2], k.shape[2]) < 1 << 20
 
 
 def qk_norm_rope(query, key, cos, sin, query_weight=None, key_weight=None, positions=None, eps=None, interleaved=False):
@@ -221,12 +223,17 @@ def _activated_grad(name, g):
     if name == "gelu":
         _, s = _gelu_parts(g)
         a = g * s
-        return a, s + a * (1.0 - s) * (2.0 * 0.7978845608) * (1.0 + 3.0 * 0.044715 * g * g)
+        t = a * (1.0 - s) * (2.0 * 0.7978845608)  # 0 for large g, and g * g may be infinite
+        return a, s + t + 3.0 * 0.044715 * (t * g) * g
     if name == "relu":
         zero = prims.full(g.shape, 0.0, g.dtype)
         return F.relu(g), F.where(prims.lt(zero, g), prims.full(g.shape, 1.0, g.dtype), zero)
     s = prims.logistic(g)
     return s, s * (1.0 - s)
+
+
+def _gated_taken(x):
+    return x.dtype in ("bfloat16", "float16") and 0 < x.shape[1] < MAX_ROW
 
 
 class _GatedLinear(Function):
@@ -241,7 +248,7 @@ class _GatedLinear(Function):
             g, u = (dot(x, w, (((1,), (1,)), ((), ())), acc, acc) for w in (gate, up))
             return [(_activated(activation, g) * u).to(x.dtype), g, u]
 
-        h, g, u = _operator("gated_linear", x.dtype in ("bfloat16", "float16"), [x, gate, up], body, activation=activation)
+        h, g, u = _operator("gated_linear", _gated_taken(x), [x, gate, up], body, activation=activation)
         ctx.activation = activation
         ctx.save_for_backward(x, gate, up, g, u)
         return h
@@ -269,7 +276,7 @@ class _GatedLinear(Function):
         def weight_grad(dgu, x):
             return [dot(dgu[:, lo:lo + n], x, (((0,), (0,)), ((), ())), acc, dtype) for lo in (0, whole)]
 
-        taken = dtype in ("bfloat16", "float16")
+        taken = _gated_taken(x)
         (dgu,) = _operator("gated_linear_grad", taken, [dh, g, u], grad, activation=ctx.activation)
         taken = taken and n < 1 << 21 and whole * -(-k // 8) * 8 < (1 << 30) - 1024
         (dx,) = _operator("gated_input_grad", taken, [dgu, gate, up], input_grad, features=n)

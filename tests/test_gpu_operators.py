@@ -698,3 +698,89 @@ def test_each_operator_captured_by_itself(hip, which):
         put(raw)
         captured.launch()
         assert all(np.array_equal(a, b) for a, b in zip(read(), want))
+
+
+def test_gated_of_no_features_and_many_rows(hip):
+    f = L.compile(_gated_program("silu"), device="hip")
+    got = f(*(_tensor(np.zeros(s), "bfloat16") for s in ((70, 0), (24, 0), (24, 0), (70, 24))))
+    assert [o.shape for o in got] == [(70, 24), (70, 0), (24, 0), (24, 0)] and not _values(got[0]).any()
+
+
+@pytest.mark.parametrize("t,k,n", [(33, 768, 4104), (64, 776, 4096 + 72), (40, 771, 4104), (64, 760, 4104)])
+def test_gated_of_wide_weights_and_few_rows(hip, t, k, n):
+    """Both sides of the rule that gives 33 to 64 rows of wide weights to the tiles of 128 rows."""
+    x, gate, up, dh = _gated_case(t + k, t, k, n, "bfloat16")
+    f = L.compile(lambda x, gate, up: [F.gated_linear(x, gate, up)], device="hip")
+    got = _values(f(*(_tensor(v, "bfloat16") for v in (x, gate, up)))[0])
+    _near(got, M.gated(x, gate, up, dh, "silu")[0], _gated_tolerances(x, gate, up, dh, "silu", "bfloat16")[0])
+
+
+@pytest.mark.parametrize("n", [8, 9])
+def test_gelu_gradient_where_the_square_overflows(hip, n):
+    """Both elementwise kernels: g of 1e25 and -1e25 have a derivative of 1 and 0."""
+    x = np.array([[1e25, 2.0], [-1e25, 2.0]])
+    gate, up, dh = np.tile([1.0, 0.0], (n, 1)), np.tile([0.0, 1.0], (n, 1)), np.full((2, n), 3.0)
+    x = _round(x, "bfloat16")
+    f = L.compile(_gated_program("gelu"), device="hip")
+    h, dx = (_values(v) for v in f(*(_tensor(v, "bfloat16") for v in (x, gate, up, dh)))[:2])
+    g = x[0, 0]
+    assert np.all(np.abs(h[0] - 2 * g) <= 2.0**-8 * 2 * g) and not h[1].any()
+    want = np.array([[6.0 * n, 3 * g * n], [0.0, 0.0]])
+    assert np.all(np.abs(dx - want) <= 1.01 * 2.0**-7 * want)  # du's rounding, then dx's
+
+
+def test_an_operand_used_twice(hip):
+    """Queries that are the keys, a gate that is the up projection, a gradient listed twice."""
+    x = _heads_case(31, 2, 9, 2, 2, 64, 64, "bfloat16", positions=False)
+    x["k"], x["wk"] = x["q"], x["wq"]
+
+    def heads(q, w, c, s, gq, gk):
+        out, pull = L.vjp(lambda q, w: F.qk_norm_rope(q, q, c, s, w, w, eps=1e-3), q, w)
+        return [*out, *pull((gq, gk))]
+
+    got = [_values(v) for v in L.compile(heads, device="hip")(*(
+        _tensor(x[n], "float32" if n in ("cos", "sin") else "bfloat16") for n in ("q", "wq", "cos", "sin", "gq", "gk")))]
+    want = M.heads(x, 1e-3, False)
+    _heads_check(got[:2], x, "bfloat16", 1e-3, False)
+    for a, parts in ((got[2], want[2:4]), (got[3], want[4:6])):
+        rows = np.prod(x["q"].shape[:3])
+        tol = U["bfloat16"] * (sum(np.abs(p) for p in parts) + np.abs(sum(parts))) * 1.01 + F32 * (rows + 104) * 8 * rows
+        _near(a, sum(parts), tol)
+    t, w, _, dh = _gated_case(32, 70, 72, 40, "bfloat16")
+
+    def gated(t, w, dh):
+        h, pull = L.vjp(lambda t, w: F.gated_linear(t, w, w), t, w)
+        return [h, *pull(dh)]
+
+    got = [_values(v) for v in L.compile(gated, device="hip")(*(_tensor(v, "bfloat16") for v in (t, w, dh)))]
+    h, dx, dg, du = M.gated(t, w, w, dh, "silu")
+    th, tdx, tdg, tdu = _gated_tolerances(t, w, w, dh, "silu", "bfloat16")
+    _near(got[0], h, th)
+    _near(got[1], dx, tdx)
+    _near(got[2], dg + du, tdg + tdu + U["bfloat16"] * 1.05 * np.abs(dg + du) + U["bfloat16"] * (tdg + tdu))
+    clip = L.compile(lambda g: (lambda c, n: [n, *c])(*F.clip_grad_norm([g, g], 1.0)), device="hip")
+    out = [_values(v) for v in clip(_tensor(t, "bfloat16"))]
+    norm = np.sqrt(2 * (t * t).sum())
+    assert abs(out[0] - norm) <= 2 * F32 * norm
+    for o in out[1:]:
+        _near(o, t / (norm + 1e-6), (U["bfloat16"] + 4 * F32) * np.abs(t / norm))
+
+
+@pytest.mark.parametrize("flags", [dict(memory_limit=1), dict(schedules=False, update_in_place=False),
+                                   dict(merge_dots=False, epilogue_fusion=False)], ids=lambda f: "-".join(f))
+def test_a_layer_in_training_under_other_flags(hip, flags):
+    """The same layer's two calls with rematerialized values, without donation and without merged
+    products: output, norm and weights within 2e-2 of the largest, as the layer is held against the oracle."""
+    runs = []
+    for patch in ({}, flags):
+        rng = np.random.default_rng(9)
+        layer = _layer(64, 96, 32, 0.5)
+        _load(layer, rng)
+        with L.config.compiler.patch(**patch):
+            f = L.compile(_train, device="hip")
+            out = []
+            for _ in range(2):
+                out += [_values(v).copy() for v in f(layer, *_layer_inputs(rng, 48, 64, 32, 16), 2, 2)]
+        runs.append(out + [_values(p).copy() for p in layer.parameters()])
+    for a, b in zip(*runs):
+        assert np.abs(a - b).max() <= 2e-2 * max(np.abs(a).max(), 1e-6)

@@ -307,6 +307,77 @@ def test_abi_refusals():
     nv.call("nhip_plan_destroy", plan)
 
 
+def test_gated_kernels_refuse_rows_of_nothing_and_rows_past_a_buffer():
+    """Above 64 rows the kernels read through buffers of at most 2^31 bytes and need a k; the trace holds primitives there."""
+    n = C.c_size_t()
+    for m, k, taken in [(64, 0, True), (65, 0, False), (65, 1 << 21, False), (64, 1 << 21, True), (65, (1 << 21) - 8, True)]:
+        d = nv.GatedDesc(m=m, n=8, k=k, x_m=k, w_n=k, dtype=1, config=-1)
+        if taken:
+            nv.call("nhip_gated_linear_workspace", C.byref(d), C.byref(n))
+        else:
+            with pytest.raises(RuntimeError, match="elements a row"):
+                nv.call("nhip_gated_linear_workspace", C.byref(d), C.byref(n))
+    for k, fusions in [(0, []), (1 << 21, []), (8, ["gated_linear"])]:
+        g = L.make_graph(F_gated)(*(_m((rows, k), "bfloat16") for rows in (70, 8, 8)))
+        assert [m.params["name"] for m in g.nodes if m.prim == "fusion"] == fusions
+
+
+def test_heads_past_a_launch_are_primitives():
+    def fn(q, k, c, s):
+        return list(F.qk_norm_rope(q, k, c, s))
+
+    for heads, fusions in [((1 << 20) - 1, 1), (1 << 20, 0)]:
+        g = L.make_graph(fn)(_m((1, 1, heads, 2), "float32"), _m((1, 1, 1, 2), "float32"), *[_m((1, 1), "float32")] * 2)
+        assert sum(m.prim == "fusion" for m in g.nodes) == fusions
+
+
+@pytest.mark.parametrize("g0", [1e25, -1e25])
+def test_gelu_gradient_where_the_square_overflows(g0):
+    """act(g) is g or 0 and act'(g) 1 or 0: exact, though g g is no float32."""
+    x, gate, up, dh = (np.array(v, np.float32) for v in ([[g0, 2.0]], [[1.0, 0.0]], [[0.0, 1.0]], [[3.0]]))
+
+    def fn(x, gate, up, dh):
+        h, pull = L.vjp(lambda x, gate, up: F.gated_linear(x, gate, up, activation="gelu"), x, gate, up)
+        return [h, *pull(dh)]
+
+    got, _ = _run(fn, x, gate, up, dh)
+    g = np.float64(np.float32(g0))
+    a, d = (g, 1.0) if g0 > 0 else (0.0, 0.0)
+    want = [[[2 * a]], [[6 * d, 3 * a]], [[6 * d * g, 12 * d]], [[3 * a * g, 6 * a]]]
+    for v, w in zip(got, want):
+        assert np.all(np.abs(v - np.array(w)) <= 2.0**-22 * np.abs(w)) or not np.isfinite(np.float32(w)).all()
+
+
+def test_an_operand_used_twice():
+    """Queries that are the keys, a gate that is the up projection, a gradient listed twice: each use has its part."""
+    rng = np.random.default_rng(21)
+    x = M.heads_inputs(rng, 1, 4, 2, 2, 8, 8, table=4, dtype="float64", positions=False)
+    x["k"], x["wk"] = x["q"], x["wq"]
+
+    def heads(q, w, c, s, gq, gk):
+        out, pull = L.vjp(lambda q, w: F.qk_norm_rope(q, q, c, s, w, w, eps=1e-3), q, w)
+        return [*out, *pull((gq, gk))]
+
+    got, _ = _run(heads, *(x[n] for n in ("q", "wq", "cos", "sin", "gq", "gk")))
+    want = M.heads(x, 1e-3, False)
+    want = [want[0], want[1], want[2] + want[3], want[4] + want[5]]
+    t, w, dh = rng.standard_normal((3, 5)), rng.standard_normal((4, 5)), rng.standard_normal((3, 4))
+
+    def gated(t, w, dh):
+        h, pull = L.vjp(lambda t, w: F.gated_linear(t, w, w), t, w)
+        return [h, *pull(dh)]
+
+    got += _run(gated, t, w, dh)[0]
+    h, dx, dg, du = M.gated(t, w, w, dh, "silu")
+    want += [h, dx, dg + du]
+    got += _run(lambda g: (lambda c, n: [n, *c])(*F.clip_grad_norm([g, g], 1.0)), t)[0]
+    scale = min(1.0, 1 / (np.sqrt(2 * (t * t).sum()) + 1e-6))
+    want += [np.sqrt(2 * (t * t).sum()), t * scale, t * scale]
+    for i, (a, b) in enumerate(zip(got, want)):
+        # float64 to a few hundred roundings; the tables and the scale are float32
+        assert np.abs(a - b).max() <= 2.0**-22 * max(1, np.abs(b).max()), i
+
+
 # ---- plans
 
 
