@@ -265,7 +265,7 @@ static __global__ __launch_bounds__(256) void gated_pad_kernel(GatedPad a) {
 }
 
 // The input's gradient: D = A[:, :k / 2] B + A[:, k / 2:] B2 with A = [dg | du] and the weights as they lie: one
-// accumulator over both products, or (parts of k) float32 sums that gemm_splitk_reduce adds. Two products and their sum write
+// accumulator over both products, or (parts of k) float32 sums that gated_sum_kernel adds. Two products and their sum write
 // and read 8 m n bytes more: [4096, 2048] of k 2 x 8192 243 us, 325.
 template <bool F16, int TM>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TM == 256 ? 1 : 2, TM == 256 ? 1 : 2))) void gated_input_grad(
@@ -281,6 +281,37 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TM == 256 ?
     GemmShape s, const uint16_t *__restrict__ a, const uint16_t *__restrict__ b, const uint16_t *, AnyStore out, int k_part) {
     extern __shared__ __align__(1024) char smem[];
     gemm_stream_tile<F16, 64, 2, true, true, true, AnyStore, TM, TM == 256 ? 3 : 0, 3>(s, a, b, out, smem, nullptr, k_part);
+}
+
+// Float32 sums of the parts, P[part][z][mn], added in order and rounded once into result z (blockIdx.y). V elements a thread:
+// four where the size and the results' alignment allow (2 parts of [4096, 2048] in 16.5 us, one a thread 24.8).
+struct GatedSum {
+    const float *part;
+    void *out[2];
+    int64_t mn;
+    int32_t parts;
+};
+template <typename T, int V>
+__global__ __launch_bounds__(256) void gated_sum_kernel(GatedSum a) {
+    typedef float vec __attribute__((ext_vector_type(V)));
+    const int64_t step = int64_t(gridDim.y) * a.mn, first = int64_t(blockIdx.y) * a.mn;
+    T *out = static_cast<T *>(a.out[blockIdx.y]);
+    for (int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * V; i < a.mn; i += int64_t(gridDim.x) * 256 * V) {
+        const float *p = a.part + first + i;
+        vec v = *reinterpret_cast<const vec *>(p);
+#pragma unroll 4
+        for (int k = 1; k < a.parts; ++k) v += *reinterpret_cast<const vec *>(p + k * step);
+        T r[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) store_f32_as(&r[k], v[k]);
+        if constexpr (V == 4) {
+            uint2 w;
+            __builtin_memcpy(&w, r, 8);
+            *reinterpret_cast<uint2 *>(out + i) = w;
+        } else {
+            out[i] = r[0];
+        }
+    }
 }
 
 // [dg | du] of 8 elements a thread (V 8: n, the strides and the pointers multiples of 16 bytes) or of one (V 1). Each half

@@ -463,10 +463,19 @@ int part_go(hipStream_t st, K kern, GemmShape s, int tm, int64_t z, const PartPl
                        p.k_part);
     const int rc = check(hipGetLastError(), "gated backward launch");
     if (rc || p.parts == 1) return rc;
-    const int64_t total = z * s.m * s.n, blocks = (total + 255) / 256;
-    hipLaunchKernelGGL(gemm_splitk_reduce, dim3(unsigned(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, s,
-                       static_cast<const float *>(ws), p.parts, total, to);
-    return check(hipGetLastError(), "gemm_splitk_reduce launch");
+    uint16_t *out = static_cast<uint16_t *>(to.d);
+    const GatedSum g{static_cast<const float *>(ws), {out, out + s.d_batch[0]}, s.m * s.n, p.parts};
+    const bool vec = g.mn % 4 == 0 && on(g.out[0], 8) && on(g.out[1], 8);
+    const int64_t blocks = ((vec ? g.mn / 4 : g.mn) + 255) / 256;
+    const dim3 grid(unsigned(blocks < 4096 ? blocks : 4096), unsigned(z));
+    if (to.dtype == NHIP_F16) {
+        if (vec) hipLaunchKernelGGL((gated_sum_kernel<f16_t, 4>), grid, dim3(256), 0, st, g);
+        else hipLaunchKernelGGL((gated_sum_kernel<f16_t, 1>), grid, dim3(256), 0, st, g);
+    } else {
+        if (vec) hipLaunchKernelGGL((gated_sum_kernel<bf16_t, 4>), grid, dim3(256), 0, st, g);
+        else hipLaunchKernelGGL((gated_sum_kernel<bf16_t, 1>), grid, dim3(256), 0, st, g);
+    }
+    return check(hipGetLastError(), "gated_sum_kernel launch");
 }
 
 // A result of no terms.
