@@ -267,20 +267,21 @@ static __global__ __launch_bounds__(256) void gated_pad_kernel(GatedPad a) {
 // The input's gradient: D = A[:, :k / 2] B + A[:, k / 2:] B2 with A = [dg | du] and the weights as they lie: one
 // accumulator over both products, or (parts of k) float32 sums that gated_sum_kernel adds. Two products and their sum write
 // and read 8 m n bytes more: [4096, 2048] of k 2 x 8192 243 us, 325.
-template <bool F16, int TM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TM == 256 ? 1 : 2, TM == 256 ? 1 : 2))) void gated_input_grad(
+// ST: 0 (tiles of 256, a workgroup a CU), 2 (128, two a CU) or 3 stages (128, one a CU, loads two tiles ahead).
+template <bool F16, int TM, int ST>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ST == 2 ? 2 : 1, ST == 2 ? 2 : 1))) void gated_input_grad(
     GemmShape s, const uint16_t *__restrict__ a, const uint16_t *__restrict__ b, const uint16_t *__restrict__ b2, AnyStore out,
     int k_part) {
     extern __shared__ __align__(1024) char smem[];
-    gemm_stream_tile<F16, 64, 2, false, true, true, AnyStore, TM, TM == 256 ? 3 : 0, 2>(s, a, b, out, smem, b2, k_part);
+    gemm_stream_tile<F16, 64, 2, false, true, true, AnyStore, TM, TM == 256 ? 3 : ST == 3 ? 1 : 0, 2, TM == 256 ? 0 : ST>(s, a, b, out, smem, b2, k_part);
 }
 
 // The weights' gradients: D_i = A_i^T X for the two halves of A = [dg | du], one batch each, over tokens of any number.
-template <bool F16, int TM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TM == 256 ? 1 : 2, TM == 256 ? 1 : 2))) void gated_weight_grad(
+template <bool F16, int TM, int ST>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ST == 2 ? 2 : 1, ST == 2 ? 2 : 1))) void gated_weight_grad(
     GemmShape s, const uint16_t *__restrict__ a, const uint16_t *__restrict__ b, const uint16_t *, AnyStore out, int k_part) {
     extern __shared__ __align__(1024) char smem[];
-    gemm_stream_tile<F16, 64, 2, true, true, true, AnyStore, TM, TM == 256 ? 3 : 0, 3>(s, a, b, out, smem, nullptr, k_part);
+    gemm_stream_tile<F16, 64, 2, true, true, true, AnyStore, TM, TM == 256 ? 3 : ST == 3 ? 1 : 0, 3, TM == 256 ? 0 : ST>(s, a, b, out, smem, nullptr, k_part);
 }
 
 // Float32 sums of the parts, P[part][z][mn], added in order and rounded once into result z (blockIdx.y). V elements a thread:

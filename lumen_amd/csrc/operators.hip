@@ -386,9 +386,10 @@ namespace {
 // (Plan._split_us), whose loops these are. longest: k tiles that a part may have at most.
 struct PartPlan {
     int tm, parts, k_part;
+    bool deep;  // at most a workgroup a CU of 128-row tiles: three stages
 };
 PartPlan part_plan(int64_t m, int64_t n, int64_t z, int64_t total, int64_t longest) {
-    PartPlan best{0, 0, 0};
+    PartPlan best{0, 0, 0, false};
     double least = 0;
     if (total < 1) total = 1;  // no tokens: nothing is launched, the workspace is asked for all the same
     for (int tm : {256, 128})
@@ -397,13 +398,16 @@ PartPlan part_plan(int64_t m, int64_t n, int64_t z, int64_t total, int64_t longe
             if (part > longest) continue;
             if (best.tm && parts > 1 && (part < 8 || parts * z * m * n * 4 > (int64_t(64) << 20))) continue;
             const int64_t t = tiles(m, tm, n, tm) * z * parts;
-            // 256: a workgroup a CU; 128: two, one alone taking 0.79 of a round of both
-            double rounds = tm == 256 ? double((t + 255) / 256) : double(t / 512);
+            // 256: a workgroup a CU; 128: two, one alone taking 0.79 of a round of both, 0.62 with three stages, whose LDS
+            // leaves room for one ([2000, 1024] x [2048, 1024] weights' gradients 30.4 -> 23.8 us; launches of more than 256
+            // are slower so: [1463, 3392] x [712, 3392] 26.7 -> 33.2)
+            const bool deep = tm == 128 && t <= 256;
+            double rounds = tm == 256 ? double((t + 255) / 256) : deep ? 0.62 : double(t / 512);
             const int64_t rest = t % 512;
-            if (tm == 128) rounds += rest == 0 ? 0.0 : rest <= 256 ? 0.79 : 1.0;
+            if (tm == 128 && !deep) rounds += rest == 0 ? 0.0 : rest <= 256 ? 0.79 : 1.0;
             const double us = 6.2 + 64.0 * double(part) * (tm == 256 ? 0.02355 : 0.0142) * rounds +
                               (parts > 1 ? 4.2 + 8.0 * double(parts) * double(z * m) * double(n) / 6.13e6 : 0.0);
-            if (least == 0 || us < least) least = us, best = PartPlan{tm, int(parts), int(part)};
+            if (least == 0 || us < least) least = us, best = PartPlan{tm, int(parts), int(part), deep};
         }
     return best;
 }
@@ -508,12 +512,15 @@ int gated_input_grad_on(hipStream_t st, const nhip_gated_desc *d, const void *dg
         return fail("nhip_gated_input_grad: weights of whole rows start on 16 bytes");
     }
     const AnyStore to{dx, d->dtype};
-    constexpr int lds256 = gemm_stream_lds_bytes<64, 2>(), lds128 = gemm_stream_lds_bytes<64, 2, 128>();
-    if (d->dtype == NHIP_F16)
-        return p.tm == 256 ? part_go(st, gated_input_grad<true, 256>, s, 256, 1, p, lds256, dgu, gate, up, to, ws)
-                           : part_go(st, gated_input_grad<true, 128>, s, 128, 1, p, lds128, dgu, gate, up, to, ws);
-    return p.tm == 256 ? part_go(st, gated_input_grad<false, 256>, s, 256, 1, p, lds256, dgu, gate, up, to, ws)
-                       : part_go(st, gated_input_grad<false, 128>, s, 128, 1, p, lds128, dgu, gate, up, to, ws);
+    constexpr int lds256 = gemm_stream_lds_bytes<64, 2>(), lds128 = gemm_stream_lds_bytes<64, 2, 128>(),
+                  deep = gemm_stream_lds_bytes<64, 2, 128, 3>();
+    auto go = [&](auto f16) {
+        constexpr bool F16 = decltype(f16)::value;
+        if (p.tm == 256) return part_go(st, gated_input_grad<F16, 256, 0>, s, 256, 1, p, lds256, dgu, gate, up, to, ws);
+        if (p.deep) return part_go(st, gated_input_grad<F16, 128, 3>, s, 128, 1, p, deep, dgu, gate, up, to, ws);
+        return part_go(st, gated_input_grad<F16, 128, 2>, s, 128, 1, p, lds128, dgu, gate, up, to, ws);
+    };
+    return d->dtype == NHIP_F16 ? go(std::true_type{}) : go(std::false_type{});
 }
 
 int gated_weight_grad_on(hipStream_t st, const nhip_gated_desc *d, const void *dgu, const void *x, void *dgate, void *dup, void *ws) {
@@ -543,12 +550,15 @@ int gated_weight_grad_on(hipStream_t st, const nhip_gated_desc *d, const void *d
         return fail("nhip_gated_weight_grad: whole rows of x start on 16 bytes");
     }
     const AnyStore to{dgate, d->dtype};
-    constexpr int lds256 = gemm_stream_lds_bytes<64, 2>(), lds128 = gemm_stream_lds_bytes<64, 2, 128>();
-    if (d->dtype == NHIP_F16)
-        return p.tm == 256 ? part_go(st, gated_weight_grad<true, 256>, s, 256, z, p, lds256, dgu, x, nullptr, to, ws)
-                           : part_go(st, gated_weight_grad<true, 128>, s, 128, z, p, lds128, dgu, x, nullptr, to, ws);
-    return p.tm == 256 ? part_go(st, gated_weight_grad<false, 256>, s, 256, z, p, lds256, dgu, x, nullptr, to, ws)
-                       : part_go(st, gated_weight_grad<false, 128>, s, 128, z, p, lds128, dgu, x, nullptr, to, ws);
+    constexpr int lds256 = gemm_stream_lds_bytes<64, 2>(), lds128 = gemm_stream_lds_bytes<64, 2, 128>(),
+                  deep = gemm_stream_lds_bytes<64, 2, 128, 3>();
+    auto go = [&](auto f16) {
+        constexpr bool F16 = decltype(f16)::value;
+        if (p.tm == 256) return part_go(st, gated_weight_grad<F16, 256, 0>, s, 256, z, p, lds256, dgu, x, nullptr, to, ws);
+        if (p.deep) return part_go(st, gated_weight_grad<F16, 128, 3>, s, 128, z, p, deep, dgu, x, nullptr, to, ws);
+        return part_go(st, gated_weight_grad<F16, 128, 2>, s, 128, z, p, lds128, dgu, x, nullptr, to, ws);
+    };
+    return d->dtype == NHIP_F16 ? go(std::true_type{}) : go(std::false_type{});
 }
 
 // ---- gradient clipping ----------------------------------------------------------------------------------

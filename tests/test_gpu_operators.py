@@ -784,3 +784,11 @@ def test_a_layer_in_training_under_other_flags(hip, flags):
         runs.append(out + [_values(p).copy() for p in layer.parameters()])
     for a, b in zip(*runs):
         assert np.abs(a - b).max() <= 2e-2 * max(np.abs(a).max(), 1e-6)
+
+
+@pytest.mark.parametrize("t,k,n,dtype", [(2901, 2891, 9, "float16"), (70, 2300, 2001, "bfloat16"), (2300, 2307, 77, "bfloat16"),
+                                         (65, 1153, 2304, "float16"), (700, 700, 12000, "bfloat16")])
+def test_gated_backward_kernels_of_many_tiles(hip, t, k, n, dtype):
+    """As above where the products' launches pass one workgroup a CU: tiles of 256 whole (dx; then the weights'), tiles of 128
+    in two stages (dx; then the weights'), and tiles of 256 in parts (dx)."""
+    test_gated_backward_kernels(hip, t, k, n, dtype)
