@@ -105,7 +105,7 @@ struct GatedOut {
                         __builtin_amdgcn_sched_barrier(0);
                     }
             wave_order();
-            stream_store_rows<WC, P>(shape, to, 0, stage, rbase + 64 * half, cbase, lane);
+            stream_store_dense<WC, P>(shape, to, 0, stage, rbase + 64 * half, cbase, lane);
             wave_order();
         };
 #pragma unroll
@@ -214,7 +214,8 @@ __global__ __launch_bounds__(64 * NW) void gated_skinny(GemmShape s, const uint1
         for (int c = 0; c < 2; ++c) {
             const int left = k - (k0 + 32 * c + 8 * g);
             auto tail = [&](const uint16_t *p) {
-                if constexpr (ANY) return left > 0 ? load8_any(p + k0 + 32 * c, left) : make_uint4(0, 0, 0, 0);
+                if constexpr (ANY)
+                    return left >= 8 ? load8_words(p + k0 + 32 * c) : left > 0 ? load8_any(p + k0 + 32 * c, left) : make_uint4(0, 0, 0, 0);
                 else return left > 0 ? get(p + k0 + 32 * c) : make_uint4(0, 0, 0, 0);
             };
             const uint4 f0 = tail(pb[0]), f1 = tail(pb[1]);
@@ -243,7 +244,7 @@ __global__ __launch_bounds__(64 * NW) void gated_skinny(GemmShape s, const uint1
 }
 
 // Rows of any length, alignment or distance, as gated_stream reads them: each of x's m rows and the weights' 2 n copied to
-// rows of kp = k rounded up to 8 elements, 16 bytes a thread, zeros past k. A pass over the operands that a product of many
+// rows of kp = k rounded up to 8 elements, 16 bytes a thread, zeros past k, a matrix each blockIdx.y. A pass over the operands that a product of many
 // rows hides and one of few rows does not need (gated_skinny reads any rows): [16384, 2047] x [8192, 2047] 60 of 970 us.
 struct GatedPad {
     const uint16_t *src[3];
@@ -251,16 +252,14 @@ struct GatedPad {
     int64_t rows[3], to_rows[3], ld[3], k, kp;  // to_rows: rows written, those past `rows` zeros
 };
 static __global__ __launch_bounds__(256) void gated_pad_kernel(GatedPad a) {
-    const int64_t per = a.kp / 8;
-    for (int which = 0; which < 3; ++which) {
-        const int64_t total = a.to_rows[which] * per;
-        for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
-            const int64_t row = i / per, c = (i - row * per) * 8;
-            const uint16_t *src = a.src[which] + row * a.ld[which] + c;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (row < a.rows[which]) v = a.k - c >= 8 ? load8_words(src) : load8_any(src, a.k - c);
-            *reinterpret_cast<uint4 *>(a.dst[which] + row * a.kp + c) = v;
-        }
+    const int which = blockIdx.y;
+    const int64_t per = a.kp / 8, total = a.to_rows[which] * per;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+        const int64_t row = i / per, c = (i - row * per) * 8;
+        const uint16_t *src = a.src[which] + row * a.ld[which] + c;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < a.rows[which]) v = a.k - c >= 8 ? load8_words(src) : load8_any(src, a.k - c);
+        *reinterpret_cast<uint4 *>(a.dst[which] + row * a.kp + c) = v;
     }
 }
 
@@ -315,8 +314,9 @@ __global__ __launch_bounds__(256) void gated_sum_kernel(GatedSum a) {
     }
 }
 
-// [dg | du] of 8 elements a thread (V 8: n, the strides and the pointers multiples of 16 bytes) or of one (V 1). Each half
-// of a row has np elements, n rounded up to 8, the last ones zeros: the products read whole chunks.
+// [dg | du] of 8 elements a thread. ANY: n, dh's rows or a pointer no multiple of 16 bytes (of [929, 5550] 13.8 us; one element
+// a thread 14.7). Each half of a row of [dg | du] has np elements, n rounded up to 8, the last ones zeros: the
+// products read whole chunks.
 struct GatedGrad {
     const void *dh;
     const float *g, *u;
@@ -324,55 +324,49 @@ struct GatedGrad {
     int64_t m, n, np, dh_m;
     int32_t act;
 };
-template <typename T, int V>
+template <typename T, bool ANY>
 __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGrad a) {
-    const int64_t per = a.np / V, total = a.m * per;
+    typedef float vec16 __attribute__((ext_vector_type(4)));
+    typedef float vec4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef std::conditional_t<ANY, vec4, vec16> vec;
+    const int64_t per = a.np / 8, total = a.m * per;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
-        const int64_t row = i / per, col = (i - row * per) * V;
-        const T *dh = static_cast<const T *>(a.dh) + row * a.dh_m + col;
+        const int64_t row = i / per, col = (i - row * per) * 8, left = a.n - col;
+        const uint16_t *dh = static_cast<const uint16_t *>(a.dh) + row * a.dh_m + col;
         const float *g = a.g + row * a.n + col, *u = a.u + row * a.n + col;
-        T *out = static_cast<T *>(a.out) + row * 2 * a.np + col;
-        if (V == 1 && col >= a.n) {
-            store_f32_as(out, 0.0f);
-            store_f32_as(out + a.np, 0.0f);
-            continue;
-        }
-        float d[V], gv[V], uv[V];
-        if constexpr (V == 8) {
-            const uint4 r = *reinterpret_cast<const uint4 *>(dh);
-            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const T lo{uint16_t(w[k] & 0xffff)}, hi{uint16_t(w[k] >> 16)};
-                d[2 * k] = load_as_f32(&lo), d[2 * k + 1] = load_as_f32(&hi);
-            }
+        uint4 r;
+        float gv[8], uv[8];
+        if (!ANY || left >= 8) {
+            if constexpr (ANY) r = load8_words(dh);
+            else r = *reinterpret_cast<const uint4 *>(dh);
 #pragma unroll
             for (int k = 0; k < 8; k += 4) {
-                const float4 p = *reinterpret_cast<const float4 *>(g + k), q = *reinterpret_cast<const float4 *>(u + k);
-                gv[k] = p.x, gv[k + 1] = p.y, gv[k + 2] = p.z, gv[k + 3] = p.w;
-                uv[k] = q.x, uv[k + 1] = q.y, uv[k + 2] = q.z, uv[k + 3] = q.w;
-            }
-        } else {
-            d[0] = load_as_f32(dh), gv[0] = *g, uv[0] = *u;
-        }
-        T dg[V], du[V];
+                const vec p = *reinterpret_cast<const vec *>(g + k), q = *reinterpret_cast<const vec *>(u + k);
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
+                for (int e = 0; e < 4; ++e) gv[k + e] = p[e], uv[k + e] = q[e];
+            }
+        } else {  // the row's last chunk: zeros past it
+            r = load8_any(dh, left);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) gv[k] = k < left ? g[k] : 0.0f, uv[k] = k < left ? u[k] : 0.0f;
+        }
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+        T dg[8], du[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const T bits{uint16_t(w[k / 2] >> (k % 2 * 16))};
+            const float d = load_as_f32(&bits);
             float act, grad;
             gated_act_grad(a.act, gv[k], act, grad);
-            store_f32_as(&dg[k], d[k] * uv[k] * grad);
-            store_f32_as(&du[k], d[k] * act);
+            store_f32_as(&dg[k], d * uv[k] * grad);
+            store_f32_as(&du[k], d * act);
         }
-        if constexpr (V == 8) {
-            uint4 p, q;
-            __builtin_memcpy(&p, dg, 16);
-            __builtin_memcpy(&q, du, 16);
-            *reinterpret_cast<uint4 *>(out) = p;
-            *reinterpret_cast<uint4 *>(out + a.np) = q;
-        } else {
-            out[0] = dg[0];
-            out[a.np] = du[0];
-        }
+        uint4 p, q;
+        __builtin_memcpy(&p, dg, 16);
+        __builtin_memcpy(&q, du, 16);
+        T *out = static_cast<T *>(a.out) + row * 2 * a.np + col;
+        *reinterpret_cast<uint4 *>(out) = p;
+        *reinterpret_cast<uint4 *>(out + a.np) = q;
     }
 }
 

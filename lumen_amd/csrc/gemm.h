@@ -432,6 +432,55 @@ __device__ __forceinline__ void stream_store_rows(const GemmShape &s, const AnyS
     }
 }
 
+// The same for row-contiguous D: where its rows do not all start on 16 bytes, the whole 16-byte chunks that lie within a row's
+// WCOLS columns with 16-byte stores, the elements before and after them (a chunk's worth a row) one at a time. All of them
+// one at a time take WCOLS stores a lane, this WCOLS / 8 + 7: the gradients of two
+// weights [12897, 443] over 12 rows 37.3 -> 23.3 us.
+template <int WCOLS, int PITCH, int ROWS = 64>
+__device__ __forceinline__ void stream_store_dense(const GemmShape &s, const AnyStore &out, int64_t od, const char *stage,
+                                                   int64_t rbase, int64_t cbase, int lane) {
+    const int64_t at = reinterpret_cast<int64_t>(out.d) + od * (out.dtype == 0 ? 4 : 2);
+    if (s.n % 8 == 0 && s.d_m % 8 == 0 && at % 16 == 0) {
+        stream_store_rows<WCOLS, PITCH, ROWS>(s, out, od, stage, rbase, cbase, lane);
+        return;
+    }
+    out.visit([&](auto stf) {
+        typedef std::remove_reference_t<decltype(*stf.d)> T;
+        constexpr int E = 16 / sizeof(T), inner = WCOLS / E - 1;
+        T *d = stf.d + od + cbase;
+        const float *sums = reinterpret_cast<const float *>(stage);
+        // the element of row gr's WCOLS columns at which its first whole chunk starts (E: an aligned row's second)
+        auto head = [&](int64_t gr) { return E - int((reinterpret_cast<uintptr_t>(d + gr * s.d_m) & 15) / sizeof(T)); };
+        auto row = [&](int r) { return sums + r * (PITCH / 4); };
+        for (int idx = lane; idx < ROWS * inner; idx += 64) {
+            const int r = idx / inner;
+            const int64_t gr = rbase + r;
+            if (gr >= s.m) continue;
+            const int c = head(gr) + idx % inner * E;
+            T v[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) store_f32_as(&v[e], row(r)[c + e]);
+            T *to = d + gr * s.d_m + c;
+            if (cbase + c + E <= s.n) {
+                uint4 w;
+                __builtin_memcpy(&w, v, 16);
+                *reinterpret_cast<uint4 *>(to) = w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (cbase + c + e < s.n) to[e] = v[e];
+            }
+        }
+        for (int idx = lane; idx < ROWS * E; idx += 64) {
+            const int r = idx / E, e = idx % E;
+            const int64_t gr = rbase + r;
+            if (gr >= s.m) continue;
+            const int h = head(gr), c = e < h ? e : WCOLS - E + e;
+            if (cbase + c < s.n) store_f32_as(d + gr * s.d_m + c, row(r)[c]);
+        }
+    });
+}
+
 // Writes the float32 sums of a wave's 64-row half `half` (MFMA tiles 2 half and 2 half + 1) to its LDS stage:
 // acc[i][j][e] is row 32 i + l32, column 32 j + 8 (e / 4) + 4 h + e % 4 of the wave's block.
 template <int FM, int FN, int PITCH>
@@ -977,7 +1026,8 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
         if constexpr (std::is_same<Out, AnyStore>::value) {
             stage_acc<FM, FN, PITCH>(acc, half, stage, l32, h);
             __syncthreads();
-            stream_store_rows<WCOLS, PITCH>(s, out, od, stage, rbase + 64 * half, cbase, lane);
+            if constexpr (PAIR >= 2) stream_store_dense<WCOLS, PITCH>(s, out, od, stage, rbase + 64 * half, cbase, lane);
+            else stream_store_rows<WCOLS, PITCH>(s, out, od, stage, rbase + 64 * half, cbase, lane);
         } else {
             constexpr int G = Out::kPrefetch < CPR ? Out::kPrefetch : CPR;
             static_assert(CPR % G == 0, "prefetch groups must divide a lane's chunks");

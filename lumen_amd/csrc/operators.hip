@@ -306,7 +306,7 @@ int gated_pad(hipStream_t st, GatedPad &p, int count, const void *const *src, co
         if (to_rows[i] > most) most = to_rows[i];
     }
     const int64_t blocks = (most * (p.kp / 8) + 255) / 256;
-    hipLaunchKernelGGL(gated_pad_kernel, dim3(unsigned(blocks < 4096 ? (blocks ? blocks : 1) : 4096)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(gated_pad_kernel, dim3(unsigned(blocks < 4096 ? (blocks ? blocks : 1) : 4096), unsigned(count)), dim3(256), 0, st, p);
     return check(hipGetLastError(), "gated_pad_kernel launch");
 }
 
@@ -366,15 +366,16 @@ int gated_grad_on(hipStream_t st, const nhip_gated_desc *d, const void *dh, cons
     if (d->m == 0 || d->n == 0) return 0;
     const int64_t np = (d->n + 7) / 8 * 8;
     GatedGrad a{dh, g, u, dgu, d->m, d->n, np, d->h_m, d->activation};
-    const bool vec = d->n % 8 == 0 && d->h_m % 8 == 0 && on(dh, 16) && on(g, 16) && on(u, 16) && on(dgu, 16);
-    const int64_t work = d->m * (vec ? np / 8 : np), blocks = (work + 255) / 256;
+    if (!on(dgu, 16)) return fail("nhip_gated_linear_grad: [dg | du] starts on 16 bytes");
+    const bool whole_rows = d->n % 8 == 0 && d->h_m % 8 == 0 && on(dh, 16) && on(g, 16) && on(u, 16);
+    const int64_t work = d->m * (np / 8), blocks = (work + 255) / 256;
     const dim3 grid(unsigned(blocks < 8192 ? blocks : 8192));
     if (d->dtype == NHIP_F16) {
-        if (vec) hipLaunchKernelGGL((gated_grad_kernel<f16_t, 8>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((gated_grad_kernel<f16_t, 1>), grid, dim3(256), 0, st, a);
+        if (whole_rows) hipLaunchKernelGGL((gated_grad_kernel<f16_t, false>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((gated_grad_kernel<f16_t, true>), grid, dim3(256), 0, st, a);
     } else {
-        if (vec) hipLaunchKernelGGL((gated_grad_kernel<bf16_t, 8>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((gated_grad_kernel<bf16_t, 1>), grid, dim3(256), 0, st, a);
+        if (whole_rows) hipLaunchKernelGGL((gated_grad_kernel<bf16_t, false>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((gated_grad_kernel<bf16_t, true>), grid, dim3(256), 0, st, a);
     }
     return check(hipGetLastError(), "gated_grad_kernel launch");
 }
