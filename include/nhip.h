@@ -272,8 +272,9 @@ int nhip_qk_norm_rope_workspace(const nhip_heads_desc *desc, size_t *bytes);
  * h [m, n] = act(x gate^T) * (x up^T) for x [m, k] and weights [n, k], bf16 or f16, contiguous along k, rows x_m and w_n
  * elements apart (both weights), h's rows h_m. The sums are float32 and rounded once, in h. g and u (both or neither):
  * float32 [m, n], the two products, which nhip_gated_linear_grad needs. Rows of a multiple of 8 elements that start on 16
- * bytes are read in place (such operands have to start there); others, above 64 rows of x, through `workspace`, of
- * nhip_gated_linear_workspace bytes from a 16-byte address. */
+ * bytes are read in place (such operands have to start there); others, above 64 rows of x, are copied. `workspace`, of
+ * nhip_gated_linear_workspace bytes from a 16-byte address, holds such copies and the sums of a product in parts (null where
+ * that is 0). k is below 2^30 up to 64 rows of x, else 1 to 2^21 - 1. */
 enum {
     NHIP_ACT_SILU = 0,
     NHIP_ACT_GELU = 1,     /* the tanh form */

@@ -9,10 +9,13 @@
 // (three roundings on the way to dx instead of two), and 16 m n bytes of traffic are 7% of the six products' time at
 // [4096, 2048] x [8192, 2048].
 //
-// Two kernels (gated_default):
+// Kernels (gated_default chooses):
 //  * gated_stream: gemm_stream_tile with PAIR 1, tiles of 256 rows x 128 columns or 128 x 64; rows that it cannot read in
 //    place (no multiple of 8 elements, off 16 bytes) are copied first (gated_pad_kernel);
+//  * gated_stream_part and gated_join_kernel: the 128 x 64 tiles over parts of k, where there are few of them;
 //  * gated_skinny: at most 64 rows, 16 columns a workgroup, the waves divide k (as gemm_skinny).
+// At [16384, 2048] x 2 [8192, 2048] 892 to 925 us by card and clock, 1.19 to 1.23 PFLOP/s, what a plain product of these sizes
+// reaches; at [16, 2048], 67 MB of weights, 13.3 us (5.1 TB/s).
 //
 // The backward's elementwise half (gated_grad_kernel) turns dh, g and u into [dg | du], one row of 2 n a token, HBM-bound:
 //   du = dh act(g), dg = dh u act'(g)
@@ -81,54 +84,83 @@ struct GatedOut {
         }
     }
 
-    // gemm_stream_tile's sums of one wave: acc[i][j] and acc[i][j + FN / 2] hold g and u of the same elements, row
-    // 32 i + l32, column 32 j + 8 (e / 4) + 4 (lane / 32) + e % 4. Through the wave's own LDS rows, 64 rows at a time, so
-    // that rows go out in 16-byte pieces; only this wave writes and reads them, which needs no barrier.
     template <int FM, int FN, int WCOLS>
     __device__ __forceinline__ void store(const GemmShape &s, const f32x16_t (&acc)[FM][FN], char *stage, int64_t rbase,
-                                          int64_t cbase, int lane) const {
-        constexpr int WC = WCOLS / 2, P = WC * 4 + 16;
-        const int l32 = lane & 31, hl = lane >> 5;
-        GemmShape full = s;  // of g and u
-        full.d_m = s.n;
-        auto out = [&](int half, auto value, const GemmShape &shape, const AnyStore &to) {
-#pragma unroll
-            for (int ii = 0; ii < 2; ++ii)
-#pragma unroll
-                for (int j = 0; j < FN / 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        const f32x16_t &g_ = acc[2 * half + ii][j], &u_ = acc[2 * half + ii][j + FN / 2];
-                        *reinterpret_cast<float4 *>(stage + (32 * ii + l32) * P + (32 * j + 2 * e + 4 * hl) * 4) =
-                            make_float4(value(g_[e], u_[e]), value(g_[e + 1], u_[e + 1]), value(g_[e + 2], u_[e + 2]),
-                                        value(g_[e + 3], u_[e + 3]));
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-            wave_order();
-            stream_store_dense<WC, P>(shape, to, 0, stage, rbase + 64 * half, cbase, lane);
-            wave_order();
-        };
-#pragma unroll
-        for (int half = 0; half < FM / 2; ++half) {
-            if (g) {
-                out(half, [](float a, float) { return a; }, full, AnyStore{g, 0});
-                out(half, [](float, float b) { return b; }, full, AnyStore{u, 0});
-            }
-            // the activation is the same for every element: its branch is taken once
-            if (act == kGatedSilu) out(half, [](float a, float b) { return gated_act(kGatedSilu, a) * b; }, s, AnyStore{h, dtype});
-            else if (act == kGatedGelu) out(half, [](float a, float b) { return gated_act(kGatedGelu, a) * b; }, s, AnyStore{h, dtype});
-            else if (act == kGatedRelu) out(half, [](float a, float b) { return gated_act(kGatedRelu, a) * b; }, s, AnyStore{h, dtype});
-            else out(half, [](float a, float b) { return gated_act(kGatedSigmoid, a) * b; }, s, AnyStore{h, dtype});
-        }
-    }
-
-    // The wave's LDS writes before its reads of them, and the other way round.
-    __device__ __forceinline__ static void wave_order() {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    }
+                                          int64_t cbase, int lane) const;
 };
+
+// The sums of part blockIdx.z of k, for gated_join_kernel: sums [parts][g, u][m, n].
+struct GatedParts {
+    float *sums;
+    template <int FM, int FN, int WCOLS>
+    __device__ __forceinline__ void store(const GemmShape &s, const f32x16_t (&acc)[FM][FN], char *stage, int64_t rbase,
+                                          int64_t cbase, int lane) const;
+};
+
+// The wave's LDS writes before its reads of them, and the other way round.
+__device__ __forceinline__ void gated_wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Stores value(g, u) of 64 rows (half `half`) of one wave's sums: acc[i][j] and acc[i][j + FN / 2] hold g and u of the same
+// elements, row 32 i + l32, column 32 j + 8 (e / 4) + 4 (lane / 32) + e % 4. Through the wave's own LDS rows, so that rows go
+// out in 16-byte pieces; only this wave writes and reads them, which needs no barrier.
+template <int FM, int FN, int WCOLS, class Value>
+__device__ __forceinline__ void gated_store_half(const f32x16_t (&acc)[FM][FN], int half, Value &&value, const GemmShape &shape,
+                                                 const AnyStore &to, char *stage, int64_t rbase, int64_t cbase, int lane) {
+    constexpr int WC = WCOLS / 2, P = WC * 4 + 16;
+    const int l32 = lane & 31, hl = lane >> 5;
+#pragma unroll
+    for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+        for (int j = 0; j < FN / 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const f32x16_t &g_ = acc[2 * half + ii][j], &u_ = acc[2 * half + ii][j + FN / 2];
+                *reinterpret_cast<float4 *>(stage + (32 * ii + l32) * P + (32 * j + 2 * e + 4 * hl) * 4) =
+                    make_float4(value(g_[e], u_[e]), value(g_[e + 1], u_[e + 1]), value(g_[e + 2], u_[e + 2]),
+                                value(g_[e + 3], u_[e + 3]));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    gated_wave_order();
+    stream_store_dense<WC, P>(shape, to, 0, stage, rbase + 64 * half, cbase, lane);
+    gated_wave_order();
+}
+
+template <int FM, int FN, int WCOLS>
+__device__ __forceinline__ void GatedOut::store(const GemmShape &s, const f32x16_t (&acc)[FM][FN], char *stage, int64_t rbase,
+                                                int64_t cbase, int lane) const {
+    GemmShape full = s;  // of g and u
+    full.d_m = s.n;
+    auto out = [&](int half, auto value, const GemmShape &shape, const AnyStore &to) {
+        gated_store_half<FM, FN, WCOLS>(acc, half, value, shape, to, stage, rbase, cbase, lane);
+    };
+#pragma unroll
+    for (int half = 0; half < FM / 2; ++half) {
+        if (g) {
+            out(half, [](float a, float) { return a; }, full, AnyStore{g, 0});
+            out(half, [](float, float b) { return b; }, full, AnyStore{u, 0});
+        }
+        // the activation is the same for every element: its branch is taken once
+        if (act == kGatedSilu) out(half, [](float a, float b) { return gated_act(kGatedSilu, a) * b; }, s, AnyStore{h, dtype});
+        else if (act == kGatedGelu) out(half, [](float a, float b) { return gated_act(kGatedGelu, a) * b; }, s, AnyStore{h, dtype});
+        else if (act == kGatedRelu) out(half, [](float a, float b) { return gated_act(kGatedRelu, a) * b; }, s, AnyStore{h, dtype});
+        else out(half, [](float a, float b) { return gated_act(kGatedSigmoid, a) * b; }, s, AnyStore{h, dtype});
+    }
+}
+
+template <int FM, int FN, int WCOLS>
+__device__ __forceinline__ void GatedParts::store(const GemmShape &s, const f32x16_t (&acc)[FM][FN], char *stage, int64_t rbase,
+                                                  int64_t cbase, int lane) const {
+    float *g = sums + int64_t(blockIdx.z) * 2 * s.m * s.n, *u = g + s.m * s.n;
+#pragma unroll
+    for (int half = 0; half < FM / 2; ++half) {
+        gated_store_half<FM, FN, WCOLS>(acc, half, [](float a, float) { return a; }, s, AnyStore{g, 0}, stage, rbase, cbase, lane);
+        gated_store_half<FM, FN, WCOLS>(acc, half, [](float, float b) { return b; }, s, AnyStore{u, 0}, stage, rbase, cbase, lane);
+    }
+}
 
 // TM x TM / 2 tiles: 256 with 8 waves and the k loop placed by hand (with 4 waves the store's 512 registers spill: [16384, 2048] x
 // [8192, 2048] 909 us, 1140), 128 with 4 waves, two workgroups a CU.
@@ -141,6 +173,35 @@ __global__ __launch_bounds__(TM * 2) __attribute__((amdgpu_waves_per_eu(ST ? 1 :
     GatedOut out) {
     extern __shared__ __align__(1024) char smem[];
     gemm_stream_tile<F16, 64, TM / 64, false, false, true, GatedOut, TM, KL, 1, ST>(s, x, gate, out, smem, up);
+}
+
+// The deep tiles over part blockIdx.z of k (k_part of its k tiles): few tiles of a long k leave CUs idle, and a tile's k loop
+// is all latency ([139, 3840] x [1464, 3840], 46 tiles: 30.1 us whole, 18.1 in 4 parts and their join).
+template <bool F16>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void gated_stream_part(
+    GemmShape s, const uint16_t *__restrict__ x, const uint16_t *__restrict__ gate, const uint16_t *__restrict__ up,
+    GatedParts out, int k_part) {
+    extern __shared__ __align__(1024) char smem[];
+    gemm_stream_tile<F16, 64, 2, false, false, true, GatedParts, 128, 1, 4, 3>(s, x, gate, out, smem, up, k_part);
+}
+
+// g and u as the sums of their parts, in order, and h of them, V elements a thread.
+template <int V>
+__global__ __launch_bounds__(256) void gated_join_kernel(GemmShape s, const float *__restrict__ sums, int parts, GatedOut out) {
+    typedef float vec __attribute__((ext_vector_type(V)));
+    const int64_t mn = s.m * s.n, per = s.n / V;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < s.m * per; i += int64_t(gridDim.x) * 256) {
+        const float *p = sums + i * V;
+        vec g = *reinterpret_cast<const vec *>(p), u = *reinterpret_cast<const vec *>(p + mn);
+#pragma unroll 4
+        for (int k = 1; k < parts; ++k) {
+            g += *reinterpret_cast<const vec *>(p + 2 * k * mn);
+            u += *reinterpret_cast<const vec *>(p + (2 * k + 1) * mn);
+        }
+        const int64_t row = i / per, col = (i - row * per) * V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) out.one(s, row, col + k, g[k], u[k]);
+    }
 }
 
 // 8 elements at p of any alignment as 4-byte words, which memory reads at full width where words at 2-byte addresses take

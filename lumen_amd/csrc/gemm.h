@@ -521,7 +521,7 @@ __device__ __forceinline__ void for_tiles(int ktiles, F &&tile) {
 // columns and the second half the second operand's same columns, so that a lane holds both of an element's sums.
 template <int PAIR, int TN, int WCOLS>
 __device__ __forceinline__ int stream_line(int wn, int j) {
-    if constexpr (PAIR == 1) return j / (WCOLS / 64) * (TN / 2) + wn * (WCOLS / 2) + 32 * (j % (WCOLS / 64));
+    if constexpr (PAIR == 1 || PAIR == 4) return j / (WCOLS / 64) * (TN / 2) + wn * (WCOLS / 2) + 32 * (j % (WCOLS / 64));
     else return wn * WCOLS + 32 * j;
 }
 
@@ -534,7 +534,7 @@ __device__ __forceinline__ int stream_line(int wn, int j) {
 // ST: the stages in LDS (0: gemm_stream_stages).
 // PAIR 1: two products of A, by B and by b2 of the same shape and strides: half of the tile's columns are B's, half the
 // same columns of b2, and out.store takes the pairs of sums. PAIR 2: the sum of two products, A's first k / 2 columns by b
-// and the others by b2, part blockIdx.z of it over k_part of the k tiles. k (k / 2) is a multiple of 8 there. PAIR 3:
+// and the others by b2, part blockIdx.z of it over k_part of the k tiles (PAIR 4: PAIR 1 in parts). k (k / 2) is a multiple of 8 there. PAIR 3:
 // one product of operands contiguous along m and n, k of any size, in parts like PAIR 2. Rows along n (and m) hold whole
 // chunks of 8 elements whatever n is. Operands are within the buffers'
 // reach.
@@ -558,8 +558,9 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     tile_of(blockIdx.x, s.tiles_m, s.tiles_n, tm, tn);
     int64_t oa, ob, od;
     batch_offsets(s, blockIdx.y, oa, ob, od);
-    static_assert(PAIR == 0 || (BUF && AT == (PAIR == 3) && BT == (PAIR >= 2) && FN % 2 == 0), "the pairs' layouts");
-    constexpr int TNB = PAIR == 1 ? TM / 2 : TM;  // columns of one B operand in the tile
+    static_assert(PAIR == 0 || (BUF && AT == (PAIR == 3) && BT == (PAIR == 2 || PAIR == 3) && FN % 2 == 0), "the pairs' layouts");
+    constexpr bool TWO = PAIR == 1 || PAIR == 4;
+    constexpr int TNB = TWO ? TM / 2 : TM;  // columns of one B operand in the tile
     const int64_t m0 = int64_t(tm) * TM, n0 = int64_t(tn) * TNB;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = wave / WN, wn = wave % WN;
@@ -568,14 +569,14 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     const int wave_u = WN == 2 ? __builtin_amdgcn_readfirstlane(wave) : wave;
     const int64_t ks = PAIR == 0 ? int64_t(blockIdx.z) * s.k : 0;  // split-k: this workgroup's first k
     od += int64_t(blockIdx.z) * s.d_split;
-    // PAIR 2 and 3: the part's first k tile; PAIR 3: the operands from its first k on
+    // PAIR 2 to 4: the part's first k tile; PAIR 3 and 4: the operands from its first k on
     const int kfirst = PAIR >= 2 ? int(blockIdx.z) * k_part : 0;
-    const int64_t kp = PAIR == 3 ? int64_t(kfirst) * BK : ks;
+    const int64_t kp = PAIR >= 3 ? int64_t(kfirst) * BK : ks;
     const uint16_t *pa = a + oa + kp * s.a_k, *pb = b + ob + kp * s.b_k;
-    const int64_t kb = PAIR == 2 ? s.k / 2 : s.k;  // k of one B operand
+    const int64_t kb = PAIR == 2 ? s.k / 2 : PAIR == 4 ? s.k - kp : s.k;  // k of one B operand
     // PAIR: k tiles of one operand, the last of them perhaps in part; a part takes k_part of all of them
     const int kth = int((kb + BK - 1) / BK);
-    const int ktiles = PAIR == 0 ? int(s.k / BK) : PAIR == 1 ? kth : min(k_part, (PAIR == 2 ? 2 * kth : kth) - kfirst);
+    const int ktiles = PAIR == 0 ? int(s.k / BK) : PAIR == 1 ? kth : min(k_part, PAIR == 4 ? kth : (PAIR == 2 ? 2 * kth : kth) - kfirst);
     const int64_t krows = PAIR == 3 ? min(s.k - kp, int64_t(k_part) * BK) : kb;
     (void)kth, (void)kfirst, (void)krows;
 
@@ -585,9 +586,9 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     // arithmetic, and rows past m / n read zeros. Operands whose tile span exceeds 2^31 bytes use 64-bit
     // global addresses instead.
     int64_t mrem = s.m - m0 < TM ? s.m - m0 : TM, nrem = s.n - n0 < TNB ? s.n - n0 : TNB;
-    if constexpr (PAIR >= 2) nrem = (nrem + 7) & ~int64_t(7);  // rows along n (and m) hold whole chunks
+    if constexpr (BT && PAIR != 0) nrem = (nrem + 7) & ~int64_t(7);  // rows along n (and m) hold whole chunks
     if constexpr (PAIR == 3) mrem = (mrem + 7) & ~int64_t(7);
-    const int64_t abytes = PAIR == 3 ? ((krows - 1) * s.a_k + mrem) * 2 : AT ? ((s.k - 1) * s.a_k + mrem) * 2 : ((mrem - 1) * s.a_m + s.k) * 2;
+    const int64_t abytes = PAIR == 3 ? ((krows - 1) * s.a_k + mrem) * 2 : AT ? ((s.k - 1) * s.a_k + mrem) * 2 : ((mrem - 1) * s.a_m + (PAIR == 4 ? kb : s.k)) * 2;
     const int64_t bbytes = PAIR == 0 ? (BT ? ((s.k - 1) * s.b_k + nrem) * 2 : ((nrem - 1) * s.b_n + s.k) * 2)
                                      : (BT ? ((krows - 1) * s.b_k + nrem) * 2 : ((nrem - 1) * s.b_n + kb) * 2);
     constexpr bool buf = BUF;  // the launcher checked stream_buffer_ok()
@@ -596,7 +597,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     const __amdgpu_buffer_rsrc_t rsb = __builtin_amdgcn_make_buffer_rsrc(
         (void *)(BT ? pb + n0 : pb + n0 * s.b_n), (short)0, int(bbytes), 0x00020000);
     const __amdgpu_buffer_rsrc_t rsb2 = __builtin_amdgcn_make_buffer_rsrc(
-        (void *)(PAIR == 0 || PAIR == 3 ? b2 : BT ? b2 + n0 : b2 + n0 * s.b_n), (short)0, int(PAIR == 0 || PAIR == 3 ? 0 : bbytes), 0x00020000);
+        (void *)(PAIR == 0 || PAIR == 3 ? b2 : BT ? b2 + n0 : b2 + n0 * s.b_n + (PAIR == 4 ? kp : 0)), (short)0, int(PAIR == 0 || PAIR == 3 ? 0 : bbytes), 0x00020000);
     (void)rsb2;
     auto issue = [&](int st, int kt, int lo, int hi) {
         char *base = smem + st * STAGE_BYTES;
@@ -644,8 +645,8 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
             const int seg = wave_u + NW * i;
             if constexpr (PAIR != 0) {
                 // PAIR 1: the upper half of a wave's segments is the second operand's
-                const bool up = PAIR == 1 ? i >= TB::segs / NW / 2 : second;
-                const int line = seg * TB::lines_per_seg + lane / TB::chunks - (PAIR == 1 && up ? TNB : 0), c = lane % TB::chunks;
+                const bool up = TWO ? i >= TB::segs / NW / 2 : second;
+                const int line = seg * TB::lines_per_seg + lane / TB::chunks - (TWO && up ? TNB : 0), c = lane % TB::chunks;
                 const int kc = (c ^ kmaj_swz<BK>(line)) << 3;  // of a line of k
                 // mn-contiguous: a line past k lies past the buffer
                 const uint32_t vo = BT ? uint32_t((line * s.b_k + ((c ^ mnmaj_swz(line)) << 3)) * 2)
@@ -1004,11 +1005,11 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
 
     // acc[i][j][e]: row m0 + wm*WR + 32 i + l32, column n0 + wn*WCOLS + 32 j + 8 (e / 4) + 4 h + e % 4.
     // Staged through LDS as float32, 64 rows of the wave at a time, then written row-wise.
-    const int64_t rbase = m0 + wm * WR, cbase = n0 + wn * (PAIR == 1 ? WCOLS / 2 : WCOLS);
+    const int64_t rbase = m0 + wm * WR, cbase = n0 + wn * (TWO ? WCOLS / 2 : WCOLS);
     constexpr int PITCH = gemm_stream_stage_pitch<WN, TM>();
     __syncthreads();  // operand stages are dead: reuse LDS for the output
     char *stage = smem + wave * (64 * PITCH);
-    if constexpr (PAIR == 1) {
+    if constexpr (TWO) {
         out.template store<FM, FN, WCOLS>(s, acc, stage, rbase, cbase, lane);
         return;
     } else {

@@ -235,7 +235,7 @@ int heads_bwd_on(hipStream_t st, const nhip_heads_desc *d, const void *q, const 
 
 namespace {
 
-enum { kSkinnyCfg = 0, kStream256, kStream128Cfg, kDeepCfg, kGatedConfigs };
+enum { kSkinnyCfg = 0, kStream256, kStream128Cfg, kDeepCfg, kPartsCfg, kGatedConfigs };
 
 int gated_check(const nhip_gated_desc *d, const char *what) {
     const std::string at(what);
@@ -257,28 +257,60 @@ bool gated_rows(const nhip_gated_desc *d) {
            stream_buffer_ok(d->m, d->n, d->k, false, false, d->x_m, 1, 1, d->w_n);
 }
 
+// Parts of k for kPartsCfg and the time that takes: the deep tiles' 5 us and 0.0065 a k, and the parts' writing and joining.
+struct GatedSplit {
+    int parts, k_part;
+    double us;
+};
+GatedSplit gated_split(const nhip_gated_desc *d) {
+    GatedSplit best{0, 0, 0.0};
+    const int64_t total = (d->k + 63) / 64, t = tiles(d->m, 128, d->n, 64);
+    for (int64_t s = 2; s <= 32; s *= 2) {
+        const int64_t part = (total + s - 1) / s, parts = (total + part - 1) / part;
+        if (best.parts && (part < 4 || t * parts > 256)) break;
+        const double us = 5.0 + 0.0065 * 64.0 * double(part) + 4.2 + 16.0 * double(parts) * double(d->m) * double(d->n) / 6.13e6;
+        if (!best.parts || us < best.us) best = GatedSplit{int(parts), int(part), us};
+    }
+    return best;
+}
+
 int gated_default(const nhip_gated_desc *d) {
+    const bool in_parts = d->k >= 1024 && gated_stream_ok(d) && tiles(d->m, 128, d->n, 64) <= 128;
     if (gated_skinny_ok(d)) {
+        if (d->m <= 32 || d->k < 768 || !gated_stream_ok(d) || !gated_rows(d)) return kSkinnyCfg;
         // 33 to 64 rows of weights that leave gated_skinny more than a workgroup a CU, which then run one after the other:
         // tiles of 128 rows are faster though half of one is empty ([64, 2048] x [8192, 2048] 19.2 us, 24.1, [64, 4096] x
         // [11008, 4096] 33.9, 64.8; of 4096 features [64, 1024] 11.8, 8.2; of 32 rows [32, 2048] x [8192, 2048] 19.2, 18.3)
-        const bool wide = d->m > 32 && d->n > 4096 && d->k >= 768 && gated_stream_ok(d) && gated_rows(d);
-        return wide ? kDeepCfg : kSkinnyCfg;
+        if (d->n > 4096) return kDeepCfg;
+        // one workgroup a CU at most: 3 us and 0.0039 (33 rows) to 0.0052 (64) a k ([64, 4096] x [1024, 4096] 23.9 us, in parts
+        // 15.5; [33, 2048] 10.3, 11.1)
+        return in_parts && gated_split(d).us < 3.0 + double(d->k) * (0.0026 + 0.00004 * double(d->m)) ? kPartsCfg : kSkinnyCfg;
     }
     if (tiles(d->m, 256, d->n, 128) >= 256) return kStream256;
-    // one workgroup a CU: 6.5 us and 0.0080 a k with three stages, 4 and 0.0115 with two
-    return tiles(d->m, 128, d->n, 64) <= 256 && d->k >= 768 ? kDeepCfg : kStream128Cfg;
+    // one workgroup a CU: three stages ([1463, 3392] x [712, 3392] 28.9 us, in two 41.2), in parts where k is long and tiles
+    // are few ([139, 3840] x [1464, 3840] 30.1 us, in parts 18.1; [500, 8192] x [2048, 8192] 60.4, 45.4; [256, 2048] x
+    // [4096, 2048] 19.5, 21.0)
+    if (tiles(d->m, 128, d->n, 64) > 256 || d->k < 768) return kStream128Cfg;
+    return in_parts && gated_split(d).us < 5.0 + 0.0065 * double(d->k) ? kPartsCfg : kDeepCfg;
+}
+
+size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+
+// Bytes of the operands' copies, which lie ahead of the parts.
+size_t gated_pad_bytes(const nhip_gated_desc *d, int cfg) {
+    if (cfg == kSkinnyCfg || gated_rows(d)) return 0;
+    return up16(size_t(d->m + 2 * d->n) * size_t((d->k + 7) / 8 * 8) * 2);
 }
 
 size_t gated_workspace(const nhip_gated_desc *d) {
     const int cfg = d->config < 0 ? gated_default(d) : d->config;
-    if (cfg == kSkinnyCfg || gated_rows(d)) return 0;
-    return size_t(d->m + 2 * d->n) * size_t((d->k + 7) / 8 * 8) * 2;
+    return gated_pad_bytes(d, cfg) + (cfg == kPartsCfg ? size_t(gated_split(d).parts) * 2 * size_t(d->m) * size_t(d->n) * 4 : 0);
 }
 
-template <class K>
+// `more`: arguments past the output; parts: blockIdx.z.
+template <class K, class Out, class... More>
 int gated_go(hipStream_t st, K kern, GemmShape s, int bm, int bn, int threads, int lds, const void *x, const void *gate,
-             const void *up, const GatedOut &out) {
+             const void *up, const Out &out, int parts = 1, More... more) {
     s.tiles_m = int((s.m + bm - 1) / bm);
     s.tiles_n = int((s.n + bn - 1) / bn);
     if ((s.m + bm - 1) / bm * ((s.n + bn - 1) / bn) > 0x7fffffff) return fail("nhip_gated_linear: too many tiles");
@@ -286,8 +318,9 @@ int gated_go(hipStream_t st, K kern, GemmShape s, int bm, int bn, int threads, i
         check(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
               "hipFuncSetAttribute"))
         return 1;
-    hipLaunchKernelGGL(kern, dim3(unsigned(s.tiles_m * s.tiles_n)), dim3(threads), lds, st, s, static_cast<const uint16_t *>(x),
-                       static_cast<const uint16_t *>(gate), static_cast<const uint16_t *>(up), out);
+    hipLaunchKernelGGL(kern, dim3(unsigned(s.tiles_m * s.tiles_n), 1, unsigned(parts)), dim3(threads), lds, st, s,
+                       static_cast<const uint16_t *>(x), static_cast<const uint16_t *>(gate), static_cast<const uint16_t *>(up),
+                       out, more...);
     return check(hipGetLastError(), "gated kernel launch");
 }
 
@@ -318,8 +351,8 @@ int gated_few(hipStream_t st, const GemmShape &s, const void *x, const void *gat
 }
 
 template <bool F16>
-int gated_run(hipStream_t st, int cfg, GemmShape s, const void *x, const void *gate, const void *up, const GatedOut &o, bool in_place,
-              void *ws) {
+int gated_run(hipStream_t st, int cfg, const nhip_gated_desc *d, GemmShape s, const void *x, const void *gate, const void *up,
+              const GatedOut &o, bool in_place, void *ws) {
     if (cfg == kSkinnyCfg) return in_place ? gated_few<F16, false>(st, s, x, gate, up, o) : gated_few<F16, true>(st, s, x, gate, up, o);
     if (!in_place) {
         GatedPad p;
@@ -329,11 +362,23 @@ int gated_run(hipStream_t st, int cfg, GemmShape s, const void *x, const void *g
         x = p.dst[0], gate = p.dst[1], up = p.dst[2];
         s.k = s.a_m = s.b_n = p.kp;
     }
+    constexpr int deep = gemm_stream_lds_bytes<64, 2, 128, 3>();
     if (cfg == kStream256)
         return gated_go(st, gated_stream<F16, 256, 3>, s, 256, 128, 512, gemm_stream_lds_bytes<64, 4>(), x, gate, up, o);
-    if (cfg == kDeepCfg)
-        return gated_go(st, gated_stream<F16, 128, 1, 3>, s, 128, 64, 256, gemm_stream_lds_bytes<64, 2, 128, 3>(), x, gate, up, o);
-    return gated_go(st, gated_stream<F16, 128, 0>, s, 128, 64, 256, gemm_stream_lds_bytes<64, 2, 128>(), x, gate, up, o);
+    if (cfg == kDeepCfg) return gated_go(st, gated_stream<F16, 128, 1, 3>, s, 128, 64, 256, deep, x, gate, up, o);
+    if (cfg == kStream128Cfg)
+        return gated_go(st, gated_stream<F16, 128, 0>, s, 128, 64, 256, gemm_stream_lds_bytes<64, 2, 128>(), x, gate, up, o);
+    const GatedSplit p = gated_split(d);
+    float *sums = reinterpret_cast<float *>(static_cast<char *>(ws) + gated_pad_bytes(d, cfg));
+    GemmShape part = s;
+    part.d_m = s.n;
+    if (gated_go(st, gated_stream_part<F16>, part, 128, 64, 256, deep, x, gate, up, GatedParts{sums}, p.parts, p.k_part)) return 1;
+    const bool vec = s.n % 4 == 0;
+    const int64_t blocks = (s.m * (vec ? s.n / 4 : s.n) + 255) / 256;
+    const dim3 grid(unsigned(blocks < 4096 ? blocks : 4096));
+    if (vec) hipLaunchKernelGGL((gated_join_kernel<4>), grid, dim3(256), 0, st, s, sums, p.parts, o);
+    else hipLaunchKernelGGL((gated_join_kernel<1>), grid, dim3(256), 0, st, s, sums, p.parts, o);
+    return check(hipGetLastError(), "gated_join_kernel launch");
 }
 
 }  // namespace
@@ -354,11 +399,11 @@ int gated_on(hipStream_t st, const nhip_gated_desc *d, const void *x, const void
     const bool in_place = rows && on(x, 16) && on(gate, 16) && on(up, 16);
     if (!in_place && cfg != kSkinnyCfg) {
         if (rows) return fail("nhip_gated_linear: operands of such rows start on 16 bytes");
-        if (!ws || !on(ws, 16)) return fail("nhip_gated_linear: no workspace, or one off 16 bytes");
     }
+    if (gated_workspace(d) && (!ws || !on(ws, 16))) return fail("nhip_gated_linear: no workspace, or one off 16 bytes");
     const GatedOut o{h, g, u, d->activation, d->dtype};
-    return d->dtype == NHIP_F16 ? gated_run<true>(st, cfg, s, x, gate, up, o, in_place, ws)
-                                : gated_run<false>(st, cfg, s, x, gate, up, o, in_place, ws);
+    return d->dtype == NHIP_F16 ? gated_run<true>(st, cfg, d, s, x, gate, up, o, in_place, ws)
+                                : gated_run<false>(st, cfg, d, s, x, gate, up, o, in_place, ws);
 }
 
 int gated_grad_on(hipStream_t st, const nhip_gated_desc *d, const void *dh, const float *g, const float *u, void *dgu) {
@@ -439,8 +484,6 @@ size_t input_grad_pad(const nhip_gated_desc *d) {
     return weights_whole(d) ? 0 : size_t(2 * whole(d->n)) * size_t(whole(d->k)) * 2;
 }
 size_t weight_grad_pad(const nhip_gated_desc *d) { return input_whole(d) ? 0 : size_t(d->m) * size_t(whole(d->k)) * 2; }
-size_t up16(size_t n) { return (n + 15) / 16 * 16; }
-
 size_t backward_workspace(const nhip_gated_desc *d) {
     const PartPlan i = input_grad_plan(d), w = weight_grad_plan(d);
     const size_t a = up16(input_grad_pad(d)) + (i.parts > 1 ? size_t(i.parts) * size_t(d->m) * size_t(d->k) * 4 : 0);

@@ -792,3 +792,23 @@ def test_gated_backward_kernels_of_many_tiles(hip, t, k, n, dtype):
     """As above where the products' launches pass one workgroup a CU: tiles of 256 whole (dx; then the weights'), tiles of 128
     in two stages (dx; then the weights'), and tiles of 256 in parts (dx)."""
     test_gated_backward_kernels(hip, t, k, n, dtype)
+
+
+@pytest.mark.parametrize("t,k,n", [(139, 2056, 72), (70, 1029, 131), (64, 4096, 40), (200, 1088, 260)])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_gated_in_parts(hip, t, k, n, dtype):
+    """Few tiles of a long k in parts, by default and by the config: k that ends inside a part's tile, odd sizes, g and u, and
+    the same bits every run."""
+    x, gate, up, dh = _gated_case(t + k, t, k, n, dtype)
+    tol, e = _gated_tolerances(x, gate, up, dh, "gelu", dtype)[0], F32 * (k + 16)
+    want = M.gated(x, gate, up, dh, "gelu")[0]
+    runs = []
+    for config in (-1, 4, 4):
+        h, g, u = _gated_abi(x, gate, up, dtype, "gelu", config, True)
+        _near(D.to_numpy_values(h[:t * n].view(D.storage(dtype)), dtype).astype(np.float64).reshape(t, n), want, tol, config)
+        for s, w in ((g, gate), (u, up)):
+            _near(s[:t * n].astype(np.float64).reshape(t, n), x @ w.T, e * (np.abs(x) @ np.abs(w).T), config)
+            assert np.all(s[t * n:] == 77.0)
+        assert np.all(h[t * n:] == 0x4242)
+        runs.append((h, g, u))
+    assert all(np.array_equal(a, b) for a, b in zip(*runs[1:]))
