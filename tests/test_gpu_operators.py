@@ -812,3 +812,55 @@ def test_gated_in_parts(hip, t, k, n, dtype):
         assert np.all(h[t * n:] == 0x4242)
         runs.append((h, g, u))
     assert all(np.array_equal(a, b) for a, b in zip(*runs[1:]))
+
+
+def test_heads_of_which_one_tensor_has_none(hip):
+    """Queries without keys' heads and keys without queries': the other's results as ever, weight gradients of zeros."""
+    for n, nkv in ((3, 0), (0, 2)):
+        x = _heads_case(40 + n, 2, 7, max(n, 1), max(nkv, 1), 64, 64, "bfloat16", positions=False)
+        want = M.heads(x, 1e-3, False)
+        empty = ("k", "gk") if nkv == 0 else ("q", "gq")
+        for m in empty:
+            x[m] = x[m][:, :, :0]
+        got = [_values(v) for v in L.compile(_heads_program(list(x), False, 1e-3), device="hip")(
+            *(_tensor(v, "float32" if m in ("cos", "sin") else "bfloat16") for m, v in x.items()))]
+        full = 0 if nkv == 0 else 1
+        rows, d = 2 * 7 * max(n, nkv), 64
+        for i in range(6):
+            if i % 2 != full:
+                assert not got[i].any() and (i >= 4 or got[i].size == 0)
+            elif i < 4:
+                _near(got[i], want[i], U["bfloat16"] * np.abs(want[i]) + F32 * (d + 40) * 8 * np.abs(want[i]).max())
+            else:
+                _near(got[i], want[i], U["bfloat16"] * np.abs(want[i]) + F32 * (rows + d + 40) * 4 * rows)
+
+
+def test_gated_of_one_axis_of_no_outputs_and_of_a_sliced_cotangent(hip):
+    """x [K] gives [F]; weights of no features give nothing and gradients of zeros; a cotangent whose rows start off 16 bytes."""
+    x, gate, up, dh = _gated_case(50, 5, 48, 40, "bfloat16")
+    tol, want = _gated_tolerances(x, gate, up, dh, "gelu", "bfloat16"), M.gated(x, gate, up, dh, "gelu")
+    one = L.compile(lambda x, gate, up: [F.gated_linear(x, gate, up, activation="gelu")], device="hip")
+    got = _values(one(_tensor(x[2], "bfloat16"), _tensor(gate, "bfloat16"), _tensor(up, "bfloat16"))[0])
+    _near(got, want[0][2], tol[0][2])
+    out = L.compile(_gated_program("silu"), device="hip")(*(_tensor(np.ones(s), "bfloat16") for s in ((70, 48), (0, 48), (0, 48), (70, 0))))
+    assert [o.shape for o in out] == [(70, 0), (70, 48), (0, 48), (0, 48)] and not _values(out[1]).any()
+    wide = np.full((5, 51), np.nan)
+    wide[:, 3:43] = dh
+
+    def fn(x, gate, up, wide):
+        h, pull = L.vjp(lambda x, gate, up: F.gated_linear(x, gate, up, activation="gelu"), x, gate, up)
+        return [h, *pull(wide[:, 3:43])]
+
+    got = L.compile(fn, device="hip")(*(_tensor(v, "bfloat16") for v in (x, gate, up, wide)))
+    for i, (a, w, t) in enumerate(zip(got, want, tol)):
+        _near(_values(a), w, t, i)
+
+
+def test_clip_of_empty_gradients_and_a_bound_that_is_infinite(hip):
+    f = L.compile(lambda *xs: (lambda c, n: [n, *c])(*F.clip_grad_norm(xs, float("inf"))), device="hip")
+    x = np.array([3.0, 4.0])
+    out = [_values(v) for v in f(_tensor(np.zeros((0, 4)), "float32"), _tensor(x, "bfloat16"), _tensor(np.zeros(0), "float16"))]
+    assert out[0] == 5.0 and np.array_equal(out[2], x) and out[1].shape == (0, 4) and out[3].shape == (0,)
+    g = L.compile(lambda x: (lambda c, n: [n, *c])(*F.clip_grad_norm([x], 1.0)), device="hip")
+    out = [_values(v) for v in g(_tensor(np.zeros((0, 4)), "float32"))]
+    assert out[0] == 0.0 and out[1].shape == (0, 4)
