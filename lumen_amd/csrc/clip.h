@@ -7,6 +7,8 @@
 // chunks of kClipChunk elements over all the tensors, which a table in the kernel's arguments maps to a tensor by
 // binary search, so many small gradients cost no more than one large one and the table needs no copy to the device.
 // The second launch walks the chunks backwards, the ones that the caches still hold first.
+// 59 bf16 gradients of 950 MB: 183 us (5.2 TB/s) and 343 us (5.5 TB/s read and written); 26 of 83 MB, which the caches hold,
+// 15.4 and 27.3; 15 of 1.3 MB 4.9 and 5.5.
 //
 // Squares are summed in float64: no gradient's square overflows or underflows, and the sum's order does not show in the
 // float32 norm. Each workgroup of the first launch leaves one sum; every workgroup of the second adds all of them up

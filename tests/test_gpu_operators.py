@@ -864,3 +864,38 @@ def test_clip_of_empty_gradients_and_a_bound_that_is_infinite(hip):
     g = L.compile(lambda x: (lambda c, n: [n, *c])(*F.clip_grad_norm([x], 1.0)), device="hip")
     out = [_values(v) for v in g(_tensor(np.zeros((0, 4)), "float32"))]
     assert out[0] == 0.0 and out[1].shape == (0, 4)
+
+
+def test_heads_of_more_rows_than_a_launch(hip):
+    """2^30 + 24 rows of one element (two launches): the last tokens' results, and weight gradients over all rows. x / |x| of
+    eps 0 is a sign, so y is the weight and dw the sum of dy; float32 sums of at most 2^17 terms a lane, then of 4096."""
+    seq, heads = (1 << 27) + 3, 8
+    rows = seq * heads
+    x, y, dy, dx = (Dev(nbytes=2 * rows) for _ in range(4))
+    nv.call("nhip_memset", C.c_void_p(x.ptr), 0x3c, C.c_size_t(2 * rows))
+    nv.call("nhip_memset", C.c_void_p(dy.ptr), 0x3c, C.c_size_t(2 * rows))
+    tail = np.random.default_rng(0).choice([-2.0, 0.5, 3.0], 24)
+    bits = np.ascontiguousarray(D.from_values(tail.astype(np.float32), "bfloat16"))
+    nv.h2d(x.ptr + 2 * (rows - 24), bits.ctypes.data, 48)
+    w, table, dw = Dev(np.array([0x4000], np.uint16)), Dev(np.zeros(4, np.float32)), Dev(nbytes=256)  # a weight of 2
+    desc = nv.HeadsDesc(batch=1, seq=seq, heads=heads, kv_heads=0, head_dim=1, rot=0, table_rows=1, dtype=1, eps=0.0)
+    for m in ("q", "oq", "dq"):
+        setattr(desc, m + "_s", heads)
+        setattr(desc, m + "_n", 1)
+    size = C.c_size_t()
+    nv.call("nhip_qk_norm_rope_workspace", C.byref(desc), C.byref(size))
+    assert size.value >= 2 * 2048 * 4
+    ws = Dev(nbytes=size.value)
+    head = [x.ptr, x.ptr, w.ptr, w.ptr, table.ptr, table.ptr, None]
+    nv.call("nhip_qk_norm_rope", C.byref(desc), *head, y.ptr, y.ptr)
+    nv.call("nhip_qk_norm_rope_bwd", C.byref(desc), *head, dy.ptr, dy.ptr, dx.ptr, dx.ptr, dw.ptr, None, ws.ptr)
+    got = np.empty(64, np.uint16)
+    for at, want in ((0, np.full(64, 2.0)), (rows - 64, np.r_[np.full(40, 2.0), 2.0 * np.sign(tail)])):
+        nv.d2h(got.ctypes.data, y.ptr + 2 * at, 128)
+        assert np.array_equal(D.to_numpy_values(got, "bfloat16"), want), at
+        nv.d2h(got.ctypes.data, dx.ptr + 2 * at, 128)
+        assert np.abs(D.to_numpy_values(got, "bfloat16").astype(np.float64)).max() <= 90 * 0.025 * 8 * F32, at
+    one = float(D.to_numpy_values(np.array([0x3c3c], np.uint16), "bfloat16")[0])
+    want = one * (rows - 24 + np.sign(tail).sum())
+    total = float(D.to_numpy_values(dw.get((1,), np.uint16), "bfloat16")[0])
+    assert abs(total - want) <= (U["bfloat16"] + 2 * (1 << 17) * F32) * want
