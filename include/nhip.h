@@ -297,12 +297,16 @@ int nhip_gated_config_count(int *count);
  * of m rows: n of dg, zeros up to a multiple of 8, n of du, zeros again. */
 int nhip_gated_linear_grad(const nhip_gated_desc *desc, const void *dh, const float *g, const float *u, void *dgu);
 /* dx [m, k] = dg gate + du up with one float32 sum over both, and d_gate, d_up [n, k] = dg^T x, du^T x, contiguous, each
- * rounded once (d_up may be null: then it is not computed); sums in a fixed order. dgu is nhip_gated_linear_grad's, from a 16-byte address; x and weights of whole
- * 16-byte rows (n, k and the strides multiples of 8) start on 16 bytes, others are copied. `workspace` of
- * nhip_gated_backward_workspace bytes (enough for either), from a 16-byte address. Weights are below 2^31 bytes. */
+ * rounded once (d_up may be null: then it is not computed); sums in a fixed order. dgu is nhip_gated_linear_grad's, from a
+ * 16-byte address; x and weights of whole 16-byte rows (n, k and the strides multiples of 8) start on 16 bytes, others are
+ * copied. `workspace` of nhip_gated_backward_workspace bytes, enough for any of the three calls, from a 16-byte address. Weights
+ * are below 2^31 bytes. nhip_gated_backward computes all of them, in one launch where nhip_gated_backward_paired says so. */
 int nhip_gated_input_grad(const nhip_gated_desc *desc, const void *dgu, const void *gate, const void *up, void *dx,
                           void *workspace);
 int nhip_gated_weight_grad(const nhip_gated_desc *desc, const void *dgu, const void *x, void *d_gate, void *d_up, void *workspace);
+int nhip_gated_backward(const nhip_gated_desc *desc, const void *dgu, const void *gate, const void *up, const void *x, void *dx,
+                        void *d_gate, void *d_up, void *workspace);
+int nhip_gated_backward_paired(const nhip_gated_desc *desc, int *paired);
 int nhip_gated_backward_workspace(const nhip_gated_desc *desc, size_t *bytes);
 
 /* ---- gradient clipping (no counterpart in the reference) -------------------------------------------------------- *
@@ -364,6 +368,7 @@ enum {
                                  5 + 2 i (or none) */
     NHIP_STEP_GATED_INPUT = 12,  /* desc: nhip_gated_desc; pointers: dgu, gate, up, dx, workspace (or none) */
     NHIP_STEP_GATED_WEIGHT = 13, /* desc: nhip_gated_desc; pointers: dgu, x, d_gate, d_up, workspace (or none) */
+    NHIP_STEP_GATED_BACKWARD = 14, /* desc: nhip_gated_desc; pointers: dgu, gate, up, x, dx, d_gate, d_up, workspace (or none) */
 };
 
 int nhip_plan_create(void **plan);

@@ -315,7 +315,7 @@ def fuse(graph: Graph, fuse_loops=True, packed=frozenset()) -> list:
                 progressed = True
         if not progressed:
             raise RuntimeError("fusion produced a cycle: " + ", ".join(s.label() for s in pending))
-    return ordered
+    return operators.pair_gradients(graph, ordered)
 
 
 REMAT = ELEMENTWISE | INDEX_ONLY | VIEWABLE

@@ -21,6 +21,8 @@ KINDS = {
     "gated_weight_grad": "gated_weight",
     "clip_grad_norm": "clip",
 }
+BOTH = "gated_both"  # a gated_weight and a gated_input step in one
+STEPS = {*KINDS.values(), BOTH}
 NHIP_DT = {"float32": 0, "bfloat16": 1, "float16": 2}
 # The last axis contiguous; and rows that start on 16 bytes, or all of a length that the library copies itself; every axis
 # contiguous; and from 16 bytes on.
@@ -42,13 +44,18 @@ def _wants(node):
     return [DENSE] * len(node.inputs)
 
 
+def _fusions(step):
+    return [n for n in step.nodes if n.prim == "fusion"]
+
+
 def layouts(steps) -> dict:
     """The layout that each value read by such a step must have (the stricter of its readers')."""
     out = {}
     for st in steps:
-        if st.kind in KINDS.values():
-            for v, want in zip(st.nodes[0].inputs, _wants(st.nodes[0])):
-                out[v] = max(want, out.get(v, ROWS), key=STRICTER.index)
+        if st.kind in STEPS:
+            for node in _fusions(st):
+                for v, want in zip(node.inputs, _wants(node)):
+                    out[v] = max(want, out.get(v, ROWS), key=STRICTER.index)
     return out
 
 
@@ -105,18 +112,45 @@ def scratch_bytes(graph, node) -> int:
     return -(-n.value // 256) * 256
 
 
-def _outputs(plan, step) -> dict:
-    """The places of the step's outputs by their index in the node's body (those that nothing reads are left out)."""
-    node = step.nodes[0]
+def pair_gradients(graph, steps) -> list:
+    """``steps`` with the weights' and the input's gradients of one gated projection as one step where the library runs
+    both in one launch and nothing between them reads the first's results."""
+    from lumen_amd import native as nv
+    from lumen_amd.compiler.fusion import Step
+
+    steps, paired = list(steps), C.c_int()
+    for weight in [st for st in steps if st.kind == "gated_weight"]:
+        node = weight.nodes[0]
+        other = next((st for st in steps if st.kind == "gated_input" and st.nodes[0].inputs[0] == node.inputs[0]), None)
+        if other is None:
+            continue
+        nv.call("nhip_gated_backward_paired", C.byref(_gated_backward_desc(graph, node)), C.byref(paired))
+        first, last = sorted((steps.index(weight), steps.index(other)))
+        if not paired.value or any(v in st.inputs for st in steps[first + 1:last + 1] for v in steps[first].outputs):
+            continue
+        both = Step(BOTH, weight.nodes + other.nodes, weight.outputs + other.outputs,
+                    weight.inputs + [v for v in other.inputs if v not in weight.inputs])
+        both.scratch = max(weight.scratch, other.scratch)
+        steps[last] = both
+        del steps[first]
+    return steps
+
+
+def _outputs(plan, step, node=None) -> dict:
+    """The places of the step's outputs by their index in the body of ``node`` (by default its first), those that nothing
+    reads left out."""
+    node = step.nodes[0] if node is None else node
     index = {n.output: n.params["index"] for n in plan.graph.nodes
              if n.prim == "fusion_output" and n.inputs[0] == node.output}
     index[node.output] = 0
-    return {index[v]: plan.loc[v] for v in step.outputs}
+    return {index[v]: plan.loc[v] for v in step.outputs if v in index}
 
 
 def lower(plan, step):
     """``(step kind, descriptor bytes, [(pointer slot, place)])`` of an operator's step."""
     name = step.nodes[0].params["name"]
+    if step.kind == BOTH:
+        return _lower_gated_both(plan, step)
     if name.startswith("qk_norm_rope"):
         return _lower_heads(plan, step)
     return {"gated_linear": _lower_gated, "gated_linear_grad": _lower_gated_grad,
@@ -193,6 +227,16 @@ def _lower_gated_backward(plan, step):
     places = [plan.loc[v] for v in node.inputs]
     places += [out[0], out.get(1)] if step.kind == "gated_weight" else [out[0]]
     return kind, bytes(_gated_backward_desc(plan.graph, node)), _slots(places + [plan.scratch.get(id(step))])
+
+
+def _lower_gated_both(plan, step):
+    from lumen_amd import native as nv
+
+    weight, given = _fusions(step)
+    dw, dx = (_outputs(plan, step, n) for n in (weight, given))
+    places = [plan.loc[v] for v in (*given.inputs, weight.inputs[1])]
+    return (nv.NHIP_STEP_GATED_BACKWARD, bytes(_gated_backward_desc(plan.graph, given)),
+            _slots(places + [dx[0], dw[0], dw.get(1), plan.scratch.get(id(step))]))
 
 
 def _lower_gated_grad(plan, step):

@@ -912,7 +912,7 @@ class Plan:
                 kind, desc, ops = attn_pass.lower(self, st)
                 rr = (nv.Reloc * len(ops))(*[reloc(i, l) for i, l in enumerate(ops)])
                 call("nhip_plan_add_builtin", plan, kind, C.byref(desc), C.sizeof(desc), rr, len(ops))
-            elif st.kind in operators.KINDS.values():
+            elif st.kind in operators.STEPS:
                 kind, desc, ops = operators.lower(self, st)
                 rr = (nv.Reloc * len(ops))(*[reloc(i, l) for i, l in ops])
                 call("nhip_plan_add_builtin", plan, kind, desc, len(desc), rr, len(ops))
@@ -1358,6 +1358,8 @@ class Plan:
         if st.kind in ("gated_input", "gated_weight"):
             dgu, other = (g.types[v] for v in st.nodes[0].inputs[:2])
             return 2 * dgu.numel() * other.shape[1], io
+        if st.kind == operators.BOTH:
+            return 4 * g.types[st.inputs[0]].numel() * g.types[st.inputs[1]].shape[1], io
         return 0, io
 
     def describe(self):

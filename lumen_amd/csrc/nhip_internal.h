@@ -37,6 +37,8 @@ int gated_input_grad_on(hipStream_t s, const nhip_gated_desc *d, const void *dgu
                         void *ws);
 int gated_weight_grad_on(hipStream_t s, const nhip_gated_desc *d, const void *dgu, const void *x, void *dgate, void *dup,
                          void *ws);
+int gated_both_grads_on(hipStream_t s, const nhip_gated_desc *d, const void *dgu, const void *gate, const void *up, const void *x,
+                        void *dx, void *dgate, void *dup, void *ws);
 int gated_grad_on(hipStream_t s, const nhip_gated_desc *d, const void *dh, const float *g, const float *u, void *dgu);
 int clip_on(hipStream_t s, const nhip_clip_desc *d, const nhip_clip_tensor *t, const double *max_at, float *norm,
             float *scale, void *ws);

@@ -433,10 +433,13 @@ namespace {
 struct PartPlan {
     int tm, parts, k_part;
     bool deep;  // at most a workgroup a CU of 128-row tiles: three stages
+    double us;
 };
+// The parts' sums, written and added, of `elements` results.
+double parts_us(int64_t elements, int64_t parts) { return parts > 1 ? 4.2 + 8.0 * double(parts) * double(elements) / 6.13e6 : 0.0; }
+
 PartPlan part_plan(int64_t m, int64_t n, int64_t z, int64_t total, int64_t longest) {
-    PartPlan best{0, 0, 0, false};
-    double least = 0;
+    PartPlan best{0, 0, 0, false, 0.0};
     if (total < 1) total = 1;  // no tokens: nothing is launched, the workspace is asked for all the same
     for (int tm : {256, 128})
         for (int s = 1; s <= 64; s *= 2) {
@@ -451,9 +454,8 @@ PartPlan part_plan(int64_t m, int64_t n, int64_t z, int64_t total, int64_t longe
             double rounds = tm == 256 ? double((t + 255) / 256) : deep ? 0.62 : double(t / 512);
             const int64_t rest = t % 512;
             if (tm == 128 && !deep) rounds += rest == 0 ? 0.0 : rest <= 256 ? 0.79 : 1.0;
-            const double us = 6.2 + 64.0 * double(part) * (tm == 256 ? 0.02355 : 0.0142) * rounds +
-                              (parts > 1 ? 4.2 + 8.0 * double(parts) * double(z * m) * double(n) / 6.13e6 : 0.0);
-            if (least == 0 || us < least) least = us, best = PartPlan{tm, int(parts), int(part), deep};
+            const double us = 6.2 + 64.0 * double(part) * (tm == 256 ? 0.02355 : 0.0142) * rounds + parts_us(z * m * n, parts);
+            if (!best.tm || us < best.us) best = PartPlan{tm, int(parts), int(part), deep, us};
         }
     return best;
 }
@@ -464,9 +466,12 @@ int64_t whole(int64_t n) { return (n + 7) / 8 * 8; }  // rounded up to 16 bytes 
 PartPlan input_grad_plan(const nhip_gated_desc *d) { return part_plan(d->m, d->k, 1, 2 * ((whole(d->n) + 63) / 64), int64_t(1) << 30); }
 
 // The weights' gradients, [n, k] each: a part's rows of [dg | du] and of x lie within 2^31 bytes.
-PartPlan weight_grad_plan(const nhip_gated_desc *d) {
+int64_t weight_grad_longest(const nhip_gated_desc *d) {
     const int64_t row = 2 * whole(d->n) > whole(d->x_m) ? 2 * whole(d->n) : whole(d->x_m);
-    return part_plan(d->n, d->k, 2, (d->m + 63) / 64, ((int64_t(1) << 30) - 1024) / (64 * (row > 0 ? row : 1)));
+    return ((int64_t(1) << 30) - 1024) / (64 * (row > 0 ? row : 1));
+}
+PartPlan weight_grad_plan(const nhip_gated_desc *d) {
+    return part_plan(d->n, d->k, 2, (d->m + 63) / 64, weight_grad_longest(d));
 }
 
 bool weights_whole(const nhip_gated_desc *d) { return d->n % 8 == 0 && d->k % 8 == 0 && d->w_n % 8 == 0; }
@@ -484,39 +489,142 @@ size_t input_grad_pad(const nhip_gated_desc *d) {
     return weights_whole(d) ? 0 : size_t(2 * whole(d->n)) * size_t(whole(d->k)) * 2;
 }
 size_t weight_grad_pad(const nhip_gated_desc *d) { return input_whole(d) ? 0 : size_t(d->m) * size_t(whole(d->k)) * 2; }
-size_t backward_workspace(const nhip_gated_desc *d) {
+// Both products in one launch of at most a workgroup a CU, each in the parts that make the longer one the shortest, where that
+// is faster than one after the other; tm 0: it is not.
+struct GradPlans {
+    PartPlan i, w;
+};
+GradPlans paired_plans(const nhip_gated_desc *d) {
+    GradPlans best;
+    std::memset(&best, 0, sizeof(best));
+    if (d->m == 0 || d->n == 0 || d->k == 0) return best;
+    const int64_t ki = 2 * ((whole(d->n) + 63) / 64), kw = (d->m + 63) / 64;
+    const int64_t ti = tiles(d->m, 128, d->k, 128), tw = 2 * tiles(d->n, 128, d->k, 128);
     const PartPlan i = input_grad_plan(d), w = weight_grad_plan(d);
-    const size_t a = up16(input_grad_pad(d)) + (i.parts > 1 ? size_t(i.parts) * size_t(d->m) * size_t(d->k) * 4 : 0);
-    const size_t b = up16(weight_grad_pad(d)) + (w.parts > 1 ? size_t(w.parts) * 2 * size_t(d->n) * size_t(d->k) * 4 : 0);
-    return a > b ? a : b;
+    if (!i.deep || !w.deep) return best;
+    double least = i.us + w.us;
+    for (int64_t a = 1; a <= 64; a *= 2)
+        for (int64_t b = 1; b <= 64; b *= 2) {
+            const int64_t pi = (ki + a - 1) / a, pw = (kw + b - 1) / b, ni = (ki + pi - 1) / pi, nw = (kw + pw - 1) / pw;
+            if (ti * ni + tw * nw > 256 || pw > weight_grad_longest(d) || (ni > 1 && pi < 4) || (nw > 1 && pw < 4)) continue;
+            const double us = 6.2 + 64.0 * double(pi > pw ? pi : pw) * 0.0142 * 0.62 + parts_us(d->m * d->k, ni) +
+                              parts_us(2 * d->n * d->k, nw);
+            if (us < least) least = us, best = GradPlans{{128, int(ni), int(pi), true, us}, {128, int(nw), int(pw), true, us}};
+        }
+    return best;
 }
 
-template <class K>
-int part_go(hipStream_t st, K kern, GemmShape s, int tm, int64_t z, const PartPlan &p, int lds, const void *a, const void *b,
-            const void *b2, const AnyStore &to, void *ws) {
-    s.tiles_m = int((s.m + tm - 1) / tm);
-    s.tiles_n = int((s.n + tm - 1) / tm);
-    if (tiles(s.m, tm, s.n, tm) > 0x7fffffff) return fail("nhip_gated_linear_grad: too many tiles");
-    GemmShape parts = s;
-    AnyStore first = to;
-    if (p.parts > 1) {
-        parts.d_m = s.n, parts.d_n = 1, parts.d_batch[0] = s.m * s.n, parts.d_split = z * s.m * s.n;
-        first = AnyStore{ws, 0};
+size_t input_grad_bytes(const nhip_gated_desc *d, const PartPlan &p) {
+    return up16(input_grad_pad(d)) + up16(p.parts > 1 ? size_t(p.parts) * size_t(d->m) * size_t(d->k) * 4 : 0);
+}
+
+size_t weight_grad_bytes(const nhip_gated_desc *d, const PartPlan &p) {
+    return up16(weight_grad_pad(d)) + up16(p.parts > 1 ? size_t(p.parts) * 2 * size_t(d->n) * size_t(d->k) * 4 : 0);
+}
+
+size_t backward_workspace(const nhip_gated_desc *d) {
+    const GradPlans both = paired_plans(d);
+    size_t most = both.i.tm ? input_grad_bytes(d, both.i) + weight_grad_bytes(d, both.w) : 0;
+    for (size_t alone : {input_grad_bytes(d, input_grad_plan(d)), weight_grad_bytes(d, weight_grad_plan(d))})
+        if (alone > most) most = alone;
+    return most;
+}
+
+// One of the backward's products, ready to be launched: z batches of s, in parts to `sums` or whole to `to`.
+struct GradProduct {
+    GemmShape s;
+    PartPlan p;
+    int64_t z;
+    const uint16_t *a, *b, *b2;
+    AnyStore to;
+    float *sums;
+
+    // What the kernel stores: the result, or the parts' sums.
+    GemmShape shape() const {
+        GemmShape q = s;
+        if (p.parts > 1) q.d_m = s.n, q.d_n = 1, q.d_batch[0] = s.m * s.n, q.d_split = z * s.m * s.n;
+        return q;
     }
-    if (check(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
-              "hipFuncSetAttribute"))
-        return 1;
-    hipLaunchKernelGGL(kern, dim3(unsigned(s.tiles_m * s.tiles_n), unsigned(z), unsigned(p.parts)), dim3(256), lds, st, parts,
-                       static_cast<const uint16_t *>(a), static_cast<const uint16_t *>(b), static_cast<const uint16_t *>(b2), first,
-                       p.k_part);
-    const int rc = check(hipGetLastError(), "gated backward launch");
-    if (rc || p.parts == 1) return rc;
-    uint16_t *out = static_cast<uint16_t *>(to.d);
-    const GatedSum g{static_cast<const float *>(ws), {out, out + s.d_batch[0]}, s.m * s.n, p.parts};
+    AnyStore store() const { return p.parts > 1 ? AnyStore{sums, 0} : to; }
+};
+
+int product_ready(GradProduct &o, const char *what) {
+    o.s.tiles_m = int((o.s.m + o.p.tm - 1) / o.p.tm);
+    o.s.tiles_n = int((o.s.n + o.p.tm - 1) / o.p.tm);
+    if (tiles(o.s.m, o.p.tm, o.s.n, o.p.tm) > 0x7fffffff) return fail(std::string(what) + ": too many tiles");
+    return 0;
+}
+
+int input_product(hipStream_t st, const nhip_gated_desc *d, const void *dgu, const void *gate, const void *up, void *dx, void *ws,
+                  const PartPlan &p, GradProduct &o) {
+    o.p = p;
+    if (!ws && input_grad_bytes(d, p)) return fail("nhip_gated_input_grad: no workspace");
+    if (!on(dgu, 16) || !on(ws, 16)) return fail("nhip_gated_input_grad: [dg | du] and the workspace start on 16 bytes");
+    if (!on(dx, 2)) return fail("nhip_gated_input_grad: the result starts on an element");
+    GemmShape &s = o.s;
+    std::memset(&s, 0, sizeof(s));
+    const int64_t np = whole(d->n);
+    s.m = d->m, s.n = d->k, s.k = 2 * np;
+    s.a_m = 2 * np, s.a_k = 1, s.b_k = d->w_n, s.b_n = 1, s.d_m = d->k, s.d_n = 1;
+    if (!weights_whole(d)) {
+        GatedPad pad;
+        const void *src[2] = {gate, up};
+        const int64_t rows[2] = {d->n, d->n}, to_rows[2] = {np, np}, ld[2] = {d->w_n, d->w_n};
+        if (gated_pad(st, pad, 2, src, rows, to_rows, ld, d->k, ws)) return 1;
+        gate = pad.dst[0], up = pad.dst[1];
+        s.b_k = pad.kp;
+    } else if (!on(gate, 16) || !on(up, 16)) {
+        return fail("nhip_gated_input_grad: weights of whole rows start on 16 bytes");
+    }
+    o.z = 1;
+    o.a = static_cast<const uint16_t *>(dgu), o.b = static_cast<const uint16_t *>(gate), o.b2 = static_cast<const uint16_t *>(up);
+    o.to = AnyStore{dx, d->dtype};
+    o.sums = reinterpret_cast<float *>(static_cast<char *>(ws) + up16(input_grad_pad(d)));
+    return product_ready(o, "nhip_gated_input_grad");
+}
+
+int weight_product(hipStream_t st, const nhip_gated_desc *d, const void *dgu, const void *x, void *dgate, void *dup, void *ws,
+                   const PartPlan &p, GradProduct &o) {
+    o.p = p;
+    if (!ws && weight_grad_bytes(d, p)) return fail("nhip_gated_weight_grad: no workspace");
+    if (!on(dgu, 16) || !on(ws, 16)) return fail("nhip_gated_weight_grad: [dg | du] and the workspace start on 16 bytes");
+    if (!on(dgate, 2) || !on(dup, 2)) return fail("nhip_gated_weight_grad: results start on an element");
+    GemmShape &s = o.s;
+    std::memset(&s, 0, sizeof(s));
+    const int64_t np = whole(d->n);
+    s.m = d->n, s.n = d->k, s.k = d->m;
+    s.a_m = 1, s.a_k = 2 * np, s.b_k = d->x_m, s.b_n = 1, s.d_m = d->k, s.d_n = 1;
+    o.z = dup ? 2 : 1;
+    s.nbatch = 1, s.batch[0] = o.z, s.a_batch[0] = np;
+    // the second result as the first one's batch, wherever it lies
+    if (dup) s.d_batch[0] = (static_cast<char *>(dup) - static_cast<char *>(dgate)) / 2;
+    if (!input_whole(d)) {
+        GatedPad pad;
+        if (gated_pad(st, pad, 1, &x, &d->m, &d->m, &d->x_m, d->k, ws)) return 1;
+        x = pad.dst[0];
+        s.b_k = pad.kp;
+    } else if (!on(x, 16)) {
+        return fail("nhip_gated_weight_grad: whole rows of x start on 16 bytes");
+    }
+    o.a = static_cast<const uint16_t *>(dgu), o.b = static_cast<const uint16_t *>(x), o.b2 = nullptr;
+    o.to = AnyStore{dgate, d->dtype};
+    o.sums = reinterpret_cast<float *>(static_cast<char *>(ws) + up16(weight_grad_pad(d)));
+    return product_ready(o, "nhip_gated_weight_grad");
+}
+
+int lds_room(const void *kern, int lds) {
+    return check(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute");
+}
+
+// The result of a product that ran in parts.
+int parts_sum(hipStream_t st, const GradProduct &o) {
+    if (o.p.parts == 1) return 0;
+    uint16_t *out = static_cast<uint16_t *>(o.to.d);
+    const GatedSum g{o.sums, {out, out + o.s.d_batch[0]}, o.s.m * o.s.n, o.p.parts};
     const bool vec = g.mn % 4 == 0 && on(g.out[0], 8) && on(g.out[1], 8);
     const int64_t blocks = ((vec ? g.mn / 4 : g.mn) + 255) / 256;
-    const dim3 grid(unsigned(blocks < 4096 ? blocks : 4096), unsigned(z));
-    if (to.dtype == NHIP_F16) {
+    const dim3 grid(unsigned(blocks < 4096 ? blocks : 4096), unsigned(o.z));
+    if (o.to.dtype == NHIP_F16) {
         if (vec) hipLaunchKernelGGL((gated_sum_kernel<f16_t, 4>), grid, dim3(256), 0, st, g);
         else hipLaunchKernelGGL((gated_sum_kernel<f16_t, 1>), grid, dim3(256), 0, st, g);
     } else {
@@ -524,6 +632,44 @@ int part_go(hipStream_t st, K kern, GemmShape s, int tm, int64_t z, const PartPl
         else hipLaunchKernelGGL((gated_sum_kernel<bf16_t, 1>), grid, dim3(256), 0, st, g);
     }
     return check(hipGetLastError(), "gated_sum_kernel launch");
+}
+
+template <class K>
+int product_go(hipStream_t st, K kern, const GradProduct &o, int lds) {
+    if (lds_room(reinterpret_cast<const void *>(kern), lds)) return 1;
+    hipLaunchKernelGGL(kern, dim3(unsigned(o.s.tiles_m * o.s.tiles_n), unsigned(o.z), unsigned(o.p.parts)), dim3(256), lds, st,
+                       o.shape(), o.a, o.b, o.b2, o.store(), o.p.k_part);
+    if (check(hipGetLastError(), "gated backward launch")) return 1;
+    return parts_sum(st, o);
+}
+
+constexpr int kGradLds256 = gemm_stream_lds_bytes<64, 2>(), kGradLds128 = gemm_stream_lds_bytes<64, 2, 128>(),
+              kGradLdsDeep = gemm_stream_lds_bytes<64, 2, 128, 3>();
+
+template <bool F16>
+int input_go(hipStream_t st, const GradProduct &o) {
+    if (o.p.tm == 256) return product_go(st, gated_input_grad<F16, 256, 0>, o, kGradLds256);
+    if (o.p.deep) return product_go(st, gated_input_grad<F16, 128, 3>, o, kGradLdsDeep);
+    return product_go(st, gated_input_grad<F16, 128, 2>, o, kGradLds128);
+}
+
+template <bool F16>
+int weight_go(hipStream_t st, const GradProduct &o) {
+    if (o.p.tm == 256) return product_go(st, gated_weight_grad<F16, 256, 0>, o, kGradLds256);
+    if (o.p.deep) return product_go(st, gated_weight_grad<F16, 128, 3>, o, kGradLdsDeep);
+    return product_go(st, gated_weight_grad<F16, 128, 2>, o, kGradLds128);
+}
+
+template <bool F16>
+int pair_go(hipStream_t st, const GradProduct &i, const GradProduct &w) {
+    auto kern = gated_both_grads<F16>;
+    if (lds_room(reinterpret_cast<const void *>(kern), kGradLdsDeep)) return 1;
+    const int ti = i.s.tiles_m * i.s.tiles_n, tw = w.s.tiles_m * w.s.tiles_n;
+    const dim3 grid(unsigned(ti > tw ? ti : tw), unsigned(w.z + 1), unsigned(i.p.parts > w.p.parts ? i.p.parts : w.p.parts));
+    const GatedHalf gi{i.shape(), i.b, i.store(), i.p.k_part, i.p.parts}, gw{w.shape(), w.b, w.store(), w.p.k_part, w.p.parts};
+    hipLaunchKernelGGL(kern, grid, dim3(256), kGradLdsDeep, st, gi, gw, i.a, i.b2);
+    if (check(hipGetLastError(), "gated_both_grads launch")) return 1;
+    return parts_sum(st, i) || parts_sum(st, w);
 }
 
 // A result of no terms.
@@ -536,73 +682,31 @@ int gated_input_grad_on(hipStream_t st, const nhip_gated_desc *d, const void *dg
     if (backward_check(d, "nhip_gated_input_grad")) return 1;
     if (d->m == 0 || d->k == 0) return 0;
     if (d->n == 0) return zero_grad(st, dx, d->m * d->k);
-    const PartPlan p = input_grad_plan(d);
-    if (!ws && (p.parts > 1 || !weights_whole(d))) return fail("nhip_gated_input_grad: no workspace");
-    if (!on(dgu, 16) || !on(ws, 16)) return fail("nhip_gated_input_grad: [dg | du] and the workspace start on 16 bytes");
-    GemmShape s;
-    std::memset(&s, 0, sizeof(s));
-    const int64_t np = whole(d->n);
-    s.m = d->m, s.n = d->k, s.k = 2 * np;
-    s.a_m = 2 * np, s.a_k = 1, s.b_k = d->w_n, s.b_n = 1, s.d_m = d->k, s.d_n = 1;
-    if (!weights_whole(d)) {
-        GatedPad pad;
-        const void *src[2] = {gate, up};
-        const int64_t rows[2] = {d->n, d->n}, to_rows[2] = {np, np}, ld[2] = {d->w_n, d->w_n};
-        if (gated_pad(st, pad, 2, src, rows, to_rows, ld, d->k, ws)) return 1;
-        gate = pad.dst[0], up = pad.dst[1];
-        s.b_k = pad.kp;
-        ws = static_cast<char *>(ws) + up16(input_grad_pad(d));
-    } else if (!on(gate, 16) || !on(up, 16)) {
-        return fail("nhip_gated_input_grad: weights of whole rows start on 16 bytes");
-    }
-    const AnyStore to{dx, d->dtype};
-    constexpr int lds256 = gemm_stream_lds_bytes<64, 2>(), lds128 = gemm_stream_lds_bytes<64, 2, 128>(),
-                  deep = gemm_stream_lds_bytes<64, 2, 128, 3>();
-    auto go = [&](auto f16) {
-        constexpr bool F16 = decltype(f16)::value;
-        if (p.tm == 256) return part_go(st, gated_input_grad<F16, 256, 0>, s, 256, 1, p, lds256, dgu, gate, up, to, ws);
-        if (p.deep) return part_go(st, gated_input_grad<F16, 128, 3>, s, 128, 1, p, deep, dgu, gate, up, to, ws);
-        return part_go(st, gated_input_grad<F16, 128, 2>, s, 128, 1, p, lds128, dgu, gate, up, to, ws);
-    };
-    return d->dtype == NHIP_F16 ? go(std::true_type{}) : go(std::false_type{});
+    GradProduct o;
+    if (input_product(st, d, dgu, gate, up, dx, ws, input_grad_plan(d), o)) return 1;
+    return d->dtype == NHIP_F16 ? input_go<true>(st, o) : input_go<false>(st, o);
 }
 
 int gated_weight_grad_on(hipStream_t st, const nhip_gated_desc *d, const void *dgu, const void *x, void *dgate, void *dup, void *ws) {
     if (backward_check(d, "nhip_gated_weight_grad")) return 1;
     if (d->n == 0 || d->k == 0) return 0;
     if (d->m == 0) return zero_grad(st, dgate, d->n * d->k) || (dup && zero_grad(st, dup, d->n * d->k));
-    const int64_t z = dup ? 2 : 1;
-    const PartPlan p = weight_grad_plan(d);
-    if (!ws && (p.parts > 1 || !input_whole(d))) return fail("nhip_gated_weight_grad: no workspace");
-    if (!on(dgu, 16) || !on(ws, 16)) return fail("nhip_gated_weight_grad: [dg | du] and the workspace start on 16 bytes");
-    if (!on(dgate, 2) || !on(dup, 2)) return fail("nhip_gated_weight_grad: results start on an element");
-    GemmShape s;
-    std::memset(&s, 0, sizeof(s));
-    const int64_t np = whole(d->n);
-    s.m = d->n, s.n = d->k, s.k = d->m;
-    s.a_m = 1, s.a_k = 2 * np, s.b_k = d->x_m, s.b_n = 1, s.d_m = d->k, s.d_n = 1;
-    s.nbatch = 1, s.batch[0] = z, s.a_batch[0] = np;
-    // the second result as the first one's batch, wherever it lies
-    if (dup) s.d_batch[0] = (static_cast<char *>(dup) - static_cast<char *>(dgate)) / 2;
-    if (!input_whole(d)) {
-        GatedPad pad;
-        if (gated_pad(st, pad, 1, &x, &d->m, &d->m, &d->x_m, d->k, ws)) return 1;
-        x = pad.dst[0];
-        s.b_k = pad.kp;
-        ws = static_cast<char *>(ws) + up16(weight_grad_pad(d));
-    } else if (!on(x, 16)) {
-        return fail("nhip_gated_weight_grad: whole rows of x start on 16 bytes");
-    }
-    const AnyStore to{dgate, d->dtype};
-    constexpr int lds256 = gemm_stream_lds_bytes<64, 2>(), lds128 = gemm_stream_lds_bytes<64, 2, 128>(),
-                  deep = gemm_stream_lds_bytes<64, 2, 128, 3>();
-    auto go = [&](auto f16) {
-        constexpr bool F16 = decltype(f16)::value;
-        if (p.tm == 256) return part_go(st, gated_weight_grad<F16, 256, 0>, s, 256, z, p, lds256, dgu, x, nullptr, to, ws);
-        if (p.deep) return part_go(st, gated_weight_grad<F16, 128, 3>, s, 128, z, p, deep, dgu, x, nullptr, to, ws);
-        return part_go(st, gated_weight_grad<F16, 128, 2>, s, 128, z, p, lds128, dgu, x, nullptr, to, ws);
-    };
-    return d->dtype == NHIP_F16 ? go(std::true_type{}) : go(std::false_type{});
+    GradProduct o;
+    if (weight_product(st, d, dgu, x, dgate, dup, ws, weight_grad_plan(d), o)) return 1;
+    return d->dtype == NHIP_F16 ? weight_go<true>(st, o) : weight_go<false>(st, o);
+}
+
+int gated_both_grads_on(hipStream_t st, const nhip_gated_desc *d, const void *dgu, const void *gate, const void *up, const void *x,
+                        void *dx, void *dgate, void *dup, void *ws) {
+    if (backward_check(d, "nhip_gated_backward")) return 1;
+    const GradPlans both = paired_plans(d);
+    if (!both.i.tm)
+        return gated_weight_grad_on(st, d, dgu, x, dgate, dup, ws) || gated_input_grad_on(st, d, dgu, gate, up, dx, ws);
+    GradProduct i, w;
+    if (input_product(st, d, dgu, gate, up, dx, ws, both.i, i)) return 1;
+    void *rest = ws ? static_cast<char *>(ws) + input_grad_bytes(d, both.i) : nullptr;
+    if (weight_product(st, d, dgu, x, dgate, dup, rest, both.w, w)) return 1;
+    return d->dtype == NHIP_F16 ? pair_go<true>(st, i, w) : pair_go<false>(st, i, w);
 }
 
 // ---- gradient clipping ----------------------------------------------------------------------------------
@@ -714,6 +818,18 @@ int nhip_gated_input_grad(const nhip_gated_desc *desc, const void *dgu, const vo
 int nhip_gated_weight_grad(const nhip_gated_desc *desc, const void *dgu, const void *x, void *d_gate, void *d_up, void *workspace) {
     NHIP_STREAM(st);
     return gated_weight_grad_on(st, desc, dgu, x, d_gate, d_up, workspace);
+}
+
+int nhip_gated_backward(const nhip_gated_desc *desc, const void *dgu, const void *gate, const void *up, const void *x, void *dx,
+                        void *d_gate, void *d_up, void *workspace) {
+    NHIP_STREAM(st);
+    return gated_both_grads_on(st, desc, dgu, gate, up, x, dx, d_gate, d_up, workspace);
+}
+
+int nhip_gated_backward_paired(const nhip_gated_desc *desc, int *paired) {
+    if (backward_check(desc, "nhip_gated_backward_paired")) return 1;
+    *paired = paired_plans(desc).i.tm != 0;
+    return 0;
 }
 
 int nhip_gated_backward_workspace(const nhip_gated_desc *desc, size_t *bytes) {

@@ -470,7 +470,7 @@ int nhip_plan_add_launch(void *plan, void *function, const uint32_t grid[3], con
 
 int nhip_plan_add_builtin(void *plan, int kind, const void *desc, size_t desc_bytes, const nhip_reloc *relocs,
                           size_t nrelocs) {
-    if (kind < NHIP_STEP_GEMM || kind > NHIP_STEP_GATED_WEIGHT) return fail("nhip_plan_add_builtin: unknown step kind");
+    if (kind < NHIP_STEP_GEMM || kind > NHIP_STEP_GATED_BACKWARD) return fail("nhip_plan_add_builtin: unknown step kind");
     // the descriptor must hold what run_steps reads for the kind
     size_t need = 0, pointers = 16;
     switch (kind) {
@@ -485,7 +485,8 @@ int nhip_plan_add_builtin(void *plan, int kind, const void *desc, size_t desc_by
         case NHIP_STEP_GATED:
         case NHIP_STEP_GATED_GRAD:
         case NHIP_STEP_GATED_INPUT:
-        case NHIP_STEP_GATED_WEIGHT: need = sizeof(nhip_gated_desc); break;
+        case NHIP_STEP_GATED_WEIGHT:
+        case NHIP_STEP_GATED_BACKWARD: need = sizeof(nhip_gated_desc); break;
         case NHIP_STEP_CLIP: {
             need = sizeof(nhip_clip_desc);
             if (desc && desc_bytes >= need) {
@@ -679,6 +680,10 @@ static int run_steps(Plan *plan, void *workspace, void *const *inputs, size_t ni
             case NHIP_STEP_GATED_WEIGHT:
                 rc = gated_weight_grad_on(s, reinterpret_cast<const nhip_gated_desc *>(st.args.data()), ptrs[0], ptrs[1],
                                           ptrs[2], ptrs[3], ptrs[4]);
+                break;
+            case NHIP_STEP_GATED_BACKWARD:
+                rc = gated_both_grads_on(s, reinterpret_cast<const nhip_gated_desc *>(st.args.data()), ptrs[0], ptrs[1], ptrs[2],
+                                         ptrs[3], ptrs[4], ptrs[5], ptrs[6], ptrs[7]);
                 break;
             case NHIP_STEP_GATED_GRAD:
                 rc = gated_grad_on(s, reinterpret_cast<const nhip_gated_desc *>(st.args.data()), ptrs[0],

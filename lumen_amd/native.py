@@ -18,7 +18,7 @@ NHIP_F32, NHIP_BF16, NHIP_F16 = 0, 1, 2
 NHIP_BASE_WORKSPACE, NHIP_BASE_INPUT = 0, 1
 NHIP_STEP_GEMM, NHIP_STEP_FLASH_FWD, NHIP_STEP_FLASH_BWD, NHIP_STEP_COPY, NHIP_STEP_FILL, NHIP_STEP_LCE = 1, 2, 3, 4, 5, 6
 NHIP_STEP_HEADS, NHIP_STEP_HEADS_BWD, NHIP_STEP_GATED, NHIP_STEP_GATED_GRAD, NHIP_STEP_CLIP = 7, 8, 9, 10, 11
-NHIP_STEP_GATED_INPUT, NHIP_STEP_GATED_WEIGHT = 12, 13
+NHIP_STEP_GATED_INPUT, NHIP_STEP_GATED_WEIGHT, NHIP_STEP_GATED_BACKWARD = 12, 13, 14
 NHIP_LCE_I32, NHIP_LCE_I64 = 0, 1
 NHIP_POS_NONE, NHIP_POS_I32, NHIP_POS_I64 = 0, 1, 2
 NHIP_ACT = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
@@ -178,6 +178,8 @@ SIGNATURES = {
     "nhip_gated_linear_workspace": ([C.POINTER(GatedDesc), C.POINTER(C.c_size_t)], C.c_int),
     "nhip_gated_input_grad": ([C.POINTER(GatedDesc)] + [C.c_void_p] * 5, C.c_int),
     "nhip_gated_weight_grad": ([C.POINTER(GatedDesc)] + [C.c_void_p] * 5, C.c_int),
+    "nhip_gated_backward": ([C.POINTER(GatedDesc)] + [C.c_void_p] * 8, C.c_int),
+    "nhip_gated_backward_paired": ([C.POINTER(GatedDesc), C.POINTER(C.c_int)], C.c_int),
     "nhip_gated_backward_workspace": ([C.POINTER(GatedDesc), C.POINTER(C.c_size_t)], C.c_int),
     "nhip_gated_config_count": ([C.POINTER(C.c_int)], C.c_int),
     "nhip_gated_linear_grad": ([C.POINTER(GatedDesc)] + [C.c_void_p] * 4, C.c_int),

@@ -899,3 +899,41 @@ def test_heads_of_more_rows_than_a_launch(hip):
     want = one * (rows - 24 + np.sign(tail).sum())
     total = float(D.to_numpy_values(dw.get((1,), np.uint16), "bfloat16")[0])
     assert abs(total - want) <= (U["bfloat16"] + 2 * (1 << 17) * F32) * want
+
+
+@pytest.mark.parametrize("t,k,n,dtype,paired", [(777, 520, 1416, "float16", True), (130, 67, 333, "bfloat16", True), (5, 1, 9, "bfloat16", True),
+                                                (65, 1153, 2304, "bfloat16", False), (17, 128, 1344, "float16", True),
+                                                (1500, 70, 72, "bfloat16", True)])
+def test_gated_gradients_in_one_call(hip, t, k, n, dtype, paired):
+    """dx and the weights' gradients together, with and without d_up, the same bits each time, nothing written behind them."""
+    whole = -(-n // 8) * 8
+    x, gate, up, _ = _gated_case(t + k, t, k, n, dtype)
+    rng = np.random.default_rng(t)
+    dg, du = (_round(rng.standard_normal((t, n)), dtype) for _ in range(2))
+    dgu = np.zeros((t, 2 * whole))
+    dgu[:, :n], dgu[:, whole:whole + n] = dg, du
+    dev = [Dev(np.ascontiguousarray(D.from_values(np.asarray(v, np.float32), dtype))) for v in (dgu, gate, up, x)]
+    desc = nv.GatedDesc(m=t, n=n, k=k, x_m=k, w_n=k, dtype={"bfloat16": 1, "float16": 2}[dtype], config=-1)
+    size, flag = C.c_size_t(), C.c_int()
+    nv.call("nhip_gated_backward_workspace", C.byref(desc), C.byref(size))
+    nv.call("nhip_gated_backward_paired", C.byref(desc), C.byref(flag))
+    assert bool(flag.value) == paired
+    ws = Dev(np.full(size.value + 256, 0x42, np.uint8))
+    place = ws.ptr if size.value else None
+    shapes = [(t, k), (n, k), (n, k)]
+    runs = []
+    for with_up in (True, False, True):
+        outs = [Dev(np.full(a * b + 64, 0x4242, np.uint16)) for a, b in shapes]
+        nv.call("nhip_gated_backward", C.byref(desc), *(v.ptr for v in dev), outs[0].ptr, outs[1].ptr,
+                outs[2].ptr if with_up else None, place)
+        runs.append([o.get((a * b + 64,), np.uint16) for o, (a, b) in zip(outs, shapes)])
+    assert all(np.array_equal(a, b) for a, b in zip(runs[0], runs[2]))
+    assert all(np.array_equal(a, b) for a, b in zip(runs[0][:2], runs[1][:2])) and np.all(runs[1][2] == 0x4242)
+    mags = np.abs(dg) @ np.abs(gate) + np.abs(du) @ np.abs(up)
+    want = [(dg @ gate + du @ up, (2 * n + 16) * mags)]
+    want += [(d.T @ x, (t + 16) * (np.abs(d).T @ np.abs(x))) for d in (dg, du)]
+    for raw, (a, b), (w, roundings) in zip(runs[0], shapes, want):
+        assert np.all(raw[a * b:] == 0x4242)
+        got = D.to_numpy_values(raw[:a * b].view(D.storage(dtype)), dtype).astype(np.float64).reshape(a, b)
+        _near(got, w, U[dtype] * np.abs(w) + F32 * roundings)
+    assert np.all(ws.get((size.value + 256,), np.uint8)[size.value:] == 0x42)

@@ -416,3 +416,21 @@ def test_clipped_gradients_scale_in_the_update_that_reads_them():
     xs = [D.bf16_bits(rng.standard_normal(s).astype(np.float32)) for s in ((8, 16), (5,), (8, 16), (5,))]
     for a, b in zip(oracle.run(g, xs), oracle.run(plan.graph, xs)):
         assert np.array_equal(a, b)
+
+
+def test_gradients_of_few_tiles_are_one_step():
+    """Few tiles: one step of all three gradients; many, or an input that needs none: the products' own steps."""
+    def plan(t, k, n, leaves):
+        def fn(x, gate, up, dh):
+            h, pull = L.vjp(lambda *w: F.gated_linear(*(w if leaves == 3 else (x, *w))), *(x, gate, up)[3 - leaves:])
+            return [h, *pull(dh)]
+
+        return Plan(L.make_graph(fn)(*(_m(s) for s in ((t, k), (n, k), (n, k), (t, n)))), build_kernels=False)
+
+    assert [st.kind for st in plan(777, 520, 1416, 3).steps] == ["gated_fwd", "gated_grad", "gated_both"]
+    assert [st.kind for st in plan(777, 520, 1416, 2).steps] == ["gated_fwd", "gated_grad", "gated_weight"]
+    assert [st.kind for st in plan(4001, 2048, 8192, 3).steps] == ["gated_fwd", "gated_grad", "gated_weight", "gated_input"]
+    steps = plan(130, 67, 333, 3).steps
+    n = C.c_size_t()
+    nv.call("nhip_gated_backward_workspace", C.byref(nv.GatedDesc(m=130, n=333, k=67, x_m=67, w_n=67, dtype=1, config=-1)), C.byref(n))
+    assert steps[-1].kind == "gated_both" and steps[-1].scratch >= n.value
