@@ -125,7 +125,7 @@ def pair_gradients(graph, steps) -> list:
         if other is None:
             continue
         nv.call("nhip_gated_backward_paired", C.byref(_gated_backward_desc(graph, node)), C.byref(paired))
-        first, last = sorted((steps.index(weight), steps.index(other)))
+        first, last = (i for i, st in enumerate(steps) if st is weight or st is other)
         if not paired.value or any(v in st.inputs for st in steps[first + 1:last + 1] for v in steps[first].outputs):
             continue
         both = Step(BOTH, weight.nodes + other.nodes, weight.outputs + other.outputs,
