@@ -165,7 +165,7 @@ __device__ __forceinline__ HeadsRow heads_row(const HeadsArgs &a, const HeadsTen
     const uint32_t k = t.heads.div(row);
     r.h = row - k * t.heads.d;
     r.token = a.token0 + k;
-    // token0 is a multiple of seq, or the launch lies within one sequence that starts at token0 - token0 % seq
+    // below 2^31: seq is below 2^30, a launch's tokens below 2^26
     const uint32_t first = uint32_t(a.token0 % a.seq);
     const uint32_t q = a.seq_div.div(first + k);
     r.b = a.token0 / a.seq + q;

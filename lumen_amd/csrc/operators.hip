@@ -15,7 +15,7 @@ bool on(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % b
 
 // ---- heads ----------------------------------------------------------------------------------------------
 
-constexpr int64_t kHeadsLaunchRows = int64_t(1) << 30;  // heads of a launch: row arithmetic is 32-bit
+constexpr int64_t kHeadsLaunchRows = int64_t(1) << 25;  // heads of a launch: 64 lanes of each stay within 2^32 threads
 // Workgroups of a backward launch at most: each leaves a row of partial sums that is read again. Two rounds of the three
 // that fit a CU with chunks of 8 elements, 2048 otherwise ([4, 4096, 16 + 16, 128] in chunks of 4: 1536 101 us, 2048 88,
 // 4096 87, whose sums take 2 us longer).

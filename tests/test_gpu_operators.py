@@ -937,3 +937,40 @@ def test_gated_gradients_in_one_call(hip, t, k, n, dtype, paired):
         got = D.to_numpy_values(raw[:a * b].view(D.storage(dtype)), dtype).astype(np.float64).reshape(a, b)
         _near(got, w, U[dtype] * np.abs(w) + F32 * roundings)
     assert np.all(ws.get((size.value + 256,), np.uint8)[size.value:] == 0x42)
+
+
+def test_heads_of_several_launches_in_sequences_that_end_inside_them(hip):
+    """3 sequences of 2^24 + 1 heads of 4 elements: launches end inside a sequence and start there again. Both directions at
+    the tokens around every boundary, positions past the table clamped."""
+    batch, seq, d, table = 3, (1 << 24) + 1, 4, 64
+    rows = batch * seq
+    rng = np.random.default_rng(3)
+    part = _round(rng.standard_normal((10007, d)) + 2, "bfloat16")
+    dpart = _round(rng.standard_normal((10007, d)), "bfloat16")
+    dev = [Dev(np.resize(D.from_values(p.astype(np.float32), "bfloat16"), (rows, d))) for p in (part, dpart)]
+    y, dx = Dev(nbytes=rows * d * 2), Dev(nbytes=rows * d * 2)
+    angle = np.arange(table)[:, None] * np.array([0.1, 0.03])
+    cos, sin = (f(angle).astype(np.float32) for f in (np.cos, np.sin))
+    dcos, dsin, w, dw = Dev(cos), Dev(sin), Dev(np.array([0x4000] * d, np.uint16)), Dev(nbytes=256)  # weights of 2
+    desc = nv.HeadsDesc(batch=batch, seq=seq, heads=1, kv_heads=0, head_dim=d, rot=d, table_rows=table, dtype=1, eps=1e-3)
+    for m in ("q", "oq", "dq"):
+        for axis, stride in (("b", seq * d), ("s", d), ("n", d)):
+            setattr(desc, f"{m}_{axis}", stride)
+    size = C.c_size_t()
+    nv.call("nhip_qk_norm_rope_workspace", C.byref(desc), C.byref(size))
+    ws = Dev(nbytes=size.value)
+    head = [dev[0].ptr, dev[0].ptr, w.ptr, w.ptr, dcos.ptr, dsin.ptr, None]
+    nv.call("nhip_qk_norm_rope", C.byref(desc), *head, y.ptr, y.ptr)
+    nv.call("nhip_qk_norm_rope_bwd", C.byref(desc), *head, dev[1].ptr, dev[1].ptr, dx.ptr, dx.ptr, dw.ptr, None, ws.ptr)
+    for at in (0, seq - 40, seq + 20, 1 << 25, (1 << 25) - 80, 2 * seq - 40, rows - 80):
+        token = np.arange(at, at + 80)
+        s = token % seq
+        x = {"q": part[token % 10007].reshape(1, 80, 1, d), "k": np.zeros((1, 80, 0, d)), "wq": np.full(d, 2.0), "wk": np.full(d, 2.0),
+             "cos": cos.astype(np.float64), "sin": sin.astype(np.float64), "positions": np.minimum(s, table - 1).reshape(1, 80),
+             "gq": dpart[token % 10007].reshape(1, 80, 1, d), "gk": np.zeros((1, 80, 0, d))}
+        want = M.heads(x, 1e-3, False)
+        for buf, i in ((y, 0), (dx, 2)):
+            got = np.empty((80, d), np.uint16)
+            nv.d2h(got.ctypes.data, buf.ptr + at * d * 2, got.nbytes)
+            ref = want[i].reshape(80, d)
+            _near(D.to_numpy_values(got, "bfloat16").astype(np.float64), ref, U["bfloat16"] * np.abs(ref) + F32 * (d + 40) * 8 * np.abs(ref).max(), at)
