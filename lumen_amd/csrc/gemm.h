@@ -534,10 +534,9 @@ __device__ __forceinline__ int stream_line(int wn, int j) {
 // ST: the stages in LDS (0: gemm_stream_stages).
 // PAIR 1: two products of A, by B and by b2 of the same shape and strides: half of the tile's columns are B's, half the
 // same columns of b2, and out.store takes the pairs of sums. PAIR 2: the sum of two products, A's first k / 2 columns by b
-// and the others by b2, part blockIdx.z of it over k_part of the k tiles (PAIR 4: PAIR 1 in parts). k (k / 2) is a multiple of 8 there. PAIR 3:
-// one product of operands contiguous along m and n, k of any size, in parts like PAIR 2. Rows along n (and m) hold whole
-// chunks of 8 elements whatever n is. Operands are within the buffers'
-// reach.
+// and the others by b2, part blockIdx.z of it over k_part of the k tiles. PAIR 3: one product of operands contiguous along m
+// and n, in parts like PAIR 2. PAIR 4: PAIR 1 in parts. k (PAIR 2: k / 2) is a multiple of 8, with PAIR 3 any number; rows
+// along n (and m) hold whole chunks of 8 elements whatever n is. Operands are within the buffers' reach.
 template <bool F16, int BK, int WN, bool AT, bool BT, bool BUF, class Out, int TM = 256, int KL = 0, int PAIR = 0, int ST = 0>
 __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint16_t *__restrict__ a,
                                                  const uint16_t *__restrict__ b, const Out &out, char *smem,

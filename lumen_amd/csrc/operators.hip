@@ -98,7 +98,8 @@ HeadsBlocks heads_blocks(const nhip_heads_desc *d, int lanes, int64_t cap) {
     auto share = [&](int64_t rows) -> int64_t {
         if (rows == 0) return 0;
         const int64_t need = (rows + groups - 1) / groups, part = 256 * rows / (q + k) + 1;
-        const int64_t want = need / 4 > part ? need / 4 : (need < part ? need : part), most = cap * rows / (q + k);  // both within the cap: one workgroup over it is a round
+        const int64_t want = need / 4 > part ? need / 4 : (need < part ? need : part);
+        const int64_t most = cap * rows / (q + k);  // both within the cap: one workgroup over it is another round
         return want < most ? want : most > 0 ? most : 1;
     };
     return {share(q), share(k)};
