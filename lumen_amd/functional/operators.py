@@ -6,6 +6,9 @@ Each is defined by elementary primitives. Where the hip kernels take its dtypes 
 body, which the plan runs as a built-in step and the oracle evaluates as written; elsewhere, and with
 ``config.compiler.fused_operators`` off, it holds the primitives themselves. The reference has no counterpart: its
 programs write these out.
+
+A tape sees neither: both directions are a ``Function`` each, whose forward runs with the tapes paused. A gradient is
+differentiated again through the primitives that define it (``_second``).
 """
 
 from __future__ import annotations
@@ -27,7 +30,11 @@ ACTIVATIONS = ("silu", "gelu", "relu", "sigmoid")
 
 
 def _fused(name, operands, body, **params):
-    """One ``fusion`` called ``name`` of ``operands``, its body what ``body(*operands)`` traces; the body's results."""
+    """One ``fusion`` called ``name`` of ``operands``, its body what ``body(*operands)`` traces; the body's results. Only
+    within a ``Function``'s forward: an open tape would take the body's nodes, whose values are of another graph, and no
+    tape takes the fusion."""
+    if tracer._TAPES:
+        raise RuntimeError(f"{name}: a fusion is traced with the tapes paused")
     graph = tracer.current_graph()
     inner = Graph()
     inputs = [TracedTensor(inner, inner.input(x.dtype, x.shape)) for x in operands]
@@ -46,6 +53,24 @@ def _operator(name, taken, operands, body, **params):
     if taken and config.compiler.fused_operators:
         return _fused(name, operands, body, **params)
     return tuple(body(*operands))
+
+
+def _second(grads, primals, cotangents):
+    """The cotangents of ``primals`` (None where there is none) for those of ``grads(*primals)``'s results."""
+    from lumen_amd.autograd.transforms import vjp
+
+    used = [p for p in primals if p is not None]
+    first = {}  # one leaf a value: of a value passed twice the first has the sum
+    for p in used:
+        first.setdefault(p.var, p)
+
+    def by_leaf(*leaves):
+        at = dict(zip(first, leaves))
+        return grads(*(None if p is None else at[p.var] for p in primals))
+
+    _, pullback = vjp(by_leaf, *first.values())
+    back = dict(zip(first, pullback(tuple(cotangents))))
+    return [None if p is None else back.pop(p.var, None) for p in primals]
 
 
 # ---- norms and rotation of heads ------------------------------------------------------------------------
@@ -77,9 +102,11 @@ def _rows(table, positions, b, s):
     return prims.gather(table, positions, 0).reshape(b, s, 1, table.shape[1])
 
 
-def _normed(x, acc, eps):
+def _normed(x, acc, eps, rules=False):
+    """``x`` over its root mean square and one over that, which ``rules`` makes of primitives with gradient rules."""
     h = x.to(acc)
-    inv = prims.rsqrt(F.mean(h * h, -1, keepdim=True) + eps)
+    square = F.mean(h * h, -1, keepdim=True) + eps
+    inv = 1.0 / prims.sqrt(square) if rules else prims.rsqrt(square)
     return h * broadcast_to(inv, h.shape), inv
 
 
@@ -113,31 +140,53 @@ class _QKNormRope(Function):
 
     @staticmethod
     def backward(ctx, gq, gk):
-        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
-        eps, interleaved = ctx.eps, ctx.interleaved
-        operands, roles = _heads_operands(q, k, wq, wk, cos, sin, positions)
-        b, s = q.shape[:2]
-
-        def body(*xs):
-            x = dict(zip(roles + ("gq", "gk"), xs))
-            acc = accum_dtype(q.dtype)
-            c, n = (_rows(x[t], x.get("positions"), b, s).to(acc) for t in ("cos", "sin"))
-            dx, dw = [], []
-            for h, w, g in (("q", "q_weight", "gq"), ("k", "k_weight", "gk")):
-                xhat, inv = _normed(x[h], acc, eps)
-                dz = _turn(x[g].to(acc), c, -n, interleaved)
-                dxhat = dz * _expand(x[w], dz) if w in x else dz
-                m = broadcast_to(F.mean(dxhat * xhat, -1, keepdim=True), xhat.shape)
-                dx.append((broadcast_to(inv, xhat.shape) * (dxhat - xhat * m)).to(q.dtype))
-                if w in x:
-                    dw.append(F.sum(dz * xhat, (0, 1, 2)).to(q.dtype))
-            return dx + dw
-
-        out = _operator("qk_norm_rope_backward", _heads_taken(q, k), operands + [gq, gk], body, roles=roles + ("gq", "gk"),
-                        eps=float(eps), interleaved=bool(interleaved))
+        _, _, wq, wk, *_ = ctx.saved_tensors
+        out = _QKNormRopeGradients.apply(gq, gk, *ctx.saved_tensors, eps=ctx.eps, interleaved=ctx.interleaved)
         dw = iter(out[2:])
         return (out[0], out[1], next(dw) if wq is not None else None, next(dw) if wk is not None else None,
                 None, None, None)
+
+
+class _QKNormRopeGradients(Function):
+    """The heads' gradients and, where there are weights, theirs."""
+
+    @staticmethod
+    def forward(ctx, gq, gk, q, k, wq, wk, cos, sin, positions, *, eps, interleaved):
+        ctx.eps, ctx.interleaved = eps, interleaved
+        ctx.save_for_backward(gq, gk, q, k, wq, wk, cos, sin, positions)
+        operands, roles = _heads_operands(q, k, wq, wk, cos, sin, positions)
+        operands, roles = operands + [gq, gk], roles + ("gq", "gk")
+        return _operator("qk_norm_rope_backward", _heads_taken(q, k), operands,
+                         lambda *xs: _heads_gradients(dict(zip(roles, xs)), eps, interleaved), roles=roles,
+                         eps=float(eps), interleaved=bool(interleaved))
+
+    @staticmethod
+    def backward(ctx, *cotangents):
+        gq, gk, q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
+
+        def grads(gq, gk, q, k, wq, wk):
+            operands, roles = _heads_operands(q, k, wq, wk, cos, sin, positions)
+            return tuple(_heads_gradients({**dict(zip(roles, operands)), "gq": gq, "gk": gk}, ctx.eps, ctx.interleaved, rules=True))
+
+        return (*_second(grads, (gq, gk, q, k, wq, wk), cotangents), None, None, None)
+
+
+def _heads_gradients(x, eps, interleaved, rules=False):
+    """``[dq, dk]`` and the gradients of the weights that there are, from the operands by role."""
+    q = x["q"]
+    b, s = q.shape[:2]
+    acc = accum_dtype(q.dtype)
+    c, n = (_rows(x[t], x.get("positions"), b, s).to(acc) for t in ("cos", "sin"))
+    dx, dw = [], []
+    for h, w, g in (("q", "q_weight", "gq"), ("k", "k_weight", "gk")):
+        xhat, inv = _normed(x[h], acc, eps, rules)
+        dz = _turn(x[g].to(acc), c, -n, interleaved)
+        dxhat = dz * _expand(x[w], dz) if w in x else dz
+        m = broadcast_to(F.mean(dxhat * xhat, -1, keepdim=True), xhat.shape)
+        dx.append((broadcast_to(inv, xhat.shape) * (dxhat - xhat * m)).to(q.dtype))
+        if w in x:
+            dw.append(F.sum(dz * xhat, (0, 1, 2)).to(q.dtype))
+    return dx + dw
 
 
 def _heads_operands(q, k, wq, wk, cos, sin, positions):
@@ -242,10 +291,8 @@ class _GatedLinear(Function):
 
     @staticmethod
     def forward(ctx, x, gate, up, *, activation):
-        acc = accum_dtype(x.dtype)
-
         def body(x, gate, up):
-            g, u = (dot(x, w, (((1,), (1,)), ((), ())), acc, acc) for w in (gate, up))
+            g, u = _gated_products(x, gate, up)
             return [(_activated(activation, g) * u).to(x.dtype), g, u]
 
         h, g, u = _operator("gated_linear", _gated_taken(x), [x, gate, up], body, activation=activation)
@@ -255,35 +302,68 @@ class _GatedLinear(Function):
 
     @staticmethod
     def backward(ctx, dh):
-        x, gate, up, g, u = ctx.saved_tensors
-        (t, k), n, acc, dtype = x.shape, gate.shape[0], accum_dtype(x.dtype), x.dtype
+        return _GatedGradients.apply(dh, *ctx.saved_tensors, activation=ctx.activation)
+
+
+def _gated_products(x, gate, up):
+    acc = accum_dtype(x.dtype)
+    return tuple(dot(x, w, (((1,), (1,)), ((), ())), acc, acc) for w in (gate, up))
+
+
+class _GatedGradients(Function):
+    """``(dx, dgate, dup)``: ``[dg | du]`` of the elements, then the products."""
+
+    @staticmethod
+    def forward(ctx, dh, x, gate, up, g, u, *, activation):
+        ctx.activation = activation
+        ctx.save_for_backward(dh, x, gate, up)
+        (t, k), n = x.shape, gate.shape[0]
         whole = -(-n // 8) * 8  # each half of [dg | du] in whole 16-byte chunks
-
-        def grad(dh, g, u):
-            a, da = _activated_grad(ctx.activation, g)
-            d = dh.to(acc)
-            halves = [(d * u * da).to(dtype), (d * a).to(dtype)]
-            if whole != n:
-                pad = prims.full((t, whole - n), 0.0, dtype)
-                halves = [halves[0], pad, halves[1], pad]
-            return [F.cat(halves, 1)]
-
-        def input_grad(dgu, gate, up):
-            dims = (((1,), (0,)), ((), ()))
-            return [(prims.dot_general(dgu[:, :n], gate, dims, acc)
-                     + prims.dot_general(dgu[:, whole:whole + n], up, dims, acc)).to(dtype)]
-
-        def weight_grad(dgu, x):
-            return [dot(dgu[:, lo:lo + n], x, (((0,), (0,)), ((), ())), acc, dtype) for lo in (0, whole)]
-
         taken = _gated_taken(x)
-        (dgu,) = _operator("gated_linear_grad", taken, [dh, g, u], grad, activation=ctx.activation)
+        (dgu,) = _operator("gated_linear_grad", taken, [dh, g, u],
+                           lambda *xs: [_gated_elements(*xs, activation, whole)], activation=activation)
         taken = taken and n < 1 << 21 and whole * -(-k // 8) * 8 < (1 << 30) - 1024
-        (dx,) = _operator("gated_input_grad", taken, [dgu, gate, up], input_grad, features=n)
+        (dx,) = _operator("gated_input_grad", taken, [dgu, gate, up],
+                          lambda *xs: [_gated_input_grad(*xs, whole)], features=n)
         # tokens in whole k tiles and whole rows: the plan's own dots, which take an update of the weight into their stores
         dots = t % 64 == 0 and n % 8 == 0 and k % 8 == 0
-        dw = _operator("gated_weight_grad", taken and not dots, [dgu, x], weight_grad, features=n)
-        return dx, dw[0], dw[1]
+        dgate, dup = _operator("gated_weight_grad", taken and not dots, [dgu, x],
+                               lambda *xs: _gated_weight_grad(*xs, n, whole), features=n)
+        return dx, dgate, dup
+
+    @staticmethod
+    def backward(ctx, *cotangents):
+        def grads(dh, x, gate, up):
+            g, u = _gated_products(x, gate, up)
+            n = gate.shape[0]
+            dgu = _gated_elements(dh, g, u, ctx.activation, n)
+            return (_gated_input_grad(dgu, gate, up, n), *_gated_weight_grad(dgu, x, n, n))
+
+        return (*_second(grads, ctx.saved_tensors, cotangents), None, None)
+
+
+def _gated_elements(dh, g, u, activation, whole):
+    """``[dg | du]``, each half ``whole`` elements wide (zeros past its features)."""
+    (t, n), dtype = dh.shape, dh.dtype
+    a, da = _activated_grad(activation, g)
+    d = dh.to(g.dtype)
+    halves = [(d * u * da).to(dtype), (d * a).to(dtype)]
+    if whole != n:
+        pad = prims.full((t, whole - n), 0.0, dtype)
+        halves = [halves[0], pad, halves[1], pad]
+    return F.cat(halves, 1)
+
+
+def _gated_input_grad(dgu, gate, up, whole):
+    n, acc = gate.shape[0], accum_dtype(dgu.dtype)
+    dims = (((1,), (0,)), ((), ()))
+    return (prims.dot_general(dgu[:, :n], gate, dims, acc)
+            + prims.dot_general(dgu[:, whole:whole + n], up, dims, acc)).to(dgu.dtype)
+
+
+def _gated_weight_grad(dgu, x, n, whole):
+    acc = accum_dtype(x.dtype)
+    return [dot(dgu[:, lo:lo + n], x, (((0,), (0,)), ((), ())), acc, x.dtype) for lo in (0, whole)]
 
 
 def gated_linear(input, gate_weight, up_weight, activation="silu"):

@@ -974,3 +974,45 @@ def test_heads_of_several_launches_in_sequences_that_end_inside_them(hip):
             nv.d2h(got.ctypes.data, buf.ptr + at * d * 2, got.nbytes)
             ref = want[i].reshape(80, d)
             _near(D.to_numpy_values(got, "bfloat16").astype(np.float64), ref, U["bfloat16"] * np.abs(ref) + F32 * (d + 40) * 8 * np.abs(ref).max(), at)
+
+
+@pytest.mark.parametrize("t,k,n,dtype", [(16, 16, 16, "bfloat16"), (65, 72, 40, "float16"), (128, 64, 64, "bfloat16")])
+def test_gated_gradients_of_two_micro_batches(hip, t, k, n, dtype):
+    """``backward()`` after each of two micro-batches: the weights' gradients are the sums of both, each rounded, and rounded
+    again; each input's gradient is its own."""
+    (x1, gate, up, dy1), (x2, _, _, dy2) = _gated_case(61, t, k, n, dtype), _gated_case(62, t, k, n, dtype)
+
+    def fn(x1, x2, gate, up, dy1, dy2):
+        for x, dy in ((x1, dy1), (x2, dy2)):
+            F.gated_linear(x, gate, up).backward(dy)
+        return [x1.grad, x2.grad, gate.grad, up.grad]
+
+    f = L.compile(fn, device="hip")
+    got = [_values(v) for v in f(*(_tensor(v, dtype) for v in (x1, x2, gate, up, dy1, dy2)))]
+    want = [M.gated(x, gate, up, dy, "silu") for x, dy in ((x1, dy1), (x2, dy2))]
+    tol = [_gated_tolerances(x, gate, up, dy, "silu", dtype) for x, dy in ((x1, dy1), (x2, dy2))]
+    assert [st.kind for st in f.plan.steps].count("gated_fwd") == 2
+    for i in range(2):
+        _near(got[i], want[i][1], tol[i][1], i)
+    for i in (2, 3):
+        w, each = want[0][i] + want[1][i], tol[0][i] + tol[1][i]
+        _near(got[i], w, each + U[dtype] * (np.abs(w) + each), i)
+
+
+def test_a_layer_of_two_micro_batches(hip):
+    """Heads, attention and the gated MLP twice in one plan, ``backward()`` after each: the weights' gradients against the sum
+    of two plans of one micro-batch each, 2e-2 of the largest, as the layer is held under other flags."""
+    rng = np.random.default_rng(7)
+    layer = _layer(64, 96, 32, 0.5)
+    _load(layer, rng)
+    (x1, dy1, cos, sin), (x2, dy2, _, _) = (_layer_inputs(rng, 48, 64, 32, 16) for _ in range(2))
+
+    def grads(layer, cos, sin, *pairs):
+        for x, dy in zip(pairs[::2], pairs[1::2]):
+            layer(x, cos, sin, 2, 2).backward(dy)
+        return [p.grad for p in layer.parameters()]
+
+    runs = [[_values(v).copy() for v in L.compile(grads, device="hip")(layer, cos, sin, *pairs)]
+            for pairs in ((x1, dy1), (x2, dy2), (x1, dy1, x2, dy2))]
+    for a, b, both in zip(*runs):
+        assert np.abs(both - a - b).max() <= 2e-2 * (np.abs(a) + np.abs(b)).max()

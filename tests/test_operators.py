@@ -434,3 +434,172 @@ def test_gradients_of_few_tiles_are_one_step():
     n = C.c_size_t()
     nv.call("nhip_gated_backward_workspace", C.byref(nv.GatedDesc(m=130, n=333, k=67, x_m=67, w_n=67, dtype=1, config=-1)), C.byref(n))
     assert steps[-1].kind == "gated_both" and steps[-1].scratch >= n.value
+
+
+# ---- the tape used again: several backward() calls in one trace, gradients of gradients
+
+
+def _bits(x, dtype="bfloat16"):
+    return np.ascontiguousarray(D.from_values(np.asarray(x, np.float32), dtype))
+
+
+def _rounded(x, dtype="bfloat16"):
+    return np.asarray(D.to_numpy_values(_bits(x, dtype), dtype), np.float64)
+
+
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("activation", M.ACTIVATIONS)
+@pytest.mark.parametrize("t,k,n", [(16, 16, 16), (5, 11, 6), (64, 16, 24)])
+def test_gated_gradients_of_two_micro_batches(t, k, n, activation, fused):
+    """``backward()`` after each micro-batch: the weights' gradients are the sums, each input's its own. Two gradients within
+    their own bounds, each of them rounded, and their sum's rounding."""
+    from tests.test_gpu_operators import _gated_tolerances
+
+    rng = np.random.default_rng(t + n)
+    gate, up = (_rounded(rng.standard_normal((n, k)) / np.sqrt(k)) for _ in range(2))
+    batches = [tuple(_rounded(rng.standard_normal(s)) for s in ((t, k), (t, n))) for _ in range(2)]
+
+    def fn(x1, x2, gate, up, dy1, dy2):
+        for x, dy in ((x1, dy1), (x2, dy2)):
+            F.gated_linear(x, gate, up, activation=activation).backward(dy)
+        return [x1.grad, x2.grad, gate.grad, up.grad]
+
+    arrays = [_bits(v) for v in (batches[0][0], batches[1][0], gate, up, batches[0][1], batches[1][1])]
+    with L.config.compiler.patch(fused_operators=fused):
+        g = _graph(fn, *arrays, dtypes=["bfloat16"] * 6)
+    got = [np.asarray(v, np.float64) for v in oracle.values(g, arrays)]
+    want = [M.gated(x, gate, up, dy, activation) for x, dy in batches]
+    tol = [_gated_tolerances(x, gate, up, dy, activation, "bfloat16") for x, dy in batches]
+    for i in range(2):
+        assert np.all(np.abs(got[i] - want[i][1]) <= tol[i][1]), i
+    for i in (2, 3):
+        w = want[0][i] + want[1][i]
+        each = tol[0][i] + tol[1][i]
+        assert np.all(np.abs(got[i] - w) <= each + 2.0**-8 * (np.abs(w) + each)), i
+
+
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("s,n,nkv,d", [(4, 4, 4, 4), (3, 3, 1, 10)])
+def test_heads_gradients_of_two_micro_batches(s, n, nkv, d, fused):
+    """As above: one rounding of the sum more than test_heads_values_and_gradients counts."""
+    rng = np.random.default_rng(s)
+    x = [M.heads_inputs(rng, 2, s, n, nkv, d, d, table=9) for _ in range(2)]
+    for m in ("wq", "wk", "cos", "sin"):
+        x[1][m] = x[0][m]
+    own = ("q", "k", "gq", "gk", "positions")
+
+    def fn(wq, wk, cos, sin, *rest):
+        parts = [dict(zip(own, rest[:5])), dict(zip(own, rest[5:]))]
+        for p in parts:
+            yq, yk = F.qk_norm_rope(p["q"], p["k"], cos, sin, wq, wk, positions=p["positions"], eps=1e-3)
+            F.sum(yq * p["gq"]).backward()
+            F.sum(yk * p["gk"]).backward()
+        return [wq.grad, wk.grad, *(p[m].grad for p in parts for m in ("q", "k"))]
+
+    got, _ = _run(fn, *(x[0][m] for m in ("wq", "wk", "cos", "sin")), *(p[m] for p in x for m in own), fused=fused)
+    a, b = (M.heads(p, 1e-3, False) for p in x)
+    for v, w in zip(got, [a[4] + b[4], a[5] + b[5], a[2], a[3], b[2], b[3]]):
+        assert np.abs(v - w).max() <= 2.0**-24 * (3 * d + 40) * 4 * max(1.0, np.abs(w).max())
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_a_later_loss_that_does_not_use_the_operator(fused):
+    """The second backward() walks a tape that holds the first one's nodes: a weight that both losses share has both
+    gradients, exactly (a plain product of small integers besides the gated one's bounds)."""
+    from tests.test_gpu_operators import _gated_tolerances
+
+    rng = np.random.default_rng(2)
+    x, dy = _rounded(rng.standard_normal((16, 16))), _rounded(rng.standard_normal((16, 16)))
+    gate, up = (_rounded(rng.standard_normal((16, 16)) / 4) for _ in range(2))
+    c = rng.integers(-2, 3, (16, 16)).astype(np.float64)
+
+    def fn(x, gate, up, dy, c):
+        F.gated_linear(x, gate, up).backward(dy)
+        F.sum(gate.float() * c.float()).backward()
+        return [x.grad, gate.grad, up.grad]
+
+    arrays = [_bits(v) for v in (x, gate, up, dy, c)]
+    with L.config.compiler.patch(fused_operators=fused):
+        g = _graph(fn, *arrays, dtypes=["bfloat16"] * 5)
+    got = [np.asarray(v, np.float64) for v in oracle.values(g, arrays)]
+    want, tol = M.gated(x, gate, up, dy, "silu")[1:], _gated_tolerances(x, gate, up, dy, "silu", "bfloat16")[1:]
+    want[1] = want[1] + c
+    for v, w, e in zip(got, want, tol):
+        assert np.all(np.abs(v - w) <= e + 2.0**-8 * (np.abs(w) + e))
+
+
+def _gated_twice(activation, tied=False):
+    """A program of the gated gradients' own gradients, by x, gate, up and dh (``tied``: gate is the up projection)."""
+    def f(x, gate, up):
+        return F.gated_linear(x, gate, up, activation=activation)
+
+    def fn(x, gate, up, dh, cx, cg, cu):
+        if tied:
+            pull = L.vjp(lambda x, w, dh: L.vjp(lambda x, w: f(x, w, w), x, w)[1](dh), x, gate, dh)[1]
+            return list(pull((cx, cg)))
+        return list(L.vjp(lambda x, gate, up, dh: L.vjp(f, x, gate, up)[1](dh), x, gate, up, dh)[1]((cx, cg, cu)))
+
+    return fn
+
+
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("activation", M.ACTIVATIONS)
+def test_gated_gradient_of_the_gradient(activation, tied):
+    """float64 against central differences of the first gradient's formula (step 1e-6: 1e-9 from its rounding and less from
+    its third derivative), and in bfloat16 the same bits fused and not."""
+    rng = np.random.default_rng(len(activation) + tied)
+    shapes = dict(x=(3, 5), gate=(4, 5), up=(4, 5), dh=(3, 4), cx=(3, 5), cg=(4, 5), cu=(4, 5))
+    x = {n: rng.standard_normal(s) for n, s in shapes.items()}
+    if tied:
+        x["up"] = x["gate"]
+
+    def value(x):
+        up = x["gate"] if tied else x["up"]
+        grads = M.gated(x["x"], x["gate"], up, x["dh"], activation)[1:]
+        if tied:
+            grads = [grads[0], grads[1] + grads[2]]
+        return sum((g * x[c]).sum() for g, c in zip(grads, ("cx", "cg", "cu")))
+
+    got, _ = _run(_gated_twice(activation, tied), *x.values())
+    for name, g in zip(("x", "gate", "dh") if tied else ("x", "gate", "up", "dh"), got):
+        assert np.abs(g - M.differences(value, x, name)).max() <= 1e-6, name
+    arrays = [_bits(v) for v in x.values()]
+    both = []
+    for fused in (True, False):
+        with L.config.compiler.patch(fused_operators=fused):
+            g = _graph(_gated_twice(activation, tied), *arrays, dtypes=["bfloat16"] * 7)
+        both.append(oracle.run(g, arrays))
+    assert all(np.array_equal(a, b) for a, b in zip(*both))
+
+
+@pytest.mark.parametrize("weights", [True, False])
+def test_heads_gradient_of_the_gradient(weights):
+    """float64 against differences of the first gradient's formula; float32 against the
+    float64 values to a few hundred roundings of the largest."""
+    rng = np.random.default_rng(5)
+    x = M.heads_inputs(rng, 1, 3, 2, 1, 8, 6, table=5, dtype="float64", weights=weights, positions=True)
+    leaves = [n for n in ("q", "k", "wq", "wk", "gq", "gk") if n in x]
+    shapes = [x[n].shape for n in leaves[:-2]]
+    cots = {f"c{i}": rng.standard_normal(s) for i, s in enumerate(shapes)}
+
+    def fn(*args):
+        t = dict(zip([*x, *cots], args))
+
+        def first(*ls):
+            v = {**t, **dict(zip(leaves, ls))}
+            f = lambda *h: F.qk_norm_rope(*h[:2], v["cos"], v["sin"], *h[2:], positions=v["positions"], eps=1e-3)  # noqa: E731
+            return L.vjp(f, *(v[n] for n in leaves[:-2]))[1]((v["gq"], v["gk"]))
+
+        return list(L.vjp(first, *(t[n] for n in leaves))[1](tuple(t[c] for c in cots)))
+
+    def value(x):
+        return sum((g * c).sum() for g, c in zip(M.heads(x, 1e-3, False)[2:], cots.values()))
+
+    got, _ = _run(fn, *x.values(), *cots.values())
+    for name, g in zip(leaves, got):
+        assert np.abs(g - M.differences(value, x, name)).max() <= 1e-6, name
+    single = {n: v if n in ("cos", "sin", "positions") else v.astype(np.float32) for n, v in {**x, **cots}.items()}
+    wide = {n: v if n in ("cos", "sin", "positions") else v.astype(np.float64) for n, v in single.items()}
+    near, _ = _run(fn, *wide.values())
+    for a, b in zip(_run(fn, *single.values())[0], near):
+        assert np.abs(a - b).max() <= 2.0**-24 * 400 * max(1.0, np.abs(b).max())
