@@ -113,9 +113,10 @@ def _row_space(graph, n):
     return (math.prod(x.shape[: r - len(axes)]), c)
 
 
-def fuse(graph: Graph, fuse_loops=True, packed=frozenset()) -> list:
+def fuse(graph: Graph, fuse_loops=True, packed=frozenset(), alone=frozenset()) -> list:
     """The steps computing ``graph``'s outputs, in an order respecting dependencies. ``packed`` holds
-    concatenations that are views (weights stored back to back)."""
+    concatenations that are views (weights stored back to back), ``alone`` row statistics that are stored instead of
+    being computed in the kernel that reads them."""
     users = graph.users()
     prod = graph.producers()
     order = {n.output: i for i, n in enumerate(graph.nodes)}
@@ -225,6 +226,9 @@ def fuse(graph: Graph, fuse_loops=True, packed=frozenset()) -> list:
             if u in kernel_of:
                 continue
             outside = {c.output for c in users.get(u, []) if c.output not in mem}
+            if u in alone:
+                must.add(u)
+                continue
             if p.prim in ("reduce_sum", "reduce_max"):
                 rs = _row_space(graph, p)
                 if rs is None or (rows[k] is not None and rows[k] != rs):
@@ -502,7 +506,7 @@ def hoist_to_producers(graph, steps):
     return _drop_unread(graph, steps)
 
 
-def absorb_rows(graph, steps):
+def absorb_rows(graph, steps, alone=frozenset()):
     """Merges a loop kernel into an earlier row kernel over the same row space when everything the loop
     reads is the row kernel's input, its output, or already in memory when the row kernel runs: the row
     kernel writes the loop's outputs in its writing pass, and the operands both read (a softmax's logits,
@@ -520,6 +524,8 @@ def absorb_rows(graph, steps):
         cands = {pos[u] for u in lt.inputs if u in pos and steps[pos[u]].kind == "row"}
         for ri in sorted(cands):
             rt = steps[ri]
+            if any(v in alone for v in rt.outputs):
+                continue
             if ri in merged or ri >= li or rt.rows is None or rt.rows[0] * rt.rows[1] != numel:
                 continue
             elem = [v for v in rt.outputs if graph.types[v].numel() == numel]

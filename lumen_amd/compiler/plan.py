@@ -193,6 +193,7 @@ class Plan:
         self.donate = dict(donate or {})
         self.source_graph = graph
         self.graph, self.packs = compiled if compiled is not None else compile_graph(graph, packable)
+        self.alone = set()  # row statistics that the generator could not compute in their readers' kernel
         self._lay_out()
         limit = config.compiler.memory_limit
         if limit and compiled is None and self.workspace_bytes > limit:
@@ -204,12 +205,22 @@ class Plan:
             if g is not self.graph:
                 self.graph = g
                 self._lay_out()
-        self.kernels = {}
-        self.sources = {}
-        self.epi_alts = {}  # epilogue GEMM step -> [(k loop variant, kernel, source)] for the autotuner
         self._native = None
-        if compiled is None or build_kernels:
-            self._gen_kernels()
+        while True:
+            self.kernels = {}
+            self.sources = {}
+            self.epi_alts = {}  # epilogue GEMM step -> [(k loop variant, kernel, source)] for the autotuner
+            if compiled is not None and not build_kernels:
+                break
+            try:
+                self._gen_kernels()
+                break
+            except codegen.Unfusable as e:
+                prim = next((n.prim for n in self.graph.nodes if n.output == e.var), None)
+                if prim not in ("reduce_sum", "reduce_max") or e.var in self.alone:
+                    raise
+                self.alone.add(e.var)
+                self._lay_out()
         if build_kernels:
             self.build()
 
@@ -249,10 +260,10 @@ class Plan:
 
     # ---- fusion with fallback: groups the generator rejects are split
     def _fuse(self):
-        steps = fusion.fuse(self.graph, fuse_loops=config.compiler.fuse, packed=self.packed)
+        steps = fusion.fuse(self.graph, fuse_loops=config.compiler.fuse, packed=self.packed, alone=self.alone)
         if config.compiler.fuse:
             steps = fusion.hoist_to_producers(self.graph, steps)
-            steps = fusion.absorb_rows(self.graph, steps)
+            steps = fusion.absorb_rows(self.graph, steps, self.alone)
             steps = fusion.column_sums(self.graph, steps)
         if config.compiler.fuse and config.compiler.horizontal_fusion:
             steps = fusion.horizontal(self.graph, steps)

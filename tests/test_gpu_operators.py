@@ -1016,3 +1016,49 @@ def test_a_layer_of_two_micro_batches(hip):
             for pairs in ((x1, dy1), (x2, dy2), (x1, dy1, x2, dy2))]
     for a, b, both in zip(*runs):
         assert np.abs(both - a - b).max() <= 2e-2 * (np.abs(a) + np.abs(b)).max()
+
+
+@pytest.mark.parametrize("fused,dtype,d,rot,interleaved", [
+    (True, "float64", 16, 16, False), (True, "float64", 10, 6, True), (True, "bfloat16", 1030, 64, True),
+    (False, "bfloat16", 16, 8, False), (False, "float32", 64, 64, False)])
+def test_heads_that_are_primitives(hip, fused, dtype, d, rot, interleaved):
+    """What the head kernels do not take, in both directions, float64 with its own roundings."""
+    x = _heads_case(70 + d, 2, 5, 4, 2, d, rot, "float32" if dtype == "float64" else dtype, interleaved)
+    exact = ("cos", "sin", "positions")
+    args = [L.from_numpy(v if m in exact else v.astype(np.float64)) if m in exact or dtype == "float64" else _tensor(v, dtype)
+            for m, v in x.items()]
+    with L.config.compiler.patch(fused_operators=fused):
+        f = L.compile(_heads_program(list(x), interleaved, 1e-3), device="hip")
+        got = [_values(t) for t in f(*args)]
+    assert not {"heads_fwd", "heads_bwd"} & {st.kind for st in f.plan.steps}
+    if dtype != "float64":
+        return _heads_check(got, x, dtype, 1e-3, interleaved)
+    step = 2.0**-53
+    for i, (a, w) in enumerate(zip(got, M.heads(x, 1e-3, interleaved))):
+        rows = np.prod(x["q" if i in (0, 2, 4) else "k"].shape[:3])
+        _near(a, w, step * (d + 40) * 8 * np.abs(w).max() if i < 4 else step * (rows + d + 40) * 4 * rows, i)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_a_gradient_of_the_gated_gradient(hip, dtype):
+    """The gradients' own gradients against the oracle on the same graph: 2e-2 of the largest in bfloat16, as the layer is
+    held, and 2^-24 times 40 sums of 63 terms in float32."""
+    from oracle import oracle
+
+    rng = np.random.default_rng(80)
+    shapes = [(65, 63), (17, 63), (17, 63), (65, 17), (65, 63), (17, 63), (17, 63)]
+    scale = [1, 63**-0.5, 63**-0.5, 1, 1, 1, 1]
+    arrays = [_round(rng.standard_normal(s) * c, dtype) for s, c in zip(shapes, scale)]
+
+    def fn(x, gate, up, dh, cx, cg, cu):
+        def first(x, gate, up, dh):
+            return L.vjp(lambda x, gate, up: F.gated_linear(x, gate, up), x, gate, up)[1](dh)
+
+        return list(L.vjp(first, x, gate, up, dh)[1]((cx, cg, cu)))
+
+    tensors = [_tensor(v, dtype) for v in arrays]
+    got = [_values(t) for t in L.compile(fn, device="hip")(*tensors)]
+    graph = L.make_graph(fn)(*[L.empty(list(s), dtype, "meta") for s in shapes])
+    for a, w in zip(got, oracle.values(graph, [t.raw() for t in tensors])):
+        w = np.asarray(w, np.float64)
+        assert np.abs(a - w).max() <= (2e-2 if dtype == "bfloat16" else 2.0**-24 * 40 * 63) * np.abs(w).max()

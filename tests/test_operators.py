@@ -603,3 +603,26 @@ def test_heads_gradient_of_the_gradient(weights):
     near, _ = _run(fn, *wide.values())
     for a, b in zip(_run(fn, *single.values())[0], near):
         assert np.abs(a - b).max() <= 2.0**-24 * 400 * max(1.0, np.abs(b).max())
+
+
+@pytest.mark.parametrize("fused,dtype,d,rot", [(True, "float64", 16, 16), (True, "float64", 10, 6), (True, "bfloat16", 1030, 64),
+                                               (False, "bfloat16", 16, 8), (False, "float32", 16, 16)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_heads_that_are_primitives_have_plans(fused, dtype, d, rot, interleaved):
+    """A turn reads a head's norm at other elements than its own, which no kernel computes that holds one row's statistics at
+    a time: the plan stores them."""
+    def both(q, k, cos, sin, wq, wk, gq, gk):
+        out, pull = L.vjp(lambda q, k, wq, wk: F.qk_norm_rope(q, k, cos, sin, wq, wk, interleaved=interleaved), q, k, wq, wk)
+        return [*out, *pull((gq, gk))]
+
+    q, k, table, w = _m((2, 5, 4, d), dtype), _m((2, 5, 2, d), dtype), _m((9, rot // 2), "float32"), _m((d,), dtype)
+    with L.config.compiler.patch(fused_operators=fused):
+        for fn, args in ((lambda *a: both(*a)[:2], (q, k, table, table, w, w, q, k)), (both, (q, k, table, table, w, w, q, k))):
+            steps = Plan(L.make_graph(fn)(*args), build_kernels=False).steps
+            assert not {"heads_fwd", "heads_bwd"} & {st.kind for st in steps}
+
+
+def test_a_gradient_of_the_gradient_has_a_plan():
+    for dtype in ("bfloat16", "float32"):
+        x, w, dh = _m((65, 63), dtype), _m((17, 63), dtype), _m((65, 17), dtype)
+        assert Plan(L.make_graph(_gated_twice("gelu"))(x, w, w, dh, x, w, w), build_kernels=False).steps
