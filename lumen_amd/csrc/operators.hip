@@ -15,7 +15,8 @@ bool on(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % b
 
 // ---- heads ----------------------------------------------------------------------------------------------
 
-constexpr int64_t kHeadsLaunchRows = int64_t(1) << 25;  // heads of a launch: 64 lanes of each stay within 2^32 threads
+// Heads of a launch, queries' and keys' together: 64 lanes of each are 2^31 threads, and a launch has to stay below 2^32.
+constexpr int64_t kHeadsLaunchRows = int64_t(1) << 25;
 // Workgroups of a backward launch at most: each leaves a row of partial sums that is read again. Two rounds of the three
 // that fit a CU with chunks of 8 elements, 2048 otherwise ([4, 4096, 16 + 16, 128] in chunks of 4: 1536 101 us, 2048 88,
 // 4096 87, whose sums take 2 us longer).
@@ -45,8 +46,7 @@ int heads_check(const nhip_heads_desc *d, const char *what) {
 
 // Tokens of one launch.
 int64_t heads_tokens(const nhip_heads_desc *d) {
-    int64_t most = d->heads > d->kv_heads ? d->heads : d->kv_heads;
-    most = kHeadsLaunchRows / (most > 0 ? most : 1);
+    const int64_t heads = d->heads + d->kv_heads, most = kHeadsLaunchRows / (heads > 0 ? heads : 1);
     const int64_t tokens = d->batch * d->seq;
     return tokens < most ? tokens : most;
 }

@@ -1062,3 +1062,25 @@ def test_a_gradient_of_the_gated_gradient(hip, dtype):
     for a, w in zip(got, oracle.values(graph, [t.raw() for t in tensors])):
         w = np.asarray(w, np.float64)
         assert np.abs(a - w).max() <= (2e-2 if dtype == "bfloat16" else 2.0**-24 * 40 * 63) * np.abs(w).max()
+
+
+def test_heads_of_as_many_queries_as_keys_past_a_launch(hip):
+    """2^21 tokens of 16 + 16 heads of 132 elements, 64 lanes each: 2^32 threads, two launches. The inputs' tokens are 64 that
+    repeat (batches that lie on one another), the results' rows at both ends and at the launches' border."""
+    batch, seq, n, d = 1 << 15, 64, 16, 132
+    x = _heads_case(90, 1, seq, n, n, d, 64, "bfloat16", positions=False)
+    dev = {m: Dev(np.ascontiguousarray(D.from_values(np.asarray(x[m], np.float32), "bfloat16"))) for m in ("q", "k", "wq", "wk")}
+    cos, sin = Dev(x["cos"]), Dev(x["sin"])
+    out = {m: Dev(nbytes=batch * seq * n * d * 2) for m in ("oq", "ok")}
+    desc = nv.HeadsDesc(batch=batch, seq=seq, heads=n, kv_heads=n, head_dim=d, rot=64, table_rows=64, dtype=1, eps=1e-3)
+    for m in ("q", "k", "oq", "ok"):
+        for axis, stride in (("b", seq * n * d if m in out else 0), ("s", n * d), ("n", d)):
+            setattr(desc, f"{m}_{axis}", stride)
+    nv.call("nhip_qk_norm_rope", C.byref(desc), dev["q"].ptr, dev["k"].ptr, dev["wq"].ptr, dev["wk"].ptr, cos.ptr, sin.ptr, None,
+            out["oq"].ptr, out["ok"].ptr)
+    got = np.empty((seq, n, d), np.uint16)
+    for m, want in zip(("oq", "ok"), M.heads(x, 1e-3, False)):
+        for b in (0, batch // 2 - 1, batch // 2, batch - 1):
+            nv.d2h(got.ctypes.data, out[m].ptr + b * got.nbytes, got.nbytes)
+            _near(D.to_numpy_values(got, "bfloat16").astype(np.float64), want[0],
+                  U["bfloat16"] * np.abs(want[0]) + F32 * (d + 40) * 8 * np.abs(want).max(), (m, b))

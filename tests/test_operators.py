@@ -626,3 +626,16 @@ def test_a_gradient_of_the_gradient_has_a_plan():
     for dtype in ("bfloat16", "float32"):
         x, w, dh = _m((65, 63), dtype), _m((17, 63), dtype), _m((65, 17), dtype)
         assert Plan(L.make_graph(_gated_twice("gelu"))(x, w, w, dh, x, w, w), build_kernels=False).steps
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(16, 16), (1, 1), (32, 8), (8, 0), (0, 8), ((1 << 20) - 1, (1 << 20) - 1)])
+def test_a_launch_of_heads_stays_below_2_to_the_32_threads(heads, kv_heads):
+    """Queries and keys go out in one launch of up to 64 lanes a head; the workspace, 2050 rows a launch, says how many
+    launches there are."""
+    n = C.c_size_t()
+    for tokens in (1 << 19, 1 << 21, (1 << 25) + 3, (1 << 29) + 1):
+        d = nv.HeadsDesc(batch=1, seq=tokens, heads=heads, kv_heads=kv_heads, head_dim=132, rot=0, table_rows=1, dtype=1)
+        nv.call("nhip_qk_norm_rope_workspace", C.byref(d), C.byref(n))
+        launches = n.value // (2050 * 132 * 4)
+        rows = -(-tokens // launches) * (heads + kv_heads)
+        assert rows * 64 + 2 * 256 < 1 << 32 and (launches == 1 or rows > 1 << 24)
