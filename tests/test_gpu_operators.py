@@ -1084,3 +1084,16 @@ def test_heads_of_as_many_queries_as_keys_past_a_launch(hip):
             nv.d2h(got.ctypes.data, out[m].ptr + b * got.nbytes, got.nbytes)
             _near(D.to_numpy_values(got, "bfloat16").astype(np.float64), want[0],
                   U["bfloat16"] * np.abs(want[0]) + F32 * (d + 40) * 8 * np.abs(want).max(), (m, b))
+
+
+@pytest.mark.parametrize("n", [8, 9])
+@pytest.mark.parametrize("dtype,most", [("bfloat16", 20.0), ("float16", 9.0)])
+def test_sigmoid_gradient_of_large_gates(hip, dtype, most, n):
+    """Both elementwise kernels, relative to the value on both sides (float16 within its normal numbers): a rounding of dg,
+    one of dx and 64 of 2^-24 between (exp(20) as 2^28.9: the exponent's rounding and its factor's are 20 each)."""
+    from tests.test_operators import sigmoid_gradient
+
+    g = np.arange(4.0, most + 0.5, 0.5)
+    *x, want = sigmoid_gradient(np.concatenate([g, -g]), n)
+    dx = _values(L.compile(_gated_program("sigmoid"), device="hip")(*(_tensor(v, dtype) for v in x))[1])
+    _near(dx, want, (2.01 * U[dtype] + 64 * F32) * want)

@@ -639,3 +639,24 @@ def test_a_launch_of_heads_stays_below_2_to_the_32_threads(heads, kv_heads):
         launches = n.value // (2050 * 132 * 4)
         rows = -(-tokens // launches) * (heads + kv_heads)
         assert rows * 64 + 2 * 256 < 1 << 32 and (launches == 1 or rows > 1 << 24)
+
+
+def sigmoid_gradient(g, n):
+    """Operands whose gate is ``g`` and whose other factors are 1, of ``n`` equal features, and dx: n s(g) s(-g), n s(g)."""
+    x = np.stack([g, np.ones_like(g)], 1)
+    gate, up = np.tile([1.0, 0.0], (n, 1)), np.tile([0.0, 1.0], (n, 1))
+    return x, gate, up, np.ones((len(g), n)), n * np.stack([1 / ((1 + np.exp(-g)) * (1 + np.exp(g))), 1 / (1 + np.exp(-g))], 1)
+
+
+@pytest.mark.parametrize("dtype,step", [("float32", 2.0**-24), ("bfloat16", 2.0**-8)])
+def test_sigmoid_gradient_of_large_gates(dtype, step):
+    """s(g) s(-g) relative to itself on both sides: a rounding of dg, one of dx and 16 of 2^-24 between."""
+    g = np.concatenate([np.arange(8.0, 20.5, 0.5), -np.arange(8.0, 20.5, 0.5)])
+    x, gate, up, dh, want = sigmoid_gradient(g, 1)
+
+    def fn(x, gate, up, dh):
+        return list(L.vjp(lambda x: F.gated_linear(x, gate, up, activation="sigmoid"), x)[1](dh))
+
+    arrays = [v.astype(np.float32) if dtype == "float32" else _bits(v) for v in (x, gate, up, dh)]
+    (got,) = oracle.values(_graph(fn, *arrays, dtypes=[dtype] * 4), arrays)
+    assert np.all(np.abs(np.asarray(got, np.float64) - want) <= (2.01 * step + 16 * 2.0**-24) * want)
