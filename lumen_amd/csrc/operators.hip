@@ -248,6 +248,12 @@ int gated_check(const nhip_gated_desc *d, const char *what) {
 
 int64_t tiles(int64_t m, int64_t bm, int64_t n, int64_t bn) { return (m + bm - 1) / bm * ((n + bn - 1) / bn); }
 
+// Whether tiles of bm x bn, a workgroup of `threads` each, are a launch of fewer than 2^32 threads (their count within 64 bits).
+bool tiles_ok(int64_t m, int64_t bm, int64_t n, int64_t bn, int threads) {
+    const int64_t a = (m + bm - 1) / bm, b = (n + bn - 1) / bn;
+    return a < (int64_t(1) << 32) && b < (int64_t(1) << 32) / (threads * (a > 0 ? a : 1));
+}
+
 // The stream kernels' k: some, and 256 rows of it within the 2^31 bytes of a buffer.
 bool gated_stream_ok(const nhip_gated_desc *d) { return d->k > 0 && d->k < (int64_t(1) << 21); }
 bool gated_skinny_ok(const nhip_gated_desc *d) { return d->m <= 64 && d->k < (int64_t(1) << 30); }
@@ -275,6 +281,15 @@ GatedSplit gated_split(const nhip_gated_desc *d) {
     return best;
 }
 
+// Tile rows, columns and threads of a config's workgroups.
+struct GatedTile {
+    int rows, columns, threads;
+};
+GatedTile gated_tile(const nhip_gated_desc *d, int cfg) {
+    if (cfg == kSkinnyCfg) return {64, 16, d->m <= 32 ? 512 : 256};
+    return cfg == kStream256 ? GatedTile{256, 128, 512} : GatedTile{128, 64, 256};
+}
+
 int gated_default(const nhip_gated_desc *d) {
     const bool in_parts = d->k >= 1024 && gated_stream_ok(d) && tiles(d->m, 128, d->n, 64) <= 128;
     if (gated_skinny_ok(d)) {
@@ -295,6 +310,11 @@ int gated_default(const nhip_gated_desc *d) {
     return in_parts && gated_split(d).us < 5.0 + 0.0065 * double(d->k) ? kPartsCfg : kDeepCfg;
 }
 
+bool gated_launch_ok(const nhip_gated_desc *d, int cfg) {
+    const GatedTile t = gated_tile(d, cfg);
+    return tiles_ok(d->m, t.rows, d->n, t.columns, t.threads);
+}
+
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 
 // Bytes of the operands' copies, which lie ahead of the parts.
@@ -310,16 +330,15 @@ size_t gated_workspace(const nhip_gated_desc *d) {
 
 // `more`: arguments past the output; parts: blockIdx.z.
 template <class K, class Out, class... More>
-int gated_go(hipStream_t st, K kern, GemmShape s, int bm, int bn, int threads, int lds, const void *x, const void *gate,
-             const void *up, const Out &out, int parts = 1, More... more) {
-    s.tiles_m = int((s.m + bm - 1) / bm);
-    s.tiles_n = int((s.n + bn - 1) / bn);
-    if ((s.m + bm - 1) / bm * ((s.n + bn - 1) / bn) > 0x7fffffff) return fail("nhip_gated_linear: too many tiles");
+int gated_go(hipStream_t st, K kern, GemmShape s, const GatedTile &t, int lds, const void *x, const void *gate, const void *up,
+             const Out &out, int parts = 1, More... more) {
+    s.tiles_m = int((s.m + t.rows - 1) / t.rows);
+    s.tiles_n = int((s.n + t.columns - 1) / t.columns);
     if (lds > 64 * 1024 &&
         check(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
               "hipFuncSetAttribute"))
         return 1;
-    hipLaunchKernelGGL(kern, dim3(unsigned(s.tiles_m * s.tiles_n), 1, unsigned(parts)), dim3(threads), lds, st, s,
+    hipLaunchKernelGGL(kern, dim3(unsigned(s.tiles_m * s.tiles_n), 1, unsigned(parts)), dim3(t.threads), lds, st, s,
                        static_cast<const uint16_t *>(x), static_cast<const uint16_t *>(gate), static_cast<const uint16_t *>(up),
                        out, more...);
     return check(hipGetLastError(), "gated kernel launch");
@@ -345,16 +364,17 @@ int gated_pad(hipStream_t st, GatedPad &p, int count, const void *const *src, co
 }
 
 template <bool F16, bool ANY>
-int gated_few(hipStream_t st, const GemmShape &s, const void *x, const void *gate, const void *up, const GatedOut &o) {
-    if (s.m <= 16) return gated_go(st, gated_skinny<F16, 1, 8, ANY>, s, 64, 16, 512, 0, x, gate, up, o);
-    if (s.m <= 32) return gated_go(st, gated_skinny<F16, 2, 8, ANY>, s, 64, 16, 512, 0, x, gate, up, o);
-    return gated_go(st, gated_skinny<F16, 4, 4, ANY>, s, 64, 16, 256, 0, x, gate, up, o);
+int gated_few(hipStream_t st, const GemmShape &s, const GatedTile &t, const void *x, const void *gate, const void *up, const GatedOut &o) {
+    if (s.m <= 16) return gated_go(st, gated_skinny<F16, 1, 8, ANY>, s, t, 0, x, gate, up, o);
+    if (s.m <= 32) return gated_go(st, gated_skinny<F16, 2, 8, ANY>, s, t, 0, x, gate, up, o);
+    return gated_go(st, gated_skinny<F16, 4, 4, ANY>, s, t, 0, x, gate, up, o);
 }
 
 template <bool F16>
 int gated_run(hipStream_t st, int cfg, const nhip_gated_desc *d, GemmShape s, const void *x, const void *gate, const void *up,
               const GatedOut &o, bool in_place, void *ws) {
-    if (cfg == kSkinnyCfg) return in_place ? gated_few<F16, false>(st, s, x, gate, up, o) : gated_few<F16, true>(st, s, x, gate, up, o);
+    const GatedTile t = gated_tile(d, cfg);
+    if (cfg == kSkinnyCfg) return in_place ? gated_few<F16, false>(st, s, t, x, gate, up, o) : gated_few<F16, true>(st, s, t, x, gate, up, o);
     if (!in_place) {
         GatedPad p;
         const int64_t rows[3] = {s.m, s.n, s.n}, ld[3] = {s.a_m, s.b_n, s.b_n};
@@ -365,15 +385,15 @@ int gated_run(hipStream_t st, int cfg, const nhip_gated_desc *d, GemmShape s, co
     }
     constexpr int deep = gemm_stream_lds_bytes<64, 2, 128, 3>();
     if (cfg == kStream256)
-        return gated_go(st, gated_stream<F16, 256, 3>, s, 256, 128, 512, gemm_stream_lds_bytes<64, 4>(), x, gate, up, o);
-    if (cfg == kDeepCfg) return gated_go(st, gated_stream<F16, 128, 1, 3>, s, 128, 64, 256, deep, x, gate, up, o);
+        return gated_go(st, gated_stream<F16, 256, 3>, s, t, gemm_stream_lds_bytes<64, 4>(), x, gate, up, o);
+    if (cfg == kDeepCfg) return gated_go(st, gated_stream<F16, 128, 1, 3>, s, t, deep, x, gate, up, o);
     if (cfg == kStream128Cfg)
-        return gated_go(st, gated_stream<F16, 128, 0>, s, 128, 64, 256, gemm_stream_lds_bytes<64, 2, 128>(), x, gate, up, o);
+        return gated_go(st, gated_stream<F16, 128, 0>, s, t, gemm_stream_lds_bytes<64, 2, 128>(), x, gate, up, o);
     const GatedSplit p = gated_split(d);
     float *sums = reinterpret_cast<float *>(static_cast<char *>(ws) + gated_pad_bytes(d, cfg));
     GemmShape part = s;
     part.d_m = s.n;
-    if (gated_go(st, gated_stream_part<F16>, part, 128, 64, 256, deep, x, gate, up, GatedParts{sums}, p.parts, p.k_part)) return 1;
+    if (gated_go(st, gated_stream_part<F16>, part, t, deep, x, gate, up, GatedParts{sums}, p.parts, p.k_part)) return 1;
     const bool vec = s.n % 4 == 0;
     const int64_t blocks = (s.m * (vec ? s.n / 4 : s.n) + 255) / 256;
     const dim3 grid(unsigned(blocks < 4096 ? blocks : 4096));
@@ -392,6 +412,7 @@ int gated_on(hipStream_t st, const nhip_gated_desc *d, const void *x, const void
     int cfg = d->config < 0 ? gated_default(d) : d->config;
     if (cfg >= kGatedConfigs || !(cfg == kSkinnyCfg ? gated_skinny_ok(d) : gated_stream_ok(d)))
         return fail("nhip_gated_linear: config " + std::to_string(cfg) + " does not take these operands");
+    if (!gated_launch_ok(d, cfg)) return fail("nhip_gated_linear: a launch of 2^32 threads");
     GemmShape s;
     std::memset(&s, 0, sizeof(s));
     s.m = d->m, s.n = d->n, s.k = d->k;
@@ -483,6 +504,9 @@ int backward_check(const nhip_gated_desc *d, const char *what) {
     if (d->n >= (int64_t(1) << 21) || whole(d->n) * (d->w_n > whole(d->k) ? d->w_n : whole(d->k)) >= (int64_t(1) << 30) - 1024 ||
         weight_grad_plan(d).tm == 0)
         return fail(std::string(what) + ": weights or rows of 2^31 bytes");
+    // the input's gradient and the weights', in the smaller tiles
+    if (!tiles_ok(d->m, 128, d->k, 128, 256) || !tiles_ok(d->n, 128, d->k, 128, 256))
+        return fail(std::string(what) + ": a launch of 2^32 threads");
     return 0;
 }
 
@@ -549,11 +573,9 @@ struct GradProduct {
     AnyStore store() const { return p.parts > 1 ? AnyStore{sums, 0} : to; }
 };
 
-int product_ready(GradProduct &o, const char *what) {
+void product_ready(GradProduct &o) {
     o.s.tiles_m = int((o.s.m + o.p.tm - 1) / o.p.tm);
     o.s.tiles_n = int((o.s.n + o.p.tm - 1) / o.p.tm);
-    if (tiles(o.s.m, o.p.tm, o.s.n, o.p.tm) > 0x7fffffff) return fail(std::string(what) + ": too many tiles");
-    return 0;
 }
 
 int input_product(hipStream_t st, const nhip_gated_desc *d, const void *dgu, const void *gate, const void *up, void *dx, void *ws,
@@ -581,7 +603,8 @@ int input_product(hipStream_t st, const nhip_gated_desc *d, const void *dgu, con
     o.a = static_cast<const uint16_t *>(dgu), o.b = static_cast<const uint16_t *>(gate), o.b2 = static_cast<const uint16_t *>(up);
     o.to = AnyStore{dx, d->dtype};
     o.sums = reinterpret_cast<float *>(static_cast<char *>(ws) + up16(input_grad_pad(d)));
-    return product_ready(o, "nhip_gated_input_grad");
+    product_ready(o);
+    return 0;
 }
 
 int weight_product(hipStream_t st, const nhip_gated_desc *d, const void *dgu, const void *x, void *dgate, void *dup, void *ws,
@@ -610,7 +633,8 @@ int weight_product(hipStream_t st, const nhip_gated_desc *d, const void *dgu, co
     o.a = static_cast<const uint16_t *>(dgu), o.b = static_cast<const uint16_t *>(x), o.b2 = nullptr;
     o.to = AnyStore{dgate, d->dtype};
     o.sums = reinterpret_cast<float *>(static_cast<char *>(ws) + up16(weight_grad_pad(d)));
-    return product_ready(o, "nhip_gated_weight_grad");
+    product_ready(o);
+    return 0;
 }
 
 int lds_room(const void *kern, int lds) {
@@ -806,6 +830,8 @@ int nhip_gated_linear(const nhip_gated_desc *desc, const void *x, const void *ga
 int nhip_gated_linear_workspace(const nhip_gated_desc *desc, size_t *bytes) {
     if (gated_check(desc, "nhip_gated_linear_workspace")) return 1;
     if (!gated_skinny_ok(desc) && !gated_stream_ok(desc)) return fail("nhip_gated_linear_workspace: 1 to 2^21 - 1 elements a row");
+    if (!gated_launch_ok(desc, desc->config < 0 ? gated_default(desc) : desc->config))
+        return fail("nhip_gated_linear_workspace: a launch of 2^32 threads");
     *bytes = gated_workspace(desc);
     return 0;
 }

@@ -26,6 +26,7 @@ from lumen_amd.graph.tracer import TracedTensor, accum_dtype, broadcast_to, dot,
 KERNEL_DTYPES = ("float32", "bfloat16", "float16")
 MAX_HEAD = 1024  # a head's elements in the head kernels
 MAX_ROW = 1 << 21  # elements of a row of the gated projections: tiles of rows within 2^31 bytes
+MAX_FEATURES = 1 << 26  # of them: workgroups of 512 threads for 16 features each within 2^31 threads
 ACTIVATIONS = ("silu", "gelu", "relu", "sigmoid")
 
 
@@ -281,8 +282,8 @@ def _activated_grad(name, g):
     return s, s * prims.logistic(-g)  # 1 - s would cancel: at g = 10 it is off by 1e-3 of itself
 
 
-def _gated_taken(x):
-    return x.dtype in ("bfloat16", "float16") and 0 < x.shape[1] < MAX_ROW
+def _gated_taken(x, features):
+    return x.dtype in ("bfloat16", "float16") and 0 < x.shape[1] < MAX_ROW and features < MAX_FEATURES
 
 
 class _GatedLinear(Function):
@@ -295,7 +296,7 @@ class _GatedLinear(Function):
             g, u = _gated_products(x, gate, up)
             return [(_activated(activation, g) * u).to(x.dtype), g, u]
 
-        h, g, u = _operator("gated_linear", _gated_taken(x), [x, gate, up], body, activation=activation)
+        h, g, u = _operator("gated_linear", _gated_taken(x, gate.shape[0]), [x, gate, up], body, activation=activation)
         ctx.activation = activation
         ctx.save_for_backward(x, gate, up, g, u)
         return h
@@ -319,7 +320,7 @@ class _GatedGradients(Function):
         ctx.save_for_backward(dh, x, gate, up)
         (t, k), n = x.shape, gate.shape[0]
         whole = -(-n // 8) * 8  # each half of [dg | du] in whole 16-byte chunks
-        taken = _gated_taken(x)
+        taken = _gated_taken(x, n)
         (dgu,) = _operator("gated_linear_grad", taken, [dh, g, u],
                            lambda *xs: [_gated_elements(*xs, activation, whole)], activation=activation)
         taken = taken and n < 1 << 21 and whole * -(-k // 8) * 8 < (1 << 30) - 1024

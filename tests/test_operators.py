@@ -660,3 +660,22 @@ def test_sigmoid_gradient_of_large_gates(dtype, step):
     arrays = [v.astype(np.float32) if dtype == "float32" else _bits(v) for v in (x, gate, up, dh)]
     (got,) = oracle.values(_graph(fn, *arrays, dtypes=[dtype] * 4), arrays)
     assert np.all(np.abs(np.asarray(got, np.float64) - want) <= (2.01 * step + 16 * 2.0**-24) * want)
+
+
+def test_gated_launches_stay_below_2_to_the_32_threads():
+    """More workgroups than a launch holds are refused before anything is queued; the trace holds primitives well before."""
+    def workspace(name, **sizes):
+        d = nv.GatedDesc(**{**dict(dtype=1, config=-1, x_m=sizes["k"], w_n=sizes["k"]), **sizes})
+        nv.call(name, C.byref(d), C.byref(C.c_size_t()))
+
+    for m, n, config, taken in [(1, (1 << 27) - 32, -1, True), (1, 1 << 27, -1, False), (33, (1 << 28) - 32, 0, True),
+                                (33, 1 << 28, 0, False), (70, (1 << 30) - 128, 2, True), (70, 1 << 30, 2, False),
+                                (1 << 19, 1 << 19, 1, False), (1 << 30, 1 << 12, 2, False), (1 << 40, 8, -1, False)]:
+        if taken:
+            workspace("nhip_gated_linear_workspace", m=m, n=n, k=8, config=config)
+        else:
+            with pytest.raises(RuntimeError, match="2\\^32 threads"):
+                workspace("nhip_gated_linear_workspace", m=m, n=n, k=8, config=config)
+    for n, fusions in [((1 << 26) - 1, ["gated_linear"]), (1 << 26, [])]:
+        g = L.make_graph(F_gated)(_m((1, 8)), _m((n, 8)), _m((n, 8)))
+        assert [m.params["name"] for m in g.nodes if m.prim == "fusion"] == fusions
