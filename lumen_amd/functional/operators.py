@@ -323,7 +323,10 @@ class _GatedGradients(Function):
         taken = _gated_taken(x, n)
         (dgu,) = _operator("gated_linear_grad", taken, [dh, g, u],
                            lambda *xs: [_gated_elements(*xs, activation, whole)], activation=activation)
-        taken = taken and n < 1 << 21 and whole * -(-k // 8) * 8 < (1 << 30) - 1024
+        row = -(-k // 8) * 8
+        taken = taken and n < 1 << 21 and whole * row < (1 << 30) - 1024
+        # the weights' gradients take tokens in at most 64 parts, the rows of each within 2^31 bytes
+        taken = taken and -(-t // 4096) <= ((1 << 30) - 1024) // (64 * max(2 * whole, row, 1))
         (dx,) = _operator("gated_input_grad", taken, [dgu, gate, up],
                           lambda *xs: [_gated_input_grad(*xs, whole)], features=n)
         # tokens in whole k tiles and whole rows: the plan's own dots, which take an update of the weight into their stores

@@ -679,3 +679,29 @@ def test_gated_launches_stay_below_2_to_the_32_threads():
     for n, fusions in [((1 << 26) - 1, ["gated_linear"]), (1 << 26, [])]:
         g = L.make_graph(F_gated)(_m((1, 8)), _m((n, 8)), _m((n, 8)))
         assert [m.params["name"] for m in g.nodes if m.prim == "fusion"] == fusions
+
+
+def test_gated_gradients_of_more_tokens_than_the_kernels_take():
+    """Tokens whose rows are past 2^31 bytes in each of 64 parts: the gradients' products are primitives, not an error."""
+    for t, kinds in ((4088 << 12, {"gated_input", "gated_weight"}), ((4088 << 12) + 1, set())):
+        g = L.make_graph(_gated_all)(*(_m(s) for s in ((t, 4100), (8, 4100), (8, 4100), (t, 8))))
+        plan = Plan(g, build_kernels=False)
+        assert {st.kind for st in plan.steps} & {"gated_input", "gated_weight", "gated_both"} == kinds
+    # either side of the border by the library's own word
+    for t, n in ((4088 << 12, 8), (1023 << 12, 8192)):  # rows of 4104 and of 2 * 8192 elements
+        size = C.c_size_t()
+        for more in (0, 1):
+            d = nv.GatedDesc(m=t + more, n=n, k=4100, x_m=4100, w_n=4100, dtype=1, config=-1)
+            g = L.make_graph(_gated_all)(*(_m(s) for s in ((t + more, 4100), (n, 4100), (n, 4100), (t + more, n))))
+            names = [m.params["name"] for m in g.nodes if m.prim == "fusion"]
+            assert ("gated_input_grad" in names) == (not more)
+            if more:
+                with pytest.raises(RuntimeError, match="2\\^31"):
+                    nv.call("nhip_gated_backward_workspace", C.byref(d), C.byref(size))
+            else:
+                nv.call("nhip_gated_backward_workspace", C.byref(d), C.byref(size))
+
+
+def _gated_all(x, gate, up, dh):
+    h, pull = L.vjp(F.gated_linear, x, gate, up)
+    return [h, *pull(dh)]
