@@ -1097,3 +1097,53 @@ def test_sigmoid_gradient_of_large_gates(hip, dtype, most, n):
     *x, want = sigmoid_gradient(np.concatenate([g, -g]), n)
     dx = _values(L.compile(_gated_program("sigmoid"), device="hip")(*(_tensor(v, dtype) for v in x))[1])
     _near(dx, want, (2.01 * U[dtype] + 64 * F32) * want)
+
+
+@pytest.mark.parametrize("b,s,n,nkv,d", [(1, 200, 16, 16, 128), (4, 300, 32, 8, 64), (3, 33, 6, 2, 80), (1, 131, 3, 3, 36), (2, 57, 5, 1, 7)])
+def test_heads_weight_gradients_hold_every_row_once(hip, b, s, n, nkv, d):
+    """float32 heads, so that no rounding of the result hides a row: each term's own error, 40 roundings (a row's sum of squares is
+    at most 8 elements a lane and 6 exchanges, its root, mean and factors a dozen more), and at most 161 additions on its way
+    (8 rows a lane, 6 exchanges, 3 waves, 2050 partial rows as 129 and 15). A row's share is over twice
+    that in some element: of one lost or counted twice more than the tolerance would be left."""
+    rot = d // 2 * 2
+    x = _heads_case(100 + d, b, s, n, nkv, d, rot, "float32", table=512)
+    f = L.compile(_heads_program(list(x), False, 1e-3), device="hip")
+    got = [_values(t) for t in f(*[L.from_numpy(v) if m in ("cos", "sin", "positions") else _tensor(v, "float32") for m, v in x.items()])]
+    want = M.heads(x, 1e-3, False)
+    for i, h, g, w in ((4, "q", "gq", "wq"), (5, "k", "gk", "wk")):
+        at = x["positions"].astype(int)
+        c, sn = (np.float64(x[t])[at][:, :, None] for t in ("cos", "sin"))
+        xhat = x[h] / np.sqrt((x[h] ** 2).mean(-1, keepdims=True) + 1e-3)
+        p, q, rest = x[g][..., :rot // 2], x[g][..., rot // 2:rot], x[g][..., rot:]
+        dz = np.concatenate([p * c + q * sn, q * c - p * sn, rest], -1)
+        terms = (dz * xhat).reshape(-1, d)
+        mags = (np.concatenate([np.abs(p) + np.abs(q), np.abs(p) + np.abs(q), np.abs(rest)], -1) * np.abs(xhat)).reshape(-1, d).sum(0)
+        assert np.allclose(terms.sum(0), want[i], rtol=1e-10, atol=1e-9)
+        tol = U["float32"] * np.abs(want[i]) + F32 * (161 + 40) * mags
+        assert np.all((np.abs(terms) / tol).max(1) > 2)
+        _near(got[i], want[i], tol, w)
+
+
+@pytest.mark.parametrize("d", [1, 4])
+def test_heads_weight_gradients_hold_every_launch_once(hip, d):
+    """2^26 + 24 rows, three launches, on the general and the vector kernel: cotangents of 1, 2, .. 64 in rows at the launches'
+    borders, zeros elsewhere. Of heads of equal elements dw is their sum, 127, which bf16 holds: exact."""
+    rows = (1 << 26) + 24
+    x, dy, dx = (Dev(nbytes=2 * rows * d) for _ in range(3))
+    nv.call("nhip_memset", C.c_void_p(x.ptr), 0x3c, C.c_size_t(2 * rows * d))
+    nv.call("nhip_memset", C.c_void_p(dy.ptr), 0, C.c_size_t(2 * rows * d))
+    for i, row in enumerate((0, 12345, (1 << 25) - 1, 1 << 25, (1 << 26) - 1, 1 << 26, rows - 1)):
+        bits = np.ascontiguousarray(D.from_values(np.full(d, 2.0**i, np.float32), "bfloat16"))
+        nv.h2d(dy.ptr + 2 * row * d, bits.ctypes.data, 2 * d)
+    w, table, dw = Dev(np.full(d, 0x3f80, np.uint16)), Dev(np.zeros(4, np.float32)), Dev(nbytes=256)
+    desc = nv.HeadsDesc(batch=1, seq=rows, heads=1, kv_heads=0, head_dim=d, rot=0, table_rows=1, dtype=1, eps=0.0)
+    for m in ("q", "oq", "dq"):
+        setattr(desc, m + "_s", d)
+        setattr(desc, m + "_n", d)
+    size = C.c_size_t()
+    nv.call("nhip_qk_norm_rope_workspace", C.byref(desc), C.byref(size))
+    assert size.value == 3 * 2050 * d * 4
+    ws = Dev(nbytes=size.value)
+    nv.call("nhip_qk_norm_rope_bwd", C.byref(desc), x.ptr, x.ptr, w.ptr, w.ptr, table.ptr, table.ptr, None, dy.ptr, dy.ptr,
+            dx.ptr, dx.ptr, dw.ptr, None, ws.ptr)
+    assert D.to_numpy_values(dw.get((d,), np.uint16), "bfloat16").tolist() == [127.0] * d
