@@ -274,7 +274,8 @@ int nhip_qk_norm_rope_workspace(const nhip_heads_desc *desc, size_t *bytes);
  * float32 [m, n], the two products, which nhip_gated_linear_grad needs. Rows of a multiple of 8 elements that start on 16
  * bytes are read in place (such operands have to start there); others, above 64 rows of x, are copied. `workspace`, of
  * nhip_gated_linear_workspace bytes from a 16-byte address, holds such copies and the sums of a product in parts (null where
- * that is 0). k is below 2^30 up to 64 rows of x, else 1 to 2^21 - 1. */
+ * that is 0). k is below 2^30 up to 64 rows of x, else 1 to 2^21 - 1. A launch has fewer than 2^32 threads: 512 (256 from 33 rows
+ * on) for each 16 of n up to 64 rows of x, 256 or 512 a tile of 128 x 64 or 256 x 128 otherwise. */
 enum {
     NHIP_ACT_SILU = 0,
     NHIP_ACT_GELU = 1,     /* the tanh form */

@@ -374,7 +374,9 @@ def gated_linear(input, gate_weight, up_weight, activation="silu"):
     """``act(input @ gate_weight^T) * (input @ up_weight^T)``, the widening half of a gated MLP: ``input`` ``[..., K]``
     and both weights ``[F, K]`` of one float dtype give ``[..., F]`` of it. ``activation`` is ``"silu"``, ``"gelu"`` (the
     tanh form), ``"relu"`` or ``"sigmoid"``. Both products and everything after them are float32 (float64 of float64
-    operands), rounded once. The backward holds the two products, float32 ``[..., F]`` each."""
+    operands), rounded once. The backward holds the two products, float32 ``[..., F]`` each, and rounds their gradients to
+    the operands' dtype, as operands of the products that give the gradients of ``input`` and the weights, which are rounded
+    again. bfloat16 and float16 run as kernels of their own, other dtypes as their primitives."""
     op = "gated_linear"
     x, gate, up = lift(input), lift(gate_weight), lift(up_weight)
     if activation not in ACTIVATIONS:
