@@ -1147,3 +1147,38 @@ def test_heads_weight_gradients_hold_every_launch_once(hip, d):
     nv.call("nhip_qk_norm_rope_bwd", C.byref(desc), x.ptr, x.ptr, w.ptr, w.ptr, table.ptr, table.ptr, None, dy.ptr, dy.ptr,
             dx.ptr, dx.ptr, dw.ptr, None, ws.ptr)
     assert D.to_numpy_values(dw.get((d,), np.uint16), "bfloat16").tolist() == [127.0] * d
+
+
+def test_operands_and_cotangents_that_are_broadcast(hip):
+    """One token's row for all rows, one head for all heads (strides of 0), and losses that are plain sums, whose cotangents are
+    ones, or take the queries alone, so that the keys' are zeros."""
+    x, gate, up, _ = _gated_case(110, 1, 64, 40, "bfloat16")
+    for t in (70, 9):
+        def gated(x, gate, up, t=t):
+            F.sum(F.gated_linear(x.expand(t, 64), gate, up).float()).backward()
+            return [F.gated_linear(x.expand(t, 64), gate, up), x.grad, gate.grad, up.grad]
+
+        rows, ones = np.repeat(x, t, 0), np.ones((t, 40))
+        want, tol = M.gated(rows, gate, up, ones, "silu"), _gated_tolerances(rows, gate, up, ones, "silu", "bfloat16")
+        got = [_values(v) for v in L.compile(gated, device="hip")(*(_tensor(v, "bfloat16") for v in (x, gate, up)))]
+        for i in (0, 2, 3):
+            _near(got[i], want[i], tol[i], i)
+        each = want[1].sum(0, keepdims=True)  # t rounded gradients and their sum's roundings
+        _near(got[1], each, tol[1].sum(0, keepdims=True) + (U["bfloat16"] + t * F32) * (np.abs(want[1]) + tol[1]).sum(0), "dx")
+    h = _heads_case(111, 2, 9, 1, 1, 64, 64, "bfloat16", positions=False)
+    args = [_tensor(h[m], "float32" if m in ("cos", "sin") else "bfloat16") for m in ("q", "k", "cos", "sin", "wq", "wk")]
+
+    def heads(q, k, cos, sin, wq, wk):
+        yq, yk = F.qk_norm_rope(q.expand(2, 9, 3, 64), k, cos, sin, wq, wk, eps=1e-3)
+        F.sum(yq.float()).backward()
+        return [yq, yk, wq.grad, k.grad if k.grad is not None else k * 0.0]
+
+    h["q"], h["gq"], h["gk"] = np.repeat(h["q"], 3, 2), np.ones((2, 9, 3, 64)), np.zeros((2, 9, 1, 64))
+    want = M.heads(h, 1e-3, False)
+    f = L.compile(heads, device="hip")
+    got = [_values(v) for v in f(*args)]
+    for a, w in zip(got[:2], want):
+        _near(a, w, U["bfloat16"] * np.abs(w) + F32 * 104 * 8 * np.abs(w).max())
+    xhat = np.abs(h["q"]) / np.sqrt((h["q"] ** 2).mean(-1, keepdims=True) + 1e-3)
+    _near(got[2], want[4], U["bfloat16"] * np.abs(want[4]) + F32 * 201 * 2 * xhat.sum((0, 1, 2)), "dw")
+    assert not got[3].any() and {"heads_fwd", "heads_bwd"} <= {st.kind for st in f.plan.steps}
