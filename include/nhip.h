@@ -332,6 +332,61 @@ int nhip_clip_grad_norm(const nhip_clip_desc *desc, const nhip_clip_tensor *tens
                         float *scale, void *workspace);
 int nhip_clip_grad_norm_workspace(const nhip_clip_desc *desc, size_t *bytes);
 
+/* ---- packed self attention (no counterpart in the reference) ------------------------------------------------------ *
+ *
+ * Attention of tokens [tokens, heads, head_dim] within sequences that lie one after another: token t is of sequence i where
+ * offsets[i] <= t < offsets[i + 1], and attends to that sequence's tokens (up to itself if causal). Offsets, sequences + 1 of
+ * them on the device, do not decrease; whatever they hold, they are read as clamped into [the one before, tokens]. Tokens of
+ * no sequence are left out: their results are zeros, and nothing of them (nor of another sequence) reaches any other.
+ * The forward writes o and, unless null, lse (float32 [heads, tokens]; only the sequences' tokens), which the backward reads.
+ * Head dims are multiples of 8 up to 128, V's (and O's) in value_head_dim where it differs (0: the same); rows start on 16
+ * bytes (strides are multiples of 8 elements). Grouped heads' dK and dV are summed over each group. The same bits every run.
+ * ds_bytes: what the backward's workspace may hold of dS (16-bit, computed once; 0, or sequences too long for it: computed
+ * again for dQ). Workspaces of nhip_packed_workspace bytes from a 16-byte address. */
+typedef struct {
+    int64_t tokens, sequences, heads, kv_heads, head_dim, value_head_dim;
+    int64_t q_s, q_n, k_s, k_n, v_s, v_n, o_s, o_n;              /* elements from a token, and a head, to the next */
+    int64_t do_s, do_n, dq_s, dq_n, dk_s, dk_n, dv_s, dv_n;      /* backward */
+    int64_t ds_bytes;
+    int32_t dtype, causal, offsets_dtype;                        /* NHIP_BF16/F16; NHIP_POS_I32/I64 */
+    float scale;
+} nhip_packed_desc;
+
+int nhip_packed_fwd(const nhip_packed_desc *desc, const void *q, const void *k, const void *v, const void *offsets, void *o, float *lse,
+                    void *workspace);
+int nhip_packed_bwd(const nhip_packed_desc *desc, const void *q, const void *k, const void *v, const void *offsets, const void *o,
+                    const void *d_o, const float *lse, void *dq, void *dk, void *dv, void *workspace);
+int nhip_packed_workspace(const nhip_packed_desc *desc, int backward, size_t *bytes);
+
+/* ---- AdamW (no counterpart in the reference) --------------------------------------------------------------------- *
+ *
+ * One step over every element of every tensor, t counting steps from 1:
+ *   m' = beta1 m + (1 - beta1) g, v' = beta2 v + (1 - beta2) g^2,
+ *   w' = w (1 - lr weight_decay) - lr / (1 - beta1^t) m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
+ * with w the master where there is one (float32, of 16-bit weights; the weight is then written and not read) and else the
+ * weight. Float32 throughout, the step's factors worked out in float64. lr_at (a device float64)
+ * and step_at (on the device too, of step_type) are read in place of lr and step where they are not null. grad_scale_at: a device float32 that every gradient is multiplied by first, rounded to
+ * its type again, or null. Results may be null where nothing reads them, and each may lie over the operand that it
+ * replaces, otherwise over none. One launch for each 44 tensors. */
+typedef struct {
+    const void *param, *grad;
+    const float *m, *v, *master;              /* master: or null */
+    void *param_out;
+    float *m_out, *v_out, *master_out;
+    int64_t numel;
+    int32_t dtype;   /* of param, grad and param_out: NHIP_F32, NHIP_BF16 or NHIP_F16 */
+    int32_t pad;
+} nhip_adamw_tensor;
+typedef struct {
+    int64_t count;   /* tensors */
+    double lr, step, beta1, beta2, eps, weight_decay;
+    int32_t step_type;   /* NHIP_POS_NONE: float64, NHIP_POS_I32, NHIP_POS_I64 */
+    int32_t pad;
+} nhip_adamw_desc;
+
+int nhip_adamw(const nhip_adamw_desc *desc, const nhip_adamw_tensor *tensors, const double *lr_at, const void *step_at,
+               const float *grad_scale_at);
+
 /* ---- static plans (lumen/plan/run.rs:356-427 execute; lumen/plan/step/cuda.rs:17-63) ----------------- *
  *
  * A plan is a list of steps run in order on the stream: generated kernels (a function of a loaded module)
@@ -370,6 +425,11 @@ enum {
     NHIP_STEP_GATED_INPUT = 12,  /* desc: nhip_gated_desc; pointers: dgu, gate, up, dx, workspace (or none) */
     NHIP_STEP_GATED_WEIGHT = 13, /* desc: nhip_gated_desc; pointers: dgu, x, d_gate, d_up, workspace (or none) */
     NHIP_STEP_GATED_BACKWARD = 14, /* desc: nhip_gated_desc; pointers: dgu, gate, up, x, dx, d_gate, d_up, workspace (or none) */
+    NHIP_STEP_ADAMW = 15,     /* desc: nhip_adamw_desc, then its nhip_adamw_tensors (pointers ignored); pointers: lr_at, step_at,
+                                 grad_scale_at (each or none), then tensor i's param, grad, m, v, master, param_out, m_out,
+                                 v_out, master_out from 3 + 9 i on (or none) */
+    NHIP_STEP_PACKED_FWD = 16, /* desc: nhip_packed_desc; pointers: q, k, v, offsets, o, lse (or none), workspace */
+    NHIP_STEP_PACKED_BWD = 17, /* desc: nhip_packed_desc; pointers: q, k, v, offsets, o, do, lse, dq, dk, dv, workspace */
 };
 
 int nhip_plan_create(void **plan);

@@ -657,10 +657,19 @@ def backward_mode(batch=0, heads=0, sq=0, sk=0) -> int:
         return 0
     if not config.compiler.attention_store_ds:
         return 2
+    return 2 if ds_bytes(batch, heads, sq, sk) > stored_ds_bytes() else 1
+
+
+def stored_ds_bytes() -> int:
+    """Bytes of dS tiles that one attention's backward may store."""
+    from lumen_amd.config import config
+
+    if not config.compiler.attention_store_ds:
+        return 0
     cap = config.compiler.attention_ds_max_bytes
     if config.compiler.memory_limit:
         cap = min(cap, config.compiler.memory_limit // 8)
-    return 2 if ds_bytes(batch, heads, sq, sk) > cap else 1
+    return cap
 
 
 def ds_bytes(batch, heads, sq, sk) -> int:

@@ -1,4 +1,4 @@
-"""Lowering of the operators of ``functional/operators.py``: a ``fusion`` of each name becomes a built-in step whose
+"""Lowering of the operators of ``functional/operators.py``, ``optimizer.py`` and ``packed.py``: a ``fusion`` of each name becomes a built-in step whose
 descriptor and pointers this module makes from the operands' places (``include/nhip.h``).
 
 Unlike the generated kernels these read rows: an operand whose view would not keep its last axis contiguous (or, where
@@ -20,14 +20,17 @@ KINDS = {
     "gated_input_grad": "gated_input",
     "gated_weight_grad": "gated_weight",
     "clip_grad_norm": "clip",
+    "adamw": "adamw",
+    "packed_attention": "packed_fwd",
+    "packed_attention_backward": "packed_bwd",
 }
 BOTH = "gated_both"  # a gated_weight and a gated_input step in one
 STEPS = {*KINDS.values(), BOTH}
 NHIP_DT = {"float32": 0, "bfloat16": 1, "float16": 2}
-# The last axis contiguous; and rows that start on 16 bytes, or all of a length that the library copies itself; every axis
-# contiguous; and from 16 bytes on.
-ROWS, WIDE_ROWS, DENSE, WIDE = "rows", "wide rows", "dense", "wide"
-STRICTER = [ROWS, WIDE_ROWS, DENSE, WIDE]
+# The last axis contiguous; rows that start on 16 bytes; these, or all of a length that the library copies itself; every
+# axis contiguous; and from 16 bytes on.
+ROWS, CHUNK_ROWS, WIDE_ROWS, DENSE, WIDE = "rows", "chunk rows", "wide rows", "dense", "wide"
+STRICTER = [ROWS, WIDE_ROWS, CHUNK_ROWS, DENSE, WIDE]
 
 
 def _wants(node):
@@ -41,6 +44,10 @@ def _wants(node):
         return [WIDE] * len(node.inputs)
     if name == "gated_linear_grad":
         return [ROWS, DENSE, DENSE]
+    if name == "packed_attention":
+        return [CHUNK_ROWS] * 3 + [DENSE]
+    if name == "packed_attention_backward":
+        return [CHUNK_ROWS] * 3 + [DENSE] + [CHUNK_ROWS] * 2 + [DENSE]
     return [DENSE] * len(node.inputs)
 
 
@@ -63,12 +70,14 @@ def reads(loc, want) -> bool:
     """Whether a place has the layout ``want`` (None: any)."""
     if want is None:
         return True
-    if want in (WIDE, WIDE_ROWS) and loc.offset * D.size_of(loc.dtype) % 16:
+    if want in (WIDE, WIDE_ROWS, CHUNK_ROWS) and loc.offset * D.size_of(loc.dtype) % 16:
         return False
     if want in (DENSE, WIDE):
         return loc.contiguous()
     if loc.shape and loc.shape[-1] != 1 and loc.strides[-1] != 1:
         return False
+    if want == CHUNK_ROWS:
+        return all(n == 1 or st % 8 == 0 for n, st in zip(loc.shape[:-1], loc.strides))
     if want == WIDE_ROWS and loc.shape[-1] % 8 == 0:  # [rows, k]; tiles of 256 rows within 2^31 bytes
         return loc.strides[0] % 8 == 0 and 256 * loc.strides[0] + loc.shape[-1] < 1 << 30
     return True
@@ -107,9 +116,14 @@ def scratch_bytes(graph, node) -> int:
         nv.call("nhip_gated_linear_workspace", C.byref(_gated_node_desc(graph, node)), C.byref(n))
     elif name in ("gated_input_grad", "gated_weight_grad"):
         nv.call("nhip_gated_backward_workspace", C.byref(_gated_backward_desc(graph, node)), C.byref(n))
+    elif name in ("packed_attention", "packed_attention_backward"):
+        n.value = _packed_workspace(graph, node)
+        if name != "packed_attention":
+            read = {m.params["index"] for m in graph.nodes if m.prim == "fusion_output" and m.inputs[0] == node.output}
+            n.value += sum(_up256(graph.types[node.inputs[i]].nbytes()) for i in (1, 2) if i not in read)
     elif name == "clip_grad_norm":
         nv.call("nhip_clip_grad_norm_workspace", C.byref(nv.ClipDesc(count=len(_clip_grads(node)))), C.byref(n))
-    return -(-n.value // 256) * 256
+    return _up256(n.value)
 
 
 def pair_gradients(graph, steps) -> list:
@@ -155,7 +169,8 @@ def lower(plan, step):
         return _lower_heads(plan, step)
     return {"gated_linear": _lower_gated, "gated_linear_grad": _lower_gated_grad,
             "gated_input_grad": _lower_gated_backward, "gated_weight_grad": _lower_gated_backward,
-            "clip_grad_norm": _lower_clip}[name](plan, step)
+            "clip_grad_norm": _lower_clip, "adamw": _lower_adamw,
+            "packed_attention": _lower_packed, "packed_attention_backward": _lower_packed}[name](plan, step)
 
 
 def _slots(places):
@@ -273,21 +288,164 @@ def _lower_clip(plan, step):
     return nv.NHIP_STEP_CLIP, bytes(d) + bytes(tensors), ops
 
 
+def _packed_desc(graph, node):
+    """``nhip_packed_desc`` of a packed attention node without its strides."""
+    from lumen_amd import native as nv
+    from lumen_amd.compiler.attention import stored_ds_bytes
+
+    q, k, v, offsets = (graph.types[u] for u in node.inputs[:4])
+    d = nv.PackedDesc(causal=int(node.params["causal"]), scale=node.params["scale"], dtype=NHIP_DT[q.dtype])
+    d.tokens, d.heads, d.head_dim = q.shape
+    d.kv_heads, d.value_head_dim, d.sequences = k.shape[1], v.shape[2], offsets.shape[0] - 1
+    d.offsets_dtype = nv.NHIP_POS_I64 if offsets.dtype == "int64" else nv.NHIP_POS_I32
+    d.ds_bytes = stored_ds_bytes()
+    return d
+
+
+def _packed_workspace(graph, node) -> int:
+    from lumen_amd import native as nv
+
+    n = C.c_size_t()
+    nv.call("nhip_packed_workspace", C.byref(_packed_desc(graph, node)), int(node.params["name"] != "packed_attention"), C.byref(n))
+    return _up256(n.value)
+
+
+def _up256(n) -> int:
+    return -(-n // 256) * 256
+
+
+def _dense(t, at):
+    """A contiguous place of type ``t`` at byte ``at`` of the workspace."""
+    from lumen_amd.compiler.plan import Loc, _contig
+
+    return Loc(("ws", 0), at // D.size_of(t.dtype), _contig(t.shape), t.dtype, t.shape)
+
+
+def _lower_packed(plan, step):
+    from lumen_amd import native as nv
+
+    node = step.nodes[0]
+    d, out = _packed_desc(plan.graph, node), _outputs(plan, step)
+    at = [plan.loc[v] for v in node.inputs]
+    backward = step.kind == "packed_bwd"
+    names = [("q", at[0]), ("k", at[1]), ("v", at[2])]
+    if backward:
+        # the kernels compute all three gradients: one that nothing reads goes into the scratch
+        spare = plan.scratch[id(step)].offset * 4 + _packed_workspace(plan.graph, node)
+        for index, operand in ((1, 1), (2, 2)):
+            if index not in out:
+                t = plan.graph.types[node.inputs[operand]]
+                out[index] = _dense(t, spare)
+                spare += _up256(t.nbytes())
+        names += [("o", at[4]), ("do", at[5]), ("dq", out[0]), ("dk", out[1]), ("dv", out[2])]
+    else:
+        names.append(("o", out[0]))
+    for name, loc in names:
+        d_s, d_n = loc.strides[:2]
+        setattr(d, f"{name}_s", d_s)
+        setattr(d, f"{name}_n", d_n)
+    scratch = plan.scratch[id(step)]
+    if not backward:
+        return nv.NHIP_STEP_PACKED_FWD, bytes(d), _slots([*at, out[0], out.get(1), scratch])
+    return nv.NHIP_STEP_PACKED_BWD, bytes(d), _slots([*at, *(loc for _, loc in names[5:]), scratch])
+
+
+def _adamw_tensors(node):
+    """The operands of each of an ``adamw`` node's weights: its values (or its master's), gradient and moments."""
+    from lumen_amd.functional.optimizer import OPERANDS, adamw_scalars
+
+    rest = node.inputs[len(adamw_scalars(node.params)):]
+    return [rest[i:i + OPERANDS] for i in range(0, len(rest), OPERANDS)]
+
+
+def _adamw_results(node):
+    """The index in the body's results of each weight's new value, moments and (None: none) master."""
+    masters = node.params["masters"]
+    n, at = len(masters), iter(range(3 * len(masters), 4 * len(masters)))
+    return [(i, n + i, 2 * n + i, next(at) if m else None) for i, m in enumerate(masters)]
+
+
+def _lower_adamw(plan, step):
+    from lumen_amd import native as nv
+    from lumen_amd.functional.optimizer import adamw_scalars
+
+    node, g, p = step.nodes[0], plan.graph, step.nodes[0].params
+    names, out = adamw_scalars(p), _outputs(plan, step)
+    weights = _adamw_tensors(node)
+    d = nv.AdamwDesc(count=len(weights), lr=p["lr"] or 0.0, step=p["step"] or 1.0, beta1=p["beta1"], beta2=p["beta2"],
+                     eps=p["eps"], weight_decay=p["weight_decay"])
+    if "step" in names:
+        d.step_type = {"int32": nv.NHIP_POS_I32, "int64": nv.NHIP_POS_I64}.get(g.types[node.inputs[names.index("step")]].dtype,
+                                                                              nv.NHIP_POS_NONE)
+    tensors = (nv.AdamwTensor * len(weights))()
+    ops = [(("lr", "step", "scale").index(n), plan.loc[v]) for n, v in zip(names, node.inputs)]
+    for i, ((w, grad, m, v), results) in enumerate(zip(weights, _adamw_results(node))):
+        t = g.types[grad]
+        tensors[i].numel, tensors[i].dtype = t.numel(), NHIP_DT[t.dtype]
+        new, first, second, master = (out.get(j) for j in results)
+        places = [None if p["masters"][i] else plan.loc[w], plan.loc[grad], plan.loc[m], plan.loc[v],
+                  plan.loc[w] if p["masters"][i] else None, new, first, second, master]
+        ops += [(3 + 9 * i + j, loc) for j, loc in enumerate(places) if loc is not None]
+    return nv.NHIP_STEP_ADAMW, bytes(d) + bytes(tensors), ops
+
+
+def writes_over(graph, node, result, operand) -> bool:
+    """Whether a step of ``node`` may write its ``result`` over its operand ``operand``, or over another value that it does
+    not read: an element of a weight's results is written by the thread that has read that element of its operands."""
+    if node.params["name"] != "adamw":
+        return False
+    index = next((n.params["index"] for n in graph.nodes if n.prim == "fusion_output" and n.output == result), 0)
+    own = next(k for k, r in enumerate(_adamw_results(node)) if index in r)
+    return operand not in node.inputs[:len(node.inputs) - sum(map(len, _adamw_tensors(node)))] \
+        and all(k == own for k, xs in enumerate(_adamw_tensors(node)) if operand in xs)
+
+
+def _clipped_steps(graph, clips, users):
+    """The ``adamw`` nodes that may take the clipping's scale themselves, by output: every gradient of theirs is a result of
+    one clipping that only such nodes (as their gradients) and elementwise ones read."""
+    from lumen_amd.functional.optimizer import OPERANDS, adamw_scalars
+
+    clipped = {n.output: n.inputs[0] for n in graph.nodes if n.prim == "fusion_output" and n.inputs[0] in clips
+               and n.params["index"] >= 2 and n.output not in graph.outputs}
+    steps = {n.output: n for n in graph.nodes if n.prim == "fusion" and n.params.get("name") == "adamw"
+             and not n.params["scaled"]}
+
+    def gradients(n):
+        return n.inputs[len(adamw_scalars(n.params)) + 1::OPERANDS]
+
+    def only_gradients(v, u):
+        return u.output in steps and u.inputs.count(v) == gradients(u).count(v)
+
+    while True:
+        bad = [k for k, n in steps.items() if len({clipped.get(v) for v in gradients(n)} | {None}) != 2
+               or any(v not in clipped or not all(u.prim in ELEMENTWISE or only_gradients(v, u) for u in users[v])
+                      for v in gradients(n))]
+        if not bad:
+            return steps
+        for k in bad:
+            del steps[k]
+
+
 def clip_in_consumers(graph: Graph) -> Graph:
-    """A clipped gradient that only elementwise nodes read (an optimizer's update) is multiplied by the scale there
-    instead of being written by the clipping step and read again: the same values, one pass over the gradient less."""
+    """A clipped gradient that only elementwise nodes and AdamW steps read (an optimizer's update) is multiplied by the
+    scale there instead of being written by the clipping step and read again: the same values, one pass over the gradient
+    less."""
+    from lumen_amd.functional.optimizer import OPERANDS, adamw_body, adamw_scalars
+    from lumen_amd.graph import tracer
     from lumen_amd.graph.ir import TensorType
 
     users = graph.users()
     clips = {n.output: n for n in graph.nodes if n.prim == "fusion" and n.params.get("name") == "clip_grad_norm"}
+    steps = _clipped_steps(graph, clips, users) if clips else {}
     moved = {}
     for n in graph.nodes:
         if n.prim == "fusion_output" and n.inputs[0] in clips and n.params["index"] >= 2 \
                 and n.output not in graph.outputs and users.get(n.output) \
-                and all(u.prim in ELEMENTWISE for u in users[n.output]):
+                and all(u.prim in ELEMENTWISE or u.output in steps for u in users[n.output]):
             moved[n.output] = _clip_grads(clips[n.inputs[0]])[n.params["index"] - 2]
     if not moved:
         return graph
+    clip_of = {n.output: n.inputs[0] for n in graph.nodes if n.output in moved}
     g = Graph()
     remap = {v: g.input(graph.types[v].dtype, graph.types[v].shape) for v in graph.inputs}
     scale = {}
@@ -299,9 +457,29 @@ def clip_in_consumers(graph: Graph) -> Graph:
             scale[clip] = g.add_node("fusion_output", (remap[clip],), {"index": 1, "ty": f32}, f32, backward)
         return scale[clip]
 
+    def scaled_step(n):
+        """The AdamW step over the gradients as they were, with their scale."""
+        names = adamw_scalars(n.params)
+        head, rest = [remap[v] for v in n.inputs[:len(names)]], list(n.inputs[len(names):])
+        clip = clip_of[rest[1]]
+        ins = head + [scale_of(clip, n.backward)] + [
+            remap[moved[v]] if i % OPERANDS == 1 else remap[v] for i, v in enumerate(rest)]
+        params = {k: v for k, v in n.params.items() if k not in ("name", "body")}
+        params["scaled"] = True
+        body = Graph()
+        xs = [tracer.TracedTensor(body, body.input(g.types[v].dtype, g.types[v].shape)) for v in ins]
+        with tracer.tracing(body):
+            body.set_outputs([r.var for r in adamw_body(xs, params)])
+        return g.add_node("fusion", tuple(ins), dict(params, name="adamw", body=body), graph.types[n.output], n.backward)
+
     for n in graph.nodes:
+        if n.output in steps:
+            remap[n.output] = scaled_step(n)
+            continue
         if n.output not in moved:
             remap[n.output] = g.add_node(n.prim, tuple(remap[v] for v in n.inputs), n.params, graph.types[n.output], n.backward)
+            continue
+        if not any(u.prim in ELEMENTWISE for u in users[n.output]):
             continue
         ty = graph.types[n.output]
         wide = TensorType("float32", ty.shape)

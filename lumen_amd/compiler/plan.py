@@ -340,6 +340,8 @@ class Plan:
                 body, others = member.nodes, [m for m in st.members if m is not member]
             elif st.kind == "dot" and getattr(st, "epi", None) is not None:
                 body, others = st.epi.nodes, [st.nodes[0]]
+            elif st.kind in operators.STEPS and operators.writes_over(g, st.nodes[0], v, u):
+                body, others = [], []
             else:
                 continue
             # nothing reads the input's memory after the step, nor in it but through `body` at its own element

@@ -209,8 +209,9 @@ template <int NW, int D = 128> struct FwdOccupancy {
 // LDS read would be taken to alias the loads just issued into the other half and wait for them (s_waitcnt vmcnt(0)
 // before the tile's first read), so that nothing overlapped. [8, 2048, 16, 128] causal 243 -> 192-203 us (679-716
 // TFLOP/s), [2, 1777, 16 / 4, 64] 43 -> 37. ONE: halves of one array after all, for fewer registers (launch_fwd_nw).
+// One workgroup's queries [32 NW qblk, 32 NW (qblk + 1)) of head n of batch b.
 template <int D, bool F16, bool CAUSAL, int NW, bool ONE = false>
-__device__ __forceinline__ void flash_fwd_body(const AttnParams &p) {
+__device__ __forceinline__ void flash_fwd_tile(const AttnParams &p, int64_t b, int64_t n, int64_t qblk) {
     constexpr int QB = 32 * NW;  // queries a workgroup
     constexpr int BN = 64;
     constexpr int DS = D / 16, DT = D / 32;
@@ -220,11 +221,6 @@ __device__ __forceinline__ void flash_fwd_body(const AttnParams &p) {
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, l32 = lane & 31;
     const int g = lane >> 4, s16 = lane & 15;
-    const int64_t nqb = (p.sq + QB - 1) / QB;
-    int64_t unit, qblk;
-    xcd_order(int64_t(gridDim.x) / nqb, nqb, unit, qblk);
-    if (CAUSAL) qblk = nqb - 1 - qblk;  // longest rows first
-    const int64_t b = unit / p.heads, n = unit % p.heads;
     const int64_t nkv = n / (p.heads / p.kv_heads);
     const int64_t q0 = qblk * QB;
     const int64_t qi = q0 + wave * 32 + l32;
@@ -372,6 +368,15 @@ __device__ __forceinline__ void flash_fwd_body(const AttnParams &p) {
     if (h == 0 && p.lse) p.lse[(b * p.heads + n) * p.sq + qi] = l > 0.0f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY;
 }
 
+template <int D, bool F16, bool CAUSAL, int NW, bool ONE = false>
+__device__ __forceinline__ void flash_fwd_body(const AttnParams &p) {
+    const int64_t nqb = (p.sq + 32 * NW - 1) / (32 * NW);
+    int64_t unit, qblk;
+    xcd_order(int64_t(gridDim.x) / nqb, nqb, unit, qblk);
+    if (CAUSAL) qblk = nqb - 1 - qblk;  // longest rows first
+    flash_fwd_tile<D, F16, CAUSAL, NW, ONE>(p, unit / p.heads, unit % p.heads, qblk);
+}
+
 template <int D, bool F16, bool CAUSAL, int NW = 4, int WAVES = FwdOccupancy<NW, D>::kBlocks>
 __global__ __launch_bounds__(64 * NW, WAVES) void flash_fwd_kernel(AttnParams p) {
     flash_fwd_body<D, F16, CAUSAL, NW, (NW == 4 && WAVES == 4)>(p);
@@ -482,8 +487,11 @@ template <bool CAUSAL, bool ATOMIC_DQ> struct DkdvPaired { static constexpr bool
 
 // STORE_DS (the deterministic mode's default): each tile's dS (rounded as for dK) is stored to p.ds for the
 // dQ = dS K kernel, instead of a second kernel recomputing S and dP.
-template <int D, bool F16, bool CAUSAL, bool ATOMIC_DQ = false, bool STORE_DS = false>
-__global__ __launch_bounds__(256) void flash_dkdv_kernel(AttnParams p, const float *lse2) {
+// Key block pidx (PAIR: and nkb - 1 - pidx) of nkb of key head nkv of batch b; a head's statistics are `ls` floats after the
+// last one's.
+template <int D, bool F16, bool CAUSAL, bool ATOMIC_DQ, bool STORE_DS, bool PAIR>
+__device__ __forceinline__ void flash_dkdv_tile(const AttnParams &p, const float *lse2, int64_t b, int64_t nkv, int64_t pidx,
+                                                int64_t nkb, int64_t ls) {
     constexpr int BM = 64;
     constexpr int DS = D / 16, DT = D / 32;
     constexpr int TILE = BM * D;
@@ -499,15 +507,6 @@ __global__ __launch_bounds__(256) void flash_dkdv_kernel(AttnParams p, const flo
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, l32 = lane & 31;
     const int g = lane >> 4, s16 = lane & 15;
-    const int64_t nkb = (p.sk + 127) / 128;
-    // causal (but for the atomic mode, whose registers it would spill): a workgroup takes key blocks i and
-    // nkb - 1 - i (every workgroup then has the same number of query tiles but for the middle block of an odd
-    // count), so no workgroup is left running alone at the end
-    constexpr bool PAIR = DkdvPaired<CAUSAL, ATOMIC_DQ>::value;
-    const int64_t per = PAIR ? (nkb + 1) / 2 : nkb;
-    int64_t unit, pidx;
-    xcd_order(int64_t(gridDim.x) / per, per, unit, pidx);
-    const int64_t b = unit / p.kv_heads, nkv = unit % p.kv_heads;
     const bool partial = p.sq % BM || (ATOMIC_DQ && p.sk % 128) || p.hd < D || p.hdv < D;
     zero_tiles(stage0, 2 * TILE, partial);
     zero_tiles(stage1, 2 * TILE, partial);
@@ -533,24 +532,24 @@ __global__ __launch_bounds__(256) void flash_dkdv_kernel(AttnParams p, const flo
     if (CAUSAL) qstart = max<int64_t>(0, kb0 - shift) / BM * BM;
     const int per_head = p.sq > qstart ? int((p.sq - qstart + BM - 1) / BM) : 0;
     const int total = per_head * int(group);
-    auto tile_src = [&](int j, const uint16_t *&qp, const uint16_t *&gp, const float *&ls, const float *&dl,
+    auto tile_src = [&](int j, const uint16_t *&qp, const uint16_t *&gp, const float *&lp, const float *&dl,
                         int64_t &q0) {
         const int64_t gi = j / per_head;
         q0 = qstart + int64_t(j % per_head) * BM;
         const int64_t n = nkv * group + gi;
         qp = p.q + b * p.q_b + n * p.q_n;
         gp = p.d_o + b * p.do_b + n * p.do_n;
-        ls = lse2 + (b * p.heads + n) * p.sq;
-        dl = p.delta + (b * p.heads + n) * p.sq;
+        lp = lse2 + (b * p.heads + n) * ls;
+        dl = p.delta + (b * p.heads + n) * ls;
     };
     auto issue = [&](int j, uint16_t *dst, float *lse_dst, float *delta_dst) __attribute__((always_inline)) {
         const uint16_t *qp, *gp;
-        const float *ls, *dl;
+        const float *lp, *dl;
         int64_t q0;
-        tile_src(j, qp, gp, ls, dl, q0);
+        tile_src(j, qp, gp, lp, dl, q0);
         load_tile_async<D>(qp, p.q_s, q0, p.sq, dst, wave, lane, p.hd);
         load_tile_async<D>(gp, p.do_s, q0, p.sq, dst + TILE, wave, lane, p.hdv);
-        if (wave == 0) load_row64_async(ls, q0, p.sq, lse_dst, lane);
+        if (wave == 0) load_row64_async(lp, q0, p.sq, lse_dst, lane);
         if (wave == 1) load_row64_async(dl, q0, p.sq, delta_dst, lane);
     };
     if constexpr (ATOMIC_DQ) {  // waited for with the first tile's loads
@@ -601,8 +600,8 @@ __global__ __launch_bounds__(256) void flash_dkdv_kernel(AttnParams p, const flo
         int64_t q0;
         {
             const uint16_t *qp, *gp;
-            const float *ls, *dl;
-            tile_src(j, qp, gp, ls, dl, q0);
+            const float *lp, *dl;
+            tile_src(j, qp, gp, lp, dl, q0);
         }
         // this thread's loads of tile j have landed; with STORE_DS the previous tile's 4 dS stores, issued after
         // them, may stay in flight (vector memory operations complete in order: vmcnt <= 4)
@@ -850,6 +849,19 @@ __global__ __launch_bounds__(256) void flash_dkdv_kernel(AttnParams p, const flo
     }
 }
 
+template <int D, bool F16, bool CAUSAL, bool ATOMIC_DQ = false, bool STORE_DS = false>
+__global__ __launch_bounds__(256) void flash_dkdv_kernel(AttnParams p, const float *lse2) {
+    const int64_t nkb = (p.sk + 127) / 128;
+    // causal (but for the atomic mode, whose registers it would spill): a workgroup takes key blocks i and
+    // nkb - 1 - i (every workgroup then has the same number of query tiles but for the middle block of an odd
+    // count), so no workgroup is left running alone at the end
+    constexpr bool PAIR = DkdvPaired<CAUSAL, ATOMIC_DQ>::value;
+    const int64_t per = PAIR ? (nkb + 1) / 2 : nkb;
+    int64_t unit, pidx;
+    xcd_order(int64_t(gridDim.x) / per, per, unit, pidx);
+    flash_dkdv_tile<D, F16, CAUSAL, ATOMIC_DQ, STORE_DS, PAIR>(p, lse2, unit / p.kv_heads, unit % p.kv_heads, pidx, nkb, p.sq);
+}
+
 // The atomic dQ accumulator (float32 [B, N, Sq, D]) rounded into dq (its strides): eight head-dim elements a
 // thread, a 16-byte store when dq's rows allow it.
 template <int D, bool F16>
@@ -886,7 +898,7 @@ __global__ __launch_bounds__(256) void flash_dq_round_kernel(AttnParams p) {
 // tile the dK/dV kernel never wrote (all its keys after the tile's queries). dS is read once from HBM: 128
 // bf16 products a byte at D = 128, so the kernel is HBM-bound below ~1 PFLOP/s.
 template <int D, bool F16, bool CAUSAL>
-__global__ __launch_bounds__(256, 2) void flash_dq_ds_kernel(AttnParams p) {
+__device__ __forceinline__ void flash_dq_ds_tile(const AttnParams &p, int64_t b, int64_t n, int64_t qb) {
     constexpr int KT = 64, QB = 256, KS = KT / 16;
     constexpr int DSB = 128 * 64;                                     // one dS tile, elements
     constexpr int FN = D / 32;                                        // 32-column MFMA tiles of the head dim
@@ -906,11 +918,6 @@ __global__ __launch_bounds__(256, 2) void flash_dq_ds_kernel(AttnParams p) {
     };
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, l32 = lane & 31;
     const int g = lane >> 4, s16 = lane & 15;
-    const int64_t nqb = (p.sq + QB - 1) / QB;
-    const int64_t units = int64_t(gridDim.x) / nqb;  // batch x heads
-    const int64_t unit = blockIdx.x % units;
-    const int64_t qb = nqb - 1 - blockIdx.x / units;  // causal: the last query blocks see the most keys; issued first
-    const int64_t b = unit / p.heads, n = unit % p.heads;
     const int64_t nkv = n / (p.heads / p.kv_heads);
     const int64_t q0 = qb * QB;
     const int64_t nkb = (p.sk + 127) / 128, nqt = (p.sq + 63) / 64;
@@ -1012,10 +1019,20 @@ __global__ __launch_bounds__(256, 2) void flash_dq_ds_kernel(AttnParams p) {
     }
 }
 
+template <int D, bool F16, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void flash_dq_ds_kernel(AttnParams p) {
+    const int64_t nqb = (p.sq + 255) / 256;
+    const int64_t units = int64_t(gridDim.x) / nqb;  // batch x heads
+    const int64_t unit = blockIdx.x % units;
+    const int64_t qb = nqb - 1 - blockIdx.x / units;  // causal: the last query blocks see the most keys; issued first
+    flash_dq_ds_tile<D, F16, CAUSAL>(p, unit / p.heads, unit % p.heads, qb);
+}
+
 // dQ for 128 queries (32 a wavefront), looping over 64-key tiles: S^T and dP^T one query a lane, dQ^T
 // accumulated in registers (deterministic: no atomics).
 template <int D, bool F16, bool CAUSAL>
-__global__ __launch_bounds__(256, 2) void flash_dq_kernel(AttnParams p, const float *lse2) {
+__device__ __forceinline__ void flash_dq_tile(const AttnParams &p, const float *lse2, int64_t b, int64_t n, int64_t qblk,
+                                              int64_t ls) {
     constexpr int BN = 64;
     constexpr int DS = D / 16, DT = D / 32;
     constexpr int TILE = BN * D;
@@ -1023,11 +1040,6 @@ __global__ __launch_bounds__(256, 2) void flash_dq_kernel(AttnParams p, const fl
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, l32 = lane & 31;
     const int g = lane >> 4, s16 = lane & 15;
-    const int64_t nqb = (p.sq + 127) / 128;
-    int64_t unit, qblk;
-    xcd_order(int64_t(gridDim.x) / nqb, nqb, unit, qblk);
-    if (CAUSAL) qblk = nqb - 1 - qblk;
-    const int64_t b = unit / p.heads, n = unit % p.heads;
     const int64_t nkv = n / (p.heads / p.kv_heads);
     const int64_t q0 = qblk * 128;
     const int64_t qi = q0 + wave * 32 + l32;
@@ -1060,8 +1072,8 @@ __global__ __launch_bounds__(256, 2) void flash_dq_kernel(AttnParams p, const fl
         gf[t] = qvalid && 16 * t + 8 * h < p.hdv ? *reinterpret_cast<const uint4 *>(gp + qi * p.do_s + 16 * t + 8 * h)
                                                  : make_uint4(0, 0, 0, 0);
     }
-    const float l2 = qvalid ? lse2[(b * p.heads + n) * p.sq + qi] : 0.0f;
-    const float dl = qvalid ? p.delta[(b * p.heads + n) * p.sq + qi] : 0.0f;
+    const float l2 = qvalid ? lse2[(b * p.heads + n) * ls + qi] : 0.0f;
+    const float dl = qvalid ? p.delta[(b * p.heads + n) * ls + qi] : 0.0f;
     const float c2 = p.scale * 1.4426950408889634f;
     f32x16_t acc[DT];
 #pragma unroll
@@ -1140,6 +1152,15 @@ __global__ __launch_bounds__(256, 2) void flash_dq_kernel(AttnParams p, const fl
             if (32 * dt + 8 * e4 < p.hd)  // padded columns are not stored
             *reinterpret_cast<uint2 *>(dqp + 32 * dt + 8 * e4 + 4 * h) =
                 make_uint2(pack2<F16>(acc[dt][4 * e4], acc[dt][4 * e4 + 1]), pack2<F16>(acc[dt][4 * e4 + 2], acc[dt][4 * e4 + 3]));
+}
+
+template <int D, bool F16, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void flash_dq_kernel(AttnParams p, const float *lse2) {
+    const int64_t nqb = (p.sq + 127) / 128;
+    int64_t unit, qblk;
+    xcd_order(int64_t(gridDim.x) / nqb, nqb, unit, qblk);
+    if (CAUSAL) qblk = nqb - 1 - qblk;
+    flash_dq_tile<D, F16, CAUSAL>(p, lse2, unit / p.heads, unit % p.heads, qblk, p.sq);
 }
 
 }  // namespace nhipk
@@ -1232,152 +1253,6 @@ inline int check_attn(const nhip_attn_desc *d, const char *what, int64_t max_hd 
     if ((d->sq + 63) / 64 * d->heads * d->batch >= (int64_t(1) << 31) || (d->sk + 127) / 128 * d->heads * d->batch >= (int64_t(1) << 31))
         return fail(std::string(what) + ": more than 2^31 workgroups");
     return 0;
-}
-
-template <int D, bool F16, bool CAUSAL, int NW>
-int launch_fwd_nw(hipStream_t s, const nhipk::AttnParams &p, const nhip_attn_desc *d) {
-    dim3 grid(unsigned((d->sq + 32 * NW - 1) / (32 * NW) * d->heads * d->batch));
-    if constexpr (D == 64 && NW == 4) {
-        // Waves a SIMD: two where a causal launch nearly fits them (FwdOccupancy); four where a launch without a mask
-        // fits them and not three, which would run a second round for a few workgroups (us with three, four: 784
-        // workgroups of 3494 keys 153.3, 148.3; 800 of 1212 58.8, 56.5; 832 of 141 17.6, 17.1; 988 of 6914 316, 308).
-        constexpr int kWaves = CAUSAL ? 2 : 4;
-        if (CAUSAL ? grid.x <= 640 : grid.x > 768 && grid.x <= 1024) {
-            hipLaunchKernelGGL((nhipk::flash_fwd_kernel<D, F16, CAUSAL, NW, kWaves>), grid, dim3(64 * NW), 0, s, p);
-            return check(hipGetLastError(), "flash_fwd launch");
-        }
-    }
-    hipLaunchKernelGGL((nhipk::flash_fwd_kernel<D, F16, CAUSAL, NW>), grid, dim3(64 * NW), 0, s, p);
-    return check(hipGetLastError(), "flash_fwd launch");
-}
-
-template <int D, bool F16, bool CAUSAL>
-int launch_fwd(hipStream_t s, const nhipk::AttnParams &p, const nhip_attn_desc *d) {
-    if constexpr (D > 128) {
-        // head dim 256: 4 waves, one workgroup a CU (its K/V tiles fill 128 KiB of LDS), whatever the config
-        return launch_fwd_nw<D, F16, CAUSAL, 4>(s, p, d);
-    } else {
-        // by default 128 queries a workgroup, or 64 at head dim 64 where there are no more and the workgroups are more
-        // than the CUs hold, three each: waves without a query hold registers that others could use ([32, 1, 32 / 8, 64]
-        // over 1 key 8.9 us, 6.6; over 65 11.6, 7.8; 64 queries over 256 keys 18.9, 16.9; but [32, 1, 16, 64] 5.8, 6.2)
-        switch (d->config >= 0 ? d->config : D == 64 && d->sq <= 64 && d->heads * d->batch > 768 ? 2 : 0) {
-            case 1: return launch_fwd_nw<D, F16, CAUSAL, 8>(s, p, d);
-            case 2: return launch_fwd_nw<D, F16, CAUSAL, 2>(s, p, d);
-            default: return launch_fwd_nw<D, F16, CAUSAL, 4>(s, p, d);
-        }
-    }
-}
-
-// Whether a forward divides the keys over waves (attention_split.h), and that launch: `ws` as
-// flash_fwd_workspace_bytes says, or null for one workgroup a row tile.
-bool split_keys(const nhip_attn_desc *d);
-int launch_split(hipStream_t s, const nhipk::AttnParams &p, const nhip_attn_desc *d, void *ws);
-
-int flash_fwd_on(hipStream_t s, const nhip_attn_desc *d, const void *q, const void *k, const void *v, void *o,
-                 float *lse, void *ws) {
-    if (check_attn(d, "flash attention", 256)) return 1;
-    if (d->sq == 0 || d->batch == 0 || d->heads == 0) return 0;
-    nhipk::AttnParams p = attn_params(d);
-    p.q = static_cast<const uint16_t *>(q);
-    p.k = static_cast<const uint16_t *>(k);
-    p.v = static_cast<const uint16_t *>(v);
-    p.o = static_cast<uint16_t *>(o);
-    p.lse = lse;
-    bool f16 = d->dtype == NHIP_F16;
-    if (split_keys(d)) return launch_split(s, p, d, ws);
-#define NHIP_FWD(DD, FF, CC) return launch_fwd<DD, FF, CC>(s, p, d)
-    const int64_t kd = kernel_dim(d);
-    if (kd == 256) {
-        if (f16) { if (d->causal) NHIP_FWD(256, true, true); NHIP_FWD(256, true, false); }
-        if (d->causal) NHIP_FWD(256, false, true);
-        NHIP_FWD(256, false, false);
-    }
-    if (kd == 128) {
-        if (f16) { if (d->causal) NHIP_FWD(128, true, true); NHIP_FWD(128, true, false); }
-        if (d->causal) NHIP_FWD(128, false, true);
-        NHIP_FWD(128, false, false);
-    }
-    if (f16) { if (d->causal) NHIP_FWD(64, true, true); NHIP_FWD(64, true, false); }
-    if (d->causal) NHIP_FWD(64, false, true);
-    NHIP_FWD(64, false, false);
-#undef NHIP_FWD
-}
-
-template <int D, bool F16, bool CAUSAL>
-int launch_bwd(hipStream_t s, const nhipk::AttnParams &p, const nhip_attn_desc *d) {
-    const bool atomic = p.dqacc != nullptr;
-    dim3 gd(unsigned((d->heads * d->sq + 3) / 4), unsigned(d->batch));
-    // dK/dV: a workgroup per key block, or per pair of key blocks (i, nkb - 1 - i) (nhipk::DkdvPaired)
-    const int64_t nkb = (d->sk + 127) / 128;
-    dim3 gk(unsigned((nhipk::DkdvPaired<CAUSAL, false>::value ? (nkb + 1) / 2 : nkb) * d->kv_heads * d->batch));
-    dim3 gka(unsigned((nhipk::DkdvPaired<CAUSAL, true>::value ? (nkb + 1) / 2 : nkb) * d->kv_heads * d->batch));
-    dim3 gq(unsigned((d->sq + 127) / 128 * d->heads * d->batch));
-    float *lse2 = p.delta + size_t(d->batch) * d->heads * d->sq;
-    // 16-byte rows: D / 8 lanes each; else one wavefront a row
-    const bool vec = d->head_dim == D && value_head_dim(d) == D && D % 8 == 0 && 64 % (D / 8 > 0 ? D / 8 : 1) == 0 && D / 8 <= 64 &&
-                     ((reinterpret_cast<uintptr_t>(p.o_in) | reinterpret_cast<uintptr_t>(p.d_o)) & 15) == 0 &&
-                     (p.o_b | p.o_n | p.o_s | p.do_b | p.do_n | p.do_s) % 8 == 0;
-    if constexpr (D % 8 == 0 && D >= 8 && D <= 512 && 64 % (D / 8) == 0) {
-        if (vec) {
-            constexpr int RPB = 256 / (D / 8);
-            dim3 gv(unsigned((d->heads * d->sq + RPB - 1) / RPB), unsigned(d->batch));
-            hipLaunchKernelGGL((nhipk::flash_prep_vec_kernel<D, F16>), gv, dim3(256), 0, s, p, lse2);
-        } else {
-            hipLaunchKernelGGL((nhipk::flash_prep_kernel<D, F16>), gd, dim3(256), 0, s, p, lse2);
-        }
-    } else {
-        hipLaunchKernelGGL((nhipk::flash_prep_kernel<D, F16>), gd, dim3(256), 0, s, p, lse2);
-    }
-    if (check(hipGetLastError(), "flash delta launch")) return 1;
-    if (atomic) {
-        hipLaunchKernelGGL((nhipk::flash_dkdv_kernel<D, F16, CAUSAL, true>), gka, dim3(256), 0, s, p, lse2);
-        if (check(hipGetLastError(), "flash dkdv+dq launch")) return 1;
-        const int64_t rows = d->batch * d->heads * d->sq;
-        dim3 gc(unsigned((rows * (D / 8) + 255) / 256));
-        hipLaunchKernelGGL((nhipk::flash_dq_round_kernel<D, F16>), gc, dim3(256), 0, s, p);
-        return check(hipGetLastError(), "flash dq rounding launch");
-    }
-    if (p.ds) {
-        hipLaunchKernelGGL((nhipk::flash_dkdv_kernel<D, F16, CAUSAL, false, true>), gk, dim3(256), 0, s, p, lse2);
-        if (check(hipGetLastError(), "flash dkdv+dS launch")) return 1;
-        dim3 gs(unsigned((d->sq + 255) / 256 * d->heads * d->batch));
-        hipLaunchKernelGGL((nhipk::flash_dq_ds_kernel<D, F16, CAUSAL>), gs, dim3(256), 0, s, p);
-        return check(hipGetLastError(), "flash dq from dS launch");
-    }
-    hipLaunchKernelGGL((nhipk::flash_dkdv_kernel<D, F16, CAUSAL>), gk, dim3(256), 0, s, p, lse2);
-    if (check(hipGetLastError(), "flash dkdv launch")) return 1;
-    hipLaunchKernelGGL((nhipk::flash_dq_kernel<D, F16, CAUSAL>), gq, dim3(256), 0, s, p, lse2);
-    return check(hipGetLastError(), "flash dq launch");
-}
-
-int flash_bwd_on(hipStream_t s, const nhip_attn_desc *d, const void *q, const void *k, const void *v, const void *o,
-                 const void *d_o, const float *lse, void *dq, void *dk, void *dv, void *ws) {
-    if (check_attn(d, "flash attention backward")) return 1;
-    if (d->batch == 0 || d->heads == 0) return 0;
-    nhipk::AttnParams p = attn_params(d);
-    p.q = static_cast<const uint16_t *>(q);
-    p.k = static_cast<const uint16_t *>(k);
-    p.v = static_cast<const uint16_t *>(v);
-    p.o_in = static_cast<const uint16_t *>(o);
-    p.d_o = static_cast<const uint16_t *>(d_o);
-    p.lse_in = lse;
-    p.dq = static_cast<uint16_t *>(dq);
-    p.dk = static_cast<uint16_t *>(dk);
-    p.dv = static_cast<uint16_t *>(dv);
-    p.delta = static_cast<float *>(ws);
-    p.dqacc = d->deterministic ? nullptr : reinterpret_cast<float *>(static_cast<char *>(ws) + flash_bwd_dq_offset(d));
-    p.ds = d->deterministic == 1 ? reinterpret_cast<uint16_t *>(static_cast<char *>(ws) + flash_bwd_dq_offset(d)) : nullptr;
-    bool f16 = d->dtype == NHIP_F16;
-#define NHIP_BWD(DD, FF, CC) return launch_bwd<DD, FF, CC>(s, p, d)
-    if (kernel_dim(d) == 128) {
-        if (f16) { if (d->causal) NHIP_BWD(128, true, true); NHIP_BWD(128, true, false); }
-        if (d->causal) NHIP_BWD(128, false, true);
-        NHIP_BWD(128, false, false);
-    }
-    if (f16) { if (d->causal) NHIP_BWD(64, true, true); NHIP_BWD(64, true, false); }
-    if (d->causal) NHIP_BWD(64, false, true);
-    NHIP_BWD(64, false, false);
-#undef NHIP_BWD
 }
 
 }  // namespace nhip

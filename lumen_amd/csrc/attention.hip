@@ -5,7 +5,7 @@
 #include <mutex>
 #include <string>
 
-#include "attention.h"
+#include "attention_launch.h"
 #include "attention_split.h"
 #include "nhip_internal.h"
 

@@ -42,5 +42,11 @@ int gated_both_grads_on(hipStream_t s, const nhip_gated_desc *d, const void *dgu
 int gated_grad_on(hipStream_t s, const nhip_gated_desc *d, const void *dh, const float *g, const float *u, void *dgu);
 int clip_on(hipStream_t s, const nhip_clip_desc *d, const nhip_clip_tensor *t, const double *max_at, float *norm,
             float *scale, void *ws);
+int adamw_on(hipStream_t s, const nhip_adamw_desc *d, const nhip_adamw_tensor *t, const double *lr_at, const void *step_at,
+             const float *scale_at);
+int packed_fwd_on(hipStream_t s, const nhip_packed_desc *d, const void *q, const void *k, const void *v, const void *offsets, void *o,
+                  float *lse, void *ws);
+int packed_bwd_on(hipStream_t s, const nhip_packed_desc *d, const void *q, const void *k, const void *v, const void *offsets,
+                  const void *o, const void *d_o, const float *lse, void *dq, void *dk, void *dv, void *ws);
 
 }  // namespace nhip

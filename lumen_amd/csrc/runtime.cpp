@@ -470,7 +470,7 @@ int nhip_plan_add_launch(void *plan, void *function, const uint32_t grid[3], con
 
 int nhip_plan_add_builtin(void *plan, int kind, const void *desc, size_t desc_bytes, const nhip_reloc *relocs,
                           size_t nrelocs) {
-    if (kind < NHIP_STEP_GEMM || kind > NHIP_STEP_GATED_BACKWARD) return fail("nhip_plan_add_builtin: unknown step kind");
+    if (kind < NHIP_STEP_GEMM || kind > NHIP_STEP_PACKED_BWD) return fail("nhip_plan_add_builtin: unknown step kind");
     // the descriptor must hold what run_steps reads for the kind
     size_t need = 0, pointers = 16;
     switch (kind) {
@@ -487,6 +487,8 @@ int nhip_plan_add_builtin(void *plan, int kind, const void *desc, size_t desc_by
         case NHIP_STEP_GATED_INPUT:
         case NHIP_STEP_GATED_WEIGHT:
         case NHIP_STEP_GATED_BACKWARD: need = sizeof(nhip_gated_desc); break;
+        case NHIP_STEP_PACKED_FWD:
+        case NHIP_STEP_PACKED_BWD: need = sizeof(nhip_packed_desc); break;
         case NHIP_STEP_CLIP: {
             need = sizeof(nhip_clip_desc);
             if (desc && desc_bytes >= need) {
@@ -494,6 +496,16 @@ int nhip_plan_add_builtin(void *plan, int kind, const void *desc, size_t desc_by
                 if (count < 0 || count > (int64_t(1) << 24)) return fail("nhip_plan_add_builtin: bad tensor count");
                 need += size_t(count) * sizeof(nhip_clip_tensor);
                 pointers = 4 + 2 * size_t(count);
+            }
+            break;
+        }
+        case NHIP_STEP_ADAMW: {
+            need = sizeof(nhip_adamw_desc);
+            if (desc && desc_bytes >= need) {
+                const int64_t count = static_cast<const nhip_adamw_desc *>(desc)->count;
+                if (count < 0 || count > (int64_t(1) << 24)) return fail("nhip_plan_add_builtin: bad tensor count");
+                need += size_t(count) * sizeof(nhip_adamw_tensor);
+                pointers = 3 + 9 * size_t(count);
             }
             break;
         }
@@ -632,6 +644,21 @@ static int run_steps(Plan *plan, void *workspace, void *const *inputs, size_t ni
                 return fail("plan step " + std::to_string(i) + ": " + g_error);
             continue;
         }
+        if (st.kind == NHIP_STEP_ADAMW) {  // the same; a tensor's pointers stand in the order of their slots
+            nhip_adamw_desc *d = reinterpret_cast<nhip_adamw_desc *>(st.args.data());
+            nhip_adamw_tensor *t = reinterpret_cast<nhip_adamw_tensor *>(d + 1);
+            static_assert(offsetof(nhip_adamw_tensor, numel) == 9 * sizeof(void *), "nine pointers, one after another");
+            for (int64_t k = 0; k < d->count; ++k) std::memset(static_cast<void *>(t + k), 0, 9 * sizeof(void *));
+            for (auto &r : st.relocs) {
+                void *p;
+                if (resolve(r, &p)) return 1;
+                if (r.slot < 3) ptrs[r.slot] = p;
+                else std::memcpy(reinterpret_cast<char *>(t + (r.slot - 3) / 9) + (r.slot - 3) % 9 * sizeof(void *), &p, sizeof(p));
+            }
+            if (adamw_on(s, d, t, static_cast<const double *>(ptrs[0]), ptrs[1], static_cast<const float *>(ptrs[2])))
+                return fail("plan step " + std::to_string(i) + ": " + g_error);
+            continue;
+        }
         for (auto &r : st.relocs)
             if (resolve(r, &ptrs[r.slot])) return 1;
         int rc = 0;
@@ -688,6 +715,15 @@ static int run_steps(Plan *plan, void *workspace, void *const *inputs, size_t ni
             case NHIP_STEP_GATED_GRAD:
                 rc = gated_grad_on(s, reinterpret_cast<const nhip_gated_desc *>(st.args.data()), ptrs[0],
                                    static_cast<const float *>(ptrs[1]), static_cast<const float *>(ptrs[2]), ptrs[3]);
+                break;
+            case NHIP_STEP_PACKED_FWD:
+                rc = packed_fwd_on(s, reinterpret_cast<const nhip_packed_desc *>(st.args.data()), ptrs[0], ptrs[1], ptrs[2],
+                                   ptrs[3], ptrs[4], static_cast<float *>(ptrs[5]), ptrs[6]);
+                break;
+            case NHIP_STEP_PACKED_BWD:
+                rc = packed_bwd_on(s, reinterpret_cast<const nhip_packed_desc *>(st.args.data()), ptrs[0], ptrs[1], ptrs[2],
+                                   ptrs[3], ptrs[4], ptrs[5], static_cast<const float *>(ptrs[6]), ptrs[7], ptrs[8], ptrs[9],
+                                   ptrs[10]);
                 break;
             case NHIP_STEP_FILL: {
                 uint64_t n;

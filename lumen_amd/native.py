@@ -19,6 +19,7 @@ NHIP_BASE_WORKSPACE, NHIP_BASE_INPUT = 0, 1
 NHIP_STEP_GEMM, NHIP_STEP_FLASH_FWD, NHIP_STEP_FLASH_BWD, NHIP_STEP_COPY, NHIP_STEP_FILL, NHIP_STEP_LCE = 1, 2, 3, 4, 5, 6
 NHIP_STEP_HEADS, NHIP_STEP_HEADS_BWD, NHIP_STEP_GATED, NHIP_STEP_GATED_GRAD, NHIP_STEP_CLIP = 7, 8, 9, 10, 11
 NHIP_STEP_GATED_INPUT, NHIP_STEP_GATED_WEIGHT, NHIP_STEP_GATED_BACKWARD = 12, 13, 14
+NHIP_STEP_ADAMW, NHIP_STEP_PACKED_FWD, NHIP_STEP_PACKED_BWD = 15, 16, 17
 NHIP_LCE_I32, NHIP_LCE_I64 = 0, 1
 NHIP_POS_NONE, NHIP_POS_I32, NHIP_POS_I64 = 0, 1, 2
 NHIP_ACT = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
@@ -117,6 +118,30 @@ class ClipDesc(C.Structure):
     _fields_ = [("count", C.c_int64), ("max_norm", C.c_double), ("eps", C.c_double)]
 
 
+class PackedDesc(C.Structure):
+    """``nhip_packed_desc``: attention within sequences packed one after another (include/nhip.h)."""
+
+    _fields_ = [(n, C.c_int64) for n in ("tokens", "sequences", "heads", "kv_heads", "head_dim", "value_head_dim")] + [
+        (f"{t}_{a}", C.c_int64) for t in ("q", "k", "v", "o", "do", "dq", "dk", "dv") for a in ("s", "n")
+    ] + [("ds_bytes", C.c_int64), ("dtype", C.c_int32), ("causal", C.c_int32), ("offsets_dtype", C.c_int32), ("scale", C.c_float)]
+
+
+class AdamwTensor(C.Structure):
+    """``nhip_adamw_tensor``: one weight, its gradient and moments, and where the new ones go."""
+
+    _fields_ = [(n, C.c_void_p) for n in ("param", "grad", "m", "v", "master", "param_out", "m_out", "v_out", "master_out")] + [
+        ("numel", C.c_int64), ("dtype", C.c_int32), ("pad", C.c_int32)
+    ]
+
+
+class AdamwDesc(C.Structure):
+    """``nhip_adamw_desc``: the tensors' count and the step's rates."""
+
+    _fields_ = [("count", C.c_int64)] + [(n, C.c_double) for n in ("lr", "step", "beta1", "beta2", "eps", "weight_decay")] + [
+        ("step_type", C.c_int32), ("pad", C.c_int32)
+    ]
+
+
 class Reloc(C.Structure):
     _fields_ = [
         ("slot", C.c_uint32),
@@ -184,6 +209,10 @@ SIGNATURES = {
     "nhip_gated_config_count": ([C.POINTER(C.c_int)], C.c_int),
     "nhip_gated_linear_grad": ([C.POINTER(GatedDesc)] + [C.c_void_p] * 4, C.c_int),
     "nhip_clip_grad_norm": ([C.POINTER(ClipDesc), C.POINTER(ClipTensor)] + [C.c_void_p] * 4, C.c_int),
+    "nhip_packed_fwd": ([C.POINTER(PackedDesc)] + [C.c_void_p] * 7, C.c_int),
+    "nhip_packed_bwd": ([C.POINTER(PackedDesc)] + [C.c_void_p] * 11, C.c_int),
+    "nhip_packed_workspace": ([C.POINTER(PackedDesc), C.c_int, C.POINTER(C.c_size_t)], C.c_int),
+    "nhip_adamw": ([C.POINTER(AdamwDesc), C.POINTER(AdamwTensor)] + [C.c_void_p] * 3, C.c_int),
     "nhip_clip_grad_norm_workspace": ([C.POINTER(ClipDesc), C.POINTER(C.c_size_t)], C.c_int),
     "nhip_plan_create": ([C.POINTER(C.c_void_p)], C.c_int),
     "nhip_plan_destroy": ([C.c_void_p], C.c_int),

@@ -128,6 +128,54 @@ class SGD(Module):
                 p.copy_(p - self.lr * p.grad)
 
 
+class AdamW(Module):
+    """``F.adamw`` over every parameter, with float32 moments, a float32 master beside each bfloat16 weight and the count of
+    steps, all held as weights of its own that a compiled step writes over."""
+
+    params: list
+    masters: list
+    exp_avgs: list
+    exp_avg_sqs: list
+    steps: L.Tensor
+    lr: float
+
+    BETAS, EPS, WEIGHT_DECAY = (0.9, 0.95), 1e-8, 0.1
+
+    def step(self, max_norm=None):
+        """One step over the parameters that have a gradient, these clipped to ``max_norm`` first unless it is None."""
+        at = [i for i, p in enumerate(self.params) if p.grad is not None]
+        held = [[xs[i] for i in at] for xs in (self.params, self.exp_avgs, self.exp_avg_sqs, self.masters)]
+        grads = [p.grad for p in held[0]]
+        if max_norm is not None:
+            grads, _ = F.clip_grad_norm(grads, max_norm)
+        self.steps.copy_(self.steps + 1)
+        params, first, second, masters = held
+        new = F.adamw(params, grads, first, second, self.steps, self.lr, betas=self.BETAS, eps=self.EPS,
+                      weight_decay=self.WEIGHT_DECAY, masters=masters)
+        for xs, values in zip(held, new):
+            for x, value in zip(xs, values):
+                x.copy_(value)
+
+
+def adamw(model, lr=1e-3):
+    """An ``AdamW`` over the model's parameters (bfloat16), its state meta weights (``load_adamw`` gives them values)."""
+    params = model.parameters()
+
+    def state():
+        return [L.empty(list(p.shape), "float32", "meta") for p in params]
+
+    return AdamW(params, state(), state(), state(), L.empty([], "int32", "meta"), lr)
+
+
+def load_adamw(opt):
+    """The state ahead of the first step: moments and count zero, each master its weight's loaded value."""
+    for p, w, m, v in zip(opt.params, opt.masters, opt.exp_avgs, opt.exp_avg_sqs):
+        w.copy_(L.Tensor(p.dtype, p.shape, "cpu", host=p.raw()))
+        for x in (m, v):
+            x.copy_(L.zeros(p.shape))
+    opt.steps.copy_(L.zeros([], "int32"))
+
+
 def loss_fn(model, ids, targets):
     h = model(ids)
     logits = F.matmul(h, model.head.t(), "float32", "float32")

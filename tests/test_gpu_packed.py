@@ -1,0 +1,262 @@
+"""packed_attention on the GPU against plain float64 NumPy (tests/training_math.py), with the tolerances derived there."""
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import lumen_amd as L
+import lumen_amd.functional as F
+from lumen_amd import dtypes as D
+from lumen_amd import native as nv
+from tests import training_math as M
+from tests.hiputil import Dev
+
+pytestmark = pytest.mark.gpu
+
+
+def _round(x, dtype):
+    return np.asarray(D.to_numpy_values(D.from_values(np.asarray(x, np.float32), dtype), dtype), np.float64)
+
+
+def _tensor(x, dtype):
+    return L.Tensor(dtype, np.shape(x), "cpu", host=np.array(D.from_values(np.asarray(x, np.float32), dtype)))
+
+
+def _values(t):
+    return np.asarray(L.to_numpy(t), np.float64)
+
+
+def _near(got, want, tol, what=""):
+    assert got.shape == want.shape, what
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (what, np.abs(got - want)[bad].max(), int(bad.sum()), np.argwhere(bad)[0], got[bad][0], want[bad][0])
+
+
+def _program(causal, scale=None):
+    def fn(q, k, v, offsets, do):
+        o, pull = L.vjp(lambda q, k, v: F.packed_attention(q, k, v, offsets, scale=scale, is_causal=causal), q, k, v)
+        return [o, *pull(do)]
+
+    return fn
+
+
+CASES = [
+    # lengths, first, tokens, n, nkv, d, dv, causal, dtype
+    ([1], 0, 1, 1, 1, 8, 8, True, "bfloat16"),
+    ([1], 0, 1, 2, 1, 64, 64, False, "float16"),
+    ([61, 17, 19], 0, 97, 4, 2, 64, 64, True, "bfloat16"),
+    ([64, 128, 63, 129, 1, 0, 65], 3, 460, 2, 2, 64, 64, True, "float16"),
+    ([64, 128, 63, 129, 1, 0, 65], 3, 460, 2, 1, 128, 128, True, "bfloat16"),
+    ([64, 128, 63, 129, 1, 0, 65], 3, 460, 2, 2, 128, 128, False, "float16"),
+    ([0, 0, 300, 0], 0, 300, 8, 8, 32, 32, True, "bfloat16"),
+    ([700], 5, 800, 3, 3, 80, 80, False, "bfloat16"),
+    ([33, 257, 255, 256], 0, 801, 8, 2, 64, 128, True, "bfloat16"),
+    ([33, 257, 255, 256], 1, 803, 4, 4, 128, 40, False, "float16"),
+    ([2, 3, 1, 1, 5, 8] * 20, 0, 420, 2, 2, 64, 64, True, "bfloat16"),
+    ([], 0, 70, 2, 2, 64, 64, True, "bfloat16"),
+    ([0], 70, 70, 2, 2, 64, 64, False, "bfloat16"),
+    ([1100, 40], 0, 1140, 2, 2, 128, 128, True, "bfloat16"),
+]
+
+
+@pytest.mark.parametrize("store", [True, False])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_packed(hip, case, store):
+    """Both directions, dS stored for dQ and computed again."""
+    lengths, first, tokens, n, nkv, d, dv, causal, dtype = CASES[case]
+    rng = np.random.default_rng(case)
+    x = {k: _round(v, dtype) for k, v in M.packed_inputs(rng, tokens, n, nkv, d, dv).items()}
+    offsets = M.offsets_of(lengths, first)
+    want, tol = M.packed(x, offsets, causal, d**-0.5, dtype)
+    args = [_tensor(x[k], dtype) for k in "qkv"] + [L.from_numpy(offsets.astype(np.int32 if case % 2 else np.int64)), _tensor(x["do"], dtype)]
+    with L.config.compiler.patch(attention_store_ds=store):
+        f = L.compile(_program(causal), device="hip")
+        for _ in range(2):
+            for name, a, w, t in zip(("o", "dq", "dk", "dv"), f(*args), want, tol):
+                _near(_values(a), w, t, name)
+    assert [st.kind for st in f.plan.steps] == ["packed_fwd", "packed_bwd"]
+
+
+def test_nothing_of_another_sequence_or_of_none(hip):
+    """NaN and infinities in the tokens of no sequence and in whole sequences: every other sequence's results are, bit for bit,
+    those without them."""
+    rng = np.random.default_rng(2)
+    lengths = [70, 1, 64, 200, 30, 129]
+    offsets = M.offsets_of(lengths, 9)
+    t = int(offsets[-1]) + 40
+    x = M.packed_inputs(rng, t, 4, 2, 64)
+    f = L.compile(_program(True), device="hip")
+
+    def run(x):
+        args = [_tensor(x[k], "bfloat16") for k in "qkv"] + [L.from_numpy(offsets.astype(np.int32)), _tensor(x["do"], "bfloat16")]
+        return [np.array(o.raw()) for o in f(*args)]
+
+    clean = run(x)
+    bad = {k: v.copy() for k, v in x.items()}
+    for v in bad.values():
+        v[:9], v[offsets[-1]:] = np.nan, np.inf
+        v[offsets[1]:offsets[2]], v[offsets[3]:offsets[4]] = np.inf, np.nan
+    kept = np.ones(t, bool)
+    kept[offsets[1]:offsets[2]] = kept[offsets[3]:offsets[4]] = False
+    for a, b in zip(clean, run(bad)):
+        assert np.array_equal(a[kept], b[kept])
+        assert not a[:9].any() and not a[offsets[-1]:].any()
+
+
+def test_heads_of_a_merged_projection(hip):
+    """Queries, keys and values read in place through a merged projection's strides, and gradients joined again."""
+    rng = np.random.default_rng(3)
+    t, n, nkv, d = 333, 8, 2, 64
+    offsets = M.offsets_of([100, 200, 30])
+    qkv, do = (_round(rng.standard_normal(s), "bfloat16") for s in ((t, (n + 2 * nkv) * d), (t, n, d)))
+
+    def heads(qkv):
+        return (qkv[:, lo * d:hi * d].reshape(t, hi - lo, d) for lo, hi in ((0, n), (n, n + nkv), (n + nkv, n + 2 * nkv)))
+
+    def fn(qkv, offsets, do):
+        o, pull = L.vjp(lambda qkv: F.packed_attention(*heads(qkv), offsets), qkv)
+        return [o, pull(do)[0]]
+
+    f = L.compile(fn, device="hip")
+    o, dqkv = (_values(a) for a in f(_tensor(qkv, "bfloat16"), L.from_numpy(offsets), _tensor(do, "bfloat16")))
+    q, k, v = (a for a in heads(qkv))
+    want, tol = M.packed({"q": q, "k": k, "v": v, "do": do}, offsets, True, d**-0.5, "bfloat16")
+    _near(o, want[0], tol[0], "o")
+    for name, a, w, tt in zip("qkv", heads(dqkv), want[1:], tol[1:]):
+        _near(a, w, tt, name)
+    assert [st.kind for st in f.plan.steps if st.kind != "view"][:2] == ["packed_fwd", "packed_bwd"]  # nothing is copied for them
+
+
+@pytest.mark.parametrize("limit", [40, 60])
+def test_ds_that_does_not_fit(hip, limit):
+    """The workspace holds `limit` dS tiles of a head: the offsets on the device decide whether they are stored or computed again;
+    the same compiled function with offsets of which all fit and of which they do not."""
+    rng = np.random.default_rng(limit)
+    t, n, d = 1024, 2, 64
+    x = {k: _round(v, "bfloat16") for k, v in M.packed_inputs(rng, t, n, n, d).items()}
+    with L.config.compiler.patch(attention_ds_max_bytes=limit * n * 128 * 64 * 2):
+        f = L.compile(_program(True), device="hip")
+        for lengths in ([1024, 0, 0, 0], [256, 256, 256, 256], [100, 500, 300, 100], [1, 2, 3, 4]):
+            offsets = M.offsets_of(lengths)
+            want, tol = M.packed(x, offsets, True, d**-0.5, "bfloat16")
+            args = [_tensor(x[k], "bfloat16") for k in "qkv"] + [L.from_numpy(offsets), _tensor(x["do"], "bfloat16")]
+            for name, a, w, tt in zip(("o", "dq", "dk", "dv"), f(*args), want, tol):
+                _near(_values(a), w, tt, (lengths, name))
+
+
+def test_more_sequences_than_a_pass_of_the_builder(hip):
+    """2500 sequences, mostly of a few tokens, some empty, some longer than eight blocks: 1024 of them a pass."""
+    rng = np.random.default_rng(8)
+    lengths = rng.integers(0, 4, 2500)
+    lengths[[5, 1023, 1024, 2100]] = [1500, 200, 1100, 64]
+    offsets = M.offsets_of(lengths, 2)
+    t = int(offsets[-1]) + 3
+    x = {k: _round(v, "float16") for k, v in M.packed_inputs(rng, t, 1, 1, 64).items()}
+    want, tol = M.packed(x, offsets, True, 0.125, "float16")
+    f = L.compile(_program(True), device="hip")
+    args = [_tensor(x[k], "float16") for k in "qkv"] + [L.from_numpy(offsets.astype(np.int32)), _tensor(x["do"], "float16")]
+    for name, a, w, tt in zip(("o", "dq", "dk", "dv"), f(*args), want, tol):
+        _near(_values(a), w, tt, name)
+
+
+def test_offsets_that_decrease_or_leave_the_tokens_are_clamped(hip):
+    """Each offset is read as clamped into [the one before, tokens]."""
+    rng = np.random.default_rng(9)
+    t = 150
+    x = {k: _round(v, "bfloat16") for k, v in M.packed_inputs(rng, t, 2, 2, 64).items()}
+    f = L.compile(_program(False), device="hip")
+    for given, read in (([-5, 60, 40, 90, 1 << 30, 7], [0, 60, 60, 90, 150, 150]), ([300, 0, 0, 0, 0, 0], [150] * 6),
+                        ([10, 5, 5, -9, 20, 30], [10, 10, 10, 10, 20, 30])):
+        want, tol = M.packed(x, read, False, 0.125, "bfloat16")
+        args = [_tensor(x[k], "bfloat16") for k in "qkv"] + [L.from_numpy(np.array(given, np.int32)), _tensor(x["do"], "bfloat16")]
+        for name, a, w, tt in zip(("o", "dq", "dk", "dv"), f(*args), want, tol):
+            _near(_values(a), w, tt, (given, name))
+
+
+@pytest.mark.parametrize("lengths,tokens,n,nkv,d", [([3000, 5, 1091], 4096, 4, 2, 128), ([2048] * 4, 8192, 2, 2, 64)])
+def test_long_sequences_against_flash_attention_of_each(hip, lengths, tokens, n, nkv, d):
+    """Each sequence's results are those of flash_attention on it alone, up to their roundings: both within the same tolerance of
+    float64, so within twice it (as 4 U of the largest value here) of one another; the same bits in every call."""
+    rng = np.random.default_rng(10)
+    x = {k: _round(v, "bfloat16") for k, v in M.packed_inputs(rng, tokens, n, nkv, d).items()}
+    offsets = M.offsets_of(lengths)
+    f = L.compile(_program(True), device="hip")
+    args = [_tensor(x[k], "bfloat16") for k in "qkv"] + [L.from_numpy(offsets.astype(np.int32)), _tensor(x["do"], "bfloat16")]
+    first = [np.array(a.raw()) for a in f(*args)]
+    again = [np.array(a.raw()) for a in f(*args)]
+    assert all(np.array_equal(a, b) for a, b in zip(first, again))
+    got = [np.asarray(D.to_numpy_values(a, "bfloat16"), np.float64) for a in first]
+
+    def alone(q, k, v, do):
+        o, pull = L.vjp(lambda q, k, v: F.flash_attention(q, k, v, is_causal=True), q, k, v)
+        return [o, *pull(do)]
+
+    g = L.compile(alone, device="hip")
+    for lo, hi in zip(offsets, offsets[1:]):
+        one = g(*(_tensor(x[k][None, lo:hi], "bfloat16") for k in ("q", "k", "v", "do")))
+        for name, a, b in zip(("o", "dq", "dk", "dv"), got, one):
+            b = _values(b)[0]
+            assert np.abs(a[lo:hi] - b).max() <= 4 * M.U["bfloat16"] * max(1.0, np.abs(b).max()), (name, lo)
+
+
+def test_captured_and_replayed(hip):
+    """One capture replayed with other offsets and operands in the same memory, a second capture of the plan between, against plain
+    runs of each."""
+    from lumen_amd.compiler.plan import Plan
+    from lumen_amd.tensor import DeviceBuffer
+
+    rng = np.random.default_rng(11)
+    t, n, nkv, d = 260, 4, 2, 64
+    dts = ["bfloat16"] * 3 + ["int32", "bfloat16"]
+    sets = []
+    for lengths in ([260, 0, 0], [100, 100, 50], [1, 0, 200], [64, 64, 128]):
+        x = M.packed_inputs(rng, t, n, nkv, d)
+        sets.append([D.from_values(x[k].astype(np.float32), "bfloat16") for k in "qkv"] +
+                    [M.offsets_of(lengths).astype(np.int32), D.from_values(x["do"].astype(np.float32), "bfloat16")])
+    plan = Plan(L.make_graph(_program(True))(*[L.empty(list(a.shape), dt, "meta") for a, dt in zip(sets[0], dts)]), "hip:0")
+    ins, ws = [DeviceBuffer(0, a.nbytes) for a in sets[0]], DeviceBuffer(0, plan.workspace_bytes)
+    ptrs = [b.ptr for b in ins]
+
+    def put(arrays):
+        for b, a in zip(ins, arrays):
+            nv.h2d(b.ptr, np.ascontiguousarray(a).ctypes.data, a.nbytes)
+
+    def read():
+        out = []
+        for loc in plan.output_locs:
+            a = np.empty(loc.shape, D.storage(loc.dtype))
+            nv.d2h(a.ctypes.data, ws.ptr + loc.offset * D.size_of(loc.dtype), a.nbytes)
+            out.append(a)
+        return out
+
+    plain = []
+    for s in sets:
+        put(s)
+        plan.run_in(ws.ptr, ptrs)
+        plain.append(read())
+    first, second = plan.capture(ws.ptr, ptrs), plan.capture(ws.ptr, ptrs)
+    for i, (s, want) in enumerate(list(zip(sets, plain)) * 2):
+        put(s)
+        (first if i % 2 else second).launch()
+        assert all(np.array_equal(a, b) for a, b in zip(read(), want))
+
+
+def test_refusals_of_the_entry_points(hip):
+    one = Dev(nbytes=4096)
+
+    def desc(**kw):
+        d = nv.PackedDesc(tokens=2, sequences=1, heads=1, kv_heads=1, head_dim=8, dtype=1, offsets_dtype=1, scale=1.0)
+        for name, v in kw.items():
+            setattr(d, name, v)
+        return C.byref(d)
+
+    with pytest.raises(RuntimeError, match="16 bytes"):
+        nv.call("nhip_packed_fwd", desc(), one.ptr + 2, one.ptr, one.ptr, one.ptr, one.ptr, None, one.ptr)
+    with pytest.raises(RuntimeError, match="workspace"):
+        nv.call("nhip_packed_fwd", desc(), one.ptr, one.ptr, one.ptr, one.ptr, one.ptr, None, None)
+    with pytest.raises(RuntimeError, match="workspace"):
+        nv.call("nhip_packed_bwd", desc(), *[one.ptr] * 10, None)
+    with pytest.raises(RuntimeError, match="head dim"):
+        nv.call("nhip_packed_fwd", desc(head_dim=12), one.ptr, one.ptr, one.ptr, one.ptr, one.ptr, None, one.ptr)
+    nv.call("nhip_packed_fwd", desc(tokens=0), None, None, None, None, None, None, None)  # nothing to do
