@@ -332,6 +332,28 @@ int nhip_clip_grad_norm(const nhip_clip_desc *desc, const nhip_clip_tensor *tens
                         float *scale, void *workspace);
 int nhip_clip_grad_norm_workspace(const nhip_clip_desc *desc, size_t *bytes);
 
+/* ---- the cross entropy of a vocabulary head with its gradients (no counterpart in the reference) ------------------- *
+ *
+ * Of rows h [rows, k], classes w [classes, k] and the logits h w^T, which never exist whole: losses (float32 [rows], or null)
+ * lse - logit[target], 0 of a row whose target is ignore_index, other targets clamped into the classes; and for the losses'
+ * cotangents g (float32 [rows]; null: no gradients) dh [rows, k] = ((softmax - onehot) g) w and dw [classes, k] =
+ * ((softmax - onehot) g)^T h (each or null), sums float32, rounded once to the operands' type, ignored rows counting for
+ * nothing. (softmax - onehot) g is rounded to the operands' type as an operand of the products, of at most piece_bytes'
+ * worth of rows at a time (at least 256). Rows of a multiple of 64 elements that start on 16 bytes are read where they lie,
+ * others (and the gradients' h) are copied. The same bits every run. `workspace` of nhip_head_loss_workspace bytes from a 256-byte address. */
+typedef struct {
+    int64_t rows, classes, k;
+    int64_t h_m, w_n;           /* elements from a row to the next */
+    int64_t ignore_index;
+    int64_t piece_bytes;
+    int32_t dtype;              /* NHIP_BF16 or NHIP_F16 */
+    int32_t target_dtype;       /* NHIP_LCE_I32 or NHIP_LCE_I64 */
+} nhip_head_desc;
+
+int nhip_head_loss(const nhip_head_desc *desc, const void *h, const void *w, const void *target, const float *g, float *losses, void *dh,
+                   void *dw, void *workspace);
+int nhip_head_loss_workspace(const nhip_head_desc *desc, int gradients, size_t *bytes);
+
 /* ---- packed self attention (no counterpart in the reference) ------------------------------------------------------ *
  *
  * Attention of tokens [tokens, heads, head_dim] within sequences that lie one after another: token t is of sequence i where
@@ -430,6 +452,7 @@ enum {
                                  v_out, master_out from 3 + 9 i on (or none) */
     NHIP_STEP_PACKED_FWD = 16, /* desc: nhip_packed_desc; pointers: q, k, v, offsets, o, lse (or none), workspace */
     NHIP_STEP_PACKED_BWD = 17, /* desc: nhip_packed_desc; pointers: q, k, v, offsets, o, do, lse, dq, dk, dv, workspace */
+    NHIP_STEP_HEAD_LOSS = 18,  /* desc: nhip_head_desc; pointers as nhip_head_loss's, those left out null */
 };
 
 int nhip_plan_create(void **plan);

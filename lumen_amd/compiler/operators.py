@@ -1,4 +1,5 @@
-"""Lowering of the operators of ``functional/operators.py``, ``optimizer.py`` and ``packed.py``: a ``fusion`` of each name becomes a built-in step whose
+"""Lowering of the operators of ``functional/operators.py``, ``optimizer.py``, ``packed.py`` and
+``linear_cross_entropy.py``: a ``fusion`` of each name becomes a built-in step whose
 descriptor and pointers this module makes from the operands' places (``include/nhip.h``).
 
 Unlike the generated kernels these read rows: an operand whose view would not keep its last axis contiguous (or, where
@@ -23,6 +24,8 @@ KINDS = {
     "adamw": "adamw",
     "packed_attention": "packed_fwd",
     "packed_attention_backward": "packed_bwd",
+    "head_loss": "head_loss",
+    "head_loss_backward": "head_loss",
 }
 BOTH = "gated_both"  # a gated_weight and a gated_input step in one
 STEPS = {*KINDS.values(), BOTH}
@@ -44,6 +47,8 @@ def _wants(node):
         return [WIDE] * len(node.inputs)
     if name == "gated_linear_grad":
         return [ROWS, DENSE, DENSE]
+    if name in ("head_loss", "head_loss_backward"):
+        return [WIDE_ROWS, WIDE] + [DENSE] * (len(node.inputs) - 2)
     if name == "packed_attention":
         return [CHUNK_ROWS] * 3 + [DENSE]
     if name == "packed_attention_backward":
@@ -116,6 +121,8 @@ def scratch_bytes(graph, node) -> int:
         nv.call("nhip_gated_linear_workspace", C.byref(_gated_node_desc(graph, node)), C.byref(n))
     elif name in ("gated_input_grad", "gated_weight_grad"):
         nv.call("nhip_gated_backward_workspace", C.byref(_gated_backward_desc(graph, node)), C.byref(n))
+    elif name in ("head_loss", "head_loss_backward"):
+        nv.call("nhip_head_loss_workspace", C.byref(_head_desc(graph, node)), int(name != "head_loss"), C.byref(n))
     elif name in ("packed_attention", "packed_attention_backward"):
         n.value = _packed_workspace(graph, node)
         if name != "packed_attention":
@@ -170,7 +177,8 @@ def lower(plan, step):
     return {"gated_linear": _lower_gated, "gated_linear_grad": _lower_gated_grad,
             "gated_input_grad": _lower_gated_backward, "gated_weight_grad": _lower_gated_backward,
             "clip_grad_norm": _lower_clip, "adamw": _lower_adamw,
-            "packed_attention": _lower_packed, "packed_attention_backward": _lower_packed}[name](plan, step)
+            "packed_attention": _lower_packed, "packed_attention_backward": _lower_packed,
+            "head_loss": _lower_head, "head_loss_backward": _lower_head}[name](plan, step)
 
 
 def _slots(places):
@@ -348,6 +356,73 @@ def _lower_packed(plan, step):
     if not backward:
         return nv.NHIP_STEP_PACKED_FWD, bytes(d), _slots([*at, out[0], out.get(1), scratch])
     return nv.NHIP_STEP_PACKED_BWD, bytes(d), _slots([*at, *(loc for _, loc in names[5:]), scratch])
+
+
+def _head_desc(graph, node):
+    from lumen_amd import native as nv
+    from lumen_amd.config import config
+
+    h, w, target = (graph.types[v] for v in node.inputs[:3])
+    d = nv.HeadDesc(rows=h.shape[0], classes=w.shape[0], k=h.shape[1], h_m=h.shape[1], w_n=h.shape[1],
+                    ignore_index=node.params["ignore"], piece_bytes=config.compiler.head_piece_bytes, dtype=NHIP_DT[h.dtype])
+    d.target_dtype = nv.NHIP_LCE_I64 if target.dtype == "int64" else nv.NHIP_LCE_I32
+    return d
+
+
+def _lower_head(plan, step):
+    from lumen_amd import native as nv
+
+    node = step.nodes[0]
+    d, out = _head_desc(plan.graph, node), _outputs(plan, step)
+    at = [plan.loc[v] for v in node.inputs]
+    if d.rows > 1:
+        d.h_m = at[0].strides[0]
+    scratch = plan.scratch.get(id(step))
+    if node.params["name"] == "head_loss":
+        return nv.NHIP_STEP_HEAD_LOSS, bytes(d), _slots([*at, None, out[0], None, None, scratch])
+    return nv.NHIP_STEP_HEAD_LOSS, bytes(d), _slots([*at, out.get(2), out[0], out.get(1), scratch])
+
+
+def losses_with_gradients(graph: Graph) -> Graph:
+    """The losses of a vocabulary head whose gradients are computed too come from the gradients' step, which computes them
+    anyway, where the losses' cotangents do not depend on them: one product over the classes less."""
+    forward = {}
+    for n in graph.nodes:
+        if n.prim == "fusion" and n.params["name"] == "head_loss":
+            forward.setdefault((n.inputs, n.params["ignore"]), n)
+    depends = {}  # value -> the losses that it depends on
+
+    def roots(v):
+        return depends.get(v, frozenset())
+
+    pairs = {}
+    for n in graph.nodes:
+        found = frozenset().union(*(roots(v) for v in n.inputs)) if n.inputs else frozenset()
+        if n.prim == "fusion" and n.params["name"] == "head_loss":
+            found |= {n.output}
+        elif n.prim == "fusion" and n.params["name"] == "head_loss_backward":
+            f = forward.get((n.inputs[:3], n.params["ignore"]))
+            if f is not None and f.output not in found and f.output not in pairs and not any(f.output in roots(v) for v in n.inputs):
+                pairs[f.output] = n
+        if found:
+            depends[n.output] = found
+    if not pairs:
+        return graph
+    gone = set(pairs)
+    # what depends on a loss that is taken over comes after everything else
+    late = [n for n in graph.nodes if roots(n.output) & gone and n.output not in gone]
+    rest = [n for n in graph.nodes if not roots(n.output) & gone]
+    g = Graph()
+    remap = {v: g.input(graph.types[v].dtype, graph.types[v].shape) for v in graph.inputs}
+    by_gradients = {b.output: v for v, b in pairs.items()}
+    for n in rest + late:
+        remap[n.output] = g.add_node(n.prim, tuple(remap[v] for v in n.inputs), n.params, graph.types[n.output], n.backward)
+        if n.output in by_gradients:
+            loss = by_gradients[n.output]
+            ty = graph.types[loss]
+            remap[loss] = g.add_node("fusion_output", (remap[n.output],), {"index": 2, "ty": ty}, ty, n.backward)
+    g.set_outputs([remap[v] for v in graph.outputs])
+    return g
 
 
 def _adamw_tensors(node):

@@ -169,7 +169,7 @@ def compile_graph(graph: Graph, packable=()) -> tuple[Graph, list]:
     simplify again. Returns the graph and merge_dots' packs (weight input positions stored back to back)."""
     g = passes.frontend(graph)
     if config.compiler.fuse:
-        g = operators.clip_in_consumers(g)
+        g = operators.clip_in_consumers(operators.losses_with_gradients(g))
     if config.compiler.flash_attention:
         g = attn_pass.match(g)
         g = passes.frontend(g)
@@ -1371,6 +1371,10 @@ class Plan:
         if st.kind in ("gated_input", "gated_weight"):
             dgu, other = (g.types[v] for v in st.nodes[0].inputs[:2])
             return 2 * dgu.numel() * other.shape[1], io
+        if st.kind == "head_loss":
+            h, w = (g.types[v] for v in st.nodes[0].inputs[:2])
+            both = st.nodes[0].params["name"] != "head_loss"
+            return (6 if both else 2) * h.numel() * w.shape[0], io
         if st.kind == operators.BOTH:
             return 4 * g.types[st.inputs[0]].numel() * g.types[st.inputs[1]].shape[1], io
         return 0, io

@@ -46,9 +46,12 @@ class CompilerFlags:
     fused_linear_cross_entropy: bool = True
     # rows a chunk of the fused linear cross entropy backward (None: off, the reference's default)
     fused_linear_cross_entropy_chunk_size: int | None = None
-    # the operators of functional/operators.py, packed.py and optimizer.py run as kernels of their own (off: traced as their
+    # the operators of functional/operators.py, packed.py, optimizer.py and
+    # linear_cross_entropy.py run as kernels of their own (off: traced as their
     # primitives)
     fused_operators: bool = True
+    # bytes of 16-bit exponentials that linear_cross_entropy's gradients hold at once (a piece of the rows', 256 at least)
+    head_piece_bytes: int = 512 << 20
     _version: int = 0
 
     def __setattr__(self, name, value):

@@ -525,6 +525,11 @@ __device__ __forceinline__ int stream_line(int wn, int j) {
     else return wn * WCOLS + 32 * j;
 }
 
+// Whether an epilogue is called for every column of a tile's rows, those past n too (a reduction over lanes that a row's
+// last tile would leave without some of them).
+template <class Out>
+struct TakesWholeRows : std::false_type {};
+
 // One workgroup's 256 x 256 output tile. `out` is AnyStore (a plain store of D), or a generated epilogue
 // functor called as out(row, col, float4, pre) with the float32 sums of four consecutive columns (col a
 // multiple of 4, within m x n) and pre = out.load(row, col), its other operands read ahead. `smem` holds gemm_stream_lds_bytes<BK, WN>() bytes.
@@ -535,7 +540,8 @@ __device__ __forceinline__ int stream_line(int wn, int j) {
 // PAIR 1: two products of A, by B and by b2 of the same shape and strides: half of the tile's columns are B's, half the
 // same columns of b2, and out.store takes the pairs of sums. PAIR 2: the sum of two products, A's first k / 2 columns by b
 // and the others by b2, part blockIdx.z of it over k_part of the k tiles. PAIR 3: one product of operands contiguous along m
-// and n, in parts like PAIR 2. PAIR 4: PAIR 1 in parts. k (PAIR 2: k / 2) is a multiple of 8, with PAIR 3 any number; rows
+// and n, in parts like PAIR 2. PAIR 4: PAIR 1 in parts. PAIR 5: one product of A along k by B along n, in parts,
+// A's rows in whole chunks of 8. k (PAIR 2: k / 2) is a multiple of 8, with PAIR 3 and 5 any number; rows
 // along n (and m) hold whole chunks of 8 elements whatever n is. Operands are within the buffers' reach.
 template <bool F16, int BK, int WN, bool AT, bool BT, bool BUF, class Out, int TM = 256, int KL = 0, int PAIR = 0, int ST = 0>
 __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint16_t *__restrict__ a,
@@ -557,7 +563,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     tile_of(blockIdx.x, s.tiles_m, s.tiles_n, tm, tn);
     int64_t oa, ob, od;
     batch_offsets(s, blockIdx.y, oa, ob, od);
-    static_assert(PAIR == 0 || (BUF && AT == (PAIR == 3) && BT == (PAIR == 2 || PAIR == 3) && FN % 2 == 0), "the pairs' layouts");
+    static_assert(PAIR == 0 || (BUF && AT == (PAIR == 3) && BT == (PAIR == 2 || PAIR == 3 || PAIR == 5) && FN % 2 == 0), "the pairs' layouts");
     constexpr bool TWO = PAIR == 1 || PAIR == 4;
     constexpr int TNB = TWO ? TM / 2 : TM;  // columns of one B operand in the tile
     const int64_t m0 = int64_t(tm) * TM, n0 = int64_t(tn) * TNB;
@@ -568,14 +574,14 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     const int wave_u = WN == 2 ? __builtin_amdgcn_readfirstlane(wave) : wave;
     const int64_t ks = PAIR == 0 ? int64_t(blockIdx.z) * s.k : 0;  // split-k: this workgroup's first k
     od += int64_t(blockIdx.z) * s.d_split;
-    // PAIR 2 to 4: the part's first k tile; PAIR 3 and 4: the operands from its first k on
+    // PAIR 2 to 5: the part's first k tile; PAIR 3 to 5: the operands from its first k on
     const int kfirst = PAIR >= 2 ? int(blockIdx.z) * k_part : 0;
     const int64_t kp = PAIR >= 3 ? int64_t(kfirst) * BK : ks;
     const uint16_t *pa = a + oa + kp * s.a_k, *pb = b + ob + kp * s.b_k;
-    const int64_t kb = PAIR == 2 ? s.k / 2 : PAIR == 4 ? s.k - kp : s.k;  // k of one B operand
+    const int64_t kb = PAIR == 2 ? s.k / 2 : PAIR >= 4 ? s.k - kp : s.k;  // k of one B operand
     // PAIR: k tiles of one operand, the last of them perhaps in part; a part takes k_part of all of them
     const int kth = int((kb + BK - 1) / BK);
-    const int ktiles = PAIR == 0 ? int(s.k / BK) : PAIR == 1 ? kth : min(k_part, PAIR == 4 ? kth : (PAIR == 2 ? 2 * kth : kth) - kfirst);
+    const int ktiles = PAIR == 0 ? int(s.k / BK) : PAIR == 1 ? kth : min(k_part, PAIR >= 4 ? kth : (PAIR == 2 ? 2 * kth : kth) - kfirst);
     const int64_t krows = PAIR == 3 ? min(s.k - kp, int64_t(k_part) * BK) : kb;
     (void)kth, (void)kfirst, (void)krows;
 
@@ -587,7 +593,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     int64_t mrem = s.m - m0 < TM ? s.m - m0 : TM, nrem = s.n - n0 < TNB ? s.n - n0 : TNB;
     if constexpr (BT && PAIR != 0) nrem = (nrem + 7) & ~int64_t(7);  // rows along n (and m) hold whole chunks
     if constexpr (PAIR == 3) mrem = (mrem + 7) & ~int64_t(7);
-    const int64_t abytes = PAIR == 3 ? ((krows - 1) * s.a_k + mrem) * 2 : AT ? ((s.k - 1) * s.a_k + mrem) * 2 : ((mrem - 1) * s.a_m + (PAIR == 4 ? kb : s.k)) * 2;
+    const int64_t abytes = PAIR == 3 ? ((krows - 1) * s.a_k + mrem) * 2 : AT ? ((s.k - 1) * s.a_k + mrem) * 2 : ((mrem - 1) * s.a_m + (PAIR == 5 ? (kb + 7) & ~int64_t(7) : PAIR == 4 ? kb : s.k)) * 2;
     const int64_t bbytes = PAIR == 0 ? (BT ? ((s.k - 1) * s.b_k + nrem) * 2 : ((nrem - 1) * s.b_n + s.k) * 2)
                                      : (BT ? ((krows - 1) * s.b_k + nrem) * 2 : ((nrem - 1) * s.b_n + kb) * 2);
     constexpr bool buf = BUF;  // the launcher checked stream_buffer_ok()
@@ -596,7 +602,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     const __amdgpu_buffer_rsrc_t rsb = __builtin_amdgcn_make_buffer_rsrc(
         (void *)(BT ? pb + n0 : pb + n0 * s.b_n), (short)0, int(bbytes), 0x00020000);
     const __amdgpu_buffer_rsrc_t rsb2 = __builtin_amdgcn_make_buffer_rsrc(
-        (void *)(PAIR == 0 || PAIR == 3 ? b2 : BT ? b2 + n0 : b2 + n0 * s.b_n + (PAIR == 4 ? kp : 0)), (short)0, int(PAIR == 0 || PAIR == 3 ? 0 : bbytes), 0x00020000);
+        (void *)(PAIR == 0 || PAIR == 3 || PAIR == 5 ? b2 : BT ? b2 + n0 : b2 + n0 * s.b_n + (PAIR == 4 ? kp : 0)), (short)0, int(PAIR == 0 || PAIR == 3 || PAIR == 5 ? 0 : bbytes), 0x00020000);
     (void)rsb2;
     auto issue = [&](int st, int kt, int lo, int hi) {
         char *base = smem + st * STAGE_BYTES;
@@ -1038,7 +1044,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
                 for (int q = 0; q < G; ++q) {
                     const int idx = lane + 64 * (g0 + q);
                     const int64_t gr = rbase + 64 * half + idx / CPR, gc = cbase + 4 * (idx % CPR);
-                    if (gr < s.m && gc < s.n) pre[q] = out.load(gr, gc);
+                    if (gr < s.m && (TakesWholeRows<Out>::value || gc < s.n)) pre[q] = out.load(gr, gc);
                 }
             };
             fetch(0);
@@ -1052,7 +1058,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
                     const int idx = lane + 64 * (g0 + q);
                     const int r = idx / CPR, ch = idx % CPR;
                     const int64_t gr = rbase + 64 * half + r, gc = cbase + 4 * ch;
-                    if (gr < s.m && gc < s.n) {
+                    if (gr < s.m && (TakesWholeRows<Out>::value || gc < s.n)) {
                         if constexpr (Out::kColSum) {
                             const float4 c4 = out(gr, gc, *reinterpret_cast<const float4 *>(stage + r * PITCH + ch * 16), pre[q]);
                             colsum.x += c4.x;

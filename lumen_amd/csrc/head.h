@@ -1,0 +1,302 @@
+// The cross entropy of a vocabulary head, and its gradients, without its logits: for rows h [t, k], classes w [v, k]
+//
+//   l = h w^T, lse = log(sum(exp(l))), loss = lse - l[target], p = exp(l - lse)
+//   d = (p - onehot(target)) g, dh = d w, dw = d^T h        (g: a row's cotangent; an ignored row's loss and d are 0)
+//
+// Six t v k multiply-adds, half of what a backward that computes the logits again would add to the forward's two: the
+// forward product's store leaves exp(l - m) as 16 bits for a piece of the rows, m being the maximum of its 64 classes, and
+// one pass turns these into d in place once the row's lse is known. A piece's values are scratch that the next piece
+// writes over; the logits exist in registers alone.
+//
+// exp(l - m) is between 0 and 1 and needs no sign: 6 bits of exponent (from 2^-63, below which it is 0) and 10 of mantissa,
+// off by 2^-11 relative to the value at most, an eighth of what bf16's p is rounded by. d is then rounded once, to the operands'
+// type, which the matrix instructions take; float16's d is taken times a power of two that puts the largest |g| at 2^13 to
+// 2^14, so that a mean's 1 / t does not push p out of its range (head_scale_kernel), and the products are divided by it again.
+// Sums are float32; over classes of a row first float32 in blocks of 64, then float64.
+#pragma once
+
+#include "device_common.h"
+#include "gemm.h"
+
+namespace nhipk {
+
+// Where a class's target stands: clamped into the classes, and whether the row is ignored.
+struct HeadTargets {
+    const void *target;
+    int64_t ignore, classes;
+    int32_t t64;
+    __device__ __forceinline__ int64_t at(int64_t r, bool &ignored) const {
+        const int64_t t = t64 ? static_cast<const int64_t *>(target)[r] : static_cast<const int32_t *>(target)[r];
+        ignored = t == ignore;
+        return t < 0 ? 0 : t >= classes ? classes - 1 : t;
+    }
+};
+
+constexpr int32_t kHeadLeast = 64 << 23;  // the float32 bits of 2^-63
+
+// A value of [0, 1] as 16 bits, rounded to nearest, and back.
+__device__ __forceinline__ uint32_t head_code(float e) {
+    const int32_t bits = __float_as_int(e) - (kHeadLeast - 0x1000);
+    return uint32_t(bits < 0 ? 0 : bits) >> 13;
+}
+__device__ __forceinline__ float head_value(uint32_t code) {
+    return code ? __int_as_float(int32_t(code << 13) + kHeadLeast) : 0.0f;
+}
+
+template <int CTRL>
+__device__ __forceinline__ float head_dpp(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+
+// The store of the forward product: gemm_stream_tile hands a lane four consecutive columns of one row, and the 16 lanes of a
+// DPP row hold a block of 64: its maximum and the float32 sum of exp(l - maximum) combine across them by rotations, the block's
+// first lane stores both, every lane its four codes, and the lane with the target's column that logit. Columns past the classes
+// count for nothing and are stored as zeros up to whole blocks.
+template <bool GRAD>
+struct HeadOut {
+    float2 *part;     // [rows, blocks]
+    float *picked;    // [rows]
+    uint16_t *codes;  // [rows, 64 blocks]
+    HeadTargets targets;
+    int64_t blocks;
+    static constexpr int kPrefetch = 8;
+    static constexpr bool kColSum = false;
+    struct Pre {
+        int64_t cls;
+    };
+    __device__ __forceinline__ Pre load(int64_t r, int64_t) const {
+        bool ignored;
+        return Pre{targets.at(r, ignored)};
+    }
+    __device__ __forceinline__ void operator()(int64_t r, int64_t c, float4 x, const Pre &pre) const {
+        const int64_t v = targets.classes;
+        if (c + 4 > v) {
+            if (c + 0 >= v) x.x = -INFINITY;
+            if (c + 1 >= v) x.y = -INFINITY;
+            if (c + 2 >= v) x.z = -INFINITY;
+            if (c + 3 >= v) x.w = -INFINITY;
+        }
+        // row_ror 8, row_ror 4, then the quad permutations [2,3,0,1] and [1,0,3,2]
+        float m = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
+        m = fmaxf(m, head_dpp<0x128>(m));
+        m = fmaxf(m, head_dpp<0x124>(m));
+        m = fmaxf(m, head_dpp<0x4e>(m));
+        m = fmaxf(m, head_dpp<0xb1>(m));
+        constexpr float kLog2e = 1.4426950408889634f;
+        float4 e = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (m != -INFINITY) {
+            e.x = __builtin_amdgcn_exp2f((x.x - m) * kLog2e), e.y = __builtin_amdgcn_exp2f((x.y - m) * kLog2e);
+            e.z = __builtin_amdgcn_exp2f((x.z - m) * kLog2e), e.w = __builtin_amdgcn_exp2f((x.w - m) * kLog2e);
+        }
+        float sum = (e.x + e.y) + (e.z + e.w);
+        sum += head_dpp<0x128>(sum);
+        sum += head_dpp<0x124>(sum);
+        sum += head_dpp<0x4e>(sum);
+        sum += head_dpp<0xb1>(sum);
+        const int64_t block = c >> 6;
+        if (block >= blocks) return;
+        if ((c & 63) == 0) part[r * blocks + block] = make_float2(m, sum);
+        if constexpr (GRAD)
+            *reinterpret_cast<uint2 *>(codes + r * blocks * 64 + c) =
+                make_uint2(head_code(e.x) | head_code(e.y) << 16, head_code(e.z) | head_code(e.w) << 16);
+        if (pre.cls >= c && pre.cls < c + 4) {
+            const int64_t q = pre.cls - c;
+            picked[r] = q == 0 ? x.x : q == 1 ? x.y : q == 2 ? x.z : x.w;
+        }
+    }
+};
+template <bool GRAD>
+struct TakesWholeRows<HeadOut<GRAD>> : std::true_type {};
+
+template <bool F16, int TM, bool GRAD>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TM == 256 ? 1 : 2, TM == 256 ? 1 : 2))) void head_logits_kernel(
+    GemmShape s, const uint16_t *__restrict__ a, const uint16_t *__restrict__ b, HeadOut<GRAD> out) {
+    extern __shared__ __align__(1024) char smem[];
+    gemm_stream_tile<F16, 64, 2, false, false, true, HeadOut<GRAD>, TM, TM == 256 ? 3 : 0>(s, a, b, out, smem);
+}
+
+// One wavefront a row: lse of its blocks' maxima and sums, and the loss.
+static __global__ __launch_bounds__(256) void head_merge_kernel(const float2 *__restrict__ part, const float *__restrict__ picked,
+                                                                HeadTargets targets, int64_t rows, int64_t blocks,
+                                                                float *__restrict__ lse, float *__restrict__ losses) {
+    const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= rows) return;  // the whole wavefront
+    const float2 *p = part + row * blocks;
+    float m = -INFINITY;
+    for (int64_t j = lane; j < blocks; j += 64) m = fmaxf(m, p[j].x);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    double sum = 0.0;
+    for (int64_t j = lane; j < blocks; j += 64) {
+        const float2 q = p[j];
+        if (q.x != -INFINITY) sum += double(q.y) * double(__builtin_amdgcn_exp2f((q.x - m) * 1.4426950408889634f));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) {
+        bool ignored;
+        targets.at(row, ignored);
+        const double l = double(m) + log(sum);
+        if (lse) lse[row] = float(l);
+        if (losses) losses[row] = ignored ? 0.0f : float(l - double(picked[row]));
+    }
+}
+
+// scale[0]: the power of two that takes the largest |g| to [2^13, 2^14) (1 where g is all zeros or not finite); scale[1]: one
+// over it.
+static __global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restrict__ g, int64_t rows, float *__restrict__ scale) {
+    __shared__ float most[16];
+    float m = 0.0f;
+    for (int64_t i = threadIdx.x; i < rows; i += 1024) m = fmaxf(m, fabsf(g[i]));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int i = 1; i < 16; ++i) m = fmaxf(m, most[i]);
+    int power = 0;
+    if (m > 0.0f && m < INFINITY) {
+        int e;
+        frexpf(m, &e);  // m in [2^(e - 1), 2^e)
+        power = 14 - e;
+        power = power < -100 ? -100 : power > 100 ? 100 : power;
+    }
+    scale[0] = ldexpf(1.0f, power), scale[1] = ldexpf(1.0f, -power);
+}
+
+// The codes of a piece's rows into d, in place: a workgroup a row, 8 classes a thread at a time. The target's is
+// g expm1(l - lse), which p - 1 would cancel.
+template <bool F16>
+__global__ __launch_bounds__(256) void head_grad_kernel(uint16_t *__restrict__ codes, const float2 *__restrict__ part,
+                                                        const float *__restrict__ picked, const float *__restrict__ lse,
+                                                        const float *__restrict__ g, const float *__restrict__ scale, HeadTargets targets,
+                                                        int64_t blocks) {
+    const int64_t row = blockIdx.x;
+    bool ignored;
+    const int64_t cls = targets.at(row, ignored);
+    const float l = lse[row], f = F16 ? g[row] * scale[0] : g[row];
+    uint16_t *p = codes + row * blocks * 64;
+    const float2 *q = part + row * blocks;
+    auto round = [](float v) { return uint32_t(F16 ? f32_to_f16(v) : f32_to_bf16(v)); };
+    for (int64_t c = 8 * threadIdx.x; c < blocks * 64; c += 2048) {
+        uint4 out = make_uint4(0, 0, 0, 0);
+        if (!ignored) {
+            const uint4 in = *reinterpret_cast<const uint4 *>(p + c);
+            const float k = f * __builtin_amdgcn_exp2f((q[c >> 6].x - l) * 1.4426950408889634f);
+            const uint32_t w[4] = {in.x, in.y, in.z, in.w};
+            uint32_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = round(head_value(w[i] & 0xffff) * k) | round(head_value(w[i] >> 16) * k) << 16;
+            if (cls >= c && cls < c + 8) {
+                const uint32_t d = round(f * expm1f(picked[row] - l)), at = uint32_t(cls - c), shift = at % 2 * 16;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i)
+                    if (at / 2 == i) o[i] = (o[i] & ~(0xffffu << shift)) | d << shift;
+            }
+            out = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        *reinterpret_cast<uint4 *>(p + c) = out;
+    }
+}
+
+// The store of a gradient's product: the float32 sums of the pieces before added, then kept as sums or rounded into the result.
+struct HeadStore {
+    const float *before;  // null: none
+    float *sums;          // null: this is the last piece
+    uint16_t *out;
+    const float *inverse;  // what the products are multiplied by, or null
+    int64_t n;             // columns, a row's elements too
+    int32_t f16;
+    static constexpr int kPrefetch = 8;
+    static constexpr bool kColSum = false;
+    struct Pre {
+        float4 v;
+    };
+    __device__ __forceinline__ Pre load(int64_t r, int64_t c) const {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (before) {
+            const float *p = before + r * n + c;
+            if (n % 4 == 0) v = *reinterpret_cast<const float4 *>(p);
+            else v = make_float4(p[0], c + 1 < n ? p[1] : 0.0f, c + 2 < n ? p[2] : 0.0f, c + 3 < n ? p[3] : 0.0f);
+        }
+        return Pre{v};
+    }
+    __device__ __forceinline__ void operator()(int64_t r, int64_t c, float4 x, const Pre &pre) const {
+        float e[4] = {x.x + pre.v.x, x.y + pre.v.y, x.z + pre.v.z, x.w + pre.v.w};
+        if (sums) {
+            float *p = sums + r * n + c;
+            if (n % 4 == 0) *reinterpret_cast<float4 *>(p) = make_float4(e[0], e[1], e[2], e[3]);
+            else
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (c + i < n) p[i] = e[i];
+            return;
+        }
+        const float k = inverse ? *inverse : 1.0f;
+        uint16_t *p = out + r * n + c;
+        uint32_t b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = f16 ? f32_to_f16(e[i] * k) : f32_to_bf16(e[i] * k);
+        if (n % 4 == 0) *reinterpret_cast<uint2 *>(p) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c + i < n) p[i] = uint16_t(b[i]);
+    }
+};
+
+// dh = d w over a piece's rows: d in whole blocks of classes, w's rows as they lie, those past v read as zeros.
+template <bool F16, int TM, int ST, class Out>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ST == 2 ? 2 : 1, ST == 2 ? 2 : 1))) void head_input_grad(
+    GemmShape s, const uint16_t *__restrict__ d, const uint16_t *__restrict__ w, Out out, int k_part) {
+    extern __shared__ __align__(1024) char smem[];
+    gemm_stream_tile<F16, 64, 2, false, true, true, Out, TM, TM == 256 ? 3 : ST == 3 ? 1 : 0, 5, TM == 256 ? 0 : ST>(s, d, w, out, smem,
+                                                                                                                  nullptr, k_part);
+}
+
+// dw = d^T h over a piece's rows.
+template <bool F16, int TM, int ST, class Out>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ST == 2 ? 2 : 1, ST == 2 ? 2 : 1))) void head_weight_grad(
+    GemmShape s, const uint16_t *__restrict__ d, const uint16_t *__restrict__ h, Out out, int k_part) {
+    extern __shared__ __align__(1024) char smem[];
+    gemm_stream_tile<F16, 64, 2, true, true, true, Out, TM, TM == 256 ? 3 : ST == 3 ? 1 : 0, 3, TM == 256 ? 0 : ST>(s, d, h, out, smem,
+                                                                                                                  nullptr, k_part);
+}
+
+// Float32 sums of a product's parts, P[part][mn], added in order and stored as HeadStore stores a tile (of one row).
+static __global__ __launch_bounds__(256) void head_sum_kernel(const float *__restrict__ part, int parts, int64_t mn, HeadStore out) {
+    out.n = mn;
+    for (int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4; i < mn; i += int64_t(gridDim.x) * 1024) {
+        float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < parts; ++k) {
+            const float *p = part + k * mn + i;
+            if (mn % 4 == 0) {
+                const float4 v = *reinterpret_cast<const float4 *>(p);
+                e[0] += v.x, e[1] += v.y, e[2] += v.z, e[3] += v.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (i + j < mn) e[j] += p[j];
+            }
+        }
+        out(0, i, make_float4(e[0], e[1], e[2], e[3]), out.load(0, i));
+    }
+}
+
+// Rows of any length, alignment or distance as the products read them: copied to rows of kp elements, zeros past k. MASK: zeros
+// in ignored rows too, whose d of 0 times a NaN or an infinity of theirs would be no 0 in dw.
+template <bool MASK>
+__global__ __launch_bounds__(256) void head_pad_kernel(const uint16_t *__restrict__ src, int64_t rows, int64_t ld, int64_t k, int64_t kp,
+                                                       uint16_t *__restrict__ dst, HeadTargets targets) {
+    const int64_t per = kp / 8, total = rows * per;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+        const int64_t row = i / per, c = (i - row * per) * 8;
+        bool ignored = false;
+        if constexpr (MASK) targets.at(row, ignored);
+        *reinterpret_cast<uint4 *>(dst + row * kp + c) =
+            c < k && !ignored ? load8_any(src + row * ld + c, k - c) : make_uint4(0, 0, 0, 0);
+    }
+}
+
+}  // namespace nhipk

@@ -1,0 +1,272 @@
+// C entry points of the cross entropy of a vocabulary head with its gradients (head.h).
+#include <algorithm>
+#include <cstring>
+#include <string>
+#include <type_traits>
+
+#include "head.h"
+#include "nhip_internal.h"
+#include "parts.h"
+
+using namespace nhip;
+using namespace nhipk;
+
+namespace nhip {
+namespace {
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+int64_t blocks_of(const nhip_head_desc *d) { return (d->classes + 63) / 64; }
+int64_t padded_k(const nhip_head_desc *d) { return up(d->k, 64); }
+
+// Rows of a piece: what fits the bytes that the desc allows for its codes, a multiple of 256 (a tile's), and pieces of one size.
+int64_t piece_rows(const nhip_head_desc *d) {
+    const int64_t row = blocks_of(d) * 64 * 2;
+    // the weight gradient reads a piece's codes through one buffer of 2^31 bytes
+    const int64_t bytes = std::min(d->piece_bytes, (int64_t(1) << 31) - (int64_t(1) << 20));
+    const int64_t most = std::max<int64_t>(bytes / row / 256 * 256, 256);
+    if (d->rows <= most) return d->rows;
+    const int64_t pieces = (d->rows + most - 1) / most;
+    return std::min(most, up((d->rows + pieces - 1) / pieces, 256));
+}
+int64_t pieces_of(const nhip_head_desc *d) { return d->rows > 0 ? (d->rows + piece_rows(d) - 1) / piece_rows(d) : 0; }
+
+PartPlan input_plan(const nhip_head_desc *d) {
+    return part_plan(piece_rows(d), d->k, 1, (d->classes + 63) / 64, int64_t(1) << 30);
+}
+PartPlan weight_plan(const nhip_head_desc *d) {
+    const int64_t total = (piece_rows(d) + 63) / 64;
+    PartPlan p = part_plan(d->classes, d->k, 1, total, int64_t(1) << 30);
+    // the pieces' sums are added in the store, which parts do without
+    if (pieces_of(d) > 1 && p.parts > 1) p = PartPlan{256, 1, int(total), false, 0.0};
+    return p;
+}
+
+// Whether rows are copied first: no whole k tiles, or not on 16 bytes. The gradients always read a copy of h (head_pad_kernel).
+bool copies(const nhip_head_desc *d, int64_t ld) { return d->k % 64 != 0 || ld % 8 != 0; }
+
+struct HeadSpace {
+    size_t h, w, part, picked, lse, scale, codes, weight_sums, input_parts, weight_parts, bytes;
+};
+HeadSpace head_space(const nhip_head_desc *d, bool grad) {
+    HeadSpace s{};
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t from = at;
+        at += up256(bytes);
+        return from;
+    };
+    const int64_t kp = padded_k(d), rows = grad ? piece_rows(d) : d->rows;
+    s.h = take(grad || copies(d, d->h_m) ? size_t(d->rows) * kp * 2 : 0);
+    s.w = take(copies(d, d->w_n) ? size_t(d->classes) * kp * 2 : 0);
+    s.part = take(size_t(rows) * blocks_of(d) * sizeof(float2));
+    s.picked = take(size_t(rows) * 4);
+    s.lse = take(size_t(rows) * 4);
+    s.scale = take(8);
+    if (grad) {
+        const PartPlan pi = input_plan(d), pw = weight_plan(d);
+        s.codes = take(size_t(rows) * blocks_of(d) * 64 * 2);
+        s.weight_sums = take(pieces_of(d) > 1 ? size_t(d->classes) * d->k * 4 : 0);
+        // the parts of one product at a time
+        s.input_parts = s.weight_parts =
+            take(std::max(pi.parts > 1 ? size_t(pi.parts) * rows * d->k * 4 : 0, pw.parts > 1 ? size_t(pw.parts) * d->classes * d->k * 4 : 0));
+    }
+    s.bytes = at;
+    return s;
+}
+
+int head_check(const nhip_head_desc *d, const char *what) {
+    const std::string at(what);
+    if (d->rows < 0 || d->classes < 1 || d->k < 1) return fail(at + ": needs rows >= 0, classes >= 1 and k >= 1");
+    if (d->dtype != NHIP_BF16 && d->dtype != NHIP_F16) return fail(at + ": bf16 or f16 operands only");
+    if (d->target_dtype != NHIP_LCE_I32 && d->target_dtype != NHIP_LCE_I64) return fail(at + ": targets must be int32 or int64");
+    if (d->h_m < 0 || d->w_n < d->k) return fail(at + ": rows that lie backwards, or classes that overlap");
+    const int64_t lim = (int64_t(1) << 30) - 1024, kp = padded_k(d);
+    if (kp >= int64_t(1) << 20 || d->h_m >= int64_t(1) << 20 || d->classes >= int64_t(1) << 22 ||
+        (d->classes + 256) * std::max(kp, d->w_n) >= lim)
+        return fail(at + ": rows below 2^20 elements, 2^22 classes, and a weight within 2^31 bytes");
+    if (d->rows >= int64_t(1) << 31 || tiles(d->rows, 128, d->classes, 128) >= int64_t(1) << 24 ||
+        tiles(d->classes, 128, d->k, 128) >= int64_t(1) << 24 || tiles(d->rows, 128, d->k, 128) >= int64_t(1) << 24)
+        return fail(at + ": a launch of 2^32 threads");
+    if (d->piece_bytes < 0) return fail(at + ": negative sizes");
+    if (256 * blocks_of(d) * 64 * 2 >= int64_t(1) << 31) return fail(at + ": a tile's rows of classes within 2^31 bytes");
+    return 0;
+}
+
+template <class... P>
+int launch(hipStream_t st, void (*kern)(P...), dim3 grid, int lds, const char *what, std::common_type_t<P>... args) {
+    if (check(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
+              "hipFuncSetAttribute"))
+        return 1;
+    hipLaunchKernelGGL(kern, grid, dim3(256), lds, st, args...);
+    return check(hipGetLastError(), what);
+}
+
+constexpr int kLds256 = gemm_stream_lds_bytes<64, 2>(), kLds128 = gemm_stream_lds_bytes<64, 2, 128>(),
+              kLdsDeep = gemm_stream_lds_bytes<64, 2, 128, 3>();
+
+GemmShape shape(int64_t m, int64_t n, int64_t k, int tm) {
+    GemmShape s;
+    std::memset(&s, 0, sizeof(s));
+    s.m = m, s.n = n, s.k = k, s.d_m = n, s.d_n = 1;
+    s.tiles_m = int((m + tm - 1) / tm), s.tiles_n = int((n + tm - 1) / tm);
+    return s;
+}
+
+template <bool F16, bool GRAD>
+int logits(hipStream_t st, const nhip_head_desc *d, int64_t rows, const uint16_t *h, int64_t h_m, const uint16_t *w, int64_t w_n,
+           const HeadOut<GRAD> &out) {
+    // 256-row tiles where they fill the CUs
+    const int tm = tiles(rows, 256, d->classes, 256) >= 256 ? 256 : 128;
+    GemmShape s = shape(rows, d->classes, padded_k(d), tm);
+    s.a_m = h_m, s.a_k = 1, s.b_k = 1, s.b_n = w_n;
+    const dim3 grid(unsigned(s.tiles_m) * unsigned(s.tiles_n));
+    if (tm == 256) return launch(st, head_logits_kernel<F16, 256, GRAD>, grid, kLds256, "head_logits_kernel launch", s, h, w, out);
+    return launch(st, head_logits_kernel<F16, 128, GRAD>, grid, kLds128, "head_logits_kernel launch", s, h, w, out);
+}
+
+int parts_sum(hipStream_t st, const float *part, const PartPlan &p, int64_t mn, const HeadStore &to) {
+    const int64_t blocks = (mn + 1023) / 1024;
+    hipLaunchKernelGGL(head_sum_kernel, dim3(unsigned(std::min<int64_t>(blocks, 4096))), dim3(256), 0, st, part, p.parts, mn, to);
+    return check(hipGetLastError(), "head_sum_kernel launch");
+}
+
+// One of the gradients' products, whole into `to` or in parts through `part`.
+#define NHIP_HEAD_PRODUCT(KERN, WHAT)                                                                                        \
+    const dim3 grid(unsigned(s.tiles_m) * unsigned(s.tiles_n), 1, unsigned(p.parts));                                         \
+    if (p.parts == 1) {                                                                                                       \
+        if (p.tm == 256) return launch(st, KERN<F16, 256, 0, HeadStore>, grid, kLds256, WHAT, s, a, b, to, p.k_part);           \
+        if (p.deep) return launch(st, KERN<F16, 128, 3, HeadStore>, grid, kLdsDeep, WHAT, s, a, b, to, p.k_part);              \
+        return launch(st, KERN<F16, 128, 2, HeadStore>, grid, kLds128, WHAT, s, a, b, to, p.k_part);                           \
+    }                                                                                                                         \
+    s.d_split = s.m * s.n;                                                                                                    \
+    const AnyStore sums{part, 0};                                                                                             \
+    if (p.tm == 256 ? launch(st, KERN<F16, 256, 0, AnyStore>, grid, kLds256, WHAT, s, a, b, sums, p.k_part)                    \
+        : p.deep    ? launch(st, KERN<F16, 128, 3, AnyStore>, grid, kLdsDeep, WHAT, s, a, b, sums, p.k_part)                   \
+                    : launch(st, KERN<F16, 128, 2, AnyStore>, grid, kLds128, WHAT, s, a, b, sums, p.k_part))                   \
+        return 1;                                                                                                             \
+    return parts_sum(st, part, p, s.m * s.n, to)
+
+template <bool F16>
+int input_grad(hipStream_t st, const nhip_head_desc *d, const PartPlan &p, int64_t rows, const uint16_t *a, const uint16_t *b, int64_t w_n,
+               float *part, const HeadStore &to) {
+    GemmShape s = shape(rows, d->k, d->classes, p.tm);
+    s.a_m = blocks_of(d) * 64, s.a_k = 1, s.b_k = w_n, s.b_n = 1;
+    NHIP_HEAD_PRODUCT(head_input_grad, "head_input_grad launch");
+}
+
+template <bool F16>
+int weight_grad(hipStream_t st, const nhip_head_desc *d, const PartPlan &p, int64_t rows, const uint16_t *a, const uint16_t *b, int64_t h_m,
+                float *part, const HeadStore &to) {
+    GemmShape s = shape(d->classes, d->k, rows, p.tm);
+    s.a_m = 1, s.a_k = blocks_of(d) * 64, s.b_k = h_m, s.b_n = 1;
+    NHIP_HEAD_PRODUCT(head_weight_grad, "head_weight_grad launch");
+}
+#undef NHIP_HEAD_PRODUCT
+
+bool on(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+template <bool MASK>
+int pad(hipStream_t st, const uint16_t *src, int64_t rows, int64_t ld, int64_t k, int64_t kp, uint16_t *dst, const HeadTargets &targets) {
+    const int64_t blocks = (rows * (kp / 8) + 255) / 256;
+    if (!blocks) return 0;
+    hipLaunchKernelGGL((head_pad_kernel<MASK>), dim3(unsigned(std::min<int64_t>(blocks, 8192))), dim3(256), 0, st, src, rows, ld, k, kp, dst,
+                       targets);
+    return check(hipGetLastError(), "head_pad_kernel launch");
+}
+
+template <bool F16>
+int head_run(hipStream_t st, const nhip_head_desc *d, const uint16_t *h, const uint16_t *w, const void *target, const float *g,
+             float *losses, uint16_t *dh, uint16_t *dw, char *ws) {
+    const bool grad = g != nullptr;
+    const HeadSpace at = head_space(d, grad);
+    const int64_t kp = padded_k(d), blocks = blocks_of(d), tsize = d->target_dtype == NHIP_LCE_I64 ? 8 : 4;
+    int64_t h_m = d->h_m, w_n = d->w_n;
+    HeadTargets targets{target, d->ignore_index, d->classes, d->target_dtype == NHIP_LCE_I64};
+    if (grad || copies(d, h_m)) {
+        uint16_t *to = reinterpret_cast<uint16_t *>(ws + at.h);
+        if (grad ? pad<true>(st, h, d->rows, h_m, d->k, kp, to, targets) : pad<false>(st, h, d->rows, h_m, d->k, kp, to, targets)) return 1;
+        h = to, h_m = kp;
+    }
+    if (copies(d, w_n)) {
+        uint16_t *to = reinterpret_cast<uint16_t *>(ws + at.w);
+        if (pad<false>(st, w, d->classes, w_n, d->k, kp, to, targets)) return 1;
+        w = to, w_n = kp;
+    }
+    float2 *part = reinterpret_cast<float2 *>(ws + at.part);
+    float *picked = reinterpret_cast<float *>(ws + at.picked), *lse = reinterpret_cast<float *>(ws + at.lse);
+    float *scale = reinterpret_cast<float *>(ws + at.scale);
+    uint16_t *codes = reinterpret_cast<uint16_t *>(ws + at.codes);
+    auto merge = [&](int64_t r0, int64_t rows) {
+        hipLaunchKernelGGL(head_merge_kernel, dim3(unsigned((rows + 3) / 4)), dim3(256), 0, st, part, picked, targets, rows, blocks,
+                           grad ? lse : nullptr, losses ? losses + r0 : nullptr);
+        return check(hipGetLastError(), "head_merge_kernel launch");
+    };
+    if (!grad) return logits<F16, false>(st, d, d->rows, h, h_m, w, w_n, HeadOut<false>{part, picked, nullptr, targets, blocks}) || merge(0, d->rows);
+    if (F16) {
+        hipLaunchKernelGGL(head_scale_kernel, dim3(1), dim3(1024), 0, st, g, d->rows, scale);
+        if (check(hipGetLastError(), "head_scale_kernel launch")) return 1;
+    }
+    const PartPlan pi = input_plan(d), pw = weight_plan(d);
+    const int64_t most = piece_rows(d), pieces = pieces_of(d);
+    float *sums = reinterpret_cast<float *>(ws + at.weight_sums), *parts = reinterpret_cast<float *>(ws + at.input_parts);
+    const float *inverse = F16 ? scale + 1 : nullptr;
+    for (int64_t i = 0, r0 = 0; i < pieces; ++i, r0 += most) {
+        const int64_t rows = std::min(most, d->rows - r0);
+        const uint16_t *hp = h + r0 * h_m;
+        targets.target = static_cast<const char *>(target) + r0 * tsize;
+        if (logits<F16, true>(st, d, rows, hp, h_m, w, w_n, HeadOut<true>{part, picked, codes, targets, blocks}) || merge(r0, rows)) return 1;
+        hipLaunchKernelGGL((head_grad_kernel<F16>), dim3(unsigned(rows)), dim3(256), 0, st, codes, part, picked, lse, g + r0, scale, targets,
+                           blocks);
+        if (check(hipGetLastError(), "head_grad_kernel launch")) return 1;
+        // a last piece of fewer rows keeps its plan: its sums are shorter, its tiles fewer
+        if (dh && input_grad<F16>(st, d, pi, rows, codes, w, w_n, parts, HeadStore{nullptr, nullptr, dh + r0 * d->k, inverse, d->k, F16}))
+            return 1;
+        if (dw) {
+            PartPlan p = pw;
+            p.k_part = int(std::min<int64_t>(p.k_part, (rows + 63) / 64));
+            if (weight_grad<F16>(st, d, p, rows, codes, hp, h_m, parts,
+                                 HeadStore{i ? sums : nullptr, i + 1 < pieces ? sums : nullptr, dw, inverse, d->k, F16}))
+                return 1;
+        }
+    }
+    return 0;
+}
+
+}  // namespace
+
+int head_on(hipStream_t st, const nhip_head_desc *d, const void *h, const void *w, const void *target, const float *g, float *losses,
+            void *dh, void *dw, void *ws) {
+    if (head_check(d, "nhip_head_loss")) return 1;
+    if (!g && (dh || dw)) return fail("nhip_head_loss: gradients need the losses' cotangents");
+    if (g && !dh && !dw) g = nullptr;
+    if (!on(ws, 256)) return fail("nhip_head_loss: the workspace starts on 256 bytes");
+    if (!on(dh, 8) || !on(dw, 8)) return fail("nhip_head_loss: gradients start on 8 bytes");
+    if ((!g && !copies(d, d->h_m) && !on(h, 16)) || (!copies(d, d->w_n) && !on(w, 16)))
+        return fail("nhip_head_loss: operands of whole rows start on 16 bytes");
+    if (d->rows == 0) return dw ? fill_on(st, dw, size_t(d->classes) * d->k * 2, 0) : 0;
+    if (!ws) return fail("nhip_head_loss: no workspace");
+    auto go = d->dtype == NHIP_F16 ? head_run<true> : head_run<false>;
+    return go(st, d, static_cast<const uint16_t *>(h), static_cast<const uint16_t *>(w), target, g, losses, static_cast<uint16_t *>(dh),
+              static_cast<uint16_t *>(dw), static_cast<char *>(ws));
+}
+
+}  // namespace nhip
+
+extern "C" {
+
+int nhip_head_loss(const nhip_head_desc *desc, const void *h, const void *w, const void *target, const float *g, float *losses, void *dh,
+                   void *dw, void *workspace) {
+    hipStream_t st = stream_of_current();
+    if (!st) return fail("no HIP stream: call nhip_set_device first");
+    return head_on(st, desc, h, w, target, g, losses, dh, dw, workspace);
+}
+
+int nhip_head_loss_workspace(const nhip_head_desc *desc, int gradients, size_t *bytes) {
+    if (head_check(desc, "nhip_head_loss_workspace")) return 1;
+    *bytes = head_space(desc, gradients != 0).bytes;
+    return 0;
+}
+
+}  // extern "C"

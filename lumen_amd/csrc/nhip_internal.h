@@ -44,6 +44,8 @@ int clip_on(hipStream_t s, const nhip_clip_desc *d, const nhip_clip_tensor *t, c
             float *scale, void *ws);
 int adamw_on(hipStream_t s, const nhip_adamw_desc *d, const nhip_adamw_tensor *t, const double *lr_at, const void *step_at,
              const float *scale_at);
+int head_on(hipStream_t s, const nhip_head_desc *d, const void *h, const void *w, const void *target, const float *g, float *losses,
+            void *dh, void *dw, void *ws);
 int packed_fwd_on(hipStream_t s, const nhip_packed_desc *d, const void *q, const void *k, const void *v, const void *offsets, void *o,
                   float *lse, void *ws);
 int packed_bwd_on(hipStream_t s, const nhip_packed_desc *d, const void *q, const void *k, const void *v, const void *offsets,

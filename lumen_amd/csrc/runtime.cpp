@@ -470,7 +470,7 @@ int nhip_plan_add_launch(void *plan, void *function, const uint32_t grid[3], con
 
 int nhip_plan_add_builtin(void *plan, int kind, const void *desc, size_t desc_bytes, const nhip_reloc *relocs,
                           size_t nrelocs) {
-    if (kind < NHIP_STEP_GEMM || kind > NHIP_STEP_PACKED_BWD) return fail("nhip_plan_add_builtin: unknown step kind");
+    if (kind < NHIP_STEP_GEMM || kind > NHIP_STEP_HEAD_LOSS) return fail("nhip_plan_add_builtin: unknown step kind");
     // the descriptor must hold what run_steps reads for the kind
     size_t need = 0, pointers = 16;
     switch (kind) {
@@ -489,6 +489,7 @@ int nhip_plan_add_builtin(void *plan, int kind, const void *desc, size_t desc_by
         case NHIP_STEP_GATED_BACKWARD: need = sizeof(nhip_gated_desc); break;
         case NHIP_STEP_PACKED_FWD:
         case NHIP_STEP_PACKED_BWD: need = sizeof(nhip_packed_desc); break;
+        case NHIP_STEP_HEAD_LOSS: need = sizeof(nhip_head_desc); break;
         case NHIP_STEP_CLIP: {
             need = sizeof(nhip_clip_desc);
             if (desc && desc_bytes >= need) {
@@ -724,6 +725,10 @@ static int run_steps(Plan *plan, void *workspace, void *const *inputs, size_t ni
                 rc = packed_bwd_on(s, reinterpret_cast<const nhip_packed_desc *>(st.args.data()), ptrs[0], ptrs[1], ptrs[2],
                                    ptrs[3], ptrs[4], ptrs[5], static_cast<const float *>(ptrs[6]), ptrs[7], ptrs[8], ptrs[9],
                                    ptrs[10]);
+                break;
+            case NHIP_STEP_HEAD_LOSS:
+                rc = head_on(s, reinterpret_cast<const nhip_head_desc *>(st.args.data()), ptrs[0], ptrs[1], ptrs[2],
+                             static_cast<const float *>(ptrs[3]), static_cast<float *>(ptrs[4]), ptrs[5], ptrs[6], ptrs[7]);
                 break;
             case NHIP_STEP_FILL: {
                 uint64_t n;

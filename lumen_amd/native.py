@@ -19,7 +19,7 @@ NHIP_BASE_WORKSPACE, NHIP_BASE_INPUT = 0, 1
 NHIP_STEP_GEMM, NHIP_STEP_FLASH_FWD, NHIP_STEP_FLASH_BWD, NHIP_STEP_COPY, NHIP_STEP_FILL, NHIP_STEP_LCE = 1, 2, 3, 4, 5, 6
 NHIP_STEP_HEADS, NHIP_STEP_HEADS_BWD, NHIP_STEP_GATED, NHIP_STEP_GATED_GRAD, NHIP_STEP_CLIP = 7, 8, 9, 10, 11
 NHIP_STEP_GATED_INPUT, NHIP_STEP_GATED_WEIGHT, NHIP_STEP_GATED_BACKWARD = 12, 13, 14
-NHIP_STEP_ADAMW, NHIP_STEP_PACKED_FWD, NHIP_STEP_PACKED_BWD = 15, 16, 17
+NHIP_STEP_ADAMW, NHIP_STEP_PACKED_FWD, NHIP_STEP_PACKED_BWD, NHIP_STEP_HEAD_LOSS = 15, 16, 17, 18
 NHIP_LCE_I32, NHIP_LCE_I64 = 0, 1
 NHIP_POS_NONE, NHIP_POS_I32, NHIP_POS_I64 = 0, 1, 2
 NHIP_ACT = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
@@ -118,6 +118,14 @@ class ClipDesc(C.Structure):
     _fields_ = [("count", C.c_int64), ("max_norm", C.c_double), ("eps", C.c_double)]
 
 
+class HeadDesc(C.Structure):
+    """``nhip_head_desc``: the cross entropy of a vocabulary head (include/nhip.h)."""
+
+    _fields_ = [(n, C.c_int64) for n in ("rows", "classes", "k", "h_m", "w_n", "ignore_index", "piece_bytes")] + [
+        ("dtype", C.c_int32), ("target_dtype", C.c_int32)
+    ]
+
+
 class PackedDesc(C.Structure):
     """``nhip_packed_desc``: attention within sequences packed one after another (include/nhip.h)."""
 
@@ -209,6 +217,8 @@ SIGNATURES = {
     "nhip_gated_config_count": ([C.POINTER(C.c_int)], C.c_int),
     "nhip_gated_linear_grad": ([C.POINTER(GatedDesc)] + [C.c_void_p] * 4, C.c_int),
     "nhip_clip_grad_norm": ([C.POINTER(ClipDesc), C.POINTER(ClipTensor)] + [C.c_void_p] * 4, C.c_int),
+    "nhip_head_loss": ([C.POINTER(HeadDesc)] + [C.c_void_p] * 8, C.c_int),
+    "nhip_head_loss_workspace": ([C.POINTER(HeadDesc), C.c_int, C.POINTER(C.c_size_t)], C.c_int),
     "nhip_packed_fwd": ([C.POINTER(PackedDesc)] + [C.c_void_p] * 7, C.c_int),
     "nhip_packed_bwd": ([C.POINTER(PackedDesc)] + [C.c_void_p] * 11, C.c_int),
     "nhip_packed_workspace": ([C.POINTER(PackedDesc), C.c_int, C.POINTER(C.c_size_t)], C.c_int),

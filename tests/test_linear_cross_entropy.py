@@ -1,0 +1,189 @@
+"""linear_cross_entropy on the CPU: what it computes (the oracle on its traced body against plain float64 NumPy), its gradients
+against differences, its refusals, and the plan it becomes."""
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import lumen_amd as L
+import lumen_amd.functional as F
+from lumen_amd import native as nv
+from lumen_amd.compiler.plan import Plan, compile_graph
+from oracle import oracle
+from tests import training_math as M
+
+
+def _meta(a, dtype=None):
+    return L.empty(list(np.shape(a)), dtype or np.asarray(a).dtype.name, "meta")
+
+
+def _program(reduction, ignore=-100):
+    def fn(h, w, target, g):
+        loss, pull = L.vjp(lambda h, w: F.linear_cross_entropy(h, w, target, ignore, reduction), h, w)
+        return [loss, *pull(g)]
+
+    return fn
+
+
+def _case(rng, lead, k, v, dtype="float64"):
+    h, w = rng.standard_normal((*lead, k)).astype(dtype), rng.standard_normal((v, k)).astype(dtype)
+    target = rng.integers(0, v, lead)
+    return h, w, np.where(rng.random(lead) < 0.3, -100, target)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("reduction", F.linear_cross_entropy.__globals__["REDUCTIONS"])
+@pytest.mark.parametrize("lead,k,v,target_type", [((9,), 5, 11, "int64"), ((2, 3), 4, 7, "int32"), ((1,), 1, 1, "int64"), ((), 3, 4, "int32")])
+def test_values_and_gradients(dtype, reduction, lead, k, v, target_type):
+    rng = np.random.default_rng(k + v)
+    h, w, target = _case(rng, lead, k, v, dtype)
+    target = target.astype(target_type)
+    rows, n = int(np.prod(lead)), int((target != -100).sum())
+    given = np.asarray(rng.standard_normal(lead if reduction == "none" else ())).astype(dtype)
+    g = L.make_graph(_program(reduction))(*(_meta(a) for a in (h, w, target, given)))
+    assert not [x for x in g.nodes if x.prim == "fusion"]
+    got = oracle.values(g, [h, w, target, given])
+    each = given.reshape(rows) if reduction == "none" else np.full(rows, given / (max(n, 1) if reduction == "mean" else 1))
+    flat = (h.reshape(rows, k), w, target.reshape(rows), -100, each)
+    losses, dh, dw = M.linear_cross_entropy(*flat)
+    tl, th, tw = M.linear_cross_entropy_tolerances(*flat, "float32")
+    loss, tol = {"none": (losses.reshape(lead), tl.reshape(lead)), "sum": (losses.sum(), tl.sum() + 1e-6 * losses.sum()),
+                 "mean": (losses.sum() / max(n, 1), tl.sum() + 1e-6 * losses.sum())}[reduction]
+    for a, b, t in zip(got, (loss, dh.reshape(h.shape), dw), (tol, th.reshape(h.shape), tw)):
+        assert np.shape(a) == np.shape(b) and np.all(np.abs(a - b) <= (t if dtype == "float32" else t * 2.0**-13 + 1e-14))
+
+
+def test_gradient_against_differences():
+    rng = np.random.default_rng(1)
+    h, w, target = _case(rng, (4,), 3, 5)
+    x, g = {"h": h, "w": w}, rng.standard_normal(4)
+    _, dh, dw = M.linear_cross_entropy(h, w, target, -100, g)
+    from tests.operator_math import differences
+
+    for name, grad in (("h", dh), ("w", dw)):
+        diff = differences(lambda x: (M.linear_cross_entropy(x["h"], x["w"], target, -100, g)[0] * g).sum(), x, name)
+        assert np.abs(diff - grad).max() <= 1e-7
+
+
+def test_a_gradient_differentiated_again():
+    """The float64 derivative of dh along a direction against differences of dh."""
+    rng = np.random.default_rng(2)
+    h, w, target = _case(rng, (4,), 3, 5)
+    u, g = rng.standard_normal(h.shape), rng.standard_normal(4)
+
+    def fn(h, w, target, g, u):
+        def along(h):
+            _, pull = L.vjp(lambda h: F.linear_cross_entropy(h, w, target, reduction="none"), h)
+            return F.sum(pull(g)[0] * u)
+
+        return [L.grad(along)(h)]
+
+    args = [h, w, target, g, u]
+    (got,) = oracle.values(L.make_graph(fn)(*(_meta(a) for a in args)), args)
+    want = [M.linear_cross_entropy(h + s * 1e-5 * u, w, target, -100, g)[1] for s in (1, -1)]
+    assert np.abs(got - (want[0] - want[1]) / 2e-5).max() <= 1e-7
+
+
+def test_targets_outside_and_another_ignored_value():
+    rng = np.random.default_rng(3)
+    h, w, _ = _case(rng, (4,), 3, 5)
+    target = np.array([2, -1, 7, 3])
+    g = L.make_graph(lambda h, w, t: [F.linear_cross_entropy(h, w, t, ignore_index=2, reduction="none")])(*(_meta(a) for a in (h, w, target)))
+    (got,) = oracle.values(g, [h, w, target])
+    want = M.linear_cross_entropy(h, w, np.array([9, 0, 4, 3]), 9, np.ones(4))[0]
+    assert np.abs(got - want).max() <= 1e-12
+
+
+def test_refusals():
+    h, w, t = L.empty([6, 8], "float32", "meta"), L.empty([10, 8], "float32", "meta"), L.empty([6], "int64", "meta")
+
+    def call(h=h, w=w, t=t, **kw):
+        L.make_graph(lambda *xs: F.linear_cross_entropy(*xs, **kw))(h, w, t)
+
+    def shaped(*s, dtype="float32"):
+        return L.empty(list(s), dtype, "meta")
+
+    call()
+    for kw in (dict(w=shaped(10, 7)), dict(w=shaped(80)), dict(w=shaped(0, 8)), dict(h=shaped(6, 0), w=shaped(10, 0)), dict(t=shaped(5, dtype="int64")),
+               dict(t=shaped(6)), dict(t=shaped(6, 1, dtype="int64")), dict(reduction="max"), dict(reduction=None), dict(ignore_index=1.0),
+               dict(ignore_index=True), dict(ignore_index=1 << 40, t=shaped(6, dtype="int32"))):
+        with pytest.raises(ValueError, match="linear_cross_entropy"):
+            call(**kw)
+    with pytest.raises(TypeError):
+        call(w=shaped(10, 8, dtype="bfloat16"))
+    with pytest.raises(TypeError):
+        call(h=shaped(6, 8, dtype="int32"), w=shaped(10, 8, dtype="int32"))
+
+
+def _graph(fn, t=300, k=128, v=777, dtype="bfloat16", g=("float32", None)):
+    metas = [L.empty([t, k], dtype, "meta"), L.empty([v, k], dtype, "meta"), L.empty([t], "int32", "meta")]
+    return L.make_graph(fn)(*metas, *([L.empty([t] if g[1] is None else [], g[0], "meta")] if g else []))
+
+
+def test_plans():
+    """One step for both directions; two where the cotangent depends on the loss; the losses' own where there are no gradients."""
+    def kinds(graph):
+        return [st.nodes[0].params["name"] for st in Plan(graph, build_kernels=False).steps if st.kind == "head_loss"]
+
+    assert kinds(_graph(_program("none"))) == ["head_loss_backward"]
+    assert kinds(_graph(_program("mean"), g=("float32", 0))) == ["head_loss_backward"]
+
+    def forward(h, w, t):
+        return [F.linear_cross_entropy(h, w, t, reduction="none")]
+
+    assert kinds(_graph(forward, g=None)) == ["head_loss"]
+
+    def dependent(h, w, t):
+        loss, pull = L.vjp(lambda h, w: F.linear_cross_entropy(h, w, t), h, w)
+        return [loss, *pull(loss * 2.0)]
+
+    assert kinds(_graph(dependent, g=None)) == ["head_loss", "head_loss_backward"]
+
+    def two(h, w, t):  # two losses of other ignored values, each with its gradients
+        a, pa = L.vjp(lambda h, w: F.linear_cross_entropy(h, w, t, 1), h, w)
+        b, pb = L.vjp(lambda h, w: F.linear_cross_entropy(h, w, t, 2), h, w)
+        return [a, b, *pa(a * 0.0 + 1.0), *pb(a)]
+
+    assert kinds(_graph(two, g=None)) == ["head_loss", "head_loss_backward", "head_loss_backward"]
+    for dtype in ("float32", "float64"):
+        assert not kinds(_graph(_program("none"), dtype=dtype, g=(dtype, None)))
+    with L.config.compiler.patch(fused_operators=False):
+        assert not [n for n in _graph(_program("none")).nodes if n.prim == "fusion"]
+    assert not [n for n in _graph(_program("none"), k=1 << 12, v=1 << 18).nodes if n.prim == "fusion"]  # a weight of 2^31 bytes
+
+
+def test_the_joined_step_keeps_its_values():
+    """The graph with one step gives what the one with two gives, evaluated as primitives; values that depend on the loss, and on
+    both, come after it."""
+    rng = np.random.default_rng(4)
+    h, w, target = _case(rng, (9,), 64, 11, "float32")
+    bits = [np.asarray(a, np.float32) for a in (h, w)]
+    from lumen_amd import dtypes as D
+
+    def fn(h, w, t):
+        loss, pull = L.vjp(lambda h, w: F.linear_cross_entropy(h, w, t), h, w)
+        dh, dw = pull(F.sum(h.float()) * 0.0 + 1.0)
+        return [loss * 3.0, dh, dw.float() * loss]
+
+    graph = L.make_graph(fn)(_meta(h, "bfloat16"), _meta(w, "bfloat16"), _meta(target))
+    compiled, _ = compile_graph(graph)
+    args = [D.bf16_bits(b) for b in bits] + [target]
+    assert [n.params["name"] for n in compiled.nodes if n.prim == "fusion"] == ["head_loss_backward"]
+    for a, b in zip(oracle.values(graph, args), oracle.values(compiled, args)):
+        assert np.array_equal(a, b)
+
+
+def test_workspace_and_pieces():
+    """Memory of the gradients: codes of a piece, and of one piece no sums of the weight's gradient."""
+    def workspace(rows, piece, gradients=1):
+        n = C.c_size_t()
+        d = nv.HeadDesc(rows=rows, classes=32000, k=512, h_m=512, w_n=512, ignore_index=-100, piece_bytes=piece, dtype=1, target_dtype=0)
+        nv.call("nhip_head_loss_workspace", C.byref(d), gradients, C.byref(n))
+        return n.value
+
+    row, sums = 32000 * 2, 32000 * 512 * 4
+    assert workspace(8192, 1 << 30) >= 8192 * row
+    assert workspace(8192, 256 * row) < 8192 * row / 8 + 2 * sums
+    assert workspace(8192, 256 * row) > 256 * row + sums
+    assert workspace(8192, 1 << 30, 0) < 8192 * row / 8

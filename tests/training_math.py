@@ -97,4 +97,37 @@ def linear_cross_entropy(h, w, target, ignore, g):
     d = e / e.sum(1, keepdims=True)
     d[rows, at] -= 1
     d *= np.where(kept, g, 0.0)[:, None]
-    return losses, d @ w, d.T @ h
+    return losses, d @ w, d.T @ np.where(kept[:, None], h, 0.0)
+
+
+def linear_cross_entropy_tolerances(h, w, target, ignore, g, dtype):
+    """Of ``(losses, dh, dw)``. A logit is a float32 sum of K products; a probability is off by that of its logit and of the lse,
+    by the float32 sums and exponentials, by its 16 bits (2^-11) and by the rounding of the logits' gradient to ``dtype`` (float16's
+    in units of at least 2^-38 of the largest cotangent); both are summed over by the products."""
+    h, w, g = (np.asarray(x, np.float64) for x in (h, w, g))
+    kept = target != ignore
+    h = np.where(kept[:, None], h, 0.0)
+    logits = h @ w.T
+    size = (np.abs(h) @ np.abs(w).T).max(1) if h.shape[1] else np.zeros(len(h))
+    el = F32 * (h.shape[1] + 8) * size
+    top = logits.max(1, keepdims=True)
+    e = np.exp(logits - top)
+    p = e / e.sum(1, keepdims=True)
+    lse = top[:, 0] + np.log(e.sum(1))
+    spread = np.abs(logits - lse[:, None])
+    tloss = np.where(kept, 2 * el + F32 * (100 + 2 * np.abs(lse) + 2 * np.abs(top[:, 0])), 1e-30)
+    g = np.where(kept, g, 0.0)
+    rows = np.arange(len(h))
+    at = np.clip(np.where(kept, target, 0), 0, len(w) - 1)
+    d = p.copy()
+    d[rows, at] -= 1
+    d = np.abs(d * g[:, None])
+    u = U[dtype]
+    low = 2.0**-38 * np.abs(g).max(initial=0) if dtype == "float16" else 0.0
+    rel = 2.0**-11 + (2 * el + F32 * 100)[:, None] + 4 * F32 * spread
+    td = u * d + low + np.abs(g)[:, None] * (p * rel + 2.0**-62)
+    td[rows, at] += np.abs(g) * tloss
+    td[~kept] = 0.0
+    tdh = u * (d @ np.abs(w)) + LOW[dtype] + td @ np.abs(w) + F32 * (len(w) + 8) * (d @ np.abs(w))
+    tdw = u * (d.T @ np.abs(h)) + LOW[dtype] + td.T @ np.abs(h) + F32 * (len(h) + 8) * (d.T @ np.abs(h))
+    return tloss, tdh + 1e-30, tdw + 1e-30
