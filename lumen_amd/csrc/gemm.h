@@ -525,10 +525,10 @@ __device__ __forceinline__ int stream_line(int wn, int j) {
     else return wn * WCOLS + 32 * j;
 }
 
-// Whether an epilogue is called for every column of a tile's rows, those past n too (a reduction over lanes that a row's
-// last tile would leave without some of them).
+// Whether an epilogue takes a wave's sums where they are, in registers, by out.store(s, acc, rbase, cbase, lane): those of rows
+// and columns past the result's too.
 template <class Out>
-struct TakesWholeRows : std::false_type {};
+struct TakesSums : std::false_type {};
 
 // One workgroup's 256 x 256 output tile. `out` is AnyStore (a plain store of D), or a generated epilogue
 // functor called as out(row, col, float4, pre) with the float32 sums of four consecutive columns (col a
@@ -1011,6 +1011,10 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     // acc[i][j][e]: row m0 + wm*WR + 32 i + l32, column n0 + wn*WCOLS + 32 j + 8 (e / 4) + 4 h + e % 4.
     // Staged through LDS as float32, 64 rows of the wave at a time, then written row-wise.
     const int64_t rbase = m0 + wm * WR, cbase = n0 + wn * (TWO ? WCOLS / 2 : WCOLS);
+    if constexpr (TakesSums<Out>::value) {
+        out.template store<FM, FN>(s, acc, rbase, cbase, lane);
+        return;
+    } else {
     constexpr int PITCH = gemm_stream_stage_pitch<WN, TM>();
     __syncthreads();  // operand stages are dead: reuse LDS for the output
     char *stage = smem + wave * (64 * PITCH);
@@ -1044,7 +1048,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
                 for (int q = 0; q < G; ++q) {
                     const int idx = lane + 64 * (g0 + q);
                     const int64_t gr = rbase + 64 * half + idx / CPR, gc = cbase + 4 * (idx % CPR);
-                    if (gr < s.m && (TakesWholeRows<Out>::value || gc < s.n)) pre[q] = out.load(gr, gc);
+                    if (gr < s.m && gc < s.n) pre[q] = out.load(gr, gc);
                 }
             };
             fetch(0);
@@ -1058,7 +1062,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
                     const int idx = lane + 64 * (g0 + q);
                     const int r = idx / CPR, ch = idx % CPR;
                     const int64_t gr = rbase + 64 * half + r, gc = cbase + 4 * ch;
-                    if (gr < s.m && (TakesWholeRows<Out>::value || gc < s.n)) {
+                    if (gr < s.m && gc < s.n) {
                         if constexpr (Out::kColSum) {
                             const float4 c4 = out(gr, gc, *reinterpret_cast<const float4 *>(stage + r * PITCH + ch * 16), pre[q]);
                             colsum.x += c4.x;
@@ -1086,6 +1090,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
             const int64_t gc = cbase + 4 * lane;
             if (lane < CPR && gc < s.n && rbase < s.m) out.colsum_add(gc, colsum);
         }
+    }
     }
     }
 }

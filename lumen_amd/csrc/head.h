@@ -43,15 +43,17 @@ __device__ __forceinline__ float head_value(uint32_t code) {
     return code ? __int_as_float(int32_t(code << 13) + kHeadLeast) : 0.0f;
 }
 
-template <int CTRL>
-__device__ __forceinline__ float head_dpp(float x) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+// What the lanes of a row's two half-waves (lane, lane ^ 32) have, by a register swap.
+typedef unsigned head_u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ head_u32x2 head_halves(float x) {
+    return __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
 }
 
-// The store of the forward product: gemm_stream_tile hands a lane four consecutive columns of one row, and the 16 lanes of a
-// DPP row hold a block of 64: its maximum and the float32 sum of exp(l - maximum) combine across them by rotations, the block's
-// first lane stores both, every lane its four codes, and the lane with the target's column that logit. Columns past the classes
-// count for nothing and are stored as zeros up to whole blocks.
+// The store of the forward product, on a wave's sums in their registers: a lane and the one 32 further hold the 64 logits of a
+// row's block, 32 each, in groups of four columns that alternate between them. The block's maximum and sum are 31 operations of
+// a lane and one swap; the codes of two groups are swapped into 16 bytes of one row a lane. Columns past the classes
+// count for nothing and are stored as zeros up to whole blocks. (Through LDS, four columns of 16 rows a lane at a time and rotations over
+// 16 lanes for a row's block, the store took twice the product: [8192, 512] x [32000, 512] 1020 us.)
 template <bool GRAD>
 struct HeadOut {
     float2 *part;     // [rows, blocks]
@@ -59,54 +61,74 @@ struct HeadOut {
     uint16_t *codes;  // [rows, 64 blocks]
     HeadTargets targets;
     int64_t blocks;
-    static constexpr int kPrefetch = 8;
-    static constexpr bool kColSum = false;
-    struct Pre {
-        int64_t cls;
-    };
-    __device__ __forceinline__ Pre load(int64_t r, int64_t) const {
-        bool ignored;
-        return Pre{targets.at(r, ignored)};
-    }
-    __device__ __forceinline__ void operator()(int64_t r, int64_t c, float4 x, const Pre &pre) const {
-        const int64_t v = targets.classes;
-        if (c + 4 > v) {
-            if (c + 0 >= v) x.x = -INFINITY;
-            if (c + 1 >= v) x.y = -INFINITY;
-            if (c + 2 >= v) x.z = -INFINITY;
-            if (c + 3 >= v) x.w = -INFINITY;
-        }
-        // row_ror 8, row_ror 4, then the quad permutations [2,3,0,1] and [1,0,3,2]
-        float m = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
-        m = fmaxf(m, head_dpp<0x128>(m));
-        m = fmaxf(m, head_dpp<0x124>(m));
-        m = fmaxf(m, head_dpp<0x4e>(m));
-        m = fmaxf(m, head_dpp<0xb1>(m));
+
+    template <int FM, int FN>
+    __device__ __forceinline__ void store(const GemmShape &s, const f32x16_t (&acc)[FM][FN], int64_t rbase, int64_t cbase, int lane) const {
         constexpr float kLog2e = 1.4426950408889634f;
-        float4 e = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (m != -INFINITY) {
-            e.x = __builtin_amdgcn_exp2f((x.x - m) * kLog2e), e.y = __builtin_amdgcn_exp2f((x.y - m) * kLog2e);
-            e.z = __builtin_amdgcn_exp2f((x.z - m) * kLog2e), e.w = __builtin_amdgcn_exp2f((x.w - m) * kLog2e);
+        const int h = lane >> 5, l32 = lane & 31;
+        int64_t cls[FM];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const int64_t r = rbase + 32 * i + l32;
+            bool ignored;
+            cls[i] = r < s.m ? targets.at(r, ignored) : -1;
         }
-        float sum = (e.x + e.y) + (e.z + e.w);
-        sum += head_dpp<0x128>(sum);
-        sum += head_dpp<0x124>(sum);
-        sum += head_dpp<0x4e>(sum);
-        sum += head_dpp<0xb1>(sum);
-        const int64_t block = c >> 6;
-        if (block >= blocks) return;
-        if ((c & 63) == 0) part[r * blocks + block] = make_float2(m, sum);
-        if constexpr (GRAD)
-            *reinterpret_cast<uint2 *>(codes + r * blocks * 64 + c) =
-                make_uint2(head_code(e.x) | head_code(e.y) << 16, head_code(e.z) | head_code(e.w) << 16);
-        if (pre.cls >= c && pre.cls < c + 4) {
-            const int64_t q = pre.cls - c;
-            picked[r] = q == 0 ? x.x : q == 1 ? x.y : q == 2 ? x.z : x.w;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const int64_t r = rbase + 32 * i + l32;
+#pragma unroll
+            for (int b = 0; b < FN / 2; ++b) {
+                const int64_t c0 = cbase + 64 * b, block = c0 >> 6;
+                if (block >= blocks) continue;  // the whole wave
+                float x[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] = acc[i][2 * b + e / 16][e % 16];
+                // element e is column c0 + 32 (e / 16) + 8 (e / 4 % 4) + 4 h + e % 4
+                const int left = int(min(targets.classes - c0, int64_t(64))) - 4 * h;
+                if (c0 + 64 > targets.classes) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (32 * (e / 16) + 8 * (e / 4 % 4) + e % 4 >= left) x[e] = -INFINITY;
+                }
+                if (__any(cls[i] >= c0 && cls[i] < c0 + 64)) {
+                    const int at = int(cls[i] - c0) - 4 * h;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (at == 32 * (e / 16) + 8 * (e / 4 % 4) + e % 4) picked[r] = x[e];
+                }
+                float m = x[0];
+#pragma unroll
+                for (int e = 1; e < 32; ++e) m = fmaxf(m, x[e]);
+                const head_u32x2 both = head_halves(m);
+                m = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+                // the difference is exact near the maximum, where the terms matter, and no exponential is above 1
+                const float ref = m == -INFINITY ? 0.0f : m;
+                float sum = 0.0f;
+                uint32_t w[16];
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    const float p = __builtin_amdgcn_exp2f((x[e] - ref) * kLog2e), q = __builtin_amdgcn_exp2f((x[e + 1] - ref) * kLog2e);
+                    sum += p + q;
+                    if constexpr (GRAD) w[e / 2] = head_code(p) | head_code(q) << 16;
+                }
+                const head_u32x2 sums = head_halves(sum);
+                sum = __uint_as_float(sums[0]) + __uint_as_float(sums[1]);
+                if (r < s.m && h == 0) part[r * blocks + block] = make_float2(m, sum);
+                if constexpr (GRAD) {
+                    uint16_t *to = codes + r * blocks * 64 + c0 + 8 * h;
+#pragma unroll
+                    for (int g = 0; g < 8; g += 2) {  // groups of eight columns g (the lower half's) and g + 1 (the upper's)
+                        const head_u32x2 lo = __builtin_amdgcn_permlane32_swap(w[2 * g], w[2 * g + 2], false, false),
+                                         hi = __builtin_amdgcn_permlane32_swap(w[2 * g + 1], w[2 * g + 3], false, false);
+                        if (r < s.m) *reinterpret_cast<uint4 *>(to + 8 * g) = make_uint4(lo[0], hi[0], lo[1], hi[1]);
+                    }
+                }
+            }
         }
     }
 };
 template <bool GRAD>
-struct TakesWholeRows<HeadOut<GRAD>> : std::true_type {};
+struct TakesSums<HeadOut<GRAD>> : std::true_type {};
 
 template <bool F16, int TM, bool GRAD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TM == 256 ? 1 : 2, TM == 256 ? 1 : 2))) void head_logits_kernel(
@@ -115,8 +137,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TM == 256 ?
     gemm_stream_tile<F16, 64, 2, false, false, true, HeadOut<GRAD>, TM, TM == 256 ? 3 : 0>(s, a, b, out, smem);
 }
 
-// One wavefront a row: lse of its blocks' maxima and sums, and the loss.
-static __global__ __launch_bounds__(256) void head_merge_kernel(const float2 *__restrict__ part, const float *__restrict__ picked,
+// One wavefront a row: lse of its blocks' maxima and sums, and the loss (which with lse takes the logit's place).
+static __global__ __launch_bounds__(256) void head_merge_kernel(const float2 *__restrict__ part, float *__restrict__ picked,
                                                                 HeadTargets targets, int64_t rows, int64_t blocks,
                                                                 float *__restrict__ lse, float *__restrict__ losses) {
     const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
@@ -138,8 +160,9 @@ static __global__ __launch_bounds__(256) void head_merge_kernel(const float2 *__
         bool ignored;
         targets.at(row, ignored);
         const double l = double(m) + log(sum);
-        if (lse) lse[row] = float(l);
-        if (losses) losses[row] = ignored ? 0.0f : float(l - double(picked[row]));
+        const float loss = float(l - double(picked[row]));
+        if (lse) lse[row] = float(l), picked[row] = loss;
+        if (losses) losses[row] = ignored ? 0.0f : loss;
     }
 }
 
@@ -166,10 +189,10 @@ static __global__ __launch_bounds__(1024) void head_scale_kernel(const float *__
 }
 
 // The codes of a piece's rows into d, in place: a workgroup a row, 8 classes a thread at a time. The target's is
-// g expm1(l - lse), which p - 1 would cancel.
+// g expm1(-loss), which p - 1 would cancel.
 template <bool F16>
 __global__ __launch_bounds__(256) void head_grad_kernel(uint16_t *__restrict__ codes, const float2 *__restrict__ part,
-                                                        const float *__restrict__ picked, const float *__restrict__ lse,
+                                                        const float *__restrict__ loss, const float *__restrict__ lse,
                                                         const float *__restrict__ g, const float *__restrict__ scale, HeadTargets targets,
                                                         int64_t blocks) {
     const int64_t row = blockIdx.x;
@@ -189,7 +212,7 @@ __global__ __launch_bounds__(256) void head_grad_kernel(uint16_t *__restrict__ c
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[i] = round(head_value(w[i] & 0xffff) * k) | round(head_value(w[i] >> 16) * k) << 16;
             if (cls >= c && cls < c + 8) {
-                const uint32_t d = round(f * expm1f(picked[row] - l)), at = uint32_t(cls - c), shift = at % 2 * 16;
+                const uint32_t d = round(f * expm1f(-loss[row])), at = uint32_t(cls - c), shift = at % 2 * 16;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i)
                     if (at / 2 == i) o[i] = (o[i] & ~(0xffffu << shift)) | d << shift;
