@@ -525,8 +525,8 @@ __device__ __forceinline__ int stream_line(int wn, int j) {
     else return wn * WCOLS + 32 * j;
 }
 
-// Whether an epilogue takes a wave's sums where they are, in registers, by out.store(s, acc, rbase, cbase, lane): those of rows
-// and columns past the result's too.
+// Whether an epilogue takes a wave's sums where they are, in registers, by out.store(s, acc, stage, rbase, cbase, lane): those of
+// rows and columns past the result's too. stage: LDS of its own, Out::kStage bytes a wave.
 template <class Out>
 struct TakesSums : std::false_type {};
 
@@ -1012,7 +1012,8 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     // Staged through LDS as float32, 64 rows of the wave at a time, then written row-wise.
     const int64_t rbase = m0 + wm * WR, cbase = n0 + wn * (TWO ? WCOLS / 2 : WCOLS);
     if constexpr (TakesSums<Out>::value) {
-        out.template store<FM, FN>(s, acc, rbase, cbase, lane);
+        __syncthreads();  // operand stages are dead
+        out.template store<FM, FN>(s, acc, smem + wave * Out::kStage, rbase, cbase, lane);
         return;
     } else {
     constexpr int PITCH = gemm_stream_stage_pitch<WN, TM>();

@@ -8,8 +8,8 @@
 // one pass turns these into d in place once the row's lse is known. A piece's values are scratch that the next piece
 // writes over; the logits exist in registers alone.
 //
-// exp(l - m) is between 0 and 1 and needs no sign: 6 bits of exponent (from 2^-63, below which it is 0) and 10 of mantissa,
-// off by 2^-11 relative to the value at most, an eighth of what bf16's p is rounded by. d is then rounded once, to the operands'
+// exp(l - m), between 0 and 1, is kept as a float16 of 2^15 times it: off by 2^-11 relative to the value at most (an eighth of
+// what a bf16 p would be) down to 2^-29, by 2^-40 below. d is then rounded once, to the operands'
 // type, which the matrix instructions take; float16's d is taken times a power of two that puts the largest |g| at 2^13 to
 // 2^14, so that a mean's 1 / t does not push p out of its range (head_scale_kernel), and the products are divided by it again.
 // Sums are float32; over classes of a row first float32 in blocks of 64, then float64.
@@ -32,15 +32,13 @@ struct HeadTargets {
     }
 };
 
-constexpr int32_t kHeadLeast = 64 << 23;  // the float32 bits of 2^-63
+constexpr float kHeadUnit = 1.0f / 32768;  // of the codes
 
-// A value of [0, 1] as 16 bits, rounded to nearest, and back.
-__device__ __forceinline__ uint32_t head_code(float e) {
-    const int32_t bits = __float_as_int(e) - (kHeadLeast - 0x1000);
-    return uint32_t(bits < 0 ? 0 : bits) >> 13;
-}
-__device__ __forceinline__ float head_value(uint32_t code) {
-    return code ? __int_as_float(int32_t(code << 13) + kHeadLeast) : 0.0f;
+// Two values, rounded to nearest.
+__device__ __forceinline__ uint32_t head_codes(float a, float b) {
+    typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+    const half2 v = {_Float16(a), _Float16(b)};
+    return __builtin_bit_cast(uint32_t, v);
 }
 
 // What the lanes of a row's two half-waves (lane, lane ^ 32) have, by a register swap.
@@ -61,9 +59,10 @@ struct HeadOut {
     uint16_t *codes;  // [rows, 64 blocks]
     HeadTargets targets;
     int64_t blocks;
+    static constexpr int kPitch = 128 + 16, kStage = 32 * kPitch;  // a block of 32 rows
 
     template <int FM, int FN>
-    __device__ __forceinline__ void store(const GemmShape &s, const f32x16_t (&acc)[FM][FN], int64_t rbase, int64_t cbase, int lane) const {
+    __device__ __forceinline__ void store(const GemmShape &s, const f32x16_t (&acc)[FM][FN], char *stage, int64_t rbase, int64_t cbase, int lane) const {
         constexpr float kLog2e = 1.4426950408889634f;
         const int h = lane >> 5, l32 = lane & 31;
         int64_t cls[FM];
@@ -107,20 +106,28 @@ struct HeadOut {
                 uint32_t w[16];
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
-                    const float p = __builtin_amdgcn_exp2f((x[e] - ref) * kLog2e), q = __builtin_amdgcn_exp2f((x[e + 1] - ref) * kLog2e);
+                    const float p = __builtin_amdgcn_exp2f(fmaf(x[e] - ref, kLog2e, 15.0f)),
+                                q = __builtin_amdgcn_exp2f(fmaf(x[e + 1] - ref, kLog2e, 15.0f));
                     sum += p + q;
-                    if constexpr (GRAD) w[e / 2] = head_code(p) | head_code(q) << 16;
+                    if constexpr (GRAD) w[e / 2] = head_codes(p, q);
                 }
                 const head_u32x2 sums = head_halves(sum);
-                sum = __uint_as_float(sums[0]) + __uint_as_float(sums[1]);
+                sum = (__uint_as_float(sums[0]) + __uint_as_float(sums[1])) * kHeadUnit;
                 if (r < s.m && h == 0) part[r * blocks + block] = make_float2(m, sum);
                 if constexpr (GRAD) {
-                    uint16_t *to = codes + r * blocks * 64 + c0 + 8 * h;
 #pragma unroll
                     for (int g = 0; g < 8; g += 2) {  // groups of eight columns g (the lower half's) and g + 1 (the upper's)
                         const head_u32x2 lo = __builtin_amdgcn_permlane32_swap(w[2 * g], w[2 * g + 2], false, false),
                                          hi = __builtin_amdgcn_permlane32_swap(w[2 * g + 1], w[2 * g + 3], false, false);
-                        if (r < s.m) *reinterpret_cast<uint4 *>(to + 8 * g) = make_uint4(lo[0], hi[0], lo[1], hi[1]);
+                        *reinterpret_cast<uint4 *>(stage + l32 * kPitch + 16 * (g + h)) = make_uint4(lo[0], hi[0], lo[1], hi[1]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int row = 8 * k + lane / 8, chunk = lane % 8;
+                        typedef unsigned head_u32x4 __attribute__((ext_vector_type(4)));
+                        const head_u32x4 v = *reinterpret_cast<const head_u32x4 *>(stage + row * kPitch + 16 * chunk);
+                        const int64_t to = rbase + 32 * i + row;
+                        if (to < s.m) __builtin_nontemporal_store(v, reinterpret_cast<head_u32x4 *>(codes + to * blocks * 64 + c0 + 8 * chunk));
                     }
                 }
             }
@@ -131,38 +138,45 @@ template <bool GRAD>
 struct TakesSums<HeadOut<GRAD>> : std::true_type {};
 
 template <bool F16, int TM, bool GRAD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(TM == 256 ? 1 : 2, TM == 256 ? 1 : 2))) void head_logits_kernel(
+__global__ __launch_bounds__(TM * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void head_logits_kernel(
     GemmShape s, const uint16_t *__restrict__ a, const uint16_t *__restrict__ b, HeadOut<GRAD> out) {
     extern __shared__ __align__(1024) char smem[];
-    gemm_stream_tile<F16, 64, 2, false, false, true, HeadOut<GRAD>, TM, TM == 256 ? 3 : 0>(s, a, b, out, smem);
+    gemm_stream_tile<F16, 64, TM / 64, false, false, true, HeadOut<GRAD>, TM, TM == 256 ? 3 : 0>(s, a, b, out, smem);
 }
 
-// One wavefront a row: lse of its blocks' maxima and sums, and the loss (which with lse takes the logit's place).
-static __global__ __launch_bounds__(256) void head_merge_kernel(const float2 *__restrict__ part, float *__restrict__ picked,
-                                                                HeadTargets targets, int64_t rows, int64_t blocks,
-                                                                float *__restrict__ lse, float *__restrict__ losses) {
-    const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (row >= rows) return;  // the whole wavefront
-    const float2 *p = part + row * blocks;
-    float m = -INFINITY;
-    for (int64_t j = lane; j < blocks; j += 64) m = fmaxf(m, p[j].x);
+// exp(x) of a block's or a wave's maximum less a larger one.
+__device__ __forceinline__ float head_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+
+// The maximum of a row's block maxima and the float64 sum of exp(l - maximum) over lanes that take a block each `step`: every
+// lane of the wavefront has both.
+__device__ __forceinline__ void head_row(const float2 *__restrict__ p, int64_t first, int64_t step, int64_t blocks, float &m, double &sum) {
+    m = -INFINITY;
+    for (int64_t j = first; j < blocks; j += step) m = fmaxf(m, p[j].x);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    double sum = 0.0;
-    for (int64_t j = lane; j < blocks; j += 64) {
+    sum = 0.0;
+    for (int64_t j = first; j < blocks; j += step) {
         const float2 q = p[j];
-        if (q.x != -INFINITY) sum += double(q.y) * double(__builtin_amdgcn_exp2f((q.x - m) * 1.4426950408889634f));
+        if (q.x != -INFINITY) sum += double(q.y) * double(head_exp(q.x - m));
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+}
+
+// The losses alone: one wavefront a row.
+static __global__ __launch_bounds__(256) void head_merge_kernel(const float2 *__restrict__ part, const float *__restrict__ picked,
+                                                                HeadTargets targets, int64_t rows, int64_t blocks,
+                                                                float *__restrict__ losses) {
+    const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= rows) return;  // the whole wavefront
+    float m;
+    double sum;
+    head_row(part + row * blocks, lane, 64, blocks, m, sum);
     if (lane == 0) {
         bool ignored;
         targets.at(row, ignored);
-        const double l = double(m) + log(sum);
-        const float loss = float(l - double(picked[row]));
-        if (lse) lse[row] = float(l), picked[row] = loss;
-        if (losses) losses[row] = ignored ? 0.0f : loss;
+        losses[row] = ignored ? 0.0f : float(double(m) + log(sum) - double(picked[row]));
     }
 }
 
@@ -188,38 +202,53 @@ static __global__ __launch_bounds__(1024) void head_scale_kernel(const float *__
     scale[0] = ldexpf(1.0f, power), scale[1] = ldexpf(1.0f, -power);
 }
 
-// The codes of a piece's rows into d, in place: a workgroup a row, 8 classes a thread at a time. The target's is
-// g expm1(-loss), which p - 1 would cancel.
+// The codes of a piece's rows into d, in place: a workgroup a row, whose lse and loss it works out first, 8 classes a thread at a
+// time. The target's d is g expm1(-loss), which p - 1 would cancel. HBM bounds it; codes are read and d written once and are more
+// than the caches hold (nontemporal).
 template <bool F16>
 __global__ __launch_bounds__(256) void head_grad_kernel(uint16_t *__restrict__ codes, const float2 *__restrict__ part,
-                                                        const float *__restrict__ loss, const float *__restrict__ lse,
-                                                        const float *__restrict__ g, const float *__restrict__ scale, HeadTargets targets,
-                                                        int64_t blocks) {
+                                                        const float *__restrict__ picked, const float *__restrict__ g,
+                                                        const float *__restrict__ scale, HeadTargets targets, int64_t blocks,
+                                                        float *__restrict__ losses) {
+    typedef uint32_t words4 __attribute__((ext_vector_type(4)));
+    __shared__ float most[4];
+    __shared__ double sums[4];
     const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const float2 *q = part + row * blocks;
+    float m;
+    double sum;
+    head_row(q, threadIdx.x, 256, blocks, m, sum);
+    if (lane == 0) most[wave] = m, sums[wave] = sum;
+    __syncthreads();
+    const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (most[i] != -INFINITY) sum += sums[i] * double(head_exp(most[i] - top));
+    const double lse = double(top) + log(sum);
     bool ignored;
     const int64_t cls = targets.at(row, ignored);
-    const float l = lse[row], f = F16 ? g[row] * scale[0] : g[row];
+    const float l = float(lse), loss = float(lse - double(picked[row])), f = F16 ? g[row] * scale[0] : g[row];
+    if (losses && threadIdx.x == 0) losses[row] = ignored ? 0.0f : loss;
     uint16_t *p = codes + row * blocks * 64;
-    const float2 *q = part + row * blocks;
     auto round = [](float v) { return uint32_t(F16 ? f32_to_f16(v) : f32_to_bf16(v)); };
     for (int64_t c = 8 * threadIdx.x; c < blocks * 64; c += 2048) {
-        uint4 out = make_uint4(0, 0, 0, 0);
+        words4 o = {0, 0, 0, 0};
         if (!ignored) {
-            const uint4 in = *reinterpret_cast<const uint4 *>(p + c);
-            const float k = f * __builtin_amdgcn_exp2f((q[c >> 6].x - l) * 1.4426950408889634f);
-            const uint32_t w[4] = {in.x, in.y, in.z, in.w};
-            uint32_t o[4];
+            const words4 w = __builtin_nontemporal_load(reinterpret_cast<const words4 *>(p + c));
+            const float k = f * kHeadUnit * head_exp(q[c >> 6].x - l);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = round(head_value(w[i] & 0xffff) * k) | round(head_value(w[i] >> 16) * k) << 16;
+            for (int i = 0; i < 4; ++i)
+                o[i] = round(f16_to_f32(uint16_t(w[i] & 0xffff)) * k) | round(f16_to_f32(uint16_t(w[i] >> 16)) * k) << 16;
             if (cls >= c && cls < c + 8) {
-                const uint32_t d = round(f * expm1f(-loss[row])), at = uint32_t(cls - c), shift = at % 2 * 16;
+                const uint32_t d = round(f * expm1f(-loss)), at = uint32_t(cls - c), shift = at % 2 * 16;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i)
                     if (at / 2 == i) o[i] = (o[i] & ~(0xffffu << shift)) | d << shift;
             }
-            out = make_uint4(o[0], o[1], o[2], o[3]);
         }
-        *reinterpret_cast<uint4 *>(p + c) = out;
+        __builtin_nontemporal_store(o, reinterpret_cast<words4 *>(p + c));
     }
 }
 

@@ -47,7 +47,7 @@ PartPlan weight_plan(const nhip_head_desc *d) {
 bool copies(const nhip_head_desc *d, int64_t ld) { return d->k % 64 != 0 || ld % 8 != 0; }
 
 struct HeadSpace {
-    size_t h, w, part, picked, lse, scale, codes, weight_sums, input_parts, weight_parts, bytes;
+    size_t h, w, part, picked, scale, codes, weight_sums, input_parts, weight_parts, bytes;
 };
 HeadSpace head_space(const nhip_head_desc *d, bool grad) {
     HeadSpace s{};
@@ -62,7 +62,6 @@ HeadSpace head_space(const nhip_head_desc *d, bool grad) {
     s.w = take(copies(d, d->w_n) ? size_t(d->classes) * kp * 2 : 0);
     s.part = take(size_t(rows) * blocks_of(d) * sizeof(float2));
     s.picked = take(size_t(rows) * 4);
-    s.lse = take(size_t(rows) * 4);
     s.scale = take(8);
     if (grad) {
         const PartPlan pi = input_plan(d), pw = weight_plan(d);
@@ -94,12 +93,12 @@ int head_check(const nhip_head_desc *d, const char *what) {
     return 0;
 }
 
-template <class... P>
+template <int THREADS = 256, class... P>
 int launch(hipStream_t st, void (*kern)(P...), dim3 grid, int lds, const char *what, std::common_type_t<P>... args) {
     if (check(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds),
               "hipFuncSetAttribute"))
         return 1;
-    hipLaunchKernelGGL(kern, grid, dim3(256), lds, st, args...);
+    hipLaunchKernelGGL(kern, grid, dim3(THREADS), lds, st, args...);
     return check(hipGetLastError(), what);
 }
 
@@ -122,7 +121,7 @@ int logits(hipStream_t st, const nhip_head_desc *d, int64_t rows, const uint16_t
     GemmShape s = shape(rows, d->classes, padded_k(d), tm);
     s.a_m = h_m, s.a_k = 1, s.b_k = 1, s.b_n = w_n;
     const dim3 grid(unsigned(s.tiles_m) * unsigned(s.tiles_n));
-    if (tm == 256) return launch(st, head_logits_kernel<F16, 256, GRAD>, grid, kLds256, "head_logits_kernel launch", s, h, w, out);
+    if (tm == 256) return launch<512>(st, head_logits_kernel<F16, 256, GRAD>, grid, gemm_stream_lds_bytes<64, 4>(), "head_logits_kernel launch", s, h, w, out);
     return launch(st, head_logits_kernel<F16, 128, GRAD>, grid, kLds128, "head_logits_kernel launch", s, h, w, out);
 }
 
@@ -195,15 +194,15 @@ int head_run(hipStream_t st, const nhip_head_desc *d, const uint16_t *h, const u
         w = to, w_n = kp;
     }
     float2 *part = reinterpret_cast<float2 *>(ws + at.part);
-    float *picked = reinterpret_cast<float *>(ws + at.picked), *lse = reinterpret_cast<float *>(ws + at.lse);
+    float *picked = reinterpret_cast<float *>(ws + at.picked);
     float *scale = reinterpret_cast<float *>(ws + at.scale);
     uint16_t *codes = reinterpret_cast<uint16_t *>(ws + at.codes);
-    auto merge = [&](int64_t r0, int64_t rows) {
-        hipLaunchKernelGGL(head_merge_kernel, dim3(unsigned((rows + 3) / 4)), dim3(256), 0, st, part, picked, targets, rows, blocks,
-                           grad ? lse : nullptr, losses ? losses + r0 : nullptr);
+    if (!grad) {
+        if (!losses) return 0;
+        if (logits<F16, false>(st, d, d->rows, h, h_m, w, w_n, HeadOut<false>{part, picked, nullptr, targets, blocks})) return 1;
+        hipLaunchKernelGGL(head_merge_kernel, dim3(unsigned((d->rows + 3) / 4)), dim3(256), 0, st, part, picked, targets, d->rows, blocks, losses);
         return check(hipGetLastError(), "head_merge_kernel launch");
-    };
-    if (!grad) return logits<F16, false>(st, d, d->rows, h, h_m, w, w_n, HeadOut<false>{part, picked, nullptr, targets, blocks}) || merge(0, d->rows);
+    }
     if (F16) {
         hipLaunchKernelGGL(head_scale_kernel, dim3(1), dim3(1024), 0, st, g, d->rows, scale);
         if (check(hipGetLastError(), "head_scale_kernel launch")) return 1;
@@ -216,9 +215,9 @@ int head_run(hipStream_t st, const nhip_head_desc *d, const uint16_t *h, const u
         const int64_t rows = std::min(most, d->rows - r0);
         const uint16_t *hp = h + r0 * h_m;
         targets.target = static_cast<const char *>(target) + r0 * tsize;
-        if (logits<F16, true>(st, d, rows, hp, h_m, w, w_n, HeadOut<true>{part, picked, codes, targets, blocks}) || merge(r0, rows)) return 1;
-        hipLaunchKernelGGL((head_grad_kernel<F16>), dim3(unsigned(rows)), dim3(256), 0, st, codes, part, picked, lse, g + r0, scale, targets,
-                           blocks);
+        if (logits<F16, true>(st, d, rows, hp, h_m, w, w_n, HeadOut<true>{part, picked, codes, targets, blocks})) return 1;
+        hipLaunchKernelGGL((head_grad_kernel<F16>), dim3(unsigned(rows)), dim3(256), 0, st, codes, part, picked, g + r0, scale, targets, blocks,
+                           losses ? losses + r0 : nullptr);
         if (check(hipGetLastError(), "head_grad_kernel launch")) return 1;
         // a last piece of fewer rows keeps its plan: its sums are shorter, its tiles fewer
         if (dh && input_grad<F16>(st, d, pi, rows, codes, w, w_n, parts, HeadStore{nullptr, nullptr, dh + r0 * d->k, inverse, d->k, F16}))

@@ -102,7 +102,7 @@ def linear_cross_entropy(h, w, target, ignore, g):
 
 def linear_cross_entropy_tolerances(h, w, target, ignore, g, dtype):
     """Of ``(losses, dh, dw)``. A logit is a float32 sum of K products; a probability is off by that of its logit and of the lse,
-    by the float32 sums and exponentials, by its 16 bits (2^-11) and by the rounding of the logits' gradient to ``dtype`` (float16's
+    by the float32 sums and exponentials, by its 16 bits (2^-11, or 2^-40 of its block's largest) and by the rounding of the logits' gradient to ``dtype`` (float16's
     in units of at least 2^-38 of the largest cotangent); both are summed over by the products."""
     h, w, g = (np.asarray(x, np.float64) for x in (h, w, g))
     kept = target != ignore
@@ -125,7 +125,7 @@ def linear_cross_entropy_tolerances(h, w, target, ignore, g, dtype):
     u = U[dtype]
     low = 2.0**-38 * np.abs(g).max(initial=0) if dtype == "float16" else 0.0
     rel = 2.0**-11 + (2 * el + F32 * 100)[:, None] + 4 * F32 * spread
-    td = u * d + low + np.abs(g)[:, None] * (p * rel + 2.0**-62)
+    td = u * d + low + np.abs(g)[:, None] * (p * rel + 2.0**-39)
     td[rows, at] += np.abs(g) * tloss
     td[~kept] = 0.0
     tdh = u * (d @ np.abs(w)) + LOW[dtype] + td @ np.abs(w) + F32 * (len(w) + 8) * (d @ np.abs(w))
