@@ -10,8 +10,9 @@
 //
 // exp(l - m), between 0 and 1, is kept as a float16 of 2^15 times it: off by 2^-11 relative to the value at most (an eighth of
 // what a bf16 p would be) down to 2^-29, by 2^-40 below. d is then rounded once, to the operands'
-// type, which the matrix instructions take; float16's d is taken times a power of two that puts the largest |g| at 2^13 to
-// 2^14, so that a mean's 1 / t does not push p out of its range (head_scale_kernel), and the products are divided by it again.
+// type, which the matrix instructions take, with the largest |g| taken to 1 (bf16: a mean's 1 / t would be rounded the
+// same way in every row whose p is near 0, a gradient 2^-9 too long) or 2^14 (float16, whose range a mean's p would leave), and
+// the products are multiplied by what it was (head_scale_kernel).
 // Sums are float32; over classes of a row first float32 in blocks of 64, then float64.
 #pragma once
 
@@ -180,26 +181,26 @@ static __global__ __launch_bounds__(256) void head_merge_kernel(const float2 *__
     }
 }
 
-// scale[0]: the power of two that takes the largest |g| to [2^13, 2^14) (1 where g is all zeros or not finite); scale[1]: one
-// over it.
-static __global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restrict__ g, int64_t rows, float *__restrict__ scale) {
+// scale[0]: what takes the largest |g| to `top` (1 where g is all zeros or not finite); scale[1]: one over it.
+static __global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restrict__ g, int64_t rows, float top, float *__restrict__ scale) {
     __shared__ float most[16];
     float m = 0.0f;
-    for (int64_t i = threadIdx.x; i < rows; i += 1024) m = fmaxf(m, fabsf(g[i]));
+    for (int64_t i = threadIdx.x; i < rows; i += 4096) {
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = i + 1024 * k < rows ? g[i + 1024 * k] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m = fmaxf(m, fabsf(v[k]));
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
     __syncthreads();
     if (threadIdx.x) return;
     for (int i = 1; i < 16; ++i) m = fmaxf(m, most[i]);
-    int power = 0;
-    if (m > 0.0f && m < INFINITY) {
-        int e;
-        frexpf(m, &e);  // m in [2^(e - 1), 2^e)
-        power = 14 - e;
-        power = power < -100 ? -100 : power > 100 ? 100 : power;
-    }
-    scale[0] = ldexpf(1.0f, power), scale[1] = ldexpf(1.0f, -power);
+    // within what a float32 and its inverse can be
+    m = m > 0.0f && m < INFINITY ? fminf(fmaxf(m, 0x1p-100f), 0x1p100f) : top;
+    scale[0] = top / m, scale[1] = m / top;
 }
 
 // The codes of a piece's rows into d, in place: a workgroup a row, whose lse and loss it works out first, 8 classes a thread at a
@@ -229,7 +230,7 @@ __global__ __launch_bounds__(256) void head_grad_kernel(uint16_t *__restrict__ c
     const double lse = double(top) + log(sum);
     bool ignored;
     const int64_t cls = targets.at(row, ignored);
-    const float l = float(lse), loss = float(lse - double(picked[row])), f = F16 ? g[row] * scale[0] : g[row];
+    const float l = float(lse), loss = float(lse - double(picked[row])), f = g[row] * scale[0];
     if (losses && threadIdx.x == 0) losses[row] = ignored ? 0.0f : loss;
     uint16_t *p = codes + row * blocks * 64;
     auto round = [](float v) { return uint32_t(F16 ? f32_to_f16(v) : f32_to_bf16(v)); };
@@ -257,7 +258,7 @@ struct HeadStore {
     const float *before;  // null: none
     float *sums;          // null: this is the last piece
     uint16_t *out;
-    const float *inverse;  // what the products are multiplied by, or null
+    const float *inverse;  // what the products are multiplied by
     int64_t n;             // columns, a row's elements too
     int32_t f16;
     static constexpr int kPrefetch = 8;
@@ -285,7 +286,7 @@ struct HeadStore {
                     if (c + i < n) p[i] = e[i];
             return;
         }
-        const float k = inverse ? *inverse : 1.0f;
+        const float k = *inverse;
         uint16_t *p = out + r * n + c;
         uint32_t b[4];
 #pragma unroll

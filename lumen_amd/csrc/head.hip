@@ -203,14 +203,12 @@ int head_run(hipStream_t st, const nhip_head_desc *d, const uint16_t *h, const u
         hipLaunchKernelGGL(head_merge_kernel, dim3(unsigned((d->rows + 3) / 4)), dim3(256), 0, st, part, picked, targets, d->rows, blocks, losses);
         return check(hipGetLastError(), "head_merge_kernel launch");
     }
-    if (F16) {
-        hipLaunchKernelGGL(head_scale_kernel, dim3(1), dim3(1024), 0, st, g, d->rows, scale);
-        if (check(hipGetLastError(), "head_scale_kernel launch")) return 1;
-    }
+    hipLaunchKernelGGL(head_scale_kernel, dim3(1), dim3(1024), 0, st, g, d->rows, F16 ? 16384.0f : 1.0f, scale);
+    if (check(hipGetLastError(), "head_scale_kernel launch")) return 1;
     const PartPlan pi = input_plan(d), pw = weight_plan(d);
     const int64_t most = piece_rows(d), pieces = pieces_of(d);
     float *sums = reinterpret_cast<float *>(ws + at.weight_sums), *parts = reinterpret_cast<float *>(ws + at.input_parts);
-    const float *inverse = F16 ? scale + 1 : nullptr;
+    const float *inverse = scale + 1;
     for (int64_t i = 0, r0 = 0; i < pieces; ++i, r0 += most) {
         const int64_t rows = std::min(most, d->rows - r0);
         const uint16_t *hp = h + r0 * h_m;
