@@ -488,10 +488,13 @@ template <bool CAUSAL, bool ATOMIC_DQ> struct DkdvPaired { static constexpr bool
 // STORE_DS (the deterministic mode's default): each tile's dS (rounded as for dK) is stored to p.ds for the
 // dQ = dS K kernel, instead of a second kernel recomputing S and dP.
 // Key block pidx (PAIR: and nkb - 1 - pidx) of nkb of key head nkv of batch b; a head's statistics are `ls` floats after the
-// last one's.
-template <int D, bool F16, bool CAUSAL, bool ATOMIC_DQ, bool STORE_DS, bool PAIR>
+// last one's. PARTS: part `part` of `parts` of the query tiles, its float32 sums to `sums` instead of dk and dv: a key's hd of dK,
+// then its hdv of dV, keys sums_s floats apart.
+template <int D, bool F16, bool CAUSAL, bool ATOMIC_DQ, bool STORE_DS, bool PAIR, bool PARTS = false>
 __device__ __forceinline__ void flash_dkdv_tile(const AttnParams &p, const float *lse2, int64_t b, int64_t nkv, int64_t pidx,
-                                                int64_t nkb, int64_t ls) {
+                                                int64_t nkb, int64_t ls, int part = 0, int parts = 1, float *sums = nullptr,
+                                                int64_t sums_s = 0) {
+    static_assert(!PARTS || (!PAIR && !ATOMIC_DQ), "parts of one key block, without atomics");
     constexpr int BM = 64;
     constexpr int DS = D / 16, DT = D / 32;
     constexpr int TILE = BM * D;
@@ -531,7 +534,8 @@ __device__ __forceinline__ void flash_dkdv_tile(const AttnParams &p, const float
     int64_t qstart = 0;
     if (CAUSAL) qstart = max<int64_t>(0, kb0 - shift) / BM * BM;
     const int per_head = p.sq > qstart ? int((p.sq - qstart + BM - 1) / BM) : 0;
-    const int total = per_head * int(group);
+    const int tiles = per_head * int(group);
+    const int begin = PARTS ? int(int64_t(tiles) * part / parts) : 0, total = PARTS ? int(int64_t(tiles) * (part + 1) / parts) : tiles;
     auto tile_src = [&](int j, const uint16_t *&qp, const uint16_t *&gp, const float *&lp, const float *&dl,
                         int64_t &q0) {
         const int64_t gi = j / per_head;
@@ -556,7 +560,7 @@ __device__ __forceinline__ void flash_dkdv_tile(const AttnParams &p, const float
         load_tile_async<D>(kp, p.k_s, kb0, p.sk, Ks, wave, lane, p.hd);
         load_tile_async<D>(kp, p.k_s, kb0 + 64, p.sk, Ks + 64 * D, wave, lane, p.hd);
     }
-    if (total > 0) issue(0, stage0, Ls0, Dl0);
+    if (total > begin) issue(begin, stage0, Ls0, Dl0);
 
     // ATOMIC_DQ: this wave's dQ share of the previous tile, waiting to be added: NQ accumulators of 32 queries
     // x 32 head-dim columns (query half qh0 + c, columns 32 * dblk ...)
@@ -605,7 +609,7 @@ __device__ __forceinline__ void flash_dkdv_tile(const AttnParams &p, const float
         }
         // this thread's loads of tile j have landed; with STORE_DS the previous tile's 4 dS stores, issued after
         // them, may stay in flight (vector memory operations complete in order: vmcnt <= 4)
-        if (STORE_DS && j > 0) __builtin_amdgcn_s_waitcnt(4 | (7 << 4));
+        if (STORE_DS && j > begin) __builtin_amdgcn_s_waitcnt(4 | (7 << 4));
         else __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         flush_dq();  // the previous tile's dQ adds, ahead of this iteration's loads
@@ -825,12 +829,28 @@ __device__ __forceinline__ void flash_dkdv_tile(const AttnParams &p, const float
             }
         }
     };
-    for (int j = 0; j < total; j += 2) {
+    for (int j = begin; j < total; j += 2) {
         tile(j, stage0, Ls0, Dl0, stage1, Ls1, Dl1);
         if (j + 1 < total) tile(j + 1, stage1, Ls1, Dl1, stage0, Ls0, Dl0);
     }
     if constexpr (ATOMIC_DQ) flush_dq();
     if (!kvalid) return;
+    if constexpr (PARTS) {
+        float *to = sums + kj * sums_s;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e4 = 0; e4 < 4; ++e4) {
+                const int d = 32 * dt + 8 * e4 + 4 * h;
+                if (32 * dt + 8 * e4 < p.hd)
+                    *reinterpret_cast<float4 *>(to + d) =
+                        make_float4(adk[dt][4 * e4], adk[dt][4 * e4 + 1], adk[dt][4 * e4 + 2], adk[dt][4 * e4 + 3]);
+                if (32 * dt + 8 * e4 < p.hdv)
+                    *reinterpret_cast<float4 *>(to + p.hd + d) =
+                        make_float4(adv[dt][4 * e4], adv[dt][4 * e4 + 1], adv[dt][4 * e4 + 2], adv[dt][4 * e4 + 3]);
+            }
+        return;
+    }
     uint16_t *dkp = p.dk + b * p.dk_b + nkv * p.dk_n + kj * p.dk_s;
     uint16_t *dvp = p.dv + b * p.dv_b + nkv * p.dv_n + kj * p.dv_s;
 #pragma unroll

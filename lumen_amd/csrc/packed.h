@@ -33,7 +33,7 @@ struct PackedTables {
     int64_t sequences, tokens;
     int32_t o64;
     int64_t ds_tiles;    // dS tiles of one head that there is room for
-    int32_t *fits;       // whether all of them do (null: nobody asks)
+    int32_t *fits;       // whether all of them do (null: nobody asks), and the first and the last sequence's end
 };
 
 constexpr int kPackedBuckets = 1024;  // also the builder's threads
@@ -55,6 +55,16 @@ __device__ __forceinline__ T packed_wave_sum(T v, int lane) {
         if (lane >= o) v += u;
     }
     return v;
+}
+
+// The entries behind the `placed` tiles: tokens of no sequence, then nothing.
+__device__ __forceinline__ void packed_rest(const PackedTable &t, int placed, int first, int last, int tokens) {
+    const int lead = (first + t.block - 1) / t.block, tail = (tokens - last + t.block - 1) / t.block;
+    for (int i = placed + threadIdx.x; i < t.most; i += blockDim.x) {
+        int j = i - placed, from = j * t.block, to = first;
+        if (j >= lead) from = last + (j - lead) * t.block, to = j < lead + tail ? tokens : from;
+        t.tiles[i] = PackedTile{from < tokens ? from : 0, min(max(to - from, 0), t.block), -1, 0};
+    }
 }
 
 // One workgroup a table. Offsets are clamped into [the one before, tokens], so that whatever they hold every tile lies within
@@ -128,7 +138,7 @@ static __global__ __launch_bounds__(kPackedBuckets) void packed_tiles_kernel(Pac
         last = max(first, carry);
         __syncthreads();
         if (pass == 1) break;
-        if (a.fits && tid == 0 && blockIdx.x == 0) *a.fits = ds_carry <= a.ds_tiles;
+        if (a.fits && tid == 0 && blockIdx.x == 0) a.fits[0] = ds_carry <= a.ds_tiles, a.fits[1] = first, a.fits[2] = last;
         // counts to places
         const int count = bucket[tid], sum = packed_wave_sum(count, lane);
         if (lane == 63) waves[wave] = sum;
@@ -137,14 +147,72 @@ static __global__ __launch_bounds__(kPackedBuckets) void packed_tiles_kernel(Pac
         for (int w = 0; w < wave; ++w) place += waves[w];
         bucket[tid] = place;
     }
-    // tokens of no sequence, then nothing
-    const int placed = bucket[kPackedBuckets - 1];  // where the last amount's tiles end
-    const int lead = (first + t.block - 1) / t.block, tail = (tokens - last + t.block - 1) / t.block;
-    for (int i = placed + tid; i < t.most; i += kPackedBuckets) {
-        int j = i - placed, from = j * t.block, to = first;
-        if (j >= lead) from = last + (j - lead) * t.block, to = j < lead + tail ? tokens : from;
-        t.tiles[i] = PackedTile{from < tokens ? from : 0, min(max(to - from, 0), t.block), -1, 0};
+    packed_rest(t, bucket[kPackedBuckets - 1], first, last, tokens);  // where the last amount's tiles end
+}
+
+// The same for fewer sequences than threads, without atomics: a tile's place is the tiles of more work, which are those of every
+// sequence's blocks past its own work, and the sequences before its own that have as many blocks (3 sequences of 97 tokens: 3.2 us,
+// 8.7 by amounts; 8 of 16384: 5.0, 11.5 by
+// amounts).
+constexpr int kPackedFew = 256;
+static __global__ __launch_bounds__(kPackedFew) void packed_tiles_few_kernel(PackedTables a) {
+    __shared__ int at[kPackedFew + 1], before[kPackedFew + 1], ds_at[kPackedFew];
+    __shared__ __align__(16) int blocks[kPackedFew];
+    __shared__ int waves[3][4];
+    const PackedTable t = a.t[blockIdx.x];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, tokens = int(a.tokens), count = int(a.sequences);
+    int v = 0;
+    if (tid <= count) {
+        const int64_t x = a.o64 ? static_cast<const int64_t *>(a.offsets)[tid] : static_cast<const int32_t *>(a.offsets)[tid];
+        v = int(x < 0 ? 0 : x > tokens ? tokens : x);
     }
+    v = packed_wave_max(v, lane);
+    if (lane == 63) waves[0][wave] = v;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) v = max(v, waves[0][w]);
+    at[tid] = v;
+    __syncthreads();
+    const int len = tid < count ? at[tid + 1] - v : 0, own = (len + t.block - 1) / t.block;
+    // dS tiles of sequences that do not fit may be past 32 bits; their sum over a wavefront's is capped ahead of that
+    const long long tiles = (long long)((len + 127) / 128) * ((len + 63) / 64);
+    const int ds_own = int(min(tiles, (long long)(1 << 24)));
+    const int sum = packed_wave_sum(own, lane), ds = packed_wave_sum(ds_own, lane);
+    if (lane == 63) waves[1][wave] = sum, waves[2][wave] = ds;
+    blocks[tid] = own;
+    __syncthreads();
+    int from = sum - own, ds_from = ds - ds_own, total = 0;
+    long long ds_total = 0;
+    for (int w = 0; w < 4; ++w) {
+        if (w < wave) from += waves[1][w], ds_from += waves[2][w];
+        total += waves[1][w], ds_total += waves[2][w];
+    }
+    before[tid] = from;
+    ds_at[tid] = ds_from;  // read only where all fit
+    const int first = at[0], last = at[count];
+    if (a.fits && tid == 0 && blockIdx.x == 0) a.fits[0] = ds_total <= a.ds_tiles, a.fits[1] = first, a.fits[2] = last;
+    __syncthreads();
+    for (int i = tid; i < total; i += kPackedFew) {
+        int k = 0, hi = count;
+        while (hi - k > 1) {
+            const int mid = (k + hi) / 2;
+            if (before[mid] <= i) k = mid;
+            else hi = mid;
+        }
+        const int j = i - before[k], n = blocks[k];
+        const int work = t.order == PACKED_RISING ? j + 1 : t.order == PACKED_FALLING ? n - j : n;
+        int place = t.order == PACKED_FLAT ? j : 0;
+        for (int s0 = 0; s0 < count; s0 += 4) {
+            const int4 b4 = *reinterpret_cast<const int4 *>(blocks + s0);
+            const int b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (t.order == PACKED_FLAT) place += b[e] > n || (b[e] == n && s0 + e < k) ? b[e] : 0;
+                else place += max(b[e] - work, 0) + (b[e] >= work && s0 + e < k ? 1 : 0);
+            }
+        }
+        t.tiles[place] = PackedTile{at[k], at[k + 1] - at[k], j, ds_at[k]};
+    }
+    packed_rest(t, total, first, last, tokens);
 }
 
 // The head and table entry of a workgroup: heads fastest, in runs that stay on one XCD (workgroups go round the eight) where
@@ -212,15 +280,18 @@ __global__ __launch_bounds__(256) void packed_prep_kernel(AttnParams p, float *l
 }
 
 // STORE: each tile's dS goes to the workspace for packed_dq_ds_kernel; else packed_dq_kernel computes it again. Where the
-// room for dS may not do both are launched, and `fits` ends one of them.
-template <int D, bool F16, bool CAUSAL, bool STORE>
+// room for dS may not do both are launched, and `fits` ends one of them. PARTS: a workgroup takes part blockIdx.y of a key
+// block's query tiles, whose sums [parts][tokens][kv heads][hd + hdv] packed_dkdv_sum_kernel adds (7 sequences of 812 tokens, 2 key
+// heads of 6, dims 80, float16: 62 us in 18 workgroups, 29 and 7 for the sums in 12 parts).
+template <int D, bool F16, bool CAUSAL, bool STORE, bool PARTS>
 __global__ __launch_bounds__(256) void packed_dkdv_kernel(AttnParams p, const float *lse2, const PackedTile *tiles, int64_t tokens,
-                                                          const int32_t *fits) {
+                                                          const int32_t *fits, float *sums) {
     if (fits && (*fits != 0) != STORE) return;
     int64_t n, idx;
     packed_place(p.kv_heads, n, idx);
     const PackedTile t = tiles[idx];
     if (t.block < 0) {
+        if (PARTS && blockIdx.y) return;
         packed_zeros(p.dk + n * p.dk_n, p.dk_s, p.hd, t);
         packed_zeros(p.dv + n * p.dv_n, p.dv_s, p.hdv, t);
         return;
@@ -229,7 +300,28 @@ __global__ __launch_bounds__(256) void packed_dkdv_kernel(AttnParams p, const fl
     p.d_o += t.start * p.do_s, p.dk += t.start * p.dk_s, p.dv += t.start * p.dv_s;
     p.delta += t.start;
     if (STORE) p.ds += t.ds * p.heads * (128 * 64);
-    flash_dkdv_tile<D, F16, CAUSAL, false, STORE, false>(p, lse2 + t.start, 0, n, t.block, (t.len + 127) / 128, tokens);
+    const int64_t row = p.hd + p.hdv;
+    if (PARTS) sums += ((int64_t(blockIdx.y) * tokens + t.start) * p.kv_heads + n) * row;
+    flash_dkdv_tile<D, F16, CAUSAL, false, STORE, false, PARTS>(p, lse2 + t.start, 0, n, t.block, (t.len + 127) / 128, tokens, int(blockIdx.y),
+                                                                int(gridDim.y), sums, p.kv_heads * row);
+}
+
+// The parts' sums of the sequences' tokens (used[1] to used[2]), added in order and rounded: four elements a thread.
+template <bool F16>
+__global__ __launch_bounds__(256) void packed_dkdv_sum_kernel(AttnParams p, const float *__restrict__ sums, int parts, int64_t tokens,
+                                                              const int32_t *__restrict__ used) {
+    const int64_t row = p.hd + p.hdv, per = p.kv_heads * (row / 4), total = (int64_t(used[2]) - used[1]) * per;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+        const int64_t t = used[1] + i / per, n = i % per / (row / 4), c = i % (row / 4) * 4;
+        const float *from = sums + (t * p.kv_heads + n) * row + c;
+        float4 v = *reinterpret_cast<const float4 *>(from);
+        for (int k = 1; k < parts; ++k) {
+            const float4 x = *reinterpret_cast<const float4 *>(from + k * tokens * p.kv_heads * row);
+            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+        }
+        uint16_t *to = c < p.hd ? p.dk + t * p.dk_s + n * p.dk_n + c : p.dv + t * p.dv_s + n * p.dv_n + (c - p.hd);
+        *reinterpret_cast<uint2 *>(to) = make_uint2(pack2<F16>(v.x, v.y), pack2<F16>(v.z, v.w));
+    }
 }
 
 template <int D, bool F16, bool CAUSAL>

@@ -36,12 +36,21 @@ int64_t most_ds(const nhip_packed_desc *d) {
 }
 int64_t ds_room(const nhip_packed_desc *d) {
     if (d->ds_bytes <= 0 || d->heads <= 0) return 0;
-    return std::min(most_ds(d), d->ds_bytes / (d->heads * 128 * 64 * 2));
+    // below 2^24: what packed_tiles_few_kernel counts to
+    return std::min<int64_t>(std::min(most_ds(d), d->ds_bytes / (d->heads * 128 * 64 * 2)), (1 << 24) - 1);
+}
+
+// Parts of a key block's query tiles: as many as give the CUs about a workgroup and a half each where whole blocks leave most
+// of them idle, their count estimated with half a block a sequence lost.
+int64_t key_parts(const nhip_packed_desc *d) {
+    const int64_t blocks = (d->tokens / kKeyBlock + std::min(d->sequences, d->tokens) / 2 + 1) * std::max<int64_t>(d->kv_heads, 1);
+    if (blocks >= 192) return 1;
+    return std::max<int64_t>(std::min<int64_t>(384 / blocks, 16), 1);
 }
 
 // The backward's workspace: delta and the base-2 LSE, the flag, both tables, dS.
 struct BwdSpace {
-    size_t stats, flag, keys, queries, ds, bytes;
+    size_t stats, flag, keys, queries, sums, ds, bytes;
 };
 BwdSpace bwd_space(const nhip_packed_desc *d) {
     BwdSpace w{};
@@ -49,7 +58,9 @@ BwdSpace bwd_space(const nhip_packed_desc *d) {
     w.flag = up256(2 * size_t(d->heads) * d->tokens * sizeof(float));
     w.keys = w.flag + 256;
     w.queries = w.keys + table_bytes(d, kKeyBlock);
-    w.ds = w.queries + table_bytes(d, kDqBlock);
+    w.sums = w.queries + table_bytes(d, kDqBlock);
+    const int64_t parts = key_parts(d);
+    w.ds = w.sums + (parts > 1 ? up256(size_t(parts) * d->tokens * d->kv_heads * (d->head_dim + value_dim(d)) * sizeof(float)) : 0);
     w.bytes = w.ds + size_t(ds_room(d)) * d->heads * (128 * 64 * 2);
     return w;
 }
@@ -107,7 +118,8 @@ PackedTable table(const nhip_packed_desc *d, int64_t block, int order, void *til
 
 int build_tables(hipStream_t st, const nhip_packed_desc *d, const void *offsets, PackedTables a, int count) {
     a.offsets = offsets, a.sequences = d->sequences, a.tokens = d->tokens, a.o64 = d->offsets_dtype == NHIP_POS_I64;
-    hipLaunchKernelGGL(packed_tiles_kernel, dim3(unsigned(count)), dim3(kPackedBuckets), 0, st, a);
+    if (d->sequences < kPackedFew) hipLaunchKernelGGL(packed_tiles_few_kernel, dim3(unsigned(count)), dim3(kPackedFew), 0, st, a);
+    else hipLaunchKernelGGL(packed_tiles_kernel, dim3(unsigned(count)), dim3(kPackedBuckets), 0, st, a);
     return check(hipGetLastError(), "packed_tiles_kernel launch");
 }
 
@@ -119,26 +131,40 @@ int fwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, const Pa
 }
 
 template <int D, bool F16, bool CAUSAL>
-int bwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, const PackedTables &a, bool store, bool again) {
+int dkdv(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, const PackedTables &a, const float *lse2, const int32_t *fits,
+         float *sums, bool store) {
+    const int64_t parts = key_parts(d);
+    const dim3 grid(unsigned(a.t[0].most * d->kv_heads), unsigned(parts));
+    auto kern = parts > 1 ? (store ? packed_dkdv_kernel<D, F16, CAUSAL, true, true> : packed_dkdv_kernel<D, F16, CAUSAL, false, true>)
+                          : (store ? packed_dkdv_kernel<D, F16, CAUSAL, true, false> : packed_dkdv_kernel<D, F16, CAUSAL, false, false>);
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, p, lse2, a.t[0].tiles, d->tokens, fits, sums);
+    return check(hipGetLastError(), "packed_dkdv_kernel launch");
+}
+
+template <int D, bool F16, bool CAUSAL>
+int bwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, const PackedTables &a, bool store, bool again, float *sums) {
     float *lse2 = p.delta + size_t(d->heads) * d->tokens;
     constexpr int RPB = 256 / (D / 8);
     hipLaunchKernelGGL((packed_prep_kernel<D, F16>), dim3(unsigned((d->heads * d->tokens + RPB - 1) / RPB)), dim3(256), 0, st, p, lse2);
     if (check(hipGetLastError(), "packed delta launch")) return 1;
-    const dim3 gk(unsigned(a.t[0].most * d->kv_heads)), gq(unsigned(a.t[1].most * d->heads));
+    const dim3 gq(unsigned(a.t[1].most * d->heads));
     const int32_t *fits = store && again ? a.fits : nullptr;
     if (store) {
-        hipLaunchKernelGGL((packed_dkdv_kernel<D, F16, CAUSAL, true>), gk, dim3(256), 0, st, p, lse2, a.t[0].tiles, d->tokens, fits);
-        if (check(hipGetLastError(), "packed_dkdv_kernel launch")) return 1;
+        if (dkdv<D, F16, CAUSAL>(st, d, p, a, lse2, fits, sums, true)) return 1;
         hipLaunchKernelGGL((packed_dq_ds_kernel<D, F16, CAUSAL>), gq, dim3(256), 0, st, p, a.t[1].tiles, fits);
         if (check(hipGetLastError(), "packed_dq_ds_kernel launch")) return 1;
     }
     if (again) {
-        hipLaunchKernelGGL((packed_dkdv_kernel<D, F16, CAUSAL, false>), gk, dim3(256), 0, st, p, lse2, a.t[0].tiles, d->tokens, fits);
-        if (check(hipGetLastError(), "packed_dkdv_kernel launch")) return 1;
+        if (dkdv<D, F16, CAUSAL>(st, d, p, a, lse2, fits, sums, false)) return 1;
         hipLaunchKernelGGL((packed_dq_kernel<D, F16, CAUSAL>), gq, dim3(256), 0, st, p, lse2, a.t[1].tiles, d->tokens, fits);
         if (check(hipGetLastError(), "packed_dq_kernel launch")) return 1;
     }
-    return 0;
+    const int64_t parts = key_parts(d);
+    if (parts == 1) return 0;
+    const int64_t work = d->tokens * d->kv_heads * (p.hd + p.hdv) / 4;
+    hipLaunchKernelGGL((packed_dkdv_sum_kernel<F16>), dim3(unsigned(std::min<int64_t>((work + 255) / 256, 2048))), dim3(256), 0, st, p, sums,
+                       int(parts), d->tokens, a.fits);
+    return check(hipGetLastError(), "packed_dkdv_sum_kernel launch");
 }
 
 }  // namespace
@@ -176,6 +202,7 @@ int packed_bwd_on(hipStream_t st, const nhip_packed_desc *d, const void *q, cons
     p.dq = static_cast<uint16_t *>(dq), p.dk = static_cast<uint16_t *>(dk), p.dv = static_cast<uint16_t *>(dv);
     p.delta = reinterpret_cast<float *>(at + w.stats);
     p.ds = reinterpret_cast<uint16_t *>(at + w.ds);
+    float *sums = reinterpret_cast<float *>(at + w.sums);
     const int64_t room = ds_room(d);
     const bool store = room > 0, again = room < most_ds(d);
     PackedTables a{};
@@ -186,8 +213,8 @@ int packed_bwd_on(hipStream_t st, const nhip_packed_desc *d, const void *q, cons
     if (build_tables(st, d, offsets, a, 2)) return 1;
     const bool f16 = d->dtype == NHIP_F16;
 #define NHIP_PACKED(DD)                                                                                                             \
-    return f16 ? (d->causal ? bwd<DD, true, true>(st, d, p, a, store, again) : bwd<DD, true, false>(st, d, p, a, store, again)) \
-               : (d->causal ? bwd<DD, false, true>(st, d, p, a, store, again) : bwd<DD, false, false>(st, d, p, a, store, again))
+    return f16 ? (d->causal ? bwd<DD, true, true>(st, d, p, a, store, again, sums) : bwd<DD, true, false>(st, d, p, a, store, again, sums)) \
+               : (d->causal ? bwd<DD, false, true>(st, d, p, a, store, again, sums) : bwd<DD, false, false>(st, d, p, a, store, again, sums))
     if (kernel_dim(d) == 64) NHIP_PACKED(64);
     NHIP_PACKED(128);
 #undef NHIP_PACKED
