@@ -166,18 +166,21 @@ class Compiled:
     def __call__(self, *args):
         target, (traced, plan, workspace, recipe) = self._prepare(args)
         ran = plan is not None
-        for a in args:  # a loop: any() of a generator costs twice as much
-            if isinstance(a, Tensor) and a.device != target and device_type(a.device) == "meta":
-                ran = False
+        tensors, others = [], []
+        for a in args:  # one loop over them: a call with many tensors is bound by the host
+            if isinstance(a, Tensor):
+                tensors.append(a)
+                if a.device != target and device_type(a.device) == "meta":
+                    ran = False
+            else:
+                others.append(a)
         if not ran:
             g = traced.graph
             outs = [Tensor(g.types[v].dtype, g.types[v].shape, "meta") for v in g.outputs]
         else:
-            keep = []
-            if recipe.args:
-                tensors = [a for a in args if isinstance(a, Tensor)]
+            keep, ptrs = [], []
             if recipe.scalars:
-                scalars = _scalars(args)
+                scalars = _scalars(others)
             for kind, k in traced.layout:
                 if kind == "arg":
                     t = tensors[k]
@@ -188,7 +191,8 @@ class Compiled:
                 else:
                     t = traced.weights[k]._placed(target)
                 keep.append(t)
-            ptrs = self._run(plan, workspace, traced, [t._buffer.ptr + t._offset for t in keep], keep)
+                ptrs.append(t._buffer.ptr + t._offset)
+            ptrs = self._run(plan, workspace, traced, ptrs, keep)
             self._last_buffers = (workspace.ptr, ptrs)
             # outputs computed over the weight they replace, or views of the workspace
             outs = [keep[i] if i is not None else Tensor.on_device(dtype, shape, target, workspace, offset)
@@ -204,12 +208,12 @@ class Compiled:
 
 
 class _Recipe:
-    """What a call of a plan does, worked out once: which kinds of inputs its layout names, where each output lies
+    """What a call of a plan does, worked out once: whether its layout names scalars, where each output lies
     (``(input position or None, dtype, shape, byte offset in the workspace)``) and the weights copied back."""
 
     def __init__(self, traced, plan):
         kinds = {kind for kind, _ in traced.layout}
-        self.args, self.scalars = "arg" in kinds, "scalar" in kinds
+        self.scalars = "scalar" in kinds
         self.outputs = [(loc.base[1] if loc.base[0] == "in" else None, loc.dtype, tuple(loc.shape),
                          loc.offset * _size(loc.dtype)) for loc in plan.output_locs]
         self.copied_back = [(traced.n_returned + j, k) for j, k in enumerate(traced.written)
