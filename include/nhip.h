@@ -360,7 +360,9 @@ int nhip_head_loss_workspace(const nhip_head_desc *desc, int gradients, size_t *
  * offsets[i] <= t < offsets[i + 1], and attends to that sequence's tokens (up to itself if causal). Offsets, sequences + 1 of
  * them on the device, do not decrease; whatever they hold, they are read as clamped into [the one before, tokens]. Tokens of
  * no sequence are left out: their results are zeros, and nothing of them (nor of another sequence) reaches any other.
- * The forward writes o and, unless null, lse (float32 [heads, tokens]; only the sequences' tokens), which the backward reads.
+ * The forward writes o and, unless null, lse (float32 [heads, tokens]; only the sequences' tokens), which the backward reads, and
+ * rest, what the rounding of o left, in o's type and dense [tokens, heads, value_head_dim], which the backward adds to o (null: o
+ * alone).
  * Head dims are multiples of 8 up to 128, V's (and O's) in value_head_dim where it differs (0: the same); rows start on 16
  * bytes (strides are multiples of 8 elements). Grouped heads' dK and dV are summed over each group. The same bits every run.
  * ds_bytes: what the backward's workspace may hold of dS (16-bit, computed once; 0, or sequences too long for it: computed
@@ -374,10 +376,10 @@ typedef struct {
     float scale;
 } nhip_packed_desc;
 
-int nhip_packed_fwd(const nhip_packed_desc *desc, const void *q, const void *k, const void *v, const void *offsets, void *o, float *lse,
-                    void *workspace);
+int nhip_packed_fwd(const nhip_packed_desc *desc, const void *q, const void *k, const void *v, const void *offsets, void *o, void *rest,
+                    float *lse, void *workspace);
 int nhip_packed_bwd(const nhip_packed_desc *desc, const void *q, const void *k, const void *v, const void *offsets, const void *o,
-                    const void *d_o, const float *lse, void *dq, void *dk, void *dv, void *workspace);
+                    const void *rest, const void *d_o, const float *lse, void *dq, void *dk, void *dv, void *workspace);
 int nhip_packed_workspace(const nhip_packed_desc *desc, int backward, size_t *bytes);
 
 /* ---- AdamW (no counterpart in the reference) --------------------------------------------------------------------- *
@@ -450,8 +452,8 @@ enum {
     NHIP_STEP_ADAMW = 15,     /* desc: nhip_adamw_desc, then its nhip_adamw_tensors (pointers ignored); pointers: lr_at, step_at,
                                  grad_scale_at (each or none), then tensor i's param, grad, m, v, master, param_out, m_out,
                                  v_out, master_out from 3 + 9 i on (or none) */
-    NHIP_STEP_PACKED_FWD = 16, /* desc: nhip_packed_desc; pointers: q, k, v, offsets, o, lse (or none), workspace */
-    NHIP_STEP_PACKED_BWD = 17, /* desc: nhip_packed_desc; pointers: q, k, v, offsets, o, do, lse, dq, dk, dv, workspace */
+    NHIP_STEP_PACKED_FWD = 16, /* desc: nhip_packed_desc; pointers: q, k, v, offsets, o, rest, lse (or none), workspace */
+    NHIP_STEP_PACKED_BWD = 17, /* desc: nhip_packed_desc; pointers: q, k, v, offsets, o, rest, do, lse, dq, dk, dv, workspace */
     NHIP_STEP_HEAD_LOSS = 18,  /* desc: nhip_head_desc; pointers as nhip_head_loss's, those left out null */
 };
 

@@ -52,7 +52,7 @@ def _wants(node):
     if name == "packed_attention":
         return [CHUNK_ROWS] * 3 + [DENSE]
     if name == "packed_attention_backward":
-        return [CHUNK_ROWS] * 3 + [DENSE] + [CHUNK_ROWS] * 2 + [DENSE]
+        return [CHUNK_ROWS] * 3 + [DENSE] + [CHUNK_ROWS, DENSE, CHUNK_ROWS, DENSE]
     return [DENSE] * len(node.inputs)
 
 
@@ -345,7 +345,7 @@ def _lower_packed(plan, step):
                 t = plan.graph.types[node.inputs[operand]]
                 out[index] = _dense(t, spare)
                 spare += _up256(t.nbytes())
-        names += [("o", at[4]), ("do", at[5]), ("dq", out[0]), ("dk", out[1]), ("dv", out[2])]
+        names += [("o", at[4]), ("do", at[6]), ("dq", out[0]), ("dk", out[1]), ("dv", out[2])]
     else:
         names.append(("o", out[0]))
     for name, loc in names:
@@ -354,7 +354,7 @@ def _lower_packed(plan, step):
         setattr(d, f"{name}_n", d_n)
     scratch = plan.scratch[id(step)]
     if not backward:
-        return nv.NHIP_STEP_PACKED_FWD, bytes(d), _slots([*at, out[0], out.get(1), scratch])
+        return nv.NHIP_STEP_PACKED_FWD, bytes(d), _slots([*at, out[0], out.get(1), out.get(2), scratch])
     return nv.NHIP_STEP_PACKED_BWD, bytes(d), _slots([*at, *(loc for _, loc in names[5:]), scratch])
 
 

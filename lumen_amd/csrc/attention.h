@@ -209,9 +209,11 @@ template <int NW, int D = 128> struct FwdOccupancy {
 // LDS read would be taken to alias the loads just issued into the other half and wait for them (s_waitcnt vmcnt(0)
 // before the tile's first read), so that nothing overlapped. [8, 2048, 16, 128] causal 243 -> 192-203 us (679-716
 // TFLOP/s), [2, 1777, 16 / 4, 64] 43 -> 37. ONE: halves of one array after all, for fewer registers (launch_fwd_nw).
-// One workgroup's queries [32 NW qblk, 32 NW (qblk + 1)) of head n of batch b.
-template <int D, bool F16, bool CAUSAL, int NW, bool ONE = false>
-__device__ __forceinline__ void flash_fwd_tile(const AttnParams &p, int64_t b, int64_t n, int64_t qblk) {
+// One workgroup's queries [32 NW qblk, 32 NW (qblk + 1)) of head n of batch b. REST: what the rounding of O leaves goes to `rest`
+// (none if null), rows rest_s apart.
+template <int D, bool F16, bool CAUSAL, int NW, bool ONE = false, bool REST = false>
+__device__ __forceinline__ void flash_fwd_tile(const AttnParams &p, int64_t b, int64_t n, int64_t qblk, uint16_t *rest = nullptr,
+                                               int64_t rest_s = 0) {
     constexpr int QB = 32 * NW;  // queries a workgroup
     constexpr int BN = 64;
     constexpr int DS = D / 16, DT = D / 32;
@@ -364,6 +366,14 @@ __device__ __forceinline__ void flash_fwd_tile(const AttnParams &p, int64_t b, i
             const uint32_t w0 = pack2<F16>(acc[dt][4 * e4 + 0] * inv, acc[dt][4 * e4 + 1] * inv);
             const uint32_t w1 = pack2<F16>(acc[dt][4 * e4 + 2] * inv, acc[dt][4 * e4 + 3] * inv);
             *reinterpret_cast<uint2 *>(op + 32 * dt + 8 * e4 + 4 * h) = make_uint2(w0, w1);
+            if constexpr (REST) {
+                auto left = [&](uint32_t w, int e) {
+                    const float lo = F16 ? f16_to_f32(uint16_t(w & 0xffffu)) : bf16_to_f32(uint16_t(w & 0xffffu));
+                    const float hi = F16 ? f16_to_f32(uint16_t(w >> 16)) : bf16_to_f32(uint16_t(w >> 16));
+                    return pack2<F16>(acc[dt][4 * e4 + e] * inv - lo, acc[dt][4 * e4 + e + 1] * inv - hi);
+                };
+                if (rest) *reinterpret_cast<uint2 *>(rest + qi * rest_s + 32 * dt + 8 * e4 + 4 * h) = make_uint2(left(w0, 0), left(w1, 2));
+            }
         }
     if (h == 0 && p.lse) p.lse[(b * p.heads + n) * p.sq + qi] = l > 0.0f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY;
 }

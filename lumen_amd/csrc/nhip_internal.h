@@ -47,8 +47,8 @@ int adamw_on(hipStream_t s, const nhip_adamw_desc *d, const nhip_adamw_tensor *t
 int head_on(hipStream_t s, const nhip_head_desc *d, const void *h, const void *w, const void *target, const float *g, float *losses,
             void *dh, void *dw, void *ws);
 int packed_fwd_on(hipStream_t s, const nhip_packed_desc *d, const void *q, const void *k, const void *v, const void *offsets, void *o,
-                  float *lse, void *ws);
+                  void *rest, float *lse, void *ws);
 int packed_bwd_on(hipStream_t s, const nhip_packed_desc *d, const void *q, const void *k, const void *v, const void *offsets,
-                  const void *o, const void *d_o, const float *lse, void *dq, void *dk, void *dv, void *ws);
+                  const void *o, const void *rest, const void *d_o, const float *lse, void *dq, void *dk, void *dv, void *ws);
 
 }  // namespace nhip

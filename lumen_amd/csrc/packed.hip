@@ -124,9 +124,9 @@ int build_tables(hipStream_t st, const nhip_packed_desc *d, const void *offsets,
 }
 
 template <int D, bool F16, bool CAUSAL>
-int fwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, const PackedTable &t) {
+int fwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, uint16_t *rest, const PackedTable &t) {
     const dim3 grid(unsigned(t.most * d->heads));
-    hipLaunchKernelGGL((packed_fwd_kernel<D, F16, CAUSAL, 4>), grid, dim3(256), 0, st, p, t.tiles, d->tokens);
+    hipLaunchKernelGGL((packed_fwd_kernel<D, F16, CAUSAL, 4>), grid, dim3(256), 0, st, p, rest, t.tiles, d->tokens);
     return check(hipGetLastError(), "packed_fwd_kernel launch");
 }
 
@@ -142,10 +142,11 @@ int dkdv(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, const P
 }
 
 template <int D, bool F16, bool CAUSAL>
-int bwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, const PackedTables &a, bool store, bool again, float *sums) {
+int bwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, const uint16_t *rest, const PackedTables &a, bool store, bool again,
+        float *sums) {
     float *lse2 = p.delta + size_t(d->heads) * d->tokens;
     constexpr int RPB = 256 / (D / 8);
-    hipLaunchKernelGGL((packed_prep_kernel<D, F16>), dim3(unsigned((d->heads * d->tokens + RPB - 1) / RPB)), dim3(256), 0, st, p, lse2);
+    hipLaunchKernelGGL((packed_prep_kernel<D, F16>), dim3(unsigned((d->heads * d->tokens + RPB - 1) / RPB)), dim3(256), 0, st, p, rest, lse2);
     if (check(hipGetLastError(), "packed delta launch")) return 1;
     const dim3 gq(unsigned(a.t[1].most * d->heads));
     const int32_t *fits = store && again ? a.fits : nullptr;
@@ -170,28 +171,29 @@ int bwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, const Pa
 }  // namespace
 
 int packed_fwd_on(hipStream_t st, const nhip_packed_desc *d, const void *q, const void *k, const void *v, const void *offsets, void *o,
-                  float *lse, void *ws) {
-    if (packed_check(d, "nhip_packed_fwd") || on16("nhip_packed_fwd", {q, k, v, o, ws})) return 1;
+                  void *rest, float *lse, void *ws) {
+    if (packed_check(d, "nhip_packed_fwd") || on16("nhip_packed_fwd", {q, k, v, o, rest, ws})) return 1;
     if (d->tokens == 0 || d->heads == 0) return 0;
     if (!ws) return fail("nhip_packed_fwd: no workspace");
     AttnParams p = packed_params(d);
     p.q = static_cast<const uint16_t *>(q), p.k = static_cast<const uint16_t *>(k), p.v = static_cast<const uint16_t *>(v);
     p.o = static_cast<uint16_t *>(o), p.lse = lse;
+    uint16_t *left = static_cast<uint16_t *>(rest);
     PackedTables a{};
     a.t[0] = table(d, fwd_block(d), PACKED_RISING, ws);
     if (build_tables(st, d, offsets, a, 1)) return 1;
     const bool f16 = d->dtype == NHIP_F16;
 #define NHIP_PACKED(DD)                                                                                      \
-    return f16 ? (d->causal ? fwd<DD, true, true>(st, d, p, a.t[0]) : fwd<DD, true, false>(st, d, p, a.t[0])) \
-               : (d->causal ? fwd<DD, false, true>(st, d, p, a.t[0]) : fwd<DD, false, false>(st, d, p, a.t[0]))
+    return f16 ? (d->causal ? fwd<DD, true, true>(st, d, p, left, a.t[0]) : fwd<DD, true, false>(st, d, p, left, a.t[0])) \
+               : (d->causal ? fwd<DD, false, true>(st, d, p, left, a.t[0]) : fwd<DD, false, false>(st, d, p, left, a.t[0]))
     if (kernel_dim(d) == 64) NHIP_PACKED(64);
     NHIP_PACKED(128);
 #undef NHIP_PACKED
 }
 
 int packed_bwd_on(hipStream_t st, const nhip_packed_desc *d, const void *q, const void *k, const void *v, const void *offsets,
-                  const void *o, const void *d_o, const float *lse, void *dq, void *dk, void *dv, void *ws) {
-    if (packed_check(d, "nhip_packed_bwd") || on16("nhip_packed_bwd", {q, k, v, o, d_o, dq, dk, dv, ws})) return 1;
+                  const void *o, const void *rest, const void *d_o, const float *lse, void *dq, void *dk, void *dv, void *ws) {
+    if (packed_check(d, "nhip_packed_bwd") || on16("nhip_packed_bwd", {q, k, v, o, rest, d_o, dq, dk, dv, ws})) return 1;
     if (d->tokens == 0 || d->heads == 0) return 0;
     if (!ws) return fail("nhip_packed_bwd: no workspace");
     const BwdSpace w = bwd_space(d);
@@ -200,6 +202,7 @@ int packed_bwd_on(hipStream_t st, const nhip_packed_desc *d, const void *q, cons
     p.q = static_cast<const uint16_t *>(q), p.k = static_cast<const uint16_t *>(k), p.v = static_cast<const uint16_t *>(v);
     p.o_in = static_cast<const uint16_t *>(o), p.d_o = static_cast<const uint16_t *>(d_o), p.lse_in = lse;
     p.dq = static_cast<uint16_t *>(dq), p.dk = static_cast<uint16_t *>(dk), p.dv = static_cast<uint16_t *>(dv);
+    const uint16_t *left = static_cast<const uint16_t *>(rest);
     p.delta = reinterpret_cast<float *>(at + w.stats);
     p.ds = reinterpret_cast<uint16_t *>(at + w.ds);
     float *sums = reinterpret_cast<float *>(at + w.sums);
@@ -213,8 +216,8 @@ int packed_bwd_on(hipStream_t st, const nhip_packed_desc *d, const void *q, cons
     if (build_tables(st, d, offsets, a, 2)) return 1;
     const bool f16 = d->dtype == NHIP_F16;
 #define NHIP_PACKED(DD)                                                                                                             \
-    return f16 ? (d->causal ? bwd<DD, true, true>(st, d, p, a, store, again, sums) : bwd<DD, true, false>(st, d, p, a, store, again, sums)) \
-               : (d->causal ? bwd<DD, false, true>(st, d, p, a, store, again, sums) : bwd<DD, false, false>(st, d, p, a, store, again, sums))
+    return f16 ? (d->causal ? bwd<DD, true, true>(st, d, p, left, a, store, again, sums) : bwd<DD, true, false>(st, d, p, left, a, store, again, sums)) \
+               : (d->causal ? bwd<DD, false, true>(st, d, p, left, a, store, again, sums) : bwd<DD, false, false>(st, d, p, left, a, store, again, sums))
     if (kernel_dim(d) == 64) NHIP_PACKED(64);
     NHIP_PACKED(128);
 #undef NHIP_PACKED
@@ -224,18 +227,18 @@ int packed_bwd_on(hipStream_t st, const nhip_packed_desc *d, const void *q, cons
 
 extern "C" {
 
-int nhip_packed_fwd(const nhip_packed_desc *desc, const void *q, const void *k, const void *v, const void *offsets, void *o, float *lse,
-                    void *workspace) {
+int nhip_packed_fwd(const nhip_packed_desc *desc, const void *q, const void *k, const void *v, const void *offsets, void *o, void *rest,
+                    float *lse, void *workspace) {
     hipStream_t st = stream_of_current();
     if (!st) return fail("no HIP stream: call nhip_set_device first");
-    return packed_fwd_on(st, desc, q, k, v, offsets, o, lse, workspace);
+    return packed_fwd_on(st, desc, q, k, v, offsets, o, rest, lse, workspace);
 }
 
 int nhip_packed_bwd(const nhip_packed_desc *desc, const void *q, const void *k, const void *v, const void *offsets, const void *o,
-                    const void *d_o, const float *lse, void *dq, void *dk, void *dv, void *workspace) {
+                    const void *rest, const void *d_o, const float *lse, void *dq, void *dk, void *dv, void *workspace) {
     hipStream_t st = stream_of_current();
     if (!st) return fail("no HIP stream: call nhip_set_device first");
-    return packed_bwd_on(st, desc, q, k, v, offsets, o, d_o, lse, dq, dk, dv, workspace);
+    return packed_bwd_on(st, desc, q, k, v, offsets, o, rest, d_o, lse, dq, dk, dv, workspace);
 }
 
 int nhip_packed_workspace(const nhip_packed_desc *desc, int backward, size_t *bytes) {

@@ -719,12 +719,12 @@ static int run_steps(Plan *plan, void *workspace, void *const *inputs, size_t ni
                 break;
             case NHIP_STEP_PACKED_FWD:
                 rc = packed_fwd_on(s, reinterpret_cast<const nhip_packed_desc *>(st.args.data()), ptrs[0], ptrs[1], ptrs[2],
-                                   ptrs[3], ptrs[4], static_cast<float *>(ptrs[5]), ptrs[6]);
+                                   ptrs[3], ptrs[4], ptrs[5], static_cast<float *>(ptrs[6]), ptrs[7]);
                 break;
             case NHIP_STEP_PACKED_BWD:
                 rc = packed_bwd_on(s, reinterpret_cast<const nhip_packed_desc *>(st.args.data()), ptrs[0], ptrs[1], ptrs[2],
-                                   ptrs[3], ptrs[4], ptrs[5], static_cast<const float *>(ptrs[6]), ptrs[7], ptrs[8], ptrs[9],
-                                   ptrs[10]);
+                                   ptrs[3], ptrs[4], ptrs[5], ptrs[6], static_cast<const float *>(ptrs[7]), ptrs[8], ptrs[9],
+                                   ptrs[10], ptrs[11]);
                 break;
             case NHIP_STEP_HEAD_LOSS:
                 rc = head_on(s, reinterpret_cast<const nhip_head_desc *>(st.args.data()), ptrs[0], ptrs[1], ptrs[2],

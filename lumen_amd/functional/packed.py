@@ -53,7 +53,8 @@ def _kept(x, mask, other=0.0):
 
 
 def _forward(q, k, v, offsets, scale, causal):
-    """``(o, lse)``: ``lse`` ``[N, T]``, 0 of a token of no sequence."""
+    """``(o, rest, lse)``: what the rounding of ``o`` left, in its dtype, and the scores' log-sum-exp ``[N, T]``, 0 of a token of no
+    sequence."""
     t, n = q.shape[:2]
     acc = accum_dtype(q.dtype)
     of, inside = _sequences(offsets, t)
@@ -67,22 +68,24 @@ def _forward(q, k, v, offsets, scale, causal):
     total = F.sum(e, -1, keepdim=True)
     total = F.where(empty, prims.full(top.shape, 1.0, acc), total)
     p = (e / broadcast_to(total, s.shape)).to(q.dtype)
-    o = dot(p, _heads(v, n), (((2,), (0,)), ((0,), (1,))), acc, q.dtype).permute(1, 0, 2)
-    return _inside(inside, o)[0], (top + F.log(total)).reshape(n, t)
+    whole = dot(p, _heads(v, n), (((2,), (0,)), ((0,), (1,))), acc, acc).permute(1, 0, 2)
+    o = whole.to(q.dtype)
+    rest = (whole - o.to(acc)).to(q.dtype)
+    return *_inside(inside, o, rest), (top + F.log(total)).reshape(n, t)
 
 
-def _gradients(q, k, v, offsets, o, lse, do, scale, causal):
-    """``[dq, dk, dv]``: probabilities again from the log-sum-exp, ``dS = P (dO V^T - rowsum(dO O))``."""
+def _gradients(q, k, v, offsets, o, rest, lse, do, scale, causal):
+    """``[dq, dk, dv]``: probabilities again from the log-sum-exp, ``dS = P (dO V^T - rowsum(dO (O + rest)))``."""
     t, n = q.shape[:2]
     nkv = k.shape[1]
     dtype, acc = q.dtype, accum_dtype(q.dtype)
     of, inside = _sequences(offsets, t)
     seen = _seen(of, inside, causal)
-    q, k, v, o, do = _inside(inside, q, k, v, o, do)
+    q, k, v, o, rest, do = _inside(inside, q, k, v, o, rest, do)
     k_full, v_full = _heads(k, n), _heads(v, n)
     s = prims.dot_general(q, k_full, _QK, acc) * scale
     p = _kept(F.exp(_kept(s - broadcast_to(lse.reshape(n, t, 1), s.shape), seen)), seen)
-    delta = F.sum(do.to(acc) * o.to(acc), -1).permute(1, 0).reshape(n, t, 1)
+    delta = F.sum(do.to(acc) * (o.to(acc) + rest.to(acc)), -1).permute(1, 0).reshape(n, t, 1)
     dp = prims.dot_general(do, v_full, _QK, acc)
     ds = _kept(p * (dp - broadcast_to(delta, dp.shape)) * scale, seen).to(dtype)
     p = p.to(dtype)
@@ -105,10 +108,10 @@ def _taken(q, k, v, offsets):
 class _PackedAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets, *, scale, causal):
-        o, lse = _operator("packed_attention", _taken(q, k, v, offsets), [q, k, v, offsets],
-                           lambda *xs: _forward(*xs, scale, causal), scale=scale, causal=causal)
+        o, rest, lse = _operator("packed_attention", _taken(q, k, v, offsets), [q, k, v, offsets],
+                                 lambda *xs: _forward(*xs, scale, causal), scale=scale, causal=causal)
         ctx.scale, ctx.causal = scale, causal
-        ctx.save_for_backward(q, k, v, offsets, o, lse)
+        ctx.save_for_backward(q, k, v, offsets, o, rest, lse)
         return o
 
     @staticmethod
@@ -118,11 +121,11 @@ class _PackedAttention(Function):
 
 class _PackedGradients(Function):
     @staticmethod
-    def forward(ctx, do, q, k, v, offsets, o, lse, *, scale, causal):
+    def forward(ctx, do, q, k, v, offsets, o, rest, lse, *, scale, causal):
         ctx.scale, ctx.causal = scale, causal
         ctx.save_for_backward(do, q, k, v, offsets)
-        return _operator("packed_attention_backward", _taken(q, k, v, offsets), [q, k, v, offsets, o, do, lse],
-                         lambda q, k, v, offsets, o, do, lse: _gradients(q, k, v, offsets, o, lse, do, scale, causal),
+        return _operator("packed_attention_backward", _taken(q, k, v, offsets), [q, k, v, offsets, o, rest, do, lse],
+                         lambda q, k, v, offsets, o, rest, do, lse: _gradients(q, k, v, offsets, o, rest, lse, do, scale, causal),
                          scale=scale, causal=causal)
 
     @staticmethod
@@ -130,10 +133,10 @@ class _PackedGradients(Function):
         do, q, k, v, offsets = ctx.saved_tensors
 
         def grads(do, q, k, v):
-            o, lse = _forward(q, k, v, offsets, ctx.scale, ctx.causal)
-            return tuple(_gradients(q, k, v, offsets, o, lse, do, ctx.scale, ctx.causal))
+            o, rest, lse = _forward(q, k, v, offsets, ctx.scale, ctx.causal)
+            return tuple(_gradients(q, k, v, offsets, o, rest, lse, do, ctx.scale, ctx.causal))
 
-        return (*_second(grads, (do, q, k, v), cotangents), None, None, None)
+        return (*_second(grads, (do, q, k, v), cotangents), None, None, None, None)
 
 
 def packed_attention(query, key, value, offsets, scale=None, is_causal=True):

@@ -219,8 +219,8 @@ SIGNATURES = {
     "nhip_clip_grad_norm": ([C.POINTER(ClipDesc), C.POINTER(ClipTensor)] + [C.c_void_p] * 4, C.c_int),
     "nhip_head_loss": ([C.POINTER(HeadDesc)] + [C.c_void_p] * 8, C.c_int),
     "nhip_head_loss_workspace": ([C.POINTER(HeadDesc), C.c_int, C.POINTER(C.c_size_t)], C.c_int),
-    "nhip_packed_fwd": ([C.POINTER(PackedDesc)] + [C.c_void_p] * 7, C.c_int),
-    "nhip_packed_bwd": ([C.POINTER(PackedDesc)] + [C.c_void_p] * 11, C.c_int),
+    "nhip_packed_fwd": ([C.POINTER(PackedDesc)] + [C.c_void_p] * 8, C.c_int),
+    "nhip_packed_bwd": ([C.POINTER(PackedDesc)] + [C.c_void_p] * 12, C.c_int),
     "nhip_packed_workspace": ([C.POINTER(PackedDesc), C.c_int, C.POINTER(C.c_size_t)], C.c_int),
     "nhip_adamw": ([C.POINTER(AdamwDesc), C.POINTER(AdamwTensor)] + [C.c_void_p] * 3, C.c_int),
     "nhip_clip_grad_norm_workspace": ([C.POINTER(ClipDesc), C.POINTER(C.c_size_t)], C.c_int),

@@ -161,6 +161,21 @@ def test_heads_enough_for_whole_key_blocks(hip, lengths, n, nkv, d, dtype, limit
             _near(_values(a), w, tt, name)
 
 
+def test_gradients_of_short_sequences_take_o_whole(hip):
+    """Rounding is off by a step's half at most, evenly: of values whose logarithms are spread evenly 2^-8 sqrt(0.541 / 3) =
+    1.66e-3 in the mean square (the mean of 1 / m^2 for a mantissa m of [1, 2) being 0.541). Of dQ and dK the result, dS and the
+    forward's P are rounded: sqrt(3) of it. O's own rounding, the same in every dS of a row, would add more than one of them."""
+    rng = np.random.default_rng(13)
+    offsets = M.offsets_of([2, 3, 4, 5, 6, 7, 8] * 20)
+    t, n, d = int(offsets[-1]), 4, 64
+    x = {k: _round(v, "bfloat16") for k, v in M.packed_inputs(rng, t, n, n, d).items()}
+    want, _ = M.packed(x, offsets, True, d**-0.5, "bfloat16")
+    f = L.compile(_program(True), device="hip")
+    got = f(*[_tensor(x[k], "bfloat16") for k in "qkv"], L.from_numpy(offsets), _tensor(x["do"], "bfloat16"))
+    for name, a, w in list(zip(("o", "dq", "dk", "dv"), got, want))[1:3]:
+        assert np.sqrt(((_values(a) - w) ** 2).sum() / (w**2).sum()) < 3**0.5 * 1.66e-3, name
+
+
 def test_more_sequences_than_a_pass_of_the_builder(hip):
     """2500 sequences, mostly of a few tokens, some empty, some longer than eight blocks: 1024 of them a pass."""
     rng = np.random.default_rng(8)
@@ -268,11 +283,11 @@ def test_refusals_of_the_entry_points(hip):
         return C.byref(d)
 
     with pytest.raises(RuntimeError, match="16 bytes"):
-        nv.call("nhip_packed_fwd", desc(), one.ptr + 2, one.ptr, one.ptr, one.ptr, one.ptr, None, one.ptr)
+        nv.call("nhip_packed_fwd", desc(), one.ptr + 2, one.ptr, one.ptr, one.ptr, one.ptr, None, None, one.ptr)
     with pytest.raises(RuntimeError, match="workspace"):
-        nv.call("nhip_packed_fwd", desc(), one.ptr, one.ptr, one.ptr, one.ptr, one.ptr, None, None)
+        nv.call("nhip_packed_fwd", desc(), one.ptr, one.ptr, one.ptr, one.ptr, one.ptr, None, None, None)
     with pytest.raises(RuntimeError, match="workspace"):
-        nv.call("nhip_packed_bwd", desc(), *[one.ptr] * 10, None)
+        nv.call("nhip_packed_bwd", desc(), *[one.ptr] * 11, None)
     with pytest.raises(RuntimeError, match="head dim"):
-        nv.call("nhip_packed_fwd", desc(head_dim=12), one.ptr, one.ptr, one.ptr, one.ptr, one.ptr, None, one.ptr)
-    nv.call("nhip_packed_fwd", desc(tokens=0), None, None, None, None, None, None, None)  # nothing to do
+        nv.call("nhip_packed_fwd", desc(head_dim=12), one.ptr, one.ptr, one.ptr, one.ptr, one.ptr, None, None, one.ptr)
+    nv.call("nhip_packed_fwd", desc(tokens=0), None, None, None, None, None, None, None, None)  # nothing to do
