@@ -1,6 +1,7 @@
 """The benchmark workloads as lumen programs: the decoder-only transformer training step of configs 4 and 5
 (``examples/transformer.py`` style: pre-norm blocks, causal flash attention, a GELU FFN, a cross-entropy head,
-autograd backward and an SGD update inside one compiled function) and its synthetic inputs.
+autograd backward and an SGD update inside one compiled function) and its synthetic inputs; and the same model's step on
+documents packed one after another (``packed_train_step``), which pads nothing and whose head never holds its logits.
 
 Weights are bfloat16 (norm scales too), every dot accumulates in float32, and the norm statistics, softmax
 and loss are float32.
@@ -57,7 +58,9 @@ class Embedding(Module):
     tokens: L.Tensor
     positions: L.Tensor
 
-    def __call__(self, ids):
+    def __call__(self, ids, places=None):
+        if places is not None:  # of packed documents, [tokens]
+            return self.tokens[ids] + self.positions[places]
         b, s = ids.shape
         return (self.tokens[ids] + self.positions).reshape(b * s, self.tokens.shape[1])
 
@@ -69,13 +72,14 @@ class Attention(Module):
     wv: L.Tensor
     wo: L.Tensor
 
-    def __call__(self, x, batch, heads):
+    def __call__(self, x, batch, heads, offsets=None):
         tokens, dim = x.shape
+        rows = (batch, tokens // batch) if offsets is None else (tokens,)
         q, k, v = (
-            F.matmul(x, w.t(), "float32", "bfloat16").reshape(batch, tokens // batch, heads, dim // heads)
+            F.matmul(x, w.t(), "float32", "bfloat16").reshape(*rows, heads, dim // heads)
             for w in (self.wq, self.wk, self.wv)
         )
-        o = F.flash_attention(q, k, v, is_causal=True)
+        o = F.flash_attention(q, k, v, is_causal=True) if offsets is None else F.packed_attention(q, k, v, offsets)
         return F.matmul(o.reshape(tokens, dim), self.wo.t(), "float32", "bfloat16")
 
 
@@ -93,10 +97,10 @@ class Block(Module):
     attn: Attention
     mlp: MLP
 
-    def __call__(self, x, batch, heads):
+    def __call__(self, x, batch, heads, offsets=None):
         r = x
         x = F.rms_norm(x.float(), x.size(-1), self.attn.norm.float()).bfloat16()
-        x = r + self.attn(x, batch, heads)
+        x = r + self.attn(x, batch, heads, offsets)
         r = x
         x = F.rms_norm(x.float(), x.size(-1), self.mlp.norm.float()).bfloat16()
         return r + self.mlp(x)
@@ -109,10 +113,12 @@ class Transformer(Module):
     head: L.Tensor
     heads: int
 
-    def __call__(self, ids):
-        h = self.embed(ids)
+    def __call__(self, ids, places=None, offsets=None):
+        """The head's inputs ``[tokens, dim]`` of ``ids`` ``[batch, seq]``; or, with ``places`` and ``offsets``, of documents packed
+        one after another: ``ids`` and each token's place in its document ``[tokens]``, ``offsets`` as ``packed_attention``'s."""
+        h = self.embed(ids, places)
         for layer in self.layers:
-            h = layer(h, ids.shape[0], self.heads)
+            h = layer(h, ids.shape[0], self.heads, offsets)
         return F.rms_norm(h.float(), h.size(-1), self.norm.float()).bfloat16()
 
 
@@ -188,6 +194,33 @@ def train_step(model, opt, ids, targets):
     loss.backward()
     opt.step()
     return loss
+
+
+def packed_loss(model, ids, places, targets, offsets):
+    """The mean loss of the tokens of packed documents (``pack``) whose target is not ignored."""
+    return F.linear_cross_entropy(model(ids, places, offsets), model.head, targets)
+
+
+def packed_train_step(model, opt, ids, places, targets, offsets, max_norm=1.0):
+    """One ``AdamW`` step on packed documents, gradients clipped to ``max_norm``; returns the loss."""
+    loss = packed_loss(model, ids, places, targets, offsets)
+    loss.backward()
+    opt.step(max_norm=max_norm)
+    return loss
+
+
+def pack(documents, tokens):
+    """``(ids, places, targets, offsets)`` of the documents' token ids one after another in ``tokens`` tokens: a token's target is
+    the next one of its document, and ignored (-100) of a document's last and of the tokens behind them."""
+    offsets = np.cumsum([0, *map(len, documents)]).astype(np.int32)
+    if offsets[-1] > tokens:
+        raise ValueError(f"pack: documents of {offsets[-1]} tokens in {tokens}")
+    ids, places, targets = np.zeros(tokens, np.int64), np.zeros(tokens, np.int64), np.full(tokens, -100, np.int64)
+    for lo, doc in zip(offsets, documents):
+        hi = lo + len(doc)
+        ids[lo:hi], places[lo:hi] = doc, np.arange(len(doc))
+        targets[lo:max(hi - 1, lo)] = doc[1:]
+    return ids, places, targets, offsets
 
 
 def build(cfg: TransformerConfig, lr=1e-2):
