@@ -181,14 +181,20 @@ static __global__ __launch_bounds__(256) void head_merge_kernel(const float2 *__
     }
 }
 
-// scale[0]: what takes the largest |g| to `top` (1 where g is all zeros or not finite); scale[1]: one over it.
-static __global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restrict__ g, int64_t rows, float top, float *__restrict__ scale) {
+// scale[0]: what takes the largest |g| of the rows that count to `top` (1 where it is zero or not finite); scale[1]: one over it.
+static __global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restrict__ g, HeadTargets targets, int64_t rows, float top,
+                                                                 float *__restrict__ scale) {
     __shared__ float most[16];
     float m = 0.0f;
     for (int64_t i = threadIdx.x; i < rows; i += 4096) {
         float v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = i + 1024 * k < rows ? g[i + 1024 * k] : 0.0f;
+        for (int k = 0; k < 4; ++k) {
+            const int64_t r = i + 1024 * k;
+            bool ignored = true;
+            if (r < rows) targets.at(r, ignored);
+            v[k] = ignored ? 0.0f : g[r];
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) m = fmaxf(m, fabsf(v[k]));
     }

@@ -23,9 +23,10 @@ int64_t padded_k(const nhip_head_desc *d) { return up(d->k, 64); }
 // Rows of a piece: what fits the bytes that the desc allows for its codes, a multiple of 256 (a tile's), and pieces of one size.
 int64_t piece_rows(const nhip_head_desc *d) {
     const int64_t row = blocks_of(d) * 64 * 2;
-    // the weight gradient reads a piece's codes through one buffer of 2^31 bytes
-    const int64_t bytes = std::min(d->piece_bytes, (int64_t(1) << 31) - (int64_t(1) << 20));
-    const int64_t most = std::max<int64_t>(bytes / row / 256 * 256, 256);
+    // the weight gradient reads a piece's codes, and its rows of h, through a buffer of 2^31 bytes each
+    const int64_t buffer = (int64_t(1) << 31) - (int64_t(1) << 20);
+    const int64_t fit = std::min(std::min(d->piece_bytes, buffer) / row, buffer / (padded_k(d) * 2));
+    const int64_t most = std::max<int64_t>(fit / 256 * 256, 256);
     if (d->rows <= most) return d->rows;
     const int64_t pieces = (d->rows + most - 1) / most;
     return std::min(most, up((d->rows + pieces - 1) / pieces, 256));
@@ -82,10 +83,11 @@ int head_check(const nhip_head_desc *d, const char *what) {
     if (d->target_dtype != NHIP_LCE_I32 && d->target_dtype != NHIP_LCE_I64) return fail(at + ": targets must be int32 or int64");
     if (d->h_m < 0 || d->w_n < d->k) return fail(at + ": rows that lie backwards, or classes that overlap");
     const int64_t lim = (int64_t(1) << 30) - 1024, kp = padded_k(d);
-    if (kp >= int64_t(1) << 20 || d->h_m >= int64_t(1) << 20 || d->classes >= int64_t(1) << 22 ||
-        (d->classes + 256) * std::max(kp, d->w_n) >= lim)
+    if (kp >= int64_t(1) << 20 || d->classes >= int64_t(1) << 22 || (d->classes + 256) * std::max(kp, d->w_n) >= lim)
         return fail(at + ": rows below 2^20 elements, 2^22 classes, and a weight within 2^31 bytes");
-    if (d->rows >= int64_t(1) << 31 || tiles(d->rows, 128, d->classes, 128) >= int64_t(1) << 24 ||
+    if (d->h_m >= int64_t(1) << 40 || (!copies(d, d->h_m) && 256 * d->h_m + kp >= lim))
+        return fail(at + ": a tile's rows of h within 2^31 bytes");
+    if (d->rows >= int64_t(1) << 26 || tiles(d->rows, 128, d->classes, 128) >= int64_t(1) << 24 ||
         tiles(d->classes, 128, d->k, 128) >= int64_t(1) << 24 || tiles(d->rows, 128, d->k, 128) >= int64_t(1) << 24)
         return fail(at + ": a launch of 2^32 threads");
     if (d->piece_bytes < 0) return fail(at + ": negative sizes");
@@ -203,7 +205,7 @@ int head_run(hipStream_t st, const nhip_head_desc *d, const uint16_t *h, const u
         hipLaunchKernelGGL(head_merge_kernel, dim3(unsigned((d->rows + 3) / 4)), dim3(256), 0, st, part, picked, targets, d->rows, blocks, losses);
         return check(hipGetLastError(), "head_merge_kernel launch");
     }
-    hipLaunchKernelGGL(head_scale_kernel, dim3(1), dim3(1024), 0, st, g, d->rows, F16 ? 16384.0f : 1.0f, scale);
+    hipLaunchKernelGGL(head_scale_kernel, dim3(1), dim3(1024), 0, st, g, targets, d->rows, F16 ? 16384.0f : 1.0f, scale);
     if (check(hipGetLastError(), "head_scale_kernel launch")) return 1;
     const PartPlan pi = input_plan(d), pw = weight_plan(d);
     const int64_t most = piece_rows(d), pieces = pieces_of(d);

@@ -68,7 +68,7 @@ def _taken(h, w):
         return -(-m // 128) * -(-n // 128) < 1 << 24
 
     return h.dtype in ("bfloat16", "float16") and 0 < kp < 1 << 20 and 0 < v < 1 << 22 and (v + 256) * kp < (1 << 30) - 1024 \
-        and t < 1 << 31 and launch(t, v) and launch(v, k) and launch(t, k)
+        and t < 1 << 26 and launch(t, v) and launch(v, k) and launch(t, k)
 
 
 class _HeadLoss(Function):
@@ -114,7 +114,7 @@ def linear_cross_entropy(input, weight, target, ignore_index=-100, reduction="me
     the ``V`` classes. ``reduction``: ``"mean"`` over the rows that count (0 of none), ``"sum"``, or ``"none"``, a loss a row
     ``[...]``. Losses and all sums are float32 (float64 of float64 operands). The gradients of the logits are rounded to the
     operands' dtype as operands of the products that give those of ``input`` and ``weight``, which are rounded again. bfloat16
-    and float16 run as kernels of their own, which hold exponentials of at most ``config.compiler.head_piece_bytes`` at a time
+    and float16 (up to 2^26 rows and a weight below 2^30 elements) run as kernels of their own, which hold exponentials of at most ``config.compiler.head_piece_bytes`` at a time
     and take six products' work for both directions; other dtypes run as primitives, over whole logits."""
     op = "linear_cross_entropy"
     h, w, target = lift(input), lift(weight), lift(target)

@@ -60,6 +60,63 @@ def _check(got, h, w, target, g, dtype, what=""):
             _near(a, b, t, (what, name))
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_cotangents_of_ignored_rows_are_not_read_into_others(hip, dtype):
+    """However large, or NaN: the largest cotangent of the rows that count sets the gradients' scale."""
+    h, w, target, g = _case(21, 200, 64, 300, dtype)
+    target[:4] = IGNORED
+    f = L.compile(_program(), device="hip")
+    args = [_tensor(h, dtype), _tensor(w, dtype), L.from_numpy(target)]
+    want = [_values(a) for a in f(*args, L.from_numpy(np.where(target == IGNORED, 0, g).astype(np.float32)))]
+    _check(want, h, w, target, g, dtype)
+    for bad in (1e30, np.inf, np.nan):
+        odd = np.where(target == IGNORED, bad, g).astype(np.float32)
+        for a, b in zip(f(*args, L.from_numpy(odd)), want):
+            assert np.array_equal(_values(a), b)
+
+
+def test_rows_far_apart(hip):
+    """Rows of a view whose rows lie 2^21 elements apart, of whole k tiles (read in place where they are near) and not."""
+    for i, k in enumerate((64, 40)):
+        h, w, target, g = _case(22 + i, 9, k, 300, "bfloat16")
+        wide = np.zeros((9, 1 << 21), np.uint16)
+        wide[:, :k] = D.from_values(h.astype(np.float32), "bfloat16")
+
+        def fn(x, w, target, g):
+            h = x[:, :k]
+            losses, pull = L.vjp(lambda h, w: F.linear_cross_entropy(h, w, target, IGNORED, "none"), h, w)
+            return [losses, *pull(g)]
+
+        x = L.Tensor("bfloat16", wide.shape, "cpu", host=wide)
+        for program in (fn, lambda *xs: [F.linear_cross_entropy(xs[0][:, :k], xs[1], xs[2], IGNORED, "none")]):
+            out = L.compile(program, device="hip")(x, _tensor(w, "bfloat16"), L.from_numpy(target), L.from_numpy(g))
+            _check([_values(a) for a in out], h, w, target, g, "bfloat16", k)
+
+
+def test_rows_of_more_than_a_buffer(hip):
+    """140000 rows of 8192 are 2^31 bytes and more: the weight's gradient is that of the few rows that are not zero, at both ends and
+    around the boundary; a row of zeros has the loss log V."""
+    t, k, v = 140000, 8192, 64
+    at = np.array([0, 1, 69999, 70000, 131070, 131071, 131072, 139998, 139999])
+    h, w, target, g = _case(20, len(at), k, v, "bfloat16", ignored=0.0)
+    whole, targets, gs = np.zeros((t, k), np.uint16), np.zeros(t, np.int64), np.ones(t, np.float32)
+    whole[at], targets[at], gs[at] = D.from_values(h.astype(np.float32), "bfloat16"), target, g
+
+    def fn(h, w, target, g):
+        losses, pull = L.vjp(lambda w: F.linear_cross_entropy(h, w, target, IGNORED, "none"), w)
+        return [losses, *pull(g)]
+
+    f = L.compile(fn, device="hip")
+    x = L.Tensor("bfloat16", whole.shape, "cpu", host=whole)
+    losses, dw = (_values(a) for a in f(x, _tensor(w, "bfloat16"), L.from_numpy(targets), L.from_numpy(gs)))
+    want = M.linear_cross_entropy(h, w, target, IGNORED, g)
+    tol = M.linear_cross_entropy_tolerances(h, w, target, IGNORED, g, "bfloat16")
+    _near(losses[at], want[0], tol[0], "losses")
+    _near(dw, want[2], tol[2], "dw")
+    rest = np.delete(losses, at)
+    assert np.abs(rest - np.log(v)).max() <= 4 * 2.0**-24 * np.log(v) + 64 * 2.0**-24
+
+
 CASES = [
     # rows, k, classes, dtype: one row, one class, one element; ragged ones; tiles of 128 and of 256 rows; parts of k
     (1, 64, 64, "bfloat16"), (1, 8, 1, "float16"), (5, 1, 3, "bfloat16"), (3, 64, 5003, "bfloat16"), (777, 520, 5003, "float16"),

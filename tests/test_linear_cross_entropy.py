@@ -187,3 +187,14 @@ def test_workspace_and_pieces():
     assert workspace(8192, 256 * row) < 8192 * row / 8 + 2 * sums
     assert workspace(8192, 256 * row) > 256 * row + sums
     assert workspace(8192, 1 << 30, 0) < 8192 * row / 8
+
+
+def test_a_piece_holds_rows_of_h_within_a_buffer():
+    """Few classes and long rows: the codes of 2^18 rows are 2^29 bytes, which one piece may hold, but their rows of h are 2^32, twice
+    what the weight gradient's product reaches: three pieces."""
+    n = C.c_size_t()
+    rows, k, v = 1 << 18, 1 << 13, 1000
+    d = nv.HeadDesc(rows=rows, classes=v, k=k, h_m=k, w_n=k, ignore_index=-100, piece_bytes=1 << 29, dtype=1, target_dtype=0)
+    nv.call("nhip_head_loss_workspace", C.byref(d), 1, C.byref(n))
+    copy, sums, codes = rows * k * 2, v * k * 4, rows * 1024 * 2
+    assert copy + sums + codes / 3 < n.value < copy + sums + codes / 2
