@@ -390,37 +390,52 @@ def losses_with_gradients(graph: Graph) -> Graph:
     for n in graph.nodes:
         if n.prim == "fusion" and n.params["name"] == "head_loss":
             forward.setdefault((n.inputs, n.params["ignore"]), n)
+    if not forward:
+        return graph
     depends = {}  # value -> the losses that it depends on
+    pairs, needs = {}, {}  # loss -> the gradients that it is to come from, and the losses that these depend on
 
-    def roots(v):
-        return depends.get(v, frozenset())
+    def from_gradients(loss, target):
+        """Whether `loss` is `target` or comes to depend on it by the pairs that there are."""
+        seen, todo = set(), [loss]
+        while todo:
+            v = todo.pop()
+            if v == target:
+                return True
+            if v not in seen:
+                seen.add(v)
+                todo += needs.get(v, ())
+        return False
 
-    pairs = {}
     for n in graph.nodes:
-        found = frozenset().union(*(roots(v) for v in n.inputs)) if n.inputs else frozenset()
+        found = frozenset().union(*(depends.get(v, ()) for v in n.inputs))
         if n.prim == "fusion" and n.params["name"] == "head_loss":
             found |= {n.output}
         elif n.prim == "fusion" and n.params["name"] == "head_loss_backward":
             f = forward.get((n.inputs[:3], n.params["ignore"]))
-            if f is not None and f.output not in found and f.output not in pairs and not any(f.output in roots(v) for v in n.inputs):
-                pairs[f.output] = n
+            if f is not None and f.output not in pairs and not any(from_gradients(v, f.output) for v in found):
+                pairs[f.output], needs[f.output] = n, found
         if found:
             depends[n.output] = found
     if not pairs:
         return graph
-    gone = set(pairs)
-    # what depends on a loss that is taken over comes after everything else
-    late = [n for n in graph.nodes if roots(n.output) & gone and n.output not in gone]
-    rest = [n for n in graph.nodes if not roots(n.output) & gone]
     g = Graph()
     remap = {v: g.input(graph.types[v].dtype, graph.types[v].shape) for v in graph.inputs}
     by_gradients = {b.output: v for v, b in pairs.items()}
-    for n in rest + late:
-        remap[n.output] = g.add_node(n.prim, tuple(remap[v] for v in n.inputs), n.params, graph.types[n.output], n.backward)
-        if n.output in by_gradients:
-            loss = by_gradients[n.output]
-            ty = graph.types[loss]
-            remap[loss] = g.add_node("fusion_output", (remap[n.output],), {"index": 2, "ty": ty}, ty, n.backward)
+    # what depends on a loss that is taken over comes after everything else
+    waiting = [n for n in graph.nodes if n.output not in pairs]
+    while waiting:
+        later = []
+        for n in waiting:
+            if not all(v in remap for v in n.inputs):
+                later.append(n)
+                continue
+            remap[n.output] = g.add_node(n.prim, tuple(remap[v] for v in n.inputs), n.params, graph.types[n.output], n.backward)
+            if n.output in by_gradients:
+                loss = by_gradients[n.output]
+                ty = graph.types[loss]
+                remap[loss] = g.add_node("fusion_output", (remap[n.output],), {"index": 2, "ty": ty}, ty, n.backward)
+        waiting = later
     g.set_outputs([remap[v] for v in graph.outputs])
     return g
 

@@ -10,6 +10,7 @@ import lumen_amd as L
 import lumen_amd.functional as F
 from lumen_amd import native as nv
 from lumen_amd.compiler.plan import Plan, compile_graph
+from lumen_amd.graph import prims
 from oracle import oracle
 from tests import training_math as M
 
@@ -146,6 +147,20 @@ def test_plans():
         return [a, b, *pa(a * 0.0 + 1.0), *pb(a)]
 
     assert kinds(_graph(two, g=None)) == ["head_loss", "head_loss_backward", "head_loss_backward"]
+
+    def crossed(h, w, t):  # the cotangent of each is the other's loss: one of them comes first
+        a, pa = L.vjp(lambda h, w: F.linear_cross_entropy(h, w, t, 1), h, w)
+        b, pb = L.vjp(lambda h, w: F.linear_cross_entropy(h, w, t, 2), h, w)
+        return [a, b, *pa(b), *pb(a)]
+
+    assert kinds(_graph(crossed, g=None)) == ["head_loss", "head_loss_backward", "head_loss_backward"]
+
+    def chained(h, w, t):  # the second's cotangent depends on the first's loss alone
+        a, pa = L.vjp(lambda h, w: F.linear_cross_entropy(h, w, t, 1), h, w)
+        b, pb = L.vjp(lambda h, w: F.linear_cross_entropy(h, w, t, 2), h, w)
+        return [a * b, *pb(a), *pa(prims.full((), 1.0, "float32"))]
+
+    assert kinds(_graph(chained, g=None)) == ["head_loss_backward"] * 2
     for dtype in ("float32", "float64"):
         assert not kinds(_graph(_program("none"), dtype=dtype, g=(dtype, None)))
     with L.config.compiler.patch(fused_operators=False):
@@ -166,12 +181,20 @@ def test_the_joined_step_keeps_its_values():
         dh, dw = pull(F.sum(h.float()) * 0.0 + 1.0)
         return [loss * 3.0, dh, dw.float() * loss]
 
-    graph = L.make_graph(fn)(_meta(h, "bfloat16"), _meta(w, "bfloat16"), _meta(target))
-    compiled, _ = compile_graph(graph)
+    def two(h, w, t, crossed):
+        a, pa = L.vjp(lambda h, w: F.linear_cross_entropy(h, w, t, 1), h, w)
+        b, pb = L.vjp(lambda h, w: F.linear_cross_entropy(h, w, t, 2), h, w)
+        late = a * b
+        return [late * 2.0, *pb(a), *pa(b if crossed else prims.full((), 1.0, "float32")), late]
+
     args = [D.bf16_bits(b) for b in bits] + [target]
-    assert [n.params["name"] for n in compiled.nodes if n.prim == "fusion"] == ["head_loss_backward"]
-    for a, b in zip(oracle.values(graph, args), oracle.values(compiled, args)):
-        assert np.array_equal(a, b)
+    for program, names in ((fn, ["head_loss_backward"]), (lambda *xs: two(*xs, False), ["head_loss_backward"] * 2),
+                           (lambda *xs: two(*xs, True), ["head_loss", "head_loss_backward", "head_loss_backward"])):
+        graph = L.make_graph(program)(_meta(h, "bfloat16"), _meta(w, "bfloat16"), _meta(target))
+        compiled, _ = compile_graph(graph)
+        assert [n.params["name"] for n in compiled.nodes if n.prim == "fusion"] == names
+        for a, b in zip(oracle.values(graph, args), oracle.values(compiled, args)):
+            assert np.array_equal(a, b)
 
 
 def test_workspace_and_pieces():
