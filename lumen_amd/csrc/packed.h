@@ -57,14 +57,17 @@ __device__ __forceinline__ T packed_wave_sum(T v, int lane) {
     return v;
 }
 
-// The entries behind the `placed` tiles: tokens of no sequence, then nothing.
-__device__ __forceinline__ void packed_rest(const PackedTable &t, int placed, int first, int last, int tokens) {
-    const int lead = (first + t.block - 1) / t.block, tail = (tokens - last + t.block - 1) / t.block;
-    for (int i = placed + threadIdx.x; i < t.most; i += blockDim.x) {
-        int j = i - placed, from = j * t.block, to = first;
-        if (j >= lead) from = last + (j - lead) * t.block, to = j < lead + tail ? tokens : from;
-        t.tiles[i] = PackedTile{from < tokens ? from : 0, min(max(to - from, 0), t.block), -1, 0};
-    }
+// Entry j behind the tiles: tokens of no sequence, then nothing.
+__device__ __forceinline__ PackedTile packed_rest(int block, int j, int first, int last, int tokens) {
+    const int lead = (first + block - 1) / block, tail = (tokens - last + block - 1) / block;
+    int from = j * block, to = first;
+    if (j >= lead) from = last + (j - lead) * block, to = j < lead + tail ? tokens : from;
+    return PackedTile{from < tokens ? from : 0, min(max(to - from, 0), block), -1, 0};
+}
+
+__device__ __forceinline__ int packed_offset(const PackedTables &a, int64_t i) {
+    const int64_t v = a.o64 ? static_cast<const int64_t *>(a.offsets)[i] : static_cast<const int32_t *>(a.offsets)[i];
+    return int(v < 0 ? 0 : v > a.tokens ? a.tokens : v);
 }
 
 // One workgroup a table. Offsets are clamped into [the one before, tokens], so that whatever they hold every tile lies within
@@ -80,12 +83,8 @@ static __global__ __launch_bounds__(kPackedBuckets) void packed_tiles_kernel(Pac
     const PackedTable t = a.t[blockIdx.x];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int tokens = int(a.tokens);
-    auto offset = [&](int64_t i) {
-        const int64_t v = a.o64 ? static_cast<const int64_t *>(a.offsets)[i] : static_cast<const int32_t *>(a.offsets)[i];
-        return int(v < 0 ? 0 : v > tokens ? tokens : v);
-    };
     bucket[tid] = 0;
-    const int first = offset(0);
+    const int first = packed_offset(a, 0);
     int last = first;
     for (int pass = 0; pass < 2; ++pass) {
         int carry = 0;
@@ -94,7 +93,7 @@ static __global__ __launch_bounds__(kPackedBuckets) void packed_tiles_kernel(Pac
             const int here = int(min(a.sequences - base, int64_t(kPackedBuckets)));
             __syncthreads();  // the chunk before is done with `at` (and `bucket` is cleared)
             // offsets base .. base + here, each at least the one before
-            int v = packed_wave_max(tid <= here ? offset(base + tid) : 0, lane);
+            int v = packed_wave_max(tid <= here ? packed_offset(a, base + tid) : 0, lane);
             if (lane == 63) waves[wave] = v;
             __syncthreads();
             int before = carry;
@@ -102,7 +101,7 @@ static __global__ __launch_bounds__(kPackedBuckets) void packed_tiles_kernel(Pac
             v = max(v, before);
             at[tid] = v;
             __syncthreads();
-            if (tid == 0) at[kPackedBuckets] = here == kPackedBuckets ? max(at[kPackedBuckets - 1], offset(base + here)) : 0;
+            if (tid == 0) at[kPackedBuckets] = here == kPackedBuckets ? max(at[kPackedBuckets - 1], packed_offset(a, base + here)) : 0;
             __syncthreads();
             carry = at[here];
             const int len = tid < here ? at[tid + 1] - at[tid] : 0;
@@ -147,26 +146,21 @@ static __global__ __launch_bounds__(kPackedBuckets) void packed_tiles_kernel(Pac
         for (int w = 0; w < wave; ++w) place += waves[w];
         bucket[tid] = place;
     }
-    packed_rest(t, bucket[kPackedBuckets - 1], first, last, tokens);  // where the last amount's tiles end
+    const int placed = bucket[kPackedBuckets - 1];  // where the last amount's tiles end
+    for (int i = placed + tid; i < t.most; i += kPackedBuckets) t.tiles[i] = packed_rest(t.block, i - placed, first, last, tokens);
 }
 
 // The same for fewer sequences than threads, without atomics: a tile's place is the tiles of more work, which are those of every
 // sequence's blocks past its own work, and the sequences before its own that have as many blocks (3 sequences of 97 tokens: 3.2 us,
-// 8.7 by amounts; 8 of 16384: 5.0, 11.5 by
-// amounts).
+// 8.7 by amounts; 8 of 16384: 5.0, 11.5).
 constexpr int kPackedFew = 256;
-static __global__ __launch_bounds__(kPackedFew) void packed_tiles_few_kernel(PackedTables a) {
+__device__ __forceinline__ void packed_tiles_few(const PackedTables &a, int table) {
     __shared__ int at[kPackedFew + 1], before[kPackedFew + 1], ds_at[kPackedFew];
     __shared__ __align__(16) int blocks[kPackedFew];
     __shared__ int waves[3][4];
-    const PackedTable t = a.t[blockIdx.x];
+    const PackedTable t = a.t[table];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, tokens = int(a.tokens), count = int(a.sequences);
-    int v = 0;
-    if (tid <= count) {
-        const int64_t x = a.o64 ? static_cast<const int64_t *>(a.offsets)[tid] : static_cast<const int32_t *>(a.offsets)[tid];
-        v = int(x < 0 ? 0 : x > tokens ? tokens : x);
-    }
-    v = packed_wave_max(v, lane);
+    int v = packed_wave_max(tid <= count ? packed_offset(a, tid) : 0, lane);
     if (lane == 63) waves[0][wave] = v;
     __syncthreads();
     for (int w = 0; w < wave; ++w) v = max(v, waves[0][w]);
@@ -189,7 +183,7 @@ static __global__ __launch_bounds__(kPackedFew) void packed_tiles_few_kernel(Pac
     before[tid] = from;
     ds_at[tid] = ds_from;  // read only where all fit
     const int first = at[0], last = at[count];
-    if (a.fits && tid == 0 && blockIdx.x == 0) a.fits[0] = ds_total <= a.ds_tiles, a.fits[1] = first, a.fits[2] = last;
+    if (a.fits && tid == 0 && table == 0) a.fits[0] = ds_total <= a.ds_tiles, a.fits[1] = first, a.fits[2] = last;
     __syncthreads();
     for (int i = tid; i < total; i += kPackedFew) {
         int k = 0, hi = count;
@@ -212,7 +206,23 @@ static __global__ __launch_bounds__(kPackedFew) void packed_tiles_few_kernel(Pac
         }
         t.tiles[place] = PackedTile{at[k], at[k + 1] - at[k], j, ds_at[k]};
     }
-    packed_rest(t, total, first, last, tokens);
+    for (int i = total + tid; i < t.most; i += kPackedFew) t.tiles[i] = packed_rest(t.block, i - total, first, last, tokens);
+}
+static __global__ __launch_bounds__(kPackedFew) void packed_tiles_few_kernel(PackedTables a) { packed_tiles_few(a, int(blockIdx.x)); }
+
+// The tile of entry `idx` of a table of fewer sequences than lanes, in the sequences' order, without a table: where a launch's
+// workgroups all run at once nothing is gained by the order (97 tokens, 16 heads: 8.2 us a call, 10.9 with a table).
+constexpr int kPackedDirect = 63;
+__device__ __forceinline__ PackedTile packed_tile(const PackedTables &a, int block, int idx) {
+    const int lane = threadIdx.x & 63, count = int(a.sequences);
+    const int v = packed_wave_max(lane <= count ? packed_offset(a, lane) : 0, lane);
+    const int next = __shfl_down(v, 1, 64), len = lane < count ? next - v : 0, own = (len + block - 1) / block;
+    const int before = packed_wave_sum(own, lane) - own;
+    const int first = __builtin_amdgcn_readlane(v, 0), last = __builtin_amdgcn_readlane(v, count),
+              total = __builtin_amdgcn_readlane(before, count);
+    if (idx >= total) return packed_rest(block, idx - total, first, last, int(a.tokens));
+    const int k = 63 - __builtin_clzll(__ballot(lane < count && before <= idx));
+    return PackedTile{__builtin_amdgcn_readlane(v, k), __builtin_amdgcn_readlane(len, k), idx - __builtin_amdgcn_readlane(before, k), 0};
 }
 
 // The head and table entry of a workgroup: heads fastest, in runs that stay on one XCD (workgroups go round the eight) where
@@ -237,10 +247,11 @@ __device__ __forceinline__ void packed_sequence(AttnParams &p, const PackedTile 
 
 template <int D, bool F16, bool CAUSAL, int NW>
 __global__ __launch_bounds__(64 * NW, (FwdOccupancy<NW, D>::kBlocks)) void packed_fwd_kernel(AttnParams p, uint16_t *rest,
-                                                                                             const PackedTile *tiles, int64_t tokens) {
+                                                                                             PackedTables a) {
     int64_t n, idx;
     packed_place(p.heads, n, idx);
-    const PackedTile t = tiles[idx];
+    const PackedTile t = a.t[0].tiles ? a.t[0].tiles[idx] : packed_tile(a, 32 * NW, int(idx));
+    const int64_t tokens = a.tokens;
     const int64_t rest_s = p.heads * p.hdv;
     if (t.block < 0) {
         packed_zeros(p.o + n * p.o_n, p.o_s, p.hdv, t);
@@ -257,12 +268,18 @@ __global__ __launch_bounds__(64 * NW, (FwdOccupancy<NW, D>::kBlocks)) void packe
 // delta = rowsum(dO O) scale and lse log2 e of every token, those of no sequence too (nothing reads theirs): D / 8 lanes a row
 // of 16 bytes each. O is taken with what its rounding left (rest, [tokens, heads, hdv], or null): without it the error of O is in
 // every dS of a row alike, and of rows of few keys is as much as dS's own rounding: the gradients of sequences of 2 to 8 tokens
-// were off by 3.1e-3 of their length (2.5e-3 with it, 1.7e-3 being their rounding), of 64 to 90 by 2.6e-3 (2.4e-3).
+// were off by 3.1e-3 of their length (2.5e-3 with it, 1.7e-3 being their rounding), of 64 to 90 by 2.6e-3 (2.4e-3). The first
+// `tables` workgroups build the tables meanwhile (packed_tiles_few): a launch less (5120 tokens, 8 heads, dims 64: 5.3 us for
+// both, 9.6 apart).
 template <int D, bool F16>
-__global__ __launch_bounds__(256) void packed_prep_kernel(AttnParams p, const uint16_t *rest, float *lse2) {
+__global__ __launch_bounds__(256) void packed_prep_kernel(AttnParams p, const uint16_t *rest, float *lse2, PackedTables a, int tables) {
+    if (int(blockIdx.x) < tables) {
+        packed_tiles_few(a, int(blockIdx.x));
+        return;
+    }
     constexpr int LPR = D / 8;
     const int sub = threadIdx.x % LPR;
-    const int64_t row = int64_t(blockIdx.x) * (256 / LPR) + threadIdx.x / LPR;  // of [heads, tokens]
+    const int64_t row = (int64_t(blockIdx.x) - tables) * (256 / LPR) + threadIdx.x / LPR;  // of [heads, tokens]
     const bool live = row < p.heads * p.sq;
     const int64_t n = live ? row / p.sq : 0, q = live ? row % p.sq : 0;
     float acc = 0.0f;

@@ -16,18 +16,21 @@ constexpr int64_t kPackedTokens = int64_t(1) << 26, kPackedSequences = int64_t(1
 int64_t value_dim(const nhip_packed_desc *d) { return d->value_head_dim ? d->value_head_dim : d->head_dim; }
 int64_t kernel_dim(const nhip_packed_desc *d) { return std::max(d->head_dim, value_dim(d)) <= 64 ? 64 : 128; }
 
-// Queries a forward workgroup takes.
-int64_t fwd_block(const nhip_packed_desc *d) {
-    (void)d;
-    return 128;
-}
-constexpr int64_t kKeyBlock = 128, kDqBlock = 256;
+// Queries a forward workgroup takes, and keys and queries the backward's.
+constexpr int64_t kFwdBlock = 128, kKeyBlock = 128, kDqBlock = 256;
 
 // Entries of a table: the most workgroups that any offsets give.
 int64_t table_entries(const nhip_packed_desc *d, int64_t block) {
     return d->tokens / block + std::min(d->sequences, d->tokens) + 2;
 }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+bool few(const nhip_packed_desc *d) { return d->sequences < kPackedFew; }
+// Whether the forward's workgroups find their tiles themselves: all run at once.
+bool direct(const nhip_packed_desc *d) {
+    constexpr int64_t CUS = 256;
+    const int64_t at_once = CUS * (kernel_dim(d) == 64 ? FwdOccupancy<4, 64>::kBlocks : FwdOccupancy<4, 128>::kBlocks);
+    return d->sequences <= kPackedDirect && table_entries(d, kFwdBlock) * d->heads <= at_once;
+}
 size_t table_bytes(const nhip_packed_desc *d, int64_t block) { return up256(table_entries(d, block) * sizeof(PackedTile)); }
 
 // The most dS tiles of a head that any offsets give: ceil(l / 128) ceil(l / 64) over lengths l that add up to the tokens.
@@ -116,17 +119,22 @@ PackedTable table(const nhip_packed_desc *d, int64_t block, int order, void *til
     return t;
 }
 
-int build_tables(hipStream_t st, const nhip_packed_desc *d, const void *offsets, PackedTables a, int count) {
+PackedTables tables_of(const nhip_packed_desc *d, const void *offsets) {
+    PackedTables a{};
     a.offsets = offsets, a.sequences = d->sequences, a.tokens = d->tokens, a.o64 = d->offsets_dtype == NHIP_POS_I64;
-    if (d->sequences < kPackedFew) hipLaunchKernelGGL(packed_tiles_few_kernel, dim3(unsigned(count)), dim3(kPackedFew), 0, st, a);
+    return a;
+}
+
+int build_tables(hipStream_t st, const nhip_packed_desc *d, const PackedTables &a, int count) {
+    if (few(d)) hipLaunchKernelGGL(packed_tiles_few_kernel, dim3(unsigned(count)), dim3(kPackedFew), 0, st, a);
     else hipLaunchKernelGGL(packed_tiles_kernel, dim3(unsigned(count)), dim3(kPackedBuckets), 0, st, a);
     return check(hipGetLastError(), "packed_tiles_kernel launch");
 }
 
 template <int D, bool F16, bool CAUSAL>
-int fwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, uint16_t *rest, const PackedTable &t) {
-    const dim3 grid(unsigned(t.most * d->heads));
-    hipLaunchKernelGGL((packed_fwd_kernel<D, F16, CAUSAL, 4>), grid, dim3(256), 0, st, p, rest, t.tiles, d->tokens);
+int fwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, uint16_t *rest, const PackedTables &a) {
+    const dim3 grid(unsigned(a.t[0].most * d->heads));
+    hipLaunchKernelGGL((packed_fwd_kernel<D, F16, CAUSAL, kFwdBlock / 32>), grid, dim3(256), 0, st, p, rest, a);
     return check(hipGetLastError(), "packed_fwd_kernel launch");
 }
 
@@ -146,7 +154,9 @@ int bwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, const ui
         float *sums) {
     float *lse2 = p.delta + size_t(d->heads) * d->tokens;
     constexpr int RPB = 256 / (D / 8);
-    hipLaunchKernelGGL((packed_prep_kernel<D, F16>), dim3(unsigned((d->heads * d->tokens + RPB - 1) / RPB)), dim3(256), 0, st, p, rest, lse2);
+    const int tables = few(d) ? 2 : 0;
+    hipLaunchKernelGGL((packed_prep_kernel<D, F16>), dim3(unsigned((d->heads * d->tokens + RPB - 1) / RPB + tables)), dim3(256), 0, st, p, rest,
+                       lse2, a, tables);
     if (check(hipGetLastError(), "packed delta launch")) return 1;
     const dim3 gq(unsigned(a.t[1].most * d->heads));
     const int32_t *fits = store && again ? a.fits : nullptr;
@@ -179,13 +189,13 @@ int packed_fwd_on(hipStream_t st, const nhip_packed_desc *d, const void *q, cons
     p.q = static_cast<const uint16_t *>(q), p.k = static_cast<const uint16_t *>(k), p.v = static_cast<const uint16_t *>(v);
     p.o = static_cast<uint16_t *>(o), p.lse = lse;
     uint16_t *left = static_cast<uint16_t *>(rest);
-    PackedTables a{};
-    a.t[0] = table(d, fwd_block(d), PACKED_RISING, ws);
-    if (build_tables(st, d, offsets, a, 1)) return 1;
+    PackedTables a = tables_of(d, offsets);
+    a.t[0] = table(d, kFwdBlock, PACKED_RISING, direct(d) ? nullptr : ws);
+    if (a.t[0].tiles && build_tables(st, d, a, 1)) return 1;
     const bool f16 = d->dtype == NHIP_F16;
 #define NHIP_PACKED(DD)                                                                                      \
-    return f16 ? (d->causal ? fwd<DD, true, true>(st, d, p, left, a.t[0]) : fwd<DD, true, false>(st, d, p, left, a.t[0])) \
-               : (d->causal ? fwd<DD, false, true>(st, d, p, left, a.t[0]) : fwd<DD, false, false>(st, d, p, left, a.t[0]))
+    return f16 ? (d->causal ? fwd<DD, true, true>(st, d, p, left, a) : fwd<DD, true, false>(st, d, p, left, a)) \
+               : (d->causal ? fwd<DD, false, true>(st, d, p, left, a) : fwd<DD, false, false>(st, d, p, left, a))
     if (kernel_dim(d) == 64) NHIP_PACKED(64);
     NHIP_PACKED(128);
 #undef NHIP_PACKED
@@ -208,12 +218,12 @@ int packed_bwd_on(hipStream_t st, const nhip_packed_desc *d, const void *q, cons
     float *sums = reinterpret_cast<float *>(at + w.sums);
     const int64_t room = ds_room(d);
     const bool store = room > 0, again = room < most_ds(d);
-    PackedTables a{};
+    PackedTables a = tables_of(d, offsets);
     a.t[0] = table(d, kKeyBlock, PACKED_FALLING, at + w.keys);
     a.t[1] = table(d, kDqBlock, PACKED_RISING, at + w.queries);
     a.ds_tiles = room;
     a.fits = reinterpret_cast<int32_t *>(at + w.flag);
-    if (build_tables(st, d, offsets, a, 2)) return 1;
+    if (!few(d) && build_tables(st, d, a, 2)) return 1;  // else the workgroups of bwd()'s first launch do
     const bool f16 = d->dtype == NHIP_F16;
 #define NHIP_PACKED(DD)                                                                                                             \
     return f16 ? (d->causal ? bwd<DD, true, true>(st, d, p, left, a, store, again, sums) : bwd<DD, true, false>(st, d, p, left, a, store, again, sums)) \
@@ -243,7 +253,7 @@ int nhip_packed_bwd(const nhip_packed_desc *desc, const void *q, const void *k, 
 
 int nhip_packed_workspace(const nhip_packed_desc *desc, int backward, size_t *bytes) {
     if (packed_check(desc, "nhip_packed_workspace")) return 1;
-    *bytes = backward ? bwd_space(desc).bytes : table_bytes(desc, fwd_block(desc));
+    *bytes = backward ? bwd_space(desc).bytes : table_bytes(desc, kFwdBlock);
     return 0;
 }
 

@@ -145,18 +145,21 @@ def test_ds_that_does_not_fit(hip, limit):
                 _near(_values(a), w, tt, (lengths, name))
 
 
-@pytest.mark.parametrize("lengths,n,nkv,d,dtype", [([700, 1, 385, 214], 32, 16, 64, "bfloat16"), ([129, 900, 0, 300], 16, 16, 128, "float16")])
+@pytest.mark.parametrize("lengths,n,nkv,d,dtype,causal", [
+    ([700, 1, 385, 214], 32, 16, 64, "bfloat16", True), ([129, 900, 0, 300], 16, 16, 128, "float16", True),
+    ([129, 130, 0, 300, 257], 64, 16, 64, "bfloat16", False), ([513, 1, 0, 200, 64], 48, 24, 128, "bfloat16", True)])
 @pytest.mark.parametrize("limit", [0, 60, 1000])
-def test_heads_enough_for_whole_key_blocks(hip, lengths, n, nkv, d, dtype, limit):
-    """So many key blocks that none is done in parts: dS computed again, stored if it fits (it does not), and stored."""
+def test_heads_enough_for_whole_key_blocks(hip, lengths, n, nkv, d, dtype, causal, limit):
+    """So many key blocks that none is done in parts: dS computed again, stored if it fits (it does not), and stored. With the most
+    heads the forward's workgroups do not all run at once, and a table orders them."""
     rng = np.random.default_rng(12)
-    offsets = M.offsets_of(lengths)
-    t = int(offsets[-1])
+    offsets = M.offsets_of(lengths, 2)
+    t = int(offsets[-1]) + 131
     x = {k: _round(v, dtype) for k, v in M.packed_inputs(rng, t, n, nkv, d).items()}
-    want, tol = M.packed(x, offsets, True, d**-0.5, dtype)
+    want, tol = M.packed(x, offsets, causal, d**-0.5, dtype)
     args = [_tensor(x[k], dtype) for k in "qkv"] + [L.from_numpy(offsets), _tensor(x["do"], dtype)]
     with L.config.compiler.patch(attention_ds_max_bytes=limit * n * 128 * 64 * 2, attention_store_ds=limit > 0):
-        f = L.compile(_program(True), device="hip")
+        f = L.compile(_program(causal), device="hip")
         for name, a, w, tt in zip(("o", "dq", "dk", "dv"), f(*args), want, tol):
             _near(_values(a), w, tt, name)
 
