@@ -12,7 +12,7 @@
 // what a bf16 p would be) down to 2^-29, by 2^-40 below. d is then rounded once, to the operands'
 // type, which the matrix instructions take, with the largest |g| taken to 1 (bf16: a mean's 1 / t would be rounded the
 // same way in every row whose p is near 0, a gradient 2^-9 too long) or 2^14 (float16, whose range a mean's p would leave), and
-// the products are multiplied by what it was (head_scale_kernel).
+// the products are multiplied by what it was (head_scale).
 // Sums are float32; over classes of a row first float32 in blocks of 64, then float64.
 #pragma once
 
@@ -148,65 +148,103 @@ __global__ __launch_bounds__(TM * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 // exp(x) of a block's or a wave's maximum less a larger one.
 __device__ __forceinline__ float head_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 
-// The maximum of a row's block maxima and the float64 sum of exp(l - maximum) over lanes that take a block each `step`: every
-// lane of the wavefront has both.
-__device__ __forceinline__ void head_row(const float2 *__restrict__ p, int64_t first, int64_t step, int64_t blocks, float &m, double &sum) {
-    m = -INFINITY;
-    for (int64_t j = first; j < blocks; j += step) m = fmaxf(m, p[j].x);
+// A row's log-sum-exp from its blocks' maxima and sums, by a workgroup: float64 from the blocks on.
+__device__ __forceinline__ double head_lse(const float2 *__restrict__ p, int64_t blocks) {
+    __shared__ float most[4];
+    __shared__ double sums[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float m = -INFINITY;
+    for (int64_t j = threadIdx.x; j < blocks; j += 256) m = fmaxf(m, p[j].x);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    sum = 0.0;
-    for (int64_t j = first; j < blocks; j += step) {
+    double sum = 0.0;
+    for (int64_t j = threadIdx.x; j < blocks; j += 256) {
         const float2 q = p[j];
         if (q.x != -INFINITY) sum += double(q.y) * double(head_exp(q.x - m));
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) most[wave] = m, sums[wave] = sum;
+    __syncthreads();
+    const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (most[i] != -INFINITY) sum += sums[i] * double(head_exp(most[i] - top));
+    return double(top) + log(sum);
 }
 
-// The losses alone: one wavefront a row.
+// The losses alone. A workgroup a row: 512 rows of 500 blocks 4.2 us (6.3 by a wavefront a row).
 static __global__ __launch_bounds__(256) void head_merge_kernel(const float2 *__restrict__ part, const float *__restrict__ picked,
                                                                 HeadTargets targets, int64_t rows, int64_t blocks,
                                                                 float *__restrict__ losses) {
-    const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (row >= rows) return;  // the whole wavefront
-    float m;
-    double sum;
-    head_row(part + row * blocks, lane, 64, blocks, m, sum);
-    if (lane == 0) {
-        bool ignored;
-        targets.at(row, ignored);
-        losses[row] = ignored ? 0.0f : float(double(m) + log(sum) - double(picked[row]));
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const double lse = head_lse(part + row * blocks, blocks);
+        if (threadIdx.x == 0) {
+            bool ignored;
+            targets.at(row, ignored);
+            losses[row] = ignored ? 0.0f : float(lse - double(picked[row]));
+        }
+        __syncthreads();  // head_lse's LDS is read
+    }
+}
+
+// Rows of any length, alignment or distance as the products read them: copied to rows of kp elements, zeros past k. `mask`: zeros
+// in ignored rows too, whose d of 0 times a NaN or an infinity of theirs would be no 0 in dw.
+constexpr int kPrepare = 1024;  // threads
+struct HeadCopy {
+    const uint16_t *src;
+    int64_t rows, ld, k, kp;
+    uint16_t *dst;
+    int32_t mask, groups;  // workgroups: 0 if nothing is copied
+};
+__device__ __forceinline__ void head_copy(const HeadCopy &c, const HeadTargets &targets, int group) {
+    const int64_t per = c.kp / 8, total = c.rows * per;
+    for (int64_t i = int64_t(group) * kPrepare + threadIdx.x; i < total; i += int64_t(c.groups) * kPrepare) {
+        const int64_t row = i / per, col = (i - row * per) * 8;
+        bool ignored = false;
+        if (c.mask) targets.at(row, ignored);
+        *reinterpret_cast<uint4 *>(c.dst + row * c.kp + col) =
+            col < c.k && !ignored ? load8_any(c.src + row * c.ld + col, c.k - col) : make_uint4(0, 0, 0, 0);
     }
 }
 
 // scale[0]: what takes the largest |g| of the rows that count to `top` (1 where it is zero or not finite); scale[1]: one over it.
-static __global__ __launch_bounds__(1024) void head_scale_kernel(const float *__restrict__ g, HeadTargets targets, int64_t rows, float top,
-                                                                 float *__restrict__ scale) {
-    __shared__ float most[16];
+__device__ __forceinline__ void head_scale(const float *__restrict__ g, const HeadTargets &targets, int64_t rows, float top,
+                                           float *__restrict__ scale) {
+    __shared__ float most[kPrepare / 64];
     float m = 0.0f;
-    for (int64_t i = threadIdx.x; i < rows; i += 4096) {
-        float v[4];
+    constexpr int FLIGHT = 8;
+    for (int64_t i = threadIdx.x; i < rows; i += kPrepare * FLIGHT) {
+        float v[FLIGHT];
+        bool ignored[FLIGHT];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int64_t r = i + 1024 * k;
-            bool ignored = true;
-            if (r < rows) targets.at(r, ignored);
-            v[k] = ignored ? 0.0f : g[r];
+        for (int k = 0; k < FLIGHT; ++k) {
+            const int64_t r = min(i + kPrepare * k, rows - 1);  // the last row again past the rows
+            targets.at(r, ignored[k]);
+            v[k] = fabsf(g[r]);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) m = fmaxf(m, fabsf(v[k]));
+        for (int k = 0; k < FLIGHT; ++k) m = fmaxf(m, ignored[k] ? 0.0f : v[k]);
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
     __syncthreads();
     if (threadIdx.x) return;
-    for (int i = 1; i < 16; ++i) m = fmaxf(m, most[i]);
+    for (int i = 1; i < kPrepare / 64; ++i) m = fmaxf(m, most[i]);
     // within what a float32 and its inverse can be
     m = m > 0.0f && m < INFINITY ? fminf(fmaxf(m, 0x1p-100f), 0x1p100f) : top;
     scale[0] = top / m, scale[1] = m / top;
+}
+
+// What comes ahead of the products, in one launch: unless g is null the scale, by the first workgroup, and the copies.
+static __global__ __launch_bounds__(kPrepare) void head_prepare_kernel(HeadCopy h, HeadCopy w, const float *__restrict__ g, HeadTargets targets,
+                                                                  int64_t rows, float top, float *__restrict__ scale) {
+    const int group = int(blockIdx.x) - (g ? 1 : 0);
+    if (group < 0) head_scale(g, targets, rows, top, scale);
+    else if (group < h.groups) head_copy(h, targets, group);
+    else head_copy(w, targets, group - h.groups);
 }
 
 // The codes of a piece's rows into d, in place: a workgroup a row, whose lse and loss it works out first, 8 classes a thread at a
@@ -218,22 +256,9 @@ __global__ __launch_bounds__(256) void head_grad_kernel(uint16_t *__restrict__ c
                                                         const float *__restrict__ scale, HeadTargets targets, int64_t blocks,
                                                         float *__restrict__ losses) {
     typedef uint32_t words4 __attribute__((ext_vector_type(4)));
-    __shared__ float most[4];
-    __shared__ double sums[4];
     const int64_t row = blockIdx.x;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const float2 *q = part + row * blocks;
-    float m;
-    double sum;
-    head_row(q, threadIdx.x, 256, blocks, m, sum);
-    if (lane == 0) most[wave] = m, sums[wave] = sum;
-    __syncthreads();
-    const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-    sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (most[i] != -INFINITY) sum += sums[i] * double(head_exp(most[i] - top));
-    const double lse = double(top) + log(sum);
+    const double lse = head_lse(q, blocks);
     bool ignored;
     const int64_t cls = targets.at(row, ignored);
     const float l = float(lse), loss = float(lse - double(picked[row])), f = g[row] * scale[0];
@@ -340,21 +365,6 @@ static __global__ __launch_bounds__(256) void head_sum_kernel(const float *__res
             }
         }
         out(0, i, make_float4(e[0], e[1], e[2], e[3]), out.load(0, i));
-    }
-}
-
-// Rows of any length, alignment or distance as the products read them: copied to rows of kp elements, zeros past k. MASK: zeros
-// in ignored rows too, whose d of 0 times a NaN or an infinity of theirs would be no 0 in dw.
-template <bool MASK>
-__global__ __launch_bounds__(256) void head_pad_kernel(const uint16_t *__restrict__ src, int64_t rows, int64_t ld, int64_t k, int64_t kp,
-                                                       uint16_t *__restrict__ dst, HeadTargets targets) {
-    const int64_t per = kp / 8, total = rows * per;
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
-        const int64_t row = i / per, c = (i - row * per) * 8;
-        bool ignored = false;
-        if constexpr (MASK) targets.at(row, ignored);
-        *reinterpret_cast<uint4 *>(dst + row * kp + c) =
-            c < k && !ignored ? load8_any(src + row * ld + c, k - c) : make_uint4(0, 0, 0, 0);
     }
 }
 

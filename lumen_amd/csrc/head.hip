@@ -44,7 +44,7 @@ PartPlan weight_plan(const nhip_head_desc *d) {
     return p;
 }
 
-// Whether rows are copied first: no whole k tiles, or not on 16 bytes. The gradients always read a copy of h (head_pad_kernel).
+// Whether rows are copied first: no whole k tiles, or not on 16 bytes. The gradients always read a copy of h (head_copy).
 bool copies(const nhip_head_desc *d, int64_t ld) { return d->k % 64 != 0 || ld % 8 != 0; }
 
 struct HeadSpace {
@@ -168,13 +168,10 @@ int weight_grad(hipStream_t st, const nhip_head_desc *d, const PartPlan &p, int6
 
 bool on(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-template <bool MASK>
-int pad(hipStream_t st, const uint16_t *src, int64_t rows, int64_t ld, int64_t k, int64_t kp, uint16_t *dst, const HeadTargets &targets) {
-    const int64_t blocks = (rows * (kp / 8) + 255) / 256;
-    if (!blocks) return 0;
-    hipLaunchKernelGGL((head_pad_kernel<MASK>), dim3(unsigned(std::min<int64_t>(blocks, 8192))), dim3(256), 0, st, src, rows, ld, k, kp, dst,
-                       targets);
-    return check(hipGetLastError(), "head_pad_kernel launch");
+// A copy of `rows` rows at `dst`, by as many workgroups as it fills.
+HeadCopy copy_of(const uint16_t *src, int64_t rows, int64_t ld, int64_t k, int64_t kp, char *dst, bool mask) {
+    const int64_t groups = (rows * (kp / 8) + kPrepare - 1) / kPrepare;
+    return HeadCopy{src, rows, ld, k, kp, reinterpret_cast<uint16_t *>(dst), mask, int32_t(std::min<int64_t>(groups, 2048))};
 }
 
 template <bool F16>
@@ -185,28 +182,31 @@ int head_run(hipStream_t st, const nhip_head_desc *d, const uint16_t *h, const u
     const int64_t kp = padded_k(d), blocks = blocks_of(d), tsize = d->target_dtype == NHIP_LCE_I64 ? 8 : 4;
     int64_t h_m = d->h_m, w_n = d->w_n;
     HeadTargets targets{target, d->ignore_index, d->classes, d->target_dtype == NHIP_LCE_I64};
+    HeadCopy hc{}, wc{};
     if (grad || copies(d, h_m)) {
-        uint16_t *to = reinterpret_cast<uint16_t *>(ws + at.h);
-        if (grad ? pad<true>(st, h, d->rows, h_m, d->k, kp, to, targets) : pad<false>(st, h, d->rows, h_m, d->k, kp, to, targets)) return 1;
-        h = to, h_m = kp;
+        hc = copy_of(h, d->rows, h_m, d->k, kp, ws + at.h, grad);
+        h = hc.dst, h_m = kp;
     }
     if (copies(d, w_n)) {
-        uint16_t *to = reinterpret_cast<uint16_t *>(ws + at.w);
-        if (pad<false>(st, w, d->classes, w_n, d->k, kp, to, targets)) return 1;
-        w = to, w_n = kp;
+        wc = copy_of(w, d->classes, w_n, d->k, kp, ws + at.w, false);
+        w = wc.dst, w_n = kp;
     }
     float2 *part = reinterpret_cast<float2 *>(ws + at.part);
     float *picked = reinterpret_cast<float *>(ws + at.picked);
     float *scale = reinterpret_cast<float *>(ws + at.scale);
     uint16_t *codes = reinterpret_cast<uint16_t *>(ws + at.codes);
+    if (!grad && !losses) return 0;
+    if (const int groups = hc.groups + wc.groups + grad) {
+        hipLaunchKernelGGL(head_prepare_kernel, dim3(unsigned(groups)), dim3(kPrepare), 0, st, hc, wc, g, targets, d->rows, F16 ? 16384.0f : 1.0f,
+                           scale);
+        if (check(hipGetLastError(), "head_prepare_kernel launch")) return 1;
+    }
     if (!grad) {
-        if (!losses) return 0;
         if (logits<F16, false>(st, d, d->rows, h, h_m, w, w_n, HeadOut<false>{part, picked, nullptr, targets, blocks})) return 1;
-        hipLaunchKernelGGL(head_merge_kernel, dim3(unsigned((d->rows + 3) / 4)), dim3(256), 0, st, part, picked, targets, d->rows, blocks, losses);
+        hipLaunchKernelGGL(head_merge_kernel, dim3(unsigned(std::min<int64_t>(d->rows, 1 << 20))), dim3(256), 0, st, part, picked, targets, d->rows,
+                           blocks, losses);
         return check(hipGetLastError(), "head_merge_kernel launch");
     }
-    hipLaunchKernelGGL(head_scale_kernel, dim3(1), dim3(1024), 0, st, g, targets, d->rows, F16 ? 16384.0f : 1.0f, scale);
-    if (check(hipGetLastError(), "head_scale_kernel launch")) return 1;
     const PartPlan pi = input_plan(d), pw = weight_plan(d);
     const int64_t most = piece_rows(d), pieces = pieces_of(d);
     float *sums = reinterpret_cast<float *>(ws + at.weight_sums), *parts = reinterpret_cast<float *>(ws + at.input_parts);
