@@ -75,7 +75,7 @@ class Compiled:
                     w._placed(target)
                 for pack in plan.packs:
                     _pack([traced.weights[traced.layout[i][1]] for i in pack], target)
-            entry = (traced, plan, workspace, plan and _Recipe(traced, plan))
+            entry = (traced, plan, workspace, plan and _Recipe(traced, plan, workspace, target))
             self._plans[key] = entry
         self._latest = key
         return target, entry
@@ -195,8 +195,7 @@ class Compiled:
             ptrs = self._run(plan, workspace, traced, ptrs, keep)
             self._last_buffers = (workspace.ptr, ptrs)
             # outputs computed over the weight they replace, or views of the workspace
-            outs = [keep[i] if i is not None else Tensor.on_device(dtype, shape, target, workspace, offset)
-                    for i, dtype, shape, offset in recipe.outputs]
+            outs = [keep[i] if fields is None else Tensor.of_fields(fields) for i, fields in recipe.outputs]
             # the other weights the function assigned: written back into their memory, in stream order
             for j, k in recipe.copied_back:
                 traced.weights[k]._placed(target).copy_(outs[j])
@@ -209,13 +208,13 @@ class Compiled:
 
 class _Recipe:
     """What a call of a plan does, worked out once: whether its layout names scalars, where each output lies
-    (``(input position or None, dtype, shape, byte offset in the workspace)``) and the weights copied back."""
+    (``(input position, None)`` or ``(None, Tensor.device_fields)`` of the workspace) and the weights copied back."""
 
-    def __init__(self, traced, plan):
+    def __init__(self, traced, plan, workspace, target):
         kinds = {kind for kind, _ in traced.layout}
         self.scalars = "scalar" in kinds
-        self.outputs = [(loc.base[1] if loc.base[0] == "in" else None, loc.dtype, tuple(loc.shape),
-                         loc.offset * _size(loc.dtype)) for loc in plan.output_locs]
+        self.outputs = [(loc.base[1], None) if loc.base[0] == "in" else (None, Tensor.device_fields(
+            loc.dtype, tuple(loc.shape), target, workspace, loc.offset * _size(loc.dtype))) for loc in plan.output_locs]
         self.copied_back = [(traced.n_returned + j, k) for j, k in enumerate(traced.written)
                             if traced.n_returned + j not in plan.in_place_outputs]
 
