@@ -498,12 +498,11 @@ template <bool CAUSAL, bool ATOMIC_DQ> struct DkdvPaired { static constexpr bool
 // STORE_DS (the deterministic mode's default): each tile's dS (rounded as for dK) is stored to p.ds for the
 // dQ = dS K kernel, instead of a second kernel recomputing S and dP.
 // Key block pidx (PAIR: and nkb - 1 - pidx) of nkb of key head nkv of batch b; a head's statistics are `ls` floats after the
-// last one's. PARTS: part `part` of `parts` of the query tiles, its float32 sums to `sums` instead of dk and dv: a key's hd of dK,
-// then its hdv of dV, keys sums_s floats apart.
+// last one's. PARTS: part `part` of `parts` of the query tiles, its float32 sums to `sums` instead of dk and dv, as the threads hold
+// them: [2 (dK, dV)][D / 8][256 threads][4].
 template <int D, bool F16, bool CAUSAL, bool ATOMIC_DQ, bool STORE_DS, bool PAIR, bool PARTS = false>
 __device__ __forceinline__ void flash_dkdv_tile(const AttnParams &p, const float *lse2, int64_t b, int64_t nkv, int64_t pidx,
-                                                int64_t nkb, int64_t ls, int part = 0, int parts = 1, float *sums = nullptr,
-                                                int64_t sums_s = 0) {
+                                                int64_t nkb, int64_t ls, int part = 0, int parts = 1, float *sums = nullptr) {
     static_assert(!PARTS || (!PAIR && !ATOMIC_DQ), "parts of one key block, without atomics");
     constexpr int BM = 64;
     constexpr int DS = D / 16, DT = D / 32;
@@ -844,23 +843,18 @@ __device__ __forceinline__ void flash_dkdv_tile(const AttnParams &p, const float
         if (j + 1 < total) tile(j + 1, stage1, Ls1, Dl1, stage0, Ls0, Dl0);
     }
     if constexpr (ATOMIC_DQ) flush_dq();
-    if (!kvalid) return;
     if constexpr (PARTS) {
-        float *to = sums + kj * sums_s;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int e4 = 0; e4 < 4; ++e4) {
-                const int d = 32 * dt + 8 * e4 + 4 * h;
-                if (32 * dt + 8 * e4 < p.hd)
-                    *reinterpret_cast<float4 *>(to + d) =
-                        make_float4(adk[dt][4 * e4], adk[dt][4 * e4 + 1], adk[dt][4 * e4 + 2], adk[dt][4 * e4 + 3]);
-                if (32 * dt + 8 * e4 < p.hdv)
-                    *reinterpret_cast<float4 *>(to + p.hd + d) =
-                        make_float4(adv[dt][4 * e4], adv[dt][4 * e4 + 1], adv[dt][4 * e4 + 2], adv[dt][4 * e4 + 3]);
+                float4 *to = reinterpret_cast<float4 *>(sums) + (4 * dt + e4) * 256 + threadIdx.x;
+                to[0] = make_float4(adk[dt][4 * e4], adk[dt][4 * e4 + 1], adk[dt][4 * e4 + 2], adk[dt][4 * e4 + 3]);
+                to[4 * DT * 256] = make_float4(adv[dt][4 * e4], adv[dt][4 * e4 + 1], adv[dt][4 * e4 + 2], adv[dt][4 * e4 + 3]);
             }
         return;
     }
+    if (!kvalid) return;
     uint16_t *dkp = p.dk + b * p.dk_b + nkv * p.dk_n + kj * p.dk_s;
     uint16_t *dvp = p.dv + b * p.dv_b + nkv * p.dv_n + kj * p.dv_s;
 #pragma unroll

@@ -33,7 +33,7 @@ struct PackedTables {
     int64_t sequences, tokens;
     int32_t o64;
     int64_t ds_tiles;    // dS tiles of one head that there is room for
-    int32_t *fits;       // whether all of them do (null: nobody asks), and the first and the last sequence's end
+    int32_t *fits;       // whether all of them do (null: nobody asks)
 };
 
 constexpr int kPackedBuckets = 1024;  // also the builder's threads
@@ -137,7 +137,7 @@ static __global__ __launch_bounds__(kPackedBuckets) void packed_tiles_kernel(Pac
         last = max(first, carry);
         __syncthreads();
         if (pass == 1) break;
-        if (a.fits && tid == 0 && blockIdx.x == 0) a.fits[0] = ds_carry <= a.ds_tiles, a.fits[1] = first, a.fits[2] = last;
+        if (a.fits && tid == 0 && blockIdx.x == 0) *a.fits = ds_carry <= a.ds_tiles;
         // counts to places
         const int count = bucket[tid], sum = packed_wave_sum(count, lane);
         if (lane == 63) waves[wave] = sum;
@@ -183,7 +183,7 @@ __device__ __forceinline__ void packed_tiles_few(const PackedTables &a, int tabl
     before[tid] = from;
     ds_at[tid] = ds_from;  // read only where all fit
     const int first = at[0], last = at[count];
-    if (a.fits && tid == 0 && table == 0) a.fits[0] = ds_total <= a.ds_tiles, a.fits[1] = first, a.fits[2] = last;
+    if (a.fits && tid == 0 && table == 0) *a.fits = ds_total <= a.ds_tiles;
     __syncthreads();
     for (int i = tid; i < total; i += kPackedFew) {
         int k = 0, hi = count;
@@ -306,8 +306,7 @@ __global__ __launch_bounds__(256) void packed_prep_kernel(AttnParams p, const ui
 
 // STORE: each tile's dS goes to the workspace for packed_dq_ds_kernel; else packed_dq_kernel computes it again. Where the
 // room for dS may not do both are launched, and `fits` ends one of them. PARTS: a workgroup takes part blockIdx.y of a key
-// block's query tiles, whose sums [parts][tokens][kv heads][hd + hdv] packed_dkdv_sum_kernel adds (7 sequences of 812 tokens, 2 key
-// heads of 6, dims 80, float16: 62 us in 18 workgroups, 29 and 7 for the sums in 12 parts).
+// block's query tiles, whose sums [parts][entries of all heads][256 D] packed_dkdv_sum_kernel adds.
 template <int D, bool F16, bool CAUSAL, bool STORE, bool PARTS>
 __global__ __launch_bounds__(256) void packed_dkdv_kernel(AttnParams p, const float *lse2, const PackedTile *tiles, int64_t tokens,
                                                           const int32_t *fits, float *sums) {
@@ -325,28 +324,40 @@ __global__ __launch_bounds__(256) void packed_dkdv_kernel(AttnParams p, const fl
     p.d_o += t.start * p.do_s, p.dk += t.start * p.dk_s, p.dv += t.start * p.dv_s;
     p.delta += t.start;
     if (STORE) p.ds += t.ds * p.heads * (128 * 64);
-    const int64_t row = p.hd + p.hdv;
-    if (PARTS) sums += ((int64_t(blockIdx.y) * tokens + t.start) * p.kv_heads + n) * row;
+    if (PARTS) sums += (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * (256 * D);
     flash_dkdv_tile<D, F16, CAUSAL, false, STORE, false, PARTS>(p, lse2 + t.start, 0, n, t.block, (t.len + 127) / 128, tokens, int(blockIdx.y),
-                                                                int(gridDim.y), sums, p.kv_heads * row);
+                                                                int(gridDim.y), sums);
 }
 
-// The parts' sums of the sequences' tokens (used[1] to used[2]), added in order and rounded: four elements a thread.
-template <bool F16>
-__global__ __launch_bounds__(256) void packed_dkdv_sum_kernel(AttnParams p, const float *__restrict__ sums, int parts, int64_t tokens,
-                                                              const int32_t *__restrict__ used) {
-    const int64_t row = p.hd + p.hdv, per = p.kv_heads * (row / 4), total = (int64_t(used[2]) - used[1]) * per;
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
-        const int64_t t = used[1] + i / per, n = i % per / (row / 4), c = i % (row / 4) * 4;
-        const float *from = sums + (t * p.kv_heads + n) * row + c;
-        float4 v = *reinterpret_cast<const float4 *>(from);
-        for (int k = 1; k < parts; ++k) {
-            const float4 x = *reinterpret_cast<const float4 *>(from + k * tokens * p.kv_heads * row);
-            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+// The parts' sums, added in order and rounded: blockIdx.y is a tile of 32 columns of dK, then of dV.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void packed_dkdv_sum_kernel(AttnParams p, const PackedTile *tiles, const float *__restrict__ sums, int parts) {
+    int64_t n, idx;
+    packed_place(p.kv_heads, n, idx);
+    const PackedTile t = tiles[idx];
+    if (t.block < 0) return;
+    const bool v = blockIdx.y >= D / 32;
+    const int dt = int(blockIdx.y) % (D / 32), cols = int(v ? p.hdv : p.hd);
+    const float4 *from = reinterpret_cast<const float4 *>(sums + int64_t(blockIdx.x) * (256 * D)) + int64_t(blockIdx.y) * 1024 + threadIdx.x;
+    float4 sum[4];
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) sum[e4] = from[256 * e4];
+#pragma unroll 4
+    for (int k = 1; k < parts; ++k)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+            const float4 x = from[int64_t(k) * gridDim.x * (64 * D) + 256 * e4];
+            sum[e4].x += x.x, sum[e4].y += x.y, sum[e4].z += x.z, sum[e4].w += x.w;
         }
-        uint16_t *to = c < p.hd ? p.dk + t * p.dk_s + n * p.dk_n + c : p.dv + t * p.dv_s + n * p.dv_n + (c - p.hd);
-        *reinterpret_cast<uint2 *>(to) = make_uint2(pack2<F16>(v.x, v.y), pack2<F16>(v.z, v.w));
-    }
+    // a key a lane, and every other four columns, as flash_dkdv_tile's
+    const int lane = threadIdx.x & 63, key = t.block * 128 + int(threadIdx.x >> 6) * 32 + (lane & 31);
+    if (key >= t.len) return;
+    uint16_t *to = v ? p.dv + n * p.dv_n + (t.start + int64_t(key)) * p.dv_s : p.dk + n * p.dk_n + (t.start + int64_t(key)) * p.dk_s;
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4)
+        if (32 * dt + 8 * e4 < cols)
+            *reinterpret_cast<uint2 *>(to + 32 * dt + 8 * e4 + 4 * (lane >> 5)) =
+                make_uint2(pack2<F16>(sum[e4].x, sum[e4].y), pack2<F16>(sum[e4].z, sum[e4].w));
 }
 
 template <int D, bool F16, bool CAUSAL>

@@ -43,12 +43,17 @@ int64_t ds_room(const nhip_packed_desc *d) {
     return std::min<int64_t>(std::min(most_ds(d), d->ds_bytes / (d->heads * 128 * 64 * 2)), (1 << 24) - 1);
 }
 
-// Parts of a key block's query tiles: as many as give the CUs about a workgroup and a half each where whole blocks leave most
-// of them idle, their count estimated with half a block a sequence lost.
+// Parts of a key block's query tiles where whole blocks leave half of the CUs or more idle: as many as give each CU a workgroup,
+// but no more than three quarters of a block's tiles, since a part costs the K and V operands' loads and its sums' traffic. Blocks
+// are estimated with half a one a sequence lost, tiles from the mean length. Us of the kernel and its sums by parts (* taken):
+//   331 + 254 + 129 + 97 tokens, 6 heads of 2, dims 80, unmasked    1: 62   2: 39  4: 27  6: 22  8: 23*(7)  12: 30  16: 34
+//   1500 + 500 + 48 tokens, 8 heads of 2, dims 128, causal          1: 259  2: 136  4: 76  6: 59  8: 55*(7)  12: 58  16: 60
+//   200 + 300 + 12 tokens, 8 heads of 8, dims 64, causal            1: 19   2: 17  3: 15*  4: 16  6: 17  8: 19  12: 24
 int64_t key_parts(const nhip_packed_desc *d) {
-    const int64_t blocks = (d->tokens / kKeyBlock + std::min(d->sequences, d->tokens) / 2 + 1) * std::max<int64_t>(d->kv_heads, 1);
-    if (blocks >= 192) return 1;
-    return std::max<int64_t>(std::min<int64_t>(384 / blocks, 16), 1);
+    const int64_t sequences = std::max<int64_t>(std::min(d->sequences, d->tokens), 1), kv_heads = std::max<int64_t>(d->kv_heads, 1);
+    const int64_t blocks = (d->tokens / kKeyBlock + sequences / 2 + 1) * kv_heads;
+    const int64_t tiles = (d->tokens / sequences + 63) / 64 * (d->heads / kv_heads);
+    return std::max<int64_t>(std::min<int64_t>({256 / blocks, (3 * tiles + 3) / 4, 16}), 1);
 }
 
 // The backward's workspace: delta and the base-2 LSE, the flag, both tables, dS.
@@ -63,7 +68,7 @@ BwdSpace bwd_space(const nhip_packed_desc *d) {
     w.queries = w.keys + table_bytes(d, kKeyBlock);
     w.sums = w.queries + table_bytes(d, kDqBlock);
     const int64_t parts = key_parts(d);
-    w.ds = w.sums + (parts > 1 ? up256(size_t(parts) * d->tokens * d->kv_heads * (d->head_dim + value_dim(d)) * sizeof(float)) : 0);
+    w.ds = w.sums + (parts > 1 ? size_t(parts) * table_entries(d, kKeyBlock) * d->kv_heads * 256 * kernel_dim(d) * sizeof(float) : 0);
     w.bytes = w.ds + size_t(ds_room(d)) * d->heads * (128 * 64 * 2);
     return w;
 }
@@ -172,9 +177,8 @@ int bwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, const ui
     }
     const int64_t parts = key_parts(d);
     if (parts == 1) return 0;
-    const int64_t work = d->tokens * d->kv_heads * (p.hd + p.hdv) / 4;
-    hipLaunchKernelGGL((packed_dkdv_sum_kernel<F16>), dim3(unsigned(std::min<int64_t>((work + 255) / 256, 2048))), dim3(256), 0, st, p, sums,
-                       int(parts), d->tokens, a.fits);
+    hipLaunchKernelGGL((packed_dkdv_sum_kernel<D, F16>), dim3(unsigned(a.t[0].most * d->kv_heads), D / 16), dim3(256), 0, st, p, a.t[0].tiles,
+                       sums, int(parts));
     return check(hipGetLastError(), "packed_dkdv_sum_kernel launch");
 }
 
