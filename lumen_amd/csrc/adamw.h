@@ -9,6 +9,9 @@
 // them, which a table in the kernel's arguments maps to a tensor by binary search, so many small weights cost no more than
 // one large one and the table needs no copy to the device.
 //
+// 39 million bf16 weights with masters (1.09 GB) 205 us, 5.3 TB/s; 203 million (5.7 GB) 1.05 to 1.06 ms, 5.4 TB/s, a copy being
+// 5.1; 12 small float32 ones (8 MB) 7.7 us.
+//
 // The moments are float32 and so is everything of an element, each operation rounded on its own: the step's factors are
 // worked out in float64 (b^t of a late step, 1 - b^t of an early one) and rounded once. A thread reads its elements
 // before it writes them, so any result may lie over the operand that it replaces.

@@ -14,6 +14,11 @@
 // same way in every row whose p is near 0, a gradient 2^-9 too long) or 2^14 (float16, whose range a mean's p would leave), and
 // the products are multiplied by what it was (head_scale).
 // Sums are float32; over classes of a row first float32 in blocks of 64, then float64.
+//
+// The products are MFMA's (gemm.h's streamed tiles) and the pass over the codes HBM's. Of 8192 rows and 32000 classes, us: the
+// forward product with its store 382 at k = 512 (0.70 PFLOP/s: the store's exponentials and 0.5 GB are as long as the product) and
+// 934 at k = 2048 (1.15), codes into d 201 (1.05 GB, 5.2 TB/s), dh 247 and 826 (1.09, 1.30), dw 242 and 927 (1.11, 1.16). Tiles
+// of 128 rows, whose stores two workgroups a CU could hide, took the forward product from 391 to 451 and from 970 to 1249.
 #pragma once
 
 #include "device_common.h"

@@ -1,11 +1,16 @@
 // Self attention of sequences packed one after another: each within its own, forward and backward, by the tiles of
-// attention.h over a table of workgroups that packed_tiles_kernel makes of the offsets on the device.
+// attention.h over a table of workgroups made of the offsets on the device (packed_tiles_kernel, packed_tiles_few; packed_tile
+// where a launch needs none).
 //
 // A workgroup's tile lies within one sequence and its loads end there, so that no row of another sequence (of padding, NaN
 // or infinite) reaches it, not even with a probability of zero. The grid covers the most tiles that any offsets give
 // (tokens / block, and one more a sequence); the table's unused entries end at once. Entries stand by falling work, whatever
 // sequence they are of, so that the longest start first and the last ones fill the gaps. Tokens of no sequence (before the
 // first offset and from the last one on) are entries too: their results are zeros.
+//
+// MFMA bounds long sequences, at the flash kernels' rates. 8 documents of 281 to 4096 tokens, 16 heads of 128, causal, us: forward
+// 271 (719 TFLOP/s), rows' sums 38 (5.3 TB/s), dK and dV with dS stored 678 (575), dQ from it 187; an empty launch of either kernel
+// of the other mode 5. Short ones are bound by launches and by the longest sequence's tiles one after another.
 #pragma once
 
 #include "attention.h"
