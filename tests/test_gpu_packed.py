@@ -9,6 +9,7 @@ import lumen_amd as L
 import lumen_amd.functional as F
 from lumen_amd import dtypes as D
 from lumen_amd import native as nv
+from lumen_amd.graph import prims
 from tests import training_math as M
 from tests.hiputil import Dev
 
@@ -162,6 +163,64 @@ def test_heads_enough_for_whole_key_blocks(hip, lengths, n, nkv, d, dtype, causa
         f = L.compile(_program(causal), device="hip")
         for name, a, w, tt in zip(("o", "dq", "dk", "dv"), f(*args), want, tol):
             _near(_values(a), w, tt, name)
+
+
+def test_rows_far_apart_within_a_sequence(hip):
+    """A sequence whose rows span more than 2^31 bytes, read in place through a view's strides; a padded head dim, whose loads reach
+    2^31 bytes, is refused."""
+    t, d, wide = 1200, 64, 1 << 20
+    rng = np.random.default_rng(14)
+    x = {k: _round(v, "bfloat16") for k, v in M.packed_inputs(rng, t, 1, 1, d).items()}
+    offsets = M.offsets_of([1150, 50])
+    base = np.zeros((t, wide), np.uint16)
+    for i, k in enumerate("qkv"):
+        base[:, i * d:(i + 1) * d] = D.from_values(x[k].reshape(t, d).astype(np.float32), "bfloat16")
+    base = L.Tensor("bfloat16", base.shape, "cpu", host=base).to(device="hip")
+
+    def program(d):
+        def fn(base, offsets, do):
+            q, k, v = (base[:, i * d:(i + 1) * d].reshape(t, 1, d) for i in range(3))
+            o, pull = L.vjp(lambda q, k, v: F.packed_attention(q, k, v, offsets), q, k, v)
+            return [o, *pull(do)]
+
+        return fn
+
+    want, tol = M.packed(x, offsets, True, d**-0.5, "bfloat16")
+    f = L.compile(program(d), device="hip")
+    for name, a, w, tt in zip(("o", "dq", "dk", "dv"), f(base, L.from_numpy(offsets), _tensor(x["do"], "bfloat16")), want, tol):
+        _near(_values(a), w, tt, name)
+    with pytest.raises(RuntimeError, match="2 GiB"):
+        L.compile(program(40), device="hip")(base, L.from_numpy(offsets), _tensor(x["do"][:, :, :40], "bfloat16"))
+
+
+def test_no_tokens_broadcasts_and_single_gradients(hip):
+    """No tokens at all; keys and values broadcast over the heads and a cotangent of one number; each gradient alone."""
+    offsets = np.array([0, 0, 0], np.int32)
+    none = np.zeros((0, 2, 64))
+    out = L.compile(_program(True), device="hip")(*(_tensor(none, "bfloat16") for _ in range(3)), L.from_numpy(offsets), _tensor(none, "bfloat16"))
+    assert [_values(a).shape for a in out] == [none.shape] * 4
+
+    rng = np.random.default_rng(15)
+    t, n, d = 150, 4, 64
+    x = {k: _round(v, "bfloat16") for k, v in M.packed_inputs(rng, t, n, 1, d).items()}
+    x["do"] = np.full((t, n, d), 0.5)
+    offsets = M.offsets_of([100, 47])
+    whole = dict(x, k=np.repeat(x["k"], n, 1), v=np.repeat(x["v"], n, 1))
+    want, tol = M.packed(whole, offsets, True, d**-0.5, "bfloat16")
+    args = [_tensor(x[k], "bfloat16") for k in "qkv"] + [L.from_numpy(offsets)]
+
+    def gradients(q, k, v, offsets):
+        def loss(q, k, v):
+            return F.sum(F.packed_attention(q, k, v, offsets).float()) * 0.5
+
+        _, pull = L.vjp(loss, q, k.expand(t, n, d), v.expand(t, n, d))
+        return list(pull(prims.full((), 1.0, "float32")))
+
+    for name, a, w, tt in zip(("dq", "dk", "dv"), L.compile(gradients, device="hip")(*args), want[1:], tol[1:]):
+        _near(_values(a), w, tt, name)
+    for i in range(3):
+        (a,) = L.compile(lambda *xs: [gradients(*xs)[i]], device="hip")(*args)
+        _near(_values(a), want[1 + i], tol[1 + i], i)
 
 
 def test_gradients_of_short_sequences_take_o_whole(hip):
