@@ -246,6 +246,7 @@ int head_on(hipStream_t st, const nhip_head_desc *d, const void *h, const void *
         return fail("nhip_head_loss: operands of whole rows start on 16 bytes");
     if (d->rows == 0) return dw ? fill_on(st, dw, size_t(d->classes) * d->k * 2, 0) : 0;
     if (!ws) return fail("nhip_head_loss: no workspace");
+    if (!h || !w || !target) return fail("nhip_head_loss: an operand without memory");
     auto go = d->dtype == NHIP_F16 ? head_run<true> : head_run<false>;
     return go(st, d, static_cast<const uint16_t *>(h), static_cast<const uint16_t *>(w), target, g, losses, static_cast<uint16_t *>(dh),
               static_cast<uint16_t *>(dw), static_cast<char *>(ws));

@@ -105,6 +105,12 @@ int on16(const char *what, std::initializer_list<const void *> ps) {
     return 0;
 }
 
+int given(const char *what, std::initializer_list<const void *> ps) {
+    for (const void *p : ps)
+        if (!p) return fail(std::string(what) + ": an operand or a result without memory");
+    return 0;
+}
+
 AttnParams packed_params(const nhip_packed_desc *d) {
     AttnParams p{};
     p.sq = p.sk = d->tokens;
@@ -189,6 +195,7 @@ int packed_fwd_on(hipStream_t st, const nhip_packed_desc *d, const void *q, cons
     if (packed_check(d, "nhip_packed_fwd") || on16("nhip_packed_fwd", {q, k, v, o, rest, ws})) return 1;
     if (d->tokens == 0 || d->heads == 0) return 0;
     if (!ws) return fail("nhip_packed_fwd: no workspace");
+    if (given("nhip_packed_fwd", {q, k, v, offsets, o})) return 1;
     AttnParams p = packed_params(d);
     p.q = static_cast<const uint16_t *>(q), p.k = static_cast<const uint16_t *>(k), p.v = static_cast<const uint16_t *>(v);
     p.o = static_cast<uint16_t *>(o), p.lse = lse;
@@ -210,6 +217,7 @@ int packed_bwd_on(hipStream_t st, const nhip_packed_desc *d, const void *q, cons
     if (packed_check(d, "nhip_packed_bwd") || on16("nhip_packed_bwd", {q, k, v, o, rest, d_o, dq, dk, dv, ws})) return 1;
     if (d->tokens == 0 || d->heads == 0) return 0;
     if (!ws) return fail("nhip_packed_bwd: no workspace");
+    if (given("nhip_packed_bwd", {q, k, v, offsets, o, d_o, lse, dq, dk, dv})) return 1;
     const BwdSpace w = bwd_space(d);
     char *at = static_cast<char *>(ws);
     AttnParams p = packed_params(d);

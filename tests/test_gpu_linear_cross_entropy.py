@@ -325,6 +325,6 @@ def test_refusals_of_the_entry_point(hip):
 
     for kw in (dict(rows=-1), dict(classes=0), dict(k=0), dict(dtype=0), dict(target_dtype=2), dict(w_n=63), dict(h_m=-64), dict(piece_bytes=-1),
                dict(classes=1 << 22), dict(classes=1 << 21, k=1 << 10, w_n=1 << 10, h_m=1 << 10), dict(g=None), dict(ws=None),
-               dict(ws=one.ptr + 16), dict(dh=one.ptr + 2), dict(g=None, dh=None, h=one.ptr + 2), dict(rows=1 << 31)):
+               dict(ws=one.ptr + 16), dict(dh=one.ptr + 2), dict(g=None, dh=None, h=one.ptr + 2), dict(rows=1 << 31), dict(h=None)):
         with pytest.raises(RuntimeError, match="nhip_head_loss"):
             call(**kw)

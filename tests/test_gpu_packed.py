@@ -352,4 +352,10 @@ def test_refusals_of_the_entry_points(hip):
         nv.call("nhip_packed_bwd", desc(), *[one.ptr] * 11, None)
     with pytest.raises(RuntimeError, match="head dim"):
         nv.call("nhip_packed_fwd", desc(head_dim=12), one.ptr, one.ptr, one.ptr, one.ptr, one.ptr, None, None, one.ptr)
+    for at in range(5):
+        with pytest.raises(RuntimeError, match="without memory"):
+            nv.call("nhip_packed_fwd", desc(), *[None if i == at else one.ptr for i in range(5)], None, None, one.ptr)
+    for at in (0, 1, 2, 3, 4, 6, 7, 8, 9, 10):  # all but the rest of o
+        with pytest.raises(RuntimeError, match="without memory"):
+            nv.call("nhip_packed_bwd", desc(), *[None if i == at else one.ptr for i in range(11)], one.ptr)
     nv.call("nhip_packed_fwd", desc(tokens=0), None, None, None, None, None, None, None, None)  # nothing to do
