@@ -530,7 +530,7 @@ __device__ __forceinline__ int stream_line(int wn, int j) {
 template <class Out>
 struct TakesSums : std::false_type {};
 
-// One workgroup's 256 x 256 output tile. `out` is AnyStore (a plain store of D), or a generated epilogue
+// One workgroup's 256 x 256 output tile `tile` (of part `part` of k, batch blockIdx.y). `out` is AnyStore (a plain store of D), or a generated epilogue
 // functor called as out(row, col, float4, pre) with the float32 sums of four consecutive columns (col a
 // multiple of 4, within m x n) and pre = out.load(row, col), its other operands read ahead. `smem` holds gemm_stream_lds_bytes<BK, WN>() bytes.
 // KL, the k loop: 0 fragments of the next k step read under the current step's MFMAs; 1 (XPF) that read also
@@ -539,14 +539,15 @@ struct TakesSums : std::false_type {};
 // ST: the stages in LDS (0: gemm_stream_stages).
 // PAIR 1: two products of A, by B and by b2 of the same shape and strides: half of the tile's columns are B's, half the
 // same columns of b2, and out.store takes the pairs of sums. PAIR 2: the sum of two products, A's first k / 2 columns by b
-// and the others by b2, part blockIdx.z of it over k_part of the k tiles. PAIR 3: one product of operands contiguous along m
+// and the others by b2, a part of it over k_part of the k tiles. PAIR 3: one product of operands contiguous along m
 // and n, in parts like PAIR 2. PAIR 4: PAIR 1 in parts. PAIR 5: one product of A along k by B along n, in parts,
 // A's rows in whole chunks of 8. k (PAIR 2: k / 2) is a multiple of 8, with PAIR 3 and 5 any number; rows
 // along n (and m) hold whole chunks of 8 elements whatever n is. Operands are within the buffers' reach.
 template <bool F16, int BK, int WN, bool AT, bool BT, bool BUF, class Out, int TM = 256, int KL = 0, int PAIR = 0, int ST = 0>
 __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint16_t *__restrict__ a,
                                                  const uint16_t *__restrict__ b, const Out &out, char *smem,
-                                                 const uint16_t *__restrict__ b2 = nullptr, int k_part = 0) {
+                                                 const uint16_t *__restrict__ b2 = nullptr, int k_part = 0,
+                                                 uint32_t tile = blockIdx.x, uint32_t part = blockIdx.z) {
     constexpr int NW = 2 * WN;       // wavefronts (2 x WN)
     constexpr int WR = TM / 2;       // rows a wave
     constexpr int FM = WR / 32;      // 32-row MFMA tiles a wave
@@ -560,7 +561,7 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     constexpr int NRD = (AT ? 2 * FM : FM) + (BT ? 2 * FN : FN);  // LDS read instructions a k step
 
     int tm, tn;
-    tile_of(blockIdx.x, s.tiles_m, s.tiles_n, tm, tn);
+    tile_of(tile, s.tiles_m, s.tiles_n, tm, tn);
     int64_t oa, ob, od;
     batch_offsets(s, blockIdx.y, oa, ob, od);
     static_assert(PAIR == 0 || (BUF && AT == (PAIR == 3) && BT == (PAIR == 2 || PAIR == 3 || PAIR == 5) && FN % 2 == 0), "the pairs' layouts");
@@ -572,10 +573,10 @@ __device__ __forceinline__ void gemm_stream_tile(const GemmShape &s, const uint1
     const int h = lane >> 5, l32 = lane & 31, g = lane >> 4, s16 = lane & 15;
     // one wave a SIMD (WN = 2): the wave index as a scalar, so the loads' LDS destinations are scalar arithmetic
     const int wave_u = WN == 2 ? __builtin_amdgcn_readfirstlane(wave) : wave;
-    const int64_t ks = PAIR == 0 ? int64_t(blockIdx.z) * s.k : 0;  // split-k: this workgroup's first k
-    od += int64_t(blockIdx.z) * s.d_split;
+    const int64_t ks = PAIR == 0 ? int64_t(part) * s.k : 0;  // split-k: this workgroup's first k
+    od += int64_t(part) * s.d_split;
     // PAIR 2 to 5: the part's first k tile; PAIR 3 to 5: the operands from its first k on
-    const int kfirst = PAIR >= 2 ? int(blockIdx.z) * k_part : 0;
+    const int kfirst = PAIR >= 2 ? int(part) * k_part : 0;
     const int64_t kp = PAIR >= 3 ? int64_t(kfirst) * BK : ks;
     const uint16_t *pa = a + oa + kp * s.a_k, *pb = b + ob + kp * s.b_k;
     const int64_t kb = PAIR == 2 ? s.k / 2 : PAIR >= 4 ? s.k - kp : s.k;  // k of one B operand

@@ -353,6 +353,29 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ST == 2 ? 2
                                                                                                                   nullptr, k_part);
 }
 
+// Both in one launch, for products whose workgroups fit the chip together, two a CU: dh's in parts first, then dw's whole. (As two
+// rows of a grid as wide and deep as either needs, the empty workgroups, which hold LDS too, cost up to 10 us.)
+template <class InOut>
+struct HeadBoth {
+    GemmShape input, weight;
+    const uint16_t *w, *h;
+    InOut input_out;
+    HeadStore weight_out;
+    int32_t parts, input_part, weight_part;  // k tiles of a part, and of all dw's
+};
+template <bool F16, class InOut>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void head_both_grads(HeadBoth<InOut> x,
+                                                                                                  const uint16_t *__restrict__ d) {
+    extern __shared__ __align__(1024) char smem[];
+    const uint32_t tiles = uint32_t(x.input.tiles_m) * uint32_t(x.input.tiles_n), at = blockIdx.x, input = tiles * uint32_t(x.parts);
+    if (at < input)
+        gemm_stream_tile<F16, 64, 2, false, true, true, InOut, 128, 0, 5, 2>(x.input, d, x.w, x.input_out, smem, nullptr, x.input_part, at % tiles,
+                                                                             at / tiles);
+    else
+        gemm_stream_tile<F16, 64, 2, true, true, true, HeadStore, 128, 0, 3, 2>(x.weight, d, x.h, x.weight_out, smem, nullptr, x.weight_part,
+                                                                                at - input, 0);
+}
+
 // Float32 sums of a product's parts, P[part][mn], added in order and stored as HeadStore stores a tile (of one row).
 static __global__ __launch_bounds__(256) void head_sum_kernel(const float *__restrict__ part, int parts, int64_t mn, HeadStore out) {
     out.n = mn;

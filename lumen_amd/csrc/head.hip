@@ -44,6 +44,29 @@ PartPlan weight_plan(const nhip_head_desc *d) {
     return p;
 }
 
+// Both products in one launch of at most two workgroups of 128-row tiles a CU, dh's in parts: parts 0 where one after the other is
+// estimated shorter, by part_plan's rates for a launch of so many workgroups. Us with the parts' sums, one after the other and together (* taken), of
+// rows, k, classes:
+//   777, 520, 5003    40  31*      200, 1024, 5000  32  23*      128, 768, 8192   33  24*      900, 256, 8000   39  28*
+//   1500, 300, 3000   40  34*      64, 256, 1000    23  17*      1024, 512, 2048  33  28*      2000, 72, 63     23* 31
+struct BothPlan {
+    int parts, k_part;
+};
+BothPlan both_plan(const nhip_head_desc *d) {
+    if (pieces_of(d) != 1) return BothPlan{0, 0};
+    const int64_t input = blocks_of(d), weight = (d->rows + 63) / 64;
+    const int64_t ti = tiles(d->rows, 128, d->k, 128), tw = tiles(d->classes, 128, d->k, 128);
+    BothPlan best{0, 0};
+    double least = input_plan(d).us + weight_plan(d).us;
+    for (int64_t s = 1; s <= 16; ++s) {
+        const int64_t part = (input + s - 1) / s, parts = (input + part - 1) / part, t = ti * parts + tw;
+        if (t > 512) break;
+        const double us = 6.2 + 64.0 * double(std::max(part, weight)) * 0.0142 * (t <= 256 ? 0.79 : 1.0) + parts_us(d->rows * d->k, parts);
+        if (us < least) least = us, best = BothPlan{int(parts), int(part)};
+    }
+    return best;
+}
+
 // Whether rows are copied first: no whole k tiles, or not on 16 bytes. The gradients always read a copy of h (head_copy).
 bool copies(const nhip_head_desc *d, int64_t ld) { return d->k % 64 != 0 || ld % 8 != 0; }
 
@@ -70,7 +93,7 @@ HeadSpace head_space(const nhip_head_desc *d, bool grad) {
         s.weight_sums = take(pieces_of(d) > 1 ? size_t(d->classes) * d->k * 4 : 0);
         // the parts of one product at a time
         s.input_parts = s.weight_parts =
-            take(std::max(pi.parts > 1 ? size_t(pi.parts) * rows * d->k * 4 : 0, pw.parts > 1 ? size_t(pw.parts) * d->classes * d->k * 4 : 0));
+            take(std::max({both_plan(d).parts > 1 ? size_t(both_plan(d).parts) * rows * d->k * 4 : 0, pi.parts > 1 ? size_t(pi.parts) * rows * d->k * 4 : 0, pw.parts > 1 ? size_t(pw.parts) * d->classes * d->k * 4 : 0}));
     }
     s.bytes = at;
     return s;
@@ -166,6 +189,26 @@ int weight_grad(hipStream_t st, const nhip_head_desc *d, const PartPlan &p, int6
 }
 #undef NHIP_HEAD_PRODUCT
 
+template <bool F16, class InOut>
+int both_go(hipStream_t st, const HeadBoth<InOut> &x, const uint16_t *d) {
+    const int ti = x.input.tiles_m * x.input.tiles_n, tw = x.weight.tiles_m * x.weight.tiles_n;
+    return launch(st, head_both_grads<F16, InOut>, dim3(unsigned(ti * x.parts + tw)), kLds128, "head_both_grads launch", x, d);
+}
+
+// input_grad and weight_grad of the only piece.
+template <bool F16>
+int both_grads(hipStream_t st, const nhip_head_desc *d, const BothPlan &p, const uint16_t *codes, const uint16_t *w, int64_t w_n,
+               const uint16_t *h, int64_t h_m, float *part, const HeadStore &dh, const HeadStore &dw) {
+    GemmShape i = shape(d->rows, d->k, d->classes, 128), s = shape(d->classes, d->k, d->rows, 128);
+    i.a_m = blocks_of(d) * 64, i.a_k = 1, i.b_k = w_n, i.b_n = 1;
+    s.a_m = 1, s.a_k = blocks_of(d) * 64, s.b_k = h_m, s.b_n = 1;
+    const int all = int((d->rows + 63) / 64);
+    if (p.parts == 1) return both_go<F16>(st, HeadBoth<HeadStore>{i, s, w, h, dh, dw, 1, p.k_part, all}, codes);
+    i.d_split = i.m * i.n;
+    if (both_go<F16>(st, HeadBoth<AnyStore>{i, s, w, h, AnyStore{part, 0}, dw, p.parts, p.k_part, all}, codes)) return 1;
+    return parts_sum(st, part, PartPlan{128, p.parts, p.k_part, false, 0.0}, i.m * i.n, dh);
+}
+
 bool on(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 // A copy of `rows` rows at `dst`, by as many workgroups as it fills.
@@ -219,6 +262,12 @@ int head_run(hipStream_t st, const nhip_head_desc *d, const uint16_t *h, const u
         hipLaunchKernelGGL((head_grad_kernel<F16>), dim3(unsigned(rows)), dim3(256), 0, st, codes, part, picked, g + r0, scale, targets, blocks,
                            losses ? losses + r0 : nullptr);
         if (check(hipGetLastError(), "head_grad_kernel launch")) return 1;
+        if (const BothPlan both = both_plan(d); both.parts && dh && dw) {
+            if (both_grads<F16>(st, d, both, codes, w, w_n, hp, h_m, parts, HeadStore{nullptr, nullptr, dh, inverse, d->k, F16},
+                                HeadStore{nullptr, nullptr, dw, inverse, d->k, F16}))
+                return 1;
+            break;
+        }
         // a last piece of fewer rows keeps its plan: its sums are shorter, its tiles fewer
         if (dh && input_grad<F16>(st, d, pi, rows, codes, w, w_n, parts, HeadStore{nullptr, nullptr, dh + r0 * d->k, inverse, d->k, F16}))
             return 1;
