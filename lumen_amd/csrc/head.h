@@ -252,8 +252,8 @@ static __global__ __launch_bounds__(kPrepare) void head_prepare_kernel(HeadCopy 
     else head_copy(w, targets, group - h.groups);
 }
 
-// The codes of a piece's rows into d, in place: a workgroup a row, whose lse and loss it works out first, 8 classes a thread at a
-// time. The target's d is g expm1(-loss), which p - 1 would cancel. HBM bounds it; codes are read and d written once and are more
+// The codes of a piece's rows into d, in place: a workgroup a row (of few rows gridDim.y of them: 118 rows of
+// 21312 classes 6.1 us, 10.9 by one each; 271 of 31856 11.2, 17.1), whose lse and loss it works out first, 8 classes a thread at a time. The target's d is g expm1(-loss), which p - 1 would cancel. HBM bounds it; codes are read and d written once and are more
 // than the caches hold (nontemporal).
 template <bool F16>
 __global__ __launch_bounds__(256) void head_grad_kernel(uint16_t *__restrict__ codes, const float2 *__restrict__ part,
@@ -267,10 +267,10 @@ __global__ __launch_bounds__(256) void head_grad_kernel(uint16_t *__restrict__ c
     bool ignored;
     const int64_t cls = targets.at(row, ignored);
     const float l = float(lse), loss = float(lse - double(picked[row])), f = g[row] * scale[0];
-    if (losses && threadIdx.x == 0) losses[row] = ignored ? 0.0f : loss;
+    if (losses && threadIdx.x == 0 && blockIdx.y == 0) losses[row] = ignored ? 0.0f : loss;
     uint16_t *p = codes + row * blocks * 64;
     auto round = [](float v) { return uint32_t(F16 ? f32_to_f16(v) : f32_to_bf16(v)); };
-    for (int64_t c = 8 * threadIdx.x; c < blocks * 64; c += 2048) {
+    for (int64_t c = 8 * (threadIdx.x + 256 * blockIdx.y); c < blocks * 64; c += 2048 * gridDim.y) {
         words4 o = {0, 0, 0, 0};
         if (!ignored) {
             const words4 w = __builtin_nontemporal_load(reinterpret_cast<const words4 *>(p + c));

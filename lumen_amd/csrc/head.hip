@@ -39,6 +39,10 @@ PartPlan input_plan(const nhip_head_desc *d) {
 PartPlan weight_plan(const nhip_head_desc *d) {
     const int64_t total = (piece_rows(d) + 63) / 64;
     PartPlan p = part_plan(d->classes, d->k, 1, total, int64_t(1) << 30);
+    // few k tiles: the store is most of a tile, and two workgroups a CU hide one another's. Us with tiles of 256 rows and 128 (*
+    // taken), of rows, k, classes: 128, 2048, 32000 114 76*; 271, 2560, 31856 170 126*; 512, 512, 32000 42 33*; 1024, 1024, 32000
+    // 108 103*; 1536, 2048, 32000 262* 274; 2048, 512, 32000 82* 87; 4096, 512, 32000 135* 173
+    if (p.tm == 256 && p.parts == 1 && total <= 16) p = PartPlan{128, 1, int(total), false, p.us};
     // the pieces' sums are added in the store, which parts do without
     if (pieces_of(d) > 1 && p.parts > 1) p = PartPlan{256, 1, int(total), false, 0.0};
     return p;
@@ -259,7 +263,8 @@ int head_run(hipStream_t st, const nhip_head_desc *d, const uint16_t *h, const u
         const uint16_t *hp = h + r0 * h_m;
         targets.target = static_cast<const char *>(target) + r0 * tsize;
         if (logits<F16, true>(st, d, rows, hp, h_m, w, w_n, HeadOut<true>{part, picked, codes, targets, blocks})) return 1;
-        hipLaunchKernelGGL((head_grad_kernel<F16>), dim3(unsigned(rows)), dim3(256), 0, st, codes, part, picked, g + r0, scale, targets, blocks,
+        const unsigned shares = unsigned(std::clamp<int64_t>(1024 / rows, 1, (blocks + 31) / 32));
+        hipLaunchKernelGGL((head_grad_kernel<F16>), dim3(unsigned(rows), shares), dim3(256), 0, st, codes, part, picked, g + r0, scale, targets, blocks,
                            losses ? losses + r0 : nullptr);
         if (check(hipGetLastError(), "head_grad_kernel launch")) return 1;
         if (const BothPlan both = both_plan(d); both.parts && dh && dw) {
