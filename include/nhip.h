@@ -340,7 +340,8 @@ int nhip_clip_grad_norm_workspace(const nhip_clip_desc *desc, size_t *bytes);
  * ((softmax - onehot) g)^T h (each or null), sums float32, rounded once to the operands' type, ignored rows counting for
  * nothing. (softmax - onehot) g is rounded to the operands' type as an operand of the products, of at most piece_bytes'
  * worth of rows at a time (at least 256). Rows of a multiple of 64 elements that start on 16 bytes are read where they lie,
- * others (and the gradients' h) are copied. The same bits every run. `workspace` of nhip_head_loss_workspace bytes from a 256-byte address. */
+ * others (and the gradients' h) are copied. The same bits every run. `workspace` of nhip_head_loss_workspace bytes from a
+ * 256-byte address; its `gradients`: whether g is given, also where dh and dw are null. */
 typedef struct {
     int64_t rows, classes, k;
     int64_t h_m, w_n;           /* elements from a row to the next */

@@ -213,6 +213,23 @@ int both_grads(hipStream_t st, const nhip_head_desc *d, const BothPlan &p, const
     return parts_sum(st, part, PartPlan{128, p.parts, p.k_part, false, 0.0}, i.m * i.n, dh);
 }
 
+// The losses alone of h's rows where the products read them, as many rows at a time as the workspace holds maxima and sums of.
+template <bool F16>
+int losses_alone(hipStream_t st, const nhip_head_desc *d, int64_t most, const uint16_t *h, int64_t h_m, const uint16_t *w, int64_t w_n,
+                 HeadTargets targets, float2 *part, float *picked, float *losses) {
+    const int64_t blocks = blocks_of(d), tsize = targets.t64 ? 8 : 4;
+    const char *target = static_cast<const char *>(targets.target);
+    for (int64_t r0 = 0; r0 < d->rows; r0 += most) {
+        const int64_t rows = std::min(most, d->rows - r0);
+        targets.target = target + r0 * tsize;
+        if (logits<F16, false>(st, d, rows, h + r0 * h_m, h_m, w, w_n, HeadOut<false>{part, picked, nullptr, targets, blocks})) return 1;
+        hipLaunchKernelGGL(head_merge_kernel, dim3(unsigned(std::min<int64_t>(rows, 1 << 20))), dim3(256), 0, st, part, picked, targets, rows,
+                           blocks, losses + r0);
+        if (check(hipGetLastError(), "head_merge_kernel launch")) return 1;
+    }
+    return 0;
+}
+
 bool on(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 // A copy of `rows` rows at `dst`, by as many workgroups as it fills.
@@ -224,8 +241,11 @@ HeadCopy copy_of(const uint16_t *src, int64_t rows, int64_t ld, int64_t k, int64
 template <bool F16>
 int head_run(hipStream_t st, const nhip_head_desc *d, const uint16_t *h, const uint16_t *w, const void *target, const float *g,
              float *losses, uint16_t *dh, uint16_t *dw, char *ws) {
-    const bool grad = g != nullptr;
-    const HeadSpace at = head_space(d, grad);
+    // the workspace is laid out by whether there are cotangents, as its size is asked for, also where neither gradient is wanted
+    const HeadSpace at = head_space(d, g != nullptr);
+    const bool grad = dh || dw;
+    const int64_t most = g ? piece_rows(d) : d->rows;
+    if (!grad) g = nullptr;
     const int64_t kp = padded_k(d), blocks = blocks_of(d), tsize = d->target_dtype == NHIP_LCE_I64 ? 8 : 4;
     int64_t h_m = d->h_m, w_n = d->w_n;
     HeadTargets targets{target, d->ignore_index, d->classes, d->target_dtype == NHIP_LCE_I64};
@@ -248,14 +268,9 @@ int head_run(hipStream_t st, const nhip_head_desc *d, const uint16_t *h, const u
                            scale);
         if (check(hipGetLastError(), "head_prepare_kernel launch")) return 1;
     }
-    if (!grad) {
-        if (logits<F16, false>(st, d, d->rows, h, h_m, w, w_n, HeadOut<false>{part, picked, nullptr, targets, blocks})) return 1;
-        hipLaunchKernelGGL(head_merge_kernel, dim3(unsigned(std::min<int64_t>(d->rows, 1 << 20))), dim3(256), 0, st, part, picked, targets, d->rows,
-                           blocks, losses);
-        return check(hipGetLastError(), "head_merge_kernel launch");
-    }
+    if (!grad) return losses_alone<F16>(st, d, most, h, h_m, w, w_n, targets, part, picked, losses);
     const PartPlan pi = input_plan(d), pw = weight_plan(d);
-    const int64_t most = piece_rows(d), pieces = pieces_of(d);
+    const int64_t pieces = pieces_of(d);
     float *sums = reinterpret_cast<float *>(ws + at.weight_sums), *parts = reinterpret_cast<float *>(ws + at.input_parts);
     const float *inverse = scale + 1;
     for (int64_t i = 0, r0 = 0; i < pieces; ++i, r0 += most) {
@@ -293,10 +308,9 @@ int head_on(hipStream_t st, const nhip_head_desc *d, const void *h, const void *
             void *dh, void *dw, void *ws) {
     if (head_check(d, "nhip_head_loss")) return 1;
     if (!g && (dh || dw)) return fail("nhip_head_loss: gradients need the losses' cotangents");
-    if (g && !dh && !dw) g = nullptr;
     if (!on(ws, 256)) return fail("nhip_head_loss: the workspace starts on 256 bytes");
     if (!on(dh, 8) || !on(dw, 8)) return fail("nhip_head_loss: gradients start on 8 bytes");
-    if ((!g && !copies(d, d->h_m) && !on(h, 16)) || (!copies(d, d->w_n) && !on(w, 16)))
+    if ((!dh && !dw && !copies(d, d->h_m) && !on(h, 16)) || (!copies(d, d->w_n) && !on(w, 16)))
         return fail("nhip_head_loss: operands of whole rows start on 16 bytes");
     if (d->rows == 0) return dw ? fill_on(st, dw, size_t(d->classes) * d->k * 2, 0) : 0;
     if (!ws) return fail("nhip_head_loss: no workspace");

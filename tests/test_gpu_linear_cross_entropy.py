@@ -328,3 +328,26 @@ def test_refusals_of_the_entry_point(hip):
                dict(ws=one.ptr + 16), dict(dh=one.ptr + 2), dict(g=None, dh=None, h=one.ptr + 2), dict(rows=1 << 31), dict(h=None)):
         with pytest.raises(RuntimeError, match="nhip_head_loss"):
             call(**kw)
+
+
+@pytest.mark.parametrize("given", [True, False])
+def test_losses_alone_stay_within_the_workspace_of_the_call(hip, given):
+    """With cotangents and neither gradient wanted the workspace is the gradients', which holds the maxima and sums of one piece's
+    rows and is smaller than those of all rows. What lies behind it is left as it was."""
+    t, k, v = 20000, 64, 3000
+    h, w, target, g = _case(31, t, k, v, "bfloat16")
+    d = nv.HeadDesc(rows=t, classes=v, k=k, h_m=k, w_n=k, ignore_index=IGNORED, piece_bytes=1, dtype=1, target_dtype=1)
+    size = C.c_size_t()
+    nv.call("nhip_head_loss_workspace", C.byref(d), int(given), C.byref(size))
+    blocks = -(-v // 64)
+    assert not given or size.value < t * blocks * 8
+    behind = t * blocks * 8
+    ws = Dev(np.full(size.value + behind, 0x5a, np.uint8))
+    dev = [Dev(np.array(D.from_values(x.astype(np.float32), "bfloat16"))) for x in (h, w)] + [Dev(target.astype(np.int64)), Dev(g)]
+    out = Dev(np.full(t, np.nan, np.float32))
+    nv.call("nhip_head_loss", C.byref(d), dev[0].ptr, dev[1].ptr, dev[2].ptr, dev[3].ptr if given else None, out.ptr, None, None, ws.ptr)
+    losses = out.get(t, np.float32)
+    for lo in range(0, t, 4000):
+        part = (h[lo:lo + 4000], w, target[lo:lo + 4000], IGNORED, g[lo:lo + 4000])
+        _near(losses[lo:lo + 4000], M.linear_cross_entropy(*part)[0], M.linear_cross_entropy_tolerances(*part, "bfloat16")[0])
+    assert np.all(ws.get(size.value + behind, np.uint8)[size.value:] == 0x5a)
