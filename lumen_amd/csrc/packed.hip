@@ -94,7 +94,7 @@ int packed_check(const nhip_packed_desc *d, const char *what) {
           attn_span_ok(d->tokens, d->v_s, hv) && attn_span_ok(d->tokens, d->do_s, hv)))
         return fail(at + ": head dims " + std::to_string(d->head_dim) + " / " + std::to_string(hv) + " are padded to " +
                     std::to_string(kd) + ", which needs each head of an operand within 2 GiB");
-    if (std::max(table_entries(d, 64), d->tokens / 8 + 1) * std::max<int64_t>(d->heads, 1) >= int64_t(1) << 24)
+    if (std::max(table_entries(d, 64), d->tokens / 8 + 1) * std::max<int64_t>({d->heads, d->kv_heads, 1}) >= int64_t(1) << 24)
         return fail(at + ": a launch of 2^32 threads");
     return 0;
 }
@@ -166,9 +166,10 @@ int bwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, const ui
     float *lse2 = p.delta + size_t(d->heads) * d->tokens;
     constexpr int RPB = 256 / (D / 8);
     const int tables = few(d) ? 2 : 0;
-    hipLaunchKernelGGL((packed_prep_kernel<D, F16>), dim3(unsigned((d->heads * d->tokens + RPB - 1) / RPB + tables)), dim3(256), 0, st, p, rest,
-                       lse2, a, tables);
-    if (check(hipGetLastError(), "packed delta launch")) return 1;
+    if (const int64_t blocks = (d->heads * d->tokens + RPB - 1) / RPB + tables) {
+        hipLaunchKernelGGL((packed_prep_kernel<D, F16>), dim3(unsigned(blocks)), dim3(256), 0, st, p, rest, lse2, a, tables);
+        if (check(hipGetLastError(), "packed delta launch")) return 1;
+    }
     const dim3 gq(unsigned(a.t[1].most * d->heads));
     const int32_t *fits = store && again ? a.fits : nullptr;
     if (store) {
@@ -178,6 +179,7 @@ int bwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, const ui
     }
     if (again) {
         if (dkdv<D, F16, CAUSAL>(st, d, p, a, lse2, fits, sums, false)) return 1;
+        if (!d->heads) return 0;  // no query: no tile to add to dK and dV, zeros
         hipLaunchKernelGGL((packed_dq_kernel<D, F16, CAUSAL>), gq, dim3(256), 0, st, p, lse2, a.t[1].tiles, d->tokens, fits);
         if (check(hipGetLastError(), "packed_dq_kernel launch")) return 1;
     }
@@ -215,9 +217,9 @@ int packed_fwd_on(hipStream_t st, const nhip_packed_desc *d, const void *q, cons
 int packed_bwd_on(hipStream_t st, const nhip_packed_desc *d, const void *q, const void *k, const void *v, const void *offsets,
                   const void *o, const void *rest, const void *d_o, const float *lse, void *dq, void *dk, void *dv, void *ws) {
     if (packed_check(d, "nhip_packed_bwd") || on16("nhip_packed_bwd", {q, k, v, o, rest, d_o, dq, dk, dv, ws})) return 1;
-    if (d->tokens == 0 || d->heads == 0) return 0;
+    if (d->tokens == 0 || d->kv_heads == 0) return 0;
     if (!ws) return fail("nhip_packed_bwd: no workspace");
-    if (given("nhip_packed_bwd", {q, k, v, offsets, o, d_o, lse, dq, dk, dv})) return 1;
+    if (given("nhip_packed_bwd", {k, v, offsets, dk, dv}) || (d->heads && given("nhip_packed_bwd", {q, o, d_o, lse, dq}))) return 1;
     const BwdSpace w = bwd_space(d);
     char *at = static_cast<char *>(ws);
     AttnParams p = packed_params(d);

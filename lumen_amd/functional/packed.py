@@ -99,10 +99,10 @@ def _gradients(q, k, v, offsets, o, rest, lse, do, scale, causal):
 
 
 def _taken(q, k, v, offsets):
-    (t, n, d), dv = q.shape, v.shape[2]
+    (t, n, d), (nkv, dv) = q.shape, v.shape[1:]
     most = max(t // 64 + min(offsets.shape[0] - 1, t) + 2, t // 8 + 1)
     return q.dtype in ("bfloat16", "float16") and all(x % 8 == 0 and 0 < x <= 128 for x in (d, dv)) \
-        and t <= MAX_TOKENS and offsets.shape[0] - 1 <= MAX_SEQUENCES and most * n < 1 << 24
+        and t <= MAX_TOKENS and offsets.shape[0] - 1 <= MAX_SEQUENCES and most * max(n, nkv) < 1 << 24
 
 
 class _PackedAttention(Function):

@@ -359,3 +359,24 @@ def test_refusals_of_the_entry_points(hip):
         with pytest.raises(RuntimeError, match="without memory"):
             nv.call("nhip_packed_bwd", desc(), *[None if i == at else one.ptr for i in range(11)], one.ptr)
     nv.call("nhip_packed_fwd", desc(tokens=0), None, None, None, None, None, None, None, None)  # nothing to do
+
+
+@pytest.mark.parametrize("sequences", [2, 300])
+def test_key_heads_without_a_query_head(hip, sequences):
+    """Nothing adds to their gradients, which are zeros and not what the memory held: of tables by either builder, a sequence's tokens
+    and those of none."""
+    t, nkv, d = 400, 2, 64
+    offsets = np.concatenate([[3], np.sort(np.random.default_rng(3).integers(3, 390, sequences))]).astype(np.int32)
+    desc = nv.PackedDesc(tokens=t, sequences=sequences, heads=0, kv_heads=nkv, head_dim=d, dtype=1, causal=1, offsets_dtype=1, scale=1.0,
+                         ds_bytes=1 << 20, k_s=nkv * d, k_n=d, v_s=nkv * d, v_n=d, dk_s=nkv * d, dk_n=d, dv_s=nkv * d, dv_n=d)
+    size = C.c_size_t()
+    nv.call("nhip_packed_workspace", C.byref(desc), 1, C.byref(size))
+    ones = Dev(np.full(t * nkv * d, 0x3f80, np.uint16))
+    dk, dv, at, ws = Dev(np.full(t * nkv * d, 0x3f80, np.uint16)), Dev(np.full(t * nkv * d, 0x3f80, np.uint16)), Dev(offsets), Dev(nbytes=size.value)
+    nv.call("nhip_packed_bwd", C.byref(desc), None, ones.ptr, ones.ptr, at.ptr, None, None, None, None, None, dk.ptr, dv.ptr, ws.ptr)
+    for x in (dk, dv):
+        assert not x.get(t * nkv * d, np.uint16).any()
+    q, kv = np.zeros((t, 0, d)), np.ones((t, nkv, d))
+    out = L.compile(_program(True), device="hip")(_tensor(q, "bfloat16"), _tensor(kv, "bfloat16"), _tensor(kv, "bfloat16"), L.from_numpy(offsets),
+                                                  _tensor(q, "bfloat16"))
+    assert [_values(a).shape for a in out] == [q.shape, q.shape, kv.shape, kv.shape] and not any(_values(a).any() for a in out)
