@@ -153,7 +153,9 @@ __global__ __launch_bounds__(TM * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 // exp(x) of a block's or a wave's maximum less a larger one.
 __device__ __forceinline__ float head_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 
-// A row's log-sum-exp from its blocks' maxima and sums, by a workgroup: float64 from the blocks on.
+// A row's log-sum-exp from its blocks' maxima and sums, by a workgroup: float64 from the blocks on. A block without a term (columns past
+// the classes, logits of -inf) has a sum of 0 and is left out by it, not by its maximum: a NaN is in its block's sum and in no
+// maximum, which of a block that holds nothing else is -inf.
 __device__ __forceinline__ double head_lse(const float2 *__restrict__ p, int64_t blocks) {
     __shared__ float most[4];
     __shared__ double sums[4];
@@ -165,7 +167,7 @@ __device__ __forceinline__ double head_lse(const float2 *__restrict__ p, int64_t
     double sum = 0.0;
     for (int64_t j = threadIdx.x; j < blocks; j += 256) {
         const float2 q = p[j];
-        if (q.x != -INFINITY) sum += double(q.y) * double(head_exp(q.x - m));
+        if (q.y != 0.0f) sum += double(q.y) * double(head_exp(q.x - m));
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
@@ -175,7 +177,7 @@ __device__ __forceinline__ double head_lse(const float2 *__restrict__ p, int64_t
     sum = 0.0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (most[i] != -INFINITY) sum += sums[i] * double(head_exp(most[i] - top));
+        if (sums[i] != 0.0) sum += sums[i] * double(head_exp(most[i] - top));
     return double(top) + log(sum);
 }
 

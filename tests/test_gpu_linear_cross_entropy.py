@@ -351,3 +351,34 @@ def test_losses_alone_stay_within_the_workspace_of_the_call(hip, given):
         part = (h[lo:lo + 4000], w, target[lo:lo + 4000], IGNORED, g[lo:lo + 4000])
         _near(losses[lo:lo + 4000], M.linear_cross_entropy(*part)[0], M.linear_cross_entropy_tolerances(*part, "bfloat16")[0])
     assert np.all(ws.get(size.value + behind, np.uint8)[size.value:] == 0x5a)
+
+
+@pytest.mark.parametrize("classes,bad", [(65, [64]), (64, [5]), (500, [130]), (9000, range(4096)), (9000, [8999])])
+def test_a_nan_among_the_weights_reaches_every_loss(hip, classes, bad):
+    """Wherever its class lies: alone in the last block of 64, among others, in every block that a wavefront adds up."""
+    t, k = 40, 64
+    h, w, target, g = _case(41, t, k, classes, "bfloat16")
+    target[:3] = [IGNORED, 1, 2]
+    w[list(bad), 7] = np.nan
+    args = [_tensor(h, "bfloat16"), _tensor(w, "bfloat16"), L.from_numpy(target)]
+    forward = L.compile(lambda h, w, target: [F.linear_cross_entropy(h, w, target, IGNORED, "none")], device="hip")
+    both = L.compile(_program(), device="hip")(*args, L.from_numpy(g))
+    kept = target != IGNORED
+    for losses in (forward(*args)[0], both[0]):
+        losses = _values(losses)
+        assert np.isnan(losses[kept]).all() and not losses[~kept].any()
+    assert np.isnan(_values(both[1])[kept]).all() and np.isnan(_values(both[2])).all()
+
+
+def test_classes_of_minus_infinity_count_for_nothing(hip):
+    """Logits of -inf, alone in the last block of 64 and throughout a wavefront's: the losses of the other classes."""
+    k = 64
+    h, w, target, g = _case(42, 40, k, 4160, "bfloat16")
+    h[:, 7] = _round(np.abs(h[:, 7]) + 0.5, "bfloat16")
+    target %= 64
+    forward = L.compile(lambda h, w, target: [F.linear_cross_entropy(h, w, target, IGNORED, "none")], device="hip")
+    for classes in (65, 4160):
+        some = w[:classes].copy()
+        some[64:, 7] = -np.inf
+        (losses,) = forward(_tensor(h, "bfloat16"), _tensor(some, "bfloat16"), L.from_numpy(target))
+        _check([_values(losses), None, None], h, w[:64], target, g, "bfloat16")
