@@ -349,7 +349,8 @@ def _lower_packed(plan, step):
     else:
         names.append(("o", out[0]))
     for name, loc in names:
-        d_s, d_n = loc.strides[:2]
+        # the library takes strides of whole 16 bytes; that of an axis of one element, any number in a view, is not used
+        d_s, d_n = (0 if n == 1 else st for n, st in zip(loc.shape, loc.strides[:2]))
         setattr(d, f"{name}_s", d_s)
         setattr(d, f"{name}_n", d_n)
     scratch = plan.scratch[id(step)]

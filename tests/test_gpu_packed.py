@@ -380,3 +380,24 @@ def test_key_heads_without_a_query_head(hip, sequences):
     out = L.compile(_program(True), device="hip")(_tensor(q, "bfloat16"), _tensor(kv, "bfloat16"), _tensor(kv, "bfloat16"), L.from_numpy(offsets),
                                                   _tensor(q, "bfloat16"))
     assert [_values(a).shape for a in out] == [q.shape, q.shape, kv.shape, kv.shape] and not any(_values(a).any() for a in out)
+
+
+@pytest.mark.parametrize("shape,view,t,n", [
+    ([40, 2, 68], lambda x: x[:, 0:1, :64], 40, 1), ([1, 1, 100], lambda x: x[:, :, :64], 1, 1), ([1, 4, 72], lambda x: x[:, :3, :64], 1, 3),
+    ([100 * 64], lambda x: x.reshape(100, 64, 1).permute(0, 2, 1) if isinstance(x, L.graph.tracer.TracedTensor) else x.reshape(100, 1, 64), 100, 1)])
+def test_axes_of_one_element_have_any_stride(hip, shape, view, t, n):
+    """One head and one token of views whose stride there is no multiple of 8 elements, read where they lie."""
+    rng = np.random.default_rng(t + n)
+    base = {name: _round(rng.standard_normal(shape), "bfloat16") for name in ("q", "k", "v", "do")}
+
+    def both(q, k, v, offsets, do):
+        return _program(True)(view(q), view(k), view(v), offsets, view(do))
+
+    offsets = np.array([0, t // 3, t])
+    want, tol = M.packed({name: view(x) for name, x in base.items()}, offsets, True, 0.125, "bfloat16")
+    f = L.compile(both, device="hip")
+    got = f(*(_tensor(base[name], "bfloat16") for name in "qkv"), L.from_numpy(offsets.astype(np.int32)), _tensor(base["do"], "bfloat16"))
+    for name, a, w, tt in zip(("o", "dq", "dk", "dv"), got, want, tol):
+        assert w.shape == (t, n, 64)
+        _near(_values(a), w, tt, name)
+    assert [st.kind for st in f.plan.steps if st.kind != "view"] == ["packed_fwd", "packed_bwd"]

@@ -162,3 +162,43 @@ def test_tables_and_stored_ds_hold_whatever_the_offsets_are():
             assert used <= tokens // block + min(count, tokens) + 2
         ds = sum(-(-x // 128) * -(-x // 64) for x in lengths)
         assert ds <= tokens * tokens // 8192 + 3 * tokens // 128 + 1 + min(count, tokens)
+
+
+def _lowered(program, *metas):
+    """``(step kind, PackedDesc, [(pointer slot, place)])`` of each packed step of the program's plan, as the library takes it: the
+    descriptor passes the checks that the launches make."""
+    from lumen_amd.compiler import operators
+
+    plan = Plan(L.make_graph(program)(*metas), build_kernels=False)
+    out = []
+    for st in plan.steps:
+        if st.kind in ("packed_fwd", "packed_bwd"):
+            _, raw, places = operators.lower(plan, st)
+            desc, n = nv.PackedDesc.from_buffer_copy(raw), C.c_size_t()
+            nv.call("nhip_packed_workspace", C.byref(desc), int(st.kind == "packed_bwd"), C.byref(n))
+            out.append((st.kind, desc, places))
+    assert out
+    return out
+
+
+UNIT_AXES = {  # a view's shape -> the operand [T, N, 64], whose axes of one element have odd strides
+    "a head of two": ([40, 2, 68], lambda x: x[:, 0:1, :64]),
+    "a token": ([1, 1, 100], lambda x: x[:, :, :64]),
+    "a token of three heads": ([1, 4, 72], lambda x: x[:, :3, :64]),
+    "a head by a permutation": ([100 * 64], lambda x: x.reshape(100, 64, 1).permute(0, 2, 1)),
+}
+
+
+@pytest.mark.parametrize("what", UNIT_AXES)
+def test_axes_of_one_element_have_any_stride(what):
+    shape, view = UNIT_AXES[what]
+
+    def both(q, k, v, offsets, do):
+        return _program(True)(view(q), view(k), view(v), offsets, view(do))
+
+    x = L.empty(shape, "bfloat16", "meta")
+    for _, desc, places in _lowered(both, x, x, x, L.empty([3], "int32", "meta"), x):
+        assert [loc.base[0] for _, loc in places][:3] == ["in"] * 3  # read where they lie
+        for name in ("q", "k", "v", "o"):
+            assert getattr(desc, f"{name}_s") == 0 or desc.tokens > 1
+            assert getattr(desc, f"{name}_n") == 0 or desc.heads > 1
