@@ -33,7 +33,6 @@ NHIP_DT = {"float32": 0, "bfloat16": 1, "float16": 2}
 # The last axis contiguous; rows that start on 16 bytes; these, or all of a length that the library copies itself; every
 # axis contiguous; and from 16 bytes on.
 ROWS, CHUNK_ROWS, WIDE_ROWS, DENSE, WIDE = "rows", "chunk rows", "wide rows", "dense", "wide"
-STRICTER = [ROWS, WIDE_ROWS, CHUNK_ROWS, DENSE, WIDE]
 
 
 def _wants(node):
@@ -61,20 +60,23 @@ def _fusions(step):
 
 
 def layouts(steps) -> dict:
-    """The layout that each value read by such a step must have (the stricter of its readers')."""
+    """The layouts that each value read by such steps must have, each of its readers' (none stands for another: rows on 16 bytes
+    need not be contiguous, nor contiguous ones start on 16)."""
     out = {}
     for st in steps:
         if st.kind in STEPS:
             for node in _fusions(st):
                 for v, want in zip(node.inputs, _wants(node)):
-                    out[v] = max(want, out.get(v, ROWS), key=STRICTER.index)
+                    out.setdefault(v, set()).add(want)
     return out
 
 
-def reads(loc, want) -> bool:
-    """Whether a place has the layout ``want`` (None: any)."""
-    if want is None:
-        return True
+def reads(loc, wants) -> bool:
+    """Whether a place has every layout of ``wants``."""
+    return all(_reads(loc, want) for want in wants)
+
+
+def _reads(loc, want) -> bool:
     if want in (WIDE, WIDE_ROWS, CHUNK_ROWS) and loc.offset * D.size_of(loc.dtype) % 16:
         return False
     if want in (DENSE, WIDE):

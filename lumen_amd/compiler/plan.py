@@ -463,7 +463,7 @@ class Plan:
                     loc = Loc(src.base, src.offset, _contig(t.shape), t.dtype, t.shape)
                 else:
                     loc = _view_of(n.prim, n.params, src, g.types[n.output])
-                if loc is not None and operators.reads(loc, layouts.get(n.output)):
+                if loc is not None and operators.reads(loc, layouts.get(n.output, ())):
                     self.loc[n.output] = loc
                     base_of[n.output] = base_of.get(n.inputs[0], n.inputs[0])
                     continue

@@ -10,6 +10,7 @@ from lumen_amd import dtypes as D
 from lumen_amd import workloads as W
 from lumen_amd.graph import prims
 from oracle import oracle
+from tests import training_math as M
 from tests.test_packed_step import documents, values
 
 pytestmark = pytest.mark.gpu
@@ -149,3 +150,33 @@ def test_the_clip_within_adamw_is_the_clip_ahead_of_it(hip):
         out = step(model, opt, *map(L.from_numpy, arrays))
         assert float(L.to_numpy(out[0])) == loss and float(L.to_numpy(out[1])) > 1.0
         assert all(np.array_equal(a, b) for a, b in zip(state, _state(opt)))
+
+
+def test_a_view_off_16_bytes_that_an_adamw_step_reads_too(hip):
+    """Its 8 bytes suit the AdamW step and not the attention or the head's loss, which have a copy of it."""
+    rng = np.random.default_rng(6)
+    t = 40
+    base = np.array(D.bf16_bits(rng.standard_normal(4 + t * 64).astype(np.float32)))
+    x = D.bf16_to_f32(base)[4:].astype(np.float64)
+    w = np.array(D.bf16_bits(rng.standard_normal((100, 64)).astype(np.float32) / 8))
+    target, offsets = rng.integers(0, 100, t), np.array([0, 13, t])
+    state = [np.zeros((t, 1, 64), np.float32), np.zeros((t, 1, 64), np.float32)]
+
+    def fn(base, m, v, offsets, target, w):
+        x = base[4:4 + t * 64].reshape(t, 1, 64)
+        rows = x.reshape(t, 64)
+        stepped = F.adamw([x, rows], [x, rows], [m, m.reshape(t, 64)], [v, v.reshape(t, 64)], 1, 0.1, weight_decay=0.0)[0]
+        return [F.packed_attention(x, x, x, offsets), F.linear_cross_entropy(rows, w, target, reduction="none"), *stepped]
+
+    args = [L.Tensor("bfloat16", base.shape, "cpu", host=base), *(L.from_numpy(a) for a in state), L.from_numpy(offsets), L.from_numpy(target),
+            L.Tensor("bfloat16", w.shape, "cpu", host=w)]
+    o, losses, *stepped = (np.asarray(L.to_numpy(a), np.float64) for a in L.compile(fn, device="hip")(*args))
+    heads = {name: x.reshape(t, 1, 64) for name in ("q", "k", "v", "do")}
+    want, tol = M.packed(heads, offsets, True, 0.125, "bfloat16")
+    assert np.all(np.abs(o - want[0]) <= tol[0])
+    row = (x.reshape(t, 64), D.bf16_to_f32(w).astype(np.float64), target, -100, np.ones(t))
+    assert np.all(np.abs(losses - M.linear_cross_entropy(*row)[0]) <= M.linear_cross_entropy_tolerances(*row, "bfloat16")[0])
+    zero = np.zeros(x.shape)
+    new, tw = M.adamw(x, x, zero, zero, 1, 0.1, (0.9, 0.999), 1e-8, 0.0)[0], M.adamw_tolerances(x, x, zero, zero, 1, 0.1, (0.9, 0.999), 1e-8, 0.0)[0]
+    for a in stepped:
+        assert np.all(np.abs(a.reshape(-1) - new) <= tw + 2.0**-8 * (np.abs(new) + tw))

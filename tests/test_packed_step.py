@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 import lumen_amd as L
+import lumen_amd.functional as F
 from lumen_amd import dtypes as D
 from lumen_amd import workloads as W
 from lumen_amd.compiler.plan import Plan
@@ -80,3 +81,33 @@ def test_the_plan_runs_the_operators():
     traced = trace(W.packed_train_step, (model, opt, *metas))
     kinds = [s.kind for s in Plan(traced.graph, build_kernels=False).steps]
     assert [kinds.count(k) for k in ("packed_fwd", "packed_bwd", "head_loss", "adamw", "clip")] == [2, 2, 1, 1, 1]
+
+
+def _places(program, *metas):
+    """The places of each operator step's pointers, by the step's kind."""
+    from lumen_amd.compiler import operators
+
+    plan = Plan(L.make_graph(program)(*metas), build_kernels=False)
+    return {st.kind: operators.lower(plan, st)[2] for st in plan.steps if st.kind in operators.STEPS}
+
+
+def test_a_view_off_16_bytes_that_an_adamw_step_reads_too():
+    """One value read where it lies (any contiguous place) by one step and from 16 bytes on by another has both."""
+    t = 40
+    base, state = L.empty([4 + t * 64], "bfloat16", "meta"), L.empty([t, 1, 64], "float32", "meta")
+    offsets, target, w = L.empty([3], "int32", "meta"), L.empty([t], "int32", "meta"), L.empty([100, 64], "bfloat16", "meta")
+
+    def attention(base, m, v, offsets):
+        x = base[4:4 + t * 64].reshape(t, 1, 64)
+        return [F.packed_attention(x, x, x, offsets), F.adamw([x], [x], [m], [v], 1, 0.1)[0][0]]
+
+    def loss(base, m, v, target, w):
+        x = base[4:4 + t * 64].reshape(t, 64)
+        m, v = m.reshape(t, 64), v.reshape(t, 64)
+        return [F.linear_cross_entropy(x, w, target), F.adamw([x], [x], [m], [v], 1, 0.1)[0][0]]
+
+    for places, kind, slots in ((_places(attention, base, state, state, offsets), "packed_fwd", (0, 1, 2)),
+                                (_places(loss, base, state, state, target, w), "head_loss", (0,))):
+        at = dict(places[kind])
+        assert all(at[s].offset * 2 % 16 == 0 for s in slots)
+        assert all(loc.contiguous() for _, loc in places["adamw"])
