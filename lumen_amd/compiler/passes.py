@@ -399,6 +399,20 @@ def _match_linear_cross_entropy(graph: Graph, dot, users, prod):
     return h, w, target, lse.output, loss.output
 
 
+def _needs_its_results(m, found, prod):
+    """Whether an operand of the match ``m`` is computed from one of its results, those of the matches ``found`` taking all of
+    their operands."""
+    seen, todo = set(), list(m[:3])
+    while todo:
+        v = todo.pop()
+        if v in m[3:]:
+            return True
+        if v not in seen:
+            seen.add(v)
+            todo += found[v][:3] if v in found else prod[v].inputs if v in prod else ()
+    return False
+
+
 def linear_cross_entropy(graph: Graph) -> Graph:
     """A cross entropy over logits h . w^T that nothing else reads becomes one ``linear_cross_entropy`` node
     (``passes/linear_cross_entropy.rs``, on by default like ``fused_linear_cross_entropy``): its [2, b] result's
@@ -409,7 +423,7 @@ def linear_cross_entropy(graph: Graph) -> Graph:
     for n in graph.nodes:
         if n.prim == "dot_general":
             m = _match_linear_cross_entropy(graph, n, users, prod)
-            if m is not None:
+            if m is not None and not _needs_its_results(m, found, prod):
                 found[m[3]] = m
                 found[m[4]] = m
     if not found:
@@ -420,22 +434,30 @@ def linear_cross_entropy(graph: Graph) -> Graph:
     remap = {}
     for v in graph.inputs:
         remap[v] = g.input(graph.types[v].dtype, graph.types[v].shape)
-    for n in graph.nodes:
-        ins = tuple(remap[v] for v in n.inputs)
-        g.backward = n.backward
-        m = found.get(n.output)
-        if m is None:
-            remap[n.output] = g.add_node(n.prim, ins, n.params, graph.types[n.output], n.backward)
-            continue
-        h, w, target, lse, loss = m
-        b = graph.types[h].shape[0]
-        if id(m) not in emitted:  # at the first of the two results, where h, w and the targets all exist
-            emitted[id(m)] = g.add_node("linear_cross_entropy", (remap[h], remap[w], remap[target]), {},
-                                        TensorType("float32", (2, b)), n.backward)
-        row = 1 if n.output == lse else 0
-        sl = g.add_node("slice", (emitted[id(m)],), {"start_indices": (row, 0), "limit_indices": (row + 1, b)},
-                        TensorType("float32", (1, b)), n.backward)
-        remap[n.output] = g.add_node("reshape", (sl,), {"new_sizes": (b,)}, TensorType("float32", (b,)), n.backward)
+    # both results take the targets, which the log-sum-exp by itself does not: what reads it waits for them
+    waiting = graph.nodes
+    while waiting:
+        later = []
+        for n in waiting:
+            m = found.get(n.output)
+            if not all(v in remap for v in (n.inputs if m is None else m[:3])):
+                later.append(n)
+                continue
+            g.backward = n.backward
+            if m is None:
+                ins = tuple(remap[v] for v in n.inputs)
+                remap[n.output] = g.add_node(n.prim, ins, n.params, graph.types[n.output], n.backward)
+                continue
+            h, w, target, lse, loss = m
+            b = graph.types[h].shape[0]
+            if id(m) not in emitted:
+                emitted[id(m)] = g.add_node("linear_cross_entropy", (remap[h], remap[w], remap[target]), {},
+                                            TensorType("float32", (2, b)), n.backward)
+            row = 1 if n.output == lse else 0
+            sl = g.add_node("slice", (emitted[id(m)],), {"start_indices": (row, 0), "limit_indices": (row + 1, b)},
+                            TensorType("float32", (1, b)), n.backward)
+            remap[n.output] = g.add_node("reshape", (sl,), {"new_sizes": (b,)}, TensorType("float32", (b,)), n.backward)
+        waiting = later
     g.backward = False
     g.set_outputs([remap[v] for v in graph.outputs])
     g.prune()

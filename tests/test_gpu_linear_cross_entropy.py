@@ -382,3 +382,15 @@ def test_classes_of_minus_infinity_count_for_nothing(hip):
         some[64:, 7] = -np.inf
         (losses,) = forward(_tensor(h, "bfloat16"), _tensor(some, "bfloat16"), L.from_numpy(target))
         _check([_values(losses), None, None], h, w[:64], target, g, "bfloat16")
+
+
+@pytest.mark.parametrize("target_type", ["int32", "int64"])
+def test_float32_losses_with_and_without_gradients(hip, target_type):
+    """As primitives, whose losses alone are the step of an eval loss over a product."""
+    h, w, target, g = _case(51, 70, 33, 130, "float32")
+    h, w = h.astype(np.float32), w.astype(np.float32)
+    args = [L.from_numpy(a) for a in (h, w, target.astype(target_type))]
+    forward = L.compile(lambda h, w, target: [F.linear_cross_entropy(h, w, target, IGNORED, "none")], device="hip")
+    _check([_values(forward(*args)[0]), None, None], h, w, target, g, "float32")
+    assert "linear_cross_entropy" in [st.kind for st in forward.plan.steps]
+    _check([_values(a) for a in L.compile(_program(), device="hip")(*args, L.from_numpy(g))], h, w, target, g, "float32")

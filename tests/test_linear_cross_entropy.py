@@ -221,3 +221,64 @@ def test_a_piece_holds_rows_of_h_within_a_buffer():
     nv.call("nhip_head_loss_workspace", C.byref(d), 1, C.byref(n))
     copy, sums, codes = rows * k * 2, v * k * 4, rows * 1024 * 2
     assert copy + sums + codes / 3 < n.value < copy + sums + codes / 2
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("target_type", ["int32", "int64"])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_losses_alone_of_primitives(dtype, target_type, reduction):
+    """Compiled and as traced, the same: targets of any type, which are clamped and converted behind the logits' sums."""
+    rng = np.random.default_rng(6)
+    h, w, target = _case(rng, (9,), 5, 11, dtype)
+    args = [h, w, target.astype(target_type)]
+    graph = L.make_graph(lambda h, w, t: [F.linear_cross_entropy(h, w, t, reduction=reduction)])(*(_meta(a) for a in args))
+    Plan(graph, build_kernels=False)
+    compiled, _ = compile_graph(graph)
+    assert [n.prim for n in compiled.nodes].count("linear_cross_entropy") == (dtype == "float32")
+    (a,), (b,) = oracle.values(graph, args), oracle.values(compiled, args)
+    losses = M.linear_cross_entropy(h, w, target, -100, np.ones(9))[0]
+    tol = M.linear_cross_entropy_tolerances(h, w, target, -100, np.ones(9), "float32")[0]
+    n = (target != -100).sum()
+    want = {"none": losses, "sum": losses.sum(), "mean": losses.sum() / n}[reduction]
+    limit = {"none": tol, "sum": tol.sum() + 1e-6 * losses.sum(), "mean": tol.sum() + 1e-6 * losses.sum()}[reduction]
+    assert np.all(np.abs(a - want) <= limit) and np.all(np.abs(b - want) <= limit)
+
+
+def test_a_target_that_depends_on_a_loss():
+    """A log-sum-exp that the targets of its own cross entropy, or of one whose log-sum-exp its targets take in turn, are computed from
+    stays as primitives; one after the other they become a step each. 1e-5: some 20 float32 roundings of values below 8."""
+    from lumen_amd.graph.tracer import dot
+
+    def parts(h, w, target):
+        t, v = h.shape[0], w.shape[0]
+        x = dot(h, w, (((1,), (1,)), ((), ())), "float32", "float32")
+        m = F.amax(x, -1, keepdim=True)
+        lse = m.reshape(t) + F.log(F.sum(F.exp(x - m), -1))
+        return x, lse, lambda target: lse - prims.gather(x.reshape(t * v), prims.iota("int64", [t], 0) * v + target, 0)
+
+    def classes(lse):
+        return F.where(prims.lt(lse, prims.full(lse.shape, 2.0, "float32")), prims.full(lse.shape, 1, "int64"), prims.full(lse.shape, 3, "int64"))
+
+    def own(h, w, u, t):
+        _, lse, loss = parts(h, w, t)
+        return [loss(classes(lse)), lse]
+
+    def crossed(h, w, u, t):
+        _, a, loss_a = parts(h, w, t)
+        _, b, loss_b = parts(h, u, t)
+        return [loss_a(classes(b)), loss_b(classes(a)), a, b]
+
+    def chained(h, w, u, t):
+        _, a, loss_a = parts(h, w, t)
+        _, b, loss_b = parts(h, u, t)
+        return [loss_a(t), loss_b(classes(a)), b]
+
+    rng = np.random.default_rng(7)
+    h, w, _ = _case(rng, (9,), 5, 11, "float32")
+    args = [h, w, rng.standard_normal((11, 5)).astype(np.float32), rng.integers(0, 11, 9)]
+    for program, count in ((own, 0), (crossed, 1), (chained, 2)):
+        graph = L.make_graph(program)(*(_meta(a) for a in args))
+        compiled, _ = compile_graph(graph)
+        assert [n.prim for n in compiled.nodes].count("linear_cross_entropy") == count, program.__name__
+        for a, b in zip(oracle.values(graph, args), oracle.values(compiled, args)):
+            assert np.abs(a - b).max() <= 1e-5
