@@ -61,13 +61,16 @@ def _fusions(step):
 
 def layouts(steps) -> dict:
     """The layouts that each value read by such steps must have, each of its readers' (none stands for another: rows on 16 bytes
-    need not be contiguous, nor contiguous ones start on 16)."""
+    need not be contiguous, nor contiguous ones start on 16). An eval loss's step over a product reads contiguous operands too."""
     out = {}
     for st in steps:
         if st.kind in STEPS:
             for node in _fusions(st):
                 for v, want in zip(node.inputs, _wants(node)):
                     out.setdefault(v, set()).add(want)
+        elif st.kind == "linear_cross_entropy":
+            for v in st.nodes[0].inputs:
+                out.setdefault(v, set()).add(DENSE)
     return out
 
 

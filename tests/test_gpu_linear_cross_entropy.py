@@ -394,3 +394,14 @@ def test_float32_losses_with_and_without_gradients(hip, target_type):
     _check([_values(forward(*args)[0]), None, None], h, w, target, g, "float32")
     assert "linear_cross_entropy" in [st.kind for st in forward.plan.steps]
     _check([_values(a) for a in L.compile(_program(), device="hip")(*args, L.from_numpy(g))], h, w, target, g, "float32")
+
+
+def test_float32_losses_of_views(hip):
+    rng = np.random.default_rng(52)
+    base, wide = rng.standard_normal((3, 10, 96)).astype(np.float32), rng.standard_normal((130, 80)).astype(np.float32)
+    target = rng.integers(0, 130, (3, 10))
+    f = L.compile(lambda x, w, t: [F.linear_cross_entropy(x[:, :, 32:], w[:, 16:], t, reduction="none")], device="hip")
+    (got,) = f(*(L.from_numpy(a) for a in (base, wide, target)))
+    rows = (base[:, :, 32:].reshape(30, 64), wide[:, 16:], target.reshape(30), IGNORED, np.ones(30))
+    _near(_values(got).reshape(30), M.linear_cross_entropy(*rows)[0], M.linear_cross_entropy_tolerances(*rows, "float32")[0])
+    assert "linear_cross_entropy" in [st.kind for st in f.plan.steps]

@@ -282,3 +282,22 @@ def test_a_target_that_depends_on_a_loss():
         assert [n.prim for n in compiled.nodes].count("linear_cross_entropy") == count, program.__name__
         for a, b in zip(oracle.values(graph, args), oracle.values(compiled, args)):
             assert np.abs(a - b).max() <= 1e-5
+
+
+STRIDED = {  # shapes of the input, weight and target, and what each is read as
+    "columns of rows of a batch": ([3, 10, 128], [50, 64], [3, 10], lambda x: x[:, :, 64:], lambda w: w, lambda t: t),
+    "columns of the weight": ([30, 64], [50, 128], [30], lambda x: x, lambda w: w[:, 64:], lambda t: t),
+    "a permuted weight": ([30, 64], [64, 10, 5], [30], lambda x: x, lambda w: w.permute(1, 2, 0).reshape(50, 64), lambda t: t),
+    "one row for all": ([1, 1, 64], [50, 64], [3, 10], lambda x: x.expand(3, 10, 64), lambda w: w, lambda t: t),
+    "a column of targets": ([30, 64], [50, 64], [30, 2], lambda x: x, lambda w: w, lambda t: t[:, 1]),
+}
+
+
+@pytest.mark.parametrize("what", STRIDED)
+def test_views_as_operands_of_primitives(what):
+    """The step that the losses alone become reads contiguous operands: the views that are none are copied."""
+    *shapes, of_x, of_w, of_t = STRIDED[what]
+    metas = [L.empty(s, d, "meta") for s, d in zip(shapes, ("float32", "float32", "int64"))]
+    plan = Plan(L.make_graph(lambda h, w, t: [F.linear_cross_entropy(of_x(h), of_w(w), of_t(t))])(*metas), build_kernels=False)
+    (step,) = [st for st in plan.steps if st.kind == "linear_cross_entropy"]
+    assert all(plan.loc[v].contiguous() for v in step.nodes[0].inputs)
