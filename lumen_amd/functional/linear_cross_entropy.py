@@ -62,12 +62,12 @@ def _gradients(h, w, target, g, ignore, p=None):
 
 def _taken(h, w):
     (t, k), v = h.shape, w.shape[0]
-    kp = -(-k // 64) * 64
+    kp, vp = -(-k // 64) * 64, -(-v // 64) * 64  # whole k tiles, and whole blocks of classes as their exponentials are kept
 
     def launch(m, n):
         return -(-m // 128) * -(-n // 128) < 1 << 24
 
-    return h.dtype in ("bfloat16", "float16") and 0 < kp < 1 << 20 and 0 < v < 1 << 22 and (v + 256) * kp < (1 << 30) - 1024 \
+    return h.dtype in ("bfloat16", "float16") and 0 < kp < 1 << 20 and 0 < vp < 1 << 22 and (v + 256) * kp < (1 << 30) - 1024 \
         and t < 1 << 26 and launch(t, v) and launch(v, k) and launch(t, k)
 
 

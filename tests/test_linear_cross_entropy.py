@@ -301,3 +301,41 @@ def test_views_as_operands_of_primitives(what):
     plan = Plan(L.make_graph(lambda h, w, t: [F.linear_cross_entropy(of_x(h), of_w(w), of_t(t))])(*metas), build_kernels=False)
     (step,) = [st for st in plan.steps if st.kind == "linear_cross_entropy"]
     assert all(plan.loc[v].contiguous() for v in step.nodes[0].inputs)
+
+
+@pytest.mark.parametrize("classes", [(1 << 22) - 64, (1 << 22) - 63, (1 << 22) - 1, 1 << 22])
+def test_the_most_classes_that_the_kernels_take(classes):
+    """What the library would refuse is primitives: blocks of 64 classes below 2^22 are the kernels'."""
+    g = _graph(lambda h, w, t: [F.linear_cross_entropy(h, w, t)], t=3, k=64, v=classes, g=None)
+    kinds = [st.kind for st in Plan(g, build_kernels=False).steps]
+    assert ("head_loss" in kinds) == (classes <= (1 << 22) - 64)
+
+
+def test_what_is_taken_is_what_the_library_takes():
+    """The sizes at which the kernels' rule ends, against the library's own check of them."""
+    from lumen_amd.functional.linear_cross_entropy import _taken
+
+    class Shaped:
+        dtype = "bfloat16"
+
+        def __init__(self, *shape):
+            self.shape = shape
+
+    def library(t, k, v):
+        n = C.c_size_t()
+        d = nv.HeadDesc(rows=t, classes=v, k=k, h_m=k, w_n=k, ignore_index=-100, piece_bytes=1 << 29, dtype=1, target_dtype=0)
+        try:
+            nv.call("nhip_head_loss_workspace", C.byref(d), 1, C.byref(n))
+        except RuntimeError:
+            return False
+        return True
+
+    seen = set()
+    for t, k, v in [(1, 64, (1 << 22) - 64 + i) for i in (-1, 0, 1, 63, 64)] + [((1 << 26) + i, 1, 1) for i in (-1, 0)] \
+            + [(1, (1 << 20) - 64 + i, 1) for i in (-1, 0, 1)] + [(1, 1024, (1 << 20) - 257 + i) for i in range(-2, 3)] \
+            + [((1 << 19) + i, 64, 128 * 4096) for i in (-128, 1)] + [(1 << 25, 64, 8192 + i) for i in (0, 1)] + [(1 << 25, 8192 + i, 64) for i in (0, 1)] \
+            + [(100, 4096, 262144 - 256 - i) for i in range(3)]:
+        taken = _taken(Shaped(t, k), Shaped(v, k))
+        seen.add(taken)
+        assert taken == library(t, k, v), (t, k, v)
+    assert seen == {True, False}
