@@ -88,8 +88,8 @@ def _reads(loc, want) -> bool:
         return False
     if want == CHUNK_ROWS:
         return all(n == 1 or st % 8 == 0 for n, st in zip(loc.shape[:-1], loc.strides))
-    if want == WIDE_ROWS and loc.shape[-1] % 8 == 0:  # [rows, k]; tiles of 256 rows within 2^31 bytes
-        return loc.strides[0] % 8 == 0 and 256 * loc.strides[0] + loc.shape[-1] < 1 << 30
+    if want == WIDE_ROWS and loc.shape[-1] % 8 == 0:  # [rows, k]; tiles of 256 rows within 2^31 bytes, as head_check has it
+        return loc.strides[0] % 8 == 0 and 256 * loc.strides[0] + loc.shape[-1] < (1 << 30) - 1024
     return True
 
 

@@ -339,3 +339,23 @@ def test_what_is_taken_is_what_the_library_takes():
         seen.add(taken)
         assert taken == library(t, k, v), (t, k, v)
     assert seen == {True, False}
+
+
+def test_rows_as_far_apart_as_the_library_reads_them():
+    """The distance up to which rows stay where they lie, against the library's own check of it."""
+    from lumen_amd.compiler import operators
+    from lumen_amd.compiler.plan import Loc
+
+    n, seen = C.c_size_t(), set()
+    for k in (64, 1024, 2048, 8192):
+        for stride in [(((1 << 30) - 1024 - k) // 256 + i) // 8 * 8 for i in range(-16, 24, 8)] + [1 << 22, 1 << 30]:
+            taken = operators.reads(Loc(("in", 0), 0, (stride, 1), "bfloat16", (300, k)), {operators.WIDE_ROWS})
+            d = nv.HeadDesc(rows=300, classes=10, k=k, h_m=stride, w_n=k, ignore_index=-100, piece_bytes=1 << 29, dtype=1, target_dtype=0)
+            try:
+                nv.call("nhip_head_loss_workspace", C.byref(d), 0, C.byref(n))
+                read = True
+            except RuntimeError:
+                read = False
+            seen.add(taken)
+            assert read or not taken, (k, stride)
+    assert seen == {True, False}
