@@ -3,6 +3,7 @@ of one length: the reference has no counterpart."""
 
 from __future__ import annotations
 
+import ctypes as C
 import math
 
 from lumen_amd.autograd.function import Function
@@ -98,17 +99,18 @@ def _gradients(q, k, v, offsets, o, rest, lse, do, scale, causal):
     return _inside(inside, *(x.to(dtype) for x in (dq, dk, dv)))
 
 
-def _taken(q, k, v, offsets):
+def _taken(q, k, v, offsets, scale):
     (t, n, d), (nkv, dv) = q.shape, v.shape[1:]
     most = max(t // 64 + min(offsets.shape[0] - 1, t) + 2, t // 8 + 1)
-    return q.dtype in ("bfloat16", "float16") and all(x % 8 == 0 and 0 < x <= 128 for x in (d, dv)) \
+    # the kernels' scale is float32: one that it rounds to 0 or to infinity is the primitives'
+    return q.dtype in ("bfloat16", "float16") and 0.0 < C.c_float(scale).value <= 3.4e38 and all(x % 8 == 0 and 0 < x <= 128 for x in (d, dv)) \
         and t <= MAX_TOKENS and offsets.shape[0] - 1 <= MAX_SEQUENCES and most * max(n, nkv) < 1 << 24
 
 
 class _PackedAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets, *, scale, causal):
-        o, rest, lse = _operator("packed_attention", _taken(q, k, v, offsets), [q, k, v, offsets],
+        o, rest, lse = _operator("packed_attention", _taken(q, k, v, offsets, scale), [q, k, v, offsets],
                                  lambda *xs: _forward(*xs, scale, causal), scale=scale, causal=causal)
         ctx.scale, ctx.causal = scale, causal
         ctx.save_for_backward(q, k, v, offsets, o, rest, lse)
@@ -124,7 +126,7 @@ class _PackedGradients(Function):
     def forward(ctx, do, q, k, v, offsets, o, rest, lse, *, scale, causal):
         ctx.scale, ctx.causal = scale, causal
         ctx.save_for_backward(do, q, k, v, offsets)
-        return _operator("packed_attention_backward", _taken(q, k, v, offsets), [q, k, v, offsets, o, rest, do, lse],
+        return _operator("packed_attention_backward", _taken(q, k, v, offsets, scale), [q, k, v, offsets, o, rest, do, lse],
                          lambda q, k, v, offsets, o, rest, do, lse: _gradients(q, k, v, offsets, o, rest, lse, do, scale, causal),
                          scale=scale, causal=causal)
 

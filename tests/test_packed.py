@@ -8,6 +8,7 @@ import pytest
 
 import lumen_amd as L
 import lumen_amd.functional as F
+from lumen_amd import dtypes as D
 from lumen_amd import native as nv
 from lumen_amd.compiler.plan import Plan
 from oracle import oracle
@@ -202,3 +203,28 @@ def test_axes_of_one_element_have_any_stride(what):
         for name in ("q", "k", "v", "o"):
             assert getattr(desc, f"{name}_s") == 0 or desc.tokens > 1
             assert getattr(desc, f"{name}_n") == 0 or desc.heads > 1
+
+
+@pytest.mark.parametrize("scale,kernel", [(1e-50, False), (1e-46, False), (2.0**-149, True), (1e-30, True), (3.4e38, True), (3.402e38, False), (1e300, False)])
+def test_scales_past_the_kernels_float32(scale, kernel):
+    """A positive number is a scale; the library takes those that are one in float32 too."""
+    def fn(q, k, v, offsets, do):
+        o, pull = L.vjp(lambda q, k, v: F.packed_attention(q, k, v, offsets, scale=scale), q, k, v)
+        return [o, *pull(do)]
+
+    kinds = [st.kind for st in Plan(_graph(20, 2, 2, 64, 2, program=fn), build_kernels=False).steps]
+    assert (kinds == ["packed_fwd", "packed_bwd"]) == kernel
+
+
+def test_a_scale_that_float32_rounds_to_zero():
+    """Scores of zero: the mean of the values seen."""
+    rng = np.random.default_rng(8)
+    offsets = M.offsets_of([2, 3])
+    x = {k: v.astype(np.float32) for k, v in M.packed_inputs(rng, 5, 2, 1, 8).items()}
+    bits = {k: D.bf16_bits(v) for k, v in x.items()}
+    g = L.make_graph(lambda q, k, v, o: [F.packed_attention(q, k, v, o, scale=1e-50)])(
+        *(_meta(bits[k], "bfloat16") for k in "qkv"), _meta(offsets))
+    (got,) = oracle.values(g, [bits["q"], bits["k"], bits["v"], offsets])
+    real = {k: D.bf16_to_f32(b).astype(np.float64) for k, b in bits.items()}
+    (want, *_), (tol, *_) = M.packed(real, offsets, True, 1e-50, "bfloat16")
+    assert np.all(np.abs(got - want) <= tol)
