@@ -1500,8 +1500,8 @@ class LoopKernel:
         O, Q = math.prod(oshape), math.prod(rshape)
         out_dt = g.types[red.output].dtype
         atomic = red.prim == "reduce_sum" and out_dt == "float32" and Q >= 64
-        chunk = max(1, min(Q, 64)) if atomic else Q
-        nchunks = -(-Q // chunk)
+        chunk = max(1, min(Q, 64) if atomic else Q)
+        nchunks = max(1, -(-Q // chunk))  # of nothing too: one that stores the identity
         if atomic and tuple(axes) == tuple(range(len(axes))) and O % 4 == 0 and O >= 256:
             # narrow sums ([8192, 512] -> [512]) take 64 columns x 16 row lanes a workgroup and longer chunks: as
             # many workgroups as 256 columns x 4 row lanes would give, a quarter of the atomic adds (the adds to

@@ -401,3 +401,19 @@ def test_axes_of_one_element_have_any_stride(hip, shape, view, t, n):
         assert w.shape == (t, n, 64)
         _near(_values(a), w, tt, name)
     assert [st.kind for st in f.plan.steps if st.kind != "view"] == ["packed_fwd", "packed_bwd"]
+
+
+@pytest.mark.parametrize("tokens,n,nkv", [(0, 2, 1), (5, 0, 2), (0, 0, 1)])
+def test_primitives_without_tokens_or_query_heads(hip, tokens, n, nkv):
+    """float32: gradients of zeros, and results of no elements."""
+    q, kv = np.zeros((tokens, n, 8), np.float32), np.ones((tokens, nkv, 8), np.float32)
+    args = [L.from_numpy(a) for a in (q, kv, kv, np.array([0, tokens // 2, tokens], np.int32), q)]
+    out = [_values(a) for a in L.compile(_program(True), device="hip")(*args)]
+    assert [a.shape for a in out] == [q.shape, q.shape, kv.shape, kv.shape] and not any(a.any() for a in out)
+
+
+def test_sums_over_nothing(hip):
+    """Of every axis, the first, the last, and both around one that is kept."""
+    f = L.compile(lambda x, y, z: [F.sum(x, 0), F.sum(y, 1), F.sum(z, (0, 2)), F.sum(x)], device="hip")
+    got = [_values(a) for a in f(*(L.from_numpy(np.zeros(s, np.float32)) for s in ((0, 300), (7, 0), (3, 5, 0))))]
+    assert [a.shape for a in got] == [(300,), (7,), (5,), ()] and not any(a.any() for a in got)

@@ -228,3 +228,10 @@ def test_a_scale_that_float32_rounds_to_zero():
     real = {k: D.bf16_to_f32(b).astype(np.float64) for k, b in bits.items()}
     (want, *_), (tol, *_) = M.packed(real, offsets, True, 1e-50, "bfloat16")
     assert np.all(np.abs(got - want) <= tol)
+
+
+@pytest.mark.parametrize("dtype,tokens,n,nkv,d", [("float32", 0, 2, 1, 8), ("float32", 5, 0, 2, 8), ("bfloat16", 0, 2, 2, 60), ("bfloat16", 5, 0, 2, 60),
+                                                  ("bfloat16", 5, 0, 2, 64)])
+def test_plans_without_tokens_or_query_heads(dtype, tokens, n, nkv, d):
+    kinds = [st.kind for st in Plan(_graph(tokens, n, nkv, d, 2, dtype), build_kernels=False).steps]
+    assert ("packed_bwd" in kinds) == (d == 64)
