@@ -932,7 +932,9 @@ class Plan:
             elif st.kind == "linear_cross_entropy":
                 n = st.nodes[0]
                 desc = self._lce_desc(n)
-                ops = [self.loc[u] for u in n.inputs] + [self.loc[n.output], self.scratch[id(st)]]
+                ops = [self.loc[u] for u in n.inputs] + [self.loc[n.output]]
+                if id(st) in self.scratch:  # none of no rows
+                    ops.append(self.scratch[id(st)])
                 rr = (nv.Reloc * len(ops))(*[reloc(i, l) for i, l in enumerate(ops)])
                 call("nhip_plan_add_builtin", plan, nv.NHIP_STEP_LCE, C.byref(desc), C.sizeof(desc), rr, len(ops))
             elif st.kind == "copy":

@@ -405,3 +405,15 @@ def test_float32_losses_of_views(hip):
     rows = (base[:, :, 32:].reshape(30, 64), wide[:, 16:], target.reshape(30), IGNORED, np.ones(30))
     _near(_values(got).reshape(30), M.linear_cross_entropy(*rows)[0], M.linear_cross_entropy_tolerances(*rows, "float32")[0])
     assert "linear_cross_entropy" in [st.kind for st in f.plan.steps]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_no_rows(hip, dtype):
+    """No loss, and gradients of zeros: of a step that nothing but the cotangent goes into, and of a mean."""
+    h, w, target, g = np.zeros((0, 24)), _round(np.ones((50, 24)), dtype), np.zeros(0, np.int64), np.zeros(0, np.float32)
+    args = [_tensor(h, dtype), _tensor(w, dtype), L.from_numpy(target)]
+    for out in (L.compile(_program(), device="hip")(*args, L.from_numpy(g)), L.compile(_program("mean"), device="hip")(*args, L.from_numpy(np.array(2.0, np.float32)))):
+        losses, dh, dw = (_values(a) for a in out)
+        assert losses.size in (0, 1) and not losses.any() and dh.shape == h.shape and dw.shape == w.shape and not dw.any()
+    (mean,) = L.compile(lambda h, w, t: [F.linear_cross_entropy(h, w, t)], device="hip")(*args)
+    assert float(_values(mean)) == 0.0
