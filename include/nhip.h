@@ -339,8 +339,9 @@ int nhip_clip_grad_norm_workspace(const nhip_clip_desc *desc, size_t *bytes);
  * cotangents g (float32 [rows]; null: no gradients) dh [rows, k] = ((softmax - onehot) g) w and dw [classes, k] =
  * ((softmax - onehot) g)^T h (each or null), sums float32, rounded once to the operands' type, ignored rows counting for
  * nothing. (softmax - onehot) g is rounded to the operands' type as an operand of the products, of at most piece_bytes'
- * worth of rows at a time (at least 256). Rows of a multiple of 64 elements that start on 16 bytes are read where they lie,
- * others (and the gradients' h) are copied. The same bits every run. `workspace` of nhip_head_loss_workspace bytes from a
+ * worth of rows at a time (at least 256); the losses alone take as many bytes' worth of maxima and sums of 64 classes.
+ * Rows of a multiple of 64 elements that start on 16 bytes are read where they lie, others (and the gradients' h) are
+ * copied. The same bits every run. `workspace` of nhip_head_loss_workspace bytes from a
  * 256-byte address; its `gradients`: whether g is given, also where dh and dw are null. */
 typedef struct {
     int64_t rows, classes, k;

@@ -50,7 +50,8 @@ class CompilerFlags:
     # linear_cross_entropy.py run as kernels of their own (off: traced as their
     # primitives)
     fused_operators: bool = True
-    # bytes of 16-bit exponentials that linear_cross_entropy's gradients hold at once (a piece of the rows', 256 at least)
+    # bytes of 16-bit exponentials that linear_cross_entropy's gradients hold at once (a piece of the rows', 256 at
+    # least); and of the float32 maxima and sums of 64 classes each that its losses alone do
     head_piece_bytes: int = 512 << 20
     _version: int = 0
 

@@ -31,6 +31,11 @@ int64_t piece_rows(const nhip_head_desc *d) {
     const int64_t pieces = (d->rows + most - 1) / most;
     return std::min(most, up((d->rows + pieces - 1) / pieces, 256));
 }
+// Rows of a piece of the losses alone: those whose blocks' maxima and sums fit the same bytes, a sixteenth of their codes.
+int64_t loss_rows(const nhip_head_desc *d) {
+    const int64_t fit = d->piece_bytes / (blocks_of(d) * int64_t(sizeof(float2)));
+    return std::min(std::max<int64_t>(fit / 256 * 256, 256), d->rows);
+}
 int64_t pieces_of(const nhip_head_desc *d) { return d->rows > 0 ? (d->rows + piece_rows(d) - 1) / piece_rows(d) : 0; }
 
 PartPlan input_plan(const nhip_head_desc *d) {
@@ -85,7 +90,7 @@ HeadSpace head_space(const nhip_head_desc *d, bool grad) {
         at += up256(bytes);
         return from;
     };
-    const int64_t kp = padded_k(d), rows = grad ? piece_rows(d) : d->rows;
+    const int64_t kp = padded_k(d), rows = grad ? piece_rows(d) : loss_rows(d);
     s.h = take(grad || copies(d, d->h_m) ? size_t(d->rows) * kp * 2 : 0);
     s.w = take(copies(d, d->w_n) ? size_t(d->classes) * kp * 2 : 0);
     s.part = take(size_t(rows) * blocks_of(d) * sizeof(float2));
@@ -244,7 +249,7 @@ int head_run(hipStream_t st, const nhip_head_desc *d, const uint16_t *h, const u
     // the workspace is laid out by whether there are cotangents, as its size is asked for, also where neither gradient is wanted
     const HeadSpace at = head_space(d, g != nullptr);
     const bool grad = dh || dw;
-    const int64_t most = g ? piece_rows(d) : d->rows;
+    const int64_t most = g ? piece_rows(d) : loss_rows(d);
     if (!grad) g = nullptr;
     const int64_t kp = padded_k(d), blocks = blocks_of(d), tsize = d->target_dtype == NHIP_LCE_I64 ? 8 : 4;
     int64_t h_m = d->h_m, w_n = d->w_n;

@@ -359,3 +359,17 @@ def test_rows_as_far_apart_as_the_library_reads_them():
             seen.add(taken)
             assert read or not taken, (k, stride)
     assert seen == {True, False}
+
+
+def test_scratch_of_the_losses_alone():
+    """Eight bytes a row and 64 classes, of as many rows as fit the piece's bytes: of 2^20 rows and 128256 classes (16.8 GB at once) 2^29."""
+    def workspace(rows, classes, piece):
+        n = C.c_size_t()
+        d = nv.HeadDesc(rows=rows, classes=classes, k=512, h_m=512, w_n=512, ignore_index=-100, piece_bytes=piece, dtype=1, target_dtype=0)
+        nv.call("nhip_head_loss_workspace", C.byref(d), 0, C.byref(n))
+        return n.value
+
+    assert workspace(1 << 20, 128256, 1 << 29) <= (1 << 29) + (1 << 20)
+    assert workspace(100, 128256, 1 << 29) >= 100 * 2004 * 8
+    assert 256 * 2004 * 8 <= workspace(1 << 20, 128256, 0) < 256 * 2004 * 8 + 2048
+    assert workspace(0, 10, 0) < 1024
