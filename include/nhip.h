@@ -391,8 +391,8 @@ int nhip_packed_workspace(const nhip_packed_desc *desc, int backward, size_t *by
  *   w' = w (1 - lr weight_decay) - lr / (1 - beta1^t) m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
  * with w the master where there is one (float32, of 16-bit weights; the weight is then written and not read) and else the
  * weight. Float32 throughout, the step's factors worked out in float64. lr_at (a device float64)
- * and step_at (on the device too, of step_type) are read in place of lr and step where they are not null. grad_scale_at: a device float32 that every gradient is multiplied by first, rounded to
- * its type again, or null. Results may be null where nothing reads them, and each may lie over the operand that it
+ * and step_at (on the device too, of step_type) are read in place of lr and step where they are not null. grad_scale_at: a
+ * device float32 that every gradient is multiplied by first, rounded to its type again, or null. Results may be null where nothing reads them, and each may lie over the operand that it
  * replaces, otherwise over none. One launch for each 44 tensors. */
 typedef struct {
     const void *param, *grad;

@@ -68,7 +68,8 @@ struct HeadOut {
     static constexpr int kPitch = 128 + 16, kStage = 32 * kPitch;  // a block of 32 rows
 
     template <int FM, int FN>
-    __device__ __forceinline__ void store(const GemmShape &s, const f32x16_t (&acc)[FM][FN], char *stage, int64_t rbase, int64_t cbase, int lane) const {
+    __device__ __forceinline__ void store(const GemmShape &s, const f32x16_t (&acc)[FM][FN], char *stage, int64_t rbase, int64_t cbase,
+                                          int lane) const {
         constexpr float kLog2e = 1.4426950408889634f;
         const int h = lane >> 5, l32 = lane & 31;
         int64_t cls[FM];
@@ -133,7 +134,8 @@ struct HeadOut {
                         typedef unsigned head_u32x4 __attribute__((ext_vector_type(4)));
                         const head_u32x4 v = *reinterpret_cast<const head_u32x4 *>(stage + row * kPitch + 16 * chunk);
                         const int64_t to = rbase + 32 * i + row;
-                        if (to < s.m) __builtin_nontemporal_store(v, reinterpret_cast<head_u32x4 *>(codes + to * blocks * 64 + c0 + 8 * chunk));
+                        uint16_t *at = codes + to * blocks * 64 + c0 + 8 * chunk;
+                        if (to < s.m) __builtin_nontemporal_store(v, reinterpret_cast<head_u32x4 *>(at));
                     }
                 }
             }
@@ -246,17 +248,19 @@ __device__ __forceinline__ void head_scale(const float *__restrict__ g, const He
 }
 
 // What comes ahead of the products, in one launch: unless g is null the scale, by the first workgroup, and the copies.
-static __global__ __launch_bounds__(kPrepare) void head_prepare_kernel(HeadCopy h, HeadCopy w, const float *__restrict__ g, HeadTargets targets,
-                                                                  int64_t rows, float top, float *__restrict__ scale) {
+static __global__ __launch_bounds__(kPrepare) void head_prepare_kernel(HeadCopy h, HeadCopy w, const float *__restrict__ g,
+                                                                       HeadTargets targets, int64_t rows, float top,
+                                                                       float *__restrict__ scale) {
     const int group = int(blockIdx.x) - (g ? 1 : 0);
     if (group < 0) head_scale(g, targets, rows, top, scale);
     else if (group < h.groups) head_copy(h, targets, group);
     else head_copy(w, targets, group - h.groups);
 }
 
-// The codes of a piece's rows into d, in place: a workgroup a row (of few rows gridDim.y of them: 118 rows of
-// 21312 classes 6.1 us, 10.9 by one each; 271 of 31856 11.2, 17.1), whose lse and loss it works out first, 8 classes a thread at a time. The target's d is g expm1(-loss), which p - 1 would cancel. HBM bounds it; codes are read and d written once and are more
-// than the caches hold (nontemporal).
+// The codes of a piece's rows into d, in place: a workgroup a row (of few rows gridDim.y of them: 118 rows of 21312 classes 6.1 us,
+// 10.9 by one each; 271 of 31856 11.2, 17.1), whose lse and loss it works out first, 8 classes a thread at a time. The target's d
+// is g expm1(-loss), which p - 1 would cancel. HBM bounds it; codes are read and d written once and are more than the caches hold
+// (nontemporal).
 template <bool F16>
 __global__ __launch_bounds__(256) void head_grad_kernel(uint16_t *__restrict__ codes, const float2 *__restrict__ part,
                                                         const float *__restrict__ picked, const float *__restrict__ g,
@@ -371,11 +375,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     extern __shared__ __align__(1024) char smem[];
     const uint32_t tiles = uint32_t(x.input.tiles_m) * uint32_t(x.input.tiles_n), at = blockIdx.x, input = tiles * uint32_t(x.parts);
     if (at < input)
-        gemm_stream_tile<F16, 64, 2, false, true, true, InOut, 128, 0, 5, 2>(x.input, d, x.w, x.input_out, smem, nullptr, x.input_part, at % tiles,
-                                                                             at / tiles);
+        gemm_stream_tile<F16, 64, 2, false, true, true, InOut, 128, 0, 5, 2>(x.input, d, x.w, x.input_out, smem, nullptr, x.input_part,
+                                                                             at % tiles, at / tiles);
     else
-        gemm_stream_tile<F16, 64, 2, true, true, true, HeadStore, 128, 0, 3, 2>(x.weight, d, x.h, x.weight_out, smem, nullptr, x.weight_part,
-                                                                                at - input, 0);
+        gemm_stream_tile<F16, 64, 2, true, true, true, HeadStore, 128, 0, 3, 2>(x.weight, d, x.h, x.weight_out, smem, nullptr,
+                                                                                x.weight_part, at - input, 0);
 }
 
 // Float32 sums of a product's parts, P[part][mn], added in order and stored as HeadStore stores a tile (of one row).

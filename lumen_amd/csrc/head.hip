@@ -54,8 +54,8 @@ PartPlan weight_plan(const nhip_head_desc *d) {
 }
 
 // Both products in one launch of at most two workgroups of 128-row tiles a CU, dh's in parts: parts 0 where one after the other is
-// estimated shorter, by part_plan's rates for a launch of so many workgroups. Us with the parts' sums, one after the other and together (* taken), of
-// rows, k, classes:
+// estimated shorter, by part_plan's rates for a launch of so many workgroups. Us with the parts' sums, one after the other and
+// together (* taken), of rows, k, classes:
 //   777, 520, 5003    40  31*      200, 1024, 5000  32  23*      128, 768, 8192   33  24*      900, 256, 8000   39  28*
 //   1500, 300, 3000   40  34*      64, 256, 1000    23  17*      1024, 512, 2048  33  28*      2000, 72, 63     23* 31
 struct BothPlan {
@@ -98,11 +98,13 @@ HeadSpace head_space(const nhip_head_desc *d, bool grad) {
     s.scale = take(8);
     if (grad) {
         const PartPlan pi = input_plan(d), pw = weight_plan(d);
+        const BothPlan both = both_plan(d);
+        auto parts_bytes = [](int64_t parts, int64_t elements) { return parts > 1 ? size_t(parts) * size_t(elements) * 4 : 0; };
         s.codes = take(size_t(rows) * blocks_of(d) * 64 * 2);
         s.weight_sums = take(pieces_of(d) > 1 ? size_t(d->classes) * d->k * 4 : 0);
         // the parts of one product at a time
         s.input_parts = s.weight_parts =
-            take(std::max({both_plan(d).parts > 1 ? size_t(both_plan(d).parts) * rows * d->k * 4 : 0, pi.parts > 1 ? size_t(pi.parts) * rows * d->k * 4 : 0, pw.parts > 1 ? size_t(pw.parts) * d->classes * d->k * 4 : 0}));
+            take(std::max({parts_bytes(both.parts, rows * d->k), parts_bytes(pi.parts, rows * d->k), parts_bytes(pw.parts, d->classes * d->k)}));
     }
     s.bytes = at;
     return s;
@@ -155,7 +157,9 @@ int logits(hipStream_t st, const nhip_head_desc *d, int64_t rows, const uint16_t
     GemmShape s = shape(rows, d->classes, padded_k(d), tm);
     s.a_m = h_m, s.a_k = 1, s.b_k = 1, s.b_n = w_n;
     const dim3 grid(unsigned(s.tiles_m) * unsigned(s.tiles_n));
-    if (tm == 256) return launch<512>(st, head_logits_kernel<F16, 256, GRAD>, grid, gemm_stream_lds_bytes<64, 4>(), "head_logits_kernel launch", s, h, w, out);
+    if (tm == 256)
+        return launch<512>(st, head_logits_kernel<F16, 256, GRAD>, grid, gemm_stream_lds_bytes<64, 4>(), "head_logits_kernel launch", s, h,
+                           w, out);
     return launch(st, head_logits_kernel<F16, 128, GRAD>, grid, kLds128, "head_logits_kernel launch", s, h, w, out);
 }
 
@@ -227,7 +231,8 @@ int losses_alone(hipStream_t st, const nhip_head_desc *d, int64_t most, const ui
     for (int64_t r0 = 0; r0 < d->rows; r0 += most) {
         const int64_t rows = std::min(most, d->rows - r0);
         targets.target = target + r0 * tsize;
-        if (logits<F16, false>(st, d, rows, h + r0 * h_m, h_m, w, w_n, HeadOut<false>{part, picked, nullptr, targets, blocks})) return 1;
+        const HeadOut<false> out{part, picked, nullptr, targets, blocks};
+        if (logits<F16, false>(st, d, rows, h + r0 * h_m, h_m, w, w_n, out)) return 1;
         hipLaunchKernelGGL(head_merge_kernel, dim3(unsigned(std::min<int64_t>(rows, 1 << 20))), dim3(256), 0, st, part, picked, targets, rows,
                            blocks, losses + r0);
         if (check(hipGetLastError(), "head_merge_kernel launch")) return 1;
@@ -269,8 +274,8 @@ int head_run(hipStream_t st, const nhip_head_desc *d, const uint16_t *h, const u
     uint16_t *codes = reinterpret_cast<uint16_t *>(ws + at.codes);
     if (!grad && !losses) return 0;
     if (const int groups = hc.groups + wc.groups + grad) {
-        hipLaunchKernelGGL(head_prepare_kernel, dim3(unsigned(groups)), dim3(kPrepare), 0, st, hc, wc, g, targets, d->rows, F16 ? 16384.0f : 1.0f,
-                           scale);
+        hipLaunchKernelGGL(head_prepare_kernel, dim3(unsigned(groups)), dim3(kPrepare), 0, st, hc, wc, g, targets, d->rows,
+                           F16 ? 16384.0f : 1.0f, scale);
         if (check(hipGetLastError(), "head_prepare_kernel launch")) return 1;
     }
     if (!grad) return losses_alone<F16>(st, d, most, h, h_m, w, w_n, targets, part, picked, losses);
@@ -284,8 +289,8 @@ int head_run(hipStream_t st, const nhip_head_desc *d, const uint16_t *h, const u
         targets.target = static_cast<const char *>(target) + r0 * tsize;
         if (logits<F16, true>(st, d, rows, hp, h_m, w, w_n, HeadOut<true>{part, picked, codes, targets, blocks})) return 1;
         const unsigned shares = unsigned(std::clamp<int64_t>(1024 / rows, 1, (blocks + 31) / 32));
-        hipLaunchKernelGGL((head_grad_kernel<F16>), dim3(unsigned(rows), shares), dim3(256), 0, st, codes, part, picked, g + r0, scale, targets, blocks,
-                           losses ? losses + r0 : nullptr);
+        hipLaunchKernelGGL((head_grad_kernel<F16>), dim3(unsigned(rows), shares), dim3(256), 0, st, codes, part, picked, g + r0, scale,
+                           targets, blocks, losses ? losses + r0 : nullptr);
         if (check(hipGetLastError(), "head_grad_kernel launch")) return 1;
         if (const BothPlan both = both_plan(d); both.parts && dh && dw) {
             if (both_grads<F16>(st, d, both, codes, w, w_n, hp, h_m, parts, HeadStore{nullptr, nullptr, dh, inverse, d->k, F16},

@@ -330,20 +330,22 @@ __global__ __launch_bounds__(256) void packed_dkdv_kernel(AttnParams p, const fl
     p.delta += t.start;
     if (STORE) p.ds += t.ds * p.heads * (128 * 64);
     if (PARTS) sums += (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * (256 * D);
-    flash_dkdv_tile<D, F16, CAUSAL, false, STORE, false, PARTS>(p, lse2 + t.start, 0, n, t.block, (t.len + 127) / 128, tokens, int(blockIdx.y),
-                                                                int(gridDim.y), sums);
+    flash_dkdv_tile<D, F16, CAUSAL, false, STORE, false, PARTS>(p, lse2 + t.start, 0, n, t.block, (t.len + 127) / 128, tokens,
+                                                                int(blockIdx.y), int(gridDim.y), sums);
 }
 
 // The parts' sums, added in order and rounded: blockIdx.y is a tile of 32 columns of dK, then of dV.
 template <int D, bool F16>
-__global__ __launch_bounds__(256) void packed_dkdv_sum_kernel(AttnParams p, const PackedTile *tiles, const float *__restrict__ sums, int parts) {
+__global__ __launch_bounds__(256) void packed_dkdv_sum_kernel(AttnParams p, const PackedTile *tiles, const float *__restrict__ sums,
+                                                              int parts) {
     int64_t n, idx;
     packed_place(p.kv_heads, n, idx);
     const PackedTile t = tiles[idx];
     if (t.block < 0) return;
     const bool v = blockIdx.y >= D / 32;
     const int dt = int(blockIdx.y) % (D / 32), cols = int(v ? p.hdv : p.hd);
-    const float4 *from = reinterpret_cast<const float4 *>(sums + int64_t(blockIdx.x) * (256 * D)) + int64_t(blockIdx.y) * 1024 + threadIdx.x;
+    const float4 *from = reinterpret_cast<const float4 *>(sums + int64_t(blockIdx.x) * (256 * D)) + int64_t(blockIdx.y) * 1024 +
+                         threadIdx.x;
     float4 sum[4];
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) sum[e4] = from[256 * e4];

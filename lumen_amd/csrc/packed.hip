@@ -185,8 +185,8 @@ int bwd(hipStream_t st, const nhip_packed_desc *d, const AttnParams &p, const ui
     }
     const int64_t parts = key_parts(d);
     if (parts == 1) return 0;
-    hipLaunchKernelGGL((packed_dkdv_sum_kernel<D, F16>), dim3(unsigned(a.t[0].most * d->kv_heads), D / 16), dim3(256), 0, st, p, a.t[0].tiles,
-                       sums, int(parts));
+    hipLaunchKernelGGL((packed_dkdv_sum_kernel<D, F16>), dim3(unsigned(a.t[0].most * d->kv_heads), D / 16), dim3(256), 0, st, p,
+                       a.t[0].tiles, sums, int(parts));
     return check(hipGetLastError(), "packed_dkdv_sum_kernel launch");
 }
 
@@ -239,9 +239,11 @@ int packed_bwd_on(hipStream_t st, const nhip_packed_desc *d, const void *q, cons
     a.fits = reinterpret_cast<int32_t *>(at + w.flag);
     if (!few(d) && build_tables(st, d, a, 2)) return 1;  // else the workgroups of bwd()'s first launch do
     const bool f16 = d->dtype == NHIP_F16;
-#define NHIP_PACKED(DD)                                                                                                             \
-    return f16 ? (d->causal ? bwd<DD, true, true>(st, d, p, left, a, store, again, sums) : bwd<DD, true, false>(st, d, p, left, a, store, again, sums)) \
-               : (d->causal ? bwd<DD, false, true>(st, d, p, left, a, store, again, sums) : bwd<DD, false, false>(st, d, p, left, a, store, again, sums))
+#define NHIP_PACKED(DD)                                                                 \
+    return f16 ? (d->causal ? bwd<DD, true, true>(st, d, p, left, a, store, again, sums)      \
+                            : bwd<DD, true, false>(st, d, p, left, a, store, again, sums))    \
+               : (d->causal ? bwd<DD, false, true>(st, d, p, left, a, store, again, sums)     \
+                            : bwd<DD, false, false>(st, d, p, left, a, store, again, sums))
     if (kernel_dim(d) == 64) NHIP_PACKED(64);
     NHIP_PACKED(128);
 #undef NHIP_PACKED

@@ -103,8 +103,8 @@ def _taken(q, k, v, offsets, scale):
     (t, n, d), (nkv, dv) = q.shape, v.shape[1:]
     most = max(t // 64 + min(offsets.shape[0] - 1, t) + 2, t // 8 + 1)
     # the kernels' scale is float32: one that it rounds to 0 or to infinity is the primitives'
-    return q.dtype in ("bfloat16", "float16") and 0.0 < C.c_float(scale).value <= 3.4e38 and all(x % 8 == 0 and 0 < x <= 128 for x in (d, dv)) \
-        and t <= MAX_TOKENS and offsets.shape[0] - 1 <= MAX_SEQUENCES and most * max(n, nkv) < 1 << 24
+    return q.dtype in ("bfloat16", "float16") and 0.0 < C.c_float(scale).value <= 3.4e38 \
+        and all(x % 8 == 0 and 0 < x <= 128 for x in (d, dv)) and t <= MAX_TOKENS and offsets.shape[0] - 1 <= MAX_SEQUENCES and most * max(n, nkv) < 1 << 24
 
 
 class _PackedAttention(Function):
