@@ -47,7 +47,7 @@ int64_t ds_room(const nhip_packed_desc *d) {
 // but no more than three quarters of a block's tiles, since a part costs the K and V operands' loads and its sums' traffic. Blocks
 // are estimated with half a one a sequence lost, tiles from the mean length. Us of the kernel and its sums by parts (* taken):
 //   331 + 254 + 129 + 97 tokens, 6 heads of 2, dims 80, unmasked    1: 62   2: 39  4: 27  6: 22  7: 22*  8: 23  12: 30  16: 34
-//   1500 + 500 + 48 tokens, 8 heads of 2, dims 128, causal          1: 259  2: 136  4: 76  6: 59  7*  8: 55  12: 58  16: 60
+//   1500 + 500 + 48 tokens, 8 heads of 2, dims 128, causal          1: 259  2: 136  4: 76  6: 59  7: 55*  8: 55  12: 58  16: 60
 //   200 + 300 + 12 tokens, 8 heads of 8, dims 64, causal            1: 19   2: 17  3: 15*  4: 16  6: 17  8: 19  12: 24
 int64_t key_parts(const nhip_packed_desc *d) {
     const int64_t sequences = std::max<int64_t>(std::min(d->sequences, d->tokens), 1), kv_heads = std::max<int64_t>(d->kv_heads, 1);

@@ -114,9 +114,10 @@ def linear_cross_entropy(input, weight, target, ignore_index=-100, reduction="me
     the ``V`` classes. ``reduction``: ``"mean"`` over the rows that count (0 of none), ``"sum"``, or ``"none"``, a loss a row
     ``[...]``. Losses and all sums are float32 (float64 of float64 operands). The gradients of the logits are rounded to the
     operands' dtype as operands of the products that give those of ``input`` and ``weight``, which are rounded again. bfloat16
-    and float16 (up to 2^26 rows, and a weight below 2^30 elements and 2^22 classes) run as kernels of their own, which take six
-    products' work for both directions and hold exponentials (the losses alone: maxima and sums of 64 classes each) of at most
-    ``config.compiler.head_piece_bytes`` at a time; other dtypes run as primitives, over whole logits."""
+    and float16 (up to 2^26 rows and 2^38 logits, and a weight below 2^30 elements and 2^22 classes) run as kernels of their own,
+    which take six products' work for both directions and hold exponentials (the losses alone: maxima and sums of 64 classes each)
+    of at most ``config.compiler.head_piece_bytes`` at a time; others run as primitives, over whole logits where there are
+    gradients."""
     op = "linear_cross_entropy"
     h, w, target = lift(input), lift(weight), lift(target)
     if not isinstance(h, TracedTensor) or h.ndim < 1:

@@ -104,7 +104,8 @@ def _taken(q, k, v, offsets, scale):
     most = max(t // 64 + min(offsets.shape[0] - 1, t) + 2, t // 8 + 1)
     # the kernels' scale is float32: one that it rounds to 0 or to infinity is the primitives'
     return q.dtype in ("bfloat16", "float16") and 0.0 < C.c_float(scale).value <= 3.4e38 \
-        and all(x % 8 == 0 and 0 < x <= 128 for x in (d, dv)) and t <= MAX_TOKENS and offsets.shape[0] - 1 <= MAX_SEQUENCES and most * max(n, nkv) < 1 << 24
+        and all(x % 8 == 0 and 0 < x <= 128 for x in (d, dv)) and t <= MAX_TOKENS and offsets.shape[0] - 1 <= MAX_SEQUENCES \
+        and most * max(n, nkv) < 1 << 24
 
 
 class _PackedAttention(Function):
@@ -152,8 +153,8 @@ def packed_attention(query, key, value, offsets, scale=None, is_causal=True):
     sequence's results; the kernels keep one of another sequence out too. ``N`` is a multiple of ``Nkv`` (grouped heads);
     ``scale`` is ``1 / sqrt(D)`` by default. The softmax and all sums are float32 (float64 of float64 operands), the
     probabilities rounded to the operands' dtype. bfloat16 and float16 with head dims that are multiples of 8 up to 128
-    (and up to 2^26 tokens and 2^20 sequences) run as kernels of their own, others as primitives, whose scores ``[N, T, T]`` exist
-    whole. The kernels of head dims other than 64 and 128 need the rows of each head of an operand within 2 GiB."""
+    (and up to 2^26 tokens and 2^20 sequences, ``N T / 8`` and ``N (T / 64 + sequences)`` below 2^24, and a scale that float32
+    holds) run as kernels of their own, others as primitives, whose scores ``[N, T, T]`` exist whole. The kernels of head dims other than 64 and 128 need the rows of each head of an operand within 2 GiB."""
     op = "packed_attention"
     q, k, v, offsets = lift(query), lift(key), lift(value), lift(offsets)
     for role, t in (("query", q), ("key", k), ("value", v)):
