@@ -154,7 +154,8 @@ def packed_attention(query, key, value, offsets, scale=None, is_causal=True):
     ``scale`` is ``1 / sqrt(D)`` by default. The softmax and all sums are float32 (float64 of float64 operands), the
     probabilities rounded to the operands' dtype. bfloat16 and float16 with head dims that are multiples of 8 up to 128
     (and up to 2^26 tokens and 2^20 sequences, ``N T / 8`` and ``N (T / 64 + sequences)`` below 2^24, and a scale that float32
-    holds) run as kernels of their own, others as primitives, whose scores ``[N, T, T]`` exist whole. The kernels of head dims other than 64 and 128 need the rows of each head of an operand within 2 GiB."""
+    holds) run as kernels of their own, others as primitives, whose scores ``[N, T, T]`` exist whole. The kernels of head dims
+    other than 64 and 128 need the rows of each head of an operand within 2 GiB."""
     op = "packed_attention"
     q, k, v, offsets = lift(query), lift(key), lift(value), lift(offsets)
     for role, t in (("query", q), ("key", k), ("value", v)):
