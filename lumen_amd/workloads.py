@@ -211,7 +211,8 @@ def packed_train_step(model, opt, ids, places, targets, offsets, max_norm=1.0):
 
 def pack(documents, tokens):
     """``(ids, places, targets, offsets)`` of the documents' token ids one after another in ``tokens`` tokens: a token's target is
-    the next one of its document, and ignored (-100) of a document's last and of the tokens behind them."""
+    the next one of its document, and ignored (-100) of a document's last and of the tokens behind them. A document's places count from
+    0: it is no longer than the model's positions, whose last a longer one's tokens would share."""
     offsets = np.cumsum([0, *map(len, documents)]).astype(np.int32)
     if offsets[-1] > tokens:
         raise ValueError(f"pack: documents of {offsets[-1]} tokens in {tokens}")

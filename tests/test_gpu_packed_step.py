@@ -180,3 +180,27 @@ def test_a_view_off_16_bytes_that_an_adamw_step_reads_too(hip):
     new, tw = M.adamw(x, x, zero, zero, 1, 0.1, (0.9, 0.999), 1e-8, 0.0)[0], M.adamw_tolerances(x, x, zero, zero, 1, 0.1, (0.9, 0.999), 1e-8, 0.0)[0]
     for a in stepped:
         assert np.all(np.abs(a.reshape(-1) - new) <= tw + 2.0**-8 * (np.abs(new) + tw))
+
+
+def test_weights_of_two_launches_in_place_and_clipped(hip):
+    """More weights than a launch of AdamW's table holds (44), written over their own memory with the clip's factor taken within the step,
+    leave the bits of the same step into other memory."""
+    cfg = W.TransformerConfig(vocab=97, dim=64, heads=2, ffn=96, seq=24, batch=1, layers=6)
+    rng = np.random.default_rng(9)
+    batches = [W.pack([rng.integers(0, cfg.vocab, n) for n in lengths], 64) for lengths in ([24, 1, 20], [7, 0, 24, 24], [3, 3])]
+    states = []
+    for in_place in (True, False):
+        model, _ = W.build(cfg)
+        W.load(model, W.init_weights(model))
+        opt = W.adamw(model, 1e-2)
+        W.load_adamw(opt)
+        assert len(opt.params) > 44
+        with L.config.compiler.patch(update_in_place=in_place):
+            step = L.compile(W.packed_train_step, device="hip")
+            losses = [float(L.to_numpy(step(model, opt, *map(L.from_numpy, b)))) for b in batches]
+        assert [st.kind for st in step.plan.steps].count("adamw") == 1
+        assert (len(step.plan.in_place_outputs) >= 4 * len(opt.params)) == in_place
+        states.append((losses, _state(opt)))
+    (a, x), (b, y) = states
+    assert a == b and np.isfinite(a).all()
+    assert all(np.array_equal(i, j) for i, j in zip(x, y))
